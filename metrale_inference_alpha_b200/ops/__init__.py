@@ -989,3 +989,6 @@ def _attention_rowwise(q, k_cache, v_cache, block_table, q_start, q_len, ctx_len
     return paged_attention(q, k_cache, v_cache, block_table[seq_of_row].contiguous(),
                            torch.arange(T, device=dev, dtype=torch.int32),
                            torch.ones(T, device=dev, dtype=torch.int32), ctx, max_q_len=1, **kw)
+
+
+from .kv_mass import kv_evict, paged_attention_mass, prompt_mass  # noqa: E402,F401  (decode attention and prompts that leave their weights; eviction by them)

@@ -1,0 +1,85 @@
+// Arguments of the launchers of kv_mass.cu and kv_observe.cu, mirrored field for field by ops/kv_mass.py, and what the kernels of a
+// decode step with weights share.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <cstddef>
+#include <cstdint>
+
+struct MbMassArgs {
+  const void* q;             // [rows, Hq, D] bf16, rows contiguous
+  const void* k_cache;       // [blocks, block, Hkv, D] bf16 or e4m3
+  const void* v_cache;
+  const int* block_table;
+  long long table_ld;
+  const int* q_start;        // prompts only
+  const int* q_len;
+  const int* ctx_len;
+  float* mass;               // [seqs, Hkv, columns], columns next to each other
+  long long mass_seq, mass_head;
+  void* out;                 // [seqs, Hq, D] bf16
+  void* ws;
+  size_t ws_bytes;
+  const float* k_scale;
+  const float* v_scale;
+  uint32_t* status;
+  long long num_blocks;
+  long long q_rows;          // prompts only: rows of q
+  int num_seqs, Hq, Hkv, D, block_size, fp8, max_ctx, max_q_len, last, sm_count;
+  float scale;
+};
+
+struct MbEvictArgs {
+  const float* mass;
+  long long mass_seq, mass_head;
+  float* mass_out;
+  long long out_seq, out_head;
+  const int* ctx_len;
+  int* kept;                 // [seqs, Hkv, keep]
+  int* new_len;              // [seqs]
+  int* first;                // [seqs, Hkv]: rows in front of this one stay where they are
+  const int* block_table;
+  long long table_ld;
+  const int* dst_table;
+  long long dst_ld;
+  void* k_cache;
+  void* v_cache;
+  long long num_blocks;
+  uint32_t* status;
+  int num_seqs, Hkv, keep, recent, max_ctx, block_size, row_bytes, in_place;
+};
+
+namespace mbm {
+
+constexpr int kMaxParts = 32;
+// A sequence's partitions, from its own length alone: part_tokens each, but at most kMaxParts of them.
+__host__ __device__ __forceinline__ int part_size(int len, int part_tokens) {
+  const int even = ((len + kMaxParts - 1) / kMaxParts + 63) & ~63;
+  return even > part_tokens ? even : part_tokens;
+}
+__host__ __device__ __forceinline__ int part_count(int len, int part_tokens) {
+  const int P = part_size(len, part_tokens);
+  return len <= P ? 1 : (len + P - 1) / P;
+}
+
+// Workspace of a decode step: logits in the log2 domain [seqs, Hkv, G, ld], what a partition's outputs are relative to and their sums
+// [seqs * Hq, parts], the outputs themselves [seqs * Hq, parts, D].
+struct DecodeWs {
+  long long ld;
+  int parts;
+  size_t z, ml, o, bytes;    // byte offsets, and the whole
+};
+inline DecodeWs decode_ws(int seqs, int Hq, int D, int max_ctx, int part_tokens) {
+  DecodeWs w;
+  w.ld = (max_ctx + 63) & ~63ll;
+  const int n = (max_ctx + part_tokens - 1) / part_tokens;
+  w.parts = n < 1 ? 1 : n > kMaxParts ? kMaxParts : n;
+  const size_t rows = (size_t)seqs * Hq;
+  w.z = 0;
+  w.o = rows * w.ld * 4;
+  w.ml = w.o + rows * w.parts * D * 4;
+  w.bytes = w.ml + rows * w.parts * 8;
+  return w;
+}
+
+}  // namespace mbm

@@ -302,6 +302,82 @@ def paged_attention(q, k_cache, v_cache, block_table, q_start, q_len, ctx_len, s
     return out
 
 
+# ----------------------------------------------------------------------------- attention weight per cached token
+def _cached_rows(cache, block_table, s: int, rows: torch.Tensor, scale=None) -> torch.Tensor:
+    """Rows of sequence s (indices into its context) of a paged cache, fp32 [n, Hkv, D]."""
+    bs = cache.shape[1]
+    x = cache.reshape(-1, *cache.shape[2:])[block_table[s].long()[rows // bs] * bs + rows % bs]
+    return from_e4m3(x) * scale if cache.dtype == torch.uint8 else x.float()
+
+
+def _weights(q, k, limits, scale: float) -> torch.Tensor:
+    """Softmax weights [W, Hkv, G, n] of queries q [W, Hkv, G, D] that see the first limits[w] rows of k [n, Hkv, D]; rows that see nothing
+    have none."""
+    z = torch.einsum("whgd,nhd->whgn", q.float(), k) * scale
+    seen = (torch.arange(k.shape[0]) < limits[:, None])[:, None, None]
+    p = torch.softmax(z.masked_fill(~seen, float("-inf")), -1)
+    return torch.where(seen, p, torch.zeros_like(p))
+
+
+def paged_attention_mass(q, k_cache, v_cache, block_table, ctx_len, mass, scale: float, k_scale=None, v_scale=None) -> torch.Tensor:
+    """One new token a sequence: attention output bf16, every cached token's weight over its group added to mass [S, Hkv, columns]."""
+    S, Hq, D = q.shape
+    Hkv = k_cache.shape[2]
+    out = torch.zeros(S, Hq, D)
+    for s in range(S):
+        n = int(ctx_len[s])
+        if n <= 0:
+            continue
+        at = torch.arange(n)
+        p = _weights(q[s].view(1, Hkv, Hq // Hkv, D), _cached_rows(k_cache, block_table, s, at, k_scale), torch.tensor([n]), scale)[0]
+        out[s] = torch.einsum("hgn,nhd->hgd", p, _cached_rows(v_cache, block_table, s, at, v_scale)).reshape(Hq, D)
+        mass[s, :, :n] += p.sum(1)
+    return out.to(torch.bfloat16)
+
+
+def prompt_mass(q, k_cache, block_table, q_start, q_len, ctx_len, mass, scale: float, last: int = 0, k_scale=None) -> torch.Tensor:
+    """Weights that the last `last` tokens (0: all) of every portion give to what is cached, added to mass."""
+    Hq, D = q.shape[1:]
+    Hkv = k_cache.shape[2]
+    for s in range(len(ctx_len)):
+        n, ql = int(ctx_len[s]), int(q_len[s])
+        w = min(last or ql, ql)
+        if n <= 0 or w <= 0:
+            continue
+        rows = q[int(q_start[s]) + ql - w:int(q_start[s]) + ql].view(w, Hkv, Hq // Hkv, D)
+        k = _cached_rows(k_cache, block_table, s, torch.arange(n), k_scale)
+        mass[s, :, :n] += _weights(rows, k, n - w + 1 + torch.arange(w), scale).sum((0, 2))
+    return mass
+
+
+def kv_evict(k_cache, v_cache, block_table, ctx_len, mass, keep: int, recent: int, max_ctx: int, mass_out, dst_table=None):
+    """Rows of the largest mass and the last `recent` ones move to the front in their order; (kept, new lengths)."""
+    S, Hkv = mass.shape[:2]
+    bs = k_cache.shape[1]
+    dst = block_table if dst_table is None else dst_table
+    kept = torch.full((S, Hkv, keep), -1, dtype=torch.int32)
+    for s in range(S):
+        n = int(ctx_len[s])
+        m = min(n, keep)
+        to = torch.arange(m)
+        to = dst[s].long()[to // bs] * bs + to % bs
+        for h in range(Hkv):
+            x = mass[s, h, :n].clone()
+            idx = torch.arange(n)
+            if n > keep:
+                old = torch.where(x.isnan(), torch.full_like(x, float("-inf")), x)[:n - recent]
+                best = torch.sort(old, descending=True, stable=True).indices[:keep - recent]
+                idx = torch.cat([torch.sort(best).values, idx[n - recent:]])
+            kept[s, h, :m] = idx.to(torch.int32)
+            at = block_table[s].long()[idx // bs] * bs + idx % bs
+            for cache in (k_cache, v_cache):
+                flat = cache.view(-1, *cache.shape[2:])
+                flat[to, h] = flat[at, h]
+            mass_out[s, h, :m] = x[idx]
+            mass_out[s, h, m:max_ctx] = 0.0
+    return kept, ctx_len.clamp(max=keep)
+
+
 # ----------------------------------------------------------------------------- gated delta net
 def gdn_gates(a, b, A_log, dt_bias):
     """decay = exp(-exp(min(A_log,20)) * softplus(min(a+dt_bias,20))), beta = sigmoid(b)

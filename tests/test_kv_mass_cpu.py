@@ -1,0 +1,158 @@
+"""The CPU form of the operators that hold a cache to a budget by attention weight, and what they refuse."""
+import math
+
+import pytest
+import torch
+
+import kv_mass_oracle as oracle
+from metrale_inference_alpha_b200 import ops
+
+
+def _decode(c, **kw):
+    return ops.paged_attention_mass(c["q"], c["k"], c["v"], c["table"], c["ctx"], c["mass"], max_ctx=c["max_ctx"], scale=c["scale"], k_scale=c["k_scale"],
+                                    v_scale=c["v_scale"], **kw)
+
+
+def _prompt(c, last, **kw):
+    return ops.prompt_mass(c["q"], c["k"], c["table"], c["q_start"], c["q_len"], c["ctx"], c["mass"], max_q_len=int(c["q_len"].max()), max_ctx=c["max_ctx"],
+                           scale=c["scale"], last=last, k_scale=c["k_scale"], **kw)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(4, 2, 64), (5, 1, 128), (3, 3, 256)])
+def test_decode_gives_outputs_and_adds_weights(fp8, heads, kv_heads, dim):
+    c = oracle.case(1, [33, 0, 1, 17], heads, kv_heads, dim, fp8, columns=40)
+    before = c["mass"].clone()
+    want, tol, mass, mtol = oracle.decode(c)
+    got = _decode(c)
+    assert ((got.double() - want).abs() <= tol).all() and ((c["mass"].double() - mass).abs() <= mtol).all()
+    assert torch.equal(got[1], torch.zeros_like(got[1])) and torch.equal(c["mass"][1], before[1])
+    gained = (c["mass"] - before).double().sum(2)
+    assert torch.allclose(gained[0], torch.full_like(gained[0], heads / kv_heads), rtol=1e-4)
+
+
+@pytest.mark.parametrize("last", [0, 1, 4])
+def test_prompt_adds_the_weights_of_its_last_tokens(last):
+    c = oracle.case(2, [40, 9, 5, 0], 6, 2, 64, False, new=[7, 9, 1, 0])
+    mass, mtol = oracle.prompt(c, last)
+    assert _prompt(c, last) is c["mass"]
+    assert ((c["mass"].double() - mass).abs() <= mtol).all()
+
+
+def test_prompt_rows_that_see_nothing_give_nothing():
+    c = oracle.case(3, [3], 2, 1, 64, False, new=[5])                     # two of five tokens lie before what is cached
+    before = c["mass"].clone()
+    _prompt(c, 0)
+    assert float((c["mass"] - before).sum()) == pytest.approx(3 * 2, rel=1e-5)
+
+
+def _poisoned(c, seed):
+    g = torch.Generator().manual_seed(seed)
+    m = c["mass"]
+    m.copy_(torch.randint(0, 6, m.shape, generator=g).float())            # many ties
+    for value in (math.nan, math.inf, -math.inf, -0.0):
+        m[torch.rand(m.shape, generator=g) < 0.05] = value
+
+
+@pytest.mark.parametrize("keep,recent", [(1, 0), (1, 1), (8, 3), (16, 16), (20, 0), (64, 5)])
+@pytest.mark.parametrize("own_blocks", [False, True])
+def test_evict_keeps_the_heaviest_and_the_latest(keep, recent, own_blocks):
+    c = oracle.case(4, [40, 1, 16, 17, 0], 4, 2, 64, False)
+    _poisoned(c, 5)
+    nb, dst = c["k"].shape[0], None
+    if own_blocks:
+        per = (keep + 15) // 16
+        dst = (torch.arange(5 * per, dtype=torch.int32) + nb).flip(0).view(5, per)
+        c["k"], c["v"] = (torch.cat([x, torch.zeros(5 * per, *x.shape[1:], dtype=x.dtype)]) for x in (c["k"], c["v"]))
+    k, v, mass, kept, length = oracle.evict(c, keep, recent, c["max_ctx"], dst)
+    got = ops.kv_evict(c["k"], c["v"], c["table"], c["ctx"], c["mass"], keep=keep, recent=recent, max_ctx=c["max_ctx"], dst_table=dst)
+    assert torch.equal(got[0], kept) and torch.equal(got[1], length)
+    for a, b in ((c["k"], k), (c["v"], v), (c["mass"], mass)):
+        assert torch.equal(a.nan_to_num(7.0), b.nan_to_num(7.0))
+
+
+def test_evict_leaves_the_source_mass_where_another_takes_it():
+    c = oracle.case(6, [30, 12], 2, 2, 64, True)
+    before, out = c["mass"].clone(), torch.full((2, 2, 35), 9.0)
+    mass = oracle.evict(c, 10, 2, 30)[2]
+    ops.kv_evict(c["k"], c["v"], c["table"], c["ctx"], c["mass"], keep=10, recent=2, max_ctx=30, mass_out=out)
+    assert torch.equal(c["mass"], before) and torch.equal(out[:, :, :30], mass) and bool((out[:, :, 30:] == 9).all())
+
+
+# ----------------------------------------------------------------------------- refusals
+def _bad_decode():
+    yield "q type", dict(q=lambda q: q.float())
+    yield "q shape", dict(q=lambda q: q[:1])
+    yield "q order", dict(q=lambda q: q.transpose(0, 1).contiguous().transpose(0, 1))
+    yield "groups", dict(q=lambda q: q[:, :3].contiguous())
+    yield "cache type", dict(k=lambda k: k.float())
+    yield "cache order", dict(k=lambda k: k.transpose(1, 2).contiguous().transpose(1, 2))
+    yield "v shape", dict(v=lambda v: v[:1])
+    yield "head dim", dict(q=lambda q: q[:, :, :32].contiguous(), k=lambda k: k[..., :32].contiguous(), v=lambda v: v[..., :32].contiguous())
+    yield "table type", dict(table=lambda t: t.long())
+    yield "table rows", dict(table=lambda t: t[:1])
+    yield "table width", dict(table=lambda t: t[:, :1])
+    yield "lengths type", dict(ctx=lambda x: x.long())
+    yield "lengths order", dict(ctx=lambda x: x.repeat_interleave(2)[::2])
+    yield "mass type", dict(mass=lambda m: m.double())
+    yield "mass columns", dict(mass=lambda m: m[:, :, :20])
+    yield "mass order", dict(mass=lambda m: m.transpose(1, 2).contiguous().transpose(1, 2))
+    yield "mass shared", dict(mass=lambda m: m[:1].expand(2, -1, -1))
+    yield "mass heads", dict(mass=lambda m: m[:, :1])
+    yield "negative length", dict(max_ctx=lambda n: -1)
+
+
+@pytest.mark.parametrize("change", [c for _, c in _bad_decode()], ids=[n for n, _ in _bad_decode()])
+def test_decode_refuses(change):
+    c = oracle.case(7, [40, 33], 4, 2, 64, False)
+    for key, f in change.items():
+        c[key] = f(c[key])
+    before = c["mass"].clone()
+    with pytest.raises(ValueError, match="paged_attention_mass"):
+        _decode(c)
+    assert torch.equal(c["mass"], before)
+
+
+def test_e4m3_caches_want_scales():
+    c = oracle.case(8, [40], 4, 2, 64, True)
+    for name in ("k_scale", "v_scale"):
+        with pytest.raises(ValueError, match="scales"):
+            _decode({**c, name: None})
+    with pytest.raises(ValueError, match="scales"):
+        _prompt({**c, "k_scale": None}, 1)
+    with pytest.raises(ValueError, match="scales"):
+        _prompt({**c, "k_scale": c["k_scale"].double()}, 1)
+
+
+@pytest.mark.parametrize("change", [dict(last=-1), dict(max_q_len=-1), dict(q_start=torch.zeros(2, dtype=torch.int64)), dict(q_len=torch.ones(3, dtype=torch.int32)),
+                                    dict(max_ctx=49)], ids=lambda c: next(iter(c)))
+def test_prompt_refuses(change):
+    c = oracle.case(9, [40, 33], 4, 2, 64, False, new=[5, 6])
+    kw = dict(q_start=c["q_start"], q_len=c["q_len"], max_q_len=6, max_ctx=40, last=0) | change
+    with pytest.raises(ValueError, match="prompt_mass"):
+        ops.prompt_mass(c["q"], c["k"], c["table"], kw.pop("q_start"), kw.pop("q_len"), c["ctx"], c["mass"], scale=c["scale"], **kw)
+
+
+@pytest.mark.parametrize("change", [dict(keep=0), dict(recent=-1), dict(recent=9), dict(max_ctx=49), dict(mass_out="narrow"), dict(mass_out="overlap"), dict(mass_out="shared"),
+                                    dict(dst_table="narrow"), dict(dst_table="type"), dict(dst_table="rows")], ids=lambda c: "-".join(map(str, next(iter(c.items())))))
+def test_evict_refuses(change):
+    c = oracle.case(10, [40, 33], 4, 2, 64, False)
+    big = torch.zeros(2, 2, 60)
+    special = {"narrow": dict(mass_out=torch.zeros(2, 2, 39), dst_table=torch.zeros(2, 0, dtype=torch.int32)), "overlap": dict(mass_out=big[:, :, 10:50]),
+               "shared": dict(mass_out=torch.zeros(1, 2, 40).expand(2, -1, -1)), "type": dict(dst_table=torch.zeros(2, 1)), "rows": dict(dst_table=torch.zeros(1, 1, dtype=torch.int32))}
+    kw = dict(keep=8, recent=2, max_ctx=40)
+    for key, v in change.items():
+        kw[key] = special[v][key] if isinstance(v, str) else v
+    mass = big[:, :, :40] if change.get("mass_out") == "overlap" else c["mass"]
+    k = c["k"].clone()
+    with pytest.raises(ValueError, match="kv_evict"):
+        ops.kv_evict(c["k"], c["v"], c["table"], c["ctx"], mass, **kw)
+    assert torch.equal(c["k"].nan_to_num(7.0), k.nan_to_num(7.0))
+
+
+def test_nothing_to_do():
+    c = oracle.case(11, [4], 2, 1, 64, False)
+    none = dict(table=c["table"][:0], ctx=c["ctx"][:0], mass=c["mass"][:0])
+    assert ops.paged_attention_mass(c["q"][:0], c["k"], c["v"], none["table"], none["ctx"], none["mass"], max_ctx=4, scale=1.0).shape == (0, 2, 64)
+    kept, length = ops.kv_evict(c["k"], c["v"], none["table"], none["ctx"], none["mass"], keep=2, recent=1, max_ctx=4)
+    assert kept.shape == (0, 1, 2) and length.shape == (0,)

@@ -1,0 +1,400 @@
+"""The kernels that hold a cache to a budget by attention weight, against 64 bits: tolerances are the oracle's bounds."""
+import math
+
+import pytest
+import torch
+
+import kv_mass_oracle as oracle
+from metrale_inference_alpha_b200 import ops
+from metrale_inference_alpha_b200.ops import _native, kv_mass
+
+pytestmark = pytest.mark.gpu
+
+
+def _cuda(c):
+    return {k: v.cuda() if isinstance(v, torch.Tensor) else v for k, v in c.items()}
+
+
+def _decode(c, **kw):
+    return ops.paged_attention_mass(c["q"], c["k"], c["v"], c["table"], c["ctx"], c["mass"], scale=c["scale"], k_scale=c["k_scale"], v_scale=c["v_scale"],
+                                    **(dict(max_ctx=c["max_ctx"]) | kw))
+
+
+def _prompt(c, last, **kw):
+    return ops.prompt_mass(c["q"], c["k"], c["table"], c["q_start"], c["q_len"], c["ctx"], c["mass"], scale=c["scale"], last=last, k_scale=c["k_scale"],
+                           **(dict(max_q_len=c["max_q_len"], max_ctx=c["max_ctx"]) | kw))
+
+
+def _within(got, want, tol, what):
+    far = (got.double().cpu() - want).abs() - tol
+    assert bool((far <= 0).all()), f"{what}: {int((far > 0).sum())} of {far.numel()} beyond their bound, by up to {float(far.max()):.3g} at {int(far.argmax())}"
+
+
+@pytest.fixture(autouse=True)
+def _status():
+    yield
+    ops.check_status("cuda")
+
+
+# ----------------------------------------------------------------------------- decode
+SHAPES = [(4, 2, 64), (40, 8, 128), (8, 8, 128), (16, 1, 128), (24, 1, 128), (32, 1, 128), (48, 1, 128), (12, 1, 64), (3, 3, 256), (16, 2, 256), (20, 1, 256)]
+LENGTHS = [[1], [700], [0, 15, 16, 17, 64, 65], [513, 1, 0, 1025, 1024, 511, 3, 2047]]
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("heads,kv_heads,dim", SHAPES)
+@pytest.mark.parametrize("ctx", LENGTHS, ids=str)
+def test_decode(fp8, heads, kv_heads, dim, ctx):
+    c = oracle.case(20, ctx, heads, kv_heads, dim, fp8, columns=max(ctx) + 5)
+    want, tol, mass, mtol = oracle.decode(c)
+    g = _cuda(c)
+    got = _decode(g)
+    _within(got, want, tol, "outputs")
+    _within(g["mass"], mass, mtol, "mass")
+    for s, n in enumerate(ctx):
+        assert torch.equal(g["mass"][s, :, n:].cpu(), c["mass"][s, :, n:])
+
+
+@pytest.mark.parametrize("block", [1, 8, 24, 32, 48, 256])
+@pytest.mark.parametrize("fp8", [False, True])
+def test_decode_block_sizes(block, fp8):
+    c = oracle.case(21, [130, 7, 600], 10, 2, 128, fp8, block=block)
+    want, tol, mass, mtol = oracle.decode(c)
+    g = _cuda(c)
+    _within(_decode(g), want, tol, "outputs")
+    _within(g["mass"], mass, mtol, "mass")
+
+
+@pytest.mark.parametrize("dim,heads,kv_heads", [(64, 8, 2), (128, 10, 2), (256, 8, 1)])
+def test_decode_of_a_long_sequence(dim, heads, kv_heads):
+    """More tokens than 32 of the shortest partitions hold."""
+    c = oracle.case(22, [40007, 33], heads, kv_heads, dim, False)
+    want, tol, mass, mtol = oracle.decode(c)
+    g = _cuda(c)
+    _within(_decode(g), want, tol, "outputs")
+    _within(g["mass"], mass, mtol, "mass")
+
+
+def test_decode_of_large_logits():
+    """Scores hundreds of powers of two apart: all but a few weights vanish, and the rest keep their bound."""
+    c = oracle.case(23, [300, 90], 8, 2, 128, False, spread=40.0)
+    want, tol, mass, mtol = oracle.decode(c)
+    g = _cuda(c)
+    _within(_decode(g), want, tol, "outputs")
+    _within(g["mass"], mass, mtol, "mass")
+
+
+def test_decode_writes_its_part_of_a_larger_buffer():
+    c = _cuda(oracle.case(24, [200, 30, 77], 8, 2, 128, True))
+    alone = c["mass"].clone()
+    lanes = torch.full((5, 3, 260), 3.0, device="cuda")
+    lanes[1:4, 1:, 7:207] = c["mass"]
+    want = _decode({**c, "mass": alone})
+    got = _decode({**c, "mass": lanes[1:4, 1:, 7:207]})
+    assert torch.equal(got, want) and torch.equal(lanes[1:4, 1:, 7:207], alone)
+    lanes[1:4, 1:, 7:207] = 3.0
+    assert bool((lanes == 3).all())
+
+
+@pytest.mark.parametrize("fp8,dim", [(True, 128), (False, 64), (False, 256)])
+def test_decode_of_a_sequence_does_not_depend_on_its_batch(fp8, dim):
+    ctx = [1500, 40, 700, 1100]
+    c = _cuda(oracle.case(25, ctx, 8, 2, dim, fp8))
+    m = c["mass"].clone()
+    out = _decode(c)
+    for s in range(4):
+        one = {**c, "q": c["q"][s:s + 1], "table": c["table"][s:s + 1], "ctx": c["ctx"][s:s + 1], "mass": m[s:s + 1]}
+        assert torch.equal(_decode(one)[0], out[s]) and torch.equal(m[s], c["mass"][s])
+
+
+def test_decode_in_several_steps_gives_the_same(monkeypatch):
+    c = _cuda(oracle.case(26, [300, 10, 0, 513, 77], 8, 2, 128, False))
+    m = c["mass"].clone()
+    out = _decode(c)
+    monkeypatch.setattr(kv_mass, "_WS_BYTES", 1)
+    assert torch.equal(_decode({**c, "mass": m}), out) and torch.equal(m, c["mass"])
+
+
+def test_decode_agrees_with_the_attention_that_leaves_no_weights():
+    c = _cuda(oracle.case(27, [700, 64, 1300], 40, 8, 128, True))
+    plain = ops.paged_attention(c["q"], c["k"], c["v"], c["table"], c["q_start"], c["q_len"], c["ctx"], max_q_len=1, max_ctx=1300, scale=c["scale"], k_scale=c["k_scale"],
+                                v_scale=c["v_scale"])
+    got = _decode(c)
+    assert float((got.float() - plain.float()).abs().max()) <= 2.0 ** -7 * float(plain.float().abs().max())
+
+
+def _graph(fn):
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        fn()
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        r = fn()
+    return g, r
+
+
+def test_two_captured_steps_share_nothing():
+    """Graphs of different batches, replayed on two streams at once."""
+    cs = [_cuda(oracle.case(28 + i, ctx, 40, 8, 128, True)) for i, ctx in enumerate(([900, 600], [1200, 30, 256]))]
+    start = [c["mass"].clone() for c in cs]
+    want = []
+    for c, m in zip(cs, start):
+        mass = m.clone()
+        want.append((_decode({**c, "mass": mass}), mass))
+    graphs = [_graph(lambda c=c: _decode(c)) for c in cs]
+    for _ in range(3):
+        for c, m in zip(cs, start):
+            c["mass"].copy_(m)
+        torch.cuda.synchronize()
+        for g, _ in graphs:
+            s = torch.cuda.Stream()
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for c, (_, out), (w, mass) in zip(cs, graphs, want):
+            assert torch.equal(out, w) and torch.equal(c["mass"], mass)
+
+
+def test_decode_reports_lengths_and_blocks_out_of_range():
+    c = _cuda(oracle.case(30, [100, 50], 8, 2, 128, False))
+    c["v"].nan_to_num_(0.0), c["k"].nan_to_num_(0.0)
+    _decode(c, max_ctx=90)
+    with pytest.raises(_native.KernelError, match="bounds"):
+        ops.check_status("cuda")
+    c["table"][0, 2] = 10 ** 6
+    _decode(c)
+    with pytest.raises(_native.KernelError, match="bounds"):
+        ops.check_status("cuda")
+
+
+# ----------------------------------------------------------------------------- prompts
+PROMPTS = [([1], [1], 0), ([700], [700], 0), ([700], [130], 32), ([300, 0, 5, 129, 128], [300, 0, 5, 1, 128], 0), ([2100, 260], [70, 257], 64), ([1000], [1000], 257)]
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(4, 2, 64), (10, 2, 128), (2, 2, 128), (16, 1, 256), (33, 1, 128)])
+@pytest.mark.parametrize("ctx,new,last", PROMPTS, ids=str)
+def test_prompt(fp8, heads, kv_heads, dim, ctx, new, last):
+    c = oracle.case(40, ctx, heads, kv_heads, dim, fp8, new=new, columns=max(ctx) + 3)
+    mass, mtol = oracle.prompt(c, last)
+    g = _cuda(c)
+    _prompt(g, last)
+    _within(g["mass"], mass, mtol, "mass")
+    for s, n in enumerate(ctx):
+        assert torch.equal(g["mass"][s, :, n:].cpu(), c["mass"][s, :, n:])
+
+
+@pytest.mark.parametrize("block", [1, 8, 24, 64, 256])
+def test_prompt_block_sizes(block):
+    c = oracle.case(41, [333, 90], 8, 2, 128, block % 16 == 0, block=block, new=[150, 90])
+    mass, mtol = oracle.prompt(c, 100)
+    g = _cuda(c)
+    _prompt(g, 100)
+    _within(g["mass"], mass, mtol, "mass")
+
+
+def test_prompt_of_large_logits():
+    c = oracle.case(42, [300, 140], 8, 2, 128, False, new=[140, 140], spread=40.0)
+    mass, mtol = oracle.prompt(c, 0)
+    g = _cuda(c)
+    _prompt(g, 0)
+    _within(g["mass"], mass, mtol, "mass")
+
+
+def test_prompt_rows_that_see_nothing_give_nothing():
+    c = _cuda(oracle.case(43, [3], 2, 1, 64, False, new=[5]))
+    before = c["mass"].clone()
+    _prompt(c, 0)
+    assert float((c["mass"] - before).sum()) == pytest.approx(3 * 2, rel=1e-5)
+
+
+def test_prompt_of_a_sequence_does_not_depend_on_its_batch():
+    c = _cuda(oracle.case(44, [1500, 300, 700], 8, 2, 128, True, new=[900, 300, 33]))
+    m = c["mass"].clone()
+    _prompt(c, 64)
+    for s in range(3):
+        one = {k: c[k][s:s + 1] for k in ("table", "ctx", "q_start", "q_len")}
+        _prompt({**c, **one, "mass": m[s:s + 1]}, 64)
+        assert torch.equal(m[s], c["mass"][s])
+
+
+def test_prompt_in_a_graph_beside_another():
+    cs = [_cuda(oracle.case(45 + i, ctx, 8, 2, 128, False, new=new)) for i, (ctx, new) in enumerate((([900, 600], [100, 600]), ([1200, 30, 256], [40, 30, 256])))]
+    start = [c["mass"].clone() for c in cs]
+    want = [_prompt({**c, "mass": m.clone()}, 64, max_q_len=600) for c, m in zip(cs, start)]
+    graphs = [_graph(lambda c=c: _prompt(c, 64, max_q_len=600))[0] for c in cs]
+    for c, m in zip(cs, start):
+        c["mass"].copy_(m)
+    torch.cuda.synchronize()
+    for g in graphs:
+        with torch.cuda.stream(torch.cuda.Stream()):
+            g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(c["mass"], w) for c, w in zip(cs, want))
+
+
+def test_prompt_reports_lengths_rows_and_blocks_out_of_range():
+    c = _cuda(oracle.case(47, [100, 50], 8, 2, 128, False, new=[20, 50]))
+    c["k"].nan_to_num_(0.0)
+    for change in (dict(max_ctx=90), dict(max_q_len=30)):
+        _prompt(c, 0, **change)
+        with pytest.raises(_native.KernelError, match="bounds"):
+            ops.check_status("cuda")
+    before = c["mass"].clone()
+    _prompt({**c, "q_start": torch.tensor([0, 21], dtype=torch.int32, device="cuda")}, 0)
+    with pytest.raises(_native.KernelError, match="bounds"):
+        ops.check_status("cuda")
+    assert torch.equal(c["mass"][1], before[1])
+    c["table"][0, 2] = -3
+    _prompt(c, 0)
+    with pytest.raises(_native.KernelError, match="bounds"):
+        ops.check_status("cuda")
+
+
+# ----------------------------------------------------------------------------- eviction
+def _poisoned(c, seed):
+    g = torch.Generator().manual_seed(seed)
+    m = c["mass"]
+    m.copy_(torch.randint(0, 50, m.shape, generator=g).float() / 16)
+    for value in (math.nan, math.inf, -math.inf, -0.0, 1e-42):
+        m[torch.rand(m.shape, generator=g) < 0.03] = value
+
+
+def _same(a, b):
+    a, b = a.cpu(), b.cpu()
+    return torch.equal(a.view(torch.uint8), b.view(torch.uint8)) if a.is_floating_point() else torch.equal(a, b)
+
+
+@pytest.mark.parametrize("keep,recent", [(1, 0), (1, 1), (128, 16), (129, 129), (500, 0), (1000, 100), (1024, 1), (5000, 7)])
+@pytest.mark.parametrize("own_blocks", [False, True])
+@pytest.mark.parametrize("fp8,dim,block", [(False, 64, 16), (True, 64, 24), (True, 128, 16), (False, 256, 1)])
+def test_evict(keep, recent, own_blocks, fp8, dim, block):
+    ctx = [1500, 1, keep, keep + 1, 0, 2049] if keep < 2000 else [1500, 1, 0, 33]
+    c = oracle.case(50, ctx, 2, 2, dim, fp8, block=block, columns=max(ctx) + 2)
+    _poisoned(c, 51)
+    dst, S = None, len(ctx)
+    if own_blocks:
+        per = (min(keep, max(ctx)) + block - 1) // block
+        dst = (torch.randperm(S * per, generator=torch.Generator().manual_seed(52)).int() + c["k"].shape[0]).view(S, per)
+        c["k"], c["v"] = (torch.cat([x, torch.zeros(S * per, *x.shape[1:], dtype=x.dtype)]) for x in (c["k"], c["v"]))
+    k, v, mass, kept, length = oracle.evict(c, keep, recent, c["max_ctx"], dst)
+    g = _cuda(c)
+    out = torch.full_like(g["mass"], 5.0) if own_blocks else None
+    got = ops.kv_evict(g["k"], g["v"], g["table"], g["ctx"], g["mass"], keep=keep, recent=recent, max_ctx=c["max_ctx"], dst_table=None if dst is None else dst.cuda(), mass_out=out)
+    assert torch.equal(got[0].cpu(), kept) and torch.equal(got[1].cpu(), length)
+    assert _same(g["k"], k) and _same(g["v"], v)
+    n = c["max_ctx"]
+    if own_blocks:
+        assert _same(out[:, :, :n], mass[:, :, :n]) and bool((out[:, :, n:] == 5).all()) and _same(g["mass"], c["mass"])
+    else:
+        assert _same(g["mass"], mass)
+
+
+@pytest.mark.parametrize("own_blocks", [False, True])
+def test_evict_from_a_long_sequence(own_blocks):
+    """Against a selection by sorting: longer than what one CTA has in registers, with long runs of equal mass."""
+    n, H, D, bs, keep, recent = 150_001, 2, 64, 16, 9000, 33
+    g = torch.Generator(device="cuda").manual_seed(53)
+    nb = (n + bs - 1) // bs
+    more = (keep + bs - 1) // bs if own_blocks else 0
+    k = torch.randint(0, 256, (nb + more, bs, H, D), generator=g, device="cuda", dtype=torch.uint8)
+    v = torch.randint(0, 256, (nb + more, bs, H, D), generator=g, device="cuda", dtype=torch.uint8)
+    table = torch.randperm(nb, generator=g, device="cuda").int().view(1, nb)
+    mass = (torch.rand(1, H, n, generator=g, device="cuda") * 40).floor()
+    mass[0, 1, 1000:] = 0.0
+    best = torch.sort(mass[0, :, :n - recent], dim=-1, descending=True, stable=True).indices[:, :keep - recent].sort(-1).values
+    idx = torch.cat([best, torch.arange(n - recent, n, device="cuda").expand(H, -1)], 1)
+    dst = (torch.arange(more, device="cuda").flip(0) + nb).int().view(1, more) if own_blocks else None
+    to_table, to = table if dst is None else dst, torch.arange(keep, device="cuda")
+    wk, wv, wm = k.clone(), v.clone(), torch.zeros_like(mass)
+    for h in range(H):
+        a = table[0, idx[h] // bs].long() * bs + idx[h] % bs
+        b = to_table[0, to // bs].long() * bs + to % bs
+        wk.flatten(0, 1)[b, h], wv.flatten(0, 1)[b, h] = k.flatten(0, 1)[a, h], v.flatten(0, 1)[a, h]
+        wm[0, h, :keep] = mass[0, h, idx[h]]
+    kept, length = ops.kv_evict(k, v, table, torch.tensor([n], dtype=torch.int32, device="cuda"), mass, keep=keep, recent=recent, max_ctx=n, dst_table=dst)
+    assert torch.equal(kept[0].long(), idx) and int(length) == keep
+    assert torch.equal(k, wk) and torch.equal(v, wv) and torch.equal(mass, wm)
+
+
+def test_evict_in_a_graph_beside_another():
+    cs = [_cuda(oracle.case(54 + i, ctx, 8, 2, 128, True)) for i, ctx in enumerate(([900, 600], [1200, 30, 256]))]
+    outs = [torch.zeros_like(c["mass"]) for c in cs]
+    first = [tuple(x.clone() for x in (c["k"], c["v"])) for c in cs]
+
+    def call(c, o):
+        return ops.kv_evict(c["k"], c["v"], c["table"], c["ctx"], c["mass"], keep=200, recent=20, max_ctx=c["max_ctx"], mass_out=o)
+    want = []
+    for c, o in zip(cs, outs):
+        kept, n = call(c, o)
+        want.append([x.clone() for x in (kept, n, o, c["k"], c["v"])])
+    graphs = [_graph(lambda c=c, o=o: call(c, o)) for c, o in zip(cs, outs)]
+    for c, (k, v) in zip(cs, first):
+        c["k"].copy_(k), c["v"].copy_(v)
+    torch.cuda.synchronize()
+    for g, _ in graphs:
+        with torch.cuda.stream(torch.cuda.Stream()):
+            g.replay()
+    torch.cuda.synchronize()
+    for c, o, (_, (kept, n)), w in zip(cs, outs, graphs, want):
+        assert all(_same(a, b) for a, b in zip((kept, n, o, c["k"], c["v"]), w))
+
+
+def test_evict_reports_lengths_and_blocks_out_of_range():
+    c = _cuda(oracle.case(56, [100, 50], 8, 2, 128, False))
+    k = c["k"].clone()
+    dst = torch.full((2, 2), 10 ** 6, dtype=torch.int32, device="cuda")
+    ops.kv_evict(c["k"], c["v"], c["table"], c["ctx"], c["mass"].clone(), keep=20, recent=2, max_ctx=100, dst_table=dst)
+    with pytest.raises(_native.KernelError, match="bounds"):
+        ops.check_status("cuda")
+    assert _same(c["k"], k)
+    kept, length = ops.kv_evict(c["k"], c["v"], c["table"], c["ctx"], c["mass"], keep=95, recent=2, max_ctx=90)
+    with pytest.raises(_native.KernelError, match="bounds"):
+        ops.check_status("cuda")
+    assert length.tolist() == [90, 50] and int(kept.max()) == 89
+
+
+# ----------------------------------------------------------------------------- together
+@pytest.mark.parametrize("fp8", [False, True])
+def test_a_prompt_is_cut_and_decoded_from(fp8):
+    """A prompt's observers, the cut into blocks of its own, then decode steps that write their rows behind what stayed, cut in place again: outputs,
+    mass and rows against the same steps in 64 bits."""
+    H, G, D, bs, keep, recent, last = 2, 4, 128, 16, 96, 16, 32
+    c = oracle.case(60, [400, 90, 230], H * G, H, D, fp8, new=[400, 90, 230], columns=400)
+    c["mass"].zero_()
+    S, per = 3, (keep + 24 + bs - 1) // bs
+    dst = (torch.arange(S * per, dtype=torch.int32) + c["k"].shape[0]).view(S, per)
+    for name in ("k", "v"):
+        c[name] = torch.cat([c[name], torch.zeros(S * per, bs, H, D, dtype=c[name].dtype)])
+    g = _cuda(c)
+    mass, mtol = oracle.prompt(c, last)
+    _prompt(g, last)
+    _within(g["mass"], mass, mtol, "the prompt's mass")
+    c["mass"] = g["mass"].cpu()                              # selections are made on the same bits
+    k, v, m, kept, length = oracle.evict(c, keep, recent, 400, dst)
+    got, n = ops.kv_evict(g["k"], g["v"], g["table"], g["ctx"], g["mass"], keep=keep, recent=recent, max_ctx=400, dst_table=dst.cuda())
+    assert torch.equal(got.cpu(), kept) and torch.equal(n.cpu(), length) and _same(g["k"], k) and _same(g["v"], v) and _same(g["mass"], m)
+    c.update(k=k, v=v, mass=m, table=dst)
+    g.update(table=dst.cuda())
+    gen = torch.Generator().manual_seed(61)
+    for step in range(20):
+        at = n.cpu().long()
+        slots = dst[torch.arange(S), at // bs].long() * bs + at % bs
+        for name in ("k", "v"):
+            row = torch.randn(S, H, D, generator=gen)
+            row = (row * 16).to(torch.float8_e4m3fn).view(torch.uint8) if fp8 else row.bfloat16()
+            c[name].flatten(0, 1)[slots] = row
+            g[name].flatten(0, 1)[slots.cuda()] = row.cuda()
+        n = n + 1
+        c.update(ctx=n.cpu(), q=torch.randn(S, H * G, D, generator=gen).bfloat16(), q_len=torch.ones(S, dtype=torch.int32), q_start=torch.arange(S, dtype=torch.int32))
+        g.update(ctx=n, q=c["q"].cuda())
+        c["mass"] = g["mass"].cpu()
+        want, tol, mass, mtol = oracle.decode(c)
+        _within(_decode(g, max_ctx=keep + 24), want, tol, f"outputs of step {step}")
+        _within(g["mass"], mass, mtol, f"mass of step {step}")
+    c["mass"] = g["mass"].cpu()
+    k, v, m, kept, length = oracle.evict(c, keep, recent, keep + 24)
+    got, n = ops.kv_evict(g["k"], g["v"], g["table"], g["ctx"], g["mass"], keep=keep, recent=recent, max_ctx=keep + 24)
+    assert torch.equal(got.cpu(), kept) and torch.equal(n.cpu(), length) and _same(g["k"], k) and _same(g["v"], v) and _same(g["mass"], m)
