@@ -1,133 +1,506 @@
 // The weight that a prompt's last tokens give to what is cached: mass[s, h, j] += sum over observed rows r of p[r, j], p = softmax of the
 // causal logits of the group's queries. K is read, V is not; the prompt's outputs are the prefill kernels' business.
 //
-// Two passes over the logits: the first leaves every observed row's maximum and sum, the second adds up the weights of a tile of keys over all
-// rows. Every output has one writer, and sums have one order.
+// The normaliser of a row is known when all of its keys are done, so the logits are computed twice:
+//   rows pass   256 query rows stay in shared memory, tiles of keys go by; a thread owns a row and keeps its maximum and sum
+//   keys pass   256 keys stay, tiles of query rows go by; a thread owns a key and adds up 2^(z - normaliser of the row)
+// Both are the same kernel with the operands exchanged: what a thread owns is a lane of the accumulator in tensor memory, so that neither pass
+// sums across lanes. Query rows of a kv head are numbered token * G + head of the group, as in attention_rows.cu.
+//
+// Roles (512 threads, one CTA per SM): warps 0-3 and 4-7 own 128 lanes each, warps 8-11 stage what goes by (an e4m3 cache becomes f16, the
+// queries are then f16 scaled by a power of two per row, which the rows pass leaves in the workspace for the keys pass), warp 12 issues the
+// products into two accumulators for either half, so that products run under the exponentials.
+//
+// Long rows and long columns are cut into parts, by rules on the sequence's own lengths alone, and joined in order: every output has one writer and
+// every sum one order.
+#include "attention_rows.cuh"
 #include "common.cuh"
 #include "kv_mass.h"
 
 namespace {
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
+using namespace mbr;
 
-// observed rows of a sequence, and its cached tokens; a length beyond what the call was sized for is reported and cut
+constexpr int kThreads = 512, kMaxKeyParts = 32, kMaxRowParts = 16, kInfo = 8;
+template <int N>
+__device__ __forceinline__ void more_regs() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void fewer_regs() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
+// observed rows of a sequence, and its cached tokens; what the call was not sized for is reported and cut
 struct Span {
-  int n, q_len, rows, q0;      // cached tokens, tokens of the portion, observed rows (tokens x group), first observed token
+  int n, rows, tok0, past;     // cached tokens, observed rows (tokens x group), first observed token, tokens in front of the portion (may be negative)
 };
 __device__ __forceinline__ Span span_of(const MbMassArgs& a, int s, int G) {
-  Span x;
-  x.n = a.ctx_len[s];
-  x.q_len = a.q_len[s];
-  if (x.n > a.max_ctx || x.q_len > a.max_q_len) {
-    if (a.status && threadIdx.x == 0) atomicCAS(a.status, 0u, MB_ST_BOUNDS);
-    x.n = min(x.n, a.max_ctx);
-    x.q_len = min(x.q_len, a.max_q_len);
+  int n = a.ctx_len[s], ql = a.q_len[s];
+  const long long start = a.q_start[s];
+  bool bad = n > a.max_ctx || ql > a.max_q_len;
+  n = max(min(n, a.max_ctx), 0);
+  ql = max(min(ql, a.max_q_len), 0);
+  if (start < 0 || start + ql > a.q_rows) {
+    bad = true;
+    ql = 0;
   }
-  x.n = max(x.n, 0);
-  x.q_len = max(x.q_len, 0);
-  if (a.q_start[s] < 0 || a.q_start[s] + (long long)x.q_len > a.q_rows) {
-    if (a.status && threadIdx.x == 0) atomicCAS(a.status, 0u, MB_ST_BOUNDS);
-    x.q_len = 0;
-  }
-  const int seen = min(a.last, x.q_len);
-  x.q0 = x.q_len - seen;
-  x.rows = seen * G;
-  return x;
+  if (bad && a.status && threadIdx.x == 0) atomicCAS(a.status, 0u, MB_ST_BOUNDS);
+  const int seen = min(a.last, ql);
+  return {n, seen * G, (int)start + ql - seen, n - seen};
 }
 
-template <bool FP8>
-__device__ __forceinline__ float logit(const MbMassArgs& a, const float* q, long long at) {
-  float acc = 0.f;
-  for (int d = 0; d < a.D; ++d)
-    acc += q[d] * (FP8 ? mb::e4m3_to_float(reinterpret_cast<const uint8_t*>(a.k_cache)[at + d])
-                       : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(a.k_cache)[at + d]));
-  return acc;
+// Keys of a part of a row, rows of a part of a column: few rows want many parts to fill the chip, many rows do that by themselves.
+__host__ __device__ __forceinline__ int key_part(int n, int rows) {
+  const int least = rows <= 512 ? 512 : rows <= 4096 ? 2048 : 8192, even = ((n + kMaxKeyParts - 1) / kMaxKeyParts + 127) & ~127;
+  return even > least ? even : least;
 }
-__device__ __forceinline__ long long row_at(const MbMassArgs& a, int s, int h, int j) {
-  const int bi = j / a.block_size;
-  int b = __ldg(a.block_table + s * a.table_ld + bi);
-  if ((unsigned)b >= (unsigned long long)a.num_blocks) {
-    if (a.status) atomicCAS(a.status, 0u, MB_ST_BOUNDS);
-    b = 0;
-  }
-  return (((long long)b * a.block_size + (j - bi * a.block_size)) * a.Hkv + h) * a.D;
+__host__ __device__ __forceinline__ int row_part(int rows) {
+  const int even = ((rows + kMaxRowParts - 1) / kMaxRowParts + 127) & ~127;
+  return even > 4096 ? even : 4096;
+}
+__host__ __device__ __forceinline__ int parts_of(int n, int part) { return n <= part ? 1 : (n + part - 1) / part; }
+
+// Workspace: {maximum, sum} of every row and part of its keys, log2 domain [seqs * Hkv * rows, key parts]; with an e4m3 cache the f16 queries
+// and the power of two that a row's scores are too large by; sums of the columns' parts [row parts, seqs * Hkv, columns]
+struct Ws {
+  long long rows, cols;
+  int key_parts, row_parts;
+  size_t q, scale, sums, bytes;
+};
+inline Ws workspace(int seqs, int Hq, int Hkv, int D, int seen, int max_ctx, bool fp8) {
+  Ws w;
+  w.rows = (long long)seen * (Hq / Hkv);
+  w.cols = (max_ctx + 3) & ~3ll;
+  // more parts than any sequence of the call has: fewer rows than the most may mean more of them
+  w.key_parts = parts_of(max_ctx, 512) < kMaxKeyParts ? parts_of(max_ctx, 512) : kMaxKeyParts;
+  w.row_parts = parts_of((int)w.rows, row_part((int)w.rows));
+  const size_t n = (size_t)seqs * Hkv * w.rows;
+  w.q = (n * w.key_parts * 8 + 15) & ~size_t(15);            // the queries are read and written in vectors of 16 bytes
+  w.scale = w.q + (fp8 ? n * D * 2 : 0);
+  w.sums = w.scale + (fp8 ? n * 4 : 0);
+  w.sums = (w.sums + 15) & ~size_t(15);
+  w.bytes = w.sums + (w.row_parts > 1 ? (size_t)w.row_parts * seqs * Hkv * w.cols * 4 : 0);
+  return w;
 }
 
-// One warp an observed row: log2 of its sum, in the log2 domain. Row r is token r / G of the observed ones, head r % G of the group.
-template <bool FP8>
-__global__ void __launch_bounds__(256) observe_rows_kernel(const MbMassArgs a, int max_rows) {
-  __shared__ float sq[8][256];
-  const int G = a.Hq / a.Hkv, h = blockIdx.y, s = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = blockIdx.x * 8 + warp;
+template <int D, bool FP8, bool KEYS>
+struct Cfg {
+  static constexpr int kN = D == 256 ? 64 : 128;             // rows of a tile that goes by
+  static constexpr int kHalves = D / 64;                     // spans of 128 bytes across a row
+  static constexpr int kStages = D == 256 ? 2 : 4;
+  // A row's factors outlive its tile: those of tile j + kInfo are written when the products of tile j + kInfo - kStages are done, whose accumulators were
+  // given back behind tile j + kInfo - kStages - 3 at least.
+  static_assert(kInfo >= kStages + 3, "factors would be written over while they are read");
+  static constexpr int kHeldB = 256 * D * 2, kTileB = kN * D * 2;
+  static constexpr int kSmem = kHeldB + kStages * kTileB + 1024;
+  static constexpr uint32_t kCols = 4 * kN;                  // two halves of the lanes, two accumulators each
+};
+
+template <int D, bool FP8, bool KEYS>
+__global__ void __launch_bounds__(kThreads, 1) observe_kernel(const MbMassArgs a, const Ws ws, int g_magic) {
+  using C = Cfg<D, FP8, KEYS>;
+  constexpr int kN = C::kN, kHalves = C::kHalves, kStages = C::kStages;
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  uint8_t* sHeld = smem_raw + ((1024u - (mb::smem_u32(smem_raw) & 1023u)) & 1023u);   // 2 x kHalves x [128 rows x 128 B]
+  uint8_t* sTile = sHeld + C::kHeldB;                        // kStages x kHalves x [kN rows x 128 B]
+  __shared__ __align__(8) uint64_t held_full, full[kStages], empty[kStages], info_full[kInfo], s_full[2][2], s_free[2][2];
+  __shared__ uint32_t s_tmem;
+  __shared__ float s_row[256];                               // rows pass, e4m3: what a row's scores are too large by
+  __shared__ __align__(16) float4 s_info[kInfo][kN / 2];     // keys pass: factors and normalisers of two query rows
+  const int h = blockIdx.y, s = blockIdx.z, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int G = a.Hq / a.Hkv;
+  mb::pdl_wait();
   const Span x = span_of(a, s, G);
-  if (r >= x.rows) return;
-  const int tok = x.q0 + r / G, limit = min(x.n, x.n - x.q_len + tok + 1);
-  const __nv_bfloat16* q = reinterpret_cast<const __nv_bfloat16*>(a.q) + ((size_t)(a.q_start[s] + tok) * a.Hq + h * G + r % G) * a.D;
-  for (int d = lane; d < a.D; d += 32) sq[warp][d] = __bfloat162float(q[d]);
-  __syncwarp();
-  const float sc = a.scale * (FP8 ? *a.k_scale : 1.f) * 1.44269504088896f;
-  float m = -INFINITY, l = 0.f;
-  for (int j = lane; j < limit; j += 32) {
-    const float z = logit<FP8>(a, sq[warp], row_at(a, s, h, j)) * sc, mx = fmaxf(m, z);
-    const float use = mx == -INFINITY ? 0.f : mx;
-    l = l * ex2(m - use) + ex2(z - use);
-    m = mx;
+  const int kp = key_part(x.n, x.rows), kparts = parts_of(x.n, kp), rp = row_part(x.rows), rparts = parts_of(x.rows, rp);
+  auto tok_of = [&](int r) { return G == 1 ? r : (int)__umulhi((unsigned)r, (unsigned)g_magic); };
+  auto limit_of = [&](int r) { return x.past + tok_of(r) + 1; };       // keys in front of this one are visible to row r
+  // ---- what stays, and the range of what goes by
+  const int parts = KEYS ? rparts : kparts, blocks = gridDim.x / (KEYS ? ws.row_parts : ws.key_parts);
+  const int part = blockIdx.x / blocks, at0 = (KEYS ? (int)blockIdx.x % blocks : blocks - 1 - (int)blockIdx.x % blocks) * 256;   // the longest first
+  const int own = KEYS ? x.n : x.rows;
+  if (part >= parts || at0 >= own || x.rows == 0 || x.n == 0) return;
+  const bool two = own - at0 > 128;
+  int begin, end;
+  if constexpr (KEYS) {
+    // the first row that sees the first of these keys
+    const int first = max(0, at0 - x.past) * G;
+    begin = max(part * rp, first & ~(kN - 1));
+    end = min(x.rows, (part + 1) * rp);
+  } else {
+    begin = part * kp;
+    end = min(min(x.n, begin + kp), limit_of(min(x.rows, at0 + 256) - 1));
   }
-  const float top = mb::warp_max(m), use = top == -INFINITY ? 0.f : top;
-  l = mb::warp_sum(l * ex2(m - use));
-  if (lane == 0) reinterpret_cast<float*>(a.ws)[((size_t)s * a.Hkv + h) * max_rows + r] = l == 0.f ? INFINITY : top + log2f(l);
+  const int tiles = end > begin ? (end - begin + kN - 1) / kN : 0;
+  const size_t row0 = ((size_t)s * a.Hkv + h) * ws.rows;     // of the workspace's rows
+  float2* ml = reinterpret_cast<float2*>(a.ws) + row0 * ws.key_parts;
+  __half* wq = reinterpret_cast<__half*>(reinterpret_cast<uint8_t*>(a.ws) + ws.q) + row0 * D;
+  float* wscale = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(a.ws) + ws.scale) + row0;
+
+  if (tid == 0) {
+    mb::mbar_init(&held_full, 8);
+    for (int i = 0; i < kStages; ++i) {
+      mb::mbar_init(&full[i], 4);
+      mb::mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < kInfo; ++i) mb::mbar_init(&info_full[i], 4);
+    for (int i = 0; i < 4; ++i) {
+      mb::mbar_init(&s_full[i >> 1][i & 1], 1);
+      mb::mbar_init(&s_free[i >> 1][i & 1], 4);
+    }
+    mb::mbar_fence_init();
+  }
+  if (warp == 12) mb::tmem_alloc(&s_tmem, C::kCols);
+  mb::tc_fence_before();
+  __syncthreads();
+  mb::tc_fence_after();
+  const uint32_t tmem = s_tmem;
+
+  // ---- where rows of either operand come from
+  const int* table = a.block_table + s * a.table_ld;
+  const int shift = (a.block_size & (a.block_size - 1)) == 0 ? 31 - __clz(a.block_size) : -1;
+  int bad = 0;
+  auto key_at = [&](int j) -> long long {                    // byte offset of cached row j < n of this kv head
+    const int bi = shift >= 0 ? j >> shift : j / a.block_size;
+    int b = __ldg(table + bi);
+    const bool out = (unsigned)b >= (unsigned long long)a.num_blocks;
+    bad |= out;
+    b = out ? 0 : b;
+    return (((long long)b * a.block_size + (j - bi * a.block_size)) * a.Hkv + h) * (D * (FP8 ? 1 : 2));
+  };
+  auto query_at = [&](int r) -> const __nv_bfloat16* {
+    const int tq = tok_of(r);
+    return reinterpret_cast<const __nv_bfloat16*>(a.q) + ((size_t)(x.tok0 + tq) * a.Hq + h * G + (r - tq * G)) * D;
+  };
+  // of a row's scores, in the log2 domain; never 0, which would make numbers of the -inf that a mask leaves
+  auto factor = [&](float row) { return fmaxf(a.scale * (FP8 ? *a.k_scale : 1.f) * 1.44269504088896f * row, 1.17549435e-38f); };
+  // 16 e4m3 values as the two 16-byte pieces of f16 that they are
+  auto widen = [](const uint4& raw, uint4& lo, uint4& hi) {
+    lo = make_uint4(e4m3x2(raw.x), e4m3x2(raw.x >> 16), e4m3x2(raw.y), e4m3x2(raw.y >> 16));
+    hi = make_uint4(e4m3x2(raw.z), e4m3x2(raw.z >> 16), e4m3x2(raw.w), e4m3x2(raw.w >> 16));
+  };
+
+  if (warp < 8) {
+    more_regs<184>();
+    const int w = warp >> 2, r = tid & 127, mine = at0 + w * 128 + r;
+    // ---- the operand that stays: 256 rows, rows behind the last one are zeros
+    constexpr int kPieces = KEYS && FP8 ? D / 16 : D / 8, kStep = 256 / kPieces, kLoads = 256 / kStep;
+    const int c = tid % kPieces;
+#pragma unroll 1
+    for (int i0 = 0; i0 < kLoads; i0 += 16) {
+      constexpr int kBatch = kLoads < 16 ? kLoads : 16;
+      uint4 v[kBatch];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const int hr = tid / kPieces + kStep * (i0 + i), at = min(at0 + hr, own - 1);
+        if constexpr (KEYS)
+          v[i] = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(a.k_cache) + key_at(at)) + c);
+        else
+          v[i] = __ldg(reinterpret_cast<const uint4*>(query_at(at)) + c);
+        if (at0 + hr >= own) v[i] = make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const int hr = tid / kPieces + kStep * (i0 + i);
+        uint8_t* dst = sHeld + (hr >> 7) * (128 * D * 2);
+        if constexpr (KEYS && FP8) {
+          uint4 lo, hi;
+          widen(v[i], lo, hi);
+          *reinterpret_cast<uint4*>(dst + (c >> 2) * (128 * 128) + sw_off(hr & 127, (c & 3) * 2)) = lo;
+          *reinterpret_cast<uint4*>(dst + (c >> 2) * (128 * 128) + sw_off(hr & 127, (c & 3) * 2 + 1)) = hi;
+        } else {
+          if constexpr (FP8) {
+            // f16 has less range than bf16: the power of two that takes the row's largest element to [2^14, 2^15); bits of a bf16 without its
+            // sign order like the values
+            const uint32_t y[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+            uint32_t top = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) top = __vmaxu2(top, y[j] & 0x7fff7fffu);
+#pragma unroll
+            for (int d = 1; d < kPieces; d <<= 1) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, d));
+            const int e = (int)(max(top & 0xffff, top >> 16) >> 7);
+            const int up = e == 255 ? 0 : 141 - max(e, 15);  // zeros and subnormal rows as if their exponent were 15, infinities and NaN as they are
+            const float f = __int_as_float((127 + up) << 23);
+            uint32_t z[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float2 t = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&y[j]));
+              z[j] = pack2<true>(t.x * f, t.y * f);
+            }
+            v[i] = make_uint4(z[0], z[1], z[2], z[3]);
+            if (c == 0) s_row[hr] = __int_as_float((127 - up) << 23);
+            if (part == 0 && at0 + hr < own) {
+              reinterpret_cast<uint4*>(wq + (size_t)(at0 + hr) * D)[c] = v[i];
+              if (c == 0) wscale[at0 + hr] = __int_as_float((127 - up) << 23);
+            }
+          }
+          *reinterpret_cast<uint4*>(dst + (c >> 3) * (128 * 128) + sw_off(hr & 127, c & 7)) = v[i];
+        }
+      }
+    }
+    fence_async_smem();
+    __syncwarp();
+    if (lane == 0) mb::mbar_arrive(&held_full);
+    if constexpr (FP8 && !KEYS) asm volatile("bar.sync 1, 256;" ::: "memory");       // the rows' scales come from other warps
+    const float sc = factor(FP8 && !KEYS ? s_row[w * 128 + r] : 1.f);
+    const int limit = KEYS ? 0 : mine < own ? limit_of(mine) : 0;
+    const uint32_t tS = tmem + ((uint32_t)((warp & 3) * 32) << 16) + w * 2 * kN;
+    float m_run = -INFINITY, l_run = 0.f;                    // keys pass: l_run is the column's sum
+    bool ok = true;
+    const int count = w == 0 || two ? tiles : 0;
+    for (int t = 0; t < count; ++t) {
+      const int b = t & 1;
+      ok = mb::mbar_wait(&s_full[w][b], (t >> 1) & 1, a.status, MB_ST_TIMEOUT_MMA);
+      if (KEYS) ok = ok && mb::mbar_wait(&info_full[t % kInfo], (t / kInfo) & 1, a.status, MB_ST_TIMEOUT_TMA);
+      if (!__all_sync(0xffffffffu, ok)) {
+        ok = false;
+        break;
+      }
+      mb::tc_fence_after();
+      float z[kN];
+#pragma unroll
+      for (int i = 0; i < kN; i += 32) mb::tmem_ld32_async(tS + b * kN + i, z + i);
+      mb::tmem_ld_wait(z);
+      mb::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mb::mbar_arrive(&s_free[w][b]);         // the accumulator is in registers
+      const int from = begin + t * kN;
+      float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+      if constexpr (KEYS) {
+        const float4* info = s_info[t % kInfo];
+        // the tile's first row sees the least: all of these keys, or a row each is asked
+        if (__any_sync(0xffffffffu, mine >= limit_of(from))) {
+#pragma unroll
+          for (int i = 0; i < kN; ++i)
+            if (mine >= limit_of(from + i)) z[i] = -INFINITY;
+        }
+#pragma unroll
+        for (int i = 0; i < kN / 2; ++i) {
+          const float4 f = info[i];
+          float2 p = fma2(make_float2(z[2 * i], z[2 * i + 1]), make_float2(f.x, f.y), make_float2(f.z, f.w));
+          p.x = ex2(p.x);
+          p.y = ex2(p.y);
+          sum[i & 1] = add2(sum[i & 1], p);
+        }
+        l_run += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+      } else {
+        const int seen = min(limit, end) - from;             // columns in front of this one are visible
+        if (!__all_sync(0xffffffffu, seen >= kN)) {
+#pragma unroll
+          for (int i = 0; i < kN; ++i)
+            if (i >= seen) z[i] = -INFINITY;
+        }
+        float mx4[4] = {z[0], z[1], z[2], z[3]};
+#pragma unroll
+        for (int i = 4; i < kN; ++i) mx4[i & 3] = fmaxf(mx4[i & 3], z[i]);
+        const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * sc;
+        if (mx > m_run + 8.f) {                              // also true on a row's first finite tile
+          l_run *= ex2(m_run - mx);
+          m_run = mx;
+        }
+        const float nm = m_run == -INFINITY ? 0.f : -m_run;
+        const float2 sc2 = make_float2(sc, sc), nm2 = make_float2(nm, nm);
+#pragma unroll
+        for (int i = 0; i < kN / 2; ++i) {
+          float2 p = fma2(make_float2(z[2 * i], z[2 * i + 1]), sc2, nm2);
+          p.x = ex2(p.x);
+          p.y = ex2(p.y);
+          sum[i & 1] = add2(sum[i & 1], p);
+        }
+        l_run += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+      }
+    }
+    if (mine < own) {
+      if constexpr (KEYS) {
+        if (ws.row_parts > 1)
+          reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(a.ws) + ws.sums)[((size_t)part * a.num_seqs * a.Hkv + (size_t)s * a.Hkv + h) * ws.cols + mine] = l_run;
+        else
+          a.mass[s * a.mass_seq + h * a.mass_head + mine] += l_run;
+      } else {
+        ml[(size_t)mine * ws.key_parts + part] = make_float2(m_run, l_run);
+      }
+    }
+    mb::tc_fence_before();
+  } else if (warp < 12) {
+    // ------------------------------------------------------------ what goes by
+    fewer_regs<80>();
+    const int t = tid - 256;
+    constexpr bool kWiden = FP8 && !KEYS;
+    constexpr int kPieces = kWiden ? D / 16 : D / 8, kStep = 128 / kPieces, kLoads = kN / kStep;
+    const int r0 = t / kPieces, c = t % kPieces;
+    bool ok = true;
+    auto announce = [&](int j) {
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        mb::mbar_arrive(&full[j % kStages]);
+        if (KEYS) mb::mbar_arrive(&info_full[j % kInfo]);
+      }
+    };
+    if constexpr (kWiden) {
+      uint4 raw[kLoads];
+      auto fetch = [&](int j) {
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+          const int k = begin + j * kN + r0 + i * kStep;
+          raw[i] = k < end ? __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(a.k_cache) + key_at(k)) + c) : make_uint4(0, 0, 0, 0);
+        }
+      };
+      fetch(0);
+      for (int j = 0; j < tiles; ++j) {
+        ok = mb::mbar_wait(&empty[j % kStages], ((j / kStages) & 1) ^ 1, a.status, MB_ST_TIMEOUT_TMA);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        uint8_t* tile = sTile + (j % kStages) * C::kTileB + (c >> 2) * (kN * 128);
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+          uint4 lo, hi;
+          widen(raw[i], lo, hi);
+          *reinterpret_cast<uint4*>(tile + sw_off(r0 + i * kStep, (c & 3) * 2)) = lo;
+          *reinterpret_cast<uint4*>(tile + sw_off(r0 + i * kStep, (c & 3) * 2 + 1)) = hi;
+        }
+        announce(j);
+        fetch(j + 1);
+      }
+    } else {
+      constexpr int kLag = kStages - 1;                      // tiles under way while the next is asked for
+      for (int j = 0; j < tiles; ++j) {
+        ok = mb::mbar_wait(&empty[j % kStages], ((j / kStages) & 1) ^ 1, a.status, MB_ST_TIMEOUT_TMA);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        uint8_t* tile = sTile + (j % kStages) * C::kTileB + (c >> 3) * (kN * 128);
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+          const int at = begin + j * kN + r0 + i * kStep, safe = min(at, end - 1);
+          const void* src;
+          if constexpr (!KEYS) src = reinterpret_cast<const uint8_t*>(a.k_cache) + key_at(safe);
+          else if constexpr (FP8) src = wq + (size_t)safe * D;
+          else src = query_at(safe);
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(mb::smem_u32(tile + sw_off(r0 + i * kStep, c & 7))),
+                       "l"(reinterpret_cast<const uint4*>(src) + c), "r"(at < end ? 16 : 0)
+                       : "memory");
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        if constexpr (KEYS) {
+          // a row's normaliser from the parts of its keys, in order; rows behind the last one add nothing
+          if (t < kN) {
+            const int at = begin + j * kN + t;
+            float f = 1.f, lse = INFINITY;
+            if (at < end) {
+              const float2* p = ml + (size_t)at * ws.key_parts;
+              float m = -INFINITY, l = 0.f;
+              for (int i = 0; i < kparts; ++i) {
+                const float2 y = p[i];
+                const float top = fmaxf(m, y.x);
+                l = (m == -INFINITY ? 0.f : l * ex2(m - top)) + (y.x == -INFINITY ? 0.f : y.y * ex2(y.x - top));
+                m = top;
+              }
+              f = factor(FP8 ? wscale[at] : 1.f);
+              if (l != 0.f) lse = m + log2f(l);
+            }
+            float* info = reinterpret_cast<float*>(&s_info[j % kInfo][t >> 1]) + (t & 1);
+            info[0] = f;
+            info[2] = -lse;
+          }
+        }
+        if (j >= kLag) {
+          asm volatile("cp.async.wait_group %0;" ::"n"(kLag) : "memory");
+          announce(j - kLag);
+        }
+      }
+      if (__all_sync(0xffffffffu, ok)) {
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        for (int j = max(0, tiles - kLag); j < tiles; ++j) announce(j);
+      }
+      asm volatile("cp.async.wait_all;" ::: "memory");
+    }
+  } else {
+    fewer_regs<48>();
+    if (warp == 12 && mb::elect_one()) {
+      // ---------------------------------------------------------- products
+      constexpr uint32_t kF = FP8 ? 0 : 1, kId = mb::umma_idesc(kF, kF, 128, kN);
+      const uint32_t aH = mb::smem_u32(sHeld), aT = mb::smem_u32(sTile);
+      bool ok = mb::mbar_wait(&held_full, 0, a.status, MB_ST_TIMEOUT_MMA);
+      for (int j = 0; j < tiles && ok; ++j) {
+        const int st = j % kStages, b = j & 1;
+        ok = mb::mbar_wait(&full[st], (j / kStages) & 1, a.status, MB_ST_TIMEOUT_MMA);
+        for (int w = 0; w < (two ? 2 : 1) && ok; ++w) {
+          ok = mb::mbar_wait(&s_free[w][b], ((j >> 1) & 1) ^ 1, a.status, MB_ST_TIMEOUT_MMA);
+          if (!ok) break;
+          mb::tc_fence_after();
+#pragma unroll
+          for (int hh = 0; hh < kHalves; ++hh)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              mb::umma_f16(tmem + (w * 2 + b) * kN, mb::umma_desc_sw128(aH + w * (128 * D * 2) + hh * (128 * 128) + k * 32),
+                           mb::umma_desc_sw128(aT + st * C::kTileB + hh * (kN * 128) + k * 32), kId, (hh | k) != 0);
+          mb::tc_commit(&s_full[w][b]);
+        }
+        if (ok) mb::tc_commit(&empty[st]);
+      }
+      // nobody may free the accumulators under products in flight
+      if (ok && tiles > 0) mb::mbar_wait(&empty[(tiles - 1) % kStages], ((tiles - 1) / kStages) & 1, a.status, MB_ST_TIMEOUT_MMA);
+    }
+    __syncwarp();
+  }
+  if (bad && a.status) atomicCAS(a.status, 0u, MB_ST_BOUNDS);
+  __syncthreads();
+  if (warp == 12) {
+    mb::tc_fence_after();
+    mb::tmem_dealloc(tmem, C::kCols);
+  }
 }
 
-// One thread a cached token: its weights over all observed rows.
-template <bool FP8>
-__global__ void __launch_bounds__(128) observe_keys_kernel(const MbMassArgs a, int max_rows) {
-  __shared__ float sq[256];
-  const int G = a.Hq / a.Hkv, h = blockIdx.y, s = blockIdx.z, j = blockIdx.x * 128 + threadIdx.x;
-  const Span x = span_of(a, s, G);
-  if (blockIdx.x * 128 >= x.n) return;
-  const float sc = a.scale * (FP8 ? *a.k_scale : 1.f) * 1.44269504088896f;
-  const float* lse = reinterpret_cast<const float*>(a.ws) + ((size_t)s * a.Hkv + h) * max_rows;
-  const long long at = j < x.n ? row_at(a, s, h, j) : 0;
+// Columns whose rows were cut into parts: their sums in order.
+__global__ void __launch_bounds__(256) observe_join_kernel(const MbMassArgs a, const Ws ws) {
+  const int h = blockIdx.y, s = blockIdx.z, j = blockIdx.x * 256 + threadIdx.x;
+  mb::pdl_wait();
+  const Span x = span_of(a, s, a.Hq / a.Hkv);
+  if (j >= x.n || x.rows == 0) return;
+  const int parts = parts_of(x.rows, row_part(x.rows));
+  const float* sums = reinterpret_cast<const float*>(reinterpret_cast<const uint8_t*>(a.ws) + ws.sums) + ((size_t)s * a.Hkv + h) * ws.cols + j;
   float sum = 0.f;
-  for (int r = 0; r < x.rows; ++r) {
-    const int tok = x.q0 + r / G, limit = x.n - x.q_len + tok + 1;
-    const __nv_bfloat16* q = reinterpret_cast<const __nv_bfloat16*>(a.q) + ((size_t)(a.q_start[s] + tok) * a.Hq + h * G + r % G) * a.D;
-    __syncthreads();
-    for (int d = threadIdx.x; d < a.D; d += 128) sq[d] = __bfloat162float(q[d]);
-    __syncthreads();
-    if (j < limit && j < x.n) sum += ex2(logit<FP8>(a, sq, at) * sc - lse[r]);
-  }
-  if (j < x.n) a.mass[s * a.mass_seq + h * a.mass_head + j] += sum;
+  for (int p = 0; p < parts; ++p) sum += sums[(size_t)p * a.num_seqs * a.Hkv * ws.cols];
+  a.mass[s * a.mass_seq + h * a.mass_head + j] += sum;
 }
 
-template <bool FP8>
-int launch(const MbMassArgs& a, int max_rows, cudaStream_t stream) {
-  observe_rows_kernel<FP8><<<dim3((max_rows + 7) / 8, a.Hkv, a.num_seqs), 256, 0, stream>>>(a, max_rows);
-  const cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return (int)e;
-  observe_keys_kernel<FP8><<<dim3((a.max_ctx + 127) / 128, a.Hkv, a.num_seqs), 128, 0, stream>>>(a, max_rows);
-  return (int)cudaGetLastError();
+template <int D, bool FP8, bool KEYS>
+int launch(const MbMassArgs& a, const Ws& ws, cudaStream_t stream) {
+  auto kern = observe_kernel<D, FP8, KEYS>;
+  static bool configured = false;
+  if (!configured) {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D, FP8, KEYS>::kSmem);
+    if (e != cudaSuccess) return (int)e;
+    configured = true;
+  }
+  const int G = a.Hq / a.Hkv;
+  const unsigned magic = G == 1 ? 0 : (unsigned)(((1ull << 32) + G - 1) / G);
+  const long long blocks = ((KEYS ? (long long)a.max_ctx : ws.rows) + 255) / 256 * (KEYS ? ws.row_parts : ws.key_parts);
+  if (blocks > 0x7fffffffll) return MB_ERR_TOO_LARGE;
+  return (int)mb::launch_kernel_ex(kern, dim3((unsigned)blocks, a.Hkv, a.num_seqs), dim3(kThreads), Cfg<D, FP8, KEYS>::kSmem, stream, 1, KEYS, a, ws, (int)magic);
+}
+
+template <int D, bool FP8>
+int both(const MbMassArgs& a, const Ws& ws, cudaStream_t stream) {
+  const int rc = launch<D, FP8, false>(a, ws, stream);
+  return rc ? rc : launch<D, FP8, true>(a, ws, stream);
 }
 
 }  // namespace
 
 extern "C" {
 
-size_t mb_prompt_mass_ws(int num_seqs, int Hq, int seen) { return (size_t)num_seqs * Hq * seen * 4; }
+size_t mb_prompt_mass_ws(int num_seqs, int Hq, int Hkv, int D, int seen, int max_ctx, int fp8) { return workspace(num_seqs, Hq, Hkv, D, seen, max_ctx, fp8 != 0).bytes; }
 
 int mb_prompt_mass(const MbMassArgs* a, cudaStream_t stream) {
   if (!a || a->num_seqs <= 0 || a->num_seqs > 65535 || a->Hkv <= 0 || a->Hkv > 65535 || a->Hq % a->Hkv || (a->D != 64 && a->D != 128 && a->D != 256) ||
       a->block_size <= 0 || a->num_blocks <= 0 || a->max_ctx <= 0 || a->last <= 0 || a->last > a->max_q_len || !a->q || !a->k_cache || !a->block_table ||
       !a->q_start || !a->q_len || !a->ctx_len || !a->mass || (a->fp8 && !a->k_scale))
     return MB_ERR_BAD_ARG;
-  const size_t need = mb_prompt_mass_ws(a->num_seqs, a->Hq, a->last);
-  if (!a->ws || a->ws_bytes < need) return MB_ERR_TOO_LARGE;
-  const long long max_rows = (long long)a->last * (a->Hq / a->Hkv);
-  if (max_rows > (1ll << 30)) return MB_ERR_TOO_LARGE;
-  return a->fp8 ? launch<true>(*a, (int)max_rows, stream) : launch<false>(*a, (int)max_rows, stream);
+  if ((reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->k_cache) | reinterpret_cast<uintptr_t>(a->ws)) & 15) return MB_ERR_UNSUPPORTED;
+  if ((long long)a->last * (a->Hq / a->Hkv) > (1ll << 25)) return MB_ERR_TOO_LARGE;     // rows that tok_of divides exactly
+  const Ws ws = workspace(a->num_seqs, a->Hq, a->Hkv, a->D, a->last, a->max_ctx, a->fp8 != 0);
+  if (!a->ws || a->ws_bytes < ws.bytes) return MB_ERR_TOO_LARGE;
+  int rc;
+  if (a->D == 64) rc = a->fp8 ? both<64, true>(*a, ws, stream) : both<64, false>(*a, ws, stream);
+  else if (a->D == 128) rc = a->fp8 ? both<128, true>(*a, ws, stream) : both<128, false>(*a, ws, stream);
+  else rc = a->fp8 ? both<256, true>(*a, ws, stream) : both<256, false>(*a, ws, stream);
+  if (rc || ws.row_parts == 1) return rc;
+  return (int)mb::launch_kernel_ex(observe_join_kernel, dim3((a->max_ctx + 255) / 256, a->Hkv, a->num_seqs), dim3(256), 0, stream, 1, true, *a, ws);
 }
 
 }  // extern "C"

@@ -89,7 +89,8 @@ def _check_places(where, tensors) -> None:
     _refuse(dev.type == "cuda" and dev.index != torch.cuda.current_device(), f"{where}: tensors lie on {dev}, the current device is another one")
 
 
-def _check_scales(where, cache, scales) -> None:
+def _check_scales(where, cache, scale, scales) -> None:
+    _refuse(not scale > 0, f"{where}: scale is positive")
     _refuse(cache.dtype == torch.uint8 and any(s is None or s.dtype != torch.float32 or s.numel() < 1 for s in scales), f"{where}: an e4m3 cache comes with fp32 scales")
 
 
@@ -118,7 +119,7 @@ def paged_attention_mass(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     Hq = q.shape[1]
     _refuse(Hq == 0 or Hq % Hkv != 0 or Hq // Hkv > MAX_GROUP, f"{where}: {Hq} query heads over {Hkv} kv heads: whole groups of up to {MAX_GROUP}")
     _refuse(not _rows_apart(mass), f"{where}: rows of mass share memory")
-    _check_scales(where, k_cache, (k_scale, v_scale))
+    _check_scales(where, k_cache, scale, (k_scale, v_scale))
     _check_places(where, (q, k_cache, v_cache, block_table, ctx_len, mass, k_scale, v_scale))
     if not q.is_cuda:
         return ref.paged_attention_mass(q, k_cache, v_cache, block_table, ctx_len, mass, scale, k_scale, v_scale)
@@ -156,7 +157,7 @@ def prompt_mass(q: torch.Tensor, k_cache: torch.Tensor, block_table: torch.Tenso
     _refuse(any(x.dtype != torch.int32 or x.shape != ctx_len.shape or not x.is_contiguous() for x in (q_start, q_len)), f"{where}: q_start and q_len are int32 [sequences]")
     _refuse(last < 0 or max_q_len < 0, f"{where}: last and max_q_len are not negative")
     _refuse(not _rows_apart(mass), f"{where}: rows of mass share memory")
-    _check_scales(where, k_cache, (k_scale,))
+    _check_scales(where, k_cache, scale, (k_scale,))
     _check_places(where, (q, k_cache, block_table, q_start, q_len, ctx_len, mass, k_scale))
     if not q.is_cuda:
         return ref.prompt_mass(q, k_cache, block_table, q_start, q_len, ctx_len, mass, scale, last, k_scale)
@@ -164,7 +165,7 @@ def prompt_mass(q: torch.Tensor, k_cache: torch.Tensor, block_table: torch.Tenso
         return mass
     from . import _count, _ptr, _stream, runtime
     seen = min(last or max_q_len, max_q_len)
-    ws = torch.empty(_sizes("mb_prompt_mass_ws")(S, Hq, seen), dtype=torch.uint8, device=q.device)
+    ws = torch.empty(_sizes("mb_prompt_mass_ws")(S, Hq, Hkv, D, seen, max_ctx, int(k_cache.dtype == torch.uint8)), dtype=torch.uint8, device=q.device)
     rt = runtime(q.device)
     a = _MassArgs(_ptr(q), _ptr(k_cache), None, _ptr(block_table), block_table.stride(0), _ptr(q_start), _ptr(q_len), _ptr(ctx_len), _ptr(mass), mass.stride(0),
                   mass.stride(1), None, _ptr(ws), ws.numel(), _ptr(k_scale), None, _ptr(rt.status), nb, q.shape[0], S, Hq, Hkv, D, bs,

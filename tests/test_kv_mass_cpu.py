@@ -99,6 +99,7 @@ def _bad_decode():
     yield "mass order", dict(mass=lambda m: m.transpose(1, 2).contiguous().transpose(1, 2))
     yield "mass shared", dict(mass=lambda m: m[:1].expand(2, -1, -1))
     yield "mass heads", dict(mass=lambda m: m[:, :1])
+    yield "scale", dict(scale=lambda x: 0.0)
     yield "negative length", dict(max_ctx=lambda n: -1)
 
 
