@@ -1,0 +1,45 @@
+// Decode attention that leaves its logits: the kernel of attention_decode.cu for one new token a sequence, called by mb_attn_mass for the
+// calls that it serves. Beside attention itself a unit writes 4 bytes a token and query row; the join of kv_mass.cu makes weights of them.
+#include "attention_decode.cuh"
+#include "kv_mass.h"
+
+bool mb_decode_mass_serves(const MbMassArgs& a) {
+  const uintptr_t al = reinterpret_cast<uintptr_t>(a.k_cache) | reinterpret_cast<uintptr_t>(a.v_cache) | reinterpret_cast<uintptr_t>(a.q);
+  return a.Hq / a.Hkv <= (a.D == 256 ? 16 : 32) && a.num_seqs <= kMaxSeqs && a.block_size % kSlice == 0 && !(al & 15) &&
+         a.num_blocks * a.block_size < (1ll << 31) && a.table_ld < (1ll << 31);
+}
+
+int mb_decode_mass(const MbMassArgs& m, const mbm::DecodeWs& w, int part_tokens, cudaStream_t stream) {
+  AttnDecodeArgs a{};
+  a.k_cache = m.k_cache; a.v_cache = m.v_cache;
+  a.num_seqs = m.num_seqs; a.max_q_len = 1; a.Hq = m.Hq; a.Hkv = m.Hkv; a.block_size = m.block_size; a.num_blocks = m.num_blocks;
+  a.sm_count = m.sm_count;
+  uint8_t* ws = reinterpret_cast<uint8_t*>(m.ws);
+  DecodeParams p{};
+  p.q = reinterpret_cast<const __nv_bfloat16*>(m.q);
+  p.block_table = m.block_table; p.max_blocks = (int)m.table_ld; p.ctx_len = m.ctx_len;
+  p.num_seqs = m.num_seqs; p.Hq = m.Hq; p.Hkv = m.Hkv; p.G = m.Hq / m.Hkv; p.g_magic = (65536 + p.G - 1) / p.G;
+  p.block_size = m.block_size;
+  p.block_shift = (m.block_size & (m.block_size - 1)) == 0 ? 31 - __builtin_clz(m.block_size) : -1;
+  p.num_blocks = m.num_blocks; p.scale = m.scale; p.k_scale = m.k_scale; p.v_scale = m.v_scale;
+  p.out = reinterpret_cast<__nv_bfloat16*>(m.out); p.out_ld = (long long)m.Hq * m.D;
+  p.status = m.status;
+  p.part_tokens = part_tokens; p.parts = w.parts;
+  p.part_o = reinterpret_cast<float*>(ws + w.o); p.part_ml = reinterpret_cast<float2*>(ws + w.ml);
+  p.z = reinterpret_cast<float*>(ws + w.z); p.z_ld = w.ld; p.max_ctx = m.max_ctx;
+  auto run = [&](auto d, auto eight) {
+    auto go = [&](auto nt) { return launch<d.value, eight.value, nt.value, true>(a, p, stream); };
+    if (p.G <= 8) return go(std::integral_constant<int, 1>{});
+    if constexpr (d.value == 256) {
+      return go(std::integral_constant<int, 2>{});
+    } else {
+      if (p.G <= 16) return go(std::integral_constant<int, 2>{});
+      return p.G <= 24 ? go(std::integral_constant<int, 3>{}) : go(std::integral_constant<int, 4>{});
+    }
+  };
+  auto by_dim = [&](auto eight) {
+    return m.D == 64 ? run(std::integral_constant<int, 64>{}, eight) : m.D == 128 ? run(std::integral_constant<int, 128>{}, eight)
+                                                                                  : run(std::integral_constant<int, 256>{}, eight);
+  };
+  return m.fp8 ? by_dim(std::true_type{}) : by_dim(std::false_type{});
+}

@@ -39,7 +39,9 @@ __device__ __forceinline__ long long slot_of(const int* table, int j, int block_
   return (long long)b * block_size + (j - bi * block_size);
 }
 
-// ---------------------------------------------------------------- decode, any block size
+// ---------------------------------------------------------------- decode
+// The tensor cores' kernel (attention_decode_mass.cu) takes whole slices of 16 tokens, so blocks of a multiple of 16, and up to 32 query rows a
+// group (16 at dim 256). This one takes the rest.
 constexpr int kTile = 128, kThreads = 128, kPartTokens = 512;
 
 template <bool FP8>
@@ -150,10 +152,11 @@ __global__ void __launch_bounds__(kThreads) mass_part_kernel(const MbMassArgs a,
 constexpr int kChunk = 1024;
 
 // Columns [chunk * 1024, ...) of a (sequence, kv head): logits become weights, weights are added to the mass. The chunks share out the
-// group's outputs among themselves.
-__global__ void __launch_bounds__(256) mass_join_kernel(const MbMassArgs a, const mbm::DecodeWs w, int part_tokens) {
+// group's outputs among themselves; `whole`: those of a single partition stand already.
+__global__ void __launch_bounds__(256) mass_join_kernel(const MbMassArgs a, const mbm::DecodeWs w, int part_tokens, int whole) {
   __shared__ float s_lse[64];
   const int G = a.Hq / a.Hkv, chunk = blockIdx.x, h = blockIdx.y, s = blockIdx.z, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  mb::pdl_wait();
   const int n = context(a.ctx_len, s, a.max_ctx, a.status), chunks = max(1, (n + kChunk - 1) / kChunk);
   if (chunk >= chunks) return;
   const int parts = n ? mbm::part_count(n, part_tokens) : 0;
@@ -166,19 +169,39 @@ __global__ void __launch_bounds__(256) mass_join_kernel(const MbMassArgs a, cons
     if (lane == 0) s_lse[g] = l == 0.f ? INFINITY : mx + log2f(l);   // a row without weight adds none
   }
   __syncthreads();
-  const float* z = reinterpret_cast<const float*>(reinterpret_cast<const uint8_t*>(a.ws) + w.z) + row0 * w.ld;
-  float* mass = a.mass + s * a.mass_seq + h * a.mass_head;
-  for (int c = chunk * kChunk + tid; c < min(n, (chunk + 1) * kChunk); c += 256) {
-    float sum = 0.f;
-    for (int g = 0; g < G; ++g) sum += ex2(z[g * w.ld + c] - s_lse[g]);
-    mass[c] += sum;
+  const int c = chunk * kChunk + tid * 4;                   // four columns a thread; a row's columns behind its context up to ld are not read from
+  if (c < n) {
+    const float* z = reinterpret_cast<const float*>(reinterpret_cast<const uint8_t*>(a.ws) + w.z) + row0 * w.ld + c;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int g = 0; g < G; ++g) {
+      const float4 x = *reinterpret_cast<const float4*>(z + g * w.ld);
+      const float l = s_lse[g];
+      sum.x += ex2(x.x - l);
+      sum.y += ex2(x.y - l);
+      sum.z += ex2(x.z - l);
+      sum.w += ex2(x.w - l);
+    }
+    float* mass = a.mass + s * a.mass_seq + h * a.mass_head + c;
+    if (c + 4 <= n && !(reinterpret_cast<uintptr_t>(mass) & 15)) {
+      float4 y = *reinterpret_cast<float4*>(mass);
+      y.x += sum.x; y.y += sum.y; y.z += sum.z; y.w += sum.w;
+      *reinterpret_cast<float4*>(mass) = y;
+    } else {
+      mass[0] += sum.x;
+      if (c + 1 < n) mass[1] += sum.y;
+      if (c + 2 < n) mass[2] += sum.z;
+      if (c + 3 < n) mass[3] += sum.w;
+    }
   }
+  if (whole && parts == 1) return;
   const float* o = reinterpret_cast<const float*>(reinterpret_cast<const uint8_t*>(a.ws) + w.o) + row0 * w.parts * a.D;
   const float vmul = a.fp8 ? *a.v_scale : 1.f;
   __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(a.out) + row0 * a.D;
   for (int g = chunk; g < G; g += chunks)
     for (int d = tid; d < a.D; d += 256) {
       float sum = 0.f;
+#pragma unroll 4
       for (int p = 0; p < parts; ++p) sum += o[((size_t)g * w.parts + p) * a.D + d] * ex2(ml[(size_t)g * w.parts + p].x - s_lse[g]);
       out[g * a.D + d] = __float2bfloat16(sum * vmul);
     }
@@ -345,13 +368,14 @@ size_t mb_attn_mass_ws(int num_seqs, int Hq, int D, int max_ctx) { return mbm::d
 
 int mb_attn_mass(const MbMassArgs* a, cudaStream_t stream) {
   if (!a || bad_shape(*a) || !a->v_cache || !a->out || (a->fp8 && !a->v_scale)) return MB_ERR_BAD_ARG;
-  const mbm::DecodeWs w = mbm::decode_ws(a->num_seqs, a->Hq, a->D, a->max_ctx, kPartTokens);
+  const bool tiled = mb_decode_mass_serves(*a);
+  const int part = tiled && a->Hkv >= 8 ? 2 * kPartTokens : kPartTokens;      // as in attention_decode.cu
+  const mbm::DecodeWs w = mbm::decode_ws(a->num_seqs, a->Hq, a->D, a->max_ctx, part);
   if (!a->ws || a->ws_bytes < w.bytes) return MB_ERR_TOO_LARGE;
-  const int rc = a->fp8 ? launch_part<true>(*a, w, stream) : launch_part<false>(*a, w, stream);
+  const int rc = tiled ? mb_decode_mass(*a, w, part, stream) : a->fp8 ? launch_part<true>(*a, w, stream) : launch_part<false>(*a, w, stream);
   if (rc) return rc;
   const int chunks = (a->max_ctx + kChunk - 1) / kChunk;
-  mass_join_kernel<<<dim3(chunks < 1 ? 1 : chunks, a->Hkv, a->num_seqs), 256, 0, stream>>>(*a, w, kPartTokens);
-  return (int)cudaGetLastError();
+  return (int)mb::launch_kernel_ex(mass_join_kernel, dim3(chunks < 1 ? 1 : chunks, a->Hkv, a->num_seqs), dim3(256), 0, stream, 1, tiled, *a, w, part, (int)tiled);
 }
 
 int mb_kv_evict(const MbEvictArgs* a, cudaStream_t stream) {

@@ -83,3 +83,7 @@ inline DecodeWs decode_ws(int seqs, int Hq, int D, int max_ctx, int part_tokens)
 }
 
 }  // namespace mbm
+
+// attention_decode_mass.cu
+bool mb_decode_mass_serves(const MbMassArgs& a);
+int mb_decode_mass(const MbMassArgs& m, const mbm::DecodeWs& w, int part_tokens, cudaStream_t stream);
