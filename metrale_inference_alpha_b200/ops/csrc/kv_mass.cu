@@ -1,8 +1,5 @@
-// Decode attention that leaves the weight of every cached token, and the eviction of cached tokens that gathered least.
-//
-//   mb_attn_mass   z[g, j] = scale <q[s, hG + g], k[j, h]>, p = softmax_j z, out = sum_j p v[j, h], mass[s, h, j] += sum_g p[g, j]
-//   mb_kv_evict    of n rows of a sequence and kv head the last `recent` and, of the others, those of the largest mass stay, in their
-//                  order, `keep` in all; rows, mass and the list of them move together
+// Decode attention that leaves the weight of every cached token:
+// z[g, j] = scale <q[s, hG + g], k[j, h]>, p = softmax_j z, out = sum_j p v[j, h], mass[s, h, j] += sum_g p[g, j].
 //
 // A token's weight needs the normaliser of its whole row, which is known when every partition of the cache is done. Until then the
 // logits wait in the workspace (4 G bytes a token and kv head beside the 2 D or 4 D of its cached rows, and L2 holds them at the sizes of
@@ -13,30 +10,13 @@
 
 namespace {
 
+using mbm::context;
+using mbm::slot_of;
+
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
-}
-
-// cached tokens of a sequence; a length beyond what the call was sized for is reported and cut
-__device__ __forceinline__ int context(const int* ctx_len, int s, int max_ctx, uint32_t* status) {
-  const int n = ctx_len[s];
-  if (n > max_ctx) {
-    if (status && threadIdx.x == 0) atomicCAS(status, 0u, MB_ST_BOUNDS);
-    return max_ctx;
-  }
-  return max(n, 0);
-}
-// flat slot of row j of a sequence; a block that the cache does not have is reported and read as block 0
-__device__ __forceinline__ long long slot_of(const int* table, int j, int block_size, long long num_blocks, uint32_t* status) {
-  const int bi = j / block_size;
-  int b = __ldg(table + bi);
-  if ((unsigned)b >= (unsigned long long)num_blocks) {
-    if (status) atomicCAS(status, 0u, MB_ST_BOUNDS);
-    b = 0;
-  }
-  return (long long)b * block_size + (j - bi * block_size);
 }
 
 // ---------------------------------------------------------------- decode
@@ -228,138 +208,6 @@ bool bad_shape(const MbMassArgs& a) {
          a.block_size <= 0 || a.num_blocks <= 0 || a.max_ctx < 0 || !a.q || !a.k_cache || !a.block_table || !a.ctx_len || !a.mass || (a.fp8 && !a.k_scale);
 }
 
-// ---------------------------------------------------------------- eviction
-// Larger key, larger mass; a NaN is the least, and both zeros are one.
-__device__ __forceinline__ uint32_t key_of(float f) {
-  if (f != f) f = -INFINITY;
-  const uint32_t u = __float_as_uint(f + 0.f);
-  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
-}
-
-// exclusive prefix of `v` over the block (1024 threads), and the block's total
-__device__ __forceinline__ int excl_scan(int v, int* warp_tot, int& total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int inc = v;
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, inc, d);
-    if (lane >= d) inc += y;
-  }
-  __syncthreads();
-  if (lane == 31) warp_tot[warp] = inc;
-  __syncthreads();
-  int before = 0, tot = 0;
-  for (int i = 0; i < 32; ++i) {
-    const int c = warp_tot[i];
-    if (i < warp) before += c;
-    tot += c;
-  }
-  total = tot;
-  return before + inc - v;
-}
-
-// One CTA a (sequence, kv head): the key of the last row that stays by digits of 8 bits from the top, then the list in order.
-__global__ void __launch_bounds__(1024) evict_select_kernel(const MbEvictArgs a) {
-  __shared__ int hist[256], warp_tot[32];
-  __shared__ uint32_t s_prefix;
-  __shared__ int s_need, s_first;
-  const int h = blockIdx.x, s = blockIdx.y, tid = threadIdx.x, lane = tid & 31;
-  const int n = context(a.ctx_len, s, a.max_ctx, a.status), m = min(n, a.keep), old = n - min(n, a.recent);
-  const float* x = a.mass + s * a.mass_seq + h * a.mass_head;
-  float* y = a.mass_out + s * a.out_seq + h * a.out_head;
-  int* kept = a.kept + ((size_t)s * a.Hkv + h) * a.keep;
-  if (tid == 0) {
-    s_first = m;
-    if (h == 0) a.new_len[s] = m;
-  }
-  uint32_t prefix = 0, mask = 0;
-  int need = n > m ? m - a.recent : old;                    // rows wanted of the first `old`
-  if (need > 0 && need < old) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      if (tid < 256) hist[tid] = 0;
-      __syncthreads();
-      for (int i = tid; i - lane < old; i += 1024) {
-        const uint32_t k = i < old ? key_of(x[i]) : 0;
-        const bool in = i < old && (k & mask) == prefix;
-        const unsigned part = __ballot_sync(0xffffffffu, in);
-        if (in) {
-          const int bin = (k >> shift) & 255;
-          const unsigned same = __match_any_sync(part, bin);
-          if (lane == __ffs(same) - 1) atomicAdd(&hist[bin], __popc(same));
-        }
-      }
-      __syncthreads();
-      const int b = 255 - tid, c = tid < 256 ? hist[b] : 0;
-      int total;
-      const int above = excl_scan(c, warp_tot, total);
-      if (tid < 256 && above < need && need <= above + c) {
-        s_prefix = prefix | ((uint32_t)b << shift);
-        s_need = need - above;
-      }
-      __syncthreads();
-      prefix = s_prefix;
-      need = s_need;
-      mask |= 255u << shift;
-      __syncthreads();
-    }
-  } else if (need <= 0) {
-    prefix = 0xffffffffu;                                   // no key is above it, and none of those equal to it is wanted
-    need = 0;
-  }                                                         // else all of them: every key is above 0
-  // ---- rows in order, 1024 at a time: those above the key, the first `need` equal to it, and the recent ones. A kept row moves
-  // forward or stays, so that a round's mass is read before any of it is written over.
-  int eq_before = 0, at = 0;
-  for (int i0 = 0; i0 < n; i0 += 1024) {
-    const int i = i0 + tid;
-    const float f = i < n ? x[i] : 0.f;
-    const uint32_t k = key_of(f);
-    const bool eq = i < old && k == prefix;
-    int total;
-    const int rank = eq_before + excl_scan(eq, warp_tot, total);
-    eq_before += total;
-    const bool in = i < n && (i >= old || k > prefix || (eq && rank < need));
-    const int to = at + excl_scan(in, warp_tot, total);
-    at += total;
-    if (in) {
-      kept[to] = i;
-      y[to] = f;
-    }
-    if (i < n && !in) atomicMin(&s_first, to);
-  }
-  __syncthreads();
-  for (int i = m + tid; i < a.keep; i += 1024) kept[i] = -1;
-  for (int i = m + tid; i < a.max_ctx; i += 1024) y[i] = 0.f;
-  if (tid == 0) a.first[s * a.Hkv + h] = a.in_place ? s_first : 0;
-}
-
-// K (z even) or V of a (sequence, kv head): its kept rows move forward, 32 bytes of their width a CTA, 128 rows a round. A row's place is never
-// behind it, so that writes of one round meet no row that a later one reads; the round itself is read before it is written.
-constexpr int kMoveRows = 128, kMoveBytes = 32;
-
-__global__ void __launch_bounds__(256) evict_move_kernel(const MbEvictArgs a) {
-  const int piece = blockIdx.x >> 1, h = blockIdx.y, s = blockIdx.z, tid = threadIdx.x;
-  const int m = a.new_len[s];
-  const int* kept = a.kept + ((size_t)s * a.Hkv + h) * a.keep;
-  uint8_t* cache = reinterpret_cast<uint8_t*>(blockIdx.x & 1 ? a.v_cache : a.k_cache);
-  const int* from = a.block_table + s * a.table_ld;
-  const int* to = a.dst_table + s * a.dst_ld;
-  const size_t pitch = (size_t)a.Hkv * a.row_bytes, col = (size_t)h * a.row_bytes + piece * kMoveBytes + (tid & 1) * 16;
-  for (int r0 = a.first[s * a.Hkv + h]; r0 < m; r0 += kMoveRows) {
-    const int r = r0 + (tid >> 1);
-    uint4 v;
-    if (r < m) v = *reinterpret_cast<const uint4*>(cache + slot_of(from, kept[r], a.block_size, a.num_blocks, a.status) * pitch + col);
-    __syncthreads();
-    if (r < m) {
-      const int bi = r / a.block_size, b = to[bi];
-      if ((unsigned)b < (unsigned long long)a.num_blocks)
-        *reinterpret_cast<uint4*>(cache + ((long long)b * a.block_size + (r - bi * a.block_size)) * pitch + col) = v;
-      else if (a.status)
-        atomicCAS(a.status, 0u, MB_ST_BOUNDS);
-    }
-    __syncthreads();
-  }
-}
-
 }  // namespace
 
 extern "C" {
@@ -376,18 +224,6 @@ int mb_attn_mass(const MbMassArgs* a, cudaStream_t stream) {
   if (rc) return rc;
   const int chunks = (a->max_ctx + kChunk - 1) / kChunk;
   return (int)mb::launch_kernel_ex(mass_join_kernel, dim3(chunks < 1 ? 1 : chunks, a->Hkv, a->num_seqs), dim3(256), 0, stream, 1, tiled, *a, w, part, (int)tiled);
-}
-
-int mb_kv_evict(const MbEvictArgs* a, cudaStream_t stream) {
-  if (!a || a->num_seqs <= 0 || a->num_seqs > 65535 || a->Hkv <= 0 || a->Hkv > 65535 || a->keep <= 0 || a->recent < 0 || a->recent > a->keep || a->max_ctx < 0 ||
-      a->block_size <= 0 || a->num_blocks <= 0 || a->row_bytes % kMoveBytes || !a->mass || !a->mass_out || !a->ctx_len || !a->kept || !a->new_len || !a->first ||
-      !a->block_table || !a->dst_table || !a->k_cache || !a->v_cache)
-    return MB_ERR_BAD_ARG;
-  evict_select_kernel<<<dim3(a->Hkv, a->num_seqs), 1024, 0, stream>>>(*a);
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return (int)e;
-  evict_move_kernel<<<dim3(2 * (a->row_bytes / kMoveBytes), a->Hkv, a->num_seqs), 256, 0, stream>>>(*a);
-  return (int)cudaGetLastError();
 }
 
 }  // extern "C"

@@ -1,6 +1,7 @@
-// Arguments of the launchers of kv_mass.cu and kv_observe.cu, mirrored field for field by ops/kv_mass.py, and what the kernels of a
+// Arguments of the launchers of kv_mass.cu, kv_observe.cu and kv_evict.cu, mirrored field for field by ops/kv_mass.py, and what the kernels of a
 // decode step with weights share.
 #pragma once
+#include "common.cuh"
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <cstddef>
@@ -46,7 +47,8 @@ struct MbEvictArgs {
   void* v_cache;
   long long num_blocks;
   uint32_t* status;
-  int num_seqs, Hkv, keep, recent, max_ctx, block_size, row_bytes, in_place;
+  int* slots;                // [seqs, Hkv, keep]: kept rows' places in the cache
+  int num_seqs, Hkv, keep, recent, max_ctx, block_size, row_bytes, in_place, block_shift;   // the launcher sets the shift
 };
 
 namespace mbm {
@@ -80,6 +82,26 @@ inline DecodeWs decode_ws(int seqs, int Hq, int D, int max_ctx, int part_tokens)
   w.ml = w.o + rows * w.parts * D * 4;
   w.bytes = w.ml + rows * w.parts * 8;
   return w;
+}
+
+// cached tokens of a sequence; a length beyond what the call was sized for is reported and cut
+__device__ __forceinline__ int context(const int* ctx_len, int s, int max_ctx, uint32_t* status) {
+  const int n = ctx_len[s];
+  if (n > max_ctx) {
+    if (status && threadIdx.x == 0) atomicCAS(status, 0u, MB_ST_BOUNDS);
+    return max_ctx;
+  }
+  return max(n, 0);
+}
+// flat slot of row j of a sequence; a block that the cache does not have is reported and read as block 0
+__device__ __forceinline__ long long slot_of(const int* table, int j, int block_size, long long num_blocks, uint32_t* status) {
+  const int bi = j / block_size;
+  int b = __ldg(table + bi);
+  if ((unsigned)b >= (unsigned long long)num_blocks) {
+    if (status) atomicCAS(status, 0u, MB_ST_BOUNDS);
+    b = 0;
+  }
+  return (long long)b * block_size + (j - bi * block_size);
 }
 
 }  // namespace mbm

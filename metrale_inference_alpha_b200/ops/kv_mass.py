@@ -43,8 +43,8 @@ class _MassArgs(C.Structure):
 class _EvictArgs(C.Structure):
     _fields_ = [("mass", _p), ("mass_seq", _ll), ("mass_head", _ll), ("mass_out", _p), ("out_seq", _ll), ("out_head", _ll), ("ctx_len", _p), ("kept", _p),
                 ("new_len", _p), ("first", _p), ("block_table", _p), ("table_ld", _ll), ("dst_table", _p), ("dst_ld", _ll), ("k_cache", _p), ("v_cache", _p),
-                ("num_blocks", _ll), ("status", _p), ("num_seqs", _i), ("Hkv", _i), ("keep", _i), ("recent", _i), ("max_ctx", _i), ("block_size", _i),
-                ("row_bytes", _i), ("in_place", _i)]
+                ("num_blocks", _ll), ("status", _p), ("slots", _p), ("num_seqs", _i), ("Hkv", _i), ("keep", _i), ("recent", _i), ("max_ctx", _i), ("block_size", _i),
+                ("row_bytes", _i), ("in_place", _i), ("block_shift", _i)]
 
 
 _native.register_optional("mb_attn_mass", [C.POINTER(_MassArgs), _p])
@@ -206,11 +206,11 @@ def kv_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Te
     new_len = torch.empty(S, dtype=torch.int32, device=k_cache.device)
     if S == 0:
         return kept, new_len
-    first = torch.empty(S, Hkv, dtype=torch.int32, device=k_cache.device)
+    own = torch.empty(S * Hkv * (keep + 1), dtype=torch.int32, device=k_cache.device)   # of a sequence and head: the rows' slots, the first that moves
     dst = block_table if dst_table is None else dst_table
-    a = _EvictArgs(_ptr(mass), mass.stride(0), mass.stride(1), _ptr(mo), mo.stride(0), mo.stride(1), _ptr(ctx_len), _ptr(kept), _ptr(new_len), _ptr(first),
-                   _ptr(block_table), block_table.stride(0), _ptr(dst), dst.stride(0), _ptr(k_cache), _ptr(v_cache), nb, _ptr(runtime(k_cache.device).status), S, Hkv,
-                   keep, recent, max_ctx, bs, D * k_cache.element_size(), int(dst_table is None))
+    a = _EvictArgs(_ptr(mass), mass.stride(0), mass.stride(1), _ptr(mo), mo.stride(0), mo.stride(1), _ptr(ctx_len), _ptr(kept), _ptr(new_len), own.data_ptr() + 4 * S * Hkv * keep,
+                   _ptr(block_table), block_table.stride(0), _ptr(dst), dst.stride(0), _ptr(k_cache), _ptr(v_cache), nb, _ptr(runtime(k_cache.device).status), _ptr(own), S, Hkv,
+                   keep, recent, max_ctx, bs, D * k_cache.element_size(), int(dst_table is None), 0)
     _native.check(_native.lib().mb_kv_evict(C.byref(a), _stream()), f"kv_evict[S={S} ctx={max_ctx} keep={keep}]")
     _count(2)
     return kept, new_len

@@ -293,9 +293,10 @@ def test_evict(keep, recent, own_blocks, fp8, dim, block):
 
 
 @pytest.mark.parametrize("own_blocks", [False, True])
-def test_evict_from_a_long_sequence(own_blocks):
-    """Against a selection by sorting: longer than what one CTA has in registers, with long runs of equal mass."""
-    n, H, D, bs, keep, recent = 150_001, 2, 64, 16, 9000, 33
+@pytest.mark.parametrize("n", [32_769, 150_001, 300_007])
+def test_evict_from_a_long_sequence(own_blocks, n):
+    """Against a selection by sorting: longer than what one CTA, and what a cluster has in registers, with long runs of equal mass."""
+    H, D, bs, keep, recent = 2, 64, 16, 9000, 33
     g = torch.Generator(device="cuda").manual_seed(53)
     nb = (n + bs - 1) // bs
     more = (keep + bs - 1) // bs if own_blocks else 0
