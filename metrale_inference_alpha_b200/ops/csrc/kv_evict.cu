@@ -2,8 +2,8 @@
 // largest mass (of equal ones the first), `keep` in all, in their order. Rows, mass and the list of them move together.
 //
 //   select  finds the mass of the last row that stays, digit by digit from the top (11, 11 and 10 bits of an order-preserving image, a histogram in
-//           shared memory each), then writes the list in order by counting ballots. A CTA holds its rows' keys in registers, 32 a thread, and up to
-//           eight CTAs of a cluster add up their histograms: mass is read once.
+//           shared memory each), then writes the list in order by counting ballots. A CTA holds its rows' mass in registers, 16 or 64 a thread, and
+//           up to eight CTAs of a cluster add up their histograms: mass is read once.
 //   move    copies the rows. A kept row's place is never behind it, so in place only a row's own round can be in its way: each round is read before
 //           any of it is written, and later rounds' rows lie behind everything that is written before them.
 #include "common.cuh"
@@ -50,20 +50,33 @@ __device__ __forceinline__ int excl_scan(int v, int* warp_tot, int& total) {
   return __reduce_add_sync(0xffffffffu, lane < warp ? c : 0) + inc - v;
 }
 
-constexpr int kMaxPer = 32, kSegment = 1024 * kMaxPer, kMaxCluster = 8, kBins = 2048;
+constexpr int kThreads = 512, kWarps = kThreads / 32, kPer = 16, kMaxPer = 64, kSegment = kThreads * kMaxPer, kMaxCluster = 8, kBins = 4 * kThreads;
 
-__device__ __forceinline__ int2 dsmem_ld_s2(const int* local, uint32_t rank) {
-  int2 v;
-  asm volatile("ld.shared::cluster.v2.s32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(mb::dsmem_addr(mb::smem_u32(local), rank)) : "memory");
+__device__ __forceinline__ int4 dsmem_ld_s4(const int* local, uint32_t rank) {
+  int4 v;
+  asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(mb::dsmem_addr(mb::smem_u32(local), rank))
+               : "memory");
+  return v;
+}
+// over the first WIDTH lanes
+template <int WIDTH = 32>
+__device__ __forceinline__ int inclusive(int v, int lane) {
+#pragma unroll
+  for (int o = 1; o < WIDTH; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += y;
+  }
   return v;
 }
 
-// A cluster of CTAs (often of one) a (sequence, kv head). CTA r has rows [r * 1024 E, ...) of it, a warp 32 E of them, E at most PER.
+// A cluster of CTAs (often of one) a (sequence, kv head). CTA r has rows [r * 512 E, ...) of it, a warp 32 E of them, E at most PER.
 template <int PER>
-__global__ void __launch_bounds__(1024) evict_select_kernel(const MbEvictArgs a) {
-  __shared__ __align__(8) int hist[3][kBins], s_total[2];
-  __shared__ int2 s_pair[1024];
-  __shared__ int warp_tot[3][32], s_gt[32], s_eq[32];
+__global__ void __launch_bounds__(kThreads) evict_select_kernel(const MbEvictArgs a) {
+  __shared__ __align__(16) int hist[3][kBins], s_total[4];
+  __shared__ __align__(16) int4 s_bins[kThreads];
+  __shared__ int warp_tot[3][kWarps], s_gt[kWarps], s_eq[kWarps];
   const int h = blockIdx.x, s = blockIdx.y, cluster = gridDim.z, rank = blockIdx.z, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   auto sync_all = [&] {
     if (cluster > 1) mb::cluster_sync_all();
@@ -72,13 +85,13 @@ __global__ void __launch_bounds__(1024) evict_select_kernel(const MbEvictArgs a)
   mb::pdl_launch_dependents();                                         // the copies' CTAs come up under this and wait for its end
   const int n = context(a.ctx_len, s, a.max_ctx, a.status), m = min(n, a.keep), old = n - min(n, a.recent);
   const float* x = a.mass + s * a.mass_seq + h * a.mass_head;
-  const int E = (n + 1024 * cluster - 1) / (1024 * cluster);           // rows of a thread
-  const int i0 = (rank * 32 + warp) * 32 * E + lane;                   // its e-th is i0 + 32 e
+  const int E = (n + kThreads * cluster - 1) / (kThreads * cluster);   // rows of a thread
+  const int i0 = (rank * kWarps + warp) * 32 * E + lane;               // its e-th is i0 + 32 e
   float f[PER];
 #pragma unroll
   for (int e = 0; e < PER; ++e) f[e] = e < E && i0 + 32 * e < n ? x[i0 + 32 * e] : 0.f;
 #pragma unroll
-  for (int i = 0; i < 3 * kBins; i += 1024) (&hist[0][0])[i + tid] = 0;
+  for (int i = 0; i < 3; ++i) *reinterpret_cast<int4*>(&hist[i][4 * tid]) = make_int4(0, 0, 0, 0);
   if (tid == 0 && rank == 0) {
     a.first[s * a.Hkv + h] = a.in_place ? m : 0;
     if (h == 0) a.new_len[s] = m;
@@ -89,7 +102,7 @@ __global__ void __launch_bounds__(1024) evict_select_kernel(const MbEvictArgs a)
   if (need > 0 && need < old) {
     uint32_t mask = 0;
     for (int d = 0; d < 3; ++d) {
-      const int shift = d == 0 ? 21 : d == 1 ? 10 : 0, bins = d < 2 ? 2048 : 1024;
+      const int shift = d == 0 ? 21 : d == 1 ? 10 : 0, bins = d < 2 ? kBins : kBins / 2;
 #pragma unroll
       for (int e = 0; e < PER; ++e)
         if (e < E) {
@@ -97,44 +110,41 @@ __global__ void __launch_bounds__(1024) evict_select_kernel(const MbEvictArgs a)
           if (i0 + 32 * e < old && (k & mask) == prefix) atomicAdd(&hist[d][(k >> shift) & (bins - 1)], 1);
         }
       sync_all();
-      // bins from the top, two a thread: b and b - 1, over the cluster
+      // bins from the top, four a thread, over the cluster
       {
-        const int b = bins - 1 - 2 * tid;
-        int2 c = make_int2(0, 0);
-        if (b > 0) {
+        const int b = bins - 4 - 4 * tid;
+        int4 c = make_int4(0, 0, 0, 0);
+        if (b >= 0) {
           if (cluster > 1) {
-            int2 y[kMaxCluster];
+            int4 y[kMaxCluster];
 #pragma unroll
-            for (int r = 0; r < kMaxCluster; ++r) y[r] = r < cluster ? dsmem_ld_s2(&hist[d][b - 1], r) : make_int2(0, 0);
+            for (int r = 0; r < kMaxCluster; ++r) y[r] = r < cluster ? dsmem_ld_s4(&hist[d][b], r) : make_int4(0, 0, 0, 0);
 #pragma unroll
-            for (int r = 0; r < kMaxCluster; ++r) c = make_int2(c.x + y[r].y, c.y + y[r].x);
+            for (int r = 0; r < kMaxCluster; ++r) c = make_int4(c.x + y[r].x, c.y + y[r].y, c.z + y[r].z, c.w + y[r].w);
           } else {
-            c = make_int2(hist[d][b], hist[d][b - 1]);
+            c = *reinterpret_cast<const int4*>(&hist[d][b]);
           }
         }
-        s_pair[tid] = c;
-        const int mine = __reduce_add_sync(0xffffffffu, c.x + c.y);
+        s_bins[tid] = c;
+        const int mine = __reduce_add_sync(0xffffffffu, c.x + c.y + c.z + c.w);
         if (lane == 0) warp_tot[d][warp] = mine;
       }
       __syncthreads();
-      // every warp finds the warp whose bins take the count across `need`, and the bin among them
-      auto inclusive = [&](int v) {
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const int y = __shfl_up_sync(0xffffffffu, v, o);
-          if (lane >= o) v += y;
-        }
-        return v;
-      };
-      const int tot = warp_tot[d][lane], upto = inclusive(tot);
-      const int w = __ffs(__ballot_sync(0xffffffffu, upto >= need)) - 1;
-      const int rest = need - __shfl_sync(0xffffffffu, upto - tot, w);
-      const int2 c = s_pair[w * 32 + lane];
-      const int in = inclusive(c.x + c.y), l = __ffs(__ballot_sync(0xffffffffu, in >= rest)) - 1;
-      const int left = rest - __shfl_sync(0xffffffffu, in - c.x - c.y, l), top = __shfl_sync(0xffffffffu, c.x, l);
-      const int b = bins - 1 - 2 * (w * 32 + l);
-      prefix |= (uint32_t)(left > top ? b - 1 : b) << shift;
-      need = left > top ? left - top : left;
+      // every warp finds the warp whose bins take the count across `need`, the lane of it and the bin
+      const int tot = lane < kWarps ? warp_tot[d][lane] : 0, upto = inclusive<kWarps>(tot, lane);
+      const int w = __ffs(__ballot_sync(0xffffffffu, lane < kWarps && upto >= need)) - 1;
+      need -= __shfl_sync(0xffffffffu, upto - tot, w);
+      const int4 c = s_bins[w * 32 + lane];
+      const int sum = c.x + c.y + c.z + c.w, in = inclusive(sum, lane), l = __ffs(__ballot_sync(0xffffffffu, in >= need)) - 1;
+      need -= __shfl_sync(0xffffffffu, in - sum, l);
+      const int4 q = s_bins[w * 32 + l];
+      int b = bins - 1 - 4 * (w * 32 + l);
+      for (const int c1 : {q.w, q.z, q.y}) {
+        if (need <= c1) break;
+        need -= c1;
+        --b;
+      }
+      prefix |= (uint32_t)b << shift;
       mask |= (uint32_t)(bins - 1) << shift;
     }
   } else if (need <= 0) {                                              // no key is above it, and none of those equal to it is wanted
@@ -142,18 +152,19 @@ __global__ void __launch_bounds__(1024) evict_select_kernel(const MbEvictArgs a)
     need = 0;
   }                                                                    // else all of them: every key is above 0
   // ---- rows that stay: those above the key and the recent ones, and the first `need` equal to it
-  uint32_t above = 0, equal = 0;                                       // bit e: this thread's e-th row
+  auto stays = [&](int e, bool& equal) {
+    const int i = i0 + 32 * e;
+    const uint32_t k = key_of(f[e]);
+    equal = i < old && k == prefix;
+    return i < n && (i >= old || k > prefix);
+  };
   int gt = 0, eq = 0;
 #pragma unroll
   for (int e = 0; e < PER; ++e)
     if (e < E) {
-      const int i = i0 + 32 * e;
-      const uint32_t k = key_of(f[e]);
-      const bool is_above = i < n && (i >= old || k > prefix), is_equal = i < old && k == prefix;
-      above |= (uint32_t)is_above << e;
-      equal |= (uint32_t)is_equal << e;
-      gt += __popc(__ballot_sync(0xffffffffu, is_above));
-      eq += __popc(__ballot_sync(0xffffffffu, is_equal));
+      bool equal;
+      gt += __popc(__ballot_sync(0xffffffffu, stays(e, equal)));
+      eq += __popc(__ballot_sync(0xffffffffu, equal));
     }
   if (lane == 0) {
     s_gt[warp] = gt;
@@ -163,15 +174,18 @@ __global__ void __launch_bounds__(1024) evict_select_kernel(const MbEvictArgs a)
   // rows in front of this warp's: of its own CTA, and of the CTAs in front
   int gt_before = __reduce_add_sync(0xffffffffu, lane < warp ? s_gt[lane] : 0), eq_before = __reduce_add_sync(0xffffffffu, lane < warp ? s_eq[lane] : 0);
   if (cluster > 1) {
-    if (warp == 31 && lane == 0) {
+    if (warp == kWarps - 1 && lane == 0) {
       s_total[0] = gt_before + gt;
       s_total[1] = eq_before + eq;
     }
     mb::cluster_sync_all();
-    for (int r = 0; r < rank; ++r) {
-      const int2 y = dsmem_ld_s2(s_total, r);
-      gt_before += y.x;
-      eq_before += y.y;
+    int4 y[kMaxCluster];
+#pragma unroll
+    for (int r = 0; r < kMaxCluster; ++r) y[r] = r < rank ? dsmem_ld_s4(s_total, r) : make_int4(0, 0, 0, 0);
+#pragma unroll
+    for (int r = 0; r < kMaxCluster; ++r) {
+      gt_before += y[r].x;
+      eq_before += y[r].y;
     }
     mb::cluster_sync_all();                                            // a CTA's shared memory outlives what others read of it
   }
@@ -186,7 +200,8 @@ __global__ void __launch_bounds__(1024) evict_select_kernel(const MbEvictArgs a)
   for (int e = 0; e < PER; ++e)
     if (e < E) {
       const int i = i0 + 32 * e;
-      const bool is_above = above >> e & 1, is_equal = equal >> e & 1;
+      bool is_equal;
+      const bool is_above = stays(e, is_equal);
       const uint32_t bg = __ballot_sync(0xffffffffu, is_above), be = __ballot_sync(0xffffffffu, is_equal);
       const int rank_eq = eq_before + __popc(be & before);
       const int to = gt_before + __popc(bg & before) + min(rank_eq, need);
@@ -200,8 +215,8 @@ __global__ void __launch_bounds__(1024) evict_select_kernel(const MbEvictArgs a)
       gt_before += __popc(bg);
       eq_before += __popc(be);
     }
-  for (int i = m + rank * 1024 + tid; i < a.keep; i += 1024 * cluster) kept[i] = -1;
-  for (int i = m + rank * 1024 + tid; i < a.max_ctx; i += 1024 * cluster) y[i] = 0.f;
+  for (int i = m + rank * kThreads + tid; i < a.keep; i += kThreads * cluster) kept[i] = -1;
+  for (int i = m + rank * kThreads + tid; i < a.max_ctx; i += kThreads * cluster) y[i] = 0.f;
   if (a.in_place) {
     first = __reduce_min_sync(0xffffffffu, first);
     if (lane == 0 && first < m) atomicMin(&a.first[s * a.Hkv + h], first);
@@ -278,36 +293,63 @@ __global__ void __launch_bounds__(1024) evict_select_long_kernel(const MbEvictAr
   if (tid == 0) a.first[s * a.Hkv + h] = a.in_place ? s_first : 0;
 }
 
-// K (x even) or V of a (sequence, kv head), 2^lane_bits pieces of 16 bytes of its rows' width a CTA, THREADS >> lane_bits times DEEP rows a round. In
-// place a CTA takes all rounds in order; into blocks of their own rows do not get into each other's way, and every CTA takes one.
-template <int THREADS, int DEEP, bool IN_PLACE>
-__global__ void __launch_bounds__(THREADS) evict_move_kernel(const MbEvictArgs a, int lane_bits) {
+// K (x even) or V of a (sequence, kv head) into blocks of its own: 256 >> bits rows at a time of 2^bits pieces of 16 bytes, eight rows a thread.
+constexpr int kDeep = 8;
+
+__global__ void __launch_bounds__(256) evict_copy_kernel(const MbEvictArgs a, int bits) {
   mb::pdl_wait();
-  const int lanes = 1 << lane_bits, strips = a.row_bytes / (16 * lanes), strip = (blockIdx.x >> 1) % strips, h = blockIdx.y, s = blockIdx.z, tid = threadIdx.x;
-  const int m = a.new_len[s], step = THREADS >> lane_bits, round = step * DEEP;
+  const int h = blockIdx.y, s = blockIdx.z, m = a.new_len[s], step = 256 >> bits, r0 = (blockIdx.x >> 1) * step * kDeep + (threadIdx.x >> bits);
   const int* slots = a.slots + ((size_t)s * a.Hkv + h) * a.keep;
   uint8_t* cache = reinterpret_cast<uint8_t*>(blockIdx.x & 1 ? a.v_cache : a.k_cache);
   const int* to = a.dst_table + s * a.dst_ld;
-  const size_t pitch = (size_t)a.Hkv * a.row_bytes, col = (size_t)h * a.row_bytes + (size_t)(strip * lanes + (tid & (lanes - 1))) * 16;
-  int r0 = (IN_PLACE ? a.first[s * a.Hkv + h] : ((int)blockIdx.x >> 1) / strips * round) + (tid >> lane_bits);
-  const int last = IN_PLACE ? m : min(m, r0 - (tid >> lane_bits) + round);
-  // whole CTAs go round together
-  for (; r0 - (tid >> lane_bits) < last; r0 += round) {
-    uint4 v[DEEP];
-    int dst[DEEP];
+  const size_t pitch = (size_t)a.Hkv * a.row_bytes, col = (size_t)h * a.row_bytes + (threadIdx.x & ((1 << bits) - 1)) * 16;
+  uint4 v[kDeep];
+  int dst[kDeep];
 #pragma unroll
-    for (int k = 0; k < DEEP; ++k) {
-      const int r = r0 + k * step;
-      dst[k] = -1;
-      if (r < m) {
-        v[k] = *reinterpret_cast<const uint4*>(cache + slots[r] * pitch + col);
-        dst[k] = slot_in<true>(a, to, r);
-      }
+  for (int k = 0; k < kDeep; ++k) {
+    const int r = r0 + k * step;
+    dst[k] = -1;
+    if (r < m) {
+      v[k] = *reinterpret_cast<const uint4*>(cache + slots[r] * pitch + col);
+      dst[k] = slot_in<true>(a, to, r);
     }
-    if (IN_PLACE) __syncthreads();
+  }
 #pragma unroll
-    for (int k = 0; k < DEEP; ++k)
-      if (dst[k] >= 0) *reinterpret_cast<uint4*>(cache + dst[k] * pitch + col) = v[k];
+  for (int k = 0; k < kDeep; ++k)
+    if (dst[k] >= 0) *reinterpret_cast<uint4*>(cache + dst[k] * pitch + col) = v[k];
+}
+
+// The same inside the sequence's own blocks. A row's place is never behind it, so that only a round's own rows can be in its way: a cluster brings
+// 64 KB a CTA into shared memory, waits for that everywhere, and writes. Later rounds' rows lie behind all that is written before them.
+constexpr int kRoundB = 64 * 1024;
+
+__global__ void __launch_bounds__(256) evict_move_kernel(const MbEvictArgs a, int bits) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  mb::pdl_wait();
+  const int cluster = gridDim.x >> 1, rank = blockIdx.x % cluster, h = blockIdx.y, s = blockIdx.z, tid = threadIdx.x, m = a.new_len[s];
+  const int* slots = a.slots + ((size_t)s * a.Hkv + h) * a.keep;
+  uint8_t* cache = reinterpret_cast<uint8_t*>(blockIdx.x / cluster ? a.v_cache : a.k_cache);
+  const int* table = a.block_table + s * a.table_ld;
+  const size_t pitch = (size_t)a.Hkv * a.row_bytes, col = (size_t)h * a.row_bytes + (tid & ((1 << bits) - 1)) * 16;
+  const int step = 256 >> bits, mine = kRoundB / 16 >> bits;           // rows at a time, rows of a round
+  constexpr int kLoads = kRoundB / (256 * 16);
+  for (int r0 = a.first[s * a.Hkv + h]; r0 < m; r0 += mine * cluster) {
+    const int b = r0 + rank * mine + (tid >> bits), e = min(m, r0 + (rank + 1) * mine);
+    int at[kLoads];
+#pragma unroll
+    for (int k = 0; k < kLoads; ++k) at[k] = b + k * step < e ? slots[b + k * step] : -1;
+#pragma unroll
+    for (int k = 0; k < kLoads; ++k)
+      if (at[k] >= 0)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(mb::smem_u32(smem + (k * 256 + tid) * 16)), "l"(cache + at[k] * pitch + col) : "memory");
+#pragma unroll
+    for (int k = 0; k < kLoads; ++k) at[k] = b + k * step < e ? slot_in<true>(a, table, b + k * step) : -1;
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    if (cluster > 1) mb::cluster_sync_all();
+    else __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kLoads; ++k)                                   // what a thread brought it takes away
+      if (at[k] >= 0) *reinterpret_cast<uint4*>(cache + at[k] * pitch + col) = *reinterpret_cast<const uint4*>(smem + (k * 256 + tid) * 16);
   }
 }
 
@@ -326,26 +368,44 @@ extern "C" int mb_kv_evict(const MbEvictArgs* given, cudaStream_t stream) {
   const long long heads = (long long)a->Hkv * a->num_seqs;
   cudaError_t e;
   if (a->max_ctx <= kSegment * kMaxCluster) {
-    // eight rows a thread, in as many CTAs as the chip holds at once; where there are more, up to 32
+    // 16 rows a thread, in as many CTAs as the chip holds at once; where there are more, up to 64
     int cluster = 1;
-    while (cluster * kSegment < a->max_ctx || (cluster < kMaxCluster && cluster * 8192 < a->max_ctx && heads * cluster * 2 <= 2 * 148)) cluster *= 2;
-    auto kern = cluster * 8192 >= a->max_ctx ? evict_select_kernel<8> : evict_select_kernel<kMaxPer>;
-    e = mb::launch_kernel_ex(kern, dim3(a->Hkv, a->num_seqs, cluster), dim3(1024), 0, stream, cluster, false, *a);
+    while (cluster * kSegment < a->max_ctx || (cluster < kMaxCluster && cluster * kThreads * kPer < a->max_ctx && heads * cluster * 2 <= 2 * 148)) cluster *= 2;
+    auto kern = cluster * kThreads * kPer >= a->max_ctx ? evict_select_kernel<kPer> : evict_select_kernel<kMaxPer>;
+    e = mb::launch_kernel_ex(kern, dim3(a->Hkv, a->num_seqs, cluster), dim3(kThreads), 0, stream, cluster, false, *a);
   } else {
     e = mb::launch_kernel_ex(evict_select_long_kernel, dim3(a->Hkv, a->num_seqs), dim3(1024), 0, stream, 1, false, *a);
   }
   if (e != cudaSuccess) return (int)e;
-  const int held = a->keep < a->max_ctx ? a->keep : a->max_ctx, pieces = a->row_bytes / 16;
+  const int held = a->keep < a->max_ctx ? a->keep : a->max_ctx;
   if (held == 0) return 0;
-  if (a->in_place) {
-    // the rows of a strip follow each other, so narrow strips, down to a sector, while they give the chip more CTAs to run at once
-    int lanes = pieces, bits = 0;
-    while (lanes > 2 && 2 * heads * (pieces / lanes) < 148) lanes /= 2;
-    while (1 << bits < lanes) ++bits;
-    return (int)mb::launch_kernel_ex(evict_move_kernel<512, 8, true>, dim3(2 * (pieces / lanes), a->Hkv, a->num_seqs), dim3(512), 0, stream, 1, true, *a, bits);
-  }
   int bits = 0;
-  while (1 << bits < pieces) ++bits;
-  const int round = (256 >> bits) * 8, rounds = (held + round - 1) / round;
-  return (int)mb::launch_kernel_ex(evict_move_kernel<256, 8, false>, dim3(2 * rounds, a->Hkv, a->num_seqs), dim3(256), 0, stream, 1, true, *a, bits);
+  while (16 << bits < a->row_bytes) ++bits;
+  if (!a->in_place) {
+    const int round = (256 >> bits) * kDeep;
+    return (int)mb::launch_kernel_ex(evict_copy_kernel, dim3(2 * ((held + round - 1) / round), a->Hkv, a->num_seqs), dim3(256), 0, stream, 1, true, *a, bits);
+  }
+  static bool configured = false;
+  if (!configured) {
+    e = cudaFuncSetAttribute(evict_move_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRoundB);
+    if (e != cudaSuccess) return (int)e;
+    configured = true;
+  }
+  const int mine = kRoundB / a->row_bytes;
+  int cluster = 1;
+  while (cluster < kMaxCluster && 2 * heads * cluster < 2 * 148 && cluster * mine < held) cluster *= 2;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(2 * cluster, a->Hkv, a->num_seqs);
+  cfg.blockDim = dim3(256);
+  cfg.dynamicSmemBytes = kRoundB;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  return (int)cudaLaunchKernelEx(&cfg, evict_move_kernel, (const MbEvictArgs)*a, bits);
 }

@@ -52,53 +52,87 @@ _native.register_optional("mb_prompt_mass", [C.POINTER(_MassArgs), _p])
 _native.register_optional("mb_kv_evict", [C.POINTER(_EvictArgs), _p])
 
 
-def _sizes(name: str):
-    fn = getattr(_native.lib(), name)
-    fn.restype = C.c_size_t
-    return fn
+_ws_bytes: dict = {}
 
 
-def _refuse(cond: bool, what: str) -> None:
-    if cond:
-        raise ValueError(what)
+def _workspace(name: str, *sizes) -> int:
+    fn = _ws_bytes.get(name)
+    if fn is None:
+        fn = getattr(_native.lib(), name)
+        fn.restype, fn.argtypes = C.c_size_t, [_i] * len(sizes)
+        _ws_bytes[name] = fn
+    return fn(*sizes)
 
 
+def _bad(where: str, what: str):
+    raise ValueError(f"{where}: {what}")
+
+
+# Checks stand in front of every call of a step that takes some ten microseconds, so their messages are put together only where they are needed.
 def _check_cache(where, k_cache, v_cache, block_table, ctx_len, mass, max_ctx) -> Tuple[int, int, int, int, int]:
-    """Shapes, types and places that all three share; (S, blocks, block, Hkv, D)."""
-    _refuse(k_cache.dim() != 4 or k_cache.dtype not in (torch.bfloat16, torch.uint8), f"{where}: k_cache is [blocks, block, kv heads, dim], bf16 or e4m3 bytes")
-    nb, bs, Hkv, D = k_cache.shape
-    _refuse(v_cache is not None and (v_cache.shape != k_cache.shape or v_cache.dtype != k_cache.dtype), f"{where}: v_cache has the shape and type of k_cache")
-    _refuse(not k_cache.is_contiguous() or (v_cache is not None and not v_cache.is_contiguous()), f"{where}: caches are contiguous")
-    _refuse(D not in HEAD_DIMS, f"{where}: head dim {D}, one of {HEAD_DIMS} is served")
-    S = ctx_len.numel()
-    _refuse(ctx_len.dtype != torch.int32 or ctx_len.dim() != 1 or not ctx_len.is_contiguous(), f"{where}: ctx_len is int32 [sequences]")
-    _refuse(block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != S or (block_table.shape[1] > 1 and block_table.stride(1) != 1),
-            f"{where}: block_table is int32 [sequences, blocks of a sequence]")
-    _refuse(mass.dtype != torch.float32 or mass.dim() != 3 or mass.shape[:2] != (S, Hkv) or (mass.shape[2] > 1 and mass.stride(2) != 1),
-            f"{where}: mass is fp32 [sequences, kv heads, columns], columns next to each other")
-    _refuse(max_ctx < 0 or mass.shape[2] < max_ctx or block_table.shape[1] * bs < max_ctx,
-            f"{where}: max_ctx {max_ctx} is beyond the columns of mass ({mass.shape[2]}) or the rows of block_table ({block_table.shape[1] * bs})")
-    _refuse(max_ctx > 1 << 30, f"{where}: max_ctx is at most 2^30")
+    """Shapes and types that all three share; (S, blocks, block, Hkv, D)."""
+    shape, dtype = k_cache.shape, k_cache.dtype
+    if len(shape) != 4 or (dtype != torch.bfloat16 and dtype != torch.uint8):
+        _bad(where, "k_cache is [blocks, block, kv heads, dim], bf16 or e4m3 bytes")
+    nb, bs, Hkv, D = shape
+    if v_cache is not None and (v_cache.shape != shape or v_cache.dtype != dtype):
+        _bad(where, "v_cache has the shape and type of k_cache")
+    if not k_cache.is_contiguous() or (v_cache is not None and not v_cache.is_contiguous()):
+        _bad(where, "caches are contiguous")
+    if D not in HEAD_DIMS:
+        _bad(where, f"head dim {D}, one of {HEAD_DIMS} is served")
+    if ctx_len.dtype != torch.int32 or ctx_len.dim() != 1 or not ctx_len.is_contiguous():
+        _bad(where, "ctx_len is int32 [sequences]")
+    S, table, m = ctx_len.shape[0], block_table.shape, mass.shape
+    if block_table.dtype != torch.int32 or len(table) != 2 or table[0] != S or (table[1] > 1 and block_table.stride(1) != 1):
+        _bad(where, "block_table is int32 [sequences, blocks of a sequence]")
+    if mass.dtype != torch.float32 or len(m) != 3 or m[0] != S or m[1] != Hkv or (m[2] > 1 and mass.stride(2) != 1):
+        _bad(where, "mass is fp32 [sequences, kv heads, columns], columns next to each other")
+    if max_ctx < 0 or m[2] < max_ctx or table[1] * bs < max_ctx:
+        _bad(where, f"max_ctx {max_ctx} is beyond the columns of mass ({m[2]}) or the rows of block_table ({table[1] * bs})")
+    if max_ctx > 1 << 30:
+        _bad(where, "max_ctx is at most 2^30")
     return S, nb, bs, Hkv, D
 
 
-def _check_places(where, tensors) -> None:
+def _check_queries(where, q, rows, Hkv, D) -> int:
+    shape = q.shape
+    if q.dtype != torch.bfloat16 or len(shape) != 3 or shape[2] != D or (rows >= 0 and shape[0] != rows) or not q.is_contiguous():
+        _bad(where, f"q is contiguous bf16 [{'rows' if rows < 0 else rows}, heads, {D}]")
+    Hq = shape[1]
+    if Hq == 0 or Hq % Hkv != 0 or Hq // Hkv > MAX_GROUP:
+        _bad(where, f"{Hq} query heads over {Hkv} kv heads: whole groups of up to {MAX_GROUP}")
+    return Hq
+
+
+def _check_places(where, *tensors) -> None:
     """CUDA: one device, the current one, whose stream the launches go to; CPU: all there."""
-    dev = tensors[0].device
-    _refuse(any(t is not None and t.device != dev for t in tensors), f"{where}: tensors lie on different devices")
-    _refuse(dev.type == "cuda" and dev.index != torch.cuda.current_device(), f"{where}: tensors lie on {dev}, the current device is another one")
+    dev = tensors[0].get_device()
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            _bad(where, "tensors lie on different devices")
+    if dev >= 0 and dev != torch._C._cuda_getDevice():
+        _bad(where, f"tensors lie on device {dev}, the current device is another one")
 
 
-def _check_scales(where, cache, scale, scales) -> None:
-    _refuse(not scale > 0, f"{where}: scale is positive")
-    _refuse(cache.dtype == torch.uint8 and any(s is None or s.dtype != torch.float32 or s.numel() < 1 for s in scales), f"{where}: an e4m3 cache comes with fp32 scales")
+def _check_scales(where, cache, scale, *scales) -> None:
+    if not scale > 0:
+        _bad(where, "scale is positive")
+    if cache.dtype == torch.uint8:
+        for s in scales:
+            if s is None or s.dtype != torch.float32 or s.numel() < 1:
+                _bad(where, "an e4m3 cache comes with fp32 scales")
 
 
-def _rows_apart(mass: torch.Tensor) -> bool:
+def _check_rows(where, name, mass) -> None:
     """No two rows of [S, H, columns] share memory."""
     S, H, n = mass.shape
-    a, b = sorted(((mass.stride(1), H), (mass.stride(0), S)))
-    return (a[1] < 2 or a[0] >= n) and (b[1] < 2 or b[0] >= (a[0] * (a[1] - 1) + n))
+    a, b = mass.stride(1), mass.stride(0)
+    if a >= n and b >= a * H:
+        return
+    (a, x), (b, y) = sorted(((a, H), (b, S)))
+    if not ((x < 2 or a >= n) and (y < 2 or b >= a * (x - 1) + n)):
+        _bad(where, f"rows of {name} share memory")
 
 
 # most bytes of logits that a decode step has under way; more sequences go in several steps
@@ -115,29 +149,32 @@ def paged_attention_mass(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     status word (`check_status`)."""
     where = "paged_attention_mass"
     S, nb, bs, Hkv, D = _check_cache(where, k_cache, v_cache, block_table, ctx_len, mass, max_ctx)
-    _refuse(q.dtype != torch.bfloat16 or q.dim() != 3 or q.shape[0] != S or q.shape[2] != D or not q.is_contiguous(), f"{where}: q is contiguous bf16 [sequences, heads, {D}]")
-    Hq = q.shape[1]
-    _refuse(Hq == 0 or Hq % Hkv != 0 or Hq // Hkv > MAX_GROUP, f"{where}: {Hq} query heads over {Hkv} kv heads: whole groups of up to {MAX_GROUP}")
-    _refuse(not _rows_apart(mass), f"{where}: rows of mass share memory")
-    _check_scales(where, k_cache, scale, (k_scale, v_scale))
-    _check_places(where, (q, k_cache, v_cache, block_table, ctx_len, mass, k_scale, v_scale))
+    Hq = _check_queries(where, q, S, Hkv, D)
+    _check_rows(where, "mass", mass)
+    _check_scales(where, k_cache, scale, k_scale, v_scale)
+    _check_places(where, q, k_cache, v_cache, block_table, ctx_len, mass, k_scale, v_scale)
     if not q.is_cuda:
         return ref.paged_attention_mass(q, k_cache, v_cache, block_table, ctx_len, mass, scale, k_scale, v_scale)
-    from . import _count, _ptr, _stream, runtime
+    from . import _count, _stream, runtime
     out = torch.empty_like(q)
     if S == 0:
         return out
-    L, rt, sizes = _native.lib(), runtime(q.device), _sizes("mb_attn_mass_ws")
-    one = sizes(1, Hq, D, max_ctx)
-    step = min(S, max(1, _WS_BYTES // max(1, one)), 1024)
-    ws = torch.empty(sizes(step, Hq, D, max_ctx), dtype=torch.uint8, device=q.device)
+    launch, rt = _native.lib().mb_attn_mass, runtime(q.device)
+    step, need = min(S, 1024), _workspace("mb_attn_mass_ws", min(S, 1024), Hq, D, max_ctx)
+    if need > _WS_BYTES:
+        step = max(1, _WS_BYTES // _workspace("mb_attn_mass_ws", 1, Hq, D, max_ctx))
+        step = min(step, S)
+        need = _workspace("mb_attn_mass_ws", step, Hq, D, max_ctx)
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+    a = _MassArgs(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), block_table.stride(0), None, None, ctx_len.data_ptr(), mass.data_ptr(),
+                  mass.stride(0), mass.stride(1), out.data_ptr(), ws.data_ptr(), need, None if k_scale is None else k_scale.data_ptr(),
+                  None if v_scale is None else v_scale.data_ptr(), rt.status.data_ptr(), nb, 0, step, Hq, Hkv, D, bs, int(k_cache.dtype == torch.uint8), max_ctx, 1, 1,
+                  rt.sm_count, scale)
     for s in range(0, S, step):
-        n = min(step, S - s)
-        a = _MassArgs(q.data_ptr() + s * Hq * D * 2, _ptr(k_cache), _ptr(v_cache), block_table.data_ptr() + s * block_table.stride(0) * 4, block_table.stride(0), None,
-                      None, ctx_len.data_ptr() + s * 4, mass.data_ptr() + s * mass.stride(0) * 4, mass.stride(0), mass.stride(1), out.data_ptr() + s * Hq * D * 2,
-                      _ptr(ws), ws.numel(), _ptr(k_scale), _ptr(v_scale), _ptr(rt.status), nb, 0, n, Hq, Hkv, D, bs, int(k_cache.dtype == torch.uint8), max_ctx, 1, 1,
-                      rt.sm_count, scale)
-        _native.check(L.mb_attn_mass(C.byref(a), _stream()), f"attn_mass[S={n} ctx={max_ctx} D={D}]")
+        if s:
+            a.q, a.out, a.ctx_len = q.data_ptr() + s * Hq * D * 2, out.data_ptr() + s * Hq * D * 2, ctx_len.data_ptr() + s * 4
+            a.block_table, a.mass, a.num_seqs = block_table.data_ptr() + s * block_table.stride(0) * 4, mass.data_ptr() + s * mass.stride(0) * 4, min(step, S - s)
+        _native.check(launch(C.byref(a), _stream()), "attn_mass")
         _count(2)
     return out
 
@@ -151,27 +188,28 @@ def prompt_mass(q: torch.Tensor, k_cache: torch.Tensor, block_table: torch.Tenso
     does not have set the status word."""
     where = "prompt_mass"
     S, nb, bs, Hkv, D = _check_cache(where, k_cache, None, block_table, ctx_len, mass, max_ctx)
-    _refuse(q.dtype != torch.bfloat16 or q.dim() != 3 or q.shape[2] != D or not q.is_contiguous(), f"{where}: q is contiguous bf16 [rows, heads, {D}]")
-    Hq = q.shape[1]
-    _refuse(Hq == 0 or Hq % Hkv != 0 or Hq // Hkv > MAX_GROUP, f"{where}: {Hq} query heads over {Hkv} kv heads: whole groups of up to {MAX_GROUP}")
-    _refuse(any(x.dtype != torch.int32 or x.shape != ctx_len.shape or not x.is_contiguous() for x in (q_start, q_len)), f"{where}: q_start and q_len are int32 [sequences]")
-    _refuse(last < 0 or max_q_len < 0, f"{where}: last and max_q_len are not negative")
-    _refuse(not _rows_apart(mass), f"{where}: rows of mass share memory")
-    _check_scales(where, k_cache, scale, (k_scale,))
-    _check_places(where, (q, k_cache, block_table, q_start, q_len, ctx_len, mass, k_scale))
+    Hq = _check_queries(where, q, -1, Hkv, D)
+    for x in (q_start, q_len):
+        if x.dtype != torch.int32 or x.shape != ctx_len.shape or not x.is_contiguous():
+            _bad(where, "q_start and q_len are int32 [sequences]")
+    if last < 0 or max_q_len < 0:
+        _bad(where, "last and max_q_len are not negative")
+    _check_rows(where, "mass", mass)
+    _check_scales(where, k_cache, scale, k_scale)
+    _check_places(where, q, k_cache, block_table, q_start, q_len, ctx_len, mass, k_scale)
     if not q.is_cuda:
         return ref.prompt_mass(q, k_cache, block_table, q_start, q_len, ctx_len, mass, scale, last, k_scale)
     if S == 0 or q.shape[0] == 0 or max_q_len == 0 or max_ctx == 0:
         return mass
-    from . import _count, _ptr, _stream, runtime
-    seen = min(last or max_q_len, max_q_len)
-    ws = torch.empty(_sizes("mb_prompt_mass_ws")(S, Hq, Hkv, D, seen, max_ctx, int(k_cache.dtype == torch.uint8)), dtype=torch.uint8, device=q.device)
-    rt = runtime(q.device)
-    a = _MassArgs(_ptr(q), _ptr(k_cache), None, _ptr(block_table), block_table.stride(0), _ptr(q_start), _ptr(q_len), _ptr(ctx_len), _ptr(mass), mass.stride(0),
-                  mass.stride(1), None, _ptr(ws), ws.numel(), _ptr(k_scale), None, _ptr(rt.status), nb, q.shape[0], S, Hq, Hkv, D, bs,
-                  int(k_cache.dtype == torch.uint8), max_ctx, max_q_len, seen, rt.sm_count, scale)
-    _native.check(_native.lib().mb_prompt_mass(C.byref(a), _stream()), f"prompt_mass[S={S} last={seen} ctx={max_ctx} D={D}]")
-    _count(2)
+    from . import _count, _stream, runtime
+    seen, fp8 = min(last or max_q_len, max_q_len), int(k_cache.dtype == torch.uint8)
+    need = _workspace("mb_prompt_mass_ws", S, Hq, Hkv, D, seen, max_ctx, fp8)
+    ws, rt = torch.empty(need, dtype=torch.uint8, device=q.device), runtime(q.device)
+    a = _MassArgs(q.data_ptr(), k_cache.data_ptr(), None, block_table.data_ptr(), block_table.stride(0), q_start.data_ptr(), q_len.data_ptr(), ctx_len.data_ptr(),
+                  mass.data_ptr(), mass.stride(0), mass.stride(1), None, ws.data_ptr(), need, None if k_scale is None else k_scale.data_ptr(), None, rt.status.data_ptr(),
+                  nb, q.shape[0], S, Hq, Hkv, D, bs, fp8, max_ctx, max_q_len, seen, rt.sm_count, scale)
+    _native.check(_native.lib().mb_prompt_mass(C.byref(a), _stream()), "prompt_mass")
+    _count(3 if seen * (Hq // Hkv) > 4096 else 2)               # columns whose rows are cut into parts are joined
     return mass
 
 
@@ -187,30 +225,36 @@ def kv_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Te
     ``max_ctx``; without it ``mass`` does. A length beyond ``max_ctx`` or a block that the cache does not have sets the status word."""
     where = "kv_evict"
     S, nb, bs, Hkv, D = _check_cache(where, k_cache, v_cache, block_table, ctx_len, mass, max_ctx)
-    _refuse(keep < 1 or recent < 0 or recent > keep, f"{where}: keep {keep} is at least 1 and recent {recent} at most keep")
-    mo = mass if mass_out is None else mass_out
-    _refuse(mo.dtype != torch.float32 or mo.dim() != 3 or mo.shape[:2] != (S, Hkv) or mo.shape[2] < max_ctx or (mo.shape[2] > 1 and mo.stride(2) != 1) or not _rows_apart(mo),
-            f"{where}: mass_out is fp32 [sequences, kv heads, at least max_ctx columns] of its own")
-    same = mo.data_ptr() == mass.data_ptr() and mo.stride() == mass.stride()
-    span = [(t.data_ptr(), t.data_ptr() + 4 * (1 + sum((n - 1) * st for n, st in zip(t.shape, t.stride())))) for t in (mass, mo)] if mass.numel() and mo.numel() else None
-    _refuse(not same and span is not None and span[0][0] < span[1][1] and span[1][0] < span[0][1], f"{where}: mass_out overlaps mass")
-    held = min(keep, max_ctx)
+    if keep < 1 or recent < 0 or recent > keep:
+        _bad(where, f"keep {keep} is at least 1 and recent {recent} at most keep")
+    mo = mass
+    if mass_out is not None:
+        mo, m = mass_out, mass_out.shape
+        if mo.dtype != torch.float32 or len(m) != 3 or m[0] != S or m[1] != Hkv or m[2] < max_ctx or (m[2] > 1 and mo.stride(2) != 1):
+            _bad(where, "mass_out is fp32 [sequences, kv heads, at least max_ctx columns]")
+        if mass.numel() and mo.numel() and not (mo.data_ptr() == mass.data_ptr() and mo.stride() == mass.stride()):
+            (a, b), (c, d) = ((t.data_ptr(), t.data_ptr() + 4 * (1 + sum((n - 1) * st for n, st in zip(t.shape, t.stride())))) for t in (mass, mo))
+            if a < d and c < b:
+                _bad(where, "mass_out overlaps mass")
+    _check_rows(where, "mass_out", mo)
     if dst_table is not None:
-        _refuse(dst_table.dtype != torch.int32 or dst_table.dim() != 2 or dst_table.shape[0] != S or dst_table.shape[1] * bs < held or
-                (dst_table.shape[1] > 1 and dst_table.stride(1) != 1), f"{where}: dst_table is int32 [sequences, blocks for {held} rows]")
-    _check_places(where, (k_cache, v_cache, block_table, ctx_len, mass, mo, dst_table))
+        m = dst_table.shape
+        if dst_table.dtype != torch.int32 or len(m) != 2 or m[0] != S or m[1] * bs < min(keep, max_ctx) or (m[1] > 1 and dst_table.stride(1) != 1):
+            _bad(where, f"dst_table is int32 [sequences, blocks for {min(keep, max_ctx)} rows]")
+    _check_places(where, k_cache, v_cache, block_table, ctx_len, mass, mo, dst_table)
     if not k_cache.is_cuda:
         return ref.kv_evict(k_cache, v_cache, block_table, ctx_len, mass, keep, recent, max_ctx, mo, dst_table)
-    from . import _count, _ptr, _stream, runtime
-    kept = torch.empty(S, Hkv, keep, dtype=torch.int32, device=k_cache.device)
-    new_len = torch.empty(S, dtype=torch.int32, device=k_cache.device)
+    from . import _count, _stream, runtime
+    dev = k_cache.device
+    kept, new_len = torch.empty(S, Hkv, keep, dtype=torch.int32, device=dev), torch.empty(S, dtype=torch.int32, device=dev)
     if S == 0:
         return kept, new_len
-    own = torch.empty(S * Hkv * (keep + 1), dtype=torch.int32, device=k_cache.device)   # of a sequence and head: the rows' slots, the first that moves
+    own = torch.empty(S * Hkv * (keep + 1), dtype=torch.int32, device=dev)     # of a sequence and head: the rows' slots, the first that moves
     dst = block_table if dst_table is None else dst_table
-    a = _EvictArgs(_ptr(mass), mass.stride(0), mass.stride(1), _ptr(mo), mo.stride(0), mo.stride(1), _ptr(ctx_len), _ptr(kept), _ptr(new_len), own.data_ptr() + 4 * S * Hkv * keep,
-                   _ptr(block_table), block_table.stride(0), _ptr(dst), dst.stride(0), _ptr(k_cache), _ptr(v_cache), nb, _ptr(runtime(k_cache.device).status), _ptr(own), S, Hkv,
-                   keep, recent, max_ctx, bs, D * k_cache.element_size(), int(dst_table is None), 0)
-    _native.check(_native.lib().mb_kv_evict(C.byref(a), _stream()), f"kv_evict[S={S} ctx={max_ctx} keep={keep}]")
+    a = _EvictArgs(mass.data_ptr(), mass.stride(0), mass.stride(1), mo.data_ptr(), mo.stride(0), mo.stride(1), ctx_len.data_ptr(), kept.data_ptr(), new_len.data_ptr(),
+                   own.data_ptr() + 4 * S * Hkv * keep, block_table.data_ptr(), block_table.stride(0), dst.data_ptr(), dst.stride(0), k_cache.data_ptr(),
+                   v_cache.data_ptr(), nb, runtime(dev).status.data_ptr(), own.data_ptr(), S, Hkv, keep, recent, max_ctx, bs, D * k_cache.element_size(),
+                   int(dst_table is None), 0)
+    _native.check(_native.lib().mb_kv_evict(C.byref(a), _stream()), "kv_evict")
     _count(2)
     return kept, new_len
