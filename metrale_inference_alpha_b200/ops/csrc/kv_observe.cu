@@ -7,9 +7,10 @@
 // Both are the same kernel with the operands exchanged: what a thread owns is a lane of the accumulator in tensor memory, so that neither pass
 // sums across lanes. Query rows of a kv head are numbered token * G + head of the group, as in attention_rows.cu.
 //
-// Roles (512 threads, one CTA per SM): warps 0-3 and 4-7 own 128 lanes each, warps 8-11 stage what goes by (an e4m3 cache becomes f16, the
-// queries are then f16 scaled by a power of two per row, which the rows pass leaves in the workspace for the keys pass), warp 12 issues the
-// products into two accumulators for either half, so that products run under the exponentials.
+// Roles (768 threads, one CTA per SM): of warps 0-15 every four own 128 lanes and half of a tile's columns, so that a scheduler has four of them to run
+// exponentials of; warps 16-19 stage what goes by (an e4m3 cache becomes f16, the queries are then f16 scaled by a power of two per row, which the rows
+// pass leaves in the workspace for the keys pass), warp 20 issues the products into two accumulators for either half of the lanes, so that products run
+// under the exponentials.
 //
 // Long rows and long columns are cut into parts, by rules on the sequence's own lengths alone, and joined in order: every output has one writer and
 // every sum one order.
@@ -21,7 +22,7 @@ namespace {
 
 using namespace mbr;
 
-constexpr int kThreads = 512, kMaxKeyParts = 32, kMaxRowParts = 16, kInfo = 8;
+constexpr int kThreads = 768, kSums = 512, kMaxKeyParts = 32, kMaxRowParts = 16, kInfo = 8;
 template <int N>
 __device__ __forceinline__ void more_regs() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N>
@@ -61,7 +62,7 @@ __host__ __device__ __forceinline__ int parts_of(int n, int part) { return n <= 
 // and the power of two that a row's scores are too large by; sums of the columns' parts [row parts, seqs * Hkv, columns]
 struct Ws {
   long long rows, cols;
-  int key_parts, row_parts;
+  int key_parts, row_parts, slices;   // slices: CTAs that a block of rows is shared out over
   size_t q, scale, sums, bytes;
 };
 inline Ws workspace(int seqs, int Hq, int Hkv, int D, int seen, int max_ctx, bool fp8) {
@@ -71,6 +72,7 @@ inline Ws workspace(int seqs, int Hq, int Hkv, int D, int seen, int max_ctx, boo
   // more parts than any sequence of the call has: fewer rows than the most may mean more of them
   w.key_parts = parts_of(max_ctx, 512) < kMaxKeyParts ? parts_of(max_ctx, 512) : kMaxKeyParts;
   w.row_parts = parts_of((int)w.rows, row_part((int)w.rows));
+  w.slices = parts_of(max_ctx, key_part(max_ctx, (int)w.rows));
   const size_t n = (size_t)seqs * Hkv * w.rows;
   w.q = (n * w.key_parts * 8 + 15) & ~size_t(15);            // the queries are read and written in vectors of 16 bytes
   w.scale = w.q + (fp8 ? n * D * 2 : 0);
@@ -83,26 +85,31 @@ inline Ws workspace(int seqs, int Hq, int Hkv, int D, int seen, int max_ctx, boo
 template <int D, bool FP8, bool KEYS>
 struct Cfg {
   static constexpr int kN = D == 256 ? 64 : 128;             // rows of a tile that goes by
-  static constexpr int kHalves = D / 64;                     // spans of 128 bytes across a row
-  static constexpr int kStages = D == 256 ? 2 : 4;
-  // A row's factors outlive its tile: those of tile j + kInfo are written when the products of tile j + kInfo - kStages are done, whose accumulators were
-  // given back behind tile j + kInfo - kStages - 3 at least.
-  static_assert(kInfo >= kStages + 3, "factors would be written over while they are read");
-  static constexpr int kHeldB = 256 * D * 2, kTileB = kN * D * 2;
-  static constexpr int kSmem = kHeldB + kStages * kTileB + 1024;
+  // A tile comes in chunks of up to 128 dims, which go round a ring of stages. An e4m3 cache's bytes wait in a ring of their own to be widened.
+  static constexpr int kDims = D == 256 ? 128 : D, kChunks = D / kDims, kSpans = kDims / 64;   // of a chunk; spans of 128 bytes across it
+  static constexpr bool kWiden = FP8 && !KEYS;
+  static constexpr int kStages = D == 256 ? (kWiden ? 4 : 5) : kWiden ? 3 : 4;
+  static constexpr int kRaw = kWiden ? 3 : 0;
+  static constexpr int kHeldB = 256 * D * 2, kChunkB = kN * kDims * 2, kRawB = kN * kDims;
+  static constexpr int kSmem = kHeldB + kStages * kChunkB + kRaw * kRawB + 1024;
   static constexpr uint32_t kCols = 4 * kN;                  // two halves of the lanes, two accumulators each
+  // A row's factors outlive its tile: those of tile j + kInfo are written when the products of kStages chunks before it are done, whose accumulators were
+  // given back two tiles later at least.
+  static_assert(kInfo >= (kStages + kChunks - 1) / kChunks + 3, "factors would be written over while they are read");
 };
 
 template <int D, bool FP8, bool KEYS>
 __global__ void __launch_bounds__(kThreads, 1) observe_kernel(const MbMassArgs a, const Ws ws, int g_magic) {
   using C = Cfg<D, FP8, KEYS>;
-  constexpr int kN = C::kN, kHalves = C::kHalves, kStages = C::kStages;
+  constexpr int kN = C::kN, kStages = C::kStages, kChunks = C::kChunks;
   extern __shared__ __align__(16) uint8_t smem_raw[];
-  uint8_t* sHeld = smem_raw + ((1024u - (mb::smem_u32(smem_raw) & 1023u)) & 1023u);   // 2 x kHalves x [128 rows x 128 B]
-  uint8_t* sTile = sHeld + C::kHeldB;                        // kStages x kHalves x [kN rows x 128 B]
+  uint8_t* sHeld = smem_raw + ((1024u - (mb::smem_u32(smem_raw) & 1023u)) & 1023u);   // 2 x D / 64 spans x [128 rows x 128 B]
+  uint8_t* sRing = sHeld + C::kHeldB;                        // kStages x kSpans x [kN rows x 128 B]
+  uint8_t* sRaw = sRing + kStages * C::kChunkB;              // kRaw x [kN rows x kDims B]
   __shared__ __align__(8) uint64_t held_full, full[kStages], empty[kStages], info_full[kInfo], s_full[2][2], s_free[2][2];
   __shared__ uint32_t s_tmem;
   __shared__ float s_row[256];                               // rows pass, e4m3: what a row's scores are too large by
+  __shared__ float2 s_half[256];                             // sums of the second half of the columns
   __shared__ __align__(16) float4 s_info[kInfo][kN / 2];     // keys pass: factors and normalisers of two query rows
   const int h = blockIdx.y, s = blockIdx.z, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int G = a.Hq / a.Hkv;
@@ -112,10 +119,12 @@ __global__ void __launch_bounds__(kThreads, 1) observe_kernel(const MbMassArgs a
   auto tok_of = [&](int r) { return G == 1 ? r : (int)__umulhi((unsigned)r, (unsigned)g_magic); };
   auto limit_of = [&](int r) { return x.past + tok_of(r) + 1; };       // keys in front of this one are visible to row r
   // ---- what stays, and the range of what goes by
-  const int parts = KEYS ? rparts : kparts, blocks = gridDim.x / (KEYS ? ws.row_parts : ws.key_parts);
-  const int part = blockIdx.x / blocks, at0 = (KEYS ? (int)blockIdx.x % blocks : blocks - 1 - (int)blockIdx.x % blocks) * 256;   // the longest first
+  // A column's parts are a CTA each. So are a row's where the call's longest portion has as many; shorter portions, whose rows have more of them, share
+  // `slices` CTAs out.
+  const int slices = KEYS ? ws.row_parts : ws.slices, blocks = gridDim.x / slices, share = KEYS ? 1 : (kparts + slices - 1) / slices;
+  const int part = blockIdx.x / blocks * share, at0 = (KEYS ? (int)blockIdx.x % blocks : blocks - 1 - (int)blockIdx.x % blocks) * 256;   // the longest first
   const int own = KEYS ? x.n : x.rows;
-  if (part >= parts || at0 >= own || x.rows == 0 || x.n == 0) return;
+  if (part >= (KEYS ? rparts : kparts) || at0 >= own || x.rows == 0 || x.n == 0) return;
   const bool two = own - at0 > 128;
   int begin, end;
   if constexpr (KEYS) {
@@ -125,7 +134,7 @@ __global__ void __launch_bounds__(kThreads, 1) observe_kernel(const MbMassArgs a
     end = min(x.rows, (part + 1) * rp);
   } else {
     begin = part * kp;
-    end = min(min(x.n, begin + kp), limit_of(min(x.rows, at0 + 256) - 1));
+    end = min(min(x.n, begin + share * kp), limit_of(min(x.rows, at0 + 256) - 1));
   }
   const int tiles = end > begin ? (end - begin + kN - 1) / kN : 0;
   const size_t row0 = ((size_t)s * a.Hkv + h) * ws.rows;     // of the workspace's rows
@@ -134,7 +143,7 @@ __global__ void __launch_bounds__(kThreads, 1) observe_kernel(const MbMassArgs a
   float* wscale = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(a.ws) + ws.scale) + row0;
 
   if (tid == 0) {
-    mb::mbar_init(&held_full, 8);
+    mb::mbar_init(&held_full, kSums / 32);
     for (int i = 0; i < kStages; ++i) {
       mb::mbar_init(&full[i], 4);
       mb::mbar_init(&empty[i], 1);
@@ -142,11 +151,11 @@ __global__ void __launch_bounds__(kThreads, 1) observe_kernel(const MbMassArgs a
     for (int i = 0; i < kInfo; ++i) mb::mbar_init(&info_full[i], 4);
     for (int i = 0; i < 4; ++i) {
       mb::mbar_init(&s_full[i >> 1][i & 1], 1);
-      mb::mbar_init(&s_free[i >> 1][i & 1], 4);
+      mb::mbar_init(&s_free[i >> 1][i & 1], 8);
     }
     mb::mbar_fence_init();
   }
-  if (warp == 12) mb::tmem_alloc(&s_tmem, C::kCols);
+  if (warp == 20) mb::tmem_alloc(&s_tmem, C::kCols);
   mb::tc_fence_before();
   __syncthreads();
   mb::tc_fence_after();
@@ -156,13 +165,15 @@ __global__ void __launch_bounds__(kThreads, 1) observe_kernel(const MbMassArgs a
   const int* table = a.block_table + s * a.table_ld;
   const int shift = (a.block_size & (a.block_size - 1)) == 0 ? 31 - __clz(a.block_size) : -1;
   int bad = 0;
-  auto key_at = [&](int j) -> long long {                    // byte offset of cached row j < n of this kv head
-    const int bi = shift >= 0 ? j >> shift : j / a.block_size;
-    int b = __ldg(table + bi);
-    const bool out = (unsigned)b >= (unsigned long long)a.num_blocks;
+  auto block_of = [&](int j) { return shift >= 0 ? j >> shift : j / a.block_size; };
+  constexpr int kRowB = D * (FP8 ? 1 : 2);
+  const uint8_t* keys = reinterpret_cast<const uint8_t*>(a.k_cache) + (size_t)h * kRowB;
+  const int pitch = a.Hkv * kRowB;
+  auto key_at = [&](int j, int b) {                          // cached row j < n, which is in block b
+    const bool out = (unsigned)b >= (unsigned)a.num_blocks;
     bad |= out;
-    b = out ? 0 : b;
-    return (((long long)b * a.block_size + (j - bi * a.block_size)) * a.Hkv + h) * (D * (FP8 ? 1 : 2));
+    const int slot = (out ? 0 : b) * a.block_size + (j - block_of(j) * a.block_size);
+    return keys + (long long)slot * pitch;
   };
   auto query_at = [&](int r) -> const __nv_bfloat16* {
     const int tq = tok_of(r);
@@ -176,21 +187,22 @@ __global__ void __launch_bounds__(kThreads, 1) observe_kernel(const MbMassArgs a
     hi = make_uint4(e4m3x2(raw.z), e4m3x2(raw.z >> 16), e4m3x2(raw.w), e4m3x2(raw.w >> 16));
   };
 
-  if (warp < 8) {
-    more_regs<184>();
-    const int w = warp >> 2, r = tid & 127, mine = at0 + w * 128 + r;
+  if (warp < 16) {
+    more_regs<88>();
+    const int w = warp >> 3, half = warp >> 2 & 1, r = tid & 127, mine = at0 + w * 128 + r;
+    constexpr int kW = kN / 2;                               // columns of a thread
     // ---- the operand that stays: 256 rows, rows behind the last one are zeros
-    constexpr int kPieces = KEYS && FP8 ? D / 16 : D / 8, kStep = 256 / kPieces, kLoads = 256 / kStep;
+    constexpr int kPieces = KEYS && FP8 ? D / 16 : D / 8, kStep = kSums / kPieces, kLoads = 256 / kStep;
     const int c = tid % kPieces;
 #pragma unroll 1
-    for (int i0 = 0; i0 < kLoads; i0 += 16) {
-      constexpr int kBatch = kLoads < 16 ? kLoads : 16;
+    for (int i0 = 0; i0 < kLoads; i0 += 8) {
+      constexpr int kBatch = kLoads < 8 ? kLoads : 8;
       uint4 v[kBatch];
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) {
         const int hr = tid / kPieces + kStep * (i0 + i), at = min(at0 + hr, own - 1);
         if constexpr (KEYS)
-          v[i] = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(a.k_cache) + key_at(at)) + c);
+          v[i] = __ldg(reinterpret_cast<const uint4*>(key_at(at, __ldg(table + block_of(at)))) + c);
         else
           v[i] = __ldg(reinterpret_cast<const uint4*>(query_at(at)) + c);
         if (at0 + hr >= own) v[i] = make_uint4(0, 0, 0, 0);
@@ -237,13 +249,30 @@ __global__ void __launch_bounds__(kThreads, 1) observe_kernel(const MbMassArgs a
     fence_async_smem();
     __syncwarp();
     if (lane == 0) mb::mbar_arrive(&held_full);
-    if constexpr (FP8 && !KEYS) asm volatile("bar.sync 1, 256;" ::: "memory");       // the rows' scales come from other warps
+    if constexpr (FP8 && !KEYS) asm volatile("bar.sync 1, 512;" ::: "memory");       // the rows' scales come from other warps
     const float sc = factor(FP8 && !KEYS ? s_row[w * 128 + r] : 1.f);
     const int limit = KEYS ? 0 : mine < own ? limit_of(mine) : 0;
-    const uint32_t tS = tmem + ((uint32_t)((warp & 3) * 32) << 16) + w * 2 * kN;
+    const uint32_t tS = tmem + ((uint32_t)((warp & 3) * 32) << 16) + w * 2 * kN + half * kW;
     float m_run = -INFINITY, l_run = 0.f;                    // keys pass: l_run is the column's sum
     bool ok = true;
     const int count = w == 0 || two ? tiles : 0;
+    // rows pass: a part of a row's keys is done; the halves of the columns are joined
+    int mine_part = part, flush_at = (part + 1) * kp;
+    auto flush = [&] {
+      if (half) s_half[w * 128 + r] = make_float2(m_run, l_run);
+      asm volatile("bar.sync %0, 256;" ::"r"(2 + w) : "memory");
+      if (!half && mine < own) {
+        const float2 y = s_half[w * 128 + r];
+        const float top = fmaxf(m_run, y.x);
+        const float l = (m_run == -INFINITY ? 0.f : l_run * ex2(m_run - top)) + (y.x == -INFINITY ? 0.f : y.y * ex2(y.x - top));
+        ml[(size_t)mine * ws.key_parts + mine_part] = make_float2(top, l);
+      }
+      asm volatile("bar.sync %0, 256;" ::"r"(2 + w) : "memory");
+      m_run = -INFINITY;
+      l_run = 0.f;
+      ++mine_part;
+      flush_at += kp;
+    };
     for (int t = 0; t < count; ++t) {
       const int b = t & 1;
       ok = mb::mbar_wait(&s_full[w][b], (t >> 1) & 1, a.status, MB_ST_TIMEOUT_MMA);
@@ -253,25 +282,25 @@ __global__ void __launch_bounds__(kThreads, 1) observe_kernel(const MbMassArgs a
         break;
       }
       mb::tc_fence_after();
-      float z[kN];
+      float z[kW];
 #pragma unroll
-      for (int i = 0; i < kN; i += 32) mb::tmem_ld32_async(tS + b * kN + i, z + i);
+      for (int i = 0; i < kW; i += 32) mb::tmem_ld32_async(tS + b * kN + i, z + i);
       mb::tmem_ld_wait(z);
       mb::tc_fence_before();
       __syncwarp();
       if (lane == 0) mb::mbar_arrive(&s_free[w][b]);         // the accumulator is in registers
-      const int from = begin + t * kN;
+      const int from = begin + t * kN + half * kW;
       float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
       if constexpr (KEYS) {
-        const float4* info = s_info[t % kInfo];
-        // the tile's first row sees the least: all of these keys, or a row each is asked
+        const float4* info = &s_info[t % kInfo][half * kW / 2];
+        // these rows' first one sees the least: all of these keys, or a row each is asked
         if (__any_sync(0xffffffffu, mine >= limit_of(from))) {
 #pragma unroll
-          for (int i = 0; i < kN; ++i)
+          for (int i = 0; i < kW; ++i)
             if (mine >= limit_of(from + i)) z[i] = -INFINITY;
         }
 #pragma unroll
-        for (int i = 0; i < kN / 2; ++i) {
+        for (int i = 0; i < kW / 2; ++i) {
           const float4 f = info[i];
           float2 p = fma2(make_float2(z[2 * i], z[2 * i + 1]), make_float2(f.x, f.y), make_float2(f.z, f.w));
           p.x = ex2(p.x);
@@ -281,165 +310,232 @@ __global__ void __launch_bounds__(kThreads, 1) observe_kernel(const MbMassArgs a
         l_run += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
       } else {
         const int seen = min(limit, end) - from;             // columns in front of this one are visible
-        if (!__all_sync(0xffffffffu, seen >= kN)) {
+        if (!__all_sync(0xffffffffu, seen >= kW)) {
 #pragma unroll
-          for (int i = 0; i < kN; ++i)
+          for (int i = 0; i < kW; ++i)
             if (i >= seen) z[i] = -INFINITY;
         }
-        float mx4[4] = {z[0], z[1], z[2], z[3]};
+        const float2 sc2 = make_float2(sc, sc);
+        auto add = [&] {
+          const float nm = m_run == -INFINITY ? 0.f : -m_run;
+          const float2 nm2 = make_float2(nm, nm);
+          sum[0] = sum[1] = make_float2(0.f, 0.f);
 #pragma unroll
-        for (int i = 4; i < kN; ++i) mx4[i & 3] = fmaxf(mx4[i & 3], z[i]);
-        const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * sc;
-        if (mx > m_run + 8.f) {                              // also true on a row's first finite tile
-          l_run *= ex2(m_run - mx);
-          m_run = mx;
-        }
-        const float nm = m_run == -INFINITY ? 0.f : -m_run;
-        const float2 sc2 = make_float2(sc, sc), nm2 = make_float2(nm, nm);
+          for (int i = 0; i < kW / 2; ++i) {
+            float2 p = fma2(make_float2(z[2 * i], z[2 * i + 1]), sc2, nm2);
+            p.x = ex2(p.x);
+            p.y = ex2(p.y);
+            sum[i & 1] = add2(sum[i & 1], p);
+          }
+          return (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+        };
+        // What a row is relative to need not be its maximum, as long as nothing overflows and something of it is near 1: the largest of its first tile
+        // with a visible column stands until a tile's sum passes 2^60.
+        float tile = add();
+        if (__any_sync(0xffffffffu, m_run == -INFINITY || !(tile < 0x1p60f))) {
+          float mx = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < kN / 2; ++i) {
-          float2 p = fma2(make_float2(z[2 * i], z[2 * i + 1]), sc2, nm2);
-          p.x = ex2(p.x);
-          p.y = ex2(p.y);
-          sum[i & 1] = add2(sum[i & 1], p);
+          for (int i = 0; i < kW; ++i) mx = fmaxf(mx, z[i]);
+          mx *= sc;
+          if (mx > m_run && (m_run == -INFINITY || !(tile < 0x1p60f))) {
+            l_run *= ex2(m_run - mx);
+            m_run = mx;
+          }
+          tile = add();
         }
-        l_run += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+        l_run += tile;
+        if (begin + (t + 1) * kN == flush_at) flush();
       }
     }
-    if (mine < own) {
-      if constexpr (KEYS) {
+    if constexpr (KEYS) {
+      if (half) s_half[w * 128 + r].y = l_run;
+      asm volatile("bar.sync 1, 512;" ::: "memory");
+      if (!half && mine < own) {
+        l_run += s_half[w * 128 + r].y;
         if (ws.row_parts > 1)
           reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(a.ws) + ws.sums)[((size_t)part * a.num_seqs * a.Hkv + (size_t)s * a.Hkv + h) * ws.cols + mine] = l_run;
         else
           a.mass[s * a.mass_seq + h * a.mass_head + mine] += l_run;
-      } else {
-        ml[(size_t)mine * ws.key_parts + part] = make_float2(m_run, l_run);
       }
+    } else if (w == 0 || two) {
+      while (mine_part < min(part + share, kparts)) flush();   // parts behind what these rows see are empty
     }
     mb::tc_fence_before();
-  } else if (warp < 12) {
+  } else if (warp < 20) {
     // ------------------------------------------------------------ what goes by
-    fewer_regs<80>();
-    const int t = tid - 256;
-    constexpr bool kWiden = FP8 && !KEYS;
-    constexpr int kPieces = kWiden ? D / 16 : D / 8, kStep = 128 / kPieces, kLoads = kN / kStep;
-    const int r0 = t / kPieces, c = t % kPieces;
+    fewer_regs<72>();
+    const int t = tid - kSums;
+    constexpr bool kWiden = C::kWiden;
+    // 16-byte pieces of a chunk's row, rows between a thread's pieces, and how many it has
+    constexpr int kPieces = kWiden ? C::kDims / 16 : C::kDims / 8, kStep = 128 / kPieces, kLoads = kN / kStep;
+    // Chunks under way while the next is asked for. A chunk is announced when kAhead more have been asked for, which waits for the products of
+    // kStages - kAhead chunks before it: two, or the products would go one by one.
+    constexpr int kAhead = kWiden ? C::kRaw - 1 : kStages - 2;
+    const int r0 = t / kPieces, c = t % kPieces, chunks = tiles * kChunks;
     bool ok = true;
-    auto announce = [&](int j) {
+    auto announce = [&](int j) {                             // chunk j
       fence_async_smem();
       __syncwarp();
       if (lane == 0) {
         mb::mbar_arrive(&full[j % kStages]);
-        if (KEYS) mb::mbar_arrive(&info_full[j % kInfo]);
+        if (KEYS && j % kChunks == 0) mb::mbar_arrive(&info_full[j / kChunks % kInfo]);
       }
     };
-    if constexpr (kWiden) {
-      uint4 raw[kLoads];
-      auto fetch = [&](int j) {
+    // rows pass: the blocks of a tile's rows are looked up a tile before they are read, and not touched until then
+    int next[KEYS ? 1 : kLoads];
+    auto places = [&](int tile) {
+      if constexpr (!KEYS)
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-          const int k = begin + j * kN + r0 + i * kStep;
-          raw[i] = k < end ? __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(a.k_cache) + key_at(k)) + c) : make_uint4(0, 0, 0, 0);
+        for (int i = 0; i < kLoads; ++i) next[i] = __ldg(table + block_of(min(begin + tile * kN + r0 + i * kStep, end - 1)));
+    };
+    // keys pass: so are the parts of a row's normaliser
+    constexpr int kTake = 4;
+    float2 y[KEYS ? kTake : 1];
+    float yscale = 1.f;
+    auto look = [&](int tile) {
+      if constexpr (KEYS) {
+        const int at = min(begin + tile * kN + t, end - 1);
+        if (t < kN) {
+#pragma unroll
+          for (int k = 0; k < kTake; ++k) y[k] = k < kparts ? ml[(size_t)at * ws.key_parts + k] : make_float2(-INFINITY, 0.f);
+          if (FP8) yscale = wscale[at];
         }
-      };
-      fetch(0);
-      for (int j = 0; j < tiles; ++j) {
-        ok = mb::mbar_wait(&empty[j % kStages], ((j / kStages) & 1) ^ 1, a.status, MB_ST_TIMEOUT_TMA);
-        if (!__all_sync(0xffffffffu, ok)) break;
-        uint8_t* tile = sTile + (j % kStages) * C::kTileB + (c >> 2) * (kN * 128);
+      }
+    };
+    auto inform = [&](int tile) {
+      if constexpr (KEYS) {
+        // a row's normaliser from the parts of its keys, in order; rows behind the last one add nothing
+        if (t < kN) {
+          const int at = begin + tile * kN + t;
+          float f = 1.f, lse = INFINITY, m = -INFINITY, l = 0.f;
+          for (int i = 0; i < kparts; i += kTake) {
+            if (i > 0) {
+#pragma unroll
+              for (int k = 0; k < kTake; ++k) y[k] = i + k < kparts ? ml[(size_t)min(at, end - 1) * ws.key_parts + i + k] : make_float2(-INFINITY, 0.f);
+            }
+#pragma unroll
+            for (int k = 0; k < kTake; ++k) {
+              const float top = fmaxf(m, y[k].x);
+              l = (m == -INFINITY ? 0.f : l * ex2(m - top)) + (y[k].x == -INFINITY ? 0.f : y[k].y * ex2(y[k].x - top));
+              m = top;
+            }
+          }
+          if (at < end) {
+            f = factor(yscale);
+            if (l != 0.f) lse = m + log2f(l);
+          }
+          float* info = reinterpret_cast<float*>(&s_info[tile % kInfo][t >> 1]) + (t & 1);
+          info[0] = f;
+          info[2] = -lse;
+        }
+      }
+    };
+    auto ask = [&](int j) {                                  // chunk j into its stage, or an e4m3 cache's into the ring of bytes
+      const int tile = j / kChunks, q = j % kChunks;
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int r = r0 + i * kStep, at = begin + tile * kN + r, safe = min(at, end - 1);
+        const uint8_t* src;
+        if constexpr (!KEYS) src = key_at(safe, next[i]);
+        else if constexpr (FP8) src = reinterpret_cast<const uint8_t*>(wq + (size_t)safe * D);
+        else src = reinterpret_cast<const uint8_t*>(query_at(safe));
+        uint8_t* dst = kWiden ? sRaw + (j % 3) * C::kRawB + (i * 128 + t) * 16 : sRing + (j % kStages) * C::kChunkB + (c >> 3) * (kN * 128) + sw_off(r, c & 7);
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(mb::smem_u32(dst)), "l"(src + (q * kPieces + c) * 16), "r"(at < end ? 16 : 0) : "memory");
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    auto wait_empty = [&](int j) {
+      ok = mb::mbar_wait(&empty[j % kStages], ((j / kStages) & 1) ^ 1, a.status, MB_ST_TIMEOUT_TMA);
+      return __all_sync(0xffffffffu, ok);
+    };
+    if (chunks > 0) {
+      places(0);
+      look(0);
+    }
+    if constexpr (kWiden) {
+      // a thread widens the bytes that it asked for itself
+      for (int j = 0; j < chunks + kAhead; ++j) {
+        if (j < chunks) {
+          ask(j);
+          if (j % kChunks == kChunks - 1) places(j / kChunks + 1);
+        } else {
+          asm volatile("cp.async.commit_group;" ::: "memory");
+        }
+        const int k = j - kAhead;
+        if (k < 0) continue;
+        asm volatile("cp.async.wait_group %0;" ::"n"(kAhead) : "memory");
+        if (!wait_empty(k)) break;
+        const uint8_t* raw = sRaw + (k % 3) * C::kRawB + t * 16;
+        uint8_t* chunk = sRing + (k % kStages) * C::kChunkB + (c >> 2) * (kN * 128);
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
           uint4 lo, hi;
-          widen(raw[i], lo, hi);
-          *reinterpret_cast<uint4*>(tile + sw_off(r0 + i * kStep, (c & 3) * 2)) = lo;
-          *reinterpret_cast<uint4*>(tile + sw_off(r0 + i * kStep, (c & 3) * 2 + 1)) = hi;
+          widen(*reinterpret_cast<const uint4*>(raw + i * 128 * 16), lo, hi);
+          *reinterpret_cast<uint4*>(chunk + sw_off(r0 + i * kStep, (c & 3) * 2)) = lo;
+          *reinterpret_cast<uint4*>(chunk + sw_off(r0 + i * kStep, (c & 3) * 2 + 1)) = hi;
         }
-        announce(j);
-        fetch(j + 1);
+        announce(k);
       }
     } else {
-      constexpr int kLag = kStages - 1;                      // tiles under way while the next is asked for
-      for (int j = 0; j < tiles; ++j) {
-        ok = mb::mbar_wait(&empty[j % kStages], ((j / kStages) & 1) ^ 1, a.status, MB_ST_TIMEOUT_TMA);
-        if (!__all_sync(0xffffffffu, ok)) break;
-        uint8_t* tile = sTile + (j % kStages) * C::kTileB + (c >> 3) * (kN * 128);
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-          const int at = begin + j * kN + r0 + i * kStep, safe = min(at, end - 1);
-          const void* src;
-          if constexpr (!KEYS) src = reinterpret_cast<const uint8_t*>(a.k_cache) + key_at(safe);
-          else if constexpr (FP8) src = wq + (size_t)safe * D;
-          else src = query_at(safe);
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(mb::smem_u32(tile + sw_off(r0 + i * kStep, c & 7))),
-                       "l"(reinterpret_cast<const uint4*>(src) + c), "r"(at < end ? 16 : 0)
-                       : "memory");
+      for (int j = 0; j < chunks; ++j) {
+        if (!wait_empty(j)) break;
+        ask(j);
+        if (KEYS && j % kChunks == 0) {
+          inform(j / kChunks);
+          look(j / kChunks + 1);
         }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-        if constexpr (KEYS) {
-          // a row's normaliser from the parts of its keys, in order; rows behind the last one add nothing
-          if (t < kN) {
-            const int at = begin + j * kN + t;
-            float f = 1.f, lse = INFINITY;
-            if (at < end) {
-              const float2* p = ml + (size_t)at * ws.key_parts;
-              float m = -INFINITY, l = 0.f;
-              for (int i = 0; i < kparts; ++i) {
-                const float2 y = p[i];
-                const float top = fmaxf(m, y.x);
-                l = (m == -INFINITY ? 0.f : l * ex2(m - top)) + (y.x == -INFINITY ? 0.f : y.y * ex2(y.x - top));
-                m = top;
-              }
-              f = factor(FP8 ? wscale[at] : 1.f);
-              if (l != 0.f) lse = m + log2f(l);
-            }
-            float* info = reinterpret_cast<float*>(&s_info[j % kInfo][t >> 1]) + (t & 1);
-            info[0] = f;
-            info[2] = -lse;
-          }
-        }
-        if (j >= kLag) {
-          asm volatile("cp.async.wait_group %0;" ::"n"(kLag) : "memory");
-          announce(j - kLag);
+        if (!KEYS && j % kChunks == kChunks - 1) places(j / kChunks + 1);
+        if (j >= kAhead) {
+          asm volatile("cp.async.wait_group %0;" ::"n"(kAhead) : "memory");
+          announce(j - kAhead);
         }
       }
       if (__all_sync(0xffffffffu, ok)) {
         asm volatile("cp.async.wait_group 0;" ::: "memory");
-        for (int j = max(0, tiles - kLag); j < tiles; ++j) announce(j);
+        for (int j = max(0, chunks - kAhead); j < chunks; ++j) announce(j);
       }
-      asm volatile("cp.async.wait_all;" ::: "memory");
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
   } else {
-    fewer_regs<48>();
-    if (warp == 12 && mb::elect_one()) {
+    fewer_regs<56>();
+    if (warp == 20 && mb::elect_one()) {
       // ---------------------------------------------------------- products
       constexpr uint32_t kF = FP8 ? 0 : 1, kId = mb::umma_idesc(kF, kF, 128, kN);
-      const uint32_t aH = mb::smem_u32(sHeld), aT = mb::smem_u32(sTile);
+      // an address is the low bits of a descriptor, in units of 16 bytes
+      const uint64_t dH = mb::umma_desc_sw128(mb::smem_u32(sHeld)), dR = mb::umma_desc_sw128(mb::smem_u32(sRing));
       bool ok = mb::mbar_wait(&held_full, 0, a.status, MB_ST_TIMEOUT_MMA);
-      for (int j = 0; j < tiles && ok; ++j) {
-        const int st = j % kStages, b = j & 1;
-        ok = mb::mbar_wait(&full[st], (j / kStages) & 1, a.status, MB_ST_TIMEOUT_MMA);
+      const int chunks = tiles * kChunks;
+      int st = 0, turn = 0;
+      for (int j = 0; j < chunks && ok; ++j) {
+        const int tile = j / kChunks, q = j % kChunks, b = tile & 1;
+        ok = mb::mbar_wait(&full[st], turn, a.status, MB_ST_TIMEOUT_MMA);
+        const uint64_t dC = dR + (uint32_t)(st * (C::kChunkB >> 4)), dQ = dH + q * (C::kSpans * 128 * 128 >> 4);
         for (int w = 0; w < (two ? 2 : 1) && ok; ++w) {
-          ok = mb::mbar_wait(&s_free[w][b], ((j >> 1) & 1) ^ 1, a.status, MB_ST_TIMEOUT_MMA);
+          if (q == 0) ok = mb::mbar_wait(&s_free[w][b], ((tile >> 1) & 1) ^ 1, a.status, MB_ST_TIMEOUT_MMA);
           if (!ok) break;
           mb::tc_fence_after();
+          const uint64_t dA = dQ + (uint32_t)(w * (128 * D * 2 >> 4));
 #pragma unroll
-          for (int hh = 0; hh < kHalves; ++hh)
+          for (int hh = 0; hh < C::kSpans; ++hh)
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              mb::umma_f16(tmem + (w * 2 + b) * kN, mb::umma_desc_sw128(aH + w * (128 * D * 2) + hh * (128 * 128) + k * 32),
-                           mb::umma_desc_sw128(aT + st * C::kTileB + hh * (kN * 128) + k * 32), kId, (hh | k) != 0);
-          mb::tc_commit(&s_full[w][b]);
+              mb::umma_f16(tmem + (w * 2 + b) * kN, dA + (hh * (128 * 128) + k * 32 >> 4), dC + (hh * (kN * 128) + k * 32 >> 4), kId, (q | hh | k) != 0);
+          if (q == kChunks - 1) mb::tc_commit(&s_full[w][b]);
         }
         if (ok) mb::tc_commit(&empty[st]);
+        if (++st == kStages) {
+          st = 0;
+          turn ^= 1;
+        }
       }
       // nobody may free the accumulators under products in flight
-      if (ok && tiles > 0) mb::mbar_wait(&empty[(tiles - 1) % kStages], ((tiles - 1) / kStages) & 1, a.status, MB_ST_TIMEOUT_MMA);
+      if (ok && chunks > 0) mb::mbar_wait(&empty[(chunks - 1) % kStages], ((chunks - 1) / kStages) & 1, a.status, MB_ST_TIMEOUT_MMA);
     }
     __syncwarp();
   }
   if (bad && a.status) atomicCAS(a.status, 0u, MB_ST_BOUNDS);
   __syncthreads();
-  if (warp == 12) {
+  if (warp == 20) {
     mb::tc_fence_after();
     mb::tmem_dealloc(tmem, C::kCols);
   }
@@ -469,7 +565,7 @@ int launch(const MbMassArgs& a, const Ws& ws, cudaStream_t stream) {
   }
   const int G = a.Hq / a.Hkv;
   const unsigned magic = G == 1 ? 0 : (unsigned)(((1ull << 32) + G - 1) / G);
-  const long long blocks = ((KEYS ? (long long)a.max_ctx : ws.rows) + 255) / 256 * (KEYS ? ws.row_parts : ws.key_parts);
+  const long long blocks = ((KEYS ? (long long)a.max_ctx : ws.rows) + 255) / 256 * (KEYS ? ws.row_parts : ws.slices);
   if (blocks > 0x7fffffffll) return MB_ERR_TOO_LARGE;
   return (int)mb::launch_kernel_ex(kern, dim3((unsigned)blocks, a.Hkv, a.num_seqs), dim3(kThreads), Cfg<D, FP8, KEYS>::kSmem, stream, 1, KEYS, a, ws, (int)magic);
 }
@@ -492,6 +588,7 @@ int mb_prompt_mass(const MbMassArgs* a, cudaStream_t stream) {
       !a->q_start || !a->q_len || !a->ctx_len || !a->mass || (a->fp8 && !a->k_scale))
     return MB_ERR_BAD_ARG;
   if ((reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->k_cache) | reinterpret_cast<uintptr_t>(a->ws)) & 15) return MB_ERR_UNSUPPORTED;
+  if (a->num_blocks * a->block_size >= (1ll << 31)) return MB_ERR_TOO_LARGE;
   if ((long long)a->last * (a->Hq / a->Hkv) > (1ll << 25)) return MB_ERR_TOO_LARGE;     // rows that tok_of divides exactly
   const Ws ws = workspace(a->num_seqs, a->Hq, a->Hkv, a->D, a->last, a->max_ctx, a->fp8 != 0);
   if (!a->ws || a->ws_bytes < ws.bytes) return MB_ERR_TOO_LARGE;
