@@ -7,22 +7,27 @@
 // Both are the same kernel with the operands exchanged: what a thread owns is a lane of the accumulator in tensor memory, so that neither pass
 // sums across lanes. Query rows of a kv head are numbered token * G + head of the group, as in attention_rows.cu.
 //
+// Both operands come by TMA: keys from the cache, 16 tokens a box, or from a copy in the workspace (an e4m3 cache's as f16, any cache's whose blocks are
+// not whole boxes), which a kernel in front makes; query rows of the keys pass from the copy that the rows pass makes of its own (with an e4m3 cache
+// f16, scaled by a power of two per row). A first form had four warps gather and widen tiles on the way into shared memory, every CTA the same ones: that
+// took the issue slots of the exponentials, 4096 observers at 8192 e4m3 tokens 819 us.
+//
 // Roles (768 threads, one CTA per SM): of warps 0-15 every four own 128 lanes and half of a tile's columns, so that a scheduler has four of them to run
-// exponentials of; warps 16-19 stage what goes by (an e4m3 cache becomes f16, the queries are then f16 scaled by a power of two per row, which the rows
-// pass leaves in the workspace for the keys pass), warp 20 issues the products into two accumulators for either half of the lanes, so that products run
-// under the exponentials.
+// exponentials of; warps 16-19 bring the rows' normalisers (keys pass), warp 20 issues the products into two accumulators for either half of the lanes,
+// so that products run under the exponentials, warp 21 the copies.
 //
 // Long rows and long columns are cut into parts, by rules on the sequence's own lengths alone, and joined in order: every output has one writer and
 // every sum one order.
 #include "attention_rows.cuh"
 #include "common.cuh"
 #include "kv_mass.h"
+#include "tensormap.h"
 
 namespace {
 
 using namespace mbr;
 
-constexpr int kThreads = 768, kSums = 512, kMaxKeyParts = 32, kMaxRowParts = 16, kInfo = 8;
+constexpr int kThreads = 768, kSums = 512, kMaxKeyParts = 32, kMaxRowParts = 16, kInfo = 8, kBox = 16;
 template <int N>
 __device__ __forceinline__ void more_regs() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N>
@@ -58,62 +63,81 @@ __host__ __device__ __forceinline__ int row_part(int rows) {
 }
 __host__ __device__ __forceinline__ int parts_of(int n, int part) { return n <= part ? 1 : (n + part - 1) / part; }
 
-// Workspace: {maximum, sum} of every row and part of its keys, log2 domain [seqs * Hkv * rows, key parts]; with an e4m3 cache the f16 queries
-// and the power of two that a row's scores are too large by; sums of the columns' parts [row parts, seqs * Hkv, columns]
+// Workspace: the query rows as operands [seqs * Hkv * rows, D], and behind them room for a tile; the keys, where they are copied [seqs * tokens, Hkv, D];
+// {maximum, sum} of every row and part of its keys, log2 domain [seqs * Hkv * rows, key parts]; with an e4m3 cache the power of two that a row's scores are
+// too large by; sums of the columns' parts [row parts, seqs * Hkv, columns]
 struct Ws {
-  long long rows, cols;
-  int key_parts, row_parts, slices;   // slices: CTAs that a block of rows is shared out over
-  size_t q, scale, sums, bytes;
+  long long rows, cols, tokens;
+  int key_parts, row_parts, slices, paged;   // slices: CTAs that a block of rows is shared out over
+  size_t keys, ml, scale, sums, bytes;
 };
-inline Ws workspace(int seqs, int Hq, int Hkv, int D, int seen, int max_ctx, bool fp8) {
+inline Ws workspace(int seqs, int Hq, int Hkv, int D, int block_size, int seen, int max_ctx, bool fp8) {
   Ws w;
+  auto even = [](size_t x) { return (x + 127) & ~size_t(127); };
   w.rows = (long long)seen * (Hq / Hkv);
   w.cols = (max_ctx + 3) & ~3ll;
+  w.tokens = (max_ctx + 255) & ~255ll;
+  w.paged = !fp8 && block_size % kBox == 0;
   // more parts than any sequence of the call has: fewer rows than the most may mean more of them
   w.key_parts = parts_of(max_ctx, 512) < kMaxKeyParts ? parts_of(max_ctx, 512) : kMaxKeyParts;
   w.row_parts = parts_of((int)w.rows, row_part((int)w.rows));
   w.slices = parts_of(max_ctx, key_part(max_ctx, (int)w.rows));
   const size_t n = (size_t)seqs * Hkv * w.rows;
-  w.q = (n * w.key_parts * 8 + 15) & ~size_t(15);            // the queries are read and written in vectors of 16 bytes
-  w.scale = w.q + (fp8 ? n * D * 2 : 0);
-  w.sums = w.scale + (fp8 ? n * 4 : 0);
-  w.sums = (w.sums + 15) & ~size_t(15);
+  w.keys = even((n + 128) * D * 2);
+  w.ml = w.keys + (w.paged ? 0 : even((size_t)seqs * w.tokens * Hkv * D * 2));
+  w.scale = w.ml + even(n * w.key_parts * 8);
+  w.sums = w.scale + (fp8 ? even(n * 4) : 0);
   w.bytes = w.sums + (w.row_parts > 1 ? (size_t)w.row_parts * seqs * Hkv * w.cols * 4 : 0);
   return w;
 }
 
-template <int D, bool FP8, bool KEYS>
+// Rows of an e4m3 cache as f16, of a bf16 cache as they are, one sequence behind the other: 16 values a thread.
+template <bool FP8>
+__global__ void __launch_bounds__(256) observe_copy_kernel(const MbMassArgs a, const Ws ws) {
+  mb::pdl_launch_dependents();
+  const int s = blockIdx.y, n = min(a.ctx_len[s], a.max_ctx), per = a.Hkv * a.D / 16;
+  const int* table = a.block_table + s * a.table_ld;
+  uint4* out = reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(a.ws) + ws.keys) + (size_t)s * ws.tokens * per * 2;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < (long long)n * per; i += (long long)gridDim.x * 256) {
+    const int j = (int)(i / per), c = (int)(i - (long long)j * per);
+    const size_t at = (size_t)mbm::slot_of(table, j, a.block_size, a.num_blocks, a.status) * per + c;
+    if constexpr (FP8) {
+      const uint4 x = __ldg(reinterpret_cast<const uint4*>(a.k_cache) + at);
+      out[2 * i] = make_uint4(e4m3x2(x.x), e4m3x2(x.x >> 16), e4m3x2(x.y), e4m3x2(x.y >> 16));
+      out[2 * i + 1] = make_uint4(e4m3x2(x.z), e4m3x2(x.z >> 16), e4m3x2(x.w), e4m3x2(x.w >> 16));
+    } else {
+      out[2 * i] = __ldg(reinterpret_cast<const uint4*>(a.k_cache) + 2 * at);
+      out[2 * i + 1] = __ldg(reinterpret_cast<const uint4*>(a.k_cache) + 2 * at + 1);
+    }
+  }
+}
+
+template <int D>
 struct Cfg {
   static constexpr int kN = D == 256 ? 64 : 128;             // rows of a tile that goes by
-  // A tile comes in chunks of up to 128 dims, which go round a ring of stages. An e4m3 cache's bytes wait in a ring of their own to be widened.
+  // A tile comes in chunks of up to 128 dims, which go round a ring of stages
   static constexpr int kDims = D == 256 ? 128 : D, kChunks = D / kDims, kSpans = kDims / 64;   // of a chunk; spans of 128 bytes across it
-  static constexpr bool kWiden = FP8 && !KEYS;
-  static constexpr int kStages = D == 256 ? (kWiden ? 4 : 5) : kWiden ? 3 : 4;
-  static constexpr int kRaw = kWiden ? 3 : 0;
-  static constexpr int kHeldB = 256 * D * 2, kChunkB = kN * kDims * 2, kRawB = kN * kDims;
-  static constexpr int kSmem = kHeldB + kStages * kChunkB + kRaw * kRawB + 1024;
+  static constexpr int kStages = D == 256 ? 5 : 4;
+  static constexpr int kHeldB = 256 * D * 2, kChunkB = kN * kDims * 2;
+  static constexpr int kSmem = kHeldB + kStages * kChunkB + 1024;
   static constexpr uint32_t kCols = 4 * kN;                  // two halves of the lanes, two accumulators each
-  // A row's factors outlive its tile: those of tile j + kInfo are written when the products of kStages chunks before it are done, whose accumulators were
-  // given back two tiles later at least.
-  static_assert(kInfo >= (kStages + kChunks - 1) / kChunks + 3, "factors would be written over while they are read");
 };
 
 template <int D, bool FP8, bool KEYS>
-__global__ void __launch_bounds__(kThreads, 1) observe_kernel(const MbMassArgs a, const Ws ws, int g_magic) {
-  using C = Cfg<D, FP8, KEYS>;
+__global__ void __launch_bounds__(kThreads, 1)
+observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmQ, const MbMassArgs a, const Ws ws, int g_magic) {
+  using C = Cfg<D>;
   constexpr int kN = C::kN, kStages = C::kStages, kChunks = C::kChunks;
   extern __shared__ __align__(16) uint8_t smem_raw[];
   uint8_t* sHeld = smem_raw + ((1024u - (mb::smem_u32(smem_raw) & 1023u)) & 1023u);   // 2 x D / 64 spans x [128 rows x 128 B]
   uint8_t* sRing = sHeld + C::kHeldB;                        // kStages x kSpans x [kN rows x 128 B]
-  uint8_t* sRaw = sRing + kStages * C::kChunkB;              // kRaw x [kN rows x kDims B]
-  __shared__ __align__(8) uint64_t held_full, full[kStages], empty[kStages], info_full[kInfo], s_full[2][2], s_free[2][2];
+  __shared__ __align__(8) uint64_t held_full, full[kStages], empty[kStages], info_full[kInfo], info_free[kInfo], s_full[2][2], s_free[2][2];
   __shared__ uint32_t s_tmem;
   __shared__ float s_row[256];                               // rows pass, e4m3: what a row's scores are too large by
   __shared__ float2 s_half[256];                             // sums of the second half of the columns
   __shared__ __align__(16) float4 s_info[kInfo][kN / 2];     // keys pass: factors and normalisers of two query rows
   const int h = blockIdx.y, s = blockIdx.z, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int G = a.Hq / a.Hkv;
-  mb::pdl_wait();
   const Span x = span_of(a, s, G);
   const int kp = key_part(x.n, x.rows), kparts = parts_of(x.n, kp), rp = row_part(x.rows), rparts = parts_of(x.rows, rp);
   auto tok_of = [&](int r) { return G == 1 ? r : (int)__umulhi((unsigned)r, (unsigned)g_magic); };
@@ -124,7 +148,10 @@ __global__ void __launch_bounds__(kThreads, 1) observe_kernel(const MbMassArgs a
   const int slices = KEYS ? ws.row_parts : ws.slices, blocks = gridDim.x / slices, share = KEYS ? 1 : (kparts + slices - 1) / slices;
   const int part = blockIdx.x / blocks * share, at0 = (KEYS ? (int)blockIdx.x % blocks : blocks - 1 - (int)blockIdx.x % blocks) * 256;   // the longest first
   const int own = KEYS ? x.n : x.rows;
-  if (part >= (KEYS ? rparts : kparts) || at0 >= own || x.rows == 0 || x.n == 0) return;
+  if (part >= (KEYS ? rparts : kparts) || at0 >= own || x.rows == 0 || x.n == 0) {
+    mb::pdl_wait();                                       // a grid ends behind the one in front of it, even where it does nothing
+    return;
+  }
   const bool two = own - at0 > 128;
   int begin, end;
   if constexpr (KEYS) {
@@ -138,85 +165,59 @@ __global__ void __launch_bounds__(kThreads, 1) observe_kernel(const MbMassArgs a
   }
   const int tiles = end > begin ? (end - begin + kN - 1) / kN : 0;
   const size_t row0 = ((size_t)s * a.Hkv + h) * ws.rows;     // of the workspace's rows
-  float2* ml = reinterpret_cast<float2*>(a.ws) + row0 * ws.key_parts;
-  __half* wq = reinterpret_cast<__half*>(reinterpret_cast<uint8_t*>(a.ws) + ws.q) + row0 * D;
+  float2* ml = reinterpret_cast<float2*>(reinterpret_cast<uint8_t*>(a.ws) + ws.ml) + row0 * ws.key_parts;
+  uint4* wq = reinterpret_cast<uint4*>(a.ws) + row0 * (D / 8);
   float* wscale = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(a.ws) + ws.scale) + row0;
 
   if (tid == 0) {
-    mb::mbar_init(&held_full, kSums / 32);
+    mb::mbar_init(&held_full, KEYS ? 1 : kSums / 32);
     for (int i = 0; i < kStages; ++i) {
-      mb::mbar_init(&full[i], 4);
+      mb::mbar_init(&full[i], 1);
       mb::mbar_init(&empty[i], 1);
     }
-    for (int i = 0; i < kInfo; ++i) mb::mbar_init(&info_full[i], 4);
+    for (int i = 0; i < kInfo; ++i) {
+      mb::mbar_init(&info_full[i], 4);
+      mb::mbar_init(&info_free[i], two ? 16 : 8);
+    }
     for (int i = 0; i < 4; ++i) {
       mb::mbar_init(&s_full[i >> 1][i & 1], 1);
       mb::mbar_init(&s_free[i >> 1][i & 1], 8);
     }
     mb::mbar_fence_init();
+    mb::tma_prefetch_desc(&tmK);
+    if (KEYS) mb::tma_prefetch_desc(&tmQ);
   }
   if (warp == 20) mb::tmem_alloc(&s_tmem, C::kCols);
   mb::tc_fence_before();
   __syncthreads();
   mb::tc_fence_after();
   const uint32_t tmem = s_tmem;
-
-  // ---- where rows of either operand come from
-  const int* table = a.block_table + s * a.table_ld;
-  const int shift = (a.block_size & (a.block_size - 1)) == 0 ? 31 - __clz(a.block_size) : -1;
-  int bad = 0;
-  auto block_of = [&](int j) { return shift >= 0 ? j >> shift : j / a.block_size; };
-  constexpr int kRowB = D * (FP8 ? 1 : 2);
-  const uint8_t* keys = reinterpret_cast<const uint8_t*>(a.k_cache) + (size_t)h * kRowB;
-  const int pitch = a.Hkv * kRowB;
-  auto key_at = [&](int j, int b) {                          // cached row j < n, which is in block b
-    const bool out = (unsigned)b >= (unsigned)a.num_blocks;
-    bad |= out;
-    const int slot = (out ? 0 : b) * a.block_size + (j - block_of(j) * a.block_size);
-    return keys + (long long)slot * pitch;
-  };
-  auto query_at = [&](int r) -> const __nv_bfloat16* {
-    const int tq = tok_of(r);
-    return reinterpret_cast<const __nv_bfloat16*>(a.q) + ((size_t)(x.tok0 + tq) * a.Hq + h * G + (r - tq * G)) * D;
-  };
+  mb::pdl_launch_dependents();                            // a dependent kernel allocates TMEM: not before this CTA has its own
+  mb::pdl_wait();
   // of a row's scores, in the log2 domain; never 0, which would make numbers of the -inf that a mask leaves
   auto factor = [&](float row) { return fmaxf(a.scale * (FP8 ? *a.k_scale : 1.f) * 1.44269504088896f * row, 1.17549435e-38f); };
-  // 16 e4m3 values as the two 16-byte pieces of f16 that they are
-  auto widen = [](const uint4& raw, uint4& lo, uint4& hi) {
-    lo = make_uint4(e4m3x2(raw.x), e4m3x2(raw.x >> 16), e4m3x2(raw.y), e4m3x2(raw.y >> 16));
-    hi = make_uint4(e4m3x2(raw.z), e4m3x2(raw.z >> 16), e4m3x2(raw.w), e4m3x2(raw.w >> 16));
-  };
 
   if (warp < 16) {
     more_regs<88>();
     const int w = warp >> 3, half = warp >> 2 & 1, r = tid & 127, mine = at0 + w * 128 + r;
     constexpr int kW = kN / 2;                               // columns of a thread
-    // ---- the operand that stays: 256 rows, rows behind the last one are zeros
-    constexpr int kPieces = KEYS && FP8 ? D / 16 : D / 8, kStep = kSums / kPieces, kLoads = 256 / kStep;
-    const int c = tid % kPieces;
+    if constexpr (!KEYS) {
+      // ---- the query rows, which stay: 256 of them, rows behind the last one are zeros. The first part's CTA leaves them for the keys pass.
+      constexpr int kPieces = D / 8, kStep = kSums / kPieces, kLoads = 256 / kStep;
+      const int c = tid % kPieces;
 #pragma unroll 1
-    for (int i0 = 0; i0 < kLoads; i0 += 8) {
-      constexpr int kBatch = kLoads < 8 ? kLoads : 8;
-      uint4 v[kBatch];
+      for (int i0 = 0; i0 < kLoads; i0 += 8) {
+        constexpr int kBatch = kLoads < 8 ? kLoads : 8;
+        uint4 v[kBatch];
 #pragma unroll
-      for (int i = 0; i < kBatch; ++i) {
-        const int hr = tid / kPieces + kStep * (i0 + i), at = min(at0 + hr, own - 1);
-        if constexpr (KEYS)
-          v[i] = __ldg(reinterpret_cast<const uint4*>(key_at(at, __ldg(table + block_of(at)))) + c);
-        else
-          v[i] = __ldg(reinterpret_cast<const uint4*>(query_at(at)) + c);
-        if (at0 + hr >= own) v[i] = make_uint4(0, 0, 0, 0);
-      }
+        for (int i = 0; i < kBatch; ++i) {
+          const int hr = tid / kPieces + kStep * (i0 + i), at = min(at0 + hr, own - 1), tq = tok_of(at);
+          v[i] = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(a.q) + ((size_t)(x.tok0 + tq) * a.Hq + h * G + (at - tq * G)) * D) + c);
+          if (at0 + hr >= own) v[i] = make_uint4(0, 0, 0, 0);
+        }
 #pragma unroll
-      for (int i = 0; i < kBatch; ++i) {
-        const int hr = tid / kPieces + kStep * (i0 + i);
-        uint8_t* dst = sHeld + (hr >> 7) * (128 * D * 2);
-        if constexpr (KEYS && FP8) {
-          uint4 lo, hi;
-          widen(v[i], lo, hi);
-          *reinterpret_cast<uint4*>(dst + (c >> 2) * (128 * 128) + sw_off(hr & 127, (c & 3) * 2)) = lo;
-          *reinterpret_cast<uint4*>(dst + (c >> 2) * (128 * 128) + sw_off(hr & 127, (c & 3) * 2 + 1)) = hi;
-        } else {
+        for (int i = 0; i < kBatch; ++i) {
+          const int hr = tid / kPieces + kStep * (i0 + i);
           if constexpr (FP8) {
             // f16 has less range than bf16: the power of two that takes the row's largest element to [2^14, 2^15); bits of a bf16 without its
             // sign order like the values
@@ -232,24 +233,24 @@ __global__ void __launch_bounds__(kThreads, 1) observe_kernel(const MbMassArgs a
             uint32_t z[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              const float2 t = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&y[j]));
-              z[j] = pack2<true>(t.x * f, t.y * f);
+              const float2 p = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&y[j]));
+              z[j] = pack2<true>(p.x * f, p.y * f);
             }
             v[i] = make_uint4(z[0], z[1], z[2], z[3]);
-            if (c == 0) s_row[hr] = __int_as_float((127 - up) << 23);
-            if (part == 0 && at0 + hr < own) {
-              reinterpret_cast<uint4*>(wq + (size_t)(at0 + hr) * D)[c] = v[i];
-              if (c == 0) wscale[at0 + hr] = __int_as_float((127 - up) << 23);
+            if (c == 0) {
+              s_row[hr] = __int_as_float((127 - up) << 23);
+              if (part == 0 && at0 + hr < own) wscale[at0 + hr] = __int_as_float((127 - up) << 23);
             }
           }
-          *reinterpret_cast<uint4*>(dst + (c >> 3) * (128 * 128) + sw_off(hr & 127, c & 7)) = v[i];
+          if (part == 0 && at0 + hr < own) wq[(size_t)(at0 + hr) * kPieces + c] = v[i];
+          *reinterpret_cast<uint4*>(sHeld + (hr >> 7) * (128 * D * 2) + (c >> 3) * (128 * 128) + sw_off(hr & 127, c & 7)) = v[i];
         }
       }
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) mb::mbar_arrive(&held_full);
+      if constexpr (FP8) asm volatile("bar.sync 1, 512;" ::: "memory");    // the rows' scales come from other warps
     }
-    fence_async_smem();
-    __syncwarp();
-    if (lane == 0) mb::mbar_arrive(&held_full);
-    if constexpr (FP8 && !KEYS) asm volatile("bar.sync 1, 512;" ::: "memory");       // the rows' scales come from other warps
     const float sc = factor(FP8 && !KEYS ? s_row[w * 128 + r] : 1.f);
     const int limit = KEYS ? 0 : mine < own ? limit_of(mine) : 0;
     const uint32_t tS = tmem + ((uint32_t)((warp & 3) * 32) << 16) + w * 2 * kN + half * kW;
@@ -293,11 +294,11 @@ __global__ void __launch_bounds__(kThreads, 1) observe_kernel(const MbMassArgs a
       float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
       if constexpr (KEYS) {
         const float4* info = &s_info[t % kInfo][half * kW / 2];
-        // these rows' first one sees the least: all of these keys, or a row each is asked
-        if (__any_sync(0xffffffffu, mine >= limit_of(from))) {
+        // these rows' first one sees the least: all of these keys, or a row each is asked. Behind the last row is whatever memory holds.
+        if (__any_sync(0xffffffffu, mine >= limit_of(from) || from + kW > end)) {
 #pragma unroll
           for (int i = 0; i < kW; ++i)
-            if (mine >= limit_of(from + i)) z[i] = -INFINITY;
+            if (mine >= limit_of(from + i) || from + i >= end) z[i] = -INFINITY;
         }
 #pragma unroll
         for (int i = 0; i < kW / 2; ++i) {
@@ -308,6 +309,8 @@ __global__ void __launch_bounds__(kThreads, 1) observe_kernel(const MbMassArgs a
           sum[i & 1] = add2(sum[i & 1], p);
         }
         l_run += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+        __syncwarp();
+        if (lane == 0) mb::mbar_arrive(&info_free[t % kInfo]);
       } else {
         const int seen = min(limit, end) - from;             // columns in front of this one are visible
         if (!__all_sync(0xffffffffu, seen >= kW)) {
@@ -362,52 +365,27 @@ __global__ void __launch_bounds__(kThreads, 1) observe_kernel(const MbMassArgs a
     }
     mb::tc_fence_before();
   } else if (warp < 20) {
-    // ------------------------------------------------------------ what goes by
+    // ------------------------------------------------------------ keys pass: factors and normalisers of a tile's rows
     fewer_regs<72>();
-    const int t = tid - kSums;
-    constexpr bool kWiden = C::kWiden;
-    // 16-byte pieces of a chunk's row, rows between a thread's pieces, and how many it has
-    constexpr int kPieces = kWiden ? C::kDims / 16 : C::kDims / 8, kStep = 128 / kPieces, kLoads = kN / kStep;
-    // Chunks under way while the next is asked for. A chunk is announced when kAhead more have been asked for, which waits for the products of
-    // kStages - kAhead chunks before it: two, or the products would go one by one.
-    constexpr int kAhead = kWiden ? C::kRaw - 1 : kStages - 2;
-    const int r0 = t / kPieces, c = t % kPieces, chunks = tiles * kChunks;
-    bool ok = true;
-    auto announce = [&](int j) {                             // chunk j
-      fence_async_smem();
-      __syncwarp();
-      if (lane == 0) {
-        mb::mbar_arrive(&full[j % kStages]);
-        if (KEYS && j % kChunks == 0) mb::mbar_arrive(&info_full[j / kChunks % kInfo]);
-      }
-    };
-    // rows pass: the blocks of a tile's rows are looked up a tile before they are read, and not touched until then
-    int next[KEYS ? 1 : kLoads];
-    auto places = [&](int tile) {
-      if constexpr (!KEYS)
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i) next[i] = __ldg(table + block_of(min(begin + tile * kN + r0 + i * kStep, end - 1)));
-    };
-    // keys pass: so are the parts of a row's normaliser
-    constexpr int kTake = 4;
-    float2 y[KEYS ? kTake : 1];
-    float yscale = 1.f;
-    auto look = [&](int tile) {
-      if constexpr (KEYS) {
+    if constexpr (KEYS) {
+      const int t = tid - kSums;
+      // the parts of the next tile's normalisers are on their way while this one's are joined
+      constexpr int kTake = 4;
+      float2 y[kTake];
+      float yscale = 1.f;
+      auto look = [&](int tile) {
         const int at = min(begin + tile * kN + t, end - 1);
         if (t < kN) {
 #pragma unroll
           for (int k = 0; k < kTake; ++k) y[k] = k < kparts ? ml[(size_t)at * ws.key_parts + k] : make_float2(-INFINITY, 0.f);
           if (FP8) yscale = wscale[at];
         }
-      }
-    };
-    auto inform = [&](int tile) {
-      if constexpr (KEYS) {
-        // a row's normaliser from the parts of its keys, in order; rows behind the last one add nothing
+      };
+      if (tiles > 0) look(0);
+      for (int tile = 0; tile < tiles; ++tile) {
+        float f = 1.f, lse = INFINITY, m = -INFINITY, l = 0.f;           // rows behind the last one add nothing
+        const int at = begin + tile * kN + t;
         if (t < kN) {
-          const int at = begin + tile * kN + t;
-          float f = 1.f, lse = INFINITY, m = -INFINITY, l = 0.f;
           for (int i = 0; i < kparts; i += kTake) {
             if (i > 0) {
 #pragma unroll
@@ -424,78 +402,19 @@ __global__ void __launch_bounds__(kThreads, 1) observe_kernel(const MbMassArgs a
             f = factor(yscale);
             if (l != 0.f) lse = m + log2f(l);
           }
+        }
+        const bool ok = mb::mbar_wait(&info_free[tile % kInfo], ((tile / kInfo) & 1) ^ 1, a.status, MB_ST_TIMEOUT_EPI);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        if (t < kN) {
           float* info = reinterpret_cast<float*>(&s_info[tile % kInfo][t >> 1]) + (t & 1);
           info[0] = f;
           info[2] = -lse;
         }
-      }
-    };
-    auto ask = [&](int j) {                                  // chunk j into its stage, or an e4m3 cache's into the ring of bytes
-      const int tile = j / kChunks, q = j % kChunks;
-#pragma unroll
-      for (int i = 0; i < kLoads; ++i) {
-        const int r = r0 + i * kStep, at = begin + tile * kN + r, safe = min(at, end - 1);
-        const uint8_t* src;
-        if constexpr (!KEYS) src = key_at(safe, next[i]);
-        else if constexpr (FP8) src = reinterpret_cast<const uint8_t*>(wq + (size_t)safe * D);
-        else src = reinterpret_cast<const uint8_t*>(query_at(safe));
-        uint8_t* dst = kWiden ? sRaw + (j % 3) * C::kRawB + (i * 128 + t) * 16 : sRing + (j % kStages) * C::kChunkB + (c >> 3) * (kN * 128) + sw_off(r, c & 7);
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(mb::smem_u32(dst)), "l"(src + (q * kPieces + c) * 16), "r"(at < end ? 16 : 0) : "memory");
-      }
-      asm volatile("cp.async.commit_group;" ::: "memory");
-    };
-    auto wait_empty = [&](int j) {
-      ok = mb::mbar_wait(&empty[j % kStages], ((j / kStages) & 1) ^ 1, a.status, MB_ST_TIMEOUT_TMA);
-      return __all_sync(0xffffffffu, ok);
-    };
-    if (chunks > 0) {
-      places(0);
-      look(0);
-    }
-    if constexpr (kWiden) {
-      // a thread widens the bytes that it asked for itself
-      for (int j = 0; j < chunks + kAhead; ++j) {
-        if (j < chunks) {
-          ask(j);
-          if (j % kChunks == kChunks - 1) places(j / kChunks + 1);
-        } else {
-          asm volatile("cp.async.commit_group;" ::: "memory");
-        }
-        const int k = j - kAhead;
-        if (k < 0) continue;
-        asm volatile("cp.async.wait_group %0;" ::"n"(kAhead) : "memory");
-        if (!wait_empty(k)) break;
-        const uint8_t* raw = sRaw + (k % 3) * C::kRawB + t * 16;
-        uint8_t* chunk = sRing + (k % kStages) * C::kChunkB + (c >> 2) * (kN * 128);
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-          uint4 lo, hi;
-          widen(*reinterpret_cast<const uint4*>(raw + i * 128 * 16), lo, hi);
-          *reinterpret_cast<uint4*>(chunk + sw_off(r0 + i * kStep, (c & 3) * 2)) = lo;
-          *reinterpret_cast<uint4*>(chunk + sw_off(r0 + i * kStep, (c & 3) * 2 + 1)) = hi;
-        }
-        announce(k);
-      }
-    } else {
-      for (int j = 0; j < chunks; ++j) {
-        if (!wait_empty(j)) break;
-        ask(j);
-        if (KEYS && j % kChunks == 0) {
-          inform(j / kChunks);
-          look(j / kChunks + 1);
-        }
-        if (!KEYS && j % kChunks == kChunks - 1) places(j / kChunks + 1);
-        if (j >= kAhead) {
-          asm volatile("cp.async.wait_group %0;" ::"n"(kAhead) : "memory");
-          announce(j - kAhead);
-        }
-      }
-      if (__all_sync(0xffffffffu, ok)) {
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
-        for (int j = max(0, chunks - kAhead); j < chunks; ++j) announce(j);
+        __syncwarp();
+        if (lane == 0) mb::mbar_arrive(&info_full[tile % kInfo]);
+        if (tile + 1 < tiles) look(tile + 1);
       }
     }
-    asm volatile("cp.async.wait_all;" ::: "memory");
   } else {
     fewer_regs<56>();
     if (warp == 20 && mb::elect_one()) {
@@ -531,9 +450,64 @@ __global__ void __launch_bounds__(kThreads, 1) observe_kernel(const MbMassArgs a
       // nobody may free the accumulators under products in flight
       if (ok && chunks > 0) mb::mbar_wait(&empty[(chunks - 1) % kStages], ((chunks - 1) / kStages) & 1, a.status, MB_ST_TIMEOUT_MMA);
     }
+    if (warp == 21) {
+      // ---------------------------------------------------------- copies
+      const int* table = a.block_table + s * a.table_ld;
+      int bad = 0;
+      // where the box of 16 tokens from key j on begins; a box behind the context reads the null block, a block that the cache does not have block 0
+      auto box_at = [&](int j) {
+        if (j >= x.n) return 0;
+        const int bi = j / a.block_size, b = __ldg(table + bi);
+        const bool out = (unsigned)b >= (unsigned)a.num_blocks;
+        bad |= out;
+        return (out ? 0 : b) * a.block_size + (j - bi * a.block_size);
+      };
+      // kN keys from `from` on, dims [q kDims, ...) of them; lane l < kN / 16 holds the places of its boxes
+      auto keys = [&](uint8_t* dst, uint32_t span_bytes, uint64_t* bar, int dim, int spans, int from, int place) {
+        if (ws.paged) {
+#pragma unroll
+          for (int b = 0; b < kN / kBox; ++b) {
+            const int at = __shfl_sync(0xffffffffu, place, b);
+            if (lane == 0)
+              for (int hh = 0; hh < spans; ++hh) mb::tma_load_3d(dst + hh * span_bytes + b * (kBox * 128), &tmK, bar, dim + hh * 64, h, at);
+          }
+        } else if (lane == 0) {
+          for (int hh = 0; hh < spans; ++hh) mb::tma_load_3d(dst + hh * span_bytes, &tmK, bar, dim + hh * 64, h, (int)(s * ws.tokens) + from);
+        }
+      };
+      if constexpr (KEYS) {
+        if (lane == 0) mb::mbar_expect_tx(&held_full, C::kHeldB);
+        for (int b = 0; b < 256 / kN; ++b) {
+          const int from = at0 + b * kN;
+          keys(sHeld + (b * kN >> 7) * (128 * D * 2) + (b * kN & 127) * 128, 128 * 128, &held_full, 0, D / 64, from, ws.paged ? box_at(from + (lane & 7) * kBox) : 0);
+        }
+      }
+      const int chunks = tiles * kChunks;
+      int st = 0, turn = 1, place = 0;
+      if (!KEYS && ws.paged && chunks > 0) place = box_at(begin + (lane & 7) * kBox);
+      for (int j = 0; j < chunks; ++j) {
+        const int tile = j / kChunks, q = j % kChunks, from = begin + tile * kN;
+        if (!__all_sync(0xffffffffu, mb::mbar_wait(&empty[st], turn, a.status, MB_ST_TIMEOUT_TMA))) break;
+        if (lane == 0) mb::mbar_expect_tx(&full[st], C::kChunkB);
+        uint8_t* dst = sRing + st * C::kChunkB;
+        if constexpr (KEYS) {
+          if (lane == 0)
+            for (int hh = 0; hh < C::kSpans; ++hh) mb::tma_load_2d(dst + hh * (kN * 128), &tmQ, &full[st], q * C::kDims + hh * 64, (int)row0 + from);
+        } else {
+          keys(dst, kN * 128, &full[st], q * C::kDims, C::kSpans, from, place);
+          if (ws.paged && q == kChunks - 1) place = box_at(from + kN + (lane & 7) * kBox);
+        }
+        if (++st == kStages) {
+          st = 0;
+          turn ^= 1;
+        }
+      }
+      if (bad && a.status) atomicCAS(a.status, 0u, MB_ST_BOUNDS);
+      // copies in flight write shared memory: the CTA stays until the products have taken the last of them
+      if (KEYS && tiles == 0) mb::mbar_wait(&held_full, 0, a.status, MB_ST_TIMEOUT_TMA);
+    }
     __syncwarp();
   }
-  if (bad && a.status) atomicCAS(a.status, 0u, MB_ST_BOUNDS);
   __syncthreads();
   if (warp == 20) {
     mb::tc_fence_after();
@@ -555,11 +529,11 @@ __global__ void __launch_bounds__(256) observe_join_kernel(const MbMassArgs a, c
 }
 
 template <int D, bool FP8, bool KEYS>
-int launch(const MbMassArgs& a, const Ws& ws, cudaStream_t stream) {
+int launch(const MbMassArgs& a, const Ws& ws, const CUtensorMap* tm, cudaStream_t stream) {
   auto kern = observe_kernel<D, FP8, KEYS>;
   static bool configured = false;
   if (!configured) {
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D, FP8, KEYS>::kSmem);
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::kSmem);
     if (e != cudaSuccess) return (int)e;
     configured = true;
   }
@@ -567,20 +541,38 @@ int launch(const MbMassArgs& a, const Ws& ws, cudaStream_t stream) {
   const unsigned magic = G == 1 ? 0 : (unsigned)(((1ull << 32) + G - 1) / G);
   const long long blocks = ((KEYS ? (long long)a.max_ctx : ws.rows) + 255) / 256 * (KEYS ? ws.row_parts : ws.slices);
   if (blocks > 0x7fffffffll) return MB_ERR_TOO_LARGE;
-  return (int)mb::launch_kernel_ex(kern, dim3((unsigned)blocks, a.Hkv, a.num_seqs), dim3(kThreads), Cfg<D, FP8, KEYS>::kSmem, stream, 1, KEYS, a, ws, (int)magic);
+  return (int)mb::launch_kernel_ex(kern, dim3((unsigned)blocks, a.Hkv, a.num_seqs), dim3(kThreads), Cfg<D>::kSmem, stream, 1, KEYS || !ws.paged, tm[0], tm[1], a, ws,
+                                   (int)magic);
 }
 
 template <int D, bool FP8>
-int both(const MbMassArgs& a, const Ws& ws, cudaStream_t stream) {
-  const int rc = launch<D, FP8, false>(a, ws, stream);
-  return rc ? rc : launch<D, FP8, true>(a, ws, stream);
+int all(const MbMassArgs& a, const Ws& ws, cudaStream_t stream) {
+  uint8_t* p = reinterpret_cast<uint8_t*>(a.ws);
+  CUtensorMap tm[2];
+  const long long slots = ws.paged ? a.num_blocks * a.block_size : a.num_seqs * ws.tokens, rows = (long long)a.num_seqs * a.Hkv * ws.rows + 128;
+  if (slots >= (1ll << 31) || rows >= (1ll << 31)) return MB_ERR_TOO_LARGE;
+  int rc = mbh::encode_3d(&tm[0], CU_TENSOR_MAP_DATA_TYPE_UINT16, ws.paged ? a.k_cache : p + ws.keys, D, a.Hkv, slots, D * 2, (uint64_t)a.Hkv * D * 2, 64, 1,
+                          ws.paged ? kBox : Cfg<D>::kN);
+  if (rc) return rc;
+  rc = mbh::encode_2d(&tm[1], CU_TENSOR_MAP_DATA_TYPE_UINT16, p, D, rows, D * 2, 64, Cfg<D>::kN);
+  if (rc) return rc;
+  if (!ws.paged) {
+    const long long work = ((long long)a.max_ctx * a.Hkv * D / 16 + 255) / 256;
+    observe_copy_kernel<FP8><<<dim3((unsigned)(work < 2048 ? work : 2048), a.num_seqs), 256, 0, stream>>>(a, ws);
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return (int)e;
+  }
+  rc = launch<D, FP8, false>(a, ws, tm, stream);
+  return rc ? rc : launch<D, FP8, true>(a, ws, tm, stream);
 }
 
 }  // namespace
 
 extern "C" {
 
-size_t mb_prompt_mass_ws(int num_seqs, int Hq, int Hkv, int D, int seen, int max_ctx, int fp8) { return workspace(num_seqs, Hq, Hkv, D, seen, max_ctx, fp8 != 0).bytes; }
+size_t mb_prompt_mass_ws(int num_seqs, int Hq, int Hkv, int D, int block_size, int seen, int max_ctx, int fp8) {
+  return workspace(num_seqs, Hq, Hkv, D, block_size, seen, max_ctx, fp8 != 0).bytes;
+}
 
 int mb_prompt_mass(const MbMassArgs* a, cudaStream_t stream) {
   if (!a || a->num_seqs <= 0 || a->num_seqs > 65535 || a->Hkv <= 0 || a->Hkv > 65535 || a->Hq % a->Hkv || (a->D != 64 && a->D != 128 && a->D != 256) ||
@@ -590,12 +582,12 @@ int mb_prompt_mass(const MbMassArgs* a, cudaStream_t stream) {
   if ((reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->k_cache) | reinterpret_cast<uintptr_t>(a->ws)) & 15) return MB_ERR_UNSUPPORTED;
   if (a->num_blocks * a->block_size >= (1ll << 31)) return MB_ERR_TOO_LARGE;
   if ((long long)a->last * (a->Hq / a->Hkv) > (1ll << 25)) return MB_ERR_TOO_LARGE;     // rows that tok_of divides exactly
-  const Ws ws = workspace(a->num_seqs, a->Hq, a->Hkv, a->D, a->last, a->max_ctx, a->fp8 != 0);
+  const Ws ws = workspace(a->num_seqs, a->Hq, a->Hkv, a->D, a->block_size, a->last, a->max_ctx, a->fp8 != 0);
   if (!a->ws || a->ws_bytes < ws.bytes) return MB_ERR_TOO_LARGE;
   int rc;
-  if (a->D == 64) rc = a->fp8 ? both<64, true>(*a, ws, stream) : both<64, false>(*a, ws, stream);
-  else if (a->D == 128) rc = a->fp8 ? both<128, true>(*a, ws, stream) : both<128, false>(*a, ws, stream);
-  else rc = a->fp8 ? both<256, true>(*a, ws, stream) : both<256, false>(*a, ws, stream);
+  if (a->D == 64) rc = a->fp8 ? all<64, true>(*a, ws, stream) : all<64, false>(*a, ws, stream);
+  else if (a->D == 128) rc = a->fp8 ? all<128, true>(*a, ws, stream) : all<128, false>(*a, ws, stream);
+  else rc = a->fp8 ? all<256, true>(*a, ws, stream) : all<256, false>(*a, ws, stream);
   if (rc || ws.row_parts == 1) return rc;
   return (int)mb::launch_kernel_ex(observe_join_kernel, dim3((a->max_ctx + 255) / 256, a->Hkv, a->num_seqs), dim3(256), 0, stream, 1, true, *a, ws);
 }

@@ -203,7 +203,7 @@ def prompt_mass(q: torch.Tensor, k_cache: torch.Tensor, block_table: torch.Tenso
         return mass
     from . import _count, _stream, runtime
     seen, fp8 = min(last or max_q_len, max_q_len), int(k_cache.dtype == torch.uint8)
-    need = _workspace("mb_prompt_mass_ws", S, Hq, Hkv, D, seen, max_ctx, fp8)
+    need = _workspace("mb_prompt_mass_ws", S, Hq, Hkv, D, bs, seen, max_ctx, fp8)
     ws, rt = torch.empty(need, dtype=torch.uint8, device=q.device), runtime(q.device)
     a = _MassArgs(q.data_ptr(), k_cache.data_ptr(), None, block_table.data_ptr(), block_table.stride(0), q_start.data_ptr(), q_len.data_ptr(), ctx_len.data_ptr(),
                   mass.data_ptr(), mass.stride(0), mass.stride(1), None, ws.data_ptr(), need, None if k_scale is None else k_scale.data_ptr(), None, rt.status.data_ptr(),
