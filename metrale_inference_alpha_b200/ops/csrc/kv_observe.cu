@@ -95,28 +95,35 @@ inline Ws workspace(int seqs, int Hq, int Hkv, int D, int block_size, int seen, 
 template <bool FP8>
 __global__ void __launch_bounds__(256) observe_copy_kernel(const MbMassArgs a, const Ws ws) {
   mb::pdl_launch_dependents();
-  const int s = blockIdx.y, n = min(a.ctx_len[s], a.max_ctx), per = a.Hkv * a.D / 16;
+  const int s = blockIdx.y, n = min(a.ctx_len[s], a.max_ctx), per = a.Hkv * a.D / 16;        // of a cached token
   const int* table = a.block_table + s * a.table_ld;
   uint4* out = reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(a.ws) + ws.keys) + (size_t)s * ws.tokens * per * 2;
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < (long long)n * per; i += (long long)gridDim.x * 256) {
-    const int j = (int)(i / per), c = (int)(i - (long long)j * per);
-    const size_t at = (size_t)mbm::slot_of(table, j, a.block_size, a.num_blocks, a.status) * per + c;
-    if constexpr (FP8) {
-      const uint4 x = __ldg(reinterpret_cast<const uint4*>(a.k_cache) + at);
-      out[2 * i] = make_uint4(e4m3x2(x.x), e4m3x2(x.x >> 16), e4m3x2(x.y), e4m3x2(x.y >> 16));
-      out[2 * i + 1] = make_uint4(e4m3x2(x.z), e4m3x2(x.z >> 16), e4m3x2(x.w), e4m3x2(x.w >> 16));
-    } else {
-      out[2 * i] = __ldg(reinterpret_cast<const uint4*>(a.k_cache) + 2 * at);
-      out[2 * i + 1] = __ldg(reinterpret_cast<const uint4*>(a.k_cache) + 2 * at + 1);
+  // a CTA takes 8192 values at a time: whole tokens, or a part of one
+  const int tokens = max(1, 512 / per), parts = (per + 511) / 512;
+  for (int u = blockIdx.x; u < (n + tokens - 1) / tokens * parts; u += gridDim.x) {
+    const int j0 = u / parts * tokens, c0 = u % parts * 512;
+    for (int i = threadIdx.x; i < 512; i += 256) {
+      const int j = j0 + i / per, c = c0 + i % per;                       // a token that takes more than 512 has i / per = 0
+      if (j >= n || i / per >= tokens || c >= per) continue;
+      const size_t at = (size_t)mbm::slot_of(table, j, a.block_size, a.num_blocks, a.status) * per + c, to = (size_t)j * per + c;
+      if constexpr (FP8) {
+        const uint4 x = __ldg(reinterpret_cast<const uint4*>(a.k_cache) + at);
+        out[2 * to] = make_uint4(e4m3x2(x.x), e4m3x2(x.x >> 16), e4m3x2(x.y), e4m3x2(x.y >> 16));
+        out[2 * to + 1] = make_uint4(e4m3x2(x.z), e4m3x2(x.z >> 16), e4m3x2(x.w), e4m3x2(x.w >> 16));
+      } else {
+        out[2 * to] = __ldg(reinterpret_cast<const uint4*>(a.k_cache) + 2 * at);
+        out[2 * to + 1] = __ldg(reinterpret_cast<const uint4*>(a.k_cache) + 2 * at + 1);
+      }
     }
   }
 }
 
 template <int D>
 struct Cfg {
-  static constexpr int kN = D == 256 ? 64 : 128;             // rows of a tile that goes by
-  // A tile comes in chunks of up to 128 dims, which go round a ring of stages
-  static constexpr int kDims = D == 256 ? 128 : D, kChunks = D / kDims, kSpans = kDims / 64;   // of a chunk; spans of 128 bytes across it
+  static constexpr int kN = 128;                             // rows of a tile that goes by
+  // A tile comes in chunks, of 64 dims where 256 dims of what stays leave little room, which go round a ring of stages. (Tiles of 64 rows would take the
+  // products as long as tiles of 128: they are bound by reading the 128 held rows from shared memory.)
+  static constexpr int kDims = D == 256 ? 64 : D, kChunks = D / kDims, kSpans = kDims / 64;   // of a chunk; spans of 128 bytes across it
   static constexpr int kStages = D == 256 ? 5 : 4;
   static constexpr int kHeldB = 256 * D * 2, kChunkB = kN * kDims * 2;
   static constexpr int kSmem = kHeldB + kStages * kChunkB + 1024;
@@ -133,9 +140,12 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
   uint8_t* sRing = sHeld + C::kHeldB;                        // kStages x kSpans x [kN rows x 128 B]
   __shared__ __align__(8) uint64_t held_full, full[kStages], empty[kStages], info_full[kInfo], info_free[kInfo], s_full[2][2], s_free[2][2];
   __shared__ uint32_t s_tmem;
-  __shared__ float s_row[256];                               // rows pass, e4m3: what a row's scores are too large by
+  __shared__ float s_row[256];                               // rows pass, e4m3: the exponent of a row's largest element
   __shared__ float2 s_half[256];                             // sums of the second half of the columns
-  __shared__ __align__(16) float4 s_info[kInfo][kN / 2];     // keys pass: factors and normalisers of two query rows
+  __shared__ __align__(16) float s_lse[kInfo][kN];           // keys pass: the query rows' normalisers, negative, and their factors
+  __shared__ __align__(16) float s_factor[KEYS && FP8 ? kInfo : 1][kN];
+  __shared__ __align__(8) int s_alike[KEYS && FP8 ? kInfo : 1][4];         // 32 rows' factors are those of the first of 64
+  __shared__ int s_top[2];                                   // rows pass, e4m3: the largest exponent of a row's largest element, and the smallest
   const int h = blockIdx.y, s = blockIdx.z, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int G = a.Hq / a.Hkv;
   const Span x = span_of(a, s, G);
@@ -170,6 +180,8 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
   float* wscale = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(a.ws) + ws.scale) + row0;
 
   if (tid == 0) {
+    s_top[0] = 0;
+    s_top[1] = 255;
     mb::mbar_init(&held_full, KEYS ? 1 : kSums / 32);
     for (int i = 0; i < kStages; ++i) {
       mb::mbar_init(&full[i], 1);
@@ -192,44 +204,72 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
   __syncthreads();
   mb::tc_fence_after();
   const uint32_t tmem = s_tmem;
-  mb::pdl_launch_dependents();                            // a dependent kernel allocates TMEM: not before this CTA has its own
-  mb::pdl_wait();
+  // A dependent kernel allocates TMEM: not before this CTA has its own. What the kernel in front writes, only some warps read, and these wait for it: the
+  // copies of keys and query rows, the normalisers.
+  mb::pdl_launch_dependents();
   // of a row's scores, in the log2 domain; never 0, which would make numbers of the -inf that a mask leaves
   auto factor = [&](float row) { return fmaxf(a.scale * (FP8 ? *a.k_scale : 1.f) * 1.44269504088896f * row, 1.17549435e-38f); };
 
   if (warp < 16) {
-    more_regs<88>();
+    more_regs<96>();
     const int w = warp >> 3, half = warp >> 2 & 1, r = tid & 127, mine = at0 + w * 128 + r;
     constexpr int kW = kN / 2;                               // columns of a thread
+    float row_scale = 1.f;                                   // what this thread's row's scores are too large by
     if constexpr (!KEYS) {
       // ---- the query rows, which stay: 256 of them, rows behind the last one are zeros. The first part's CTA leaves them for the keys pass.
-      constexpr int kPieces = D / 8, kStep = kSums / kPieces, kLoads = 256 / kStep;
-      const int c = tid % kPieces;
-#pragma unroll 1
-      for (int i0 = 0; i0 < kLoads; i0 += 8) {
-        constexpr int kBatch = kLoads < 8 ? kLoads : 8;
-        uint4 v[kBatch];
+      constexpr int kPieces = D / 8, kStep = kSums / kPieces, kLoads = 256 / kStep, kBatch = kLoads < 8 ? kLoads : 8;
+      const int c = tid % kPieces, hr0 = tid / kPieces;
+      uint4 v[kBatch];
+      auto load = [&](int i0) {
 #pragma unroll
         for (int i = 0; i < kBatch; ++i) {
-          const int hr = tid / kPieces + kStep * (i0 + i), at = min(at0 + hr, own - 1), tq = tok_of(at);
+          const int hr = hr0 + kStep * (i0 + i), at = min(at0 + hr, own - 1), tq = tok_of(at);
           v[i] = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(a.q) + ((size_t)(x.tok0 + tq) * a.Hq + h * G + (at - tq * G)) * D) + c);
           if (at0 + hr >= own) v[i] = make_uint4(0, 0, 0, 0);
         }
+      };
+      int up = 0;
+      bool alike = true;
+      // f16 has less range than bf16: the power of two that takes a row's largest element to [2^14, 2^15). Zeros and subnormal rows as if their
+      // exponent were 15, infinities and NaN as they are.
+      auto lift = [](int e) { return e == 255 ? 0 : 141 - max(e, 15); };
+      if constexpr (FP8) {
+        // the exponent of a row's largest element; bits of a bf16 without its sign order like the values
+#pragma unroll 1
+        for (int i0 = 0; i0 < kLoads; i0 += kBatch) {
+          load(i0);
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-          const int hr = tid / kPieces + kStep * (i0 + i);
-          if constexpr (FP8) {
-            // f16 has less range than bf16: the power of two that takes the row's largest element to [2^14, 2^15); bits of a bf16 without its
-            // sign order like the values
-            const uint32_t y[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-            uint32_t top = 0;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) top = __vmaxu2(top, y[j] & 0x7fff7fffu);
+          for (int i = 0; i < kBatch; ++i) {
+            uint32_t top = __vmaxu2(__vmaxu2(v[i].x & 0x7fff7fffu, v[i].y & 0x7fff7fffu), __vmaxu2(v[i].z & 0x7fff7fffu, v[i].w & 0x7fff7fffu));
 #pragma unroll
             for (int d = 1; d < kPieces; d <<= 1) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, d));
             const int e = (int)(max(top & 0xffff, top >> 16) >> 7);
-            const int up = e == 255 ? 0 : 141 - max(e, 15);  // zeros and subnormal rows as if their exponent were 15, infinities and NaN as they are
-            const float f = __int_as_float((127 + up) << 23);
+            if (c == 0) {
+              s_row[hr0 + kStep * (i0 + i)] = __int_as_float(e);
+              if (e > 0) {
+                atomicMax(&s_top[0], e);
+                atomicMin(&s_top[1], e);
+              }
+            }
+          }
+        }
+        asm volatile("bar.sync 1, 512;" ::: "memory");
+        // Rows whose largest elements are within 2^12 of each other take the power of the largest, so that their scores have one factor: the smallest then
+        // still keeps 8 bits of elements down to 2^-19 of its largest, and the rest to 2^-27 of it.
+        const int hi = s_top[0], lo = s_top[1];
+        alike = hi < 255 && hi - lo <= 12;
+        up = lift(hi);
+      }
+#pragma unroll 1
+      for (int i0 = 0; i0 < kLoads; i0 += kBatch) {
+        if (!FP8 || kLoads > kBatch) load(i0);
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+          const int hr = hr0 + kStep * (i0 + i);
+          if constexpr (FP8) {
+            const int mine_up = alike ? up : lift(__float_as_int(s_row[hr]));
+            const float f = __int_as_float((127 + mine_up) << 23);
+            const uint32_t y[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
             uint32_t z[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -237,10 +277,7 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
               z[j] = pack2<true>(p.x * f, p.y * f);
             }
             v[i] = make_uint4(z[0], z[1], z[2], z[3]);
-            if (c == 0) {
-              s_row[hr] = __int_as_float((127 - up) << 23);
-              if (part == 0 && at0 + hr < own) wscale[at0 + hr] = __int_as_float((127 - up) << 23);
-            }
+            if (c == 0 && part == 0 && at0 + hr < own) wscale[at0 + hr] = __int_as_float((127 - mine_up) << 23);
           }
           if (part == 0 && at0 + hr < own) wq[(size_t)(at0 + hr) * kPieces + c] = v[i];
           *reinterpret_cast<uint4*>(sHeld + (hr >> 7) * (128 * D * 2) + (c >> 3) * (128 * 128) + sw_off(hr & 127, c & 7)) = v[i];
@@ -249,9 +286,9 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
       fence_async_smem();
       __syncwarp();
       if (lane == 0) mb::mbar_arrive(&held_full);
-      if constexpr (FP8) asm volatile("bar.sync 1, 512;" ::: "memory");    // the rows' scales come from other warps
+      if constexpr (FP8) row_scale = __int_as_float((127 - (alike ? up : lift(__float_as_int(s_row[w * 128 + r])))) << 23);
     }
-    const float sc = factor(FP8 && !KEYS ? s_row[w * 128 + r] : 1.f);
+    const float sc = factor(row_scale);
     const int limit = KEYS ? 0 : mine < own ? limit_of(mine) : 0;
     const uint32_t tS = tmem + ((uint32_t)((warp & 3) * 32) << 16) + w * 2 * kN + half * kW;
     float m_run = -INFINITY, l_run = 0.f;                    // keys pass: l_run is the column's sum
@@ -293,20 +330,40 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
       const int from = begin + t * kN + half * kW;
       float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
       if constexpr (KEYS) {
-        const float4* info = &s_info[t % kInfo][half * kW / 2];
         // these rows' first one sees the least: all of these keys, or a row each is asked. Behind the last row is whatever memory holds.
         if (__any_sync(0xffffffffu, mine >= limit_of(from) || from + kW > end)) {
 #pragma unroll
           for (int i = 0; i < kW; ++i)
             if (mine >= limit_of(from + i) || from + i >= end) z[i] = -INFINITY;
         }
+        const float4* lse = reinterpret_cast<const float4*>(&s_lse[t % kInfo][half * kW]);
+        auto add = [&](auto factors) {
 #pragma unroll
-        for (int i = 0; i < kW / 2; ++i) {
-          const float4 f = info[i];
-          float2 p = fma2(make_float2(z[2 * i], z[2 * i + 1]), make_float2(f.x, f.y), make_float2(f.z, f.w));
-          p.x = ex2(p.x);
-          p.y = ex2(p.y);
-          sum[i & 1] = add2(sum[i & 1], p);
+          for (int i = 0; i < kW / 4; ++i) {
+            const float4 n4 = lse[i], f4 = factors(i);
+            float2 p = fma2(make_float2(z[4 * i], z[4 * i + 1]), make_float2(f4.x, f4.y), make_float2(n4.x, n4.y));
+            float2 q = fma2(make_float2(z[4 * i + 2], z[4 * i + 3]), make_float2(f4.z, f4.w), make_float2(n4.z, n4.w));
+            p.x = ex2(p.x);
+            p.y = ex2(p.y);
+            q.x = ex2(q.x);
+            q.y = ex2(q.y);
+            sum[0] = add2(sum[0], p);
+            sum[1] = add2(sum[1], q);
+          }
+        };
+        if constexpr (FP8) {
+          const float4* own4 = reinterpret_cast<const float4*>(&s_factor[t % kInfo][half * kW]);
+          const int2 alike = *reinterpret_cast<const int2*>(&s_alike[t % kInfo][half * 2]);
+          if (alike.x && alike.y) {
+            const float f = own4->x;
+            const float4 same = make_float4(f, f, f, f);
+            add([&](int) { return same; });
+          } else {
+            add([&](int i) { return own4[i]; });
+          }
+        } else {
+          const float4 same = make_float4(sc, sc, sc, sc);
+          add([&](int) { return same; });
         }
         l_run += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
         __syncwarp();
@@ -334,17 +391,19 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
         };
         // What a row is relative to need not be its maximum, as long as nothing overflows and something of it is near 1: the largest of its first tile
         // with a visible column stands until a tile's sum passes 2^60.
-        float tile = add();
-        if (__any_sync(0xffffffffu, m_run == -INFINITY || !(tile < 0x1p60f))) {
-          float mx = -INFINITY;
+        float tile;
+        for (int again = 0;; again = 1) {
+          tile = add();
+          const bool move = m_run == -INFINITY || !(tile < 0x1p60f);
+          if (again || !__any_sync(0xffffffffu, move)) break;
+          float mx4[4] = {z[0], z[1], z[2], z[3]};
 #pragma unroll
-          for (int i = 0; i < kW; ++i) mx = fmaxf(mx, z[i]);
-          mx *= sc;
-          if (mx > m_run && (m_run == -INFINITY || !(tile < 0x1p60f))) {
+          for (int i = 4; i < kW; ++i) mx4[i & 3] = fmaxf(mx4[i & 3], z[i]);
+          const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * sc;
+          if (move && mx > m_run) {
             l_run *= ex2(m_run - mx);
             m_run = mx;
           }
-          tile = add();
         }
         l_run += tile;
         if (begin + (t + 1) * kN == flush_at) flush();
@@ -366,9 +425,10 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
     mb::tc_fence_before();
   } else if (warp < 20) {
     // ------------------------------------------------------------ keys pass: factors and normalisers of a tile's rows
-    fewer_regs<72>();
+    fewer_regs<40>();
     if constexpr (KEYS) {
       const int t = tid - kSums;
+      mb::pdl_wait();
       // the parts of the next tile's normalisers are on their way while this one's are joined
       constexpr int kTake = 4;
       float2 y[kTake];
@@ -406,9 +466,13 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
         const bool ok = mb::mbar_wait(&info_free[tile % kInfo], ((tile / kInfo) & 1) ^ 1, a.status, MB_ST_TIMEOUT_EPI);
         if (!__all_sync(0xffffffffu, ok)) break;
         if (t < kN) {
-          float* info = reinterpret_cast<float*>(&s_info[tile % kInfo][t >> 1]) + (t & 1);
-          info[0] = f;
-          info[2] = -lse;
+          s_lse[tile % kInfo][t] = -lse;
+          if constexpr (FP8) s_factor[tile % kInfo][t] = f;
+        }
+        if constexpr (FP8) {
+          asm volatile("bar.sync 4, 128;" ::: "memory");
+          const bool alike = __all_sync(0xffffffffu, at >= end || f == s_factor[tile % kInfo][t & 64]);
+          if (lane == 0) s_alike[tile % kInfo][warp & 3] = alike;
         }
         __syncwarp();
         if (lane == 0) mb::mbar_arrive(&info_full[tile % kInfo]);
@@ -475,6 +539,7 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
           for (int hh = 0; hh < spans; ++hh) mb::tma_load_3d(dst + hh * span_bytes, &tmK, bar, dim + hh * 64, h, (int)(s * ws.tokens) + from);
         }
       };
+      if (!KEYS || !ws.paged) mb::pdl_wait();
       if constexpr (KEYS) {
         if (lane == 0) mb::mbar_expect_tx(&held_full, C::kHeldB);
         for (int b = 0; b < 256 / kN; ++b) {
@@ -482,6 +547,7 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
           keys(sHeld + (b * kN >> 7) * (128 * D * 2) + (b * kN & 127) * 128, 128 * 128, &held_full, 0, D / 64, from, ws.paged ? box_at(from + (lane & 7) * kBox) : 0);
         }
       }
+      if (KEYS && ws.paged) mb::pdl_wait();
       const int chunks = tiles * kChunks;
       int st = 0, turn = 1, place = 0;
       if (!KEYS && ws.paged && chunks > 0) place = box_at(begin + (lane & 7) * kBox);
@@ -557,8 +623,8 @@ int all(const MbMassArgs& a, const Ws& ws, cudaStream_t stream) {
   rc = mbh::encode_2d(&tm[1], CU_TENSOR_MAP_DATA_TYPE_UINT16, p, D, rows, D * 2, 64, Cfg<D>::kN);
   if (rc) return rc;
   if (!ws.paged) {
-    const long long work = ((long long)a.max_ctx * a.Hkv * D / 16 + 255) / 256;
-    observe_copy_kernel<FP8><<<dim3((unsigned)(work < 2048 ? work : 2048), a.num_seqs), 256, 0, stream>>>(a, ws);
+    const long long work = (long long)a.max_ctx * a.Hkv * D / 8192 + 1;
+    observe_copy_kernel<FP8><<<dim3((unsigned)(work < 4096 ? work : 4096), a.num_seqs), 256, 0, stream>>>(a, ws);
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return (int)e;
   }
