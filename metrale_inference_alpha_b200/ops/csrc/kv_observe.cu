@@ -2,8 +2,8 @@
 // causal logits of the group's queries. K is read, V is not; the prompt's outputs are the prefill kernels' business.
 //
 // The normaliser of a row is known when all of its keys are done, so the logits are computed twice:
-//   rows pass   256 query rows stay in shared memory, tiles of keys go by; a thread owns a row and keeps its maximum and sum
-//   keys pass   256 keys stay, tiles of query rows go by; a thread owns a key and adds up 2^(z - normaliser of the row)
+//   rows pass   128 query rows stay in shared memory, tiles of keys go by; a thread owns a row and keeps its maximum and sum
+//   keys pass   128 keys stay, tiles of query rows go by; a thread owns a key and adds up 2^(z - normaliser of the row)
 // Both are the same kernel with the operands exchanged: what a thread owns is a lane of the accumulator in tensor memory, so that neither pass
 // sums across lanes. Query rows of a kv head are numbered token * G + head of the group, as in attention_rows.cu.
 //
@@ -12,9 +12,10 @@
 // f16, scaled by a power of two per row). A first form had four warps gather and widen tiles on the way into shared memory, every CTA the same ones: that
 // took the issue slots of the exponentials, 4096 observers at 8192 e4m3 tokens 819 us.
 //
-// Roles (768 threads, one CTA per SM): of warps 0-15 every four own 128 lanes and half of a tile's columns, so that a scheduler has four of them to run
-// exponentials of; warps 16-19 bring the rows' normalisers (keys pass), warp 20 issues the products into two accumulators for either half of the lanes,
-// so that products run under the exponentials, warp 21 the copies.
+// Roles (384 threads, two CTAs per SM, so that one's beginning and end are under the other's exponentials): warps 0-3 and 4-7 own 128 lanes each and half
+// of a tile's columns; warps 8 and 9 bring the rows' normalisers (keys pass), warp 10 issues the products into two accumulators, so that products run
+// under the exponentials, warp 11 the copies. With 256 lanes a CTA and one of them per SM, 4096 observers at 8192 e4m3 tokens took 766 us, sixteen prompts
+// of 17 to 1151 tokens under 64 observers 55.
 //
 // Long rows and long columns are cut into parts, by rules on the sequence's own lengths alone, and joined in order: every output has one writer and
 // every sum one order.
@@ -27,7 +28,7 @@ namespace {
 
 using namespace mbr;
 
-constexpr int kThreads = 768, kSums = 512, kMaxKeyParts = 32, kMaxRowParts = 16, kInfo = 8, kBox = 16;
+constexpr int kThreads = 384, kSums = 256, kHeld = 128, kMaxKeyParts = 32, kMaxRowParts = 16, kInfo = 8, kBox = 16;
 template <int N>
 __device__ __forceinline__ void more_regs() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N>
@@ -121,27 +122,27 @@ __global__ void __launch_bounds__(256) observe_copy_kernel(const MbMassArgs a, c
 template <int D>
 struct Cfg {
   static constexpr int kN = 128;                             // rows of a tile that goes by
-  // A tile comes in chunks, of 64 dims where 256 dims of what stays leave little room, which go round a ring of stages. (Tiles of 64 rows would take the
-  // products as long as tiles of 128: they are bound by reading the 128 held rows from shared memory.)
-  static constexpr int kDims = D == 256 ? 64 : D, kChunks = D / kDims, kSpans = kDims / 64;   // of a chunk; spans of 128 bytes across it
-  static constexpr int kStages = D == 256 ? 5 : 4;
-  static constexpr int kHeldB = 256 * D * 2, kChunkB = kN * kDims * 2;
+  // A tile comes in chunks of 64 dims, a swizzled span of 128 bytes each, which go round a ring of stages. (Tiles of 64 rows would take the products as
+  // long as tiles of 128: they are bound by reading the 128 held rows from shared memory.)
+  static constexpr int kDims = 64, kChunks = D / kDims;
+  static constexpr int kStages = D == 256 ? 2 : 4;
+  static constexpr int kHeldB = kHeld * D * 2, kChunkB = kN * kDims * 2;
   static constexpr int kSmem = kHeldB + kStages * kChunkB + 1024;
-  static constexpr uint32_t kCols = 4 * kN;                  // two halves of the lanes, two accumulators each
+  static constexpr uint32_t kCols = 2 * kN;                  // two accumulators
 };
 
 template <int D, bool FP8, bool KEYS>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kThreads, 2)
 observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmQ, const MbMassArgs a, const Ws ws, int g_magic) {
   using C = Cfg<D>;
   constexpr int kN = C::kN, kStages = C::kStages, kChunks = C::kChunks;
   extern __shared__ __align__(16) uint8_t smem_raw[];
-  uint8_t* sHeld = smem_raw + ((1024u - (mb::smem_u32(smem_raw) & 1023u)) & 1023u);   // 2 x D / 64 spans x [128 rows x 128 B]
-  uint8_t* sRing = sHeld + C::kHeldB;                        // kStages x kSpans x [kN rows x 128 B]
-  __shared__ __align__(8) uint64_t held_full, full[kStages], empty[kStages], info_full[kInfo], info_free[kInfo], s_full[2][2], s_free[2][2];
+  uint8_t* sHeld = smem_raw + ((1024u - (mb::smem_u32(smem_raw) & 1023u)) & 1023u);   // D / 64 spans x [128 rows x 128 B]
+  uint8_t* sRing = sHeld + C::kHeldB;                        // kStages x [kN rows x 128 B]
+  __shared__ __align__(8) uint64_t held_full, full[kStages], empty[kStages], info_full[kInfo], info_free[kInfo], s_full[2], s_free[2];
   __shared__ uint32_t s_tmem;
-  __shared__ float s_row[256];                               // rows pass, e4m3: the exponent of a row's largest element
-  __shared__ float2 s_half[256];                             // sums of the second half of the columns
+  __shared__ float s_row[kHeld];                               // rows pass, e4m3: the exponent of a row's largest element
+  __shared__ float2 s_half[kHeld];                             // sums of the second half of the columns
   __shared__ __align__(16) float s_lse[kInfo][kN];           // keys pass: the query rows' normalisers, negative, and their factors
   __shared__ __align__(16) float s_factor[KEYS && FP8 ? kInfo : 1][kN];
   __shared__ __align__(8) int s_alike[KEYS && FP8 ? kInfo : 1][4];         // 32 rows' factors are those of the first of 64
@@ -156,13 +157,12 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
   // A column's parts are a CTA each. So are a row's where the call's longest portion has as many; shorter portions, whose rows have more of them, share
   // `slices` CTAs out.
   const int slices = KEYS ? ws.row_parts : ws.slices, blocks = gridDim.x / slices, share = KEYS ? 1 : (kparts + slices - 1) / slices;
-  const int part = blockIdx.x / blocks * share, at0 = (KEYS ? (int)blockIdx.x % blocks : blocks - 1 - (int)blockIdx.x % blocks) * 256;   // the longest first
+  const int part = blockIdx.x / blocks * share, at0 = (KEYS ? (int)blockIdx.x % blocks : blocks - 1 - (int)blockIdx.x % blocks) * kHeld;   // the longest first
   const int own = KEYS ? x.n : x.rows;
   if (part >= (KEYS ? rparts : kparts) || at0 >= own || x.rows == 0 || x.n == 0) {
     mb::pdl_wait();                                       // a grid ends behind the one in front of it, even where it does nothing
     return;
   }
-  const bool two = own - at0 > 128;
   int begin, end;
   if constexpr (KEYS) {
     // the first row that sees the first of these keys
@@ -171,7 +171,7 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
     end = min(x.rows, (part + 1) * rp);
   } else {
     begin = part * kp;
-    end = min(min(x.n, begin + share * kp), limit_of(min(x.rows, at0 + 256) - 1));
+    end = min(min(x.n, begin + share * kp), limit_of(min(x.rows, at0 + kHeld) - 1));
   }
   const int tiles = end > begin ? (end - begin + kN - 1) / kN : 0;
   const size_t row0 = ((size_t)s * a.Hkv + h) * ws.rows;     // of the workspace's rows
@@ -188,18 +188,18 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
       mb::mbar_init(&empty[i], 1);
     }
     for (int i = 0; i < kInfo; ++i) {
-      mb::mbar_init(&info_full[i], 4);
-      mb::mbar_init(&info_free[i], two ? 16 : 8);
+      mb::mbar_init(&info_full[i], 2);
+      mb::mbar_init(&info_free[i], kSums / 32);
     }
-    for (int i = 0; i < 4; ++i) {
-      mb::mbar_init(&s_full[i >> 1][i & 1], 1);
-      mb::mbar_init(&s_free[i >> 1][i & 1], 8);
+    for (int i = 0; i < 2; ++i) {
+      mb::mbar_init(&s_full[i], 1);
+      mb::mbar_init(&s_free[i], kSums / 32);
     }
     mb::mbar_fence_init();
     mb::tma_prefetch_desc(&tmK);
     if (KEYS) mb::tma_prefetch_desc(&tmQ);
   }
-  if (warp == 20) mb::tmem_alloc(&s_tmem, C::kCols);
+  if (warp == 10) mb::tmem_alloc(&s_tmem, C::kCols);
   mb::tc_fence_before();
   __syncthreads();
   mb::tc_fence_after();
@@ -210,14 +210,14 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
   // of a row's scores, in the log2 domain; never 0, which would make numbers of the -inf that a mask leaves
   auto factor = [&](float row) { return fmaxf(a.scale * (FP8 ? *a.k_scale : 1.f) * 1.44269504088896f * row, 1.17549435e-38f); };
 
-  if (warp < 16) {
-    more_regs<96>();
-    const int w = warp >> 3, half = warp >> 2 & 1, r = tid & 127, mine = at0 + w * 128 + r;
+  if (warp < 8) {
+    more_regs<88>();
+    const int half = warp >> 2, r = tid & 127, mine = at0 + r;
     constexpr int kW = kN / 2;                               // columns of a thread
     float row_scale = 1.f;                                   // what this thread's row's scores are too large by
     if constexpr (!KEYS) {
-      // ---- the query rows, which stay: 256 of them, rows behind the last one are zeros. The first part's CTA leaves them for the keys pass.
-      constexpr int kPieces = D / 8, kStep = kSums / kPieces, kLoads = 256 / kStep, kBatch = kLoads < 8 ? kLoads : 8;
+      // ---- the query rows, which stay: 128 of them, rows behind the last one are zeros. The first part's CTA leaves them for the keys pass.
+      constexpr int kPieces = D / 8, kStep = kSums / kPieces, kLoads = kHeld / kStep, kBatch = kLoads < 8 ? kLoads : 8;
       const int c = tid % kPieces, hr0 = tid / kPieces;
       uint4 v[kBatch];
       auto load = [&](int i0) {
@@ -253,7 +253,7 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
             }
           }
         }
-        asm volatile("bar.sync 1, 512;" ::: "memory");
+        asm volatile("bar.sync 1, 256;" ::: "memory");
         // Rows whose largest elements are within 2^12 of each other take the power of the largest, so that their scores have one factor: the smallest then
         // still keeps 8 bits of elements down to 2^-19 of its largest, and the rest to 2^-27 of it.
         const int hi = s_top[0], lo = s_top[1];
@@ -280,40 +280,39 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
             if (c == 0 && part == 0 && at0 + hr < own) wscale[at0 + hr] = __int_as_float((127 - mine_up) << 23);
           }
           if (part == 0 && at0 + hr < own) wq[(size_t)(at0 + hr) * kPieces + c] = v[i];
-          *reinterpret_cast<uint4*>(sHeld + (hr >> 7) * (128 * D * 2) + (c >> 3) * (128 * 128) + sw_off(hr & 127, c & 7)) = v[i];
+          *reinterpret_cast<uint4*>(sHeld + (c >> 3) * (kHeld * 128) + sw_off(hr, c & 7)) = v[i];
         }
       }
       fence_async_smem();
       __syncwarp();
       if (lane == 0) mb::mbar_arrive(&held_full);
-      if constexpr (FP8) row_scale = __int_as_float((127 - (alike ? up : lift(__float_as_int(s_row[w * 128 + r])))) << 23);
+      if constexpr (FP8) row_scale = __int_as_float((127 - (alike ? up : lift(__float_as_int(s_row[r])))) << 23);
     }
     const float sc = factor(row_scale);
     const int limit = KEYS ? 0 : mine < own ? limit_of(mine) : 0;
-    const uint32_t tS = tmem + ((uint32_t)((warp & 3) * 32) << 16) + w * 2 * kN + half * kW;
+    const uint32_t tS = tmem + ((uint32_t)((warp & 3) * 32) << 16) + half * kW;
     float m_run = -INFINITY, l_run = 0.f;                    // keys pass: l_run is the column's sum
     bool ok = true;
-    const int count = w == 0 || two ? tiles : 0;
     // rows pass: a part of a row's keys is done; the halves of the columns are joined
     int mine_part = part, flush_at = (part + 1) * kp;
     auto flush = [&] {
-      if (half) s_half[w * 128 + r] = make_float2(m_run, l_run);
-      asm volatile("bar.sync %0, 256;" ::"r"(2 + w) : "memory");
+      if (half) s_half[r] = make_float2(m_run, l_run);
+      asm volatile("bar.sync 1, 256;" ::: "memory");
       if (!half && mine < own) {
-        const float2 y = s_half[w * 128 + r];
+        const float2 y = s_half[r];
         const float top = fmaxf(m_run, y.x);
         const float l = (m_run == -INFINITY ? 0.f : l_run * ex2(m_run - top)) + (y.x == -INFINITY ? 0.f : y.y * ex2(y.x - top));
         ml[(size_t)mine * ws.key_parts + mine_part] = make_float2(top, l);
       }
-      asm volatile("bar.sync %0, 256;" ::"r"(2 + w) : "memory");
+      asm volatile("bar.sync 1, 256;" ::: "memory");
       m_run = -INFINITY;
       l_run = 0.f;
       ++mine_part;
       flush_at += kp;
     };
-    for (int t = 0; t < count; ++t) {
+    for (int t = 0; t < tiles; ++t) {
       const int b = t & 1;
-      ok = mb::mbar_wait(&s_full[w][b], (t >> 1) & 1, a.status, MB_ST_TIMEOUT_MMA);
+      ok = mb::mbar_wait(&s_full[b], (t >> 1) & 1, a.status, MB_ST_TIMEOUT_MMA);
       if (KEYS) ok = ok && mb::mbar_wait(&info_full[t % kInfo], (t / kInfo) & 1, a.status, MB_ST_TIMEOUT_TMA);
       if (!__all_sync(0xffffffffu, ok)) {
         ok = false;
@@ -326,7 +325,7 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
       mb::tmem_ld_wait(z);
       mb::tc_fence_before();
       __syncwarp();
-      if (lane == 0) mb::mbar_arrive(&s_free[w][b]);         // the accumulator is in registers
+      if (lane == 0) mb::mbar_arrive(&s_free[b]);         // the accumulator is in registers
       const int from = begin + t * kN + half * kW;
       float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
       if constexpr (KEYS) {
@@ -410,78 +409,82 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
       }
     }
     if constexpr (KEYS) {
-      if (half) s_half[w * 128 + r].y = l_run;
-      asm volatile("bar.sync 1, 512;" ::: "memory");
+      if (half) s_half[r].y = l_run;
+      asm volatile("bar.sync 1, 256;" ::: "memory");
       if (!half && mine < own) {
-        l_run += s_half[w * 128 + r].y;
+        l_run += s_half[r].y;
         if (ws.row_parts > 1)
           reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(a.ws) + ws.sums)[((size_t)part * a.num_seqs * a.Hkv + (size_t)s * a.Hkv + h) * ws.cols + mine] = l_run;
         else
           a.mass[s * a.mass_seq + h * a.mass_head + mine] += l_run;
       }
-    } else if (w == 0 || two) {
+    } else {
       while (mine_part < min(part + share, kparts)) flush();   // parts behind what these rows see are empty
     }
     mb::tc_fence_before();
-  } else if (warp < 20) {
-    // ------------------------------------------------------------ keys pass: factors and normalisers of a tile's rows
-    fewer_regs<40>();
-    if constexpr (KEYS) {
+  } else {
+    fewer_regs<64>();
+    if (KEYS && warp < 10) {
+      // ---------------------------------------------------------- factors and normalisers of a tile's rows, two a thread
       const int t = tid - kSums;
       mb::pdl_wait();
       // the parts of the next tile's normalisers are on their way while this one's are joined
       constexpr int kTake = 4;
-      float2 y[kTake];
-      float yscale = 1.f;
+      float2 y[2][kTake];
+      float yscale[2] = {1.f, 1.f};
       auto look = [&](int tile) {
-        const int at = min(begin + tile * kN + t, end - 1);
-        if (t < kN) {
 #pragma unroll
-          for (int k = 0; k < kTake; ++k) y[k] = k < kparts ? ml[(size_t)at * ws.key_parts + k] : make_float2(-INFINITY, 0.f);
-          if (FP8) yscale = wscale[at];
+        for (int e = 0; e < 2; ++e) {
+          const int at = min(begin + tile * kN + t + 64 * e, end - 1);
+#pragma unroll
+          for (int k = 0; k < kTake; ++k) y[e][k] = k < kparts ? ml[(size_t)at * ws.key_parts + k] : make_float2(-INFINITY, 0.f);
+          if (FP8) yscale[e] = wscale[at];
         }
       };
       if (tiles > 0) look(0);
       for (int tile = 0; tile < tiles; ++tile) {
-        float f = 1.f, lse = INFINITY, m = -INFINITY, l = 0.f;           // rows behind the last one add nothing
-        const int at = begin + tile * kN + t;
-        if (t < kN) {
+        const int slot = tile % kInfo;
+        float f[2], lse[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int at = begin + tile * kN + t + 64 * e;
+          float m = -INFINITY, l = 0.f;
           for (int i = 0; i < kparts; i += kTake) {
             if (i > 0) {
 #pragma unroll
-              for (int k = 0; k < kTake; ++k) y[k] = i + k < kparts ? ml[(size_t)min(at, end - 1) * ws.key_parts + i + k] : make_float2(-INFINITY, 0.f);
+              for (int k = 0; k < kTake; ++k) y[e][k] = i + k < kparts ? ml[(size_t)min(at, end - 1) * ws.key_parts + i + k] : make_float2(-INFINITY, 0.f);
             }
 #pragma unroll
             for (int k = 0; k < kTake; ++k) {
-              const float top = fmaxf(m, y[k].x);
-              l = (m == -INFINITY ? 0.f : l * ex2(m - top)) + (y[k].x == -INFINITY ? 0.f : y[k].y * ex2(y[k].x - top));
+              const float top = fmaxf(m, y[e][k].x);
+              l = (m == -INFINITY ? 0.f : l * ex2(m - top)) + (y[e][k].x == -INFINITY ? 0.f : y[e][k].y * ex2(y[e][k].x - top));
               m = top;
             }
           }
-          if (at < end) {
-            f = factor(yscale);
-            if (l != 0.f) lse = m + log2f(l);
-          }
+          f[e] = factor(yscale[e]);
+          lse[e] = at < end && l != 0.f ? m + log2f(l) : INFINITY;       // rows behind the last one and rows without weight add nothing
         }
-        const bool ok = mb::mbar_wait(&info_free[tile % kInfo], ((tile / kInfo) & 1) ^ 1, a.status, MB_ST_TIMEOUT_EPI);
+        const bool ok = mb::mbar_wait(&info_free[slot], ((tile / kInfo) & 1) ^ 1, a.status, MB_ST_TIMEOUT_EPI);
         if (!__all_sync(0xffffffffu, ok)) break;
-        if (t < kN) {
-          s_lse[tile % kInfo][t] = -lse;
-          if constexpr (FP8) s_factor[tile % kInfo][t] = f;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          s_lse[slot][t + 64 * e] = -lse[e];
+          if constexpr (FP8) s_factor[slot][t + 64 * e] = f[e];
         }
         if constexpr (FP8) {
-          asm volatile("bar.sync 4, 128;" ::: "memory");
-          const bool alike = __all_sync(0xffffffffu, at >= end || f == s_factor[tile % kInfo][t & 64]);
-          if (lane == 0) s_alike[tile % kInfo][warp & 3] = alike;
+          asm volatile("bar.sync 2, 64;" ::: "memory");
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const bool alike = __all_sync(0xffffffffu, f[e] == s_factor[slot][64 * e]);
+            if (lane == 0) s_alike[slot][2 * e + (warp & 1)] = alike;
+          }
         }
         __syncwarp();
-        if (lane == 0) mb::mbar_arrive(&info_full[tile % kInfo]);
+        if (lane == 0) mb::mbar_arrive(&info_full[slot]);
         if (tile + 1 < tiles) look(tile + 1);
       }
     }
-  } else {
-    fewer_regs<56>();
-    if (warp == 20 && mb::elect_one()) {
+    if (warp == 10 && mb::elect_one()) {
       // ---------------------------------------------------------- products
       constexpr uint32_t kF = FP8 ? 0 : 1, kId = mb::umma_idesc(kF, kF, 128, kN);
       // an address is the low bits of a descriptor, in units of 16 bytes
@@ -492,20 +495,14 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
       for (int j = 0; j < chunks && ok; ++j) {
         const int tile = j / kChunks, q = j % kChunks, b = tile & 1;
         ok = mb::mbar_wait(&full[st], turn, a.status, MB_ST_TIMEOUT_MMA);
-        const uint64_t dC = dR + (uint32_t)(st * (C::kChunkB >> 4)), dQ = dH + q * (C::kSpans * 128 * 128 >> 4);
-        for (int w = 0; w < (two ? 2 : 1) && ok; ++w) {
-          if (q == 0) ok = mb::mbar_wait(&s_free[w][b], ((tile >> 1) & 1) ^ 1, a.status, MB_ST_TIMEOUT_MMA);
-          if (!ok) break;
-          mb::tc_fence_after();
-          const uint64_t dA = dQ + (uint32_t)(w * (128 * D * 2 >> 4));
+        if (q == 0) ok = ok && mb::mbar_wait(&s_free[b], ((tile >> 1) & 1) ^ 1, a.status, MB_ST_TIMEOUT_MMA);
+        if (!ok) break;
+        mb::tc_fence_after();
+        const uint64_t dC = dR + (uint32_t)(st * (C::kChunkB >> 4)), dA = dH + (uint32_t)(q * (kHeld * 128 >> 4));
 #pragma unroll
-          for (int hh = 0; hh < C::kSpans; ++hh)
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              mb::umma_f16(tmem + (w * 2 + b) * kN, dA + (hh * (128 * 128) + k * 32 >> 4), dC + (hh * (kN * 128) + k * 32 >> 4), kId, (q | hh | k) != 0);
-          if (q == kChunks - 1) mb::tc_commit(&s_full[w][b]);
-        }
-        if (ok) mb::tc_commit(&empty[st]);
+        for (int k = 0; k < 4; ++k) mb::umma_f16(tmem + b * kN, dA + (k * 32 >> 4), dC + (k * 32 >> 4), kId, (q | k) != 0);
+        if (q == kChunks - 1) mb::tc_commit(&s_full[b]);
+        mb::tc_commit(&empty[st]);
         if (++st == kStages) {
           st = 0;
           turn ^= 1;
@@ -514,7 +511,7 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
       // nobody may free the accumulators under products in flight
       if (ok && chunks > 0) mb::mbar_wait(&empty[(chunks - 1) % kStages], ((chunks - 1) / kStages) & 1, a.status, MB_ST_TIMEOUT_MMA);
     }
-    if (warp == 21) {
+    if (warp == 11) {
       // ---------------------------------------------------------- copies
       const int* table = a.block_table + s * a.table_ld;
       int bad = 0;
@@ -526,26 +523,23 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
         bad |= out;
         return (out ? 0 : b) * a.block_size + (j - bi * a.block_size);
       };
-      // kN keys from `from` on, dims [q kDims, ...) of them; lane l < kN / 16 holds the places of its boxes
-      auto keys = [&](uint8_t* dst, uint32_t span_bytes, uint64_t* bar, int dim, int spans, int from, int place) {
+      // 64 dims of 128 keys from `from` on; lane l < 8 holds the places of their boxes
+      auto keys = [&](uint8_t* dst, uint64_t* bar, int dim, int from, int place) {
         if (ws.paged) {
 #pragma unroll
           for (int b = 0; b < kN / kBox; ++b) {
             const int at = __shfl_sync(0xffffffffu, place, b);
-            if (lane == 0)
-              for (int hh = 0; hh < spans; ++hh) mb::tma_load_3d(dst + hh * span_bytes + b * (kBox * 128), &tmK, bar, dim + hh * 64, h, at);
+            if (lane == 0) mb::tma_load_3d(dst + b * (kBox * 128), &tmK, bar, dim, h, at);
           }
         } else if (lane == 0) {
-          for (int hh = 0; hh < spans; ++hh) mb::tma_load_3d(dst + hh * span_bytes, &tmK, bar, dim + hh * 64, h, (int)(s * ws.tokens) + from);
+          mb::tma_load_3d(dst, &tmK, bar, dim, h, (int)(s * ws.tokens) + from);
         }
       };
       if (!KEYS || !ws.paged) mb::pdl_wait();
       if constexpr (KEYS) {
         if (lane == 0) mb::mbar_expect_tx(&held_full, C::kHeldB);
-        for (int b = 0; b < 256 / kN; ++b) {
-          const int from = at0 + b * kN;
-          keys(sHeld + (b * kN >> 7) * (128 * D * 2) + (b * kN & 127) * 128, 128 * 128, &held_full, 0, D / 64, from, ws.paged ? box_at(from + (lane & 7) * kBox) : 0);
-        }
+        const int place = ws.paged ? box_at(at0 + (lane & 7) * kBox) : 0;
+        for (int q = 0; q < kChunks; ++q) keys(sHeld + q * (kHeld * 128), &held_full, q * 64, at0, place);
       }
       if (KEYS && ws.paged) mb::pdl_wait();
       const int chunks = tiles * kChunks;
@@ -557,10 +551,9 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
         if (lane == 0) mb::mbar_expect_tx(&full[st], C::kChunkB);
         uint8_t* dst = sRing + st * C::kChunkB;
         if constexpr (KEYS) {
-          if (lane == 0)
-            for (int hh = 0; hh < C::kSpans; ++hh) mb::tma_load_2d(dst + hh * (kN * 128), &tmQ, &full[st], q * C::kDims + hh * 64, (int)row0 + from);
+          if (lane == 0) mb::tma_load_2d(dst, &tmQ, &full[st], q * 64, (int)row0 + from);
         } else {
-          keys(dst, kN * 128, &full[st], q * C::kDims, C::kSpans, from, place);
+          keys(dst, &full[st], q * 64, from, place);
           if (ws.paged && q == kChunks - 1) place = box_at(from + kN + (lane & 7) * kBox);
         }
         if (++st == kStages) {
@@ -575,7 +568,7 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
     __syncwarp();
   }
   __syncthreads();
-  if (warp == 20) {
+  if (warp == 10) {
     mb::tc_fence_after();
     mb::tmem_dealloc(tmem, C::kCols);
   }
@@ -605,7 +598,7 @@ int launch(const MbMassArgs& a, const Ws& ws, const CUtensorMap* tm, cudaStream_
   }
   const int G = a.Hq / a.Hkv;
   const unsigned magic = G == 1 ? 0 : (unsigned)(((1ull << 32) + G - 1) / G);
-  const long long blocks = ((KEYS ? (long long)a.max_ctx : ws.rows) + 255) / 256 * (KEYS ? ws.row_parts : ws.slices);
+  const long long blocks = ((KEYS ? (long long)a.max_ctx : ws.rows) + kHeld - 1) / kHeld * (KEYS ? ws.row_parts : ws.slices);
   if (blocks > 0x7fffffffll) return MB_ERR_TOO_LARGE;
   return (int)mb::launch_kernel_ex(kern, dim3((unsigned)blocks, a.Hkv, a.num_seqs), dim3(kThreads), Cfg<D>::kSmem, stream, 1, KEYS || !ws.paged, tm[0], tm[1], a, ws,
                                    (int)magic);
