@@ -72,13 +72,16 @@ struct Ws {
   int key_parts, row_parts, slices, paged;   // slices: CTAs that a block of rows is shared out over
   size_t keys, ml, scale, sums, bytes;
 };
+// From this many observed rows on, a bf16 cache's keys are copied too: every tile of them goes by often, and comes as one box instead of eight
+constexpr int kCopyRows = 1024;
+
 inline Ws workspace(int seqs, int Hq, int Hkv, int D, int block_size, int seen, int max_ctx, bool fp8) {
   Ws w;
   auto even = [](size_t x) { return (x + 127) & ~size_t(127); };
   w.rows = (long long)seen * (Hq / Hkv);
   w.cols = (max_ctx + 3) & ~3ll;
   w.tokens = (max_ctx + 255) & ~255ll;
-  w.paged = !fp8 && block_size % kBox == 0;
+  w.paged = !fp8 && block_size % kBox == 0 && w.rows < kCopyRows;
   // more parts than any sequence of the call has: fewer rows than the most may mean more of them
   w.key_parts = parts_of(max_ctx, 512) < kMaxKeyParts ? parts_of(max_ctx, 512) : kMaxKeyParts;
   w.row_parts = parts_of((int)w.rows, row_part((int)w.rows));
@@ -213,7 +216,7 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
   if (warp < 8) {
     more_regs<88>();
     const int half = warp >> 2, r = tid & 127, mine = at0 + r;
-    constexpr int kW = kN / 2;                               // columns of a thread
+    constexpr int kCols = kN / 2, kW = 32;                   // columns of a thread, and of a round
     float row_scale = 1.f;                                   // what this thread's row's scores are too large by
     if constexpr (!KEYS) {
       // ---- the query rows, which stay: 128 of them, rows behind the last one are zeros. The first part's CTA leaves them for the keys pass.
@@ -290,7 +293,7 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
     }
     const float sc = factor(row_scale);
     const int limit = KEYS ? 0 : mine < own ? limit_of(mine) : 0;
-    const uint32_t tS = tmem + ((uint32_t)((warp & 3) * 32) << 16) + half * kW;
+    const uint32_t tS = tmem + ((uint32_t)((warp & 3) * 32) << 16) + half * kCols;
     float m_run = -INFINITY, l_run = 0.f;                    // keys pass: l_run is the column's sum
     bool ok = true;
     // rows pass: a part of a row's keys is done; the halves of the columns are joined
@@ -319,94 +322,101 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
         break;
       }
       mb::tc_fence_after();
-      float z[kW];
-#pragma unroll
-      for (int i = 0; i < kW; i += 32) mb::tmem_ld32_async(tS + b * kN + i, z + i);
-      mb::tmem_ld_wait(z);
-      mb::tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mb::mbar_arrive(&s_free[b]);         // the accumulator is in registers
-      const int from = begin + t * kN + half * kW;
-      float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-      if constexpr (KEYS) {
-        // these rows' first one sees the least: all of these keys, or a row each is asked. Behind the last row is whatever memory holds.
-        if (__any_sync(0xffffffffu, mine >= limit_of(from) || from + kW > end)) {
-#pragma unroll
-          for (int i = 0; i < kW; ++i)
-            if (mine >= limit_of(from + i) || from + i >= end) z[i] = -INFINITY;
+      // 32 columns at a time: the code of a tile is half as long, which a short call waits for from L2
+#pragma unroll 1
+      for (int c0 = 0; c0 < kCols; c0 += kW) {
+        float z[kW];
+        mb::tmem_ld32_async(tS + b * kN + c0, z);
+        mb::tmem_ld_wait(z);
+        if (c0 + kW == kCols) {
+          mb::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mb::mbar_arrive(&s_free[b]);       // the accumulator is in registers
         }
-        const float4* lse = reinterpret_cast<const float4*>(&s_lse[t % kInfo][half * kW]);
-        auto add = [&](auto factors) {
+        const int from = begin + t * kN + half * kCols + c0;
+        float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        if constexpr (KEYS) {
+          // these rows' first one sees the least: all of these keys, or a row each is asked. Behind the last row is whatever memory holds.
+          if (__any_sync(0xffffffffu, mine >= limit_of(from) || from + kW > end)) {
 #pragma unroll
-          for (int i = 0; i < kW / 4; ++i) {
-            const float4 n4 = lse[i], f4 = factors(i);
-            float2 p = fma2(make_float2(z[4 * i], z[4 * i + 1]), make_float2(f4.x, f4.y), make_float2(n4.x, n4.y));
-            float2 q = fma2(make_float2(z[4 * i + 2], z[4 * i + 3]), make_float2(f4.z, f4.w), make_float2(n4.z, n4.w));
-            p.x = ex2(p.x);
-            p.y = ex2(p.y);
-            q.x = ex2(q.x);
-            q.y = ex2(q.y);
-            sum[0] = add2(sum[0], p);
-            sum[1] = add2(sum[1], q);
+            for (int i = 0; i < kW; ++i)
+              if (mine >= limit_of(from + i) || from + i >= end) z[i] = -INFINITY;
           }
-        };
-        if constexpr (FP8) {
-          const float4* own4 = reinterpret_cast<const float4*>(&s_factor[t % kInfo][half * kW]);
-          const int2 alike = *reinterpret_cast<const int2*>(&s_alike[t % kInfo][half * 2]);
-          if (alike.x && alike.y) {
-            const float f = own4->x;
-            const float4 same = make_float4(f, f, f, f);
-            add([&](int) { return same; });
+          const float4* lse = reinterpret_cast<const float4*>(&s_lse[t % kInfo][half * kCols + c0]);
+          auto add = [&](auto factors) {
+#pragma unroll
+            for (int i = 0; i < kW / 4; ++i) {
+              const float4 n4 = lse[i], f4 = factors(i);
+              float2 p = fma2(make_float2(z[4 * i], z[4 * i + 1]), make_float2(f4.x, f4.y), make_float2(n4.x, n4.y));
+              float2 q = fma2(make_float2(z[4 * i + 2], z[4 * i + 3]), make_float2(f4.z, f4.w), make_float2(n4.z, n4.w));
+              p.x = ex2(p.x);
+              p.y = ex2(p.y);
+              q.x = ex2(q.x);
+              q.y = ex2(q.y);
+              sum[0] = add2(sum[0], p);
+              sum[1] = add2(sum[1], q);
+            }
+          };
+          if constexpr (FP8) {
+            const float4* own4 = reinterpret_cast<const float4*>(&s_factor[t % kInfo][half * kCols + c0]);
+            const int2 alike = *reinterpret_cast<const int2*>(&s_alike[t % kInfo][half * 2]);
+            if (alike.x && alike.y) {
+              const float f = own4->x;
+              const float4 same = make_float4(f, f, f, f);
+              add([&](int) { return same; });
+            } else {
+              add([&](int i) { return own4[i]; });
+            }
           } else {
-            add([&](int i) { return own4[i]; });
+            const float4 same = make_float4(sc, sc, sc, sc);
+            add([&](int) { return same; });
+          }
+          l_run += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+          if (c0 + kW == kCols) {
+            __syncwarp();
+            if (lane == 0) mb::mbar_arrive(&info_free[t % kInfo]);
           }
         } else {
-          const float4 same = make_float4(sc, sc, sc, sc);
-          add([&](int) { return same; });
-        }
-        l_run += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-        __syncwarp();
-        if (lane == 0) mb::mbar_arrive(&info_free[t % kInfo]);
-      } else {
-        const int seen = min(limit, end) - from;             // columns in front of this one are visible
-        if (!__all_sync(0xffffffffu, seen >= kW)) {
+          const int seen = min(limit, end) - from;             // columns in front of this one are visible
+          if (!__all_sync(0xffffffffu, seen >= kW)) {
 #pragma unroll
-          for (int i = 0; i < kW; ++i)
-            if (i >= seen) z[i] = -INFINITY;
-        }
-        const float2 sc2 = make_float2(sc, sc);
-        auto add = [&] {
-          const float nm = m_run == -INFINITY ? 0.f : -m_run;
-          const float2 nm2 = make_float2(nm, nm);
-          sum[0] = sum[1] = make_float2(0.f, 0.f);
-#pragma unroll
-          for (int i = 0; i < kW / 2; ++i) {
-            float2 p = fma2(make_float2(z[2 * i], z[2 * i + 1]), sc2, nm2);
-            p.x = ex2(p.x);
-            p.y = ex2(p.y);
-            sum[i & 1] = add2(sum[i & 1], p);
+            for (int i = 0; i < kW; ++i)
+              if (i >= seen) z[i] = -INFINITY;
           }
-          return (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-        };
-        // What a row is relative to need not be its maximum, as long as nothing overflows and something of it is near 1: the largest of its first tile
-        // with a visible column stands until a tile's sum passes 2^60.
-        float tile;
-        for (int again = 0;; again = 1) {
-          tile = add();
-          const bool move = m_run == -INFINITY || !(tile < 0x1p60f);
-          if (again || !__any_sync(0xffffffffu, move)) break;
-          float mx4[4] = {z[0], z[1], z[2], z[3]};
+          const float2 sc2 = make_float2(sc, sc);
+          auto add = [&] {
+            const float nm = m_run == -INFINITY ? 0.f : -m_run;
+            const float2 nm2 = make_float2(nm, nm);
+            sum[0] = sum[1] = make_float2(0.f, 0.f);
 #pragma unroll
-          for (int i = 4; i < kW; ++i) mx4[i & 3] = fmaxf(mx4[i & 3], z[i]);
-          const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * sc;
-          if (move && mx > m_run) {
-            l_run *= ex2(m_run - mx);
-            m_run = mx;
+            for (int i = 0; i < kW / 2; ++i) {
+              float2 p = fma2(make_float2(z[2 * i], z[2 * i + 1]), sc2, nm2);
+              p.x = ex2(p.x);
+              p.y = ex2(p.y);
+              sum[i & 1] = add2(sum[i & 1], p);
+            }
+            return (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+          };
+          // What a row is relative to need not be its maximum, as long as nothing overflows and something of it is near 1: the largest of its first tile
+          // with a visible column stands until a tile's sum passes 2^60.
+          float tile;
+          for (int again = 0;; again = 1) {
+            tile = add();
+            const bool move = m_run == -INFINITY || !(tile < 0x1p60f);
+            if (again || !__any_sync(0xffffffffu, move)) break;
+            float mx4[4] = {z[0], z[1], z[2], z[3]};
+#pragma unroll
+            for (int i = 4; i < kW; ++i) mx4[i & 3] = fmaxf(mx4[i & 3], z[i]);
+            const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * sc;
+            if (move && mx > m_run) {
+              l_run *= ex2(m_run - mx);
+              m_run = mx;
+            }
           }
+          l_run += tile;
         }
-        l_run += tile;
-        if (begin + (t + 1) * kN == flush_at) flush();
       }
+      if (!KEYS && begin + (t + 1) * kN == flush_at) flush();
     }
     if constexpr (KEYS) {
       if (half) s_half[r].y = l_run;
@@ -526,11 +536,7 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
       // 64 dims of 128 keys from `from` on; lane l < 8 holds the places of their boxes
       auto keys = [&](uint8_t* dst, uint64_t* bar, int dim, int from, int place) {
         if (ws.paged) {
-#pragma unroll
-          for (int b = 0; b < kN / kBox; ++b) {
-            const int at = __shfl_sync(0xffffffffu, place, b);
-            if (lane == 0) mb::tma_load_3d(dst + b * (kBox * 128), &tmK, bar, dim, h, at);
-          }
+          if (lane < kN / kBox) mb::tma_load_3d(dst + lane * (kBox * 128), &tmK, bar, dim, h, place);
         } else if (lane == 0) {
           mb::tma_load_3d(dst, &tmK, bar, dim, h, (int)(s * ws.tokens) + from);
         }
@@ -538,6 +544,7 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
       if (!KEYS || !ws.paged) mb::pdl_wait();
       if constexpr (KEYS) {
         if (lane == 0) mb::mbar_expect_tx(&held_full, C::kHeldB);
+        __syncwarp();
         const int place = ws.paged ? box_at(at0 + (lane & 7) * kBox) : 0;
         for (int q = 0; q < kChunks; ++q) keys(sHeld + q * (kHeld * 128), &held_full, q * 64, at0, place);
       }
@@ -549,6 +556,7 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
         const int tile = j / kChunks, q = j % kChunks, from = begin + tile * kN;
         if (!__all_sync(0xffffffffu, mb::mbar_wait(&empty[st], turn, a.status, MB_ST_TIMEOUT_TMA))) break;
         if (lane == 0) mb::mbar_expect_tx(&full[st], C::kChunkB);
+        __syncwarp();
         uint8_t* dst = sRing + st * C::kChunkB;
         if constexpr (KEYS) {
           if (lane == 0) mb::tma_load_2d(dst, &tmQ, &full[st], q * 64, (int)row0 + from);
