@@ -93,6 +93,19 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+__device__ __forceinline__ uint64_t evict_first() {
+  uint64_t policy;
+  asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
+  return policy;
+}
+__device__ __forceinline__ void tma_load_3d_once(void* dst, const CUtensorMap* m, uint64_t* bar, int c0, int c1, int c2, uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
+      " [%0], [%1, {%3, %4, %5}], [%2], %6;" ::"r"(mb::smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(m)), "r"(mb::smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "l"(policy)
+      : "memory");
+}
+
 // NT: eights of query rows
 template <int D, bool FP8, int NT>
 struct DecodeCfg {
@@ -226,6 +239,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
     }
   };
   const uint32_t my = mb::smem_u32(smem) + warp * C::kSlot;
+  const uint64_t once = MASS ? evict_first() : 0;
   auto issue = [&](const Unit& x, int i, int slot) {         // whole warp; one lane issues
     const int place = x.blk * p.block_size + x.within;
     uint64_t* bar = &bars[slot * 4 + warp];
@@ -237,8 +251,14 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
       if (lane == 0) {
 #pragma unroll
         for (int h = 0; h < kSpans; ++h) {
-          mb::tma_load_3d(dst + (b * kSpans + h) * (kSlice * kSpanB), &tmK, bar, h * kSpanB, x.kvh, tok);
-          mb::tma_load_3d(dst + C::kHalf + (b * kSpans + h) * (kSlice * kSpanB), &tmV, bar, h * kSpanB, x.kvh, tok);
+          uint8_t *k = dst + (b * kSpans + h) * (kSlice * kSpanB), *v = k + C::kHalf;
+          if constexpr (MASS) {                              // L2 keeps the logits for the join rather than rows that are read once
+            tma_load_3d_once(k, &tmK, bar, h * kSpanB, x.kvh, tok, once);
+            tma_load_3d_once(v, &tmV, bar, h * kSpanB, x.kvh, tok, once);
+          } else {
+            mb::tma_load_3d(k, &tmK, bar, h * kSpanB, x.kvh, tok);
+            mb::tma_load_3d(v, &tmV, bar, h * kSpanB, x.kvh, tok);
+          }
         }
       }
     }

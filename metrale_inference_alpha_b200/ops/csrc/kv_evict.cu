@@ -2,7 +2,7 @@
 // largest mass (of equal ones the first), `keep` in all, in their order. Rows, mass and the list of them move together.
 //
 //   select  finds the mass of the last row that stays, digit by digit from the top (11, 11 and 10 bits of an order-preserving image, a histogram in
-//           shared memory each), then writes the list in order by counting ballots. A CTA holds its rows' mass in registers, 16 or 64 a thread, and
+//           shared memory each), then writes the list in order by counting ballots. A CTA holds its rows' mass in registers, up to 64 a thread, and
 //           up to eight CTAs of a cluster add up their histograms: mass is read once.
 //   move    copies the rows. A kept row's place is never behind it, so in place only a row's own round can be in its way: each round is read before
 //           any of it is written, and later rounds' rows lie behind everything that is written before them.
@@ -15,15 +15,21 @@ using mbm::context;
 
 // Flat slot of row j of a sequence, which a cache of the device's memory holds in 31 bits; a block that the cache does not have is reported and read as
 // block 0, or not written (-1).
+__device__ __forceinline__ int block_of(const MbEvictArgs& a, int j) {
+  return (int)((unsigned long long)(unsigned)j * a.block_magic >> a.block_shift);        // j / block_size for j < 2^30
+}
 template <bool WRITE = false>
-__device__ __forceinline__ int slot_in(const MbEvictArgs& a, const int* table, int j) {
-  const int bi = a.block_shift >= 0 ? j >> a.block_shift : j / a.block_size;
-  const int b = __ldg(table + bi);
+__device__ __forceinline__ int slot_of(const MbEvictArgs& a, int j, int b) {
+  const int bi = block_of(a, j);
   if ((unsigned)b >= (unsigned long long)a.num_blocks) {
     if (a.status) atomicCAS(a.status, 0u, MB_ST_BOUNDS);
     return WRITE ? -1 : j - bi * a.block_size;
   }
   return b * a.block_size + (j - bi * a.block_size);
+}
+template <bool WRITE = false>
+__device__ __forceinline__ int slot_in(const MbEvictArgs& a, const int* table, int j) {
+  return slot_of<WRITE>(a, j, __ldg(table + block_of(a, j)));
 }
 
 // Larger key, larger mass; a NaN is the least, and both zeros are one.
@@ -50,7 +56,7 @@ __device__ __forceinline__ int excl_scan(int v, int* warp_tot, int& total) {
   return __reduce_add_sync(0xffffffffu, lane < warp ? c : 0) + inc - v;
 }
 
-constexpr int kThreads = 512, kWarps = kThreads / 32, kPer = 16, kMaxPer = 64, kSegment = kThreads * kMaxPer, kMaxCluster = 8, kBins = 4 * kThreads;
+constexpr int kThreads = 512, kWarps = kThreads / 32, kMaxPer = 64, kSegment = kThreads * kMaxPer, kMaxCluster = 8, kBins = 4 * kThreads, kStaged = 2048;
 
 __device__ __forceinline__ int4 dsmem_ld_s4(const int* local, uint32_t rank) {
   int4 v;
@@ -73,10 +79,10 @@ __device__ __forceinline__ int inclusive(int v, int lane) {
 
 // A cluster of CTAs (often of one) a (sequence, kv head). CTA r has rows [r * 512 E, ...) of it, a warp 32 E of them, E at most PER.
 template <int PER>
-__global__ void __launch_bounds__(kThreads) evict_select_kernel(const MbEvictArgs a) {
+__global__ void __launch_bounds__(kThreads, PER <= 16 ? 2 : 1) evict_select_kernel(const MbEvictArgs a) {
   __shared__ __align__(16) int hist[3][kBins], s_total[4];
   __shared__ __align__(16) int4 s_bins[kThreads];
-  __shared__ int warp_tot[3][kWarps], s_gt[kWarps], s_eq[kWarps];
+  __shared__ int warp_tot[3][kWarps], s_gt[kWarps], s_eq[kWarps], s_block[kStaged];
   const int h = blockIdx.x, s = blockIdx.y, cluster = gridDim.z, rank = blockIdx.z, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   auto sync_all = [&] {
     if (cluster > 1) mb::cluster_sync_all();
@@ -90,6 +96,12 @@ __global__ void __launch_bounds__(kThreads) evict_select_kernel(const MbEvictArg
   float f[PER];
 #pragma unroll
   for (int e = 0; e < PER; ++e) f[e] = e < E && i0 + 32 * e < n ? x[i0 + 32 * e] : 0.f;
+  // the CTA's rows' blocks come along: looked up one by one behind the selection they were a third of the time
+  const int* table = a.block_table + s * a.table_ld;
+  const int row0 = rank * kThreads * E, block0 = block_of(a, row0), blocks = row0 < n ? block_of(a, min(n, row0 + kThreads * E) - 1) - block0 + 1 : 0;
+  const bool staged = blocks <= kStaged;
+  if (staged)
+    for (int i = tid; i < blocks; i += kThreads) s_block[i] = __ldg(table + block0 + i);
 #pragma unroll
   for (int i = 0; i < 3; ++i) *reinterpret_cast<int4*>(&hist[i][4 * tid]) = make_int4(0, 0, 0, 0);
   if (tid == 0 && rank == 0) {
@@ -116,11 +128,13 @@ __global__ void __launch_bounds__(kThreads) evict_select_kernel(const MbEvictArg
         int4 c = make_int4(0, 0, 0, 0);
         if (b >= 0) {
           if (cluster > 1) {
-            int4 y[kMaxCluster];
+            for (int r0 = 0; r0 < cluster; r0 += 4) {
+              int4 y[4];
 #pragma unroll
-            for (int r = 0; r < kMaxCluster; ++r) y[r] = r < cluster ? dsmem_ld_s4(&hist[d][b], r) : make_int4(0, 0, 0, 0);
+              for (int r = 0; r < 4; ++r) y[r] = r0 + r < cluster ? dsmem_ld_s4(&hist[d][b], r0 + r) : make_int4(0, 0, 0, 0);
 #pragma unroll
-            for (int r = 0; r < kMaxCluster; ++r) c = make_int4(c.x + y[r].x, c.y + y[r].y, c.z + y[r].z, c.w + y[r].w);
+              for (int r = 0; r < 4; ++r) c = make_int4(c.x + y[r].x, c.y + y[r].y, c.z + y[r].z, c.w + y[r].w);
+            }
           } else {
             c = *reinterpret_cast<const int4*>(&hist[d][b]);
           }
@@ -179,21 +193,15 @@ __global__ void __launch_bounds__(kThreads) evict_select_kernel(const MbEvictArg
       s_total[1] = eq_before + eq;
     }
     mb::cluster_sync_all();
-    int4 y[kMaxCluster];
-#pragma unroll
-    for (int r = 0; r < kMaxCluster; ++r) y[r] = r < rank ? dsmem_ld_s4(s_total, r) : make_int4(0, 0, 0, 0);
-#pragma unroll
-    for (int r = 0; r < kMaxCluster; ++r) {
-      gt_before += y[r].x;
-      eq_before += y[r].y;
-    }
+    const int4 y = lane < rank ? dsmem_ld_s4(s_total, lane) : make_int4(0, 0, 0, 0);       // a lane a CTA
+    gt_before += __reduce_add_sync(0xffffffffu, y.x);
+    eq_before += __reduce_add_sync(0xffffffffu, y.y);
     mb::cluster_sync_all();                                            // a CTA's shared memory outlives what others read of it
   }
   // every row's mass is in registers by now, in all CTAs: it may be written over
   float* y = a.mass_out + s * a.out_seq + h * a.out_head;
   int* kept = a.kept + ((size_t)s * a.Hkv + h) * a.keep;
   int* slots = a.slots + ((size_t)s * a.Hkv + h) * a.keep;
-  const int* table = a.block_table + s * a.table_ld;
   const uint32_t before = (1u << lane) - 1;
   int first = 0x7fffffff;
 #pragma unroll
@@ -207,7 +215,7 @@ __global__ void __launch_bounds__(kThreads) evict_select_kernel(const MbEvictArg
       const int to = gt_before + __popc(bg & before) + min(rank_eq, need);
       if (is_above || (is_equal && rank_eq < need)) {
         kept[to] = i;
-        slots[to] = slot_in(a, table, i);
+        slots[to] = staged ? slot_of(a, i, s_block[block_of(a, i) - block0]) : slot_in(a, table, i);
         y[to] = f[e];
       } else if (i < n) {
         first = min(first, i);
@@ -303,17 +311,17 @@ __global__ void __launch_bounds__(256) evict_copy_kernel(const MbEvictArgs a, in
   uint8_t* cache = reinterpret_cast<uint8_t*>(blockIdx.x & 1 ? a.v_cache : a.k_cache);
   const int* to = a.dst_table + s * a.dst_ld;
   const size_t pitch = (size_t)a.Hkv * a.row_bytes, col = (size_t)h * a.row_bytes + (threadIdx.x & ((1 << bits) - 1)) * 16;
+  int src[kDeep], dst[kDeep];
   uint4 v[kDeep];
-  int dst[kDeep];
 #pragma unroll
-  for (int k = 0; k < kDeep; ++k) {
-    const int r = r0 + k * step;
-    dst[k] = -1;
-    if (r < m) {
-      v[k] = *reinterpret_cast<const uint4*>(cache + slots[r] * pitch + col);
-      dst[k] = slot_in<true>(a, to, r);
-    }
-  }
+  for (int k = 0; k < kDeep; ++k) src[k] = r0 + k * step < m ? slots[r0 + k * step] : -1;
+#pragma unroll
+  for (int k = 0; k < kDeep; ++k) dst[k] = src[k] >= 0 ? __ldg(to + block_of(a, r0 + k * step)) : -1;
+#pragma unroll
+  for (int k = 0; k < kDeep; ++k)
+    if (src[k] >= 0) v[k] = *reinterpret_cast<const uint4*>(cache + src[k] * pitch + col);
+#pragma unroll
+  for (int k = 0; k < kDeep; ++k) dst[k] = src[k] >= 0 ? slot_of<true>(a, r0 + k * step, dst[k]) : -1;
 #pragma unroll
   for (int k = 0; k < kDeep; ++k)
     if (dst[k] >= 0) *reinterpret_cast<uint4*>(cache + dst[k] * pitch + col) = v[k];
@@ -364,14 +372,19 @@ extern "C" int mb_kv_evict(const MbEvictArgs* given, cudaStream_t stream) {
     return MB_ERR_BAD_ARG;
   if ((reinterpret_cast<uintptr_t>(a->k_cache) | reinterpret_cast<uintptr_t>(a->v_cache)) & 15) return MB_ERR_UNSUPPORTED;
   if (a->num_blocks * a->block_size >= (1ll << 31)) return MB_ERR_TOO_LARGE;
-  a->block_shift = (a->block_size & (a->block_size - 1)) == 0 ? 31 - __builtin_clz(a->block_size) : -1;
+  // ceil(2^k / d) with 2^(k - 30) >= d, so that the product is off by less than 1 / d below 2^30
+  int k = 30;
+  while (1ll << (k - 30) < a->block_size) ++k;
+  a->block_shift = k;
+  a->block_magic = (unsigned)(((1ull << k) + a->block_size - 1) / a->block_size);
   const long long heads = (long long)a->Hkv * a->num_seqs;
   cudaError_t e;
   if (a->max_ctx <= kSegment * kMaxCluster) {
-    // 16 rows a thread, in as many CTAs as the chip holds at once; where there are more, up to 64
+    // 16 rows a thread, in as many CTAs as the chip holds at once; where there are more, up to 64. Fewer take a kernel with less of its loops to pass.
     int cluster = 1;
-    while (cluster * kSegment < a->max_ctx || (cluster < kMaxCluster && cluster * kThreads * kPer < a->max_ctx && heads * cluster * 2 <= 2 * 148)) cluster *= 2;
-    auto kern = cluster * kThreads * kPer >= a->max_ctx ? evict_select_kernel<kPer> : evict_select_kernel<kMaxPer>;
+    while (cluster * kSegment < a->max_ctx || (cluster < kMaxCluster && cluster * kThreads * 16 < a->max_ctx && heads * cluster * 2 <= 2 * 148)) cluster *= 2;
+    const int per = (a->max_ctx + cluster * kThreads - 1) / (cluster * kThreads);
+    auto kern = per <= 1 ? evict_select_kernel<1> : per <= 4 ? evict_select_kernel<4> : per <= 16 ? evict_select_kernel<16> : evict_select_kernel<kMaxPer>;
     e = mb::launch_kernel_ex(kern, dim3(a->Hkv, a->num_seqs, cluster), dim3(kThreads), 0, stream, cluster, false, *a);
   } else {
     e = mb::launch_kernel_ex(evict_select_long_kernel, dim3(a->Hkv, a->num_seqs), dim3(1024), 0, stream, 1, false, *a);

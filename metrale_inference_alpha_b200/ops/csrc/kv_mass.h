@@ -49,6 +49,7 @@ struct MbEvictArgs {
   uint32_t* status;
   int* slots;                // [seqs, Hkv, keep]: kept rows' places in the cache
   int num_seqs, Hkv, keep, recent, max_ctx, block_size, row_bytes, in_place, block_shift;   // the launcher sets the shift
+  unsigned block_magic;      // and this: a division by block_size
 };
 
 namespace mbm {

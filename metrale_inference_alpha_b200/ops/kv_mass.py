@@ -21,35 +21,23 @@ the fp32 restatements in ``reference.py``.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from typing import Optional, Tuple
 
 import torch
 
-from . import _native, reference as ref
-
-_p, _i, _ll = C.c_void_p, C.c_int, C.c_longlong
+from . import _count, _native, _stream, reference as ref, runtime
 
 HEAD_DIMS = (64, 128, 256)
 MAX_GROUP = 64                   # query heads that share a kv head
 
+# MbMassArgs and MbEvictArgs of csrc/kv_mass.h, field by field. Calls of some ten microseconds pack them at once: a ctypes structure of as many fields takes
+# twice as long to fill.
+_MASS_ARGS = struct.Struct("@4P q 4P 2q 2P N 3P 2q 10i f 4x")
+_EVICT_ARGS = struct.Struct("@P 2q P 2q 5P q P q 2P q 2P 10i")
 
-class _MassArgs(C.Structure):
-    _fields_ = [("q", _p), ("k_cache", _p), ("v_cache", _p), ("block_table", _p), ("table_ld", _ll), ("q_start", _p), ("q_len", _p), ("ctx_len", _p),
-                ("mass", _p), ("mass_seq", _ll), ("mass_head", _ll), ("out", _p), ("ws", _p), ("ws_bytes", C.c_size_t), ("k_scale", _p), ("v_scale", _p),
-                ("status", _p), ("num_blocks", _ll), ("q_rows", _ll), ("num_seqs", _i), ("Hq", _i), ("Hkv", _i), ("D", _i), ("block_size", _i), ("fp8", _i),
-                ("max_ctx", _i), ("max_q_len", _i), ("last", _i), ("sm_count", _i), ("scale", C.c_float)]
-
-
-class _EvictArgs(C.Structure):
-    _fields_ = [("mass", _p), ("mass_seq", _ll), ("mass_head", _ll), ("mass_out", _p), ("out_seq", _ll), ("out_head", _ll), ("ctx_len", _p), ("kept", _p),
-                ("new_len", _p), ("first", _p), ("block_table", _p), ("table_ld", _ll), ("dst_table", _p), ("dst_ld", _ll), ("k_cache", _p), ("v_cache", _p),
-                ("num_blocks", _ll), ("status", _p), ("slots", _p), ("num_seqs", _i), ("Hkv", _i), ("keep", _i), ("recent", _i), ("max_ctx", _i), ("block_size", _i),
-                ("row_bytes", _i), ("in_place", _i), ("block_shift", _i)]
-
-
-_native.register_optional("mb_attn_mass", [C.POINTER(_MassArgs), _p])
-_native.register_optional("mb_prompt_mass", [C.POINTER(_MassArgs), _p])
-_native.register_optional("mb_kv_evict", [C.POINTER(_EvictArgs), _p])
+for _name in ("mb_attn_mass", "mb_prompt_mass", "mb_kv_evict"):
+    _native.register_optional(_name, [C.c_char_p, C.c_void_p])
 
 
 _ws_bytes: dict = {}
@@ -59,7 +47,7 @@ def _workspace(name: str, *sizes) -> int:
     fn = _ws_bytes.get(name)
     if fn is None:
         fn = getattr(_native.lib(), name)
-        fn.restype, fn.argtypes = C.c_size_t, [_i] * len(sizes)
+        fn.restype, fn.argtypes = C.c_size_t, [C.c_int] * len(sizes)
         _ws_bytes[name] = fn
     return fn(*sizes)
 
@@ -155,7 +143,6 @@ def paged_attention_mass(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     _check_places(where, q, k_cache, v_cache, block_table, ctx_len, mass, k_scale, v_scale)
     if not q.is_cuda:
         return ref.paged_attention_mass(q, k_cache, v_cache, block_table, ctx_len, mass, scale, k_scale, v_scale)
-    from . import _count, _stream, runtime
     out = torch.empty_like(q)
     if S == 0:
         return out
@@ -166,15 +153,14 @@ def paged_attention_mass(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
         step = min(step, S)
         need = _workspace("mb_attn_mass_ws", step, Hq, D, max_ctx)
     ws = torch.empty(need, dtype=torch.uint8, device=q.device)
-    a = _MassArgs(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), block_table.stride(0), None, None, ctx_len.data_ptr(), mass.data_ptr(),
-                  mass.stride(0), mass.stride(1), out.data_ptr(), ws.data_ptr(), need, None if k_scale is None else k_scale.data_ptr(),
-                  None if v_scale is None else v_scale.data_ptr(), rt.status.data_ptr(), nb, 0, step, Hq, Hkv, D, bs, int(k_cache.dtype == torch.uint8), max_ctx, 1, 1,
-                  rt.sm_count, scale)
+    fp8 = int(k_cache.dtype == torch.uint8)
+    ks, vs = (k_scale.data_ptr(), v_scale.data_ptr()) if fp8 else (0, 0)
+    qp, op, tp, cp, mp = q.data_ptr(), out.data_ptr(), block_table.data_ptr(), ctx_len.data_ptr(), mass.data_ptr()
+    tld, mseq, mhead, row = block_table.stride(0), mass.stride(0), mass.stride(1), Hq * D * 2
     for s in range(0, S, step):
-        if s:
-            a.q, a.out, a.ctx_len = q.data_ptr() + s * Hq * D * 2, out.data_ptr() + s * Hq * D * 2, ctx_len.data_ptr() + s * 4
-            a.block_table, a.mass, a.num_seqs = block_table.data_ptr() + s * block_table.stride(0) * 4, mass.data_ptr() + s * mass.stride(0) * 4, min(step, S - s)
-        _native.check(launch(C.byref(a), _stream()), "attn_mass")
+        a = _MASS_ARGS.pack(qp + s * row, k_cache.data_ptr(), v_cache.data_ptr(), tp + 4 * s * tld, tld, 0, 0, cp + 4 * s, mp + 4 * s * mseq, mseq, mhead, op + s * row,
+                            ws.data_ptr(), need, ks, vs, rt.status.data_ptr(), nb, 0, min(step, S - s), Hq, Hkv, D, bs, fp8, max_ctx, 1, 1, rt.sm_count, scale)
+        _native.check(launch(a, _stream()), "attn_mass")
         _count(2)
     return out
 
@@ -201,14 +187,13 @@ def prompt_mass(q: torch.Tensor, k_cache: torch.Tensor, block_table: torch.Tenso
         return ref.prompt_mass(q, k_cache, block_table, q_start, q_len, ctx_len, mass, scale, last, k_scale)
     if S == 0 or q.shape[0] == 0 or max_q_len == 0 or max_ctx == 0:
         return mass
-    from . import _count, _stream, runtime
     seen, fp8 = min(last or max_q_len, max_q_len), int(k_cache.dtype == torch.uint8)
     need = _workspace("mb_prompt_mass_ws", S, Hq, Hkv, D, bs, seen, max_ctx, fp8)
     ws, rt = torch.empty(need, dtype=torch.uint8, device=q.device), runtime(q.device)
-    a = _MassArgs(q.data_ptr(), k_cache.data_ptr(), None, block_table.data_ptr(), block_table.stride(0), q_start.data_ptr(), q_len.data_ptr(), ctx_len.data_ptr(),
-                  mass.data_ptr(), mass.stride(0), mass.stride(1), None, ws.data_ptr(), need, None if k_scale is None else k_scale.data_ptr(), None, rt.status.data_ptr(),
-                  nb, q.shape[0], S, Hq, Hkv, D, bs, fp8, max_ctx, max_q_len, seen, rt.sm_count, scale)
-    _native.check(_native.lib().mb_prompt_mass(C.byref(a), _stream()), "prompt_mass")
+    a = _MASS_ARGS.pack(q.data_ptr(), k_cache.data_ptr(), 0, block_table.data_ptr(), block_table.stride(0), q_start.data_ptr(), q_len.data_ptr(), ctx_len.data_ptr(),
+                        mass.data_ptr(), mass.stride(0), mass.stride(1), 0, ws.data_ptr(), need, k_scale.data_ptr() if fp8 else 0, 0, rt.status.data_ptr(), nb, q.shape[0],
+                        S, Hq, Hkv, D, bs, fp8, max_ctx, max_q_len, seen, rt.sm_count, scale)
+    _native.check(_native.lib().mb_prompt_mass(a, _stream()), "prompt_mass")
     _count(3 if seen * (Hq // Hkv) > 4096 else 2)               # columns whose rows are cut into parts are joined
     return mass
 
@@ -244,17 +229,16 @@ def kv_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Te
     _check_places(where, k_cache, v_cache, block_table, ctx_len, mass, mo, dst_table)
     if not k_cache.is_cuda:
         return ref.kv_evict(k_cache, v_cache, block_table, ctx_len, mass, keep, recent, max_ctx, mo, dst_table)
-    from . import _count, _stream, runtime
     dev = k_cache.device
     kept, new_len = torch.empty(S, Hkv, keep, dtype=torch.int32, device=dev), torch.empty(S, dtype=torch.int32, device=dev)
     if S == 0:
         return kept, new_len
     own = torch.empty(S * Hkv * (keep + 1), dtype=torch.int32, device=dev)     # of a sequence and head: the rows' slots, the first that moves
     dst = block_table if dst_table is None else dst_table
-    a = _EvictArgs(mass.data_ptr(), mass.stride(0), mass.stride(1), mo.data_ptr(), mo.stride(0), mo.stride(1), ctx_len.data_ptr(), kept.data_ptr(), new_len.data_ptr(),
-                   own.data_ptr() + 4 * S * Hkv * keep, block_table.data_ptr(), block_table.stride(0), dst.data_ptr(), dst.stride(0), k_cache.data_ptr(),
-                   v_cache.data_ptr(), nb, runtime(dev).status.data_ptr(), own.data_ptr(), S, Hkv, keep, recent, max_ctx, bs, D * k_cache.element_size(),
-                   int(dst_table is None), 0)
-    _native.check(_native.lib().mb_kv_evict(C.byref(a), _stream()), "kv_evict")
+    a = _EVICT_ARGS.pack(mass.data_ptr(), mass.stride(0), mass.stride(1), mo.data_ptr(), mo.stride(0), mo.stride(1), ctx_len.data_ptr(), kept.data_ptr(),
+                         new_len.data_ptr(), own.data_ptr() + 4 * S * Hkv * keep, block_table.data_ptr(), block_table.stride(0), dst.data_ptr(), dst.stride(0),
+                         k_cache.data_ptr(), v_cache.data_ptr(), nb, runtime(dev).status.data_ptr(), own.data_ptr(), S, Hkv, keep, recent, max_ctx, bs,
+                         D * k_cache.element_size(), dst_table is None, 0, 0)
+    _native.check(_native.lib().mb_kv_evict(a, _stream()), "kv_evict")
     _count(2)
     return kept, new_len
