@@ -44,6 +44,8 @@ struct DecodeParams {
   float* z;                                  // MASS: logits in the log2 domain [seqs * Hq, z_ld], a column a cached token
   long long z_ld;
   int max_ctx;                               // MASS: longer sequences are reported and cut
+  int group, group0;                         // MASS: query heads of a kv head, the first of the G that this launch takes
+  int box_bits;                              // MASS: log2 of a slice's TMA boxes, 16 / the greatest common divisor of 16 and block_size
 };
 
 __device__ __forceinline__ void mma16816_f16(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
@@ -224,8 +226,9 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
     x.slices = (n - warp + 3) >> 2;
   };
   // places of the slices of this warp's steps i0 .. i0 + 32 / kSub - 1, one per lane
+  const int box_bits = MASS ? p.box_bits : 0, step_bits = box_bits + kSub / 2, per = 1 << step_bits;   // boxes of a slice, of a step
   auto blocks = [&](Unit& x, int i0) {
-    const int i = i0 + lane / kSub, tok = x.begin + (warp + 4 * i) * kTok + lane % kSub * kSlice;
+    const int i = i0 + (lane >> step_bits), tok = x.begin + (warp + 4 * i) * kTok + (lane & (per - 1)) * (kSlice >> box_bits);
     x.blk = x.within = 0;                                    // a slice behind the context reads the null block
     if (i < x.slices && tok < x.ctx) {
       const int bi = p.block_shift >= 0 ? tok >> p.block_shift : tok / p.block_size;
@@ -240,35 +243,47 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
   };
   const uint32_t my = mb::smem_u32(smem) + warp * C::kSlot;
   const uint64_t once = MASS ? evict_first() : 0;
-  auto issue = [&](const Unit& x, int i, int slot) {         // whole warp; one lane issues
+  auto issue = [&](Unit& x, int i, int slot) {               // whole warp; one lane issues, MASS: each lane its box
+    if constexpr (MASS)
+      if (i > 0 && (i << step_bits & 31) == 0) blocks(x, i);        // the lanes' places reach 32 / per steps
     const int place = x.blk * p.block_size + x.within;
     uint64_t* bar = &bars[slot * 4 + warp];
     uint8_t* dst = smem + (slot * 4 + warp) * C::kSlot;
     if (lane == 0) mb::mbar_expect_tx(bar, C::kSlot);
+    if constexpr (MASS) {
+      __syncwarp();
+      const int j = lane - (i << step_bits & 31);
+      if (j >= 0 && j < per) {
+#pragma unroll
+        for (int h = 0; h < kSpans; ++h) {
+          // L2 keeps the logits for the join rather than rows that are read once
+          uint8_t* k = dst + ((j >> box_bits) * kSpans + h) * (kSlice * kSpanB) + (j & ((1 << box_bits) - 1)) * ((kSlice >> box_bits) * kSpanB);
+          tma_load_3d_once(k, &tmK, bar, h * kSpanB, x.kvh, place, once);
+          tma_load_3d_once(k + C::kHalf, &tmV, bar, h * kSpanB, x.kvh, place, once);
+        }
+      }
+      return;
+    }
 #pragma unroll
     for (int b = 0; b < kSub; ++b) {
       const int tok = __shfl_sync(0xffffffffu, place, (i * kSub + b) & 31);
       if (lane == 0) {
 #pragma unroll
         for (int h = 0; h < kSpans; ++h) {
-          uint8_t *k = dst + (b * kSpans + h) * (kSlice * kSpanB), *v = k + C::kHalf;
-          if constexpr (MASS) {                              // L2 keeps the logits for the join rather than rows that are read once
-            tma_load_3d_once(k, &tmK, bar, h * kSpanB, x.kvh, tok, once);
-            tma_load_3d_once(v, &tmV, bar, h * kSpanB, x.kvh, tok, once);
-          } else {
-            mb::tma_load_3d(k, &tmK, bar, h * kSpanB, x.kvh, tok);
-            mb::tma_load_3d(v, &tmV, bar, h * kSpanB, x.kvh, tok);
-          }
+          mb::tma_load_3d(dst + (b * kSpans + h) * (kSlice * kSpanB), &tmK, bar, h * kSpanB, x.kvh, tok);
+          mb::tma_load_3d(dst + C::kHalf + (b * kSpans + h) * (kSlice * kSpanB), &tmV, bar, h * kSpanB, x.kvh, tok);
         }
       }
     }
   };
+  // the query head of row r, which is of token tq
+  auto head_of = [&](const Unit& x, int r, int tq) { return MASS ? x.kvh * p.group + p.group0 + r : x.kvh * p.G + (r - tq * p.G); };
   // the unit's query rows into shared memory: the whole CTA, 16 bytes a copy
   auto fetch_q = [&](const Unit& x) {
     const int n = p.G * x.qlen * (D / 8);
     for (int i = tid; i < n; i += 128) {
       const int r = i / (D / 8), c = i % (D / 8), tq = (r * p.g_magic) >> 16;
-      const __nv_bfloat16* src = p.q + ((size_t)(x.qs + tq) * p.Hq + x.kvh * p.G + (r - tq * p.G)) * D + c * 8;
+      const __nv_bfloat16* src = p.q + ((size_t)(x.qs + tq) * p.Hq + head_of(x, r, tq)) * D + c * 8;
       asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(mb::smem_u32(s_q + r * C::kQPitch + c * 16)), "l"(src) : "memory");
     }
   };
@@ -299,7 +314,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
   while (u < units) {
     const int R = p.G * cur.qlen;
     float* zrow = nullptr;
-    if constexpr (MASS) zrow = p.z + ((size_t)cur.seq * p.Hq + cur.kvh * p.G) * p.z_ld;
+    if constexpr (MASS) zrow = p.z + ((size_t)cur.seq * p.Hq + head_of(cur, 0, 0)) * p.z_ld;
     // A lane has scores and outputs of two rows of a tile, g and g + 8 or 2 t and 2 t + 1; of row e the elements at(e, 0) and at(e, 1) of
     // every fragment. The lanes of a row differ in the bits of `t` or in those of `g`.
     auto row_of = [&](int tile, int e) { return kPairs ? tile * 16 + g + 8 * e : tile * 8 + 2 * t + e; };
@@ -534,7 +549,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
       __syncwarp();                                          // every lane has read the slot
       const int nx = i + slots;
       if (nx < cur.slices) {
-        if (nx * kSub % 32 == 0) blocks(cur, nx);
+        if (!MASS && nx * kSub % 32 == 0) blocks(cur, nx);
         issue(cur, nx, slot);
       }
       slot = slot + 1 == slots ? 0 : slot + 1;
@@ -586,7 +601,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
     __syncthreads();
     // final values of four dims of row r: the group's head, the token's row, bf16 or a quantised block (four lanes a block of 16)
     auto store = [&](int r, int c4, float4 a) {
-      const int tq = (r * p.g_magic) >> 16, head = cur.kvh * p.G + r - tq * p.G;
+      const int tq = (r * p.g_magic) >> 16, head = head_of(cur, r, tq);
       const uint32_t m = cur.qs + tq;
       // 17 rows and more quantise the bf16 value, as the row kernel behind this one did: the same bits as with it. Up to 16 the 32-bit one.
       if (kThroughBf16 && p.outq) {
@@ -633,10 +648,10 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         const float inv = l > 0.f ? vmul / l : 0.f;
         store(r, c4, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
         if constexpr (MASS)
-          if (c4 == 0) p.part_ml[((size_t)cur.seq * p.Hq + cur.kvh * p.G + r) * p.parts] = make_float2(mx, l);
+          if (c4 == 0) p.part_ml[((size_t)cur.seq * p.Hq + head_of(cur, r, 0)) * p.parts] = make_float2(mx, l);
       } else {                                               // sums as they are, relative to 2^mx
         const int tq = (r * p.g_magic) >> 16;
-        const size_t row = ((size_t)(cur.qs + tq) * p.Hq + cur.kvh * p.G + r - tq * p.G) * p.parts + cur.part;
+        const size_t row = ((size_t)(cur.qs + tq) * p.Hq + head_of(cur, r, tq)) * p.parts + cur.part;
         *reinterpret_cast<float4*>(p.part_o + row * D + c4 * 4) = acc;
         if (c4 == 0) p.part_ml[row] = make_float2(mx, l);
       }
@@ -728,7 +743,7 @@ int launch(const AttnDecodeArgs& a, DecodeParams& p, cudaStream_t stream) {
   CUtensorMap tm[2];
   for (int i = 0; i < 2; ++i) {
     const int rc = mbh::encode_3d(&tm[i], CU_TENSOR_MAP_DATA_TYPE_UINT8, i ? a.v_cache : a.k_cache, C::kRowB, a.Hkv, (uint64_t)a.num_blocks * a.block_size,
-                                  C::kRowB, (uint64_t)a.Hkv * C::kRowB, C::kSpanB, 1, kSlice,
+                                  C::kRowB, (uint64_t)a.Hkv * C::kRowB, C::kSpanB, 1, MASS ? kSlice >> p.box_bits : kSlice,
                                   C::kSpanB == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc) return rc;
   }

@@ -5,7 +5,7 @@
 
 bool mb_decode_mass_serves(const MbMassArgs& a) {
   const uintptr_t al = reinterpret_cast<uintptr_t>(a.k_cache) | reinterpret_cast<uintptr_t>(a.v_cache) | reinterpret_cast<uintptr_t>(a.q);
-  return a.Hq / a.Hkv <= (a.D == 256 ? 16 : 32) && a.num_seqs <= kMaxSeqs && a.block_size % kSlice == 0 && !(al & 15) &&
+  return a.num_seqs <= kMaxSeqs && !(al & 15) &&
          a.num_blocks * a.block_size < (1ll << 31) && a.table_ld < (1ll << 31);
 }
 
@@ -18,7 +18,7 @@ int mb_decode_mass(const MbMassArgs& m, const mbm::DecodeWs& w, int part_tokens,
   DecodeParams p{};
   p.q = reinterpret_cast<const __nv_bfloat16*>(m.q);
   p.block_table = m.block_table; p.max_blocks = (int)m.table_ld; p.ctx_len = m.ctx_len;
-  p.num_seqs = m.num_seqs; p.Hq = m.Hq; p.Hkv = m.Hkv; p.G = m.Hq / m.Hkv; p.g_magic = (65536 + p.G - 1) / p.G;
+  p.num_seqs = m.num_seqs; p.Hq = m.Hq; p.Hkv = m.Hkv; p.group = m.Hq / m.Hkv;
   p.block_size = m.block_size;
   p.block_shift = (m.block_size & (m.block_size - 1)) == 0 ? 31 - __builtin_clz(m.block_size) : -1;
   p.num_blocks = m.num_blocks; p.scale = m.scale; p.k_scale = m.k_scale; p.v_scale = m.v_scale;
@@ -27,15 +27,23 @@ int mb_decode_mass(const MbMassArgs& m, const mbm::DecodeWs& w, int part_tokens,
   p.part_tokens = part_tokens; p.parts = w.parts;
   p.part_o = reinterpret_cast<float*>(ws + w.o); p.part_ml = reinterpret_cast<float2*>(ws + w.ml);
   p.z = reinterpret_cast<float*>(ws + w.z); p.z_ld = w.ld; p.max_ctx = m.max_ctx;
+  p.box_bits = 0;
+  while (m.block_size % (kSlice >> p.box_bits)) ++p.box_bits;
   auto run = [&](auto d, auto eight) {
+    constexpr int kMost = d.value == 256 ? 16 : 32;          // query rows that the kernel takes
     auto go = [&](auto nt) { return launch<d.value, eight.value, nt.value, true>(a, p, stream); };
-    if (p.G <= 8) return go(std::integral_constant<int, 1>{});
-    if constexpr (d.value == 256) {
-      return go(std::integral_constant<int, 2>{});
-    } else {
-      if (p.G <= 16) return go(std::integral_constant<int, 2>{});
-      return p.G <= 24 ? go(std::integral_constant<int, 3>{}) : go(std::integral_constant<int, 4>{});
+    const int takes = (p.group + kMost - 1) / kMost, each = (p.group + takes - 1) / takes;
+    for (p.group0 = 0; p.group0 < p.group; p.group0 += each) {
+      p.G = min(each, p.group - p.group0);
+      a.Hq = p.G * a.Hkv;
+      p.g_magic = 1;                                         // one token a sequence: r / G is 0
+      int rc;
+      if (p.G <= 8) rc = go(std::integral_constant<int, 1>{});
+      else if constexpr (d.value == 256) rc = go(std::integral_constant<int, 2>{});
+      else rc = p.G <= 16 ? go(std::integral_constant<int, 2>{}) : p.G <= 24 ? go(std::integral_constant<int, 3>{}) : go(std::integral_constant<int, 4>{});
+      if (rc) return rc;
     }
+    return 0;
   };
   auto by_dim = [&](auto eight) {
     return m.D == 64 ? run(std::integral_constant<int, 64>{}, eight) : m.D == 128 ? run(std::integral_constant<int, 128>{}, eight)
