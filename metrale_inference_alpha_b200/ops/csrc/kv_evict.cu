@@ -366,7 +366,7 @@ __global__ void __launch_bounds__(256) evict_move_kernel(const MbEvictArgs a, in
 extern "C" int mb_kv_evict(const MbEvictArgs* given, cudaStream_t stream) {
   if (!given) return MB_ERR_BAD_ARG;
   MbEvictArgs args = *given, *a = &args;
-  if ( a->num_seqs <= 0 || a->num_seqs > 65535 || a->Hkv <= 0 || a->Hkv > 65535 || a->keep <= 0 || a->recent < 0 || a->recent > a->keep || a->max_ctx < 0 ||
+  if ( a->num_seqs <= 0 || a->num_seqs > 65535 || a->Hkv <= 0 || a->Hkv > 65535 || a->keep <= 0 || a->recent < 0 || a->recent > a->keep || a->max_ctx <= 0 ||
       a->block_size <= 0 || a->num_blocks <= 0 || a->row_bytes < 64 || (a->row_bytes & (a->row_bytes - 1)) || !a->mass || !a->mass_out || !a->ctx_len || !a->kept ||
       !a->new_len || !a->first || !a->slots || !a->block_table || !a->dst_table || !a->k_cache || !a->v_cache)
     return MB_ERR_BAD_ARG;
@@ -391,7 +391,6 @@ extern "C" int mb_kv_evict(const MbEvictArgs* given, cudaStream_t stream) {
   }
   if (e != cudaSuccess) return (int)e;
   const int held = a->keep < a->max_ctx ? a->keep : a->max_ctx;
-  if (held == 0) return 0;
   int bits = 0;
   while (16 << bits < a->row_bytes) ++bits;
   if (!a->in_place) {

@@ -18,9 +18,7 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-constexpr int kPartTokens = 512;
-
-constexpr int kChunk = 1024;
+constexpr int kPartTokens = 512, kChunk = 1024;
 
 // Columns [chunk * 1024, ...) of a (sequence, kv head): logits become weights, weights are added to the mass. The chunks share out the
 // group's outputs among themselves; those of a single partition stand already. Logits, mass and partitions are asked for together: with one
@@ -104,7 +102,7 @@ __global__ void __launch_bounds__(256) mass_join_kernel(const MbMassArgs a, cons
 
 bool bad_shape(const MbMassArgs& a) {
   return a.num_seqs <= 0 || a.num_seqs > 65535 || a.Hkv <= 0 || a.Hkv > 65535 || a.Hq % a.Hkv || a.Hq / a.Hkv > 64 || (a.D != 64 && a.D != 128 && a.D != 256) ||
-         a.block_size <= 0 || a.num_blocks <= 0 || a.max_ctx < 0 || !a.q || !a.k_cache || !a.block_table || !a.ctx_len || !a.mass || (a.fp8 && !a.k_scale);
+         a.block_size <= 0 || a.num_blocks <= 0 || a.max_ctx <= 0 || !a.q || !a.k_cache || !a.block_table || !a.ctx_len || !a.mass || (a.fp8 && !a.k_scale);
 }
 
 }  // namespace
@@ -124,7 +122,7 @@ int mb_attn_mass(const MbMassArgs* a, cudaStream_t stream) {
   const int rc = mb_decode_mass(*a, w, part, stream);
   if (rc) return rc;
   const int chunks = (a->max_ctx + kChunk - 1) / kChunk;
-  return (int)mb::launch_kernel_ex(mass_join_kernel, dim3(chunks < 1 ? 1 : chunks, a->Hkv, a->num_seqs), dim3(256), 0, stream, 1, true, *a, w, part);
+  return (int)mb::launch_kernel_ex(mass_join_kernel, dim3(chunks, a->Hkv, a->num_seqs), dim3(256), 0, stream, 1, true, *a, w, part);
 }
 
 }  // extern "C"

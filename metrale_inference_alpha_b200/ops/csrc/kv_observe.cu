@@ -99,7 +99,7 @@ inline Ws workspace(int seqs, int Hq, int Hkv, int D, int block_size, int seen, 
 template <bool FP8>
 __global__ void __launch_bounds__(256) observe_copy_kernel(const MbMassArgs a, const Ws ws) {
   mb::pdl_launch_dependents();
-  const int s = blockIdx.y, n = min(a.ctx_len[s], a.max_ctx), per = a.Hkv * a.D / 16;        // of a cached token
+  const int s = blockIdx.y, n = a.q_len[s] > 0 ? min(a.ctx_len[s], a.max_ctx) : 0, per = a.Hkv * a.D / 16;        // of a cached token
   const int* table = a.block_table + s * a.table_ld;
   uint4* out = reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(a.ws) + ws.keys) + (size_t)s * ws.tokens * per * 2;
   // a CTA takes 8192 values at a time: whole tokens, or a part of one

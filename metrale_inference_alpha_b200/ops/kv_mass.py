@@ -123,8 +123,18 @@ def _check_rows(where, name, mass) -> None:
         _bad(where, f"rows of {name} share memory")
 
 
-# most bytes of logits that a decode step has under way; more sequences go in several steps
+# most bytes of workspace that a call has under way (a decode step's logits, a prompt's queries and the copy of its keys): more sequences go in several steps
 _WS_BYTES = 1 << 30
+
+
+def _step(name: str, S: int, most: int, *sizes) -> Tuple[int, int]:
+    """Sequences that are worked on at once, and their workspace."""
+    step = min(S, most)
+    need = _workspace(name, step, *sizes)
+    if need > _WS_BYTES and step > 1:
+        step = min(step, max(1, _WS_BYTES // _workspace(name, 1, *sizes)))
+        need = _workspace(name, step, *sizes)
+    return step, need
 
 
 def paged_attention_mass(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor, ctx_len: torch.Tensor,
@@ -143,15 +153,11 @@ def paged_attention_mass(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     _check_places(where, q, k_cache, v_cache, block_table, ctx_len, mass, k_scale, v_scale)
     if not q.is_cuda:
         return ref.paged_attention_mass(q, k_cache, v_cache, block_table, ctx_len, mass, scale, k_scale, v_scale)
+    if S == 0 or max_ctx == 0:
+        return torch.zeros_like(q)
     out = torch.empty_like(q)
-    if S == 0:
-        return out
     launch, rt = _native.lib().mb_attn_mass, runtime(q.device)
-    step, need = min(S, 1024), _workspace("mb_attn_mass_ws", min(S, 1024), Hq, D, max_ctx)
-    if need > _WS_BYTES:
-        step = max(1, _WS_BYTES // _workspace("mb_attn_mass_ws", 1, Hq, D, max_ctx))
-        step = min(step, S)
-        need = _workspace("mb_attn_mass_ws", step, Hq, D, max_ctx)
+    step, need = _step("mb_attn_mass_ws", S, 1024, Hq, D, max_ctx)
     ws = torch.empty(need, dtype=torch.uint8, device=q.device)
     fp8 = int(k_cache.dtype == torch.uint8)
     ks, vs = (k_scale.data_ptr(), v_scale.data_ptr()) if fp8 else (0, 0)
@@ -188,13 +194,20 @@ def prompt_mass(q: torch.Tensor, k_cache: torch.Tensor, block_table: torch.Tenso
     if S == 0 or q.shape[0] == 0 or max_q_len == 0 or max_ctx == 0:
         return mass
     seen, fp8 = min(last or max_q_len, max_q_len), int(k_cache.dtype == torch.uint8)
-    need = _workspace("mb_prompt_mass_ws", S, Hq, Hkv, D, bs, seen, max_ctx, fp8)
-    ws, rt = torch.empty(need, dtype=torch.uint8, device=q.device), runtime(q.device)
-    a = _MASS_ARGS.pack(q.data_ptr(), k_cache.data_ptr(), 0, block_table.data_ptr(), block_table.stride(0), q_start.data_ptr(), q_len.data_ptr(), ctx_len.data_ptr(),
-                        mass.data_ptr(), mass.stride(0), mass.stride(1), 0, ws.data_ptr(), need, k_scale.data_ptr() if fp8 else 0, 0, rt.status.data_ptr(), nb, q.shape[0],
-                        S, Hq, Hkv, D, bs, fp8, max_ctx, max_q_len, seen, rt.sm_count, scale)
-    _native.check(_native.lib().mb_prompt_mass(a, _stream()), "prompt_mass")
-    _count(3 if seen * (Hq // Hkv) > 4096 else 2)               # columns whose rows are cut into parts are joined
+    if seen * (Hq // Hkv) > 1 << 25:
+        _bad(where, f"{seen} tokens of {Hq // Hkv} heads a group are more than 2^25 rows")
+    step, need = _step("mb_prompt_mass_ws", S, 65535, Hq, Hkv, D, bs, seen, max_ctx, fp8)
+    ws, rt, launch = torch.empty(need, dtype=torch.uint8, device=q.device), runtime(q.device), _native.lib().mb_prompt_mass
+    tp, qs, ql, cp, mp, tld, mseq = (block_table.data_ptr(), q_start.data_ptr(), q_len.data_ptr(), ctx_len.data_ptr(), mass.data_ptr(), block_table.stride(0),
+                                     mass.stride(0))
+    for s in range(0, S, step):
+        a = _MASS_ARGS.pack(q.data_ptr(), k_cache.data_ptr(), 0, tp + 4 * s * tld, tld, qs + 4 * s, ql + 4 * s, cp + 4 * s, mp + 4 * s * mseq, mseq, mass.stride(1), 0,
+                            ws.data_ptr(), need, k_scale.data_ptr() if fp8 else 0, 0, rt.status.data_ptr(), nb, q.shape[0], min(step, S - s), Hq, Hkv, D, bs, fp8,
+                            max_ctx, max_q_len, seen, rt.sm_count, scale)
+        _native.check(launch(a, _stream()), "prompt_mass")
+        # beside the two passes a copy of the keys (see csrc/kv_observe.cu) and the join of columns whose rows are cut into parts
+        rows = seen * (Hq // Hkv)
+        _count(2 + (fp8 or bs % 16 != 0 or rows >= 1024) + (rows > 4096))
     return mass
 
 
@@ -231,8 +244,8 @@ def kv_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Te
         return ref.kv_evict(k_cache, v_cache, block_table, ctx_len, mass, keep, recent, max_ctx, mo, dst_table)
     dev = k_cache.device
     kept, new_len = torch.empty(S, Hkv, keep, dtype=torch.int32, device=dev), torch.empty(S, dtype=torch.int32, device=dev)
-    if S == 0:
-        return kept, new_len
+    if S == 0 or max_ctx == 0:
+        return kept.fill_(-1), new_len.zero_()
     own = torch.empty(S * Hkv * (keep + 1), dtype=torch.int32, device=dev)     # of a sequence and head: the rows' slots, the first that moves
     dst = block_table if dst_table is None else dst_table
     a = _EVICT_ARGS.pack(mass.data_ptr(), mass.stride(0), mass.stride(1), mo.data_ptr(), mo.stride(0), mo.stride(1), ctx_len.data_ptr(), kept.data_ptr(),

@@ -115,6 +115,36 @@ def test_decode_in_several_steps_gives_the_same(monkeypatch):
     assert torch.equal(_decode({**c, "mass": m}), out) and torch.equal(m, c["mass"])
 
 
+def test_decode_of_more_sequences_than_a_launch_takes():
+    n = 1100
+    c = oracle.case(31, [1 + i % 5 for i in range(n)], 4, 2, 64, False)
+    want, tol, mass, mtol = oracle.decode(c)
+    g = _cuda(c)
+    _within(_decode(g), want, tol, "outputs")
+    _within(g["mass"], mass, mtol, "mass")
+
+
+def test_decode_of_lanes_that_pad_the_batch():
+    """Lengths of zero and less, and a call all of whose lanes are such."""
+    c = _cuda(oracle.case(32, [40, 3, 20], 4, 2, 64, True))
+    c["ctx"] = torch.tensor([0, -7, 20], dtype=torch.int32, device="cuda")
+    before = c["mass"].clone()
+    out = _decode(c)
+    assert not out[:2].any() and torch.equal(c["mass"][:2], before[:2]) and bool((c["mass"][2] != before[2]).any())
+    none = torch.zeros(3, 2, 0, device="cuda")
+    assert not _decode({**c, "ctx": torch.zeros_like(c["ctx"]), "mass": none, "table": c["table"][:, :0]}, max_ctx=0).any()
+
+
+def test_decode_of_infinities_and_nan():
+    """A query that is not a number makes its group's mass one; a key that is one of infinity takes all the weight or the row with it, as in 64 bits."""
+    c = oracle.case(33, [50, 60], 8, 2, 128, False)
+    c["q"][0, 1, 5] = float("nan")
+    g = _cuda(c)
+    out = _decode(g)
+    assert out[0, 1].isnan().all() and g["mass"][0, 0, :50].isnan().all()
+    assert not out[0, 2:].isnan().any() and not g["mass"][0, 1].isnan().any() and not g["mass"][1].isnan().any()
+
+
 def test_decode_agrees_with_the_attention_that_leaves_no_weights():
     c = _cuda(oracle.case(27, [700, 64, 1300], 40, 8, 128, True))
     plain = ops.paged_attention(c["q"], c["k"], c["v"], c["table"], c["q_start"], c["q_len"], c["ctx"], max_q_len=1, max_ctx=1300, scale=c["scale"], k_scale=c["k_scale"],
@@ -218,6 +248,42 @@ def test_prompt_of_a_sequence_does_not_depend_on_its_batch():
         one = {k: c[k][s:s + 1] for k in ("table", "ctx", "q_start", "q_len")}
         _prompt({**c, **one, "mass": m[s:s + 1]}, 64)
         assert torch.equal(m[s], c["mass"][s])
+
+
+def test_prompt_in_several_steps_gives_the_same(monkeypatch):
+    c = _cuda(oracle.case(48, [300, 40, 0, 513, 77], 8, 2, 128, True, new=[200, 40, 0, 13, 77]))
+    m = c["mass"].clone()
+    _prompt(c, 64)
+    monkeypatch.setattr(kv_mass, "_WS_BYTES", 1)
+    _prompt({**c, "mass": m}, 64)
+    assert torch.equal(m, c["mass"])
+
+
+@pytest.mark.parametrize("apart", [2.0 ** -9, 2.0 ** 9, 2.0 ** 40])
+def test_prompt_of_rows_far_apart(apart):
+    """An e4m3 cache's queries become f16: rows whose sizes differ by little share a factor, others have their own; none loses its range."""
+    c = oracle.case(49, [300, 150], 8, 2, 128, True, new=[200, 150])
+    c["scale"] /= max(1.0, apart)
+    c["q"][::3] *= apart
+    c["q"][5::7] = 0
+    mass, mtol = oracle.prompt(c, 0)
+    g = _cuda(c)
+    _prompt(g, 0)
+    _within(g["mass"], mass, mtol, "mass")
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_prompt_of_a_query_that_is_not_a_number(fp8):
+    c = oracle.case(57, [200, 100], 8, 2, 128, fp8, new=[100, 100])
+    c["q"][20, 1, 3] = float("nan")                          # sequence 0, sees the first 121 tokens; head 1 is of kv head 0
+    g = _cuda(c)
+    _prompt(g, 0)
+    assert g["mass"][0, 0, :121].isnan().all() and not g["mass"][0, 0, 121:].isnan().any()
+    assert not g["mass"][0, 1].isnan().any() and not g["mass"][1].isnan().any()
+    c["q"][20, 1, 3] = 0
+    g = _cuda(c)
+    _prompt({**g, "q": g["q"].masked_fill(torch.arange(200, device="cuda")[:, None, None] == 20, float("nan"))}, 50)   # among those that do not observe
+    assert not g["mass"].isnan().any()
 
 
 def test_prompt_in_a_graph_beside_another():
@@ -355,6 +421,16 @@ def test_evict_reports_lengths_and_blocks_out_of_range():
     with pytest.raises(_native.KernelError, match="bounds"):
         ops.check_status("cuda")
     assert length.tolist() == [90, 50] and int(kept.max()) == 89
+
+
+def test_evict_of_nothing():
+    c = _cuda(oracle.case(58, [40, 9], 4, 2, 64, False))
+    none = torch.zeros(2, 2, 0, device="cuda")
+    kept, length = ops.kv_evict(c["k"], c["v"], c["table"][:, :0], torch.zeros_like(c["ctx"]), none, keep=3, recent=1, max_ctx=0)
+    assert bool((kept == -1).all()) and not length.any()
+    k = c["k"].clone()
+    kept, length = ops.kv_evict(c["k"], c["v"], c["table"], torch.tensor([0, -4], dtype=torch.int32, device="cuda"), c["mass"], keep=3, recent=1, max_ctx=40)
+    assert bool((kept == -1).all()) and not length.any() and _same(c["k"], k) and not c["mass"].any()
 
 
 # ----------------------------------------------------------------------------- together
