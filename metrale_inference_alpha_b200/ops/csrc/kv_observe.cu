@@ -144,12 +144,12 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
   uint8_t* sRing = sHeld + C::kHeldB;                        // kStages x [kN rows x 128 B]
   __shared__ __align__(8) uint64_t held_full, full[kStages], empty[kStages], info_full[kInfo], info_free[kInfo], s_full[2], s_free[2];
   __shared__ uint32_t s_tmem;
-  __shared__ float s_row[kHeld];                               // rows pass, e4m3: the exponent of a row's largest element
+  __shared__ int s_row[kHeld];                                 // rows pass, e4m3: the exponent of a row's largest element
   __shared__ float2 s_half[kHeld];                             // sums of the second half of the columns
   __shared__ __align__(16) float s_lse[kInfo][kN];           // keys pass: the query rows' normalisers, negative, and their factors
   __shared__ __align__(16) float s_factor[KEYS && FP8 ? kInfo : 1][kN];
   __shared__ __align__(8) int s_alike[KEYS && FP8 ? kInfo : 1][4];         // 32 rows' factors are those of the first of 64
-  __shared__ int s_top[2];                                   // rows pass, e4m3: the largest exponent of a row's largest element, and the smallest
+  __shared__ int2 s_top[kSums / 32];                         // rows pass, e4m3: the largest exponent of a row's largest element, and the smallest
   const int h = blockIdx.y, s = blockIdx.z, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int G = a.Hq / a.Hkv;
   const Span x = span_of(a, s, G);
@@ -182,9 +182,44 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
   uint4* wq = reinterpret_cast<uint4*>(a.ws) + row0 * (D / 8);
   float* wscale = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(a.ws) + ws.scale) + row0;
 
-  if (tid == 0) {
-    s_top[0] = 0;
-    s_top[1] = 255;
+  // ---- rows pass: the query rows, which stay: 128 of them, rows behind the last one are zeros. They are asked for while the barriers are made.
+  constexpr int kPieces = D / 8, kStep = kSums / kPieces, kLoads = kHeld / kStep, kBatch = kLoads < 8 ? kLoads : 8;
+  const int c = tid % kPieces, hr0 = tid / kPieces;
+  uint4 v[kBatch];
+  auto load = [&](int i0) {
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int hr = hr0 + kStep * (i0 + i), at = min(at0 + hr, own - 1), tq = tok_of(at);
+      v[i] = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(a.q) + ((size_t)(x.tok0 + tq) * a.Hq + h * G + (at - tq * G)) * D) + c);
+      if (at0 + hr >= own) v[i] = make_uint4(0, 0, 0, 0);
+    }
+  };
+  if (!KEYS && warp < 8) {
+    int hi = 0, lo = 255;
+#pragma unroll 1
+    for (int i0 = 0; i0 < (FP8 ? kLoads : kBatch); i0 += kBatch) {
+      load(i0);
+      if constexpr (FP8) {
+        // the exponent of a row's largest element; bits of a bf16 without its sign order like the values
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+          uint32_t top = __vmaxu2(__vmaxu2(v[i].x & 0x7fff7fffu, v[i].y & 0x7fff7fffu), __vmaxu2(v[i].z & 0x7fff7fffu, v[i].w & 0x7fff7fffu));
+#pragma unroll
+          for (int d = 1; d < kPieces; d <<= 1) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, d));
+          const int e = (int)(max(top & 0xffff, top >> 16) >> 7);
+          if (c == 0) s_row[hr0 + kStep * (i0 + i)] = e;
+          hi = max(hi, e);
+          if (e > 0) lo = min(lo, e);
+        }
+      }
+    }
+    if constexpr (FP8) {
+      hi = __reduce_max_sync(0xffffffffu, hi);
+      lo = __reduce_min_sync(0xffffffffu, lo);
+      if (lane == 0) s_top[warp] = make_int2(hi, lo);
+    }
+  }
+  if (tid == kThreads - 1) {
     mb::mbar_init(&held_full, KEYS ? 1 : kSums / 32);
     for (int i = 0; i < kStages; ++i) {
       mb::mbar_init(&full[i], 1);
@@ -219,58 +254,32 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
     constexpr int kCols = kN / 2, kW = 32;                   // columns of a thread, and of a round
     float row_scale = 1.f;                                   // what this thread's row's scores are too large by
     if constexpr (!KEYS) {
-      // ---- the query rows, which stay: 128 of them, rows behind the last one are zeros. The first part's CTA leaves them for the keys pass.
-      constexpr int kPieces = D / 8, kStep = kSums / kPieces, kLoads = kHeld / kStep, kBatch = kLoads < 8 ? kLoads : 8;
-      const int c = tid % kPieces, hr0 = tid / kPieces;
-      uint4 v[kBatch];
-      auto load = [&](int i0) {
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-          const int hr = hr0 + kStep * (i0 + i), at = min(at0 + hr, own - 1), tq = tok_of(at);
-          v[i] = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(a.q) + ((size_t)(x.tok0 + tq) * a.Hq + h * G + (at - tq * G)) * D) + c);
-          if (at0 + hr >= own) v[i] = make_uint4(0, 0, 0, 0);
-        }
-      };
-      int up = 0;
-      bool alike = true;
       // f16 has less range than bf16: the power of two that takes a row's largest element to [2^14, 2^15). Zeros and subnormal rows as if their
       // exponent were 15, infinities and NaN as they are.
       auto lift = [](int e) { return e == 255 ? 0 : 141 - max(e, 15); };
+      int up = 0;
+      bool alike = true;
       if constexpr (FP8) {
-        // the exponent of a row's largest element; bits of a bf16 without its sign order like the values
-#pragma unroll 1
-        for (int i0 = 0; i0 < kLoads; i0 += kBatch) {
-          load(i0);
-#pragma unroll
-          for (int i = 0; i < kBatch; ++i) {
-            uint32_t top = __vmaxu2(__vmaxu2(v[i].x & 0x7fff7fffu, v[i].y & 0x7fff7fffu), __vmaxu2(v[i].z & 0x7fff7fffu, v[i].w & 0x7fff7fffu));
-#pragma unroll
-            for (int d = 1; d < kPieces; d <<= 1) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, d));
-            const int e = (int)(max(top & 0xffff, top >> 16) >> 7);
-            if (c == 0) {
-              s_row[hr0 + kStep * (i0 + i)] = __int_as_float(e);
-              if (e > 0) {
-                atomicMax(&s_top[0], e);
-                atomicMin(&s_top[1], e);
-              }
-            }
-          }
-        }
-        asm volatile("bar.sync 1, 256;" ::: "memory");
         // Rows whose largest elements are within 2^12 of each other take the power of the largest, so that their scores have one factor: the smallest then
         // still keeps 8 bits of elements down to 2^-19 of its largest, and the rest to 2^-27 of it.
-        const int hi = s_top[0], lo = s_top[1];
+        int hi = 0, lo = 255;
+#pragma unroll
+        for (int i = 0; i < kSums / 32; ++i) {
+          hi = max(hi, s_top[i].x);
+          lo = min(lo, s_top[i].y);
+        }
         alike = hi < 255 && hi - lo <= 12;
         up = lift(hi);
       }
+      // The first part's CTA leaves the rows for the keys pass.
 #pragma unroll 1
       for (int i0 = 0; i0 < kLoads; i0 += kBatch) {
-        if (!FP8 || kLoads > kBatch) load(i0);
+        if (kLoads > kBatch && (FP8 || i0 > 0)) load(i0);
 #pragma unroll
         for (int i = 0; i < kBatch; ++i) {
           const int hr = hr0 + kStep * (i0 + i);
           if constexpr (FP8) {
-            const int mine_up = alike ? up : lift(__float_as_int(s_row[hr]));
+            const int mine_up = alike ? up : lift(s_row[hr]);
             const float f = __int_as_float((127 + mine_up) << 23);
             const uint32_t y[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
             uint32_t z[4];
@@ -289,7 +298,7 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
       fence_async_smem();
       __syncwarp();
       if (lane == 0) mb::mbar_arrive(&held_full);
-      if constexpr (FP8) row_scale = __int_as_float((127 - (alike ? up : lift(__float_as_int(s_row[r])))) << 23);
+      if constexpr (FP8) row_scale = __int_as_float((127 - (alike ? up : lift(s_row[r]))) << 23);
     }
     const float sc = factor(row_scale);
     const int limit = KEYS ? 0 : mine < own ? limit_of(mine) : 0;
