@@ -5,7 +5,8 @@
 
 bool mb_decode_mass_serves(const MbMassArgs& a) {
   const uintptr_t al = reinterpret_cast<uintptr_t>(a.k_cache) | reinterpret_cast<uintptr_t>(a.v_cache) | reinterpret_cast<uintptr_t>(a.q);
-  return a.num_seqs <= kMaxSeqs && !(al & 15) &&
+  // a TMA box begins on 128 bytes of shared memory: rows of 64 bytes come two at least
+  return (a.D > 64 || !a.fp8 || a.block_size % 2 == 0) && a.num_seqs <= kMaxSeqs && !(al & 15) &&
          a.num_blocks * a.block_size < (1ll << 31) && a.table_ld < (1ll << 31);
 }
 

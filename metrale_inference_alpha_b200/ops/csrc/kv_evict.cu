@@ -366,7 +366,7 @@ __global__ void __launch_bounds__(256) evict_move_kernel(const MbEvictArgs a, in
 extern "C" int mb_kv_evict(const MbEvictArgs* given, cudaStream_t stream) {
   if (!given) return MB_ERR_BAD_ARG;
   MbEvictArgs args = *given, *a = &args;
-  if ( a->num_seqs <= 0 || a->num_seqs > 65535 || a->Hkv <= 0 || a->Hkv > 65535 || a->keep <= 0 || a->recent < 0 || a->recent > a->keep || a->max_ctx <= 0 ||
+  if (a->num_seqs <= 0 || a->num_seqs > 65535 || a->Hkv <= 0 || a->Hkv > 65535 || a->keep <= 0 || a->recent < 0 || a->recent > a->keep || a->max_ctx <= 0 ||
       a->block_size <= 0 || a->num_blocks <= 0 || a->row_bytes < 64 || (a->row_bytes & (a->row_bytes - 1)) || !a->mass || !a->mass_out || !a->ctx_len || !a->kept ||
       !a->new_len || !a->first || !a->slots || !a->block_table || !a->dst_table || !a->k_cache || !a->v_cache)
     return MB_ERR_BAD_ARG;
@@ -380,7 +380,7 @@ extern "C" int mb_kv_evict(const MbEvictArgs* given, cudaStream_t stream) {
   const long long heads = (long long)a->Hkv * a->num_seqs;
   cudaError_t e;
   if (a->max_ctx <= kSegment * kMaxCluster) {
-    // 16 rows a thread, in as many CTAs as the chip holds at once; where there are more, up to 64. Fewer take a kernel with less of its loops to pass.
+    // 16 rows a thread, in as many CTAs as the chip's 148 SMs hold at once (two each); where there are more, up to 64. Fewer take a kernel with less of its loops to pass.
     int cluster = 1;
     while (cluster * kSegment < a->max_ctx || (cluster < kMaxCluster && cluster * kThreads * 16 < a->max_ctx && heads * cluster * 2 <= 2 * 148)) cluster *= 2;
     const int per = (a->max_ctx + cluster * kThreads - 1) / (cluster * kThreads);
@@ -395,7 +395,7 @@ extern "C" int mb_kv_evict(const MbEvictArgs* given, cudaStream_t stream) {
   while (16 << bits < a->row_bytes) ++bits;
   if (!a->in_place) {
     const int round = (256 >> bits) * kDeep;
-    return (int)mb::launch_kernel_ex(evict_copy_kernel, dim3(2 * ((held + round - 1) / round), a->Hkv, a->num_seqs), dim3(256), 0, stream, 1, true, *a, bits);
+    return (int)mb::launch_kernel_ex(evict_copy_kernel, dim3(2 * ((held + round - 1) / round), a->Hkv, a->num_seqs), dim3(256), 0, stream, 1, mb_pdl_enabled() != 0, *a, bits);
   }
   static bool configured = false;
   if (!configured) {
@@ -404,7 +404,7 @@ extern "C" int mb_kv_evict(const MbEvictArgs* given, cudaStream_t stream) {
     configured = true;
   }
   const int mine = kRoundB / a->row_bytes;
-  int cluster = 1;
+  int cluster = 1;                                                     // rounds as large as leave the chip (148 SMs) something to do
   while (cluster < kMaxCluster && 2 * heads * cluster < 2 * 148 && cluster * mine < held) cluster *= 2;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(2 * cluster, a->Hkv, a->num_seqs);
@@ -412,12 +412,12 @@ extern "C" int mb_kv_evict(const MbEvictArgs* given, cudaStream_t stream) {
   cfg.dynamicSmemBytes = kRoundB;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = cluster;
-  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cluster;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  cfg.numAttrs = mb_pdl_enabled() ? 2 : 1;
   return (int)cudaLaunchKernelEx(&cfg, evict_move_kernel, (const MbEvictArgs)*a, bits);
 }

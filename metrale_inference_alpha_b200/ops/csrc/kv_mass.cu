@@ -25,7 +25,7 @@ constexpr int kPartTokens = 512, kChunk = 1024;
 // waiting for the other a chunk took three times the latency, and 128 sequences of 129 to 1151 tokens 58 us instead of 53.
 constexpr int kAtOnce = 8;     // query rows whose logits are in registers at once
 
-__global__ void __launch_bounds__(256) mass_join_kernel(const MbMassArgs a, const mbm::DecodeWs w, int part_tokens) {
+__global__ void __launch_bounds__(256, 4) mass_join_kernel(const MbMassArgs a, const mbm::DecodeWs w, int part_tokens) {
   __shared__ float s_lse[64];
   const int G = a.Hq / a.Hkv, chunk = blockIdx.x, h = blockIdx.y, s = blockIdx.z, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const size_t row0 = (size_t)s * a.Hq + h * G;
@@ -122,7 +122,7 @@ int mb_attn_mass(const MbMassArgs* a, cudaStream_t stream) {
   const int rc = mb_decode_mass(*a, w, part, stream);
   if (rc) return rc;
   const int chunks = (a->max_ctx + kChunk - 1) / kChunk;
-  return (int)mb::launch_kernel_ex(mass_join_kernel, dim3(chunks, a->Hkv, a->num_seqs), dim3(256), 0, stream, 1, true, *a, w, part);
+  return (int)mb::launch_kernel_ex(mass_join_kernel, dim3(chunks, a->Hkv, a->num_seqs), dim3(256), 0, stream, 1, mb_pdl_enabled() != 0, *a, w, part);
 }
 
 }  // extern "C"

@@ -617,7 +617,7 @@ int launch(const MbMassArgs& a, const Ws& ws, const CUtensorMap* tm, cudaStream_
   const unsigned magic = G == 1 ? 0 : (unsigned)(((1ull << 32) + G - 1) / G);
   const long long blocks = ((KEYS ? (long long)a.max_ctx : ws.rows) + kHeld - 1) / kHeld * (KEYS ? ws.row_parts : ws.slices);
   if (blocks > 0x7fffffffll) return MB_ERR_TOO_LARGE;
-  return (int)mb::launch_kernel_ex(kern, dim3((unsigned)blocks, a.Hkv, a.num_seqs), dim3(kThreads), Cfg<D>::kSmem, stream, 1, KEYS || !ws.paged, tm[0], tm[1], a, ws,
+  return (int)mb::launch_kernel_ex(kern, dim3((unsigned)blocks, a.Hkv, a.num_seqs), dim3(kThreads), Cfg<D>::kSmem, stream, 1, mb_pdl_enabled() && (KEYS || !ws.paged), tm[0], tm[1], a, ws,
                                    (int)magic);
 }
 
@@ -665,7 +665,7 @@ int mb_prompt_mass(const MbMassArgs* a, cudaStream_t stream) {
   else if (a->D == 128) rc = a->fp8 ? all<128, true>(*a, ws, stream) : all<128, false>(*a, ws, stream);
   else rc = a->fp8 ? all<256, true>(*a, ws, stream) : all<256, false>(*a, ws, stream);
   if (rc || ws.row_parts == 1) return rc;
-  return (int)mb::launch_kernel_ex(observe_join_kernel, dim3((a->max_ctx + 255) / 256, a->Hkv, a->num_seqs), dim3(256), 0, stream, 1, true, *a, ws);
+  return (int)mb::launch_kernel_ex(observe_join_kernel, dim3((a->max_ctx + 255) / 256, a->Hkv, a->num_seqs), dim3(256), 0, stream, 1, mb_pdl_enabled() != 0, *a, ws);
 }
 
 }  // extern "C"

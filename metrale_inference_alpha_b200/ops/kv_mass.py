@@ -148,6 +148,8 @@ def paged_attention_mass(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     where = "paged_attention_mass"
     S, nb, bs, Hkv, D = _check_cache(where, k_cache, v_cache, block_table, ctx_len, mass, max_ctx)
     Hq = _check_queries(where, q, S, Hkv, D)
+    if D == 64 and bs % 2 and k_cache.dtype == torch.uint8:
+        _bad(where, f"an e4m3 cache of head dim 64 has blocks of an even number of tokens, not {bs}")
     _check_rows(where, "mass", mass)
     _check_scales(where, k_cache, scale, k_scale, v_scale)
     _check_places(where, q, k_cache, v_cache, block_table, ctx_len, mass, k_scale, v_scale)

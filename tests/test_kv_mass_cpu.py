@@ -114,6 +114,14 @@ def test_decode_refuses(change):
     assert torch.equal(c["mass"], before)
 
 
+def test_decode_refuses_odd_blocks_of_64_byte_rows():
+    """A copy into shared memory begins on 128 bytes."""
+    for block in (1, 3, 15):
+        with pytest.raises(ValueError, match="even number"):
+            _decode(oracle.case(12, [40], 4, 2, 64, True, block=block))
+        _decode(oracle.case(12, [40], 4, 2, 64, False, block=block))
+
+
 def test_e4m3_caches_want_scales():
     c = oracle.case(8, [40], 4, 2, 64, True)
     for name in ("k_scale", "v_scale"):

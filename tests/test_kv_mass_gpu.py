@@ -65,6 +65,16 @@ def test_decode_block_sizes(block, fp8):
     _within(g["mass"], mass, mtol, "mass")
 
 
+@pytest.mark.parametrize("block,fp8", [(2, True), (6, True), (12, True), (24, True), (1, False), (7, False)])
+@pytest.mark.parametrize("heads,dim", [(4, 64), (20, 64), (6, 256)])
+def test_decode_block_sizes_of_other_heads(block, fp8, heads, dim):
+    c = oracle.case(34, [130, 7, 600, 0, 17], heads, 2, dim, fp8, block=block)
+    want, tol, mass, mtol = oracle.decode(c)
+    g = _cuda(c)
+    _within(_decode(g), want, tol, "outputs")
+    _within(g["mass"], mass, mtol, "mass")
+
+
 @pytest.mark.parametrize("dim,heads,kv_heads", [(64, 8, 2), (128, 10, 2), (256, 8, 1)])
 def test_decode_of_a_long_sequence(dim, heads, kv_heads):
     """More tokens than 32 of the shortest partitions hold."""
@@ -431,6 +441,30 @@ def test_evict_of_nothing():
     k = c["k"].clone()
     kept, length = ops.kv_evict(c["k"], c["v"], c["table"], torch.tensor([0, -4], dtype=torch.int32, device="cuda"), c["mass"], keep=3, recent=1, max_ctx=40)
     assert bool((kept == -1).all()) and not length.any() and _same(c["k"], k) and not c["mass"].any()
+
+
+# ----------------------------------------------------------------------------- far into a large cache
+def test_places_beyond_32_bits():
+    """Blocks at the end of caches of 6.6 GB each: the same bits as from a small cache."""
+    small = _cuda(oracle.case(59, [300, 77], 16, 8, 128, False, new=[40, 40]))
+    far = 200_000
+    big = dict(small)
+    shift = far - small["k"].shape[0]
+    for name in ("k", "v"):
+        big[name] = torch.empty(far, 16, 8, 128, dtype=torch.bfloat16, device="cuda")
+        big[name][shift:] = small[name]
+        big[name][0] = 0                                     # the null block is read, and masked
+    assert big["k"].numel() * 2 > 1 << 32
+    big["table"] = small["table"] + shift
+    big["mass"] = small["mass"].clone()
+    results = []
+    for c in (small, big):
+        one = {**c, "q": c["q"][:2].contiguous()}
+        out = _decode(one)
+        _prompt(c, 0)
+        kept, length = ops.kv_evict(c["k"], c["v"], c["table"], c["ctx"], c["mass"], keep=100, recent=10, max_ctx=c["max_ctx"])
+        results.append((out, c["mass"], kept, length, c["k"][shift if c is big else 0:], c["v"][shift if c is big else 0:]))
+    assert all(_same(a, b) for a, b in zip(*results))
 
 
 # ----------------------------------------------------------------------------- together
