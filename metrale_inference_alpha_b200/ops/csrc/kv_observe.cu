@@ -53,9 +53,10 @@ __device__ __forceinline__ Span span_of(const MbMassArgs& a, int s, int G) {
   return {n, seen * G, (int)start + ql - seen, n - seen};
 }
 
-// Keys of a part of a row, rows of a part of a column: few rows want many parts to fill the chip, many rows do that by themselves.
+// Keys of a part of a row, rows of a part of a column: few rows want many parts to fill the chip, many rows do that by themselves. (512 or 1024 keys,
+// 64 observers: sixteen prompts of 17 to 1151 tokens 48 / 44 us, one of 16000 35 / 40.)
 __host__ __device__ __forceinline__ int key_part(int n, int rows) {
-  const int least = rows <= 512 ? 512 : rows <= 4096 ? 2048 : 8192, even = ((n + kMaxKeyParts - 1) / kMaxKeyParts + 127) & ~127;
+  const int least = rows <= 512 ? (n <= 2048 ? 1024 : 512) : rows <= 4096 ? 2048 : 8192, even = ((n + kMaxKeyParts - 1) / kMaxKeyParts + 127) & ~127;
   return even > least ? even : least;
 }
 __host__ __device__ __forceinline__ int row_part(int rows) {
@@ -69,11 +70,14 @@ __host__ __device__ __forceinline__ int parts_of(int n, int part) { return n <= 
 // too large by; sums of the columns' parts [row parts, seqs * Hkv, columns]
 struct Ws {
   long long rows, cols, tokens;
-  int key_parts, row_parts, slices, paged;   // slices: CTAs that a block of rows is shared out over
+  int key_parts, row_parts, slices, paged, joined;   // slices: CTAs that a block of rows is shared out over; joined: a row's parts are, before the keys pass
   size_t keys, ml, scale, sums, bytes;
 };
 // From this many observed rows on, a bf16 cache's keys are copied too: every tile of them goes by often, and comes as one box instead of eight
 constexpr int kCopyRows = 1024;
+// With more parts of a row than this they are joined by a kernel of its own: every CTA of the keys pass would join them again, for all rows. 64 observers at
+// 16000 bf16 tokens, 16 / 2 heads of 256 (32 parts) 47 -> 35 us, 32 at 8192 e4m3, 40 / 8 of 128 (16) 44 -> 41
+constexpr int kJoin = 4;
 
 inline Ws workspace(int seqs, int Hq, int Hkv, int D, int block_size, int seen, int max_ctx, bool fp8) {
   Ws w;
@@ -86,6 +90,7 @@ inline Ws workspace(int seqs, int Hq, int Hkv, int D, int block_size, int seen, 
   w.key_parts = parts_of(max_ctx, 512) < kMaxKeyParts ? parts_of(max_ctx, 512) : kMaxKeyParts;
   w.row_parts = parts_of((int)w.rows, row_part((int)w.rows));
   w.slices = parts_of(max_ctx, key_part(max_ctx, (int)w.rows));
+  w.joined = w.slices > kJoin;
   const size_t n = (size_t)seqs * Hkv * w.rows;
   w.keys = even((n + 128) * D * 2);
   w.ml = w.keys + (w.paged ? 0 : even((size_t)seqs * w.tokens * Hkv * D * 2));
@@ -445,7 +450,7 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
     fewer_regs<64>();
     if (KEYS && warp < 10) {
       // ---------------------------------------------------------- factors and normalisers of a tile's rows, two a thread
-      const int t = tid - kSums;
+      const int t = tid - kSums, left = ws.joined ? 1 : kparts;
       mb::pdl_wait();
       // the parts of the next tile's normalisers are on their way while this one's are joined
       constexpr int kTake = 4;
@@ -456,7 +461,7 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
         for (int e = 0; e < 2; ++e) {
           const int at = min(begin + tile * kN + t + 64 * e, end - 1);
 #pragma unroll
-          for (int k = 0; k < kTake; ++k) y[e][k] = k < kparts ? ml[(size_t)at * ws.key_parts + k] : make_float2(-INFINITY, 0.f);
+          for (int k = 0; k < kTake; ++k) y[e][k] = k < left ? ml[(size_t)at * ws.key_parts + k] : make_float2(-INFINITY, 0.f);
           if (FP8) yscale[e] = wscale[at];
         }
       };
@@ -468,10 +473,10 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
         for (int e = 0; e < 2; ++e) {
           const int at = begin + tile * kN + t + 64 * e;
           float m = -INFINITY, l = 0.f;
-          for (int i = 0; i < kparts; i += kTake) {
+          for (int i = 0; i < left; i += kTake) {
             if (i > 0) {
 #pragma unroll
-              for (int k = 0; k < kTake; ++k) y[e][k] = i + k < kparts ? ml[(size_t)min(at, end - 1) * ws.key_parts + i + k] : make_float2(-INFINITY, 0.f);
+              for (int k = 0; k < kTake; ++k) y[e][k] = i + k < left ? ml[(size_t)min(at, end - 1) * ws.key_parts + i + k] : make_float2(-INFINITY, 0.f);
             }
 #pragma unroll
             for (int k = 0; k < kTake; ++k) {
@@ -591,6 +596,32 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
   }
 }
 
+// Rows whose keys were cut into parts: {maximum, sum} over them in order, in the place of the first.
+__device__ __forceinline__ float2 joined(const float2* p, int parts) {
+  float m = -INFINITY, l = 0.f;
+  for (int i = 0; i < parts; i += 8) {                       // eight parts' loads in flight
+    float2 y[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) y[k] = i + k < parts ? p[i + k] : make_float2(-INFINITY, 0.f);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float top = fmaxf(m, y[k].x);
+      l = (m == -INFINITY ? 0.f : l * ex2(m - top)) + (y[k].x == -INFINITY ? 0.f : y[k].y * ex2(y[k].x - top));
+      m = top;
+    }
+  }
+  return make_float2(m, l);
+}
+__global__ void __launch_bounds__(128) observe_rows_join_kernel(const MbMassArgs a, const Ws ws) {
+  mb::pdl_launch_dependents();
+  const int h = blockIdx.y, s = blockIdx.z, row = blockIdx.x * 128 + threadIdx.x;
+  const Span x = span_of(a, s, a.Hq / a.Hkv);
+  mb::pdl_wait();
+  if (row >= x.rows) return;
+  float2* ml = reinterpret_cast<float2*>(reinterpret_cast<uint8_t*>(a.ws) + ws.ml) + (((size_t)s * a.Hkv + h) * ws.rows + row) * ws.key_parts;
+  *ml = joined(ml, parts_of(x.n, key_part(x.n, x.rows)));
+}
+
 // Columns whose rows were cut into parts: their sums in order.
 __global__ void __launch_bounds__(256) observe_join_kernel(const MbMassArgs a, const Ws ws) {
   const int h = blockIdx.y, s = blockIdx.z, j = blockIdx.x * 256 + threadIdx.x;
@@ -639,6 +670,9 @@ int all(const MbMassArgs& a, const Ws& ws, cudaStream_t stream) {
     if (e != cudaSuccess) return (int)e;
   }
   rc = launch<D, FP8, false>(a, ws, tm, stream);
+  if (!rc && ws.joined)
+    rc = (int)mb::launch_kernel_ex(observe_rows_join_kernel, dim3((unsigned)((ws.rows + 127) / 128), a.Hkv, a.num_seqs), dim3(128), 0, stream, 1, mb_pdl_enabled() != 0,
+                                   a, ws);
   return rc ? rc : launch<D, FP8, true>(a, ws, tm, stream);
 }
 

