@@ -9,13 +9,17 @@
 //
 // Both operands come by TMA: keys from the cache, 16 tokens a box, or from a copy in the workspace (an e4m3 cache's as f16, any cache's whose blocks are
 // not whole boxes), which a kernel in front makes; query rows of the keys pass from the copy that the rows pass makes of its own (with an e4m3 cache
-// f16, scaled by a power of two per row). A first form had four warps gather and widen tiles on the way into shared memory, every CTA the same ones: that
+// f16, scaled by a power of two, one for 128 rows that are alike, else one per row). A first form had four warps gather and widen tiles on the way into shared memory, every CTA the same ones: that
 // took the issue slots of the exponentials, 4096 observers at 8192 e4m3 tokens 819 us.
 //
 // Roles (384 threads, two CTAs per SM, so that one's beginning and end are under the other's exponentials): warps 0-3 and 4-7 own 128 lanes each and half
 // of a tile's columns; warps 8 and 9 bring the rows' normalisers (keys pass), warp 10 issues the products into two accumulators, so that products run
 // under the exponentials, warp 11 the copies. With 256 lanes a CTA and one of them per SM, 4096 observers at 8192 e4m3 tokens took 766 us, sixteen prompts
 // of 17 to 1151 tokens under 64 observers 55.
+//
+// Bound by its exponentials, two a logit at 16 a cycle and SM: 4096 observers at 8192 e4m3 tokens, 40 / 8 heads of 128, take 717 us (1.0 G logits a
+// pass, 2.8 T exponentials a second; the special function units 79 and 70 % busy, the tensor pipe 39 and 33), 32 observers 41. At dim 256 products from
+// shared memory count as much: 2 prompts of 1001 and 1531 at up to 4431 tokens, 16 / 2 heads, 164 us. (B200, in a graph.)
 //
 // Long rows and long columns are cut into parts, by rules on the sequence's own lengths alone, and joined in order: every output has one writer and
 // every sum one order.
