@@ -223,6 +223,8 @@ def kv_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Te
     ``max_ctx``; without it ``mass`` does. A length beyond ``max_ctx`` or a block that the cache does not have sets the status word."""
     where = "kv_evict"
     S, nb, bs, Hkv, D = _check_cache(where, k_cache, v_cache, block_table, ctx_len, mass, max_ctx)
+    if abs(k_cache.data_ptr() - v_cache.data_ptr()) < k_cache.numel() * k_cache.element_size():
+        _bad(where, "k_cache and v_cache share memory")     # they move side by side: the one would write rows that the other has not read
     if keep < 1 or recent < 0 or recent > keep:
         _bad(where, f"keep {keep} is at least 1 and recent {recent} at most keep")
     mo = mass

@@ -159,6 +159,20 @@ def test_evict_refuses(change):
     assert torch.equal(c["k"].nan_to_num(7.0), k.nan_to_num(7.0))
 
 
+def test_evict_refuses_keys_and_values_that_share_memory():
+    """They move side by side: the one would write rows that the other has not read."""
+    c = oracle.case(13, [40, 33], 4, 2, 64, False)
+    k = c["k"].nan_to_num(0.0)
+    both = torch.cat([k, k])
+    for v in (k, both[1:1 + len(k)]):
+        source = k if v is k else both[:len(k)]
+        before = source.clone()
+        with pytest.raises(ValueError, match="kv_evict: k_cache and v_cache share memory"):
+            ops.kv_evict(source, v, c["table"], c["ctx"], c["mass"], keep=8, recent=2, max_ctx=40)
+        assert torch.equal(source, before)
+    ops.kv_evict(both[:len(k)], both[len(k):], c["table"], c["ctx"], c["mass"], keep=8, recent=2, max_ctx=40)      # next to each other is not shared
+
+
 def test_nothing_to_do():
     c = oracle.case(11, [4], 2, 1, 64, False)
     none = dict(table=c["table"][:0], ctx=c["ctx"][:0], mass=c["mass"][:0])
