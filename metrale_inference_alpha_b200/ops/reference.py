@@ -357,7 +357,7 @@ def kv_evict(k_cache, v_cache, block_table, ctx_len, mass, keep: int, recent: in
     dst = block_table if dst_table is None else dst_table
     kept = torch.full((S, Hkv, keep), -1, dtype=torch.int32)
     for s in range(S):
-        n = int(ctx_len[s])
+        n = max(int(ctx_len[s]), 0)
         m = min(n, keep)
         to = torch.arange(m)
         to = dst[s].long()[to // bs] * bs + to % bs
@@ -375,7 +375,7 @@ def kv_evict(k_cache, v_cache, block_table, ctx_len, mass, keep: int, recent: in
                 flat[to, h] = flat[at, h]
             mass_out[s, h, :m] = x[idx]
             mass_out[s, h, m:max_ctx] = 0.0
-    return kept, ctx_len.clamp(max=keep)
+    return kept, ctx_len.clamp(0, keep)
 
 
 # ----------------------------------------------------------------------------- gated delta net

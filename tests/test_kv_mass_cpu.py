@@ -173,6 +173,17 @@ def test_evict_refuses_keys_and_values_that_share_memory():
     ops.kv_evict(both[:len(k)], both[len(k):], c["table"], c["ctx"], c["mass"], keep=8, recent=2, max_ctx=40)      # next to each other is not shared
 
 
+def test_lengths_below_zero_are_zero():
+    c = oracle.case(14, [40, 33], 4, 2, 64, False, new=[1, 1])
+    c["ctx"][0] = -3
+    before = c["mass"].clone()
+    _prompt(c, 1)
+    c["q"] = c["q"][:2]
+    assert not _decode(c)[0].any() and torch.equal(c["mass"][0], before[0])
+    kept, length = ops.kv_evict(c["k"], c["v"], c["table"], c["ctx"], c["mass"], keep=8, recent=2, max_ctx=40)
+    assert length.tolist() == [0, 8] and length.dtype == torch.int32 and bool((kept[0] == -1).all()) and not c["mass"][0].any()
+
+
 def test_nothing_to_do():
     c = oracle.case(11, [4], 2, 1, 64, False)
     none = dict(table=c["table"][:0], ctx=c["ctx"][:0], mass=c["mass"][:0])
