@@ -67,6 +67,8 @@ def _check_cache(where, k_cache, v_cache, block_table, ctx_len, mass, max_ctx) -
         _bad(where, "v_cache has the shape and type of k_cache")
     if not k_cache.is_contiguous() or (v_cache is not None and not v_cache.is_contiguous()):
         _bad(where, "caches are contiguous")
+    if bs == 0 or Hkv == 0 or (nb == 0 and max_ctx > 0):
+        _bad(where, f"a cache of {nb} blocks of {bs} tokens and {Hkv} kv heads holds nothing")
     if D not in HEAD_DIMS:
         _bad(where, f"head dim {D}, one of {HEAD_DIMS} is served")
     if ctx_len.dtype != torch.int32 or ctx_len.dim() != 1 or not ctx_len.is_contiguous():
@@ -188,6 +190,8 @@ def prompt_mass(q: torch.Tensor, k_cache: torch.Tensor, block_table: torch.Tenso
             _bad(where, "q_start and q_len are int32 [sequences]")
     if last < 0 or max_q_len < 0:
         _bad(where, "last and max_q_len are not negative")
+    if max_q_len > 1 << 30:
+        _bad(where, "max_q_len is at most 2^30")
     _check_rows(where, "mass", mass)
     _check_scales(where, k_cache, scale, k_scale)
     _check_places(where, q, k_cache, block_table, q_start, q_len, ctx_len, mass, k_scale)
@@ -225,8 +229,8 @@ def kv_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Te
     S, nb, bs, Hkv, D = _check_cache(where, k_cache, v_cache, block_table, ctx_len, mass, max_ctx)
     if abs(k_cache.data_ptr() - v_cache.data_ptr()) < k_cache.numel() * k_cache.element_size():
         _bad(where, "k_cache and v_cache share memory")     # they move side by side: the one would write rows that the other has not read
-    if keep < 1 or recent < 0 or recent > keep:
-        _bad(where, f"keep {keep} is at least 1 and recent {recent} at most keep")
+    if keep < 1 or keep > 1 << 30 or recent < 0 or recent > keep:
+        _bad(where, f"keep {keep} is from 1 to 2^30 and recent {recent} at most keep")
     mo = mass
     if mass_out is not None:
         mo, m = mass_out, mass_out.shape

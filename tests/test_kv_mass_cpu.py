@@ -184,6 +184,23 @@ def test_lengths_below_zero_are_zero():
     assert length.tolist() == [0, 8] and length.dtype == torch.int32 and bool((kept[0] == -1).all()) and not c["mass"][0].any()
 
 
+def test_caches_without_heads_or_rows_and_sizes_beyond_32_bits_are_refused():
+    c = oracle.case(15, [40, 33], 4, 2, 64, False, new=[1, 1])
+    none = dict(k=c["k"][:, :, :0].contiguous(), v=c["v"][:, :, :0].contiguous(), mass=c["mass"][:, :0])
+    with pytest.raises(ValueError, match="paged_attention_mass"):
+        _decode({**c, **none, "q": c["q"][:2]})
+    with pytest.raises(ValueError, match="prompt_mass"):
+        _prompt({**c, **none}, 1)
+    with pytest.raises(ValueError, match="paged_attention_mass"):
+        _decode({**c, "k": c["k"][:, :0].contiguous(), "v": c["v"][:, :0].contiguous(), "q": c["q"][:2], "max_ctx": 0})
+    with pytest.raises(ValueError, match="paged_attention_mass"):
+        _decode({**c, "k": c["k"][:0], "v": c["v"][:0], "q": c["q"][:2]})
+    with pytest.raises(ValueError, match="prompt_mass"):
+        ops.prompt_mass(c["q"], c["k"], c["table"], c["q_start"], c["q_len"], c["ctx"], c["mass"], max_q_len=1 << 31, max_ctx=40, scale=1.0, last=1)
+    with pytest.raises(ValueError, match="kv_evict"):
+        ops.kv_evict(c["k"], c["v"], c["table"], c["ctx"], c["mass"], keep=1 << 31, recent=2, max_ctx=40)
+
+
 def test_nothing_to_do():
     c = oracle.case(11, [4], 2, 1, 64, False)
     none = dict(table=c["table"][:0], ctx=c["ctx"][:0], mass=c["mass"][:0])
