@@ -443,6 +443,28 @@ def test_evict_of_nothing():
     assert bool((kept == -1).all()) and not length.any() and _same(c["k"], k) and not c["mass"].any()
 
 
+@pytest.mark.parametrize("fp8", [False, True])
+def test_sequences_that_share_a_table(fp8):
+    """A table that is one row for all (stride 0), its blocks read by every sequence and cut into blocks of their own: bits as from a table a sequence."""
+    S, n, bs = 3, 150, 16
+    c = _cuda(oracle.case(60, [n] * S, 8, 2, 128, fp8, block=bs, new=[20] * S))
+    k0, v0 = c["k"], c["v"]
+    one = c["table"][:1].clone()
+    spare = torch.zeros(S * 4, *k0.shape[1:], dtype=k0.dtype, device="cuda")
+    own = (len(k0) + torch.arange(S * 4, dtype=torch.int32, device="cuda")).view(S, 4)
+    got = []
+    for table in (one.expand(S, -1), one.repeat(S, 1)):
+        d = {**c, "k": torch.cat([k0, spare]), "v": torch.cat([v0, spare]), "table": table, "mass": c["mass"].clone()}
+        _prompt(d, 7)
+        out = _decode({**d, "q": d["q"][:S].contiguous()})
+        kept, length = ops.kv_evict(d["k"], d["v"], table, d["ctx"], d["mass"], keep=60, recent=5, max_ctx=n, dst_table=own)
+        assert _same(d["k"][:len(k0)], k0) and _same(d["v"][:len(v0)], v0) and length.tolist() == [60] * S
+        got.append((out, d["mass"], kept, d["k"], d["v"]))
+    assert table.stride(0) and one.expand(S, -1).stride(0) == 0
+    for x, y in zip(*got):
+        assert _same(x, y)
+
+
 # ----------------------------------------------------------------------------- far into a large cache
 def test_places_beyond_32_bits():
     """Blocks at the end of caches of 6.6 GB each: the same bits as from a small cache."""
