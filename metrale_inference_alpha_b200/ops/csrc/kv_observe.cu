@@ -331,8 +331,11 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
       ++mine_part;
       flush_at += kp;
     };
+    // Columns that count for any lane of this warp end here; the others' weights are zeros, whose exponentials few rows would pay for (160 rows of 5 heads: a
+    // block of 128 and one of 32).
+    const int reach = KEYS ? (at0 + (warp & 3) * 32 < own ? end : 0) : min(end, __reduce_max_sync(0xffffffffu, limit));
     for (int t = 0; t < tiles; ++t) {
-      const int b = t & 1;
+      const int b = t & 1, used = min(reach - (begin + t * kN + half * kCols), kCols);
       ok = mb::mbar_wait(&s_full[b], (t >> 1) & 1, a.status, MB_ST_TIMEOUT_MMA);
       if (KEYS) ok = ok && mb::mbar_wait(&info_full[t % kInfo], (t / kInfo) & 1, a.status, MB_ST_TIMEOUT_TMA);
       if (!__all_sync(0xffffffffu, ok)) {
@@ -340,16 +343,24 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
         break;
       }
       mb::tc_fence_after();
+      auto taken = [&](uint64_t* bar) {
+        __syncwarp();
+        if (lane == 0) mb::mbar_arrive(bar);
+      };
+      if (used <= 0) {
+        mb::tc_fence_before();
+        taken(&s_free[b]);
+        if (KEYS) taken(&info_free[t % kInfo]);
+      }
       // 32 columns at a time: the code of a tile is half as long, which a short call waits for from L2
 #pragma unroll 1
-      for (int c0 = 0; c0 < kCols; c0 += kW) {
+      for (int c0 = 0; c0 < used; c0 += kW) {
         float z[kW];
         mb::tmem_ld32_async(tS + b * kN + c0, z);
         mb::tmem_ld_wait(z);
-        if (c0 + kW == kCols) {
+        if (c0 + kW >= used) {
           mb::tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mb::mbar_arrive(&s_free[b]);       // the accumulator is in registers
+          taken(&s_free[b]);                                // the accumulator is in registers
         }
         const int from = begin + t * kN + half * kCols + c0;
         float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
@@ -390,10 +401,7 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
             add([&](int) { return same; });
           }
           l_run += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-          if (c0 + kW == kCols) {
-            __syncwarp();
-            if (lane == 0) mb::mbar_arrive(&info_free[t % kInfo]);
-          }
+          if (c0 + kW >= used) taken(&info_free[t % kInfo]);
         } else {
           const int seen = min(limit, end) - from;             // columns in front of this one are visible
           if (!__all_sync(0xffffffffu, seen >= kW)) {
