@@ -158,6 +158,7 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
   __shared__ __align__(16) float s_lse[kInfo][kN];           // keys pass: the query rows' normalisers, negative, and their factors
   __shared__ __align__(16) float s_factor[KEYS && FP8 ? kInfo : 1][kN];
   __shared__ __align__(8) int s_alike[KEYS && FP8 ? kInfo : 1][4];         // 32 rows' factors are those of the first of 64
+  __shared__ int s_nan[2];                                   // keys pass: the last row whose normaliser is not a number, of each of two warps' rows
   __shared__ int2 s_top[kSums / 32];                         // rows pass, e4m3: the largest exponent of a row's largest element, and the smallest
   const int h = blockIdx.y, s = blockIdx.z, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int G = a.Hq / a.Hkv;
@@ -242,6 +243,7 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
       mb::mbar_init(&s_full[i], 1);
       mb::mbar_init(&s_free[i], kSums / 32);
     }
+    s_nan[0] = s_nan[1] = -1;
     mb::mbar_fence_init();
     mb::tma_prefetch_desc(&tmK);
     if (KEYS) mb::tma_prefetch_desc(&tmQ);
@@ -445,6 +447,8 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
       if (!KEYS && begin + (t + 1) * kN == flush_at) flush();
     }
     if constexpr (KEYS) {
+      const int nan = max(s_nan[0], s_nan[1]);               // written in front of the last tile's normalisers
+      if (nan >= 0 && mine < limit_of(nan)) l_run = NAN;
       if (half) s_half[r].y = l_run;
       asm volatile("bar.sync 1, 256;" ::: "memory");
       if (!half && mine < own) {
@@ -463,6 +467,7 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
     if (KEYS && warp < 10) {
       // ---------------------------------------------------------- factors and normalisers of a tile's rows, two a thread
       const int t = tid - kSums, left = ws.joined ? 1 : kparts;
+      int nan = -1;
       mb::pdl_wait();
       // the parts of the next tile's normalisers are on their way while this one's are joined
       constexpr int kTake = 4;
@@ -499,7 +504,14 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
           }
           f[e] = factor(yscale[e]);
           lse[e] = at < end && l != 0.f ? m + log2f(l) : INFINITY;       // rows behind the last one and rows without weight add nothing
+          // An infinite query's is NaN, which the -inf of a mask would not survive. Its row adds nothing here; since later rows see more, the last such row
+          // says which keys have no number in the end.
+          if (lse[e] != lse[e]) {
+            nan = at;
+            lse[e] = INFINITY;
+          }
         }
+        nan = __reduce_max_sync(0xffffffffu, nan);
         const bool ok = mb::mbar_wait(&info_free[slot], ((tile / kInfo) & 1) ^ 1, a.status, MB_ST_TIMEOUT_EPI);
         if (!__all_sync(0xffffffffu, ok)) break;
 #pragma unroll
@@ -507,6 +519,7 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
           s_lse[slot][t + 64 * e] = -lse[e];
           if constexpr (FP8) s_factor[slot][t + 64 * e] = f[e];
         }
+        if (lane == 0) s_nan[warp & 1] = nan;
         if constexpr (FP8) {
           asm volatile("bar.sync 2, 64;" ::: "memory");
 #pragma unroll

@@ -296,6 +296,23 @@ def test_prompt_of_a_query_that_is_not_a_number(fp8):
     assert not g["mass"].isnan().any()
 
 
+@pytest.mark.parametrize("value", [math.inf, -math.inf])
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(8, 2, 128), (1, 1, 64), (4, 2, 256)])
+def test_prompt_of_an_infinite_query(heads, kv_heads, dim, fp8, value):
+    """Its row has no weights that are numbers; what it does not see keeps those of the rows beside it."""
+    c = oracle.case(61, [200, 100], heads, kv_heads, dim, fp8, new=[100, 100])
+    want, tol = oracle.prompt(c, 0)
+    c["q"][20, 0, 3] = value                                 # sequence 0, sees the first 121 tokens; head 0 is of kv head 0
+    g = _cuda(c)
+    _prompt(g, 0)
+    assert g["mass"][0, 0, :121].isnan().all()
+    got = g["mass"].clone()
+    got[0, 0, :121] = want[0, 0, :121] = 0
+    assert not got.isnan().any()
+    _within(got, want, tol, "mass")
+
+
 def test_prompt_in_a_graph_beside_another():
     cs = [_cuda(oracle.case(45 + i, ctx, 8, 2, 128, False, new=new)) for i, (ctx, new) in enumerate((([900, 600], [100, 600]), ([1200, 30, 256], [40, 30, 256])))]
     start = [c["mass"].clone() for c in cs]
