@@ -3,8 +3,9 @@
 //
 // The normaliser of a row is known when all of its keys are done, so the logits are computed twice:
 //   rows pass   128 query rows stay in shared memory, tiles of keys go by; a thread owns a row and keeps its maximum and sum
-//   keys pass   128 keys stay, tiles of query rows go by; a thread owns a key and adds up 2^(z - normaliser of the row)
-// Both are the same kernel with the operands exchanged: what a thread owns is a lane of the accumulator in tensor memory, so that neither pass
+//   keys pass   128 keys stay, tiles of query rows go by; a thread owns a key and adds up 2^(z - normaliser of the row). Where there are few rows these
+//               stay and blocks of keys go by
+// They are the same kernel with the operands exchanged: what a thread owns is a lane of the accumulator in tensor memory, so that neither pass
 // sums across lanes. Query rows of a kv head are numbered token * G + head of the group, as in attention_rows.cu.
 //
 // Both operands come by TMA: keys from the cache, 16 tokens a box, or from a copy in the workspace (an e4m3 cache's as f16, any cache's whose blocks are
@@ -74,14 +75,20 @@ __host__ __device__ __forceinline__ int parts_of(int n, int part) { return n <= 
 // too large by; sums of the columns' parts [row parts, seqs * Hkv, columns]
 struct Ws {
   long long rows, cols, tokens;
-  int key_parts, row_parts, slices, paged, joined;   // slices: CTAs that a block of rows is shared out over; joined: a row's parts are, before the keys pass
+  int key_parts, row_parts, slices, paged, joined, few, each;   // slices: CTAs that a block of rows is shared out over; joined: a row's parts are, before the keys pass;
+                                                     // few: tiles of rows that stay in a CTA of the keys pass, where keys go by, `each` blocks of them; else 0
   size_t keys, ml, scale, sums, bytes;
 };
 // From this many observed rows on, a bf16 cache's keys are copied too: every tile of them goes by often, and comes as one box instead of eight
 constexpr int kCopyRows = 1024;
 // With more parts of a row than this they are joined by a kernel of its own: every CTA of the keys pass would join them again, for all rows. 64 observers at
-// 16000 bf16 tokens, 16 / 2 heads of 256 (32 parts) 47 -> 35 us, 32 at 8192 e4m3, 40 / 8 of 128 (16) 44 -> 41
-constexpr int kJoin = 4;
+// 16000 bf16 tokens, 16 / 2 heads of 256 (32 parts) 47 -> 35 us, 32 at 8192 e4m3, 40 / 8 of 128 (16) 44 -> 41. CTAs with few rows are fewer and join more
+// themselves: 8 prompts of 4000 to 8192 tokens, 128 rows (16 parts) 80 -> 71, one of 32768, 160 rows (32 parts) 65.5 -> 63.2 with the kernel.
+constexpr int kJoin = 4, kFewJoin = 16;
+// Up to so many tiles of 128 rows stay in a CTA of the keys pass while keys go by, two at 64 and 128 dims and one at 256, which shared memory holds beside a
+// ring. With a CTA a block of keys, which brings them and their normalisers each time: 32 at 8192 e4m3 34 us instead of 31, 8 prompts of 4000 to 8192, 128
+// rows 118 instead of 71, one of 32768, 160 rows 85 instead of 63. The sums and their order are the same.
+constexpr int kFewCtas = 2 * 148;                          // as many as the chip holds at once (148: one of 32768 81 us, 592: 69)
 
 inline Ws workspace(int seqs, int Hq, int Hkv, int D, int block_size, int seen, int max_ctx, bool fp8) {
   Ws w;
@@ -94,7 +101,10 @@ inline Ws workspace(int seqs, int Hq, int Hkv, int D, int block_size, int seen, 
   w.key_parts = parts_of(max_ctx, 512) < kMaxKeyParts ? parts_of(max_ctx, 512) : kMaxKeyParts;
   w.row_parts = parts_of((int)w.rows, row_part((int)w.rows));
   w.slices = parts_of(max_ctx, key_part(max_ctx, (int)w.rows));
-  w.joined = w.slices > kJoin;
+  w.few = w.rows <= (D == 256 ? kHeld : 2 * kHeld) ? (int)((w.rows + kHeld - 1) / kHeld) : 0;
+  w.joined = w.slices > (w.few ? kFewJoin : kJoin);
+  const long long units = (long long)seqs * Hkv * ((max_ctx + kHeld - 1) / kHeld);
+  w.each = (int)((units + kFewCtas - 1) / kFewCtas);
   const size_t n = (size_t)seqs * Hkv * w.rows;
   w.keys = even((n + 128) * D * 2);
   w.ml = w.keys + (w.paged ? 0 : even((size_t)seqs * w.tokens * Hkv * D * 2));
@@ -143,18 +153,27 @@ struct Cfg {
   static constexpr uint32_t kCols = 2 * kN;                  // two accumulators
 };
 
-template <int D, bool FP8, bool KEYS>
+// stages of a ring beside few rows' tiles that stay; two tiles go over a block of keys twice, which the ring then holds whole
+__host__ __device__ constexpr int few_stages(int D, int tiles) { return D == 256 || (D == 128 && tiles == 2) ? 2 : 4; }
+template <int D>
+constexpr int few_smem(int tiles) { return tiles * Cfg<D>::kHeldB + few_stages(D, tiles) * Cfg<D>::kChunkB + 1024; }
+
+enum Pass { kRowsPass, kKeysPass, kFewPass };
+
+template <int D, bool FP8, Pass PASS>
 __global__ void __launch_bounds__(kThreads, 2)
 observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmQ, const MbMassArgs a, const Ws ws, int g_magic) {
   using C = Cfg<D>;
-  constexpr int kN = C::kN, kStages = C::kStages, kChunks = C::kChunks;
+  constexpr bool KEYS = PASS != kRowsPass, FEW = PASS == kFewPass;        // a thread owns a key; and these go by
+  constexpr int kN = C::kN, kMost = FEW ? 4 : C::kStages, kChunks = C::kChunks;
+  const int kStages = FEW ? few_stages(D, ws.few) : C::kStages;
   extern __shared__ __align__(16) uint8_t smem_raw[];
   uint8_t* sHeld = smem_raw + ((1024u - (mb::smem_u32(smem_raw) & 1023u)) & 1023u);   // D / 64 spans x [128 rows x 128 B]
-  uint8_t* sRing = sHeld + C::kHeldB;                        // kStages x [kN rows x 128 B]
-  __shared__ __align__(8) uint64_t held_full, full[kStages], empty[kStages], info_full[kInfo], info_free[kInfo], s_full[2], s_free[2];
+  uint8_t* sRing = sHeld + (FEW ? ws.few : 1) * C::kHeldB;                        // kStages x [kN rows x 128 B]
+  __shared__ __align__(8) uint64_t held_full, full[kMost], empty[kMost], info_full[kInfo], info_free[kInfo], s_full[2], s_free[2];
   __shared__ uint32_t s_tmem;
   __shared__ int s_row[kHeld];                                 // rows pass, e4m3: the exponent of a row's largest element
-  __shared__ float2 s_half[kHeld];                             // sums of the second half of the columns
+  __shared__ float2 s_half[FEW ? 2 : 1][kHeld];                           // sums of the second half of the columns
   __shared__ __align__(16) float s_lse[kInfo][kN];           // keys pass: the query rows' normalisers, negative, and their factors
   __shared__ __align__(16) float s_factor[KEYS && FP8 ? kInfo : 1][kN];
   __shared__ __align__(8) int s_alike[KEYS && FP8 ? kInfo : 1][4];         // 32 rows' factors are those of the first of 64
@@ -170,14 +189,17 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
   // A column's parts are a CTA each. So are a row's where the call's longest portion has as many; shorter portions, whose rows have more of them, share
   // `slices` CTAs out.
   const int slices = KEYS ? ws.row_parts : ws.slices, blocks = gridDim.x / slices, share = KEYS ? 1 : (kparts + slices - 1) / slices;
-  const int part = blockIdx.x / blocks * share, at0 = (KEYS ? (int)blockIdx.x % blocks : blocks - 1 - (int)blockIdx.x % blocks) * kHeld;   // the longest first
+  const int part = FEW ? 0 : blockIdx.x / blocks * share, at0 = FEW ? blockIdx.x * ws.each * kHeld : (KEYS ? (int)blockIdx.x % blocks : blocks - 1 - (int)blockIdx.x % blocks) * kHeld;   // the longest first
   const int own = KEYS ? x.n : x.rows;
   if (part >= (KEYS ? rparts : kparts) || at0 >= own || x.rows == 0 || x.n == 0) {
     mb::pdl_wait();                                       // a grid ends behind the one in front of it, even where it does nothing
     return;
   }
   int begin, end;
-  if constexpr (KEYS) {
+  if constexpr (FEW) {
+    begin = 0;
+    end = x.rows;
+  } else if constexpr (KEYS) {
     // the first row that sees the first of these keys
     const int first = max(0, at0 - x.past) * G;
     begin = max(part * rp, first & ~(kN - 1));
@@ -186,7 +208,9 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
     begin = part * kp;
     end = min(min(x.n, begin + share * kp), limit_of(min(x.rows, at0 + kHeld) - 1));
   }
-  const int tiles = end > begin ? (end - begin + kN - 1) / kN : 0;
+  // few rows: their tiles one after the other for each block of keys
+  const int turns = FEW ? (x.rows + kN - 1) / kN : 1, more = turns - 1;
+  const int tiles = FEW ? min(ws.each, (own - at0 + kHeld - 1) / kHeld) * turns : end > begin ? (end - begin + kN - 1) / kN : 0;
   const size_t row0 = ((size_t)s * a.Hkv + h) * ws.rows;     // of the workspace's rows
   float2* ml = reinterpret_cast<float2*>(reinterpret_cast<uint8_t*>(a.ws) + ws.ml) + row0 * ws.key_parts;
   uint4* wq = reinterpret_cast<uint4*>(a.ws) + row0 * (D / 8);
@@ -231,7 +255,7 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
   }
   if (tid == kThreads - 1) {
     mb::mbar_init(&held_full, KEYS ? 1 : kSums / 32);
-    for (int i = 0; i < kStages; ++i) {
+    for (int i = 0; i < kMost; ++i) {
       mb::mbar_init(&full[i], 1);
       mb::mbar_init(&empty[i], 1);
     }
@@ -261,7 +285,8 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
 
   if (warp < 8) {
     more_regs<88>();
-    const int half = warp >> 2, r = tid & 127, mine = at0 + r;
+    const int half = warp >> 2, r = tid & 127;
+    int mine = at0 + r;
     constexpr int kCols = kN / 2, kW = 32;                   // columns of a thread, and of a round
     float row_scale = 1.f;                                   // what this thread's row's scores are too large by
     if constexpr (!KEYS) {
@@ -319,10 +344,10 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
     // rows pass: a part of a row's keys is done; the halves of the columns are joined
     int mine_part = part, flush_at = (part + 1) * kp;
     auto flush = [&] {
-      if (half) s_half[r] = make_float2(m_run, l_run);
+      if (half) s_half[0][r] = make_float2(m_run, l_run);
       asm volatile("bar.sync 1, 256;" ::: "memory");
       if (!half && mine < own) {
-        const float2 y = s_half[r];
+        const float2 y = s_half[0][r];
         const float top = fmaxf(m_run, y.x);
         const float l = (m_run == -INFINITY ? 0.f : l_run * ex2(m_run - top)) + (y.x == -INFINITY ? 0.f : y.y * ex2(y.x - top));
         ml[(size_t)mine * ws.key_parts + mine_part] = make_float2(top, l);
@@ -335,11 +360,15 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
     };
     // Columns that count for any lane of this warp end here; the others' weights are zeros, whose exponentials few rows would pay for (160 rows of 5 heads: a
     // block of 128 and one of 32).
-    const int reach = KEYS ? (at0 + (warp & 3) * 32 < own ? end : 0) : min(end, __reduce_max_sync(0xffffffffu, limit));
+    int reach = KEYS ? (at0 + (warp & 3) * 32 < own ? end : 0) : min(end, __reduce_max_sync(0xffffffffu, limit));
+    float old = 0.f;                                         // few rows: the mass that is added to
+    int blocks_left = FEW ? tiles / turns : 0;
     for (int t = 0; t < tiles; ++t) {
-      const int b = t & 1, used = min(reach - (begin + t * kN + half * kCols), kCols);
+      const int at_row = FEW ? (t & more) * kN : begin + t * kN, slot = FEW ? t & more : t % kInfo;
+      const int b = t & 1, used = min(reach - (at_row + half * kCols), kCols);
+      if (FEW && (t & more) == 0 && !half && mine < own) old = a.mass[s * a.mass_seq + h * a.mass_head + mine];
       ok = mb::mbar_wait(&s_full[b], (t >> 1) & 1, a.status, MB_ST_TIMEOUT_MMA);
-      if (KEYS) ok = ok && mb::mbar_wait(&info_full[t % kInfo], (t / kInfo) & 1, a.status, MB_ST_TIMEOUT_TMA);
+      if (KEYS) ok = ok && mb::mbar_wait(&info_full[slot], FEW ? 0 : (t / kInfo) & 1, a.status, MB_ST_TIMEOUT_TMA);
       if (!__all_sync(0xffffffffu, ok)) {
         ok = false;
         break;
@@ -352,7 +381,7 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
       if (used <= 0) {
         mb::tc_fence_before();
         taken(&s_free[b]);
-        if (KEYS) taken(&info_free[t % kInfo]);
+        if (KEYS && !FEW) taken(&info_free[slot]);
       }
       // 32 columns at a time: the code of a tile is half as long, which a short call waits for from L2
 #pragma unroll 1
@@ -364,7 +393,7 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
           mb::tc_fence_before();
           taken(&s_free[b]);                                // the accumulator is in registers
         }
-        const int from = begin + t * kN + half * kCols + c0;
+        const int from = at_row + half * kCols + c0;
         float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
         if constexpr (KEYS) {
           // these rows' first one sees the least: all of these keys, or a row each is asked. Behind the last row is whatever memory holds.
@@ -373,7 +402,7 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
             for (int i = 0; i < kW; ++i)
               if (mine >= limit_of(from + i) || from + i >= end) z[i] = -INFINITY;
           }
-          const float4* lse = reinterpret_cast<const float4*>(&s_lse[t % kInfo][half * kCols + c0]);
+          const float4* lse = reinterpret_cast<const float4*>(&s_lse[slot][half * kCols + c0]);
           auto add = [&](auto factors) {
 #pragma unroll
             for (int i = 0; i < kW / 4; ++i) {
@@ -389,8 +418,8 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
             }
           };
           if constexpr (FP8) {
-            const float4* own4 = reinterpret_cast<const float4*>(&s_factor[t % kInfo][half * kCols + c0]);
-            const int2 alike = *reinterpret_cast<const int2*>(&s_alike[t % kInfo][half * 2]);
+            const float4* own4 = reinterpret_cast<const float4*>(&s_factor[slot][half * kCols + c0]);
+            const int2 alike = *reinterpret_cast<const int2*>(&s_alike[slot][half * 2]);
             if (alike.x && alike.y) {
               const float f = own4->x;
               const float4 same = make_float4(f, f, f, f);
@@ -403,7 +432,7 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
             add([&](int) { return same; });
           }
           l_run += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-          if (c0 + kW >= used) taken(&info_free[t % kInfo]);
+          if (!FEW && c0 + kW >= used) taken(&info_free[slot]);
         } else {
           const int seen = min(limit, end) - from;             // columns in front of this one are visible
           if (!__all_sync(0xffffffffu, seen >= kW)) {
@@ -445,20 +474,33 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
         }
       }
       if (!KEYS && begin + (t + 1) * kN == flush_at) flush();
+      if (FEW && (t & more) == more) {
+        // a block of keys is done; the other half's sums have two places, so that one barrier a block is enough
+        const int nan = max(s_nan[0], s_nan[1]), place = (t / turns) & 1;
+        if (nan >= 0 && mine < limit_of(nan)) l_run = NAN;
+        if (half) s_half[place][r].y = l_run;
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        if (!half && mine < own) a.mass[s * a.mass_seq + h * a.mass_head + mine] = old + (l_run + s_half[place][r].y);
+        --blocks_left;
+        l_run = 0.f;
+        mine += kHeld;
+        reach = mine - lane < own ? end : 0;
+      }
     }
-    if constexpr (KEYS) {
+    for (; blocks_left > 0; --blocks_left) asm volatile("bar.sync 1, 256;" ::: "memory");    // a wait ran out: the other warps' barriers count this one
+    if constexpr (KEYS && !FEW) {
       const int nan = max(s_nan[0], s_nan[1]);               // written in front of the last tile's normalisers
       if (nan >= 0 && mine < limit_of(nan)) l_run = NAN;
-      if (half) s_half[r].y = l_run;
+      if (half) s_half[0][r].y = l_run;
       asm volatile("bar.sync 1, 256;" ::: "memory");
       if (!half && mine < own) {
-        l_run += s_half[r].y;
+        l_run += s_half[0][r].y;
         if (ws.row_parts > 1)
           reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(a.ws) + ws.sums)[((size_t)part * a.num_seqs * a.Hkv + (size_t)s * a.Hkv + h) * ws.cols + mine] = l_run;
         else
           a.mass[s * a.mass_seq + h * a.mass_head + mine] += l_run;
       }
-    } else {
+    } else if constexpr (!KEYS) {
       while (mine_part < min(part + share, kparts)) flush();   // parts behind what these rows see are empty
     }
     mb::tc_fence_before();
@@ -470,7 +512,7 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
       int nan = -1;
       mb::pdl_wait();
       // the parts of the next tile's normalisers are on their way while this one's are joined
-      constexpr int kTake = 4;
+      constexpr int kTake = FEW ? 8 : 4;
       float2 y[2][kTake];
       float yscale[2] = {1.f, 1.f};
       auto look = [&](int tile) {
@@ -482,8 +524,9 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
           if (FP8) yscale[e] = wscale[at];
         }
       };
-      if (tiles > 0) look(0);
-      for (int tile = 0; tile < tiles; ++tile) {
+      const int infos = FEW ? turns : tiles;
+      if (infos > 0) look(0);
+      for (int tile = 0; tile < infos; ++tile) {
         const int slot = tile % kInfo;
         float f[2], lse[2];
 #pragma unroll
@@ -530,7 +573,7 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
         }
         __syncwarp();
         if (lane == 0) mb::mbar_arrive(&info_full[slot]);
-        if (tile + 1 < tiles) look(tile + 1);
+        if (tile + 1 < infos) look(tile + 1);
       }
     }
     if (warp == 10 && mb::elect_one()) {
@@ -542,23 +585,31 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
       const int chunks = tiles * kChunks;
       int st = 0, turn = 0;
       for (int j = 0; j < chunks && ok; ++j) {
-        const int tile = j / kChunks, q = j % kChunks, b = tile & 1;
+        const int tile = j / kChunks, q = j % kChunks, b = tile & 1, row_tile = FEW ? tile & more : 0;
+        if (FEW && q == 0 && row_tile > 0) {                 // the same chunks again, all of which are in the ring
+          st -= kChunks;
+          if (st < 0) {
+            st += kStages;
+            turn ^= 1;
+          }
+        }
         ok = mb::mbar_wait(&full[st], turn, a.status, MB_ST_TIMEOUT_MMA);
         if (q == 0) ok = ok && mb::mbar_wait(&s_free[b], ((tile >> 1) & 1) ^ 1, a.status, MB_ST_TIMEOUT_MMA);
         if (!ok) break;
         mb::tc_fence_after();
-        const uint64_t dC = dR + (uint32_t)(st * (C::kChunkB >> 4)), dA = dH + (uint32_t)(q * (kHeld * 128 >> 4));
+        const uint64_t dC = dR + (uint32_t)(st * (C::kChunkB >> 4)), dA = dH + (uint32_t)((row_tile * kChunks + q) * (kHeld * 128 >> 4));
 #pragma unroll
-        for (int k = 0; k < 4; ++k) mb::umma_f16(tmem + b * kN, dA + (k * 32 >> 4), dC + (k * 32 >> 4), kId, (q | k) != 0);
+        for (int k = 0; k < 4; ++k) mb::umma_f16(tmem + b * kN, (FEW ? dC : dA) + (k * 32 >> 4), (FEW ? dA : dC) + (k * 32 >> 4), kId, (q | k) != 0);
         if (q == kChunks - 1) mb::tc_commit(&s_full[b]);
-        mb::tc_commit(&empty[st]);
+        if (row_tile == more) mb::tc_commit(&empty[st]);
         if (++st == kStages) {
           st = 0;
           turn ^= 1;
         }
       }
       // nobody may free the accumulators under products in flight
-      if (ok && chunks > 0) mb::mbar_wait(&empty[(chunks - 1) % kStages], ((chunks - 1) / kStages) & 1, a.status, MB_ST_TIMEOUT_MMA);
+      const int last = chunks / turns - 1;                   // of the chunks that came
+      if (ok && last >= 0) mb::mbar_wait(&empty[last % kStages], (last / kStages) & 1, a.status, MB_ST_TIMEOUT_MMA);
     }
     if (warp == 11) {
       // ---------------------------------------------------------- copies
@@ -581,23 +632,33 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
         }
       };
       if (!KEYS || !ws.paged) mb::pdl_wait();
-      if constexpr (KEYS) {
+      // few rows stay, once the kernel in front has left them
+      auto hold = [&] {
+        if (ws.paged) mb::pdl_wait();
+        if (lane == 0) {
+          mb::mbar_expect_tx(&held_full, turns * C::kHeldB);
+          for (int i = 0; i < turns * kChunks; ++i) mb::tma_load_2d(sHeld + i * (kHeld * 128), &tmQ, &held_full, i % kChunks * 64, (int)row0 + i / kChunks * kN);
+        }
+        __syncwarp();
+      };
+      if constexpr (KEYS && !FEW) {
         if (lane == 0) mb::mbar_expect_tx(&held_full, C::kHeldB);
         __syncwarp();
         const int place = ws.paged ? box_at(at0 + (lane & 7) * kBox) : 0;
         for (int q = 0; q < kChunks; ++q) keys(sHeld + q * (kHeld * 128), &held_full, q * 64, at0, place);
       }
-      if (KEYS && ws.paged) mb::pdl_wait();
-      const int chunks = tiles * kChunks;
+      if (KEYS && !FEW && ws.paged) mb::pdl_wait();
+      const int chunks = tiles / turns * kChunks, key0 = FEW ? at0 : begin;
       int st = 0, turn = 1, place = 0;
-      if (!KEYS && ws.paged && chunks > 0) place = box_at(begin + (lane & 7) * kBox);
+      if ((!KEYS || FEW) && ws.paged && chunks > 0) place = box_at(key0 + (lane & 7) * kBox);
       for (int j = 0; j < chunks; ++j) {
-        const int tile = j / kChunks, q = j % kChunks, from = begin + tile * kN;
+        const int tile = j / kChunks, q = j % kChunks, from = key0 + tile * kN;
+        if (FEW && j == min(kStages, chunks) - 1) hold();    // keys of the cache need not wait for it
         if (!__all_sync(0xffffffffu, mb::mbar_wait(&empty[st], turn, a.status, MB_ST_TIMEOUT_TMA))) break;
         if (lane == 0) mb::mbar_expect_tx(&full[st], C::kChunkB);
         __syncwarp();
         uint8_t* dst = sRing + st * C::kChunkB;
-        if constexpr (KEYS) {
+        if constexpr (KEYS && !FEW) {
           if (lane == 0) mb::tma_load_2d(dst, &tmQ, &full[st], q * 64, (int)row0 + from);
         } else {
           keys(dst, &full[st], q * 64, from, place);
@@ -610,7 +671,7 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
       }
       if (bad && a.status) atomicCAS(a.status, 0u, MB_ST_BOUNDS);
       // copies in flight write shared memory: the CTA stays until the products have taken the last of them
-      if (KEYS && tiles == 0) mb::mbar_wait(&held_full, 0, a.status, MB_ST_TIMEOUT_TMA);
+      if (KEYS && !FEW && tiles == 0) mb::mbar_wait(&held_full, 0, a.status, MB_ST_TIMEOUT_TMA);
     }
     __syncwarp();
   }
@@ -660,20 +721,22 @@ __global__ void __launch_bounds__(256) observe_join_kernel(const MbMassArgs a, c
   a.mass[s * a.mass_seq + h * a.mass_head + j] += sum;
 }
 
-template <int D, bool FP8, bool KEYS>
+template <int D, bool FP8, Pass PASS>
 int launch(const MbMassArgs& a, const Ws& ws, const CUtensorMap* tm, cudaStream_t stream) {
-  auto kern = observe_kernel<D, FP8, KEYS>;
+  constexpr bool KEYS = PASS != kRowsPass;
+  auto kern = observe_kernel<D, FP8, PASS>;
+  const int smem = PASS == kFewPass ? few_smem<D>(ws.few) : Cfg<D>::kSmem;
   static bool configured = false;
   if (!configured) {
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::kSmem);
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, PASS == kFewPass ? few_smem<D>(D == 256 ? 1 : 2) : Cfg<D>::kSmem);
     if (e != cudaSuccess) return (int)e;
     configured = true;
   }
   const int G = a.Hq / a.Hkv;
   const unsigned magic = G == 1 ? 0 : (unsigned)(((1ull << 32) + G - 1) / G);
-  const long long blocks = ((KEYS ? (long long)a.max_ctx : ws.rows) + kHeld - 1) / kHeld * (KEYS ? ws.row_parts : ws.slices);
+  const long long blocks = PASS == kFewPass ? ((a.max_ctx + kHeld - 1) / kHeld + ws.each - 1) / ws.each : ((KEYS ? (long long)a.max_ctx : ws.rows) + kHeld - 1) / kHeld * (KEYS ? ws.row_parts : ws.slices);
   if (blocks > 0x7fffffffll) return MB_ERR_TOO_LARGE;
-  return (int)mb::launch_kernel_ex(kern, dim3((unsigned)blocks, a.Hkv, a.num_seqs), dim3(kThreads), Cfg<D>::kSmem, stream, 1, mb_pdl_enabled() && (KEYS || !ws.paged), tm[0], tm[1], a, ws,
+  return (int)mb::launch_kernel_ex(kern, dim3((unsigned)blocks, a.Hkv, a.num_seqs), dim3(kThreads), smem, stream, 1, mb_pdl_enabled() && (KEYS || !ws.paged), tm[0], tm[1], a, ws,
                                    (int)magic);
 }
 
@@ -694,11 +757,11 @@ int all(const MbMassArgs& a, const Ws& ws, cudaStream_t stream) {
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return (int)e;
   }
-  rc = launch<D, FP8, false>(a, ws, tm, stream);
+  rc = launch<D, FP8, kRowsPass>(a, ws, tm, stream);
   if (!rc && ws.joined)
     rc = (int)mb::launch_kernel_ex(observe_rows_join_kernel, dim3((unsigned)((ws.rows + 127) / 128), a.Hkv, a.num_seqs), dim3(128), 0, stream, 1, mb_pdl_enabled() != 0,
                                    a, ws);
-  return rc ? rc : launch<D, FP8, true>(a, ws, tm, stream);
+  return rc ? rc : ws.few ? launch<D, FP8, kFewPass>(a, ws, tm, stream) : launch<D, FP8, kKeysPass>(a, ws, tm, stream);
 }
 
 }  // namespace

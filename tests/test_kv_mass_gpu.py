@@ -269,6 +269,27 @@ def test_prompt_in_several_steps_gives_the_same(monkeypatch):
     assert torch.equal(m, c["mass"])
 
 
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("heads,kv_heads,dim,block", [(8, 2, 128, 16), (4, 4, 64, 16), (5, 1, 128, 24), (16, 2, 256, 16), (64, 1, 64, 32), (12, 3, 256, 5)])
+def test_prompt_of_few_rows_does_not_depend_on_its_batch(heads, kv_heads, dim, block, fp8):
+    """Few rows stay in a CTA of the keys pass, those of a call with a longer portion go by: the same bits."""
+    G = heads // kv_heads
+    new = [1, 128 // G, 128 // G + 1, 256 // G, 3, 600 // G + 300]
+    c = _cuda(oracle.case(62, [700, 129, 2500, 1024, 5000, 1300], heads, kv_heads, dim, fp8, block=block, new=new))
+    c["q"][4, 0, 7] = math.nan
+    c["q"][new[0] + new[1] + 5 % new[2], 0, 1] = math.inf    # of sequence 2
+    m = c["mass"].clone()
+    _prompt(c, 0)
+    want = c["mass"].clone()
+    for s in range(5):
+        one = {k: c[k][s:s + 1] for k in ("table", "ctx", "q_start", "q_len")}
+        c["mass"] = m.clone()
+        _prompt({**c, **one, "mass": c["mass"][s:s + 1]}, 0, max_q_len=new[s])
+        assert _same(c["mass"][s].nan_to_num(-1.0), want[s].nan_to_num(-1.0))
+        assert _same(c["mass"][:s], m[:s]) and _same(c["mass"][s + 1:], m[s + 1:])
+    assert want.isnan().any() and not want.isnan().all()
+
+
 @pytest.mark.parametrize("apart", [2.0 ** -9, 2.0 ** 9, 2.0 ** 40])
 def test_prompt_of_rows_far_apart(apart):
     """An e4m3 cache's queries become f16: rows whose sizes differ by little share a factor, others have their own; none loses its range."""
