@@ -10,8 +10,8 @@
 //
 // Both operands come by TMA: keys from the cache, 16 tokens a box, or from a copy in the workspace (an e4m3 cache's as f16, any cache's whose blocks are
 // not whole boxes), which a kernel in front makes; query rows of the keys pass from the copy that the rows pass makes of its own (with an e4m3 cache
-// f16, scaled by a power of two, one for 128 rows that are alike, else one per row). A first form had four warps gather and widen tiles on the way into shared memory, every CTA the same ones: that
-// took the issue slots of the exponentials, 4096 observers at 8192 e4m3 tokens 819 us.
+// f16, scaled by a power of two, one for 128 rows that are alike, else one per row). A first form had four warps gather and widen tiles on the way into
+// shared memory, every CTA the same ones: that took the issue slots of the exponentials, 4096 observers at 8192 e4m3 tokens 819 us.
 //
 // Roles (384 threads, two CTAs per SM, so that one's beginning and end are under the other's exponentials): warps 0-3 and 4-7 own 128 lanes each and half
 // of a tile's columns; warps 8 and 9 bring the rows' normalisers (keys pass), warp 10 issues the products into two accumulators, so that products run
@@ -177,7 +177,7 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
   __shared__ __align__(16) float s_lse[kInfo][kN];           // keys pass: the query rows' normalisers, negative, and their factors
   __shared__ __align__(16) float s_factor[KEYS && FP8 ? kInfo : 1][kN];
   __shared__ __align__(8) int s_alike[KEYS && FP8 ? kInfo : 1][4];         // 32 rows' factors are those of the first of 64
-  __shared__ int s_nan[2];                                   // keys pass: the last row whose normaliser is not a number, of each of two warps' rows
+  __shared__ int s_nan;                                      // keys pass: the last row whose normaliser is not a number
   __shared__ int2 s_top[kSums / 32];                         // rows pass, e4m3: the largest exponent of a row's largest element, and the smallest
   const int h = blockIdx.y, s = blockIdx.z, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int G = a.Hq / a.Hkv;
@@ -267,7 +267,7 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
       mb::mbar_init(&s_full[i], 1);
       mb::mbar_init(&s_free[i], kSums / 32);
     }
-    s_nan[0] = s_nan[1] = -1;
+    s_nan = -1;
     mb::mbar_fence_init();
     mb::tma_prefetch_desc(&tmK);
     if (KEYS) mb::tma_prefetch_desc(&tmQ);
@@ -476,8 +476,8 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
       if (!KEYS && begin + (t + 1) * kN == flush_at) flush();
       if (FEW && (t & more) == more) {
         // a block of keys is done; the other half's sums have two places, so that one barrier a block is enough
-        const int nan = max(s_nan[0], s_nan[1]), place = (t / turns) & 1;
-        if (nan >= 0 && mine < limit_of(nan)) l_run = NAN;
+        const int place = (t / turns) & 1;
+        if (s_nan >= 0 && mine < limit_of(s_nan)) l_run = NAN;
         if (half) s_half[place][r].y = l_run;
         asm volatile("bar.sync 1, 256;" ::: "memory");
         if (!half && mine < own) a.mass[s * a.mass_seq + h * a.mass_head + mine] = old + (l_run + s_half[place][r].y);
@@ -489,8 +489,7 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
     }
     for (; blocks_left > 0; --blocks_left) asm volatile("bar.sync 1, 256;" ::: "memory");    // a wait ran out: the other warps' barriers count this one
     if constexpr (KEYS && !FEW) {
-      const int nan = max(s_nan[0], s_nan[1]);               // written in front of the last tile's normalisers
-      if (nan >= 0 && mine < limit_of(nan)) l_run = NAN;
+      if (s_nan >= 0 && mine < limit_of(s_nan)) l_run = NAN;
       if (half) s_half[0][r].y = l_run;
       asm volatile("bar.sync 1, 256;" ::: "memory");
       if (!half && mine < own) {
@@ -509,7 +508,6 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
     if (KEYS && warp < 10) {
       // ---------------------------------------------------------- factors and normalisers of a tile's rows, two a thread
       const int t = tid - kSums, left = ws.joined ? 1 : kparts;
-      int nan = -1;
       mb::pdl_wait();
       // the parts of the next tile's normalisers are on their way while this one's are joined
       constexpr int kTake = FEW ? 8 : 4;
@@ -550,11 +548,10 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
           // An infinite query's is NaN, which the -inf of a mask would not survive. Its row adds nothing here; since later rows see more, the last such row
           // says which keys have no number in the end.
           if (lse[e] != lse[e]) {
-            nan = at;
+            atomicMax(&s_nan, at);
             lse[e] = INFINITY;
           }
         }
-        nan = __reduce_max_sync(0xffffffffu, nan);
         const bool ok = mb::mbar_wait(&info_free[slot], ((tile / kInfo) & 1) ^ 1, a.status, MB_ST_TIMEOUT_EPI);
         if (!__all_sync(0xffffffffu, ok)) break;
 #pragma unroll
@@ -562,7 +559,6 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
           s_lse[slot][t + 64 * e] = -lse[e];
           if constexpr (FP8) s_factor[slot][t + 64 * e] = f[e];
         }
-        if (lane == 0) s_nan[warp & 1] = nan;
         if constexpr (FP8) {
           asm volatile("bar.sync 2, 64;" ::: "memory");
 #pragma unroll
