@@ -18,9 +18,9 @@
 // under the exponentials, warp 11 the copies. With 256 lanes a CTA and one of them per SM, 4096 observers at 8192 e4m3 tokens took 766 us, sixteen prompts
 // of 17 to 1151 tokens under 64 observers 55.
 //
-// Bound by its exponentials, two a logit at 16 a cycle and SM: 4096 observers at 8192 e4m3 tokens, 40 / 8 heads of 128, take 717 us (1.0 G logits a
-// pass, 2.8 T exponentials a second; the special function units 79 and 70 % busy, the tensor pipe 39 and 33), 32 observers 41. At dim 256 products from
-// shared memory count as much: 2 prompts of 1001 and 1531 at up to 4431 tokens, 16 / 2 heads, 164 us. (B200, in a graph.)
+// Bound by its exponentials, two a logit at 16 a cycle and SM: 4096 observers at 8192 e4m3 tokens, 40 / 8 heads of 128, take 727 us (1.0 G logits a
+// pass, 2.8 T exponentials a second; the special function units 76 and 68 % busy, the tensor pipe 38 and 32), 32 observers 31, a launch's latency three times. At dim 256 products from
+// shared memory count as much: 2 prompts of 1001 and 1531 at up to 4431 tokens, 16 / 2 heads, 163 us. (B200, in a graph.)
 //
 // Long rows and long columns are cut into parts, by rules on the sequence's own lengths alone, and joined in order: every output has one writer and
 // every sum one order.
@@ -359,7 +359,7 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
       flush_at += kp;
     };
     // Columns that count for any lane of this warp end here; the others' weights are zeros, whose exponentials few rows would pay for (160 rows of 5 heads: a
-    // block of 128 and one of 32).
+    // block of 128 and one of 32; 32 observers at 8192 e4m3 tokens 41 -> 34 us, at the price of 716 -> 723 for 4096).
     int reach = KEYS ? (at0 + (warp & 3) * 32 < own ? end : 0) : min(end, __reduce_max_sync(0xffffffffu, limit));
     float old = 0.f;                                         // few rows: the mass that is added to
     int blocks_left = FEW ? tiles / turns : 0;
