@@ -19,8 +19,8 @@
 // of 17 to 1151 tokens under 64 observers 55.
 //
 // Bound by its exponentials, two a logit at 16 a cycle and SM: 4096 observers at 8192 e4m3 tokens, 40 / 8 heads of 128, take 727 us (1.0 G logits a
-// pass, 2.8 T exponentials a second; the special function units 76 and 68 % busy, the tensor pipe 38 and 32), 32 observers 31, a launch's latency three times. At dim 256 products from
-// shared memory count as much: 2 prompts of 1001 and 1531 at up to 4431 tokens, 16 / 2 heads, 163 us. (B200, in a graph.)
+// pass, 2.8 T exponentials a second; the special function units 76 and 68 % busy, the tensor pipe 38 and 32), 32 observers 31, a launch's
+// latency three times. At dim 256 products from shared memory count as much: 2 prompts of 1001 and 1531 at up to 4431 tokens, 16 / 2 heads, 163 us. (B200, in a graph.)
 //
 // Long rows and long columns are cut into parts, by rules on the sequence's own lengths alone, and joined in order: every output has one writer and
 // every sum one order.
@@ -75,14 +75,15 @@ __host__ __device__ __forceinline__ int parts_of(int n, int part) { return n <= 
 // too large by; sums of the columns' parts [row parts, seqs * Hkv, columns]
 struct Ws {
   long long rows, cols, tokens;
-  int key_parts, row_parts, slices, paged, joined, few, each;   // slices: CTAs that a block of rows is shared out over; joined: a row's parts are, before the keys pass;
-                                                     // few: tiles of rows that stay in a CTA of the keys pass, where keys go by, `each` blocks of them; else 0
+  // slices: CTAs that a block of rows is shared out over; joined: a row's parts are, before the keys pass; few: tiles of rows that stay in a CTA of the
+  // keys pass, where keys go by, `each` blocks of them, else 0
+  int key_parts, row_parts, slices, paged, joined, few, each;
   size_t keys, ml, scale, sums, bytes;
 };
 // From this many observed rows on, a bf16 cache's keys are copied too: every tile of them goes by often, and comes as one box instead of eight
 constexpr int kCopyRows = 1024;
 // With more parts of a row than this they are joined by a kernel of its own: every CTA of the keys pass would join them again, for all rows. 64 observers at
-// 16000 bf16 tokens, 16 / 2 heads of 256 (32 parts) 47 -> 35 us, 32 at 8192 e4m3, 40 / 8 of 128 (16) 44 -> 41. CTAs with few rows are fewer and join more
+// 16000 bf16 tokens, 16 / 2 heads of 256 (32 parts) 47 -> 35 us, three of 16207, 16 / 1 of 128 (16 parts, 1024 rows) 74 -> 67. CTAs with few rows are fewer and join more
 // themselves: 8 prompts of 4000 to 8192 tokens, 128 rows (16 parts) 80 -> 71, one of 32768, 160 rows (32 parts) 65.5 -> 63.2 with the kernel.
 constexpr int kJoin = 4, kFewJoin = 16;
 // Up to so many tiles of 128 rows stay in a CTA of the keys pass while keys go by, two at 64 and 128 dims and one at 256, which shared memory holds beside a
@@ -189,7 +190,8 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
   // A column's parts are a CTA each. So are a row's where the call's longest portion has as many; shorter portions, whose rows have more of them, share
   // `slices` CTAs out.
   const int slices = KEYS ? ws.row_parts : ws.slices, blocks = gridDim.x / slices, share = KEYS ? 1 : (kparts + slices - 1) / slices;
-  const int part = FEW ? 0 : blockIdx.x / blocks * share, at0 = FEW ? blockIdx.x * ws.each * kHeld : (KEYS ? (int)blockIdx.x % blocks : blocks - 1 - (int)blockIdx.x % blocks) * kHeld;   // the longest first
+  const int part = FEW ? 0 : blockIdx.x / blocks * share;
+  const int at0 = (FEW ? blockIdx.x * ws.each : KEYS ? (int)blockIdx.x % blocks : blocks - 1 - (int)blockIdx.x % blocks) * kHeld;   // the longest first
   const int own = KEYS ? x.n : x.rows;
   if (part >= (KEYS ? rparts : kparts) || at0 >= own || x.rows == 0 || x.n == 0) {
     mb::pdl_wait();                                       // a grid ends behind the one in front of it, even where it does nothing
