@@ -191,7 +191,7 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
   // `slices` CTAs out.
   const int slices = KEYS ? ws.row_parts : ws.slices, blocks = gridDim.x / slices, share = KEYS ? 1 : (kparts + slices - 1) / slices;
   const int part = FEW ? 0 : blockIdx.x / blocks * share;
-  const int at0 = (FEW ? blockIdx.x * ws.each : KEYS ? (int)blockIdx.x % blocks : blocks - 1 - (int)blockIdx.x % blocks) * kHeld;   // the longest first
+  const int at0 = (FEW ? (int)blockIdx.x * ws.each : KEYS ? (int)blockIdx.x % blocks : blocks - 1 - (int)blockIdx.x % blocks) * kHeld;   // the longest first
   const int own = KEYS ? x.n : x.rows;
   if (part >= (KEYS ? rparts : kparts) || at0 >= own || x.rows == 0 || x.n == 0) {
     mb::pdl_wait();                                       // a grid ends behind the one in front of it, even where it does nothing
