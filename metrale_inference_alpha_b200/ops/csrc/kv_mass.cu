@@ -64,7 +64,7 @@ __global__ void __launch_bounds__(256, 4) mass_join_kernel(const MbMassArgs a, c
     float2 v = g == warp ? first : lane < parts ? __ldcg(ml + (size_t)g * w.parts + lane) : make_float2(-INFINITY, 0.f);
     if (lane >= parts) v = make_float2(-INFINITY, 0.f);
     const float mx = mb::warp_max(v.x);
-    const float l = mb::warp_sum(v.x == -INFINITY ? 0.f : v.y * ex2(v.x - mx));
+    const float l = mb::warp_sum(v.y * (v.x == -INFINITY ? 0.f : ex2(v.x - mx)));    // scores that are all NaN have no maximum, but a sum that is NaN
     if (lane == 0) s_lse[g] = l == 0.f ? INFINITY : mx + log2f(l);   // a row without weight adds none
   }
   __syncthreads();

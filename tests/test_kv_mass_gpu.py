@@ -569,3 +569,104 @@ def test_a_prompt_is_cut_and_decoded_from(fp8):
     k, v, m, kept, length = oracle.evict(c, keep, recent, keep + 24)
     got, n = ops.kv_evict(g["k"], g["v"], g["table"], g["ctx"], g["mass"], keep=keep, recent=recent, max_ctx=keep + 24)
     assert torch.equal(got.cpu(), kept) and torch.equal(n.cpu(), length) and _same(g["k"], k) and _same(g["v"], v) and _same(g["mass"], m)
+
+
+# ----------------------------------------------------------------------------- keys that are no numbers
+def _defined(c, last):
+    """(mass, outputs of each sequence's last token) of the definition in 64 bits, NaN where a row's softmax has no numbers, and the mass's bound, from what is
+    finite of the case: oracle.weights divides rows by their sums whole, so that what such a row does not see would be NaN as well."""
+    S, H, D = len(c["ctx"]), c["k"].shape[2], c["k"].shape[3]
+    G = c["q"].shape[1] // H
+    calm = {**c, **{n: c[n] if c[n].dtype == torch.uint8 else c[n].nan_to_num(0.0, 0.0, 0.0) for n in ("q", "k")}}
+    if c["k"].dtype == torch.uint8:
+        calm["k"] = torch.where(c["k"] & 0x7f == 0x7f, 0, c["k"])
+    mass, tol, out = c["mass"].double().clone(), torch.zeros(c["mass"].shape, dtype=torch.float64), torch.zeros(S, G * H, D, dtype=torch.float64)
+    for s in range(S):
+        n, ql = int(c["ctx"][s]), int(c["q_len"][s])
+        w = min(last or ql, ql)
+        if n <= 0 or w <= 0:
+            continue
+        k = oracle.rows_of(c["k"], c["table"], s, torch.arange(n), c["k_scale"])
+        v = oracle.rows_of(c["v"], c["table"], s, torch.arange(n), c["v_scale"])
+        q0 = int(c["q_start"][s]) + ql
+        for h in range(H):
+            z = torch.einsum("wgd,nd->wgn", c["q"][q0 - w:q0, h * G:(h + 1) * G].double(), k[:, h]) * c["scale"]
+            seen = (torch.arange(n) < (n - w + 1 + torch.arange(w))[:, None])[:, None].expand_as(z)
+            p = torch.softmax(z.masked_fill(~seen, -math.inf), -1)
+            p = torch.where(seen, p, 0.0)
+            out[s, h * G:(h + 1) * G] = p[-1] @ v[:, h]
+            r = oracle.weight_error(c, D, oracle.weights(calm, s, h, G, last)[1])
+            add = p.sum((0, 1))
+            mass[s, h, :n] += add
+            tol[s, h, :n] = ((r + w * G * 2.0 ** -24) * add + 2.0 ** -23 * mass[s, h, :n]).nan_to_num(0.0) + 1e-30
+    return mass, out, tol
+
+
+def _as_defined(got, want, tol):
+    assert torch.equal(got.cpu().isnan(), want.isnan())
+    _within(got.cpu().nan_to_num(0.0), want.nan_to_num(0.0), tol, "mass")
+
+
+def _set_key(c, s, j, h, value, dim=None):
+    """Key j of sequence s and kv head h, or one element of it."""
+    bs = c["k"].shape[1]
+    row = c["k"][int(c["table"][s, j // bs]), j % bs, h]
+    if c["k"].dtype == torch.uint8:
+        assert math.isnan(value)
+        value = 0x7f
+    if dim is None:
+        row[:] = value
+    else:
+        row[dim] = value
+
+
+# what the newest key is alone in: half of a tile, a part of a row's keys, a decode partition (of 512 and of 1024 tokens)
+ALONE = [17, 33, 65, 129, 513, 1025, 2049, 4097, 8193]
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("n", ALONE)
+@pytest.mark.parametrize("back", [0, 1, 9])
+@pytest.mark.parametrize("heads,kv_heads,dim,rows", [(4, 2, 128, 1), (6, 2, 64, 3), (4, 2, 256, 1), (4, 2, 128, 140)])
+def test_prompt_of_a_key_that_is_not_a_number(heads, kv_heads, dim, rows, back, n, fp8):
+    """Rows that see it have no weights that are numbers, however their keys are cut into parts."""
+    c = oracle.case(70, [n, 40], heads, kv_heads, dim, fp8, new=[min(rows, n), 5])
+    _set_key(c, 0, n - 1 - back, 0, math.nan, dim // 2)
+    want, _, tol = _defined(c, 0)
+    g = _cuda(c)
+    _prompt(g, 0)
+    _as_defined(g["mass"], want, tol)
+    assert want[0, 0].isnan().any() and not want[0, 1].isnan().any()
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("n", ALONE)
+@pytest.mark.parametrize("back", [0, 1, 700])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(4, 2, 128), (8, 8, 128), (20, 2, 64), (4, 2, 256), (34, 1, 128)])
+def test_decode_of_a_key_that_is_not_a_number(heads, kv_heads, dim, back, n, fp8):
+    """Its group's outputs and mass are NaN, both of them and whole, however the keys are cut into partitions."""
+    c = oracle.case(71, [n, 40], heads, kv_heads, dim, fp8)
+    _set_key(c, 0, max(0, n - 1 - back), 0, math.nan, 5)
+    want, out, tol = _defined(c, 0)
+    g = _cuda(c)
+    got = _decode(g)
+    _as_defined(g["mass"], want, tol)
+    assert torch.equal(got.cpu().isnan(), out.isnan()) and out[0, :heads // kv_heads].isnan().all() and not out[1].isnan().any()
+
+
+@pytest.mark.parametrize("value", [math.inf, -math.inf])
+@pytest.mark.parametrize("n,at", [(65, 64), (1025, 1024), (1025, 3), (4097, 4096), (700, 350)])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(2, 2, 64), (4, 4, 128), (8, 2, 128), (3, 3, 256)])
+def test_an_infinite_key(heads, kv_heads, dim, n, at, value):
+    """A score of -inf is a weight of zero, one of +inf leaves its row no number; heads meet both."""
+    c = oracle.case(72, [n, 40], heads, kv_heads, dim, False, new=[1, 1])
+    for h in range(kv_heads):
+        _set_key(c, 0, at, h, value, 7 + h)
+    want, out, tol = _defined(c, 0)
+    g = _cuda(c)
+    got = _decode(g)
+    _as_defined(g["mass"], want, tol)
+    assert torch.equal(got.cpu().isnan(), out.isnan())
+    g = _cuda(c)
+    _prompt(g, 0)
+    _as_defined(g["mass"], want, tol)
