@@ -142,6 +142,8 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
   __shared__ __align__(8) uint64_t bars[4 * kMaxSlots];
   const int slots = p.slots;
   __shared__ int s_last, s_wsum[4];
+  constexpr bool kLift = MASS && FP8;
+  __shared__ float s_sc[kLift ? 4 : 1][kLift ? NT * 8 : 1];  // kLift: rows' scores come to the log2 domain by these, a copy a warp
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   float* s_o = reinterpret_cast<float*>(smem + p.merge_off);                  // [4 warps][rows][D], see C::place
   int* s_off = reinterpret_cast<int*>(smem + p.tail_off);                     // [seqs + 1]
@@ -334,14 +336,39 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         const int r = kPairs ? tile * 16 + g + hr * 8 : tile * 8 + g;
         const bool live = r < R;
         const uint8_t* qrow = s_q + r * C::kQPitch;
+        __nv_bfloat162 lift;
+        uint2 v[kLift ? D / 16 : 1];
+        if constexpr (kLift) {
+          // With an e4m3 cache queries are f16, which has less range than bf16: the power of two that takes a row's largest element to [2^14, 2^15), as in
+          // kv_observe.cu; infinities and NaN stay what they are. Its latency costs 128 sequences of 129 to 1151 tokens 52.2 -> 53.5 us, one of 700 13.5 -> 13.8.
+          // Factors in registers took 20 query rows of 700 tokens 27.8 us instead of 26.5; found once for all warps behind the rows' copies, or only where a
+          // row's sums had been lost, they cost no less (53.4, 53.7).
+          __nv_bfloat162 most = __float2bfloat162_rn(0.f);
+#pragma unroll
+          for (int ks = 0; ks < D / 16; ++ks) {
+            v[ks] = live ? *reinterpret_cast<const uint2*>(qrow + ks * 32 + 8 * t) : make_uint2(0, 0);
+            most = __hmax2(most, __hmax2(__habs2(*reinterpret_cast<__nv_bfloat162*>(&v[ks].x)), __habs2(*reinterpret_cast<__nv_bfloat162*>(&v[ks].y))));
+          }
+          uint32_t top = __bfloat16_as_ushort(__hmax(most.x, most.y));       // bits of a bf16 without its sign order like the values
+          top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+          top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+          const int e = (int)(top >> 7), up = e == 255 ? 0 : 141 - max(e, 15);
+          lift = __bfloat162bfloat162(__ushort_as_bfloat16((unsigned short)((127 + up) << 7)));
+          if (t == 0) s_sc[warp][r] = sc_log2 * __int_as_float((127 - up) << 23);
+        }
 #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks) {
           uint32_t a = 0, b = 0;
           if (live) {
             if constexpr (FP8) {                             // four neighbouring dims: the order e4m3 fragments come in
-              const uint2 v = *reinterpret_cast<const uint2*>(qrow + ks * 32 + 8 * t);
-              const float2 f0 = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v.x));
-              const float2 f1 = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v.y));
+              if constexpr (!kLift) v[0] = *reinterpret_cast<const uint2*>(qrow + ks * 32 + 8 * t);
+              const uint2 w = v[kLift ? ks : 0];
+              __nv_bfloat162 x0 = *reinterpret_cast<const __nv_bfloat162*>(&w.x), x1 = *reinterpret_cast<const __nv_bfloat162*>(&w.y);
+              if constexpr (kLift) {                         // exact: a power of two, within the type's range
+                x0 = __hmul2(x0, lift);
+                x1 = __hmul2(x1, lift);
+              }
+              const float2 f0 = __bfloat1622float2(x0), f1 = __bfloat1622float2(x1);
               a = pack2<true>(f0.x, f0.y);
               b = pack2<true>(f1.x, f1.y);
             } else {
@@ -360,6 +387,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         min_limit = min(min_limit, lim[tile][e]);
       }
     }
+    if constexpr (kLift) __syncwarp();
     // over all rows of the tiles
 #pragma unroll
     for (int o = kPairs ? 4 : 1; o < (kPairs ? 32 : 4); o <<= 1) min_limit = min(min_limit, __shfl_xor_sync(0xffffffffu, min_limit, o));
@@ -449,13 +477,14 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
       for (int tile = 0; tile < kTiles; ++tile) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float mx = -INFINITY;
+          float mx = -INFINITY, sc = sc_log2;
+          if constexpr (kLift) sc = s_sc[warp][row_of(tile, e)];
 #pragma unroll
           for (int n = 0; n < kS; ++n)
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
               float& v = s[tile][n][at(e, j)];
-              v *= sc_log2;
+              v *= sc;
               if (mask && pos0 + (kPairs ? n * 8 + 2 * t + j : n * 16 + j * 8 + g) >= lim[tile][e]) v = -INFINITY;
               mx = fmaxf(mx, v);
             }

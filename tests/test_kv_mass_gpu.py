@@ -670,3 +670,34 @@ def test_an_infinite_key(heads, kv_heads, dim, n, at, value):
     g = _cuda(c)
     _prompt(g, 0)
     _as_defined(g["mass"], want, tol)
+
+
+# ----------------------------------------------------------------------------- queries beyond the range of f16
+@pytest.mark.parametrize("apart", [2.0 ** -30, 2.0 ** -9, 2.0 ** 9, 2.0 ** 15, 2.0 ** 40, 2.0 ** 100])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(8, 2, 128), (12, 1, 64), (20, 1, 128), (30, 1, 128), (33, 1, 128), (16, 2, 256), (8, 8, 64)])
+def test_decode_of_rows_far_apart(heads, kv_heads, dim, apart):
+    """An e4m3 cache's queries become f16, each row behind a power of two of its own: none loses its range, whatever the rows beside it are. That takes a row's
+    largest element to 2^14 at least, where f16 is off by 2^-11 of an element down to 2^-28 of it and by 2^-39 of it below: exact for bf16's eight bits in the
+    first case, and in the second less than what the bound has for the products' sum."""
+    c = oracle.case(80, [300, 150, 1], heads, kv_heads, dim, True)
+    c["scale"] /= max(1.0, apart)
+    c["q"][:, ::3] *= apart
+    c["q"][1, 5::7] = 0
+    want, tol, mass, mtol = oracle.decode(c)
+    g = _cuda(c)
+    got = _decode(g)
+    _within(got, want, tol, "outputs")
+    _within(g["mass"], mass, mtol, "mass")
+
+
+def test_decode_of_the_largest_and_smallest_queries():
+    """Elements at either end of bf16 within one row, and rows of subnormal numbers."""
+    c = oracle.case(81, [200, 90], 8, 2, 128, True)
+    top, tiny = torch.finfo(torch.bfloat16).max, 2.0 ** -133
+    c["scale"] = 2.0 ** -120
+    c["q"][0, 0, ::2], c["q"][0, 1] = top, tiny
+    c["q"][0, 2] = torch.where(torch.arange(128) == 5, top, c["q"][0, 2].float()).bfloat16()
+    want, tol, mass, mtol = oracle.decode(c)
+    g = _cuda(c)
+    _within(_decode(g), want, tol, "outputs")
+    _within(g["mass"], mass, mtol, "mass")
