@@ -3,6 +3,7 @@
 #pragma once
 #include "common.cuh"
 #include "attention_decode.h"
+#include "smem_limit.h"
 #include "tensormap.h"
 #include <type_traits>
 
@@ -794,13 +795,10 @@ int launch(const AttnDecodeArgs& a, DecodeParams& p, cudaStream_t stream) {
   p.merge_off = l.merge_off;
   p.tail_off = l.tail_off;
   p.len_off = l.len_off;
-  static size_t configured = 0;
   if (l.smem > 220 * 1024) return MB_ERR_TOO_LARGE;
-  if (l.smem > configured) {
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024);
-    if (e != cudaSuccess) return (int)e;
-    configured = 220 * 1024;
-  }
+  static std::atomic<uint64_t> asked{0};
+  const cudaError_t e = mb::allow_smem(reinterpret_cast<const void*>(kern), 220 * 1024, asked);
+  if (e != cudaSuccess) return (int)e;
   const int grid = most < (long long)sms * l.per_sm ? (int)most : sms * l.per_sm;
   p.early = a.early && mb_pdl_enabled() == 2;
   return (int)mb::launch_kernel_ex(kern, dim3(grid), dim3(128), l.smem, stream, 1, p.early || mb_pdl_enabled() == 1, tm[0], tm[1], p);

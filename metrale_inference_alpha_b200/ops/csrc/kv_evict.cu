@@ -12,6 +12,7 @@
 // in place, e4m3, 20 us, three of 70 to 500 to 128 8: latency of both. (B200, in a graph.)
 #include "common.cuh"
 #include "kv_mass.h"
+#include "smem_limit.h"
 
 namespace {
 
@@ -401,12 +402,9 @@ extern "C" int mb_kv_evict(const MbEvictArgs* given, cudaStream_t stream) {
     const int round = (256 >> bits) * kDeep;
     return (int)mb::launch_kernel_ex(evict_copy_kernel, dim3(2 * ((held + round - 1) / round), a->Hkv, a->num_seqs), dim3(256), 0, stream, 1, mb_pdl_enabled() != 0, *a, bits);
   }
-  static bool configured = false;
-  if (!configured) {
-    e = cudaFuncSetAttribute(evict_move_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRoundB);
-    if (e != cudaSuccess) return (int)e;
-    configured = true;
-  }
+  static std::atomic<uint64_t> asked{0};
+  e = mb::allow_smem(reinterpret_cast<const void*>(evict_move_kernel), kRoundB, asked);
+  if (e != cudaSuccess) return (int)e;
   const int mine = kRoundB / a->row_bytes;
   int cluster = 1;                                                     // rounds as large as leave the chip (148 SMs) something to do
   while (cluster < kMaxCluster && 2 * heads * cluster < 2 * 148 && cluster * mine < held) cluster *= 2;

@@ -27,6 +27,7 @@
 #include "attention_rows.cuh"
 #include "common.cuh"
 #include "kv_mass.h"
+#include "smem_limit.h"
 #include "tensormap.h"
 
 namespace {
@@ -728,12 +729,9 @@ int launch(const MbMassArgs& a, const Ws& ws, const CUtensorMap* tm, cudaStream_
   constexpr bool KEYS = PASS != kRowsPass;
   auto kern = observe_kernel<D, FP8, PASS>;
   const int smem = PASS == kFewPass ? few_smem<D>(ws.few) : Cfg<D>::kSmem;
-  static bool configured = false;
-  if (!configured) {
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, PASS == kFewPass ? few_smem<D>(D == 256 ? 1 : 2) : Cfg<D>::kSmem);
-    if (e != cudaSuccess) return (int)e;
-    configured = true;
-  }
+  static std::atomic<uint64_t> asked{0};
+  const cudaError_t e = mb::allow_smem(reinterpret_cast<const void*>(kern), PASS == kFewPass ? few_smem<D>(D == 256 ? 1 : 2) : Cfg<D>::kSmem, asked);
+  if (e != cudaSuccess) return (int)e;
   const int G = a.Hq / a.Hkv;
   const unsigned magic = G == 1 ? 0 : (unsigned)(((1ull << 32) + G - 1) / G);
   const long long blocks = PASS == kFewPass ? ((a.max_ctx + kHeld - 1) / kHeld + ws.each - 1) / ws.each : ((KEYS ? (long long)a.max_ctx : ws.rows) + kHeld - 1) / kHeld * (KEYS ? ws.row_parts : ws.slices);
