@@ -207,3 +207,30 @@ def test_nothing_to_do():
     assert ops.paged_attention_mass(c["q"][:0], c["k"], c["v"], none["table"], none["ctx"], none["mass"], max_ctx=4, scale=1.0).shape == (0, 2, 64)
     kept, length = ops.kv_evict(c["k"], c["v"], none["table"], none["ctx"], none["mass"], keep=2, recent=1, max_ctx=4)
     assert kept.shape == (0, 1, 2) and length.shape == (0,)
+
+
+# ----------------------------------------------------------------------------- cuts that would read what they write
+def _cut(c, table, **kw):
+    return ops.kv_evict(c["k"], c["v"], table, c["ctx"], c["mass"], **(dict(keep=8, recent=2, max_ctx=40) | kw))
+
+
+def test_evict_in_place_refuses_sequences_that_share_blocks():
+    """One row of a table for all, or rows that overlap: each sequence would move the others' rows."""
+    c = oracle.case(16, [40, 40], 4, 2, 64, False)
+    wide = torch.arange(1, 6, dtype=torch.int32)
+    k = c["k"].clone()
+    for table in (c["table"][:1].expand(2, -1), wide.as_strided((2, 3), (1, 1))):
+        with pytest.raises(ValueError, match="kv_evict: sequences share rows of block_table"):
+            _cut(c, table)
+        assert torch.equal(c["k"].view(torch.int16), k.view(torch.int16))
+    assert _cut(c, c["table"][:1].expand(2, -1), keep=40)[1].tolist() == [40, 40]                    # nothing moves
+    assert _cut({**c, "ctx": c["ctx"][:1], "mass": c["mass"][:1]}, c["table"][:1].expand(1, -1))[1].tolist() == [8]
+
+
+def test_evict_refuses_blocks_that_several_sequences_are_to_take():
+    c = oracle.case(17, [40, 40], 4, 2, 64, False)
+    c["k"], c["v"] = (torch.cat([x, torch.zeros(2, *x.shape[1:], dtype=x.dtype)]) for x in (c["k"], c["v"]))
+    own = torch.tensor([[len(c["k"]) - 2], [len(c["k"]) - 1]], dtype=torch.int32)
+    with pytest.raises(ValueError, match="kv_evict: sequences share rows of dst_table"):
+        _cut(c, c["table"], dst_table=own[:1].expand(2, -1))
+    assert _cut(c, c["table"], dst_table=own)[1].tolist() == [8, 8]
