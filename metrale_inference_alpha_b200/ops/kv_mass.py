@@ -245,6 +245,10 @@ def kv_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Te
         m = dst_table.shape
         if dst_table.dtype != torch.int32 or len(m) != 2 or m[0] != S or m[1] * bs < min(keep, max_ctx) or (m[1] > 1 and dst_table.stride(1) != 1):
             _bad(where, f"dst_table is int32 [sequences, blocks for {min(keep, max_ctx)} rows]")
+    moved = min(keep, max_ctx) if dst_table is not None else max_ctx if keep < max_ctx else 0       # rows of a sequence that others may not have
+    taken = block_table if dst_table is None else dst_table
+    if S > 1 and taken.stride(0) < (moved + bs - 1) // bs:
+        _bad(where, f"sequences share rows of {'block_table, which are moved in place' if dst_table is None else 'dst_table'}")
     _check_places(where, k_cache, v_cache, block_table, ctx_len, mass, mo, dst_table)
     if not k_cache.is_cuda:
         return ref.kv_evict(k_cache, v_cache, block_table, ctx_len, mass, keep, recent, max_ctx, mo, dst_table)
