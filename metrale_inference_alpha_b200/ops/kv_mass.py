@@ -125,6 +125,18 @@ def _check_rows(where, name, mass) -> None:
         _bad(where, f"rows of {name} share memory")
 
 
+def _tables_overlap(a, b) -> bool:
+    """Whether two int32 tables of as many rows share memory; columns of a table lie next to each other."""
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    (S, m), n, d = a.shape, b.shape[1], (b.data_ptr() - a.data_ptr()) // 4
+    x, y = a.stride(0), b.stride(0)
+    if d >= (S - 1) * x + m or -d >= (S - 1) * y + n:
+        return False
+    # between each other: slices of the rows of one buffer
+    return not (S > 1 and x == y and x >= max(m, n) and d % x >= m and x - d % x >= n)
+
+
 # most bytes of workspace that a call has under way (a decode step's logits, a prompt's queries and the copy of its keys): more sequences go in several steps
 _WS_BYTES = 1 << 30
 
@@ -245,6 +257,8 @@ def kv_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Te
         m = dst_table.shape
         if dst_table.dtype != torch.int32 or len(m) != 2 or m[0] != S or m[1] * bs < min(keep, max_ctx) or (m[1] > 1 and dst_table.stride(1) != 1):
             _bad(where, f"dst_table is int32 [sequences, blocks for {min(keep, max_ctx)} rows]")
+    if dst_table is not None and _tables_overlap(block_table, dst_table):
+        _bad(where, "dst_table and block_table share memory; without dst_table rows move in place")
     moved = min(keep, max_ctx) if dst_table is not None else max_ctx if keep < max_ctx else 0       # rows of a sequence that others may not have
     taken = block_table if dst_table is None else dst_table
     if S > 1 and taken.stride(0) < (moved + bs - 1) // bs:

@@ -234,3 +234,30 @@ def test_evict_refuses_blocks_that_several_sequences_are_to_take():
     with pytest.raises(ValueError, match="kv_evict: sequences share rows of dst_table"):
         _cut(c, c["table"], dst_table=own[:1].expand(2, -1))
     assert _cut(c, c["table"], dst_table=own)[1].tolist() == [8, 8]
+
+
+def test_evict_refuses_its_own_table_as_the_destination():
+    """Cuts in place go without dst_table: rows copied to other blocks are written in any order."""
+    c = oracle.case(18, [40, 40], 4, 2, 64, False)
+    k = c["k"].clone()
+    for dst in (c["table"], c["table"][:, :1], c["table"][:, 1:], c["table"].view(2, -1)):
+        with pytest.raises(ValueError, match="kv_evict: dst_table and block_table share memory"):
+            _cut(c, c["table"], dst_table=dst)
+        assert torch.equal(c["k"].view(torch.int16), k.view(torch.int16))
+
+
+def test_evict_takes_tables_that_lie_beside_each_other():
+    """Halves of one buffer's rows, either of them first, and buffers one behind the other."""
+    for order in (0, 1):
+        c = oracle.case(19, [40, 33], 4, 2, 64, False)
+        n = len(c["k"])
+        c["k"], c["v"] = (torch.cat([x, torch.zeros(2, *x.shape[1:], dtype=x.dtype)]) for x in (c["k"], c["v"]))
+        own = torch.tensor([[n], [n + 1]], dtype=torch.int32)
+        both = torch.cat([own, c["table"]] if order else [c["table"], own], 1)
+        table, dst = (both[:, 1:], both[:, :1]) if order else (both[:, :3], both[:, 3:])
+        k, v, mass, kept, length = oracle.evict(c, 8, 2, 40, own)
+        got = _cut(c, table, dst_table=dst)
+        assert torch.equal(got[0], kept) and torch.equal(got[1], length) and torch.equal(c["k"].view(torch.int16), k.view(torch.int16))
+    c = oracle.case(19, [40, 33], 4, 2, 64, False)
+    flat = torch.cat([c["table"].flatten(), torch.tensor([len(c["k"]) - 2, len(c["k"]) - 1], dtype=torch.int32)])
+    _cut(c, flat[:6].view(2, 3), dst_table=flat[6:].view(2, 1), keep=3, recent=1)
