@@ -272,10 +272,13 @@ def kv_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Te
         return kept.fill_(-1), new_len.zero_()
     own = torch.empty(S * Hkv * (keep + 1), dtype=torch.int32, device=dev)     # of a sequence and head: the rows' slots, the first that moves
     dst = block_table if dst_table is None else dst_table
-    a = _EVICT_ARGS.pack(mass.data_ptr(), mass.stride(0), mass.stride(1), mo.data_ptr(), mo.stride(0), mo.stride(1), ctx_len.data_ptr(), kept.data_ptr(),
-                         new_len.data_ptr(), own.data_ptr() + 4 * S * Hkv * keep, block_table.data_ptr(), block_table.stride(0), dst.data_ptr(), dst.stride(0),
-                         k_cache.data_ptr(), v_cache.data_ptr(), nb, runtime(dev).status.data_ptr(), own.data_ptr(), S, Hkv, keep, recent, max_ctx, bs,
-                         D * k_cache.element_size(), dst_table is None, 0, 0)
-    _native.check(_native.lib().mb_kv_evict(a, _stream()), "kv_evict")
-    _count(2)
+    launch, status = _native.lib().mb_kv_evict, runtime(dev).status.data_ptr()
+    slots, first, tld, dld, row = own.data_ptr(), own.data_ptr() + 4 * S * Hkv * keep, block_table.stride(0), dst.stride(0), 4 * Hkv * keep
+    for s in range(0, S, 65535):
+        a = _EVICT_ARGS.pack(mass.data_ptr() + 4 * s * mass.stride(0), mass.stride(0), mass.stride(1), mo.data_ptr() + 4 * s * mo.stride(0), mo.stride(0), mo.stride(1),
+                             ctx_len.data_ptr() + 4 * s, kept.data_ptr() + s * row, new_len.data_ptr() + 4 * s, first + 4 * s * Hkv, block_table.data_ptr() + 4 * s * tld,
+                             tld, dst.data_ptr() + 4 * s * dld, dld, k_cache.data_ptr(), v_cache.data_ptr(), nb, status, slots + s * row, min(65535, S - s), Hkv, keep,
+                             recent, max_ctx, bs, D * k_cache.element_size(), dst_table is None, 0, 0)
+        _native.check(launch(a, _stream()), "kv_evict")
+        _count(2)
     return kept, new_len

@@ -701,3 +701,50 @@ def test_decode_of_the_largest_and_smallest_queries():
     g = _cuda(c)
     _within(_decode(g), want, tol, "outputs")
     _within(g["mass"], mass, mtol, "mass")
+
+
+# ----------------------------------------------------------------------------- more sequences than a launch takes
+@pytest.mark.parametrize("own_blocks", [False, True])
+def test_evict_of_more_sequences_than_a_launch_takes(own_blocks):
+    """One block each, of three rows, the heavier two of which stay: against indexing."""
+    S, H, D, bs = 65_540, 1, 64, 4
+    g = torch.Generator(device="cuda").manual_seed(90)
+    k, v = (torch.randint(0, 256, (2 * S if own_blocks else S, bs, H, D), generator=g, device="cuda", dtype=torch.uint8) for _ in "kv")
+    table = torch.randperm(S, generator=g, device="cuda").int().view(S, 1)
+    dst = (torch.randperm(S, generator=g, device="cuda").int() + S).view(S, 1) if own_blocks else None
+    ctx = torch.full((S,), 3, dtype=torch.int32, device="cuda")
+    ctx[::7] = 1
+    mass = torch.randperm(4 * S, generator=g, device="cuda").float().view(S, H, 4)          # no two alike
+    first, k0, v0 = mass.clone(), k.clone(), v.clone()
+    least = first[:, 0, :3].argmin(-1)
+    want = torch.stack([(least == 0).long(), 2 - (least == 2).long()], 1)
+    want[::7] = torch.tensor([0, -1], device="cuda")
+    kept, length = ops.kv_evict(k, v, table, ctx, mass, keep=2, recent=0, max_ctx=3, dst_table=dst)
+    assert torch.equal(kept[:, 0].long(), want) and torch.equal(length, ctx.clamp(max=2))
+    live, to = want >= 0, (table if dst is None else dst).long()[:, 0]
+    assert torch.equal(mass[:, 0, :2], torch.where(live, first[:, 0].gather(1, want.clamp(min=0)), 0.0)) and not mass[:, 0, 2].any() and torch.equal(mass[:, :, 3], first[:, :, 3])
+    for new, old in ((k, k0), (v, v0)):
+        rows = old[table.long()[:, 0]][torch.arange(S, device="cuda")[:, None], want.clamp(min=0)]
+        assert torch.equal(new[to][:, :2][live], rows[live])
+
+
+def test_prompts_and_decode_of_more_sequences_than_a_launch_takes():
+    """Single tokens that see one or two rows: against the weights of two."""
+    S, D = 65_540, 64
+    g = torch.Generator(device="cuda").manual_seed(91)
+    k = torch.randn(S, 2, 1, D, generator=g, device="cuda").bfloat16()
+    q = torch.randn(S, 1, D, generator=g, device="cuda").bfloat16()
+    ctx = torch.ones(S, dtype=torch.int32, device="cuda")
+    ctx[1::3] = 2
+    table, start = torch.randperm(S, generator=g, device="cuda").int().view(S, 1), torch.arange(S, dtype=torch.int32, device="cuda")
+    z = torch.einsum("sd,snd->sn", q[:, 0].double(), k[table[:, 0].long()][:, :, 0].double()) * D ** -0.5
+    z[ctx == 1, 1] = -math.inf
+    want = torch.softmax(z, -1)
+    for form in ("prompt", "decode"):
+        mass = torch.zeros(S, 1, 2, device="cuda")
+        if form == "prompt":
+            ops.prompt_mass(q, k, table, start, torch.ones_like(start), ctx, mass, max_q_len=1, max_ctx=2, scale=D ** -0.5)
+        else:
+            ops.paged_attention_mass(q, k, k, table, ctx, mass, max_ctx=2, scale=D ** -0.5)
+        # scores of some 50 terms of size one, 64 additions off by 2^-23 of 12 each at most
+        assert float((mass[:, 0].double() - want).abs().max()) <= 64 * 2.0 ** -23 * 12
