@@ -105,6 +105,16 @@ def _check_places(where, *tensors) -> None:
         _bad(where, f"tensors lie on device {dev}, the current device is another one")
 
 
+def _check_values(where, nb, bs, ctx_len, max_ctx, *tables) -> None:
+    """CPU: what the kernels cut and report is refused. Each of `tables` comes with the rows of every sequence that are looked up in it."""
+    if bool((ctx_len > max_ctx).any()):
+        _bad(where, f"a length of ctx_len is beyond max_ctx {max_ctx}")
+    for table, rows in tables:
+        used = torch.arange(table.shape[1]) * bs < rows[:, None]
+        if bool((used & ((table < 0) | (table >= nb))).any()):
+            _bad(where, f"a table has a block that the cache of {nb} does not have")
+
+
 def _check_scales(where, cache, scale, *scales) -> None:
     if not scale > 0:
         _bad(where, "scale is positive")
@@ -158,7 +168,7 @@ def paged_attention_mass(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     q [S, Hq, D] bf16 -> [S, Hq, D] bf16, and mass[s, h, j] grows by the weights that the query heads of kv head h give to
     cached row j (they sum to Hq / Hkv over j). The new token's own row is one of the ``ctx_len``. A sequence of length 0 (a lane
     that pads the batch) gives zeros and leaves its mass. A length beyond ``max_ctx`` or a block that the cache does not have sets the
-    status word (`check_status`)."""
+    status word (`check_status`); on the CPU it is refused. A CUDA call of no sequences or with a ``max_ctx`` of 0 looks at neither."""
     where = "paged_attention_mass"
     S, nb, bs, Hkv, D = _check_cache(where, k_cache, v_cache, block_table, ctx_len, mass, max_ctx)
     Hq = _check_queries(where, q, S, Hkv, D)
@@ -168,6 +178,7 @@ def paged_attention_mass(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     _check_scales(where, k_cache, scale, k_scale, v_scale)
     _check_places(where, q, k_cache, v_cache, block_table, ctx_len, mass, k_scale, v_scale)
     if not q.is_cuda:
+        _check_values(where, nb, bs, ctx_len, max_ctx, (block_table, ctx_len))
         return ref.paged_attention_mass(q, k_cache, v_cache, block_table, ctx_len, mass, scale, k_scale, v_scale)
     if S == 0 or max_ctx == 0:
         return torch.zeros_like(q)
@@ -193,7 +204,7 @@ def prompt_mass(q: torch.Tensor, k_cache: torch.Tensor, block_table: torch.Tenso
     ``mass``, which is returned. q [rows, Hq, D] bf16 holds the portions one behind the other as for ``paged_attention`` (sequence s: rows
     q_start[s] to q_start[s] + q_len[s], the last q_len[s] of its ctx_len[s] cached tokens; each token sees those up to itself). Rows
     that see nothing give nothing. A length beyond ``max_q_len`` or ``max_ctx``, rows that q does not have and blocks that the cache
-    does not have set the status word."""
+    does not have set the status word; on the CPU they are refused. A CUDA call of no sequences, no rows or with a maximum of 0 looks at none of them."""
     where = "prompt_mass"
     S, nb, bs, Hkv, D = _check_cache(where, k_cache, None, block_table, ctx_len, mass, max_ctx)
     Hq = _check_queries(where, q, -1, Hkv, D)
@@ -208,6 +219,11 @@ def prompt_mass(q: torch.Tensor, k_cache: torch.Tensor, block_table: torch.Tenso
     _check_scales(where, k_cache, scale, k_scale)
     _check_places(where, q, k_cache, block_table, q_start, q_len, ctx_len, mass, k_scale)
     if not q.is_cuda:
+        _check_values(where, nb, bs, ctx_len, max_ctx, (block_table, torch.where(q_len > 0, ctx_len, 0)))
+        if bool((q_len > max_q_len).any()):
+            _bad(where, f"a length of q_len is beyond max_q_len {max_q_len}")
+        if bool(((q_len > 0) & ((q_start < 0) | (q_start.long() + q_len > q.shape[0]))).any()):
+            _bad(where, f"a portion has rows of q beyond its {q.shape[0]}")
         return ref.prompt_mass(q, k_cache, block_table, q_start, q_len, ctx_len, mass, scale, last, k_scale)
     if S == 0 or q.shape[0] == 0 or max_q_len == 0 or max_ctx == 0:
         return mass
@@ -236,7 +252,8 @@ def kv_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Te
     ``dst_table`` [S, >= keep rows' blocks]: blocks that take the rows, none of which a sequence of the call reads; the source's stay as
     they were, so that they may be shared with a prefix cache or other sequences. Without it the rows move inside the sequence's own
     blocks, which then no other sequence may hold. ``mass_out`` takes the mass of the rows that stay and zeros behind them up to column
-    ``max_ctx``; without it ``mass`` does. A length beyond ``max_ctx`` or a block that the cache does not have sets the status word."""
+    ``max_ctx``; without it ``mass`` does. A length beyond ``max_ctx`` or a block that the cache does not have sets the status word; on the CPU it is
+    refused. A CUDA call of no sequences or with a ``max_ctx`` of 0 looks at neither."""
     where = "kv_evict"
     S, nb, bs, Hkv, D = _check_cache(where, k_cache, v_cache, block_table, ctx_len, mass, max_ctx)
     if abs(k_cache.data_ptr() - v_cache.data_ptr()) < k_cache.numel() * k_cache.element_size():
@@ -265,6 +282,7 @@ def kv_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Te
         _bad(where, f"sequences share rows of {'block_table, which are moved in place' if dst_table is None else 'dst_table'}")
     _check_places(where, k_cache, v_cache, block_table, ctx_len, mass, mo, dst_table)
     if not k_cache.is_cuda:
+        _check_values(where, nb, bs, ctx_len, max_ctx, (block_table, ctx_len), *([] if dst_table is None else [(dst_table, ctx_len.clamp(max=keep))]))
         return ref.kv_evict(k_cache, v_cache, block_table, ctx_len, mass, keep, recent, max_ctx, mo, dst_table)
     dev = k_cache.device
     kept, new_len = torch.empty(S, Hkv, keep, dtype=torch.int32, device=dev), torch.empty(S, dtype=torch.int32, device=dev)

@@ -261,3 +261,52 @@ def test_evict_takes_tables_that_lie_beside_each_other():
     c = oracle.case(19, [40, 33], 4, 2, 64, False)
     flat = torch.cat([c["table"].flatten(), torch.tensor([len(c["k"]) - 2, len(c["k"]) - 1], dtype=torch.int32)])
     _cut(c, flat[:6].view(2, 3), dst_table=flat[6:].view(2, 1), keep=3, recent=1)
+
+
+# ----------------------------------------------------------------------------- what the kernels report
+def _state(c):
+    return [x.clone().view(torch.uint8) for x in (c["k"], c["v"], c["mass"])]
+
+
+def test_lengths_and_blocks_out_of_range_are_refused_on_the_cpu():
+    """A CUDA call cuts them and sets the status word; here nothing is written."""
+    c = oracle.case(21, [40, 33], 4, 2, 64, False, new=[3, 2], columns=50)
+    one = {**c, "q": c["q"][:2]}
+    before = _state(c)
+    bad = c["table"].clone()
+    bad[1, 1] = len(c["k"])
+    negative = c["table"].clone()
+    negative[0, 2] = -1
+    for table in (bad, negative):
+        with pytest.raises(ValueError, match="paged_attention_mass: .*block"):
+            _decode({**one, "table": table})
+        with pytest.raises(ValueError, match="prompt_mass: .*block"):
+            _prompt({**c, "table": table}, 0)
+        with pytest.raises(ValueError, match="kv_evict: .*block"):
+            ops.kv_evict(c["k"], c["v"], table, c["ctx"], c["mass"], keep=8, recent=2, max_ctx=40)
+        with pytest.raises(ValueError, match="kv_evict: .*block"):
+            ops.kv_evict(c["k"], c["v"], c["table"], c["ctx"], c["mass"], keep=40, recent=2, max_ctx=40, dst_table=table.clone() - 1000)
+    with pytest.raises(ValueError, match="paged_attention_mass: .*max_ctx"):
+        _decode({**one, "max_ctx": 39})
+    with pytest.raises(ValueError, match="prompt_mass: .*max_ctx"):
+        _prompt({**c, "max_ctx": 39}, 0)
+    with pytest.raises(ValueError, match="kv_evict: .*max_ctx"):
+        ops.kv_evict(c["k"], c["v"], c["table"], c["ctx"], c["mass"], keep=8, recent=2, max_ctx=20)
+    call = dict(max_q_len=3, max_ctx=40, scale=c["scale"], last=0)
+    with pytest.raises(ValueError, match="prompt_mass: .*max_q_len"):
+        ops.prompt_mass(c["q"], c["k"], c["table"], c["q_start"], c["q_len"], c["ctx"], c["mass"], **{**call, "max_q_len": 2})
+    for start in ([-5, 3], [0, 4]):
+        with pytest.raises(ValueError, match="prompt_mass: .*rows of q"):
+            ops.prompt_mass(c["q"], c["k"], c["table"], torch.tensor(start, dtype=torch.int32), c["q_len"], c["ctx"], c["mass"], **call)
+    assert all(torch.equal(a, b) for a, b in zip(before, _state(c)))
+
+
+def test_blocks_that_no_row_lies_in_are_not_looked_at():
+    """Columns of a table behind a sequence's last block, and rows of sequences without tokens, may hold anything."""
+    c = oracle.case(22, [40, 17, 0], 4, 2, 64, False, new=[3, 2, 0])
+    c["table"][1, 2], c["table"][2] = 10 ** 6, -7
+    before = c["mass"].clone()
+    _prompt(c, 0)
+    _decode({**c, "q": c["q"][:3]})
+    assert torch.equal(c["mass"][2], before[2]) and bool((c["mass"][1, :, :17] != before[1, :, :17]).any())
+    assert ops.kv_evict(c["k"], c["v"], c["table"], c["ctx"], c["mass"], keep=8, recent=2, max_ctx=40)[1].tolist() == [8, 8, 0]
