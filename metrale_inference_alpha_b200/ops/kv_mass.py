@@ -167,7 +167,7 @@ def paged_attention_mass(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     """Attention of one new token a sequence over a paged cache, as ``paged_attention``, whose weights are added up:
     q [S, Hq, D] bf16 -> [S, Hq, D] bf16, and mass[s, h, j] grows by the weights that the query heads of kv head h give to
     cached row j (they sum to Hq / Hkv over j). The new token's own row is one of the ``ctx_len``. A sequence of length 0 (a lane
-    that pads the batch) gives zeros and leaves its mass. A length beyond ``max_ctx`` or a block that the cache does not have sets the
+    that pads the batch) gives zeros and leaves its mass, and so does a row whose scores are all -inf. A length beyond ``max_ctx`` or a block that the cache does not have sets the
     status word (`check_status`); on the CPU it is refused. A CUDA call of no sequences or with a ``max_ctx`` of 0 looks at neither."""
     where = "paged_attention_mass"
     S, nb, bs, Hkv, D = _check_cache(where, k_cache, v_cache, block_table, ctx_len, mass, max_ctx)
@@ -203,7 +203,7 @@ def prompt_mass(q: torch.Tensor, k_cache: torch.Tensor, block_table: torch.Tenso
     """The weights that the last ``last`` tokens of every sequence's portion (0: all of them) give to what is cached, added to
     ``mass``, which is returned. q [rows, Hq, D] bf16 holds the portions one behind the other as for ``paged_attention`` (sequence s: rows
     q_start[s] to q_start[s] + q_len[s], the last q_len[s] of its ctx_len[s] cached tokens; each token sees those up to itself). Rows
-    that see nothing give nothing. A length beyond ``max_q_len`` or ``max_ctx``, rows that q does not have and blocks that the cache
+    that see nothing, or nothing but scores of -inf, give nothing. A length beyond ``max_q_len`` or ``max_ctx``, rows that q does not have and blocks that the cache
     does not have set the status word; on the CPU they are refused. A CUDA call of no sequences, no rows or with a maximum of 0 looks at none of them."""
     where = "prompt_mass"
     S, nb, bs, Hkv, D = _check_cache(where, k_cache, None, block_table, ctx_len, mass, max_ctx)

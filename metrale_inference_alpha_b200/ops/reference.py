@@ -312,11 +312,11 @@ def _cached_rows(cache, block_table, s: int, rows: torch.Tensor, scale=None) -> 
 
 def _weights(q, k, limits, scale: float) -> torch.Tensor:
     """Softmax weights [W, Hkv, G, n] of queries q [W, Hkv, G, D] that see the first limits[w] rows of k [n, Hkv, D]; rows that see nothing
-    have none."""
+    have none, nor do rows whose scores are all -inf."""
     z = torch.einsum("whgd,nhd->whgn", q.float(), k) * scale
     seen = (torch.arange(k.shape[0]) < limits[:, None])[:, None, None]
-    p = torch.softmax(z.masked_fill(~seen, float("-inf")), -1)
-    return torch.where(seen, p, torch.zeros_like(p))
+    z = z.masked_fill(~seen, float("-inf"))
+    return torch.where(seen & (z.amax(-1, keepdim=True) != float("-inf")), torch.softmax(z, -1), 0.0)
 
 
 def paged_attention_mass(q, k_cache, v_cache, block_table, ctx_len, mass, scale: float, k_scale=None, v_scale=None) -> torch.Tensor:

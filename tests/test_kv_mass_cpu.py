@@ -310,3 +310,15 @@ def test_blocks_that_no_row_lies_in_are_not_looked_at():
     _decode({**c, "q": c["q"][:3]})
     assert torch.equal(c["mass"][2], before[2]) and bool((c["mass"][1, :, :17] != before[1, :, :17]).any())
     assert ops.kv_evict(c["k"], c["v"], c["table"], c["ctx"], c["mass"], keep=8, recent=2, max_ctx=40)[1].tolist() == [8, 8, 0]
+
+
+def test_rows_whose_scores_are_all_minus_infinity_give_nothing():
+    """As rows that see nothing, here and in the kernels: no key has a weight."""
+    c = oracle.case(23, [1, 20], 2, 2, 64, False, new=[1, 3])
+    c["k"][c["table"][0, 0], 0, 1, 5] = -math.inf
+    c["q"][0, 1, 5] = 1.0
+    before = c["mass"].clone()
+    _prompt(c, 0)
+    assert float(c["mass"][0, 0, 0]) == pytest.approx(float(before[0, 0, 0]) + 1) and torch.equal(c["mass"][0, 1], before[0, 1]) and not c["mass"].isnan().any()
+    out = _decode({**c, "q": c["q"][[0, 3]].contiguous()})
+    assert not out[0, 1].any() and out[0, 0].any() and torch.equal(c["mass"][0, 1], before[0, 1]) and not c["mass"].isnan().any()

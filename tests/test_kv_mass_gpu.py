@@ -748,3 +748,23 @@ def test_prompts_and_decode_of_more_sequences_than_a_launch_takes():
             ops.paged_attention_mass(q, k, k, table, ctx, mass, max_ctx=2, scale=D ** -0.5)
         # scores of some 50 terms of size one, 64 additions off by 2^-23 of 12 each at most
         assert float((mass[:, 0].double() - want).abs().max()) <= 64 * 2.0 ** -23 * 12
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_rows_whose_scores_are_all_minus_infinity_give_nothing(dim):
+    c = oracle.case(74, [1, 700, 1100], 2, 2, dim, False, new=[1, 3, 1])
+    c["q"][:, 1, 5] = 1.0
+    for s, n in ((0, 1), (1, 699), (2, 1100)):               # all that the only row sees; all but what the newest row sees last; all
+        for j in range(n):
+            _set_key(c, s, j, 1, -math.inf, 5)
+    g = _cuda(c)
+    before = g["mass"].clone()
+    _prompt(g, 0)
+    gained = (g["mass"] - before).double().sum(-1)
+    # two of the second sequence's three rows see only what weighs nothing
+    assert torch.allclose(gained.cpu(), torch.tensor([[1.0, 0.0], [3.0, 1.0], [1.0, 0.0]]).double(), atol=1e-3)
+    before = g["mass"].clone()
+    out = _decode({**g, "q": g["q"][[0, 3, 4]].contiguous()})
+    assert not out[0, 1].any() and not out[2, 1].any() and not out.isnan().any() and out[1, 1].any()
+    gained = (g["mass"] - before).double().sum(-1)
+    assert torch.allclose(gained.cpu(), torch.tensor([[1.0, 0.0], [1.0, 1.0], [1.0, 0.0]]).double(), atol=1e-3)
