@@ -50,7 +50,7 @@ __device__ __forceinline__ Span span_of(const MbMassArgs& a, int s, int G) {
   bool bad = n > a.max_ctx || ql > a.max_q_len;
   n = max(min(n, a.max_ctx), 0);
   ql = max(min(ql, a.max_q_len), 0);
-  if (start < 0 || start + ql > a.q_rows) {
+  if (ql > 0 && (start < 0 || start + ql > a.q_rows)) {
     bad = true;
     ql = 0;
   }

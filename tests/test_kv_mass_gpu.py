@@ -768,3 +768,15 @@ def test_rows_whose_scores_are_all_minus_infinity_give_nothing(dim):
     assert not out[0, 1].any() and not out[2, 1].any() and not out.isnan().any() and out[1, 1].any()
     gained = (g["mass"] - before).double().sum(-1)
     assert torch.allclose(gained.cpu(), torch.tensor([[1.0, 0.0], [1.0, 1.0], [1.0, 0.0]]).double(), atol=1e-3)
+
+
+def test_prompt_lanes_without_rows_may_begin_anywhere():
+    """Lanes that pad a batch: no rows, so their start is not looked at (the fixture sees that nothing is reported)."""
+    c = _cuda(oracle.case(75, [200, 60, 90], 8, 2, 128, False, new=[40, 0, 90]))
+    m = c["mass"].clone()
+    _prompt(c, 0)
+    for start in (-1, 10 ** 6, 2 ** 31 - 1, -2 ** 31):
+        again = m.clone()
+        _prompt({**c, "mass": again, "q_start": torch.tensor([0, start, 40], dtype=torch.int32, device="cuda")}, 0)
+        ops.check_status("cuda")
+        assert _same(again, c["mass"])
