@@ -113,6 +113,9 @@ bool bad_shape(const MbMassArgs& a) {
 
 extern "C" {
 
+// Sizes of the argument structures, which the caller packs by hand and compares before its first call.
+size_t mb_kv_mass_args(int which) { return which == 0 ? sizeof(MbMassArgs) : which == 1 ? sizeof(MbEvictArgs) : 0; }
+
 size_t mb_attn_mass_ws(int num_seqs, int Hq, int D, int max_ctx) { return mbm::decode_ws(num_seqs, Hq, D, max_ctx, kPartTokens).bytes; }
 
 int mb_attn_mass(const MbMassArgs* a, cudaStream_t stream) {

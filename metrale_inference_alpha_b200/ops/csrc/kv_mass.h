@@ -52,6 +52,10 @@ struct MbEvictArgs {
   unsigned block_magic;      // and this: a division by block_size
 };
 
+// as ops/kv_mass.py packs them
+static_assert(sizeof(MbMassArgs) == 200, "field by field in ops/kv_mass.py too");
+static_assert(sizeof(MbEvictArgs) == 192, "field by field in ops/kv_mass.py too");
+
 namespace mbm {
 
 constexpr int kMaxParts = 32;

@@ -40,13 +40,29 @@ for _name in ("mb_attn_mass", "mb_prompt_mass", "mb_kv_evict"):
     _native.register_optional(_name, [C.c_char_p, C.c_void_p])
 
 
+_lib = None
+
+
+def _library():
+    """The kernel library, once its structures have been found to be those that are packed here."""
+    global _lib
+    if _lib is None:
+        L = _native.lib()
+        size = L.mb_kv_mass_args
+        size.argtypes, size.restype = [C.c_int], C.c_size_t
+        if (size(0), size(1)) != (_MASS_ARGS.size, _EVICT_ARGS.size):
+            raise RuntimeError(f"{_native.LIB_PATH} has argument structures of other sizes: build it again")
+        _lib = L
+    return _lib
+
+
 _ws_bytes: dict = {}
 
 
 def _workspace(name: str, *sizes) -> int:
     fn = _ws_bytes.get(name)
     if fn is None:
-        fn = getattr(_native.lib(), name)
+        fn = getattr(_library(), name)
         fn.restype, fn.argtypes = C.c_size_t, [C.c_int] * len(sizes)
         _ws_bytes[name] = fn
     return fn(*sizes)
@@ -183,7 +199,7 @@ def paged_attention_mass(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     if S == 0 or max_ctx == 0:
         return torch.zeros_like(q)
     out = torch.empty_like(q)
-    launch, rt = _native.lib().mb_attn_mass, runtime(q.device)
+    launch, rt = _library().mb_attn_mass, runtime(q.device)
     step, need = _step("mb_attn_mass_ws", S, 1024, Hq, D, max_ctx)
     ws = torch.empty(need, dtype=torch.uint8, device=q.device)
     fp8 = int(k_cache.dtype == torch.uint8)
@@ -231,7 +247,7 @@ def prompt_mass(q: torch.Tensor, k_cache: torch.Tensor, block_table: torch.Tenso
     if seen * (Hq // Hkv) > 1 << 25:
         _bad(where, f"{seen} tokens of {Hq // Hkv} heads a group are more than 2^25 rows")
     step, need = _step("mb_prompt_mass_ws", S, 65535, Hq, Hkv, D, bs, seen, max_ctx, fp8)
-    ws, rt, launch = torch.empty(need, dtype=torch.uint8, device=q.device), runtime(q.device), _native.lib().mb_prompt_mass
+    ws, rt, launch = torch.empty(need, dtype=torch.uint8, device=q.device), runtime(q.device), _library().mb_prompt_mass
     tp, qs, ql, cp, mp, tld, mseq = (block_table.data_ptr(), q_start.data_ptr(), q_len.data_ptr(), ctx_len.data_ptr(), mass.data_ptr(), block_table.stride(0),
                                      mass.stride(0))
     for s in range(0, S, step):
@@ -290,7 +306,7 @@ def kv_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Te
         return kept.fill_(-1), new_len.zero_()
     own = torch.empty(S * Hkv * (keep + 1), dtype=torch.int32, device=dev)     # of a sequence and head: the rows' slots, the first that moves
     dst = block_table if dst_table is None else dst_table
-    launch, status = _native.lib().mb_kv_evict, runtime(dev).status.data_ptr()
+    launch, status = _library().mb_kv_evict, runtime(dev).status.data_ptr()
     slots, first, tld, dld, row = own.data_ptr(), own.data_ptr() + 4 * S * Hkv * keep, block_table.stride(0), dst.stride(0), 4 * Hkv * keep
     for s in range(0, S, 65535):
         a = _EVICT_ARGS.pack(mass.data_ptr() + 4 * s * mass.stride(0), mass.stride(0), mass.stride(1), mo.data_ptr() + 4 * s * mo.stride(0), mo.stride(0), mo.stride(1),

@@ -1,5 +1,8 @@
 """The CPU form of the operators that hold a cache to a budget by attention weight, and what they refuse."""
 import math
+import re
+import struct
+from pathlib import Path
 
 import pytest
 import torch
@@ -322,3 +325,39 @@ def test_rows_whose_scores_are_all_minus_infinity_give_nothing():
     assert float(c["mass"][0, 0, 0]) == pytest.approx(float(before[0, 0, 0]) + 1) and torch.equal(c["mass"][0, 1], before[0, 1]) and not c["mass"].isnan().any()
     out = _decode({**c, "q": c["q"][[0, 3]].contiguous()})
     assert not out[0, 1].any() and out[0, 0].any() and torch.equal(c["mass"][0, 1], before[0, 1]) and not c["mass"].isnan().any()
+
+
+# ----------------------------------------------------------------------------- packed arguments
+def _fields(name):
+    """Codes of the struct module for the fields of a C structure of kv_mass.h, in order."""
+    path = Path(ops.__file__).parent / "csrc" / "kv_mass.h"
+    body = re.search(r"struct %s \{(.*?)\n\};" % name, path.read_text(), re.S).group(1)
+    codes = ""
+    for decl in re.sub(r"//[^\n]*", "", body).replace("\n", " ").split(";"):
+        if not decl.strip():
+            continue
+        kind, names = re.match(r"\s*(const void\*|void\*|const int\*|int\*|const float\*|float\*|uint32_t\*|long long|size_t|unsigned|int|float)\s+(.*)", decl).groups()
+        codes += ("P" if kind.endswith("*") else {"long long": "q", "size_t": "N", "unsigned": "i", "int": "i", "float": "f"}[kind]) * len(names.split(","))
+    return codes
+
+
+@pytest.mark.parametrize("name", ["MbMassArgs", "MbEvictArgs"])
+def test_packed_arguments_are_the_structures_of_the_library(name):
+    from metrale_inference_alpha_b200.ops import kv_mass
+    packed = kv_mass._MASS_ARGS if name == "MbMassArgs" else kv_mass._EVICT_ARGS
+    form = packed.format
+    assert form[0] == "@" and "".join(code * int(n or 1) for n, code in re.findall(r"(\d*)([A-Za-z])", form) if code != "x") == _fields(name)
+    sizes = re.search(r"static_assert\(sizeof\(%s\) == (\d+)" % name, (Path(ops.__file__).parent / "csrc" / "kv_mass.h").read_text())
+    assert int(sizes.group(1)) == packed.size
+
+
+def test_packed_arguments_of_another_size_are_refused(monkeypatch):
+    """The launchers copy a structure whole: the sides have to agree on its size before a call is made."""
+    from metrale_inference_alpha_b200.ops import kv_mass
+    monkeypatch.setattr(kv_mass, "_lib", None)
+    size = kv_mass._library().mb_kv_mass_args
+    assert [size(0), size(1), size(2)] == [kv_mass._MASS_ARGS.size, kv_mass._EVICT_ARGS.size, 0]
+    monkeypatch.setattr(kv_mass, "_lib", None)
+    monkeypatch.setattr(kv_mass, "_EVICT_ARGS", struct.Struct(kv_mass._EVICT_ARGS.format + "q"))
+    with pytest.raises(RuntimeError, match="build it again"):
+        kv_mass._library()
