@@ -780,3 +780,89 @@ def test_prompt_lanes_without_rows_may_begin_anywhere():
         _prompt({**c, "mass": again, "q_start": torch.tensor([0, start, 40], dtype=torch.int32, device="cuda")}, 0)
         ops.check_status("cuda")
         assert _same(again, c["mass"])
+
+
+# ----------------------------------------------------------------------------- few observers over long contexts, and very many rows
+# More parts of a row than a CTA joins by itself (8193 tokens on), parts that grow with the context (16385 on), at one and two tiles of rows
+LONG = [8193, 16385, 33000]
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("n", LONG)
+@pytest.mark.parametrize("heads,kv_heads,dim,last", [(10, 2, 128, 24), (10, 2, 128, 32), (3, 1, 64, 64), (16, 1, 256, 8), (16, 1, 256, 32), (4, 4, 128, 300)])
+def test_prompt_of_a_long_context(heads, kv_heads, dim, last, n, fp8):
+    """In a batch with short ones, against 64 bits, and alone with the same bits."""
+    ctx, new = [n, 700, 40], [min(n, last + 7), 300, 40]
+    c = oracle.case(76, ctx, heads, kv_heads, dim, fp8, new=new)
+    mass, mtol = oracle.prompt(c, last)
+    g = _cuda(c)
+    m = g["mass"].clone()
+    _prompt(g, last)
+    _within(g["mass"], mass, mtol, "mass")
+    for s in range(3):
+        one = {k: g[k][s:s + 1] for k in ("table", "ctx", "q_start", "q_len")}
+        _prompt({**g, **one, "mass": m[s:s + 1]}, last, max_q_len=new[s], max_ctx=ctx[s])
+        assert _same(m[s], g["mass"][s])
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("last", [32, 60])
+def test_prompt_of_a_long_context_with_keys_that_are_no_numbers(last, fp8):
+    """As the first, a middle and the newest key, through the join of many parts."""
+    for at in (0, 9000, 16999):
+        c = oracle.case(77, [17000, 300], 8, 2, 128, fp8, new=[64, 64])
+        _set_key(c, 0, at, 1, math.nan, 3)
+        want, _, tol = _defined(c, last)
+        g = _cuda(c)
+        _prompt(g, last)
+        _as_defined(g["mass"], want, tol)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_prompt_of_more_than_65536_rows(fp8):
+    """Where parts of a column are longer than the least: 64 heads a kv head, against 64 bits on the device."""
+    n, G, D = 1100, 64, 64
+    c = _cuda(oracle.case(78, [n, 50], G, 1, D, fp8, new=[n, 50]))
+    before = c["mass"].clone()
+    _prompt(c, 0)
+    q0 = 0
+    for s, m in enumerate((n, 50)):
+        k = oracle.rows_of(c["k"], c["table"], s, torch.arange(m, device="cuda"), c["k_scale"])[:, 0]
+        add, size = torch.zeros(m, dtype=torch.float64, device="cuda"), 0.0
+        unseen = torch.arange(m, device="cuda") > torch.arange(m, device="cuda")[:, None]
+        for h in range(G):
+            q = c["q"][q0:q0 + m, h].double()
+            add += torch.softmax((q @ k.T * c["scale"]).masked_fill(unseen, -math.inf), -1).sum(0)
+            size = max(size, float((q.abs() @ k.abs().T).max()) * c["scale"] * oracle.LOG2E)
+        q0 += m
+        want = before[s, 0, :m].double() + add
+        tol = (oracle.weight_error({**c, "k": c["k"].cpu()}, D, size) + m * G * 2.0 ** -24) * add + 2.0 ** -23 * want
+        _within(c["mass"][s, 0, :m], want.cpu(), tol.cpu(), f"mass of sequence {s}")
+
+
+# ----------------------------------------------------------------------------- without programmatic dependence, and with it everywhere
+@pytest.mark.parametrize("fp8", [False, True])
+def test_the_same_bits_however_kernels_are_launched(fp8):
+    """Launches that wait for the one in front as a whole, the default, and all of them programmatic, where each kernel has to wait by itself: a prompt, its
+    cut, decode and a cut in place, one behind the other."""
+    base = _cuda(oracle.case(79, [900, 130, 2100], 10, 2, 128, fp8, new=[60, 130, 300]))
+    gen = torch.Generator(device="cuda").manual_seed(80)
+    q1 = torch.randn(3, 10, 128, generator=gen, device="cuda").bfloat16()
+    own = (len(base["k"]) + torch.arange(3 * 20, dtype=torch.int32, device="cuda")).view(3, 20)
+    spare = torch.zeros(60, *base["k"].shape[1:], dtype=base["k"].dtype, device="cuda")
+    lib, results = _native.lib(), []
+    default = lib.mb_pdl_enabled()
+    try:
+        for mode in (0, 1, 2, 1, 0):
+            lib.mb_set_pdl(mode)
+            c = {**base, "k": torch.cat([base["k"], spare]), "v": torch.cat([base["v"], spare]), "mass": base["mass"].clone()}
+            for last in (0, 20):
+                _prompt(c, last)
+            kept, n = ops.kv_evict(c["k"], c["v"], c["table"], c["ctx"], c["mass"], keep=310, recent=10, max_ctx=c["max_ctx"], dst_table=own)
+            outs = [_decode({**c, "q": q1, "table": own, "ctx": n}, max_ctx=320) for _ in range(3)]
+            again, n2 = ops.kv_evict(c["k"], c["v"], own, n, c["mass"], keep=128, recent=10, max_ctx=320)
+            results.append((*outs, kept, n, again, n2, c["mass"], c["k"], c["v"]))
+    finally:
+        lib.mb_set_pdl(default)
+    for r in results[1:]:
+        assert all(_same(a, b) for a, b in zip(results[0], r))
