@@ -136,8 +136,8 @@ def _check_scales(where, cache, scale, *scales) -> None:
         _bad(where, "scale is positive")
     if cache.dtype == torch.uint8:
         for s in scales:
-            if s is None or s.dtype != torch.float32 or s.numel() < 1:
-                _bad(where, "an e4m3 cache comes with fp32 scales")
+            if s is None or s.dtype != torch.float32 or s.numel() != 1:
+                _bad(where, "an e4m3 cache comes with fp32 scales of one element")
 
 
 def _check_rows(where, name, mass) -> None:

@@ -361,3 +361,17 @@ def test_packed_arguments_of_another_size_are_refused(monkeypatch):
     monkeypatch.setattr(kv_mass, "_EVICT_ARGS", struct.Struct(kv_mass._EVICT_ARGS.format + "q"))
     with pytest.raises(RuntimeError, match="build it again"):
         kv_mass._library()
+
+
+def test_scales_of_several_elements_are_refused():
+    """A cache has one scale for its keys and one for its values; the kernels would take the first of several."""
+    c = oracle.case(24, [40], 4, 2, 64, True)
+    for name in ("k_scale", "v_scale"):
+        for wrong in (c[name].repeat(2), torch.ones(2, 1), torch.ones(0)):
+            with pytest.raises(ValueError, match="scales of one element"):
+                _decode({**c, name: wrong})
+    with pytest.raises(ValueError, match="scales of one element"):
+        _prompt({**c, "k_scale": torch.ones(2)}, 1)
+    before = c["mass"].clone()
+    _decode({**c, "k_scale": c["k_scale"][0], "v_scale": c["v_scale"].view(1, 1)})
+    assert bool((c["mass"] != before).any())
