@@ -151,6 +151,23 @@ def _check_rows(where, name, mass) -> None:
         _bad(where, f"rows of {name} share memory")
 
 
+def _columns_overlap(x, y) -> bool:
+    """Whether two fp32 buffers [S, H, columns] of as many rows share memory, or may: of those that lie between each other parts of one buffer are told apart."""
+    if x.numel() == 0 or y.numel() == 0:
+        return False
+    d = (y.data_ptr() - x.data_ptr()) // 4
+    reach = [1 + sum((n - 1) * st for n, st in zip(t.shape, t.stride())) for t in (x, y)]
+    if d >= reach[0] or -d >= reach[1]:
+        return False
+    (a, b, _), (S, H, n), m = x.stride(), x.shape, y.shape[2]
+    if y.stride()[:2] != (a, b):
+        return True
+    for step, p, q in ((a, (H - 1) * b + n, (H - 1) * b + m), (b if S == 1 or b and a % b == 0 else 0, n, m)):       # windows of a sequence, of a row
+        if step and d % step >= p and step - d % step >= q:
+            return False
+    return True
+
+
 def _tables_overlap(a, b) -> bool:
     """Whether two int32 tables of as many rows share memory; columns of a table lie next to each other."""
     if a.numel() == 0 or b.numel() == 0:
@@ -281,10 +298,8 @@ def kv_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Te
         mo, m = mass_out, mass_out.shape
         if mo.dtype != torch.float32 or len(m) != 3 or m[0] != S or m[1] != Hkv or m[2] < max_ctx or (m[2] > 1 and mo.stride(2) != 1):
             _bad(where, "mass_out is fp32 [sequences, kv heads, at least max_ctx columns]")
-        if mass.numel() and mo.numel() and not (mo.data_ptr() == mass.data_ptr() and mo.stride() == mass.stride()):
-            (a, b), (c, d) = ((t.data_ptr(), t.data_ptr() + 4 * (1 + sum((n - 1) * st for n, st in zip(t.shape, t.stride())))) for t in (mass, mo))
-            if a < d and c < b:
-                _bad(where, "mass_out overlaps mass")
+        if not (mo.data_ptr() == mass.data_ptr() and mo.stride() == mass.stride()) and _columns_overlap(mass, mo):
+            _bad(where, "mass_out overlaps mass")
     _check_rows(where, "mass_out", mo)
     if dst_table is not None:
         m = dst_table.shape

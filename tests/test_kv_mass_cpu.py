@@ -375,3 +375,28 @@ def test_scales_of_several_elements_are_refused():
     before = c["mass"].clone()
     _decode({**c, "k_scale": c["k_scale"][0], "v_scale": c["v_scale"].view(1, 1)})
     assert bool((c["mass"] != before).any())
+
+
+@pytest.mark.parametrize("cut", ["columns", "columns turned", "heads", "sequences", "lanes"])
+def test_evict_takes_mass_and_mass_out_of_one_buffer(cut):
+    """Parts of a buffer that share no element, though they lie between each other."""
+    c = oracle.case(25, [40, 33, 0], 4, 2, 64, False)
+    S, H, n = c["mass"].shape
+    big = torch.full({"heads": (S, 2 * H, n), "sequences": (2 * S, H, n), "lanes": (2 * S, H, n)}.get(cut, (S, H, 2 * n + 1)), 9.0)
+    mass, out = {"columns": (big[:, :, :n], big[:, :, n:2 * n]), "columns turned": (big[:, :, n + 1:], big[:, :, :n]), "heads": (big[:, :H], big[:, H:]),
+                 "sequences": (big[:S], big[S:]), "lanes": (big[::2], big[1::2])}[cut]
+    mass.copy_(c["mass"])
+    want = oracle.evict(c, 10, 2, 40)
+    kept, length = ops.kv_evict(c["k"], c["v"], c["table"], c["ctx"], mass, keep=10, recent=2, max_ctx=40, mass_out=out)
+    assert torch.equal(kept, want[3]) and torch.equal(out, want[2]) and torch.equal(mass, c["mass"])
+    if cut == "columns":
+        assert bool((big[:, :, 2 * n] == 9).all())
+
+
+@pytest.mark.parametrize("shift", [1, 39, 41, 59, 60 * 2 - 1])
+def test_evict_refuses_a_mass_out_that_shares_elements_with_mass(shift):
+    c = oracle.case(26, [40, 33], 4, 2, 64, False)
+    flat = torch.zeros(600)
+    mass, out = flat.as_strided((2, 2, 40), (120, 60, 1)), flat.as_strided((2, 2, 40), (120, 60, 1), shift)
+    with pytest.raises(ValueError, match="kv_evict: mass_out overlaps mass"):
+        ops.kv_evict(c["k"], c["v"], c["table"], c["ctx"], mass, keep=10, recent=2, max_ctx=40, mass_out=out)
