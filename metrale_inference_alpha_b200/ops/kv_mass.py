@@ -11,9 +11,10 @@ differently; a batch of lanes may pass a slice of a larger buffer (columns next 
 
     prompt_mass(q, k, ..., mass, last=32)            # per layer, behind the prompt's attention
     kept, ctx_len = kv_evict(k, v, ..., mass, keep=4096, recent=64, dst_table=blocks)
-    out = paged_attention_mass(q, k, v, blocks, ctx_len + 1, mass, ...)
+    ctx_len = ctx_len + 1                            # a token, its row written at the former ctx_len
+    out = paged_attention_mass(q, k, v, blocks, ctx_len, mass, ...)
 
-with the new token's row written at slot ctx_len and positions counted on as if nothing had gone: a cached key holds its
+with positions counted on as if nothing had gone: a cached key holds its
 own rotation, so rows keep the distances that they had. Eviction leaves a head's rows in the order of their positions;
 they belong to different tokens in different heads, and all have the same number. CUDA tensors run the kernels, CPU tensors
 the fp32 restatements in ``reference.py``.

@@ -400,3 +400,18 @@ def test_evict_refuses_a_mass_out_that_shares_elements_with_mass(shift):
     mass, out = flat.as_strided((2, 2, 40), (120, 60, 1)), flat.as_strided((2, 2, 40), (120, 60, 1), shift)
     with pytest.raises(ValueError, match="kv_evict: mass_out overlaps mass"):
         ops.kv_evict(c["k"], c["v"], c["table"], c["ctx"], mass, keep=10, recent=2, max_ctx=40, mass_out=out)
+
+
+def test_the_loop_of_the_readme_keeps_the_row_of_its_token():
+    """Run as it stands, on sequences that its budget holds whole."""
+    code = re.search(r"```python\n(ops\.prompt_mass.*?)```", (Path(ops.__file__).parents[2] / "README.md").read_text(), re.S).group(1)
+    c = oracle.case(27, [40, 33], 4, 2, 64, False, new=[3, 2], columns=4352)
+    nb = len(c["k"])
+    own = torch.arange(nb, nb + 2 * 272, dtype=torch.int32).view(2, 272)
+    k, v = (torch.cat([x, torch.zeros(2 * 272, *x.shape[1:], dtype=x.dtype)]) for x in (c["k"], c["v"]))
+    names = dict(ops=ops, q=c["q"], new_q=c["q"][:2].contiguous(), k_cache=k, v_cache=v, table=c["table"], own=own, q_start=c["q_start"], q_len=c["q_len"], ctx=c["ctx"],
+                 mass=c["mass"].zero_(), s=c["scale"])
+    exec(code.replace("max_q_len=..., max_ctx=...", "max_q_len=3, max_ctx=40").replace("max_ctx=...", "max_ctx=40"), names)
+    assert names["n"].tolist() == [41, 34] and bool((names["kept"][:, :, 33] == 33).all())
+    gathered = names["mass"].sum(-1)
+    assert torch.allclose(gathered, torch.tensor([[4 * 2.0] * 2, [3 * 2.0] * 2]), rtol=1e-4)
