@@ -287,8 +287,12 @@ observe_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
   // A dependent kernel allocates TMEM: not before this CTA has its own. What the kernel in front writes, only some warps read, and these wait for it: the
   // copies of keys and query rows, the normalisers.
   mb::pdl_launch_dependents();
-  // of a row's scores, in the log2 domain; never 0, which would make numbers of the -inf that a mask leaves
-  auto factor = [&](float row) { return fmaxf(a.scale * (FP8 ? *a.k_scale : 1.f) * 1.44269504088896f * row, 1.17549435e-38f); };
+  // of a row's scores, in the log2 domain; never 0, which would make numbers of the -inf that a mask leaves. A cache's scale that is negative or NaN is none, and
+  // leaves no numbers.
+  auto factor = [&](float row) {
+    const float f = a.scale * (FP8 ? *a.k_scale : 1.f) * 1.44269504088896f * row;
+    return !FP8 || f >= 0.f ? fmaxf(f, 1.17549435e-38f) : NAN;
+  };
 
   if (warp < 8) {
     more_regs<88>();

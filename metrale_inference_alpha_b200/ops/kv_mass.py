@@ -237,7 +237,7 @@ def prompt_mass(q: torch.Tensor, k_cache: torch.Tensor, block_table: torch.Tenso
     """The weights that the last ``last`` tokens of every sequence's portion (0: all of them) give to what is cached, added to
     ``mass``, which is returned. q [rows, Hq, D] bf16 holds the portions one behind the other as for ``paged_attention`` (sequence s: rows
     q_start[s] to q_start[s] + q_len[s], the last q_len[s] of its ctx_len[s] cached tokens; each token sees those up to itself). Rows
-    that see nothing, or nothing but scores of -inf, give nothing. A length beyond ``max_q_len`` or ``max_ctx``, rows that q does not have and blocks that the cache
+    that see nothing, or nothing but scores of -inf, give nothing. ``k_scale`` is positive (what is not leaves NaN). A length beyond ``max_q_len`` or ``max_ctx``, rows that q does not have and blocks that the cache
     does not have set the status word; on the CPU they are refused. A CUDA call of no sequences, no rows or with a maximum of 0 looks at none of them."""
     where = "prompt_mass"
     S, nb, bs, Hkv, D = _check_cache(where, k_cache, None, block_table, ctx_len, mass, max_ctx)

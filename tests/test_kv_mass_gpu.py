@@ -866,3 +866,17 @@ def test_the_same_bits_however_kernels_are_launched(fp8):
         lib.mb_set_pdl(default)
     for r in results[1:]:
         assert all(_same(a, b) for a, b in zip(results[0], r))
+
+
+@pytest.mark.parametrize("last", [4, 0])
+@pytest.mark.parametrize("value", [math.nan, -0.0625])
+def test_prompt_of_a_scale_that_is_none(value, last):
+    """Scales of a cache are positive: weights behind another are no numbers, and not those of equal scores. A scale of zero makes scores equal."""
+    c = _cuda(oracle.case(82, [300, 40], 8, 2, 128, True, new=[300, 3]))
+    m = c["mass"].clone()
+    _prompt({**c, "k_scale": torch.tensor([value], device="cuda")}, last)
+    assert c["mass"][0, :, :300].isnan().all() and c["mass"][1, :, :40].isnan().all()
+    c["mass"] = m.clone()
+    _prompt({**c, "k_scale": torch.zeros(1, device="cuda")}, 1)
+    gained = (c["mass"] - m)[0, :, :300]
+    assert torch.allclose(gained, torch.full_like(gained, 4 / 300), rtol=1e-4)
