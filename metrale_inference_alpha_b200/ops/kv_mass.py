@@ -153,20 +153,18 @@ def _check_rows(where, name, mass) -> None:
 
 
 def _columns_overlap(x, y) -> bool:
-    """Whether two fp32 buffers [S, H, columns] of as many rows share memory, or may: of those that lie between each other parts of one buffer are told apart."""
-    if x.numel() == 0 or y.numel() == 0:
-        return False
+    """Whether two fp32 buffers [S, H, columns] of as many rows share memory, or may, and are not the same rows: of those that lie between each other parts of
+    one buffer are told apart."""
+    (S, H, n), m, (a, b, _), (c, e, _) = x.shape, y.shape[2], x.stride(), y.stride()
     d = (y.data_ptr() - x.data_ptr()) // 4
-    reach = [1 + sum((n - 1) * st for n, st in zip(t.shape, t.stride())) for t in (x, y)]
-    if d >= reach[0] or -d >= reach[1]:
+    if d >= (S - 1) * a + (H - 1) * b + n or -d >= (S - 1) * c + (H - 1) * e + m or not (S and H and n and m):
         return False
-    (a, b, _), (S, H, n), m = x.stride(), x.shape, y.shape[2]
-    if y.stride()[:2] != (a, b):
+    if (a != c and S > 1) or (b != e and H > 1):
         return True
     for step, p, q in ((a, (H - 1) * b + n, (H - 1) * b + m), (b if S == 1 or b and a % b == 0 else 0, n, m)):       # windows of a sequence, of a row
         if step and d % step >= p and step - d % step >= q:
             return False
-    return True
+    return d != 0
 
 
 def _tables_overlap(a, b) -> bool:
@@ -299,18 +297,17 @@ def kv_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Te
         mo, m = mass_out, mass_out.shape
         if mo.dtype != torch.float32 or len(m) != 3 or m[0] != S or m[1] != Hkv or m[2] < max_ctx or (m[2] > 1 and mo.stride(2) != 1):
             _bad(where, "mass_out is fp32 [sequences, kv heads, at least max_ctx columns]")
-        if not (mo.data_ptr() == mass.data_ptr() and mo.stride() == mass.stride()) and _columns_overlap(mass, mo):
+        if _columns_overlap(mass, mo):
             _bad(where, "mass_out overlaps mass")
     _check_rows(where, "mass_out", mo)
+    dst, moved = block_table, max_ctx if keep < max_ctx else 0                 # and the rows of a sequence that others may not have
     if dst_table is not None:
-        m = dst_table.shape
-        if dst_table.dtype != torch.int32 or len(m) != 2 or m[0] != S or m[1] * bs < min(keep, max_ctx) or (m[1] > 1 and dst_table.stride(1) != 1):
-            _bad(where, f"dst_table is int32 [sequences, blocks for {min(keep, max_ctx)} rows]")
-    if dst_table is not None and _tables_overlap(block_table, dst_table):
-        _bad(where, "dst_table and block_table share memory; without dst_table rows move in place")
-    moved = min(keep, max_ctx) if dst_table is not None else max_ctx if keep < max_ctx else 0       # rows of a sequence that others may not have
-    taken = block_table if dst_table is None else dst_table
-    if S > 1 and taken.stride(0) < (moved + bs - 1) // bs:
+        dst, m, moved = dst_table, dst_table.shape, min(keep, max_ctx)
+        if dst_table.dtype != torch.int32 or len(m) != 2 or m[0] != S or m[1] * bs < moved or (m[1] > 1 and dst_table.stride(1) != 1):
+            _bad(where, f"dst_table is int32 [sequences, blocks for {moved} rows]")
+        if _tables_overlap(block_table, dst_table):
+            _bad(where, "dst_table and block_table share memory; without dst_table rows move in place")
+    if S > 1 and dst.stride(0) < (moved + bs - 1) // bs:
         _bad(where, f"sequences share rows of {'block_table, which are moved in place' if dst_table is None else 'dst_table'}")
     _check_places(where, k_cache, v_cache, block_table, ctx_len, mass, mo, dst_table)
     if not k_cache.is_cuda:
@@ -321,14 +318,14 @@ def kv_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Te
     if S == 0 or max_ctx == 0:
         return kept.fill_(-1), new_len.zero_()
     own = torch.empty(S * Hkv * (keep + 1), dtype=torch.int32, device=dev)     # of a sequence and head: the rows' slots, the first that moves
-    dst = block_table if dst_table is None else dst_table
     launch, status = _library().mb_kv_evict, runtime(dev).status.data_ptr()
-    slots, first, tld, dld, row = own.data_ptr(), own.data_ptr() + 4 * S * Hkv * keep, block_table.stride(0), dst.stride(0), 4 * Hkv * keep
+    (ma, mb, _), (oa, ob, _), tld, dld, row, slots = mass.stride(), mo.stride(), block_table.stride(0), dst.stride(0), 4 * Hkv * keep, own.data_ptr()
+    mp, op, cp, kp, np, tp, dp, first = (mass.data_ptr(), mo.data_ptr(), ctx_len.data_ptr(), kept.data_ptr(), new_len.data_ptr(), block_table.data_ptr(), dst.data_ptr(),
+                                         slots + S * row)
     for s in range(0, S, 65535):
-        a = _EVICT_ARGS.pack(mass.data_ptr() + 4 * s * mass.stride(0), mass.stride(0), mass.stride(1), mo.data_ptr() + 4 * s * mo.stride(0), mo.stride(0), mo.stride(1),
-                             ctx_len.data_ptr() + 4 * s, kept.data_ptr() + s * row, new_len.data_ptr() + 4 * s, first + 4 * s * Hkv, block_table.data_ptr() + 4 * s * tld,
-                             tld, dst.data_ptr() + 4 * s * dld, dld, k_cache.data_ptr(), v_cache.data_ptr(), nb, status, slots + s * row, min(65535, S - s), Hkv, keep,
-                             recent, max_ctx, bs, D * k_cache.element_size(), dst_table is None, 0, 0)
+        a = _EVICT_ARGS.pack(mp + 4 * s * ma, ma, mb, op + 4 * s * oa, oa, ob, cp + 4 * s, kp + s * row, np + 4 * s, first + 4 * s * Hkv, tp + 4 * s * tld, tld,
+                             dp + 4 * s * dld, dld, k_cache.data_ptr(), v_cache.data_ptr(), nb, status, slots + s * row, min(65535, S - s), Hkv, keep, recent, max_ctx, bs,
+                             D * k_cache.element_size(), dst_table is None, 0, 0)
         _native.check(launch(a, _stream()), "kv_evict")
         _count(2)
     return kept, new_len
