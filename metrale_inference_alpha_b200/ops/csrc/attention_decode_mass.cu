@@ -1,5 +1,7 @@
 // Decode attention that leaves its logits: the kernel of attention_decode.cu for one new token a sequence, called by mb_attn_mass for the
 // calls that it serves. Beside attention itself a unit writes 4 bytes a token and query row; the join of kv_mass.cu makes weights of them.
+// Logits, maxima, sums and outputs are 32 bits. Weights go into the product with V as bf16, or f16 with an e4m3 cache, since the matrix units take no more, as in
+// plain attention: off by half a step each, which the bf16 result hides; the mass is made of the 32-bit logits.
 #include "attention_decode.cuh"
 #include "kv_mass.h"
 

@@ -236,7 +236,8 @@ __global__ void __launch_bounds__(kThreads, PER <= 16 ? 2 : 1) evict_select_kern
   }
 }
 
-// More rows than a cluster holds: one CTA, which reads the mass again for every digit of 8 bits and for the list.
+// More rows than a cluster holds: one CTA, which reads the mass again for every digit of 8 bits and for the list. Bound by that CTA's passes: 8 heads of 300007
+// e4m3 rows to 4096, with their copies, 461 us, a million 1500 (262144, in a cluster, 61); contexts of this length are cut seldom.
 __global__ void __launch_bounds__(1024) evict_select_long_kernel(const MbEvictArgs a) {
   __shared__ int hist[256], warp_tot[32];
   __shared__ uint32_t s_prefix;

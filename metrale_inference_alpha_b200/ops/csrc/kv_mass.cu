@@ -6,9 +6,9 @@
 // a step); the join turns them into weights and adds these up over the group. No atomics: every output has one writer, and sums have
 // one order, which depends on the sequence's own length alone.
 //
-// Measured with the join (B200, in a graph): 16 sequences of 8001 to 32749 bf16 tokens, 32 / 8 heads of 128, 245 us, K and V at 5.6 TB/s: memory, and
-// 209 of it attention itself. 128 of 129 to 1151 e4m3 tokens, 40 / 8 heads, 52.5, of which 44 attention (49 % of DRAM's rate: instructions around its
-// tiles); one of 700 13.5, latency of both launches.
+// Measured with the join (B200, in a graph): 16 sequences of 8001 to 32749 bf16 tokens, 32 / 8 heads of 128, 249 us, K and V at 5.6 TB/s: memory, and
+// 215 of it attention itself. 128 of 129 to 1151 e4m3 tokens, 40 / 8 heads, 53.5, of which 45 attention (48 % of DRAM's rate: instructions around its
+// tiles); one of 700 13.8, eight CTAs that walk it and then the join.
 #include "common.cuh"
 #include "kv_mass.h"
 

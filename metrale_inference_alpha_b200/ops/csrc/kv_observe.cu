@@ -18,7 +18,7 @@
 // under the exponentials, warp 11 the copies. With 256 lanes a CTA and one of them per SM, 4096 observers at 8192 e4m3 tokens took 766 us, sixteen prompts
 // of 17 to 1151 tokens under 64 observers 55.
 //
-// Bound by its exponentials, two a logit at 16 a cycle and SM: 4096 observers at 8192 e4m3 tokens, 40 / 8 heads of 128, take 727 us (1.0 G logits a
+// Bound by its exponentials, two a logit at 16 a cycle and SM: 4096 observers at 8192 e4m3 tokens, 40 / 8 heads of 128, take 729 us (1.0 G logits a
 // pass, 2.8 T exponentials a second; the special function units 76 and 68 % busy, the tensor pipe 38 and 32), 32 observers 31, a launch's
 // latency three times. At dim 256 products from shared memory count as much: 2 prompts of 1001 and 1531 at up to 4431 tokens, 16 / 2 heads, 163 us. (B200, in a graph.)
 //
