@@ -992,3 +992,5 @@ def _attention_rowwise(q, k_cache, v_cache, block_table, q_start, q_len, ctx_len
 
 
 from .kv_mass import kv_evict, paged_attention_mass, prompt_mass  # noqa: E402,F401  (decode attention and prompts that leave their weights; eviction by them)
+from .shared_attn import merge_attention, shared_prefix_attention  # noqa: E402,F401  (batches that share prefixes; attention in parts, joined)
+from .mla_prompt import mla_prompt_attention  # noqa: E402,F401  (prompts over a latent cache, expanded)

@@ -568,3 +568,63 @@ def sigmoid_gated_rmsnorm(x, gate, w, eps: float):
     """x [.., D] fp32: x * rsqrt(mean(x^2) + eps) * w * sigmoid(gate) (kda_layer_ops.cu::kda_o_norm_gated)."""
     x = x.float()
     return x * torch.rsqrt(x.pow(2).mean(-1, keepdim=True) + eps) * w.float() * torch.sigmoid(gate.float())
+
+
+# ----------------------------------------------------------------------------- attention in parts
+def _attend(q, parts, limits, scale: float):
+    """q [W, Hkv, G, D] over `parts` (k, v) [n, Hkv, D] one behind the other, of which row w sees the first limits[w]: (out [W, Hkv, G, D], lse)."""
+    k, v = (torch.cat([p[i] for p in parts]) for i in (0, 1))
+    z = torch.einsum("whgd,nhd->whgn", q.float(), k) * scale
+    seen = (torch.arange(k.shape[0]) < limits[:, None])[:, None, None]
+    z = z.masked_fill(~seen, float("-inf"))
+    lse = torch.logsumexp(z, -1)
+    p = torch.where(seen & (lse != float("-inf"))[..., None], torch.exp(z - lse[..., None]), 0.0)
+    # a row's unseen values do not count, whatever they are
+    out = torch.stack([torch.einsum("hgn,nhd->hgd", p[w, :, :, :n], v[:n]) for w, n in enumerate(limits.clamp(min=0).tolist())])
+    return out, lse
+
+
+def shared_prefix_attention(q, k_cache, v_cache, prefix_table, prefix_len, group_start, block_table, ctx_len, q_len: int, scale: float, k_scale=None, v_scale=None):
+    """`q_len` new tokens a sequence over its group's prefix and its own rows: (out bf16, lse fp32)."""
+    T, Hq, D = q.shape
+    Hkv, start = k_cache.shape[2], group_start.tolist()
+    out, lse = torch.zeros(T, Hq, D), torch.full((T, Hq), float("-inf"))
+    for s in range(ctx_len.shape[0]):
+        n = max(int(ctx_len[s]), 0)
+        places = [(block_table, s, n)]
+        for g, (a, b) in enumerate(zip(start, start[1:])):
+            if a <= s < b:
+                places.insert(0, (prefix_table, g, max(int(prefix_len[g]), 0)))
+        parts = [tuple(_cached_rows(c, t, i, torch.arange(m), x) for c, x in ((k_cache, k_scale), (v_cache, v_scale))) for t, i, m in places]
+        own = (n - q_len + 1 + torch.arange(q_len)).clamp(min=0)
+        rows = slice(s * q_len, (s + 1) * q_len)
+        o, l = _attend(q[rows].view(q_len, Hkv, Hq // Hkv, D), parts, sum(m for _, _, m in places) - n + own, scale)
+        out[rows], lse[rows] = o.reshape(q_len, Hq, D), l.reshape(q_len, Hq)
+    return out.to(torch.bfloat16), lse
+
+
+def merge_attention(outs, lses):
+    l = torch.stack(list(lses))
+    lse = torch.logsumexp(torch.where(l == float("inf"), float("nan"), l), 0)
+    total = torch.zeros(outs[0].shape)
+    for o, x in zip(outs, lses):
+        total += torch.where((x == float("-inf"))[..., None], 0.0, torch.exp(x - lse)[..., None] * o.float())
+    return total.to(outs[0].dtype), lse
+
+
+def mla_prompt_attention(q, cache, block_table, q_start, q_len, ctx_len, w_kv, scale: float) -> torch.Tensor:
+    """Prompts over a latent cache, keys and values made for every head."""
+    T, H, qk = q.shape
+    L = w_kv.shape[2]
+    nope = qk - (cache.shape[3] - L)
+    out = torch.zeros(T, H, w_kv.shape[1] - nope)
+    for s in range(ctx_len.shape[0]):
+        n, ql, at = max(int(ctx_len[s]), 0), int(q_len[s]), int(q_start[s])
+        if ql <= 0:
+            continue
+        x = _cached_rows(cache, block_table, s, torch.arange(n))[:, 0]
+        kv = torch.einsum("nl,hdl->nhd", x[:, :L], w_kv.float()).to(torch.bfloat16).float()
+        k = torch.cat([kv[:, :, :nope], x[:, None, L:].expand(-1, H, -1)], -1)
+        o, _ = _attend(q[at:at + ql].view(ql, H, 1, qk), [(k, kv[:, :, nope:])], n - ql + 1 + torch.arange(ql), scale)
+        out[at:at + ql] = o[:, :, 0]
+    return out.to(torch.bfloat16)
