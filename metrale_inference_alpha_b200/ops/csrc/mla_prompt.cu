@@ -2,7 +2,9 @@
 // as usual. Per head and pair 192 + 128 multiply-adds instead of the 576 + 512 of the absorbed form, for 512 x 256 a cached row and head in front.
 #include "common.cuh"
 #include "shared_attn.h"
+#include "attention_rows.cuh"
 #include "smem_limit.h"
+#include "tensormap.h"
 
 namespace {
 
@@ -91,76 +93,269 @@ __global__ void __launch_bounds__(256) gather_kernel(const GatherParams p) {
   }
 }
 
-constexpr int kTile = 16, kRows = 16;
+// ---- attention: two tiles of 128 query tokens of one head a CTA in turn on the tensor cores, as in attention_rows.cu
+//   warps 0-3, 4-7   softmax of row tile 0 / 1, thread = row: S from TMEM, P back to TMEM (over S), the output row at the end
+//   warp 8           copies by TMA: Q once; per 128 cached tokens five pieces of 16 KB in a ring of eight: K in three spans of 64 dims (the
+//                    third is the rotated part, which all heads share), V in two halves of 64 tokens
+//   warp 9           issues the products: S0 S1 | PV0 S0' PV1 S1' | ... so that one tile's softmax runs under the other tile's products
+//   warps 10, 11     give their registers to the softmax
+constexpr int kT = 128, kPiece = 16384, kRing = 8, kPer = 5, kThreads = 384;
+constexpr int kQTile = 3 * kPiece;
+constexpr int kSmem = 2 * kQTile + kRing * kPiece + 1024;
 
-__global__ void __launch_bounds__(128) mla_simple_kernel(const MbMlaPromptArgs p) {
-  __shared__ float sQ[kRows][kQk], sK[kTile][kQk + 1], sV[kTile][kV], sS[kRows][kTile], sM[kRows], sL[kRows], sA[kRows];
-  const int s = blockIdx.z, h = blockIdx.y, tid = threadIdx.x;
+using namespace mbr;
+template <int N>
+__device__ __forceinline__ void more_regs() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void fewer_regs() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
+__global__ void __launch_bounds__(kThreads, 1)
+mla_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                  const __grid_constant__ CUtensorMap tmR, const MbMlaPromptArgs p) {
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  uint8_t* sQ = smem_raw + ((1024u - (mb::smem_u32(smem_raw) & 1023u)) & 1023u);   // 2 row tiles x 3 spans x [128 rows x 128 B]
+  uint8_t* sR = sQ + 2 * kQTile;
+  __shared__ __align__(8) uint64_t q_full, full[kRing], empty[kRing], s_full[2], p_full[2], o_full[2];
+  __shared__ uint32_t s_tmem;
+  const int h = blockIdx.x, seq = blockIdx.z, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   mb::pdl_wait();
-  const int qlen = p.q_len[s], qs = p.q_start[s], ctx = min(max(p.ctx_len[s], 0), p.max_ctx), t0 = blockIdx.x * kRows;
-  const long long first = p.first[s];
-  if (t0 >= qlen) return;
-  if (qlen > p.max_q_len || qs < 0 || (long long)qs + qlen > p.q_rows || first + ctx > p.kv_rows) {
+  const int qlen = p.q_len[seq], qs = p.q_start[seq], ctx = min(max(p.ctx_len[seq], 0), p.max_ctx);
+  const long long first = p.first[seq];
+  const int row0 = ((int)gridDim.y - 1 - (int)blockIdx.y) * 256;                   // the longest rows first
+  if (row0 >= qlen) return;
+  if (qlen > p.max_q_len || qs < 0 || (long long)qs + qlen > p.q_rows || first + ((ctx + 127) & ~127) > p.kv_rows) {
     if (tid == 0 && p.status) atomicCAS(p.status, 0u, MB_ST_BOUNDS);
     return;
   }
-  const int rows = min(kRows, qlen - t0), past = ctx - qlen;
-  for (int i = tid; i < rows * kQk; i += 128)
-    sQ[i / kQk][i % kQk] = __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p.q)[((size_t)(qs + t0 + i / kQk) * p.H + p.head0 + h) * kQk + i % kQk]) * p.scale;
-  if (tid < kRows) {
-    sM[tid] = -INFINITY;
-    sL[tid] = 0.f;
+  const int past = ctx - qlen;
+  auto tiles_of = [&](int w) {                            // cached tiles that row tile w sees
+    const int rows = min(qlen - row0 - w * 128, 128);
+    return rows <= 0 ? 0 : (max(past + row0 + w * 128 + rows, 0) + kT - 1) / kT;
+  };
+  const int n0 = tiles_of(0), n1 = tiles_of(1), n = max(n0, n1);
+
+  if (tid == 0) {
+    mb::mbar_init(&q_full, 1);
+    for (int i = 0; i < kRing; ++i) {
+      mb::mbar_init(&full[i], 1);
+      mb::mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mb::mbar_init(&s_full[i], 1);
+      mb::mbar_init(&p_full[i], 4);
+      mb::mbar_init(&o_full[i], 1);
+    }
+    mb::mbar_fence_init();
   }
-  float o[kRows];
-#pragma unroll
-  for (int r = 0; r < kRows; ++r) o[r] = 0.f;
-  const int last = past + t0 + rows;
-  int bad = 0x7fffffff;
-  for (int j = 0; j < last; j += 128) bad = min(bad, p.bad[(first + j) / 128]);
+  if (warp == 9) mb::tmem_alloc(&s_tmem, 512);
+  mb::tc_fence_before();
   __syncthreads();
-  for (int j0 = 0; j0 < last; j0 += kTile) {
-    const int m = min(kTile, last - j0);
-    for (int i = tid; i < m * 320; i += 128) {
-      const int j = i / 320, d = i % 320;
-      const size_t row = first + j0 + j;
-      if (d < 64) sK[j][kNope + d] = __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p.lat)[row * kRow + kLat + d]);
-      else {
-        const float x = __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p.kv)[(row * p.heads + h) * 256 + d - 64]);
-        if (d < 192) sK[j][d - 64] = x;
-        else sV[j][d - 192] = x;
+  mb::tc_fence_after();
+  mb::pdl_launch_dependents();                            // a dependent kernel allocates TMEM: not before this CTA has its own
+  const uint32_t tmem = s_tmem;                           // S0 0-127, S1 128-255, O0 256-383, O1 384-511
+
+  if (warp < 8) {
+    // ------------------------------------------------------------ softmax
+    more_regs<216>();                                     // 216 + 216 + 72 are the 3 x 168 of the launch
+    const int w = warp >> 2, tok = row0 + w * 128 + (tid & 127);
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t tS = tmem + lanes + w * 128, tO = tmem + lanes + 256 + w * 128;
+    const bool live = tok < qlen;
+    const int limit = live ? past + tok + 1 : 0;          // cached tokens [0, limit) are visible
+    const int mine = w ? n1 : n0;
+    const float sc = p.scale * 1.44269504088896f;
+    float m_run = -INFINITY, l_run = 0.f;
+    bool ok = true;
+    for (int j = 0; j < mine; ++j) {
+      ok = mb::mbar_wait(&s_full[w], j & 1, p.status, MB_ST_TIMEOUT_MMA);
+      if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+      mb::tc_fence_after();
+      float s[kT];
+#pragma unroll
+      for (int c = 0; c < kT; c += 32) mb::tmem_ld32_async(tS + c, s + c);
+      mb::tmem_ld_wait(s);
+      const int seen = limit - j * kT;                    // columns below this are visible
+      if (!__all_sync(0xffffffffu, seen >= kT)) {
+#pragma unroll
+        for (int i = 0; i < kT; ++i)
+          if (i >= seen) s[i] = -INFINITY;
+      }
+      float mx4[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+      for (int i = 4; i < kT; ++i) mx4[i & 3] = fmaxf(mx4[i & 3], s[i]);
+      const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * sc;
+      float alpha = 1.f;
+      const bool move = mx > m_run + 8.f;                 // also true on a row's first finite tile
+      if (move) {
+        alpha = ex2(m_run - mx);                          // 0 when the row had seen nothing yet
+        m_run = mx;
+      }
+      if (j > 0 && __any_sync(0xffffffffu, move)) {
+#pragma unroll
+        for (int c = 0; c < kV; c += 16) {
+          float ov[16];
+          mb::tmem_ld16(tO + c, ov);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) ov[i] *= alpha;
+          mb::tmem_st16(tO + c, ov);
+        }
+      }
+      const float nm = m_run == -INFINITY ? 0.f : -m_run;
+      const float2 sc2 = make_float2(sc, sc), nm2 = make_float2(nm, nm);
+      float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        uint32_t pk[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          float2 t = fma2(make_float2(s[q * 64 + 2 * i], s[q * 64 + 2 * i + 1]), sc2, nm2);
+          t.x = ex2(t.x);
+          t.y = ex2(t.y);
+          sum[i & 1] = add2(sum[i & 1], t);
+          pk[i] = pack2<false>(t.x, t.y);
+        }
+        tmem_st32(tS + q * 32, pk);
+      }
+      mb::tmem_st_wait();
+      mb::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mb::mbar_arrive(&p_full[w]);
+      l_run = l_run * alpha + ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y));
+    }
+    // the first cached token that is no number, of those that the tile sees: it lies in the expanded rows as zeros
+    int bad = 0x7fffffff;
+    for (int j = lane; j < mine; j += 32) bad = min(bad, p.bad[first / kT + j]);
+    bad = __reduce_min_sync(0xffffffffu, bad);
+    if (ok && mine > 0) {
+      ok = mb::mbar_wait(&o_full[w], 0, p.status, MB_ST_TIMEOUT_MMA);
+      mb::tc_fence_after();
+    }
+    if (__all_sync(0xffffffffu, ok)) {                    // uniform: tcgen05.ld is a whole-warp instruction
+      const float inv = limit > bad ? __int_as_float(0x7fffffff) : l_run == 0.f ? 0.f : 1.f / l_run;
+      uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(p.out) + ((size_t)(qs + (live ? tok : 0)) * p.H + p.head0 + h) * kV);
+#pragma unroll 1
+      for (int c0 = 0; c0 < kV; c0 += 64) {
+        float o[64];
+        if (mine > 0) {
+          mb::tmem_ld32_async(tO + c0, o);
+          mb::tmem_ld32_async(tO + c0 + 32, o + 32);
+          mb::tmem_ld_wait(o);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 64; ++i) o[i] = 0.f;
+        }
+        if (live) {
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            uint32_t v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = inv == 0.f ? 0u : pack2<false>(o[c * 8 + 2 * i] * inv, o[c * 8 + 2 * i + 1] * inv);
+            dst[c0 / 8 + c] = make_uint4(v[0], v[1], v[2], v[3]);
+          }
+        }
       }
     }
-    __syncthreads();
-    for (int i = tid; i < rows * m; i += 128) {
-      const int r = i / m, j = i % m;
-      float z = 0.f;
-      for (int d = 0; d < kQk; ++d) z += sQ[r][d] * sK[j][d];
-      sS[r][j] = j0 + j < past + t0 + r + 1 ? z : -INFINITY;
+    mb::tc_fence_before();
+  } else {
+    fewer_regs<72>();
+    if (warp == 8 && mb::elect_one() && n > 0) {
+      // ---------------------------------------------------------- copies
+      const int hq = (p.head0 + h) * kQk, hk = h * 256;
+      mb::mbar_expect_tx(&q_full, n1 ? 2 * kQTile : kQTile);
+      for (int w = 0; w < (n1 ? 2 : 1); ++w)
+        for (int c = 0; c < 3; ++c) mb::tma_load_2d(sQ + w * kQTile + c * kPiece, &tmQ, &q_full, hq + c * 64, qs + row0 + w * 128);
+      int slot = 0, i = 0;
+      uint32_t parity = 1;
+      bool ok = true;
+      for (int j = 0; j < n && ok; ++j) {
+        const int at = (int)first + j * kT;
+        for (int c = 0; c < kPer; ++c) {
+          ok = mb::mbar_wait(&empty[slot], parity, p.status, MB_ST_TIMEOUT_TMA);
+          if (!ok) break;
+          uint8_t* dst = sR + slot * kPiece;
+          mb::mbar_expect_tx(&full[slot], kPiece);
+          if (c < 2) {
+            mb::tma_load_2d(dst, &tmK, &full[slot], hk + c * 64, at);
+          } else if (c == 2) {
+            mb::tma_load_2d(dst, &tmR, &full[slot], kLat, at);
+          } else {
+            for (int d = 0; d < 2; ++d) mb::tma_load_2d(dst + d * (kPiece / 2), &tmV, &full[slot], hk + kNope + d * 64, at + (c - 3) * 64);
+          }
+          ++i;
+          if (++slot == kRing) {
+            slot = 0;
+            parity ^= 1;
+          }
+        }
+      }
+      // given up: no copy may still be under way when the CTA ends
+      if (!ok) {
+        mb::mbar_wait(&q_full, 0, p.status, MB_ST_TIMEOUT_TMA);
+        for (int k = max(0, i - kRing); k < i; ++k) mb::mbar_wait(&full[k % kRing], (k / kRing) & 1, p.status, MB_ST_TIMEOUT_TMA);
+      }
     }
-    __syncthreads();
-    if (tid < rows) {
-      float mx = sM[tid], sum = 0.f;
-      for (int j = 0; j < m; ++j) mx = fmaxf(mx, sS[tid][j]);
-      const float base = mx == -INFINITY ? 0.f : mx;
-      sA[tid] = sM[tid] == -INFINITY ? 0.f : expf(sM[tid] - base);
-      for (int j = 0; j < m; ++j) sum += sS[tid][j] = expf(sS[tid][j] - base);
-      sL[tid] = sL[tid] * sA[tid] + sum;
-      sM[tid] = mx;
-    }
-    __syncthreads();
+    if (warp == 9 && mb::elect_one() && n > 0) {
+      // ---------------------------------------------------------- products
+      constexpr uint32_t kIdS = mb::umma_idesc(1, 1, 128, kT), kIdO = mb::umma_idesc(1, 1, 128, kV, 0, 1);
+      const uint32_t aQ = mb::smem_u32(sQ), aR = mb::smem_u32(sR);
+      auto there = [&](int i) { return mb::mbar_wait(&full[i % kRing], (i / kRing) & 1, p.status, MB_ST_TIMEOUT_MMA); };
+      auto release = [&](int i) { mb::tc_commit(&empty[i % kRing]); };
+      auto scores = [&](int w, int j) {
+        for (int c = 0; c < 3; ++c) {
+          if (!there(j * kPer + c)) return false;
+          mb::tc_fence_after();
 #pragma unroll
-    for (int r = 0; r < kRows; ++r) {
-      if (r >= rows) break;
-      o[r] *= sA[r];
-      for (int j = 0; j < m; ++j) o[r] += sS[r][j] * sV[j][tid];
+          for (int s = 0; s < 4; ++s)
+            mb::umma_f16(tmem + w * 128, mb::umma_desc_sw128(aQ + w * kQTile + c * kPiece + s * 32),
+                         mb::umma_desc_sw128(aR + (j * kPer + c) % kRing * kPiece + s * 32), kIdS, (c | s) != 0);
+        }
+        mb::tc_commit(&s_full[w]);
+        return true;
+      };
+      auto values = [&](int w, int j) {
+        if (!mb::mbar_wait(&p_full[w], j & 1, p.status, MB_ST_TIMEOUT_MMA)) return false;
+        for (int c = 0; c < 2; ++c) {
+          if (!there(j * kPer + 3 + c)) return false;
+          mb::tc_fence_after();
+#pragma unroll
+          for (int s = 0; s < 4; ++s)
+            umma_f16_ta(tmem + 256 + w * 128, tmem + w * 128 + (c * 4 + s) * 8,
+                        mb::umma_desc_sw128_mn(aR + (j * kPer + 3 + c) % kRing * kPiece + s * 2048, kPiece / 2, 1024), kIdO, (j | c | s) != 0);
+        }
+        return true;
+      };
+      bool ok = mb::mbar_wait(&q_full, 0, p.status, MB_ST_TIMEOUT_MMA);
+      if (ok && n0 > 0) ok = scores(0, 0);
+      if (ok && n1 > 0) ok = scores(1, 0);
+      if (ok)
+        for (int c = 0; c < 3; ++c) release(c);
+      for (int j = 0; j < n && ok; ++j) {
+        if (j < n0) {
+          ok = values(0, j);
+          if (!ok) break;
+          if (j + 1 < n0) ok = scores(0, j + 1);
+          else mb::tc_commit(&o_full[0]);
+          if (!ok) break;
+        }
+        if (j < n1) {
+          ok = values(1, j);
+          if (!ok) break;
+        }
+        for (int c = 3; c < kPer; ++c) release(j * kPer + c);
+        if (j + 1 < n1) ok = scores(1, j + 1);
+        else if (j + 1 == n1) mb::tc_commit(&o_full[1]);
+        if (!ok) break;
+        if (j + 1 < n)
+          for (int c = 0; c < 3; ++c) release((j + 1) * kPer + c);
+      }
     }
-    __syncthreads();
+    __syncwarp();
   }
-#pragma unroll
-  for (int r = 0; r < kRows; ++r)
-    if (r < rows)
-      reinterpret_cast<__nv_bfloat16*>(p.out)[((size_t)(qs + t0 + r) * p.H + p.head0 + h) * kV + tid] =
-          __float2bfloat16(past + t0 + r + 1 > bad ? __int_as_float(0x7fffffff) : sL[r] == 0.f ? 0.f : o[r] / sL[r]);
+  __syncthreads();
+  if (warp == 9) {
+    mb::tc_fence_after();
+    mb::tmem_dealloc(tmem, 512);
+  }
 }
 
 }  // namespace
@@ -179,7 +374,19 @@ int mb_mla_prompt(const MbMlaPromptArgs* a, cudaStream_t stream) {
   if (!a || !a->q || !a->kv || !a->lat || !a->q_start || !a->q_len || !a->ctx_len || !a->first || !a->bad || !a->out || a->num_seqs <= 0 || a->num_seqs > 65535 ||
       a->H <= 0 || a->heads <= 0 || a->heads > 65535 || a->head0 < 0 || a->head0 + a->heads > a->H || a->max_q_len <= 0 || a->max_ctx <= 0)
     return MB_ERR_BAD_ARG;
-  return (int)mb::launch_kernel(mla_simple_kernel, dim3((a->max_q_len + kRows - 1) / kRows, a->heads, a->num_seqs), dim3(128), 0, stream, *a);
+  const unsigned tiles = (a->max_q_len + 255) / 256;
+  if (tiles > 65535 || a->q_rows <= 0 || a->kv_rows <= 0 || a->kv_rows % kT) return MB_ERR_TOO_LARGE;
+  CUtensorMap tm[4];
+  const uint64_t pitch = (uint64_t)a->heads * 512;
+  int rc = mbh::encode_2d(&tm[0], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, a->q, (uint64_t)a->H * kQk, a->q_rows, (uint64_t)a->H * kQk * 2, 64, 128);
+  if (!rc) rc = mbh::encode_2d(&tm[1], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, a->kv, (uint64_t)a->heads * 256, a->kv_rows, pitch, 64, 128);
+  if (!rc) rc = mbh::encode_2d(&tm[2], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, a->kv, (uint64_t)a->heads * 256, a->kv_rows, pitch, 64, 64);
+  if (!rc) rc = mbh::encode_2d(&tm[3], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, a->lat, kRow, a->kv_rows, kRow * 2, 64, 128);
+  if (rc) return rc;
+  static std::atomic<uint64_t> asked{0};
+  const cudaError_t e = mb::allow_smem(reinterpret_cast<const void*>(mla_prompt_kernel), kSmem, asked);
+  if (e != cudaSuccess) return (int)e;
+  return (int)mb::launch_kernel(mla_prompt_kernel, dim3(a->heads, tiles, a->num_seqs), dim3(kThreads), kSmem, stream, tm[0], tm[1], tm[2], tm[3], *a);
 }
 
 }  // extern "C"
