@@ -1,5 +1,6 @@
 // The kernel of attention_decode.cu, which says how it goes about its work, and its launch. MASS (attention_decode_mass.cu): the same for one
-// new token a sequence, which leaves its logits and its partitions' maxima and sums to a join behind it.
+// new token a sequence, which leaves its logits and its partitions' maxima and sums to a join behind it. PARTS (attention_decode_parts.cu): the
+// same again, one token at a time of `per` new ones a sequence, which leaves every partition's outputs, maxima and sums to a join and nothing else.
 #pragma once
 #include "common.cuh"
 #include "attention_decode.h"
@@ -42,11 +43,12 @@ struct DecodeParams {
   uint32_t merge_off, tail_off, len_off;     // byte offsets of the merge buffer and of what lies behind both
   int over;                                  // the merge buffer lies over slots of the ring
   uint32_t* status;
+  int per, tok0;                             // PARTS: new tokens of a sequence, the token of the batch that is the launch's first
   float* z;                                  // MASS: logits in the log2 domain [seqs * Hq, z_ld], a column a cached token
   long long z_ld;
-  int max_ctx;                               // MASS: longer sequences are reported and cut
-  int group, group0;                         // MASS: query heads of a kv head, the first of the G that this launch takes
-  int box_bits;                              // MASS: log2 of a slice's TMA boxes, 16 / the greatest common divisor of 16 and block_size
+  int max_ctx;                               // MASS, PARTS: longer sequences are reported and cut
+  int group, group0;                         // MASS, PARTS: query heads of a kv head, the first of the G that this launch takes
+  int box_bits;                              // MASS, PARTS: log2 of a slice's TMA boxes, 16 / the greatest common divisor of 16 and block_size
 };
 
 __device__ __forceinline__ void mma16816_f16(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
@@ -101,6 +103,11 @@ __device__ __forceinline__ uint64_t evict_first() {
   asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
   return policy;
 }
+__device__ __forceinline__ uint64_t evict_normal() {
+  uint64_t policy;
+  asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(policy));
+  return policy;
+}
 __device__ __forceinline__ void tma_load_3d_once(void* dst, const CUtensorMap* m, uint64_t* bar, int c0, int c1, int c2, uint64_t policy) {
   asm volatile(
       "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
@@ -132,18 +139,19 @@ struct DecodeCfg {
   static __device__ __forceinline__ int place(int r, int dim) { return kPairs ? dim : dim ^ ((r & 6) << 2); }
 };
 
-template <int D, bool FP8, int NT, bool MASS>
+// MODE: 0, MASS 1, PARTS 2
+template <int D, bool FP8, int NT, int MODE>
 __global__ void __launch_bounds__(128, DecodeCfg<D, FP8, NT>::kCtas)
 attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const DecodeParams p) {
   using C = DecodeCfg<D, FP8, NT>;
   constexpr int kSpans = C::kSpans, kSpanB = C::kSpanB, kSub = C::kSub, kTok = C::kTok, kTiles = C::kTiles;
-  constexpr bool kPairs = C::kPairs, kThroughBf16 = NT > 2;
+  constexpr bool kPairs = C::kPairs, kThroughBf16 = NT > 2, MASS = MODE == 1, PARTS = MODE == 2, kOne = MODE != 0;     // kOne: one query token a sequence
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ __align__(8) uint64_t bars[4 * kMaxSlots];
   const int slots = p.slots;
   __shared__ int s_last, s_wsum[4];
-  constexpr bool kLift = MASS && FP8;
+  constexpr bool kLift = kOne && FP8;
   __shared__ float s_sc[kLift ? 4 : 1][kLift ? NT * 8 : 1];  // kLift: rows' scores come to the log2 domain by these, a copy a warp
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   float* s_o = reinterpret_cast<float*>(smem + p.merge_off);                  // [4 warps][rows][D], see C::place
@@ -169,11 +177,16 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
       int n = 0;
       if (s < p.num_seqs) {
         int4 x;
-        if constexpr (MASS) {
-          x = make_int4(1, max(p.ctx_len[s], 0), s, 0);
+        if constexpr (kOne) {
+          const int owner = PARTS ? (s + p.tok0) / p.per : s;
+          x = make_int4(1, max(p.ctx_len[owner], 0), s, 0);
           if (x.y > p.max_ctx) {
             if (p.status) atomicCAS(p.status, 0u, MB_ST_BOUNDS);
             x.y = p.max_ctx;
+          }
+          if constexpr (PARTS) {                             // w: the row of the block table; the token sees what is cached up to itself
+            x.w = owner;
+            x.y = max(0, x.y - p.per + (s + p.tok0 - owner * p.per) + 1);
           }
         } else {
           x = make_int4(p.q_len[s], p.ctx_len[s], p.q_start[s], 0);
@@ -229,13 +242,13 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
     x.slices = (n - warp + 3) >> 2;
   };
   // places of the slices of this warp's steps i0 .. i0 + 32 / kSub - 1, one per lane
-  const int box_bits = MASS ? p.box_bits : 0, step_bits = box_bits + kSub / 2, per = 1 << step_bits;   // boxes of a slice, of a step
+  const int box_bits = kOne ? p.box_bits : 0, step_bits = box_bits + kSub / 2, per = 1 << step_bits;   // boxes of a slice, of a step
   auto blocks = [&](Unit& x, int i0) {
     const int i = i0 + (lane >> step_bits), tok = x.begin + (warp + 4 * i) * kTok + (lane & (per - 1)) * (kSlice >> box_bits);
     x.blk = x.within = 0;                                    // a slice behind the context reads the null block
     if (i < x.slices && tok < x.ctx) {
       const int bi = p.block_shift >= 0 ? tok >> p.block_shift : tok / p.block_size;
-      int b = __ldg(p.block_table + (size_t)x.seq * p.max_blocks + bi);
+      int b = __ldg(p.block_table + (size_t)(PARTS ? s_len[x.seq].w : x.seq) * p.max_blocks + bi);
       if (b < 0 || b >= p.num_blocks) {
         if (p.status) atomicCAS(p.status, 0u, MB_ST_BOUNDS);
         b = 0;
@@ -245,15 +258,15 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
     }
   };
   const uint32_t my = mb::smem_u32(smem) + warp * C::kSlot;
-  const uint64_t once = MASS ? evict_first() : 0;
-  auto issue = [&](Unit& x, int i, int slot) {               // whole warp; one lane issues, MASS: each lane its box
-    if constexpr (MASS)
+  const uint64_t once = MASS || (PARTS && p.per == 1) ? evict_first() : PARTS ? evict_normal() : 0;   // PARTS: the other tokens read the same rows
+  auto issue = [&](Unit& x, int i, int slot) {               // whole warp; one lane issues, kOne: each lane its box
+    if constexpr (kOne)
       if (i > 0 && (i << step_bits & 31) == 0) blocks(x, i);        // the lanes' places reach 32 / per steps
     const int place = x.blk * p.block_size + x.within;
     uint64_t* bar = &bars[slot * 4 + warp];
     uint8_t* dst = smem + (slot * 4 + warp) * C::kSlot;
     if (lane == 0) mb::mbar_expect_tx(bar, C::kSlot);
-    if constexpr (MASS) {
+    if constexpr (kOne) {
       __syncwarp();
       const int j = lane - (i << step_bits & 31);
       if (j >= 0 && j < per) {
@@ -280,7 +293,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
     }
   };
   // the query head of row r, which is of token tq
-  auto head_of = [&](const Unit& x, int r, int tq) { return MASS ? x.kvh * p.group + p.group0 + r : x.kvh * p.G + (r - tq * p.G); };
+  auto head_of = [&](const Unit& x, int r, int tq) { return kOne ? x.kvh * p.group + p.group0 + r : x.kvh * p.G + (r - tq * p.G); };
   // the unit's query rows into shared memory: the whole CTA, 16 bytes a copy
   auto fetch_q = [&](const Unit& x) {
     const int n = p.G * x.qlen * (D / 8);
@@ -301,10 +314,10 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
     blocks(cur, 0);
     // slices of tokens that were cached before this step travel under the end of the kernel in front, which writes the step's own
     const int old = max(0, cur.ctx - cur.qlen - cur.begin) / kTok;
-    if (p.early)
+    if (!PARTS && p.early)
       for (; begun < min(min(cur.slices, slots), (old - warp + 3) >> 2); ++begun) issue(cur, begun, begun);
   }
-  if (p.early) mb::pdl_wait();
+  if (!PARTS && p.early) mb::pdl_wait();
   mb::pdl_launch_dependents();
   if (u < units) {
     for (; begun < min(cur.slices, slots); ++begun) issue(cur, begun, begun);
@@ -579,7 +592,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
       __syncwarp();                                          // every lane has read the slot
       const int nx = i + slots;
       if (nx < cur.slices) {
-        if (!MASS && nx * kSub % 32 == 0) blocks(cur, nx);
+        if (!kOne && nx * kSub % 32 == 0) blocks(cur, nx);
         issue(cur, nx, slot);
       }
       slot = slot + 1 == slots ? 0 : slot + 1;
@@ -674,7 +687,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         l += ml[w].y * f;
         acc.x += ov.x * f; acc.y += ov.y * f; acc.z += ov.z * f; acc.w += ov.w * f;
       }
-      if (cur.nparts == 1) {
+      if (!PARTS && cur.nparts == 1) {
         const float inv = l > 0.f ? vmul / l : 0.f;
         store(r, c4, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
         if constexpr (MASS)
@@ -686,7 +699,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         if (c4 == 0) p.part_ml[row] = make_float2(mx, l);
       }
     }
-    if (!MASS && cur.nparts > 1) {
+    if (!kOne && cur.nparts > 1) {
       // the last partition of this (sequence, kv head) to arrive sums all of them in order and re-arms the counter
       __threadfence();
       __syncthreads();
@@ -735,6 +748,9 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
     cur = next;
     u = un;
   }
+  // PARTS under the kernel in front, which it does not read from: whoever waits for this kernel has waited for both
+  if constexpr (PARTS)
+    if (p.early) mb::pdl_wait();
 }
 
 struct Layout {
@@ -766,14 +782,14 @@ Layout layout(int rows, int num_seqs, int slots = 2) {
   return l;
 }
 
-template <int D, bool FP8, int NT, bool MASS = false>
+template <int D, bool FP8, int NT, int MODE = 0>
 int launch(const AttnDecodeArgs& a, DecodeParams& p, cudaStream_t stream) {
   using C = DecodeCfg<D, FP8, NT>;
-  auto kern = attn_decode_kernel<D, FP8, NT, MASS>;
+  auto kern = attn_decode_kernel<D, FP8, NT, MODE>;
   CUtensorMap tm[2];
   for (int i = 0; i < 2; ++i) {
     const int rc = mbh::encode_3d(&tm[i], CU_TENSOR_MAP_DATA_TYPE_UINT8, i ? a.v_cache : a.k_cache, C::kRowB, a.Hkv, (uint64_t)a.num_blocks * a.block_size,
-                                  C::kRowB, (uint64_t)a.Hkv * C::kRowB, C::kSpanB, 1, MASS ? kSlice >> p.box_bits : kSlice,
+                                  C::kRowB, (uint64_t)a.Hkv * C::kRowB, C::kSpanB, 1, MODE ? kSlice >> p.box_bits : kSlice,
                                   C::kSpanB == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc) return rc;
   }
@@ -800,7 +816,7 @@ int launch(const AttnDecodeArgs& a, DecodeParams& p, cudaStream_t stream) {
   const cudaError_t e = mb::allow_smem(reinterpret_cast<const void*>(kern), 220 * 1024, asked);
   if (e != cudaSuccess) return (int)e;
   const int grid = most < (long long)sms * l.per_sm ? (int)most : sms * l.per_sm;
-  p.early = a.early && mb_pdl_enabled() == 2;
+  p.early = a.early && (MODE == 2 ? mb_pdl_enabled() != 0 : mb_pdl_enabled() == 2);
   return (int)mb::launch_kernel_ex(kern, dim3(grid), dim3(128), l.smem, stream, 1, p.early || mb_pdl_enabled() == 1, tm[0], tm[1], p);
 }
 

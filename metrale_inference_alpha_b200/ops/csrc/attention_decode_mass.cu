@@ -34,7 +34,7 @@ int mb_decode_mass(const MbMassArgs& m, const mbm::DecodeWs& w, int part_tokens,
   while (m.block_size % (kSlice >> p.box_bits)) ++p.box_bits;
   auto run = [&](auto d, auto eight) {
     constexpr int kMost = d.value == 256 ? 16 : 32;          // query rows that the kernel takes
-    auto go = [&](auto nt) { return launch<d.value, eight.value, nt.value, true>(a, p, stream); };
+    auto go = [&](auto nt) { return launch<d.value, eight.value, nt.value, 1>(a, p, stream); };
     const int takes = (p.group + kMost - 1) / kMost, each = (p.group + takes - 1) / takes;
     for (p.group0 = 0; p.group0 < p.group; p.group0 += each) {
       p.G = min(each, p.group - p.group0);

@@ -1,110 +1,166 @@
 // Decode and verify attention of a batch whose sequences share long prefixes:
 // z[j] = scale <q, k[j]> over the rows of the sequence's prefix (all of them) and its own (up to the token itself), out = softmax(z) v, lse = ln sum exp z.
-#include "common.cuh"
-#include "shared_attn.h"
-#include "smem_limit.h"
+//
+// What has no need of the rest is computed on its own: all rows behind a prefix over that prefix, which is read once for all of them (shared_prefix.cuh),
+// and every token over what its sequence has of its own (the decode kernel, attention_decode_parts.cu). Either leaves outputs relative to 2^m, m and sums,
+// and the join here adds them up. The decode kernel comes up under the prefix kernel and does not wait for it until its end, so that the two share the GPU.
+// No atomics: every partial result has one writer, and the join adds them in the order of the tokens.
+#include "attention_decode_parts.h"
+#include "shared_prefix.cuh"
 
 namespace {
 
-constexpr int kTile = 32, kThreads = 128;
+using namespace mbs;
 
-__device__ __forceinline__ float load(const void* cache, size_t i, bool fp8) {
-  return fp8 ? mb::e4m3_to_float(reinterpret_cast<const uint8_t*>(cache)[i]) : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(cache)[i]);
+constexpr size_t kOwnBytes = size_t(512) << 20;            // most bytes of own rows' partial results: more tokens go in several steps
+
+Ws workspace(const MbSharedArgs& a) {
+  Ws w{};
+  const size_t rows = (size_t)a.num_seqs * a.q_len * (a.Hq / a.Hkv), all = rows * a.Hkv, tokens = (size_t)a.num_seqs * a.q_len;
+  w.ctas = a.sm_count > 0 ? a.sm_count : 148;
+  auto take = [&](size_t bytes) {
+    const size_t at = w.bytes;
+    w.bytes += (bytes + 255) & ~size_t(255);
+    return at;
+  };
+  if (a.groups > 0 && a.max_prefix > 0) {
+    const size_t sides = a.D == 256 ? 1 : 2;
+    w.first = take(sides * all * a.D * 4);
+    w.first_ml = take(sides * all * 8);
+    w.rest = take((size_t)w.ctas * 2 * kRowTile * a.D * 4);
+    w.rest_ml = take((size_t)w.ctas * 2 * kRowTile * 8);
+  }
+  if (a.max_ctx > 0) {
+    const int part = part_tokens_of(a.Hkv, a.D);
+    const long long n = ((long long)a.max_ctx + part - 1) / part;
+    w.parts = n > kMaxOwnParts ? kMaxOwnParts : (int)n;
+    const size_t each = (size_t)a.Hq * w.parts * (a.D * 4 + 8);
+    size_t step = kOwnBytes / each;
+    step = step < 1 ? 1 : step > (size_t)kMaxTokens ? (size_t)kMaxTokens : step;
+    if (step > tokens) step = tokens;
+    w.step = (int)step;
+    w.own = take(step * a.Hq * w.parts * a.D * 4);
+    w.own_ml = take(step * a.Hq * w.parts * 8);
+  } else {
+    w.step = tokens < size_t(1) << 20 ? (int)tokens : 1 << 20;
+  }
+  return w;
 }
 
-__global__ void __launch_bounds__(kThreads) shared_simple_kernel(const MbSharedArgs p) {
-  extern __shared__ float smem[];
-  const int tok = blockIdx.x, kvh = blockIdx.y, tid = threadIdx.x, D = p.D, G = p.Hq / p.Hkv;
-  float *sK = smem, *sV = sK + kTile * (D + 1), *sQ = sV + kTile * D, *sO = sQ + G * D, *sS = sO + G * D, *sM = sS + G * kTile, *sL = sM + G, *sA = sL + G;
+// 32 rows (tokens x heads of a group) of a kv head a CTA, lane = row; warp w has dims w D / 8 to (w + 1) D / 8 of them.
+template <int D, bool FP8>
+__global__ void __launch_bounds__(256) shared_join_kernel(const MbSharedArgs p, const Ws ws, int tok0, int tokens) {
+  __shared__ Plan plan;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = p.Hq / p.Hkv, kvh = blockIdx.y;
   mb::pdl_wait();
-  const int seq = tok / p.q_len, at = tok - seq * p.q_len;
-  int prefix = 0, group = -1;
-  {
-    int start = 0;
-    for (int g = 0, next = 0; g < p.groups; ++g) {
-      const int a = p.group_start[g], b = p.group_start[g + 1];
-      start = max(next, min(max(a, 0), p.num_seqs));
-      next = max(start, min(max(b, 0), p.num_seqs));
-      if (tid == 0 && p.status && (a < 0 || a > b || b > p.num_seqs)) atomicCAS(p.status, 0u, MB_ST_BOUNDS);
-      if (seq >= start && seq < next) group = g;
+  const bool prefixes = p.groups > 0 && p.max_prefix > 0;
+  if (prefixes) {
+    if (warp == 0) make_plan<D>(p, plan, lane);
+    __syncthreads();
+  }
+  const long long R = (long long)blockIdx.x * 32 + lane;   // of the step's rows
+  if (R >= (long long)tokens * G) return;
+  const int step_tok = (int)(R / G), head = (int)(R - (long long)step_tok * G), tok = tok0 + step_tok, seq = tok / p.q_len;
+  constexpr int kC = D / 32;                               // fours of dims of a thread
+  float m = -INFINITY, l = 0.f;
+  float4 acc[kC];
+#pragma unroll
+  for (int c = 0; c < kC; ++c) acc[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto add = [&](float2 ml, auto&& out) {
+    if (ml.y == 0.f) return;                               // nothing seen: what lies there is not looked at
+    const float mn = fmaxf(m, ml.x), base = mn == -INFINITY ? 0.f : mn;      // all scores NaN leave no maximum, but a sum that is NaN
+    const float fa = m == -INFINITY ? 0.f : ex2(m - base), fb = ex2(ml.x - base);
+    const float fb1 = ml.x == -INFINITY ? 1.f : fb;
+    m = mn;
+    l = l * fa + ml.y * fb1;
+#pragma unroll
+    for (int c = 0; c < kC; ++c) {
+      const float4 x = out(c);
+      acc[c].x = acc[c].x * fa + x.x * fb1;
+      acc[c].y = acc[c].y * fa + x.y * fb1;
+      acc[c].z = acc[c].z * fa + x.z * fb1;
+      acc[c].w = acc[c].w * fa + x.w * fb1;
     }
-  }
-  if (group >= 0) prefix = max(p.prefix_len[group], 0);
-  int own = max(p.ctx_len[seq], 0);
-  if (prefix > p.max_prefix || own > p.max_ctx) {
-    if (tid == 0 && p.status) atomicCAS(p.status, 0u, MB_ST_BOUNDS);
-    prefix = min(prefix, p.max_prefix);
-    own = min(own, p.max_ctx);
-  }
-  own = max(0, own - p.q_len + at + 1);
-  const __nv_bfloat16* q = reinterpret_cast<const __nv_bfloat16*>(p.q) + ((size_t)tok * p.Hq + kvh * G) * D;
-  for (int i = tid; i < G * D; i += kThreads) {
-    sQ[i] = __bfloat162float(q[i]);
-    sO[i] = 0.f;
-  }
-  for (int g = tid; g < G; g += kThreads) {
-    sM[g] = -INFINITY;
-    sL[g] = 0.f;
-  }
-  __syncthreads();
-  const float sc = p.scale * (p.fp8 ? *p.k_scale : 1.f);
-  for (int side = 0; side < 2; ++side) {
-    const int n = side ? own : prefix;
-    const int* table = side ? p.block_table + (size_t)seq * p.table_ld : p.prefix_table + (size_t)max(group, 0) * p.prefix_ld;
-    for (int j0 = 0; j0 < n; j0 += kTile) {
-      const int m = min(kTile, n - j0);
-      for (int i = tid; i < m * D; i += kThreads) {
-        const int j = i / D, d = i - j * D, bi = (j0 + j) / p.block_size;
-        int b = table[bi];
-        if (b < 0 || b >= p.num_blocks) {
-          if (p.status) atomicCAS(p.status, 0u, MB_ST_BOUNDS);
-          b = 0;
+  };
+  if (prefixes && seq >= plan.start[0] && seq < plan.start[p.groups]) {
+    int lo = 0, hi = p.groups;                             // start[lo] <= seq < start[hi]
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (plan.start[mid] <= seq) lo = mid;
+      else hi = mid;
+    }
+    const int rows = row_count(p, plan, lo), tiles = (plan.len[lo] + Shape<D>::kT - 1) / Shape<D>::kT;
+    if (tiles > 0) {
+      const int row = (tok - plan.start[lo] * p.q_len) * G + head;
+      int doubles, singles;
+      unit_count<D>(rows, doubles, singles);
+      const long long W = plan.base[p.groups];
+      const int two = row < doubles * 256, u = two ? row >> 8 : (row - doubles * 256) >> 7;
+      const long long at = plan.base[lo] + kvh * line_of_head<D>(rows, tiles) + (two ? 2ll * tiles * u : (2ll * doubles + u) * tiles);
+      const int side = two ? (row >> 7) & 1 : 0, sides = two || D == 256 ? 1 : 2;
+      const int c0 = cta_of(at, ws.ctas, W), c1 = cta_of(at + ((long long)(tiles - 1) << two), ws.ctas, W);
+      for (int c = c0; c <= c1; ++c) {
+        int t0, t1;
+        tiles_in(at, tiles, two, place_of(c, ws.ctas, W), place_of(c + 1, ws.ctas, W), t0, t1);
+        if (t1 <= t0) continue;
+        for (int k = 0; k < sides; ++k) {
+          const Place from = t0 == 0 ? place_first<D>(p, ws, plan, lo, kvh, row, k) : place_rest<D>(p, ws, c, two ? side : k);
+          const int r = t0 == 0 ? 0 : row & 127;
+          add(__ldcg(from.ml + r), [&](int i) { return __ldcg(from.o + (warp * kC + i) * from.pitch + r); });
         }
-        const size_t from = (((size_t)b * p.block_size + (j0 + j - bi * p.block_size)) * p.Hkv + kvh) * D + d;
-        sK[j * (D + 1) + d] = load(p.k_cache, from, p.fp8);
-        sV[i] = load(p.v_cache, from, p.fp8);
       }
-      __syncthreads();
-      for (int i = tid; i < G * m; i += kThreads) {
-        const int g = i / m, j = i - g * m;
-        float z = 0.f;
-        for (int d = 0; d < D; ++d) z += sQ[g * D + d] * sK[j * (D + 1) + d];
-        sS[g * kTile + j] = z * sc;
-      }
-      __syncthreads();
-      for (int g = tid; g < G; g += kThreads) {
-        float mx = sM[g], sum = 0.f;
-        for (int j = 0; j < m; ++j) mx = fmaxf(mx, sS[g * kTile + j]);
-        const float base = mx == -INFINITY ? 0.f : mx, alpha = sM[g] == -INFINITY ? 0.f : expf(sM[g] - base);
-        for (int j = 0; j < m; ++j) sum += sS[g * kTile + j] = expf(sS[g * kTile + j] - base);
-        sL[g] = sL[g] * alpha + sum;
-        sM[g] = mx;
-        sA[g] = alpha;
-      }
-      __syncthreads();
-      for (int i = tid; i < G * D; i += kThreads) {
-        const int g = i / D, d = i - g * D;
-        float o = sO[i] * sA[g];
-        for (int j = 0; j < m; ++j) o += sS[g * kTile + j] * sV[j * D + d];
-        sO[i] = o;
-      }
-      __syncthreads();
     }
   }
-  const float vs = p.fp8 ? *p.v_scale : 1.f;
-  __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(p.out) + ((size_t)tok * p.Hq + kvh * G) * D;
-  for (int i = tid; i < G * D; i += kThreads) {
-    const float l = sL[i / D];
-    out[i] = __float2bfloat16(l == 0.f ? 0.f : sO[i] * vs / l);
+  if (p.max_ctx > 0) {
+    int own = min(max(p.ctx_len[seq], 0), p.max_ctx);
+    own = max(0, own - p.q_len + (tok - seq * p.q_len) + 1);
+    if (own > 0) {
+      const int parts = own_part_count(own, part_tokens_of(p.Hkv, D));
+      const size_t at = ((size_t)step_tok * p.Hq + kvh * G + head) * ws.parts;
+      const float4* o = reinterpret_cast<const float4*>(reinterpret_cast<const uint8_t*>(p.ws) + ws.own) + at * (D / 4) + warp * kC;
+      const float2* ml = reinterpret_cast<const float2*>(reinterpret_cast<const uint8_t*>(p.ws) + ws.own_ml) + at;
+      for (int i = 0; i < parts; ++i) add(__ldcg(ml + i), [&](int c) { return __ldcg(o + (size_t)i * (D / 4) + c); });
+    }
   }
-  if (p.lse)
-    for (int g = tid; g < G; g += kThreads) p.lse[(size_t)tok * p.Hq + kvh * G + g] = sL[g] == 0.f ? -INFINITY : sM[g] + logf(sL[g]);
+  const float inv = l == 0.f ? 0.f : (FP8 ? *p.v_scale : 1.f) / l;
+  const size_t row = (size_t)tok * p.Hq + kvh * G + head;
+  uint32_t y[2 * kC];
+#pragma unroll
+  for (int c = 0; c < kC; ++c) {
+    y[2 * c] = pack2<false>(acc[c].x * inv, acc[c].y * inv);
+    y[2 * c + 1] = pack2<false>(acc[c].z * inv, acc[c].w * inv);
+  }
+  uint4* out = reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(p.out) + row * D + warp * (D / 8));
+#pragma unroll
+  for (int c = 0; c < kC / 2; ++c) out[c] = make_uint4(y[4 * c], y[4 * c + 1], y[4 * c + 2], y[4 * c + 3]);
+  if (p.lse && warp == 0) p.lse[row] = l == 0.f ? -INFINITY : ((m == -INFINITY ? 0.f : m) + log2f(l)) * 0.693147180559945f;
 }
 
 bool bad_shape(const MbSharedArgs& a) {
   return a.num_seqs <= 0 || a.q_len <= 0 || a.Hkv <= 0 || a.Hkv > 65535 || a.Hq % a.Hkv || a.Hq / a.Hkv > 64 || (a.D != 64 && a.D != 128 && a.D != 256) ||
-         a.block_size <= 0 || a.num_blocks <= 0 || a.max_prefix < 0 || a.max_ctx < 0 || !a.q || !a.k_cache || !a.v_cache || !a.ctx_len || !a.out ||
-         (a.fp8 && (!a.k_scale || !a.v_scale)) || a.groups < 0 || (a.groups > 0 && (!a.prefix_table || !a.prefix_len || !a.group_start));
+         a.block_size <= 0 || a.num_blocks <= 0 || a.num_blocks * a.block_size >= (1ll << 31) || a.table_ld >= (1ll << 31) || a.max_prefix < 0 || a.max_ctx < 0 || !a.q ||
+         !a.k_cache || !a.v_cache || !a.ctx_len || !a.out || (a.fp8 && (!a.k_scale || !a.v_scale)) || a.groups < 0 || a.groups > kMaxGroups ||
+         (a.groups > 0 && (!a.prefix_table || !a.prefix_len || !a.group_start)) ||
+         ((reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.k_cache) | reinterpret_cast<uintptr_t>(a.v_cache) | reinterpret_cast<uintptr_t>(a.out)) & 15);
+}
+
+template <int D, bool FP8>
+int run(const MbSharedArgs& a, const Ws& w, cudaStream_t stream) {
+  const int tokens = a.num_seqs * a.q_len, G = a.Hq / a.Hkv;
+  const bool prefixes = a.groups > 0 && a.max_prefix > 0;
+  if (prefixes)
+    if (const int rc = launch_prefix<D, FP8>(a, w, stream)) return rc;
+  uint8_t* ws = reinterpret_cast<uint8_t*>(a.ws);
+  for (int t = 0; t < tokens; t += w.step) {
+    const int n = tokens - t < w.step ? tokens - t : w.step;
+    // only the first step stands directly behind the prefix kernel; a later one's results take the place of what the join in front reads
+    if (a.max_ctx > 0)
+      if (const int rc = mb_decode_parts(a, t, n, reinterpret_cast<float*>(ws + w.own), reinterpret_cast<float*>(ws + w.own_ml), w.parts, prefixes && t == 0, stream)) return rc;
+    const long long blocks = ((long long)n * G + 31) / 32;
+    const cudaError_t e = mb::launch_kernel_ex(shared_join_kernel<D, FP8>, dim3((unsigned)blocks, a.Hkv), dim3(256), 0, stream, 1, mb_pdl_enabled() != 0, a, w, t, n);
+    if (e != cudaSuccess) return (int)e;
+  }
+  return 0;
 }
 
 }  // namespace
@@ -115,14 +171,22 @@ size_t mb_shared_attn_args(int which) {
   return which == 0 ? sizeof(MbSharedArgs) : which == 1 ? sizeof(MbMergeArgs) : which == 2 ? sizeof(MbMlaPromptArgs) : 0;
 }
 
+size_t mb_shared_attn_ws(int num_seqs, int q_len, int groups, int Hq, int Hkv, int D, int max_prefix, int max_ctx, int sm_count) {
+  if (num_seqs <= 0 || q_len <= 0 || Hkv <= 0 || Hq < Hkv) return 0;
+  MbSharedArgs a{};
+  a.num_seqs = num_seqs; a.q_len = q_len; a.groups = groups; a.Hq = Hq; a.Hkv = Hkv; a.D = D; a.max_prefix = max_prefix; a.max_ctx = max_ctx; a.sm_count = sm_count;
+  return workspace(a).bytes;
+}
+
 int mb_shared_attn(const MbSharedArgs* a, cudaStream_t stream) {
   if (!a || bad_shape(*a)) return MB_ERR_BAD_ARG;
-  const int G = a->Hq / a->Hkv;
-  const size_t smem = 4 * ((size_t)kTile * (2 * a->D + 1) + (size_t)G * (2 * a->D + kTile + 3));
-  static std::atomic<uint64_t> asked{0};
-  const cudaError_t e = mb::allow_smem(reinterpret_cast<const void*>(shared_simple_kernel), 220 * 1024, asked);
-  if (e != cudaSuccess) return (int)e;
-  return (int)mb::launch_kernel(shared_simple_kernel, dim3(a->num_seqs * a->q_len, a->Hkv), dim3(kThreads), smem, stream, *a);
+  const Ws w = workspace(*a);
+  if (w.bytes > 0 && (!a->ws || a->ws_bytes < w.bytes)) return MB_ERR_TOO_LARGE;
+  switch (a->D) {
+    case 64: return a->fp8 ? run<64, true>(*a, w, stream) : run<64, false>(*a, w, stream);
+    case 128: return a->fp8 ? run<128, true>(*a, w, stream) : run<128, false>(*a, w, stream);
+    default: return a->fp8 ? run<256, true>(*a, w, stream) : run<256, false>(*a, w, stream);
+  }
 }
 
 }  // extern "C"

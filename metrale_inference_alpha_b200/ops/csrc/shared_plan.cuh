@@ -1,0 +1,160 @@
+// How the work over prefixes is shared out: what the kernels of shared_prefix.cuh and the join of shared_attn.cu compute alike.
+//
+// Per kv head, the query rows behind a prefix (tokens x heads of a group) are numbered token * G + head and cut into units of 2 * 128 rows, or one of
+// 128 where no more are left (heads of 256 dims: all of 128). All units' tiles of cached tokens lie one behind the other on a line; a tile of a double
+// unit takes two places of it, since it takes about twice the time. Of the line's W places every CTA takes as many, give or take one: units that it covers
+// whole, and parts of its first and last one. A part that holds a unit's first tile leaves its outputs by row (`first`), the others, at most
+// one a CTA, by CTA (`rest`).
+#pragma once
+#include "common.cuh"
+#include "shared_attn.h"
+
+namespace mbs {
+
+constexpr int kMaxGroups = 1024, kRowTile = 128;
+
+template <int D>
+struct Shape {
+  static constexpr bool kDouble = D <= 128;                // double units
+  static constexpr int kT = kDouble ? 128 : 64;            // cached tokens of a tile
+};
+
+// Groups of a call, in shared memory: first sequences (rising and inside the batch, whatever the caller's are), rows of the prefix, first place on the line
+struct Plan {
+  int start[kMaxGroups + 1];
+  int len[kMaxGroups];
+  long long base[kMaxGroups + 1];
+};
+
+__device__ __forceinline__ int row_count(const MbSharedArgs& p, const Plan& s, int g) { return (s.start[g + 1] - s.start[g]) * p.q_len * (p.Hq / p.Hkv); }
+
+// units of a group for a kv head: double ones, and single ones behind them
+template <int D>
+__device__ __forceinline__ void unit_count(int rows, int& doubles, int& singles) {
+  if constexpr (Shape<D>::kDouble) {
+    const int rest = rows & 255;
+    doubles = (rows >> 8) + (rest > 128);
+    singles = rest > 0 && rest <= 128;
+  } else {
+    doubles = 0;
+    singles = (rows + 127) >> 7;
+  }
+}
+template <int D>
+__device__ __forceinline__ long long line_of_head(int rows, int tiles) {
+  int doubles, singles;
+  unit_count<D>(rows, doubles, singles);
+  return (long long)tiles * (2 * doubles + singles);
+}
+
+// by one warp
+template <int D>
+__device__ __forceinline__ void make_plan(const MbSharedArgs& p, Plan& s, int lane) {
+  int top = 0;
+  for (int g0 = 0; g0 <= p.groups; g0 += 32) {
+    const int g = g0 + lane;
+    int a = 0;
+    if (g <= p.groups) {
+      a = p.group_start[g];
+      const int next = g < p.groups ? p.group_start[g + 1] : a;
+      if (p.status && (a < 0 || a > p.num_seqs || next < a)) atomicCAS(p.status, 0u, MB_ST_BOUNDS);
+      a = min(max(a, 0), p.num_seqs);
+    }
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, a, d);
+      if (lane >= d) a = max(a, y);
+    }
+    a = max(a, top);
+    if (g <= p.groups) s.start[g] = a;
+    top = __shfl_sync(0xffffffffu, a, 31);
+  }
+  __syncwarp();
+  long long at = 0;
+  for (int g0 = 0; g0 < p.groups; g0 += 32) {
+    const int g = g0 + lane;
+    long long n = 0;
+    if (g < p.groups) {
+      int len = 0;
+      if (s.start[g + 1] > s.start[g]) {
+        len = max(p.prefix_len[g], 0);
+        if (len > p.max_prefix) {
+          if (p.status) atomicCAS(p.status, 0u, MB_ST_BOUNDS);
+          len = p.max_prefix;
+        }
+      }
+      s.len[g] = len;
+      n = p.Hkv * line_of_head<D>(row_count(p, s, g), (len + Shape<D>::kT - 1) / Shape<D>::kT);
+    }
+    long long x = n;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const long long y = __shfl_up_sync(0xffffffffu, x, d);
+      if (lane >= d) x += y;
+    }
+    if (g < p.groups) s.base[g] = at + x - n;
+    at += __shfl_sync(0xffffffffu, x, 31);
+  }
+  if (lane == 0) s.base[p.groups] = at;
+}
+
+// first place of CTA c of `ctas`, and the CTA that has place x
+__device__ __forceinline__ long long place_of(int c, int ctas, long long W) { return c * W / ctas; }
+__device__ __forceinline__ int cta_of(long long x, int ctas, long long W) { return (int)(((x + 1) * ctas + W - 1) / W) - 1; }
+
+struct Part {
+  int group, kvh, row0, rows, two;         // a unit: its first row in the group, its rows, whether it is a double one
+  int t0, t1;                              // tiles of the part
+};
+// tiles [t0, t1) of a unit that begins at place `at` with `tiles` of them, which lie in places [b0, b1)
+__device__ __forceinline__ void tiles_in(long long at, int tiles, int two, long long b0, long long b1, int& t0, int& t1) {
+  const long long a = max(b0 - at, 0ll), b = min(max(b1 - at, 0ll), (long long)tiles << two);
+  t0 = (int)((a + two) >> two);
+  t1 = (int)((b + two) >> two);
+}
+
+// The part at `pos`, which moves behind it; false at the end. Parts without tiles are left out.
+template <int D>
+__device__ __forceinline__ bool next_part(const MbSharedArgs& p, const Plan& s, long long& pos, long long end, Part& x) {
+  while (pos < end) {
+    int lo = 0, hi = p.groups;             // base[lo] <= pos < base[hi]
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (s.base[mid] <= pos) lo = mid;
+      else hi = mid;
+    }
+    x.group = lo;
+    const int rows = row_count(p, s, lo), tiles = (s.len[lo] + Shape<D>::kT - 1) / Shape<D>::kT;
+    int doubles, singles;
+    unit_count<D>(rows, doubles, singles);
+    const long long head = (long long)tiles * (2 * doubles + singles), in = pos - s.base[lo];
+    x.kvh = (int)(in / head);
+    const long long w = in - x.kvh * head, d = 2ll * tiles * doubles;
+    long long at;
+    if (w < d) {
+      const int u = (int)(w / (2ll * tiles));
+      x.two = 1;
+      x.row0 = u * 256;
+      at = pos - (w - 2ll * tiles * u);
+    } else {
+      const int u = (int)((w - d) / tiles);
+      x.two = 0;
+      x.row0 = doubles * 256 + u * 128;
+      at = pos - (w - d - (long long)tiles * u);
+    }
+    x.rows = min(rows - x.row0, x.two ? 256 : 128);
+    tiles_in(at, tiles, x.two, pos, end, x.t0, x.t1);
+    pos = min(end, at + ((long long)tiles << x.two));
+    if (x.t1 > x.t0) return true;
+  }
+  return false;
+}
+
+// Workspace of a call: `first` outputs [2][Hkv][D / 4][rows] of four dims, `rest` [ctas][2][D / 4][128], each with maxima (log2 domain) and sums. A single
+// unit's tiles are taken in turn by two accumulators, whose results are the two of the leading dim; double units and heads of 256 dims use the first.
+struct Ws {
+  size_t first, first_ml, rest, rest_ml, own, own_ml, bytes;
+  int ctas, parts, step;                   // parts of a sequence's own rows; tokens whose own rows are attended at once
+};
+
+}  // namespace mbs

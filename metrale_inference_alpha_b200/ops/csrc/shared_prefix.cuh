@@ -1,0 +1,713 @@
+// Attention of all query rows behind a prefix over that prefix, heads of 64 and 128 dims: outputs, maxima and sums of every part (shared_plan.cuh) for the
+// join of shared_attn.cu.
+//
+// As in attention_rows.cu the rows are tokens x heads of a group, 128 a tile, products on the tensor cores with S, P and O in TMEM, and two tiles in
+// turn, so that the softmax of one runs under the products of the other. Behind a prefix few rows are the rule: where a unit has one tile of rows (up to
+// 128), both accumulators take the cached tiles of this one in turn. Roles (512 threads, one CTA an SM, registers moved with setmaxnreg):
+//   warps 0-3, 4-7   softmax of accumulator 0 / 1, thread = row; they load their rows' queries and write their outputs
+//   warps 8-11       K and V tiles of 128 cached tokens into two stages, an e4m3 cache as f16 (exact), a bf16 cache by asynchronous copies
+//   warp 12          the products
+// The loading warps and the products run on from part to part; queries wait for the products of the part in front of theirs only.
+// With an e4m3 cache a row's queries are scaled by the power of two that takes their largest to [2^14, 2^15) and weights are held 2^7 larger, as
+// there: neither then loses the range that bf16 gives.
+#pragma once
+#include "attention_rows.cuh"
+#include "shared_plan.cuh"
+#include "smem_limit.h"
+
+namespace mbs {
+
+using namespace mbr;
+template <int N>
+__device__ __forceinline__ void more_regs() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void fewer_regs() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
+constexpr float kLift = 7.f;                              // log2 of what f16 weights are held larger by
+
+// Where a part's results lie: element (r, dims 4 c .. 4 c + 3) at o[c * pitch + r], maximum and sum at ml[r]
+struct Place {
+  float4* o;
+  float2* ml;
+  size_t pitch;
+};
+template <int D>
+__device__ __forceinline__ Place place_first(const MbSharedArgs& p, const Ws& w, const Plan& s, int group, int kvh, int row, int side) {
+  const size_t R = (size_t)p.num_seqs * p.q_len * (p.Hq / p.Hkv), at = (size_t)s.start[group] * p.q_len * (p.Hq / p.Hkv) + row, h = (size_t)side * p.Hkv + kvh;
+  uint8_t* ws = reinterpret_cast<uint8_t*>(p.ws);
+  return {reinterpret_cast<float4*>(ws + w.first) + h * (D / 4) * R + at, reinterpret_cast<float2*>(ws + w.first_ml) + h * R + at, R};
+}
+template <int D>
+__device__ __forceinline__ Place place_rest(const MbSharedArgs& p, const Ws& w, int cta, int side) {
+  const size_t i = (size_t)cta * 2 + side;
+  uint8_t* ws = reinterpret_cast<uint8_t*>(p.ws);
+  return {reinterpret_cast<float4*>(ws + w.rest) + i * (D / 4) * kRowTile, reinterpret_cast<float2*>(ws + w.rest_ml) + i * kRowTile, kRowTile};
+}
+
+// Queries of row r0 + r of a unit, 16-byte piece c of D / 8; an e4m3 cache wants them in f16, scaled (`scale`: what scores are then too small by)
+template <int D, bool FP8>
+__device__ __forceinline__ uint4 query_piece(uint4 v, float& scale) {
+  if constexpr (FP8) {
+    // bf16 bits without the sign order like the values: the row's largest over its D / 8 lanes
+    const uint32_t x[4] = {v.x, v.y, v.z, v.w};
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) top = __vmaxu2(top, x[j] & 0x7fff7fffu);
+#pragma unroll
+    for (int d = 1; d < D / 8; d <<= 1) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, d));
+    const int e = (int)(max(top & 0xffff, top >> 16) >> 7);
+    const int up = e == 255 ? 0 : 141 - max(e, 15);        // zeros and subnormal rows as if their exponent were 15, infinities and NaN as they are
+    const float f = __int_as_float((127 + up) << 23);
+    uint32_t h[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 y = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&x[j]));
+      h[j] = pack2<true>(y.x * f, y.y * f);
+    }
+    scale = __int_as_float((127 - up) << 23);
+    return make_uint4(h[0], h[1], h[2], h[3]);
+  }
+  return v;
+}
+
+// K and V tiles of kT cached tokens of this CTA's parts, one after the other, into two stages each: 128 threads, t the number of this one
+template <int D, bool FP8, int kT>
+__device__ __forceinline__ void load_tiles(const MbSharedArgs& p, const Plan& plan, long long begin, long long end, uint8_t* sK, uint8_t* sV, uint64_t* k_full,
+                                           uint64_t* k_empty, uint64_t* v_full, uint64_t* v_empty, int t) {
+  constexpr int kTileB = kT * D * 2;
+  const int lane = t & 31;
+  constexpr int kPieces = FP8 ? D / 16 : D / 8;         // 16-byte pieces of a cached row
+  constexpr int kStep = 128 / kPieces, kN = kT / kStep; // rows between a thread's pieces, and how many it has
+  const int r0 = t / kPieces, c = t % kPieces;
+  const size_t row_bytes = (size_t)D * (FP8 ? 1 : 2), pitch = (size_t)p.Hkv * row_bytes;
+  const int shift = (p.block_size & (p.block_size - 1)) == 0 ? 31 - __clz(p.block_size) : -1;
+  long long pos = begin;
+  Part x;
+  x.t0 = x.t1 = 0;
+  int at = 0;                                           // the tile whose places are looked up next
+  bool more = true;
+  // the places in the cache of this thread's rows of the next tile (-1: behind the prefix, or no tile), looked up a tile before they are read
+  int bad = 0;
+  auto places = [&](int* place, size_t& off) {
+    if (more && at == x.t1) {
+      more = next_part<D>(p, plan, pos, end, x);
+      at = x.t0;
+    }
+    if (!more) {
+#pragma unroll
+      for (int i = 0; i < kN; ++i) place[i] = -1;
+      return false;
+    }
+    const int len = plan.len[x.group];
+    const int* bt = p.prefix_table + (size_t)x.group * p.prefix_ld;
+    off = x.kvh * row_bytes + (size_t)c * 16;
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+      const int tok = at * kT + r0 + i * kStep, in = min(tok, len - 1);
+      const int bi = shift >= 0 ? in >> shift : in / p.block_size;
+      int blk = bt[bi];
+      const bool out = (unsigned)blk >= (unsigned long long)p.num_blocks;
+      bad |= out;
+      blk = out ? 0 : blk;
+      place[i] = tok < len ? blk * p.block_size + (in - bi * p.block_size) : -1;
+    }
+    ++at;
+    return true;
+  };
+  bool ok = true;
+  if constexpr (FP8) {
+    uint4 kr[kN], vr[kN];
+    int next[kN];
+    size_t off = 0;
+    auto fetch = [&](const void* cache, uint4* raw) {
+      const uint8_t* base = reinterpret_cast<const uint8_t*>(cache) + off;
+#pragma unroll
+      for (int i = 0; i < kN; ++i)
+        raw[i] = next[i] >= 0 ? __ldg(reinterpret_cast<const uint4*>(base + (size_t)next[i] * pitch)) : make_uint4(0, 0, 0, 0);
+    };
+    auto put = [&](uint8_t* tile, const uint4* raw) {
+#pragma unroll
+      for (int i = 0; i < kN; ++i) {
+        const int r = r0 + i * kStep;
+        const uint32_t y[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+        uint32_t h[8];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          h[2 * k] = e4m3x2(y[k]);
+          h[2 * k + 1] = e4m3x2(y[k] >> 16);
+        }
+        uint8_t* half = tile + (c >> 2) * (kT * 128);
+        *reinterpret_cast<uint4*>(half + sw_off(r, (c & 3) * 2)) = make_uint4(h[0], h[1], h[2], h[3]);
+        *reinterpret_cast<uint4*>(half + sw_off(r, (c & 3) * 2 + 1)) = make_uint4(h[4], h[5], h[6], h[7]);
+      }
+    };
+    bool have = places(next, off);
+    fetch(p.k_cache, kr);
+    fetch(p.v_cache, vr);
+    bool then = places(next, off);
+    for (int j = 0; have; ++j) {
+      const int b = j & 1;
+      const uint32_t ph = ((j >> 1) & 1) ^ 1;
+      ok = mb::mbar_wait(&k_empty[b], ph, p.status, MB_ST_TIMEOUT_TMA);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      put(sK + b * kTileB, kr);
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) mb::mbar_arrive(&k_full[b]);
+      fetch(p.k_cache, kr);
+      ok = mb::mbar_wait(&v_empty[b], ph, p.status, MB_ST_TIMEOUT_TMA);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      put(sV + b * kTileB, vr);
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) mb::mbar_arrive(&v_full[b]);
+      fetch(p.v_cache, vr);
+      have = then;
+      then = places(next, off);
+    }
+  } else {
+    int now[kN], next[kN];
+    size_t off = 0, ahead = 0;
+    auto copy = [&](const void* cache, uint8_t* tile) {
+      const uint8_t* base = reinterpret_cast<const uint8_t*>(cache) + off;
+#pragma unroll
+      for (int i = 0; i < kN; ++i) {
+        const int r = r0 + i * kStep;
+        const bool there = now[i] >= 0;
+        const uint8_t* src = base + (there ? (size_t)now[i] * pitch : 0);
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(mb::smem_u32(tile + (c >> 3) * (kT * 128) + sw_off(r, c & 7))),
+                     "l"(src), "r"(there ? 16 : 0)
+                     : "memory");
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    // the copies of a tile are announced while the next tile's are in flight
+    auto announce = [&](uint64_t* bar) {
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) mb::mbar_arrive(bar);
+    };
+    bool have = places(next, ahead);
+    int j = 0;
+    for (; have; ++j) {
+      const int b = j & 1;
+      const uint32_t ph = ((j >> 1) & 1) ^ 1;
+#pragma unroll
+      for (int i = 0; i < kN; ++i) now[i] = next[i];
+      off = ahead;
+      have = places(next, ahead);
+      ok = mb::mbar_wait(&k_empty[b], ph, p.status, MB_ST_TIMEOUT_TMA);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      copy(p.k_cache, sK + b * kTileB);
+      if (j > 0) {
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+        announce(&v_full[b ^ 1]);
+      }
+      ok = mb::mbar_wait(&v_empty[b], ph, p.status, MB_ST_TIMEOUT_TMA);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      copy(p.v_cache, sV + b * kTileB);
+      asm volatile("cp.async.wait_group 1;" ::: "memory");
+      announce(&k_full[b]);
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    if (__all_sync(0xffffffffu, ok) && j > 0) announce(&v_full[(j - 1) & 1]);
+  }
+  if (bad && p.status) atomicCAS(p.status, 0u, MB_ST_BOUNDS);
+}
+
+template <int D, bool FP8>
+struct PrefixCfg {
+  static constexpr int kT = 128, kThreads = 512;
+  static constexpr int kQB = 128 * D * 2, kTileB = kT * D * 2;
+  static constexpr int kSmem = 2 * kQB + 4 * kTileB + 1024 + (int)sizeof(Plan);
+};
+
+template <int D, bool FP8>
+__global__ void __launch_bounds__(512, 1) shared_prefix_kernel(const MbSharedArgs p, const Ws ws) {
+  using C = PrefixCfg<D, FP8>;
+  constexpr int kT = C::kT, kQB = C::kQB, kTileB = C::kTileB, kSpans = D / 64;
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  uint8_t* sQ = smem_raw + ((1024u - (mb::smem_u32(smem_raw) & 1023u)) & 1023u);   // 2 row tiles x spans of 64 dims x [128 rows x 128 B]
+  uint8_t* sK = sQ + 2 * kQB;                             // 2 stages x spans x [128 tokens x 128 B]
+  uint8_t* sV = sK + 2 * kTileB;
+  Plan& plan = *reinterpret_cast<Plan*>(sV + 2 * kTileB);
+  __shared__ __align__(8) uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2];
+  __shared__ uint32_t s_tmem;
+  __shared__ float s_qscale[2][2][128];                   // what a row's scores are too large by (e4m3 cache), of parts in turn
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = p.Hq / p.Hkv;
+  mb::pdl_wait();
+  if (warp == 0) {
+    make_plan<D>(p, plan, lane);
+  } else if (warp == 1 && lane == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mb::mbar_init(&q_full[i], 4);
+      mb::mbar_init(&k_full[i], 4);
+      mb::mbar_init(&v_full[i], 4);
+      mb::mbar_init(&k_empty[i], 1);
+      mb::mbar_init(&v_empty[i], 1);
+      mb::mbar_init(&s_full[i], 1);
+      mb::mbar_init(&p_full[i], 4);
+      mb::mbar_init(&o_full[i], 1);
+    }
+    mb::mbar_fence_init();
+  }
+  if (warp == 12) mb::tmem_alloc(&s_tmem, 512);
+  mb::tc_fence_before();
+  __syncthreads();
+  mb::tc_fence_after();
+  mb::pdl_launch_dependents();                            // behind this kernel's own wait: what the step before it wrote is there for them too
+  const uint32_t tmem = s_tmem;                           // S0 0-127, S1 128-255, O0 256-, O1 384-
+  const long long W = plan.base[p.groups];
+  const long long begin = place_of(blockIdx.x, ws.ctas, W), end = place_of(blockIdx.x + 1, ws.ctas, W);
+
+  if (warp < 8) {
+    // ------------------------------------------------------------ softmax
+    more_regs<184>();
+    const int w = warp >> 2, r = tid & 127;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t tS = tmem + lanes + w * 128, tO = tmem + lanes + 256 + w * 128;
+    const float sc0 = p.scale * (FP8 ? *p.k_scale : 1.f) * 1.44269504088896f;
+    uint32_t part = 0, done = 0, outs = 0;                // parts, tiles and outputs that this accumulator has had
+    bool ok = true;
+    long long pos = begin;
+    Part x;
+    while (ok && next_part<D>(p, plan, pos, end, x)) {
+      const int n = x.t1 - x.t0, mine = x.two ? n : (n + 1 - w) / 2;
+      const size_t row0 = (size_t)plan.start[x.group] * p.q_len * G + x.row0;      // of the kv head's rows
+      if (x.two || w == 0) {
+        // 128 rows x D / 8 pieces of 8 dims, a thread's loads in flight together (rows past the last one read it again and become zeros)
+        constexpr int kPieces = D / 8, kQ = kPieces, kStep = 128 / kPieces;
+        const int c = r % kPieces, first = r / kPieces, last = x.rows - w * 128 - 1;
+        uint4 v[kQ];
+#pragma unroll
+        for (int i = 0; i < kQ; ++i) {
+          const size_t at = row0 + w * 128 + min(first + kStep * i, last), tok = at / G;
+          v[i] = *(reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(p.q) + (tok * p.Hq + x.kvh * G + (at - tok * G)) * D) + c);
+        }
+#pragma unroll
+        for (int i = 0; i < kQ; ++i) {
+          const int qr = first + kStep * i;
+          if (qr > last) v[i] = make_uint4(0, 0, 0, 0);
+          float back = 1.f;
+          v[i] = query_piece<D, FP8>(v[i], back);
+          if (FP8 && c == 0) s_qscale[part & 1][w][qr] = back;
+          *reinterpret_cast<uint4*>(sQ + w * kQB + (c >> 3) * (128 * 128) + sw_off(qr, c & 7)) = v[i];
+        }
+        fence_async_smem();
+      }
+      // A wait tells a phase from its neighbours only, so no warp may be a part ahead of one that waits: where the rows are those of the other
+      // accumulator, their arrival is seen before this one's is announced, which the products and with them the next part wait for
+      const int side = x.two ? w : 0;                     // whose rows these are
+      if (side != w) {
+        ok = mb::mbar_wait(&q_full[side], part & 1, p.status, MB_ST_TIMEOUT_MMA);
+        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+      }
+      __syncwarp();
+      if (lane == 0) mb::mbar_arrive(&q_full[w]);
+      float sc = sc0;
+      if constexpr (FP8) {                                // the rows' scales come from other softmax warps
+        if (side == w) ok = mb::mbar_wait(&q_full[w], part & 1, p.status, MB_ST_TIMEOUT_MMA);
+        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+        sc *= s_qscale[part & 1][side][r];
+      }
+      const int left = x.two ? x.rows - w * 128 : x.rows; // rows of this tile
+      const bool live = r < left, some = (warp & 3) * 32 < left;
+      const int len = plan.len[x.group];
+      float m_run = -INFINITY, l_run = 0.f;
+      for (int i = 0; i < mine; ++i) {
+        const int t = x.t0 + (x.two ? i : 2 * i + w);
+        ok = mb::mbar_wait(&s_full[w], (done + i) & 1, p.status, MB_ST_TIMEOUT_MMA);
+        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+        mb::tc_fence_after();
+        if (some) {                                       // warps without rows hand on what the columns hold: it meets no other row
+          float s[kT];
+#pragma unroll
+          for (int c = 0; c < kT; c += 32) mb::tmem_ld32_async(tS + c, s + c);
+          mb::tmem_ld_wait(s);
+          const int seen = len - t * kT;                  // columns below this are cached tokens
+          if (seen < kT) {
+#pragma unroll
+            for (int k = 0; k < kT; ++k)
+              if (k >= seen) s[k] = -INFINITY;
+          }
+          float mx4[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+          for (int k = 4; k < kT; ++k) mx4[k & 3] = fmaxf(mx4[k & 3], s[k]);
+          const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * sc;
+          float alpha = 1.f;
+          const bool move = mx > m_run + 8.f;             // also true on a row's first finite tile
+          if (move) {
+            alpha = ex2(m_run - mx);                      // 0 when the row had seen nothing yet
+            m_run = mx;
+          }
+          if (i > 0 && __any_sync(0xffffffffu, move)) {
+#pragma unroll
+            for (int c = 0; c < D; c += 16) {
+              float ov[16];
+              mb::tmem_ld16(tO + c, ov);
+#pragma unroll
+              for (int k = 0; k < 16; ++k) ov[k] *= alpha;
+              mb::tmem_st16(tO + c, ov);
+            }
+          }
+          const float nm = m_run == -INFINITY ? 0.f : (FP8 ? kLift : 0.f) - m_run;
+          const float2 sc2 = make_float2(sc, sc), nm2 = make_float2(nm, nm);
+          float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t pk[32];
+#pragma unroll
+            for (int k = 0; k < 32; ++k) {
+              float2 e = fma2(make_float2(s[h * 64 + 2 * k], s[h * 64 + 2 * k + 1]), sc2, nm2);
+              e.x = ex2(e.x);
+              e.y = ex2(e.y);
+              sum[k & 1] = add2(sum[k & 1], e);
+              pk[k] = pack2<FP8>(e.x, e.y);
+            }
+            tmem_st32(tS + h * 32, pk);
+          }
+          mb::tmem_st_wait();
+          l_run = l_run * alpha + ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y));
+        }
+        mb::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mb::mbar_arrive(&p_full[w]);
+      }
+      if (!ok) break;
+      // without a tile of its own an accumulator waits for the other's outputs, which every part has: its rows are announced a part at a time
+      ok = mine > 0 ? mb::mbar_wait(&o_full[w], outs & 1, p.status, MB_ST_TIMEOUT_MMA) : mb::mbar_wait(&o_full[0], part & 1, p.status, MB_ST_TIMEOUT_MMA);
+      if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+      mb::tc_fence_after();
+      outs += mine > 0;
+      const Place to = x.t0 == 0 ? place_first<D>(p, ws, plan, x.group, x.kvh, x.row0 + (x.two ? w * 128 : 0), x.two ? 0 : w) : place_rest<D>(p, ws, blockIdx.x, w);
+      if (mine > 0 && some) {
+#pragma unroll 1
+        for (int c0 = 0; c0 < D; c0 += 32) {
+          float o[32];
+          mb::tmem_ld32_async(tO + c0, o);
+          mb::tmem_ld_wait(o);
+          if (live)
+#pragma unroll
+            for (int c = 0; c < 8; ++c) to.o[(c0 / 4 + c) * to.pitch + r] = make_float4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
+        }
+      }
+      if (live) to.ml[r] = make_float2(m_run - (FP8 ? kLift : 0.f), l_run);
+      mb::tc_fence_before();
+      done += mine;
+      ++part;
+    }
+  } else if (warp < 12) {
+    // ------------------------------------------------------------ loader
+    fewer_regs<96>();
+    load_tiles<D, FP8, kT>(p, plan, begin, end, sK, sV, k_full, k_empty, v_full, v_empty, tid - 256);
+  } else {
+    fewer_regs<48>();
+    if (warp == 12 && mb::elect_one()) {
+      // ---------------------------------------------------------- products
+      constexpr uint32_t kF = FP8 ? 0 : 1;
+      constexpr uint32_t kIdS = mb::umma_idesc(kF, kF, 128, kT), kIdO = mb::umma_idesc(kF, kF, 128, D, 0, 1);
+      const uint32_t aQ = mb::smem_u32(sQ), aK = mb::smem_u32(sK), aV = mb::smem_u32(sV);
+      uint32_t part = 0, base = 0, done[2] = {0, 0};      // parts, tiles brought, tiles that either accumulator has had
+      bool ok = true;
+      long long pos = begin;
+      Part x;
+      while (ok && next_part<D>(p, plan, pos, end, x)) {
+        const int n = x.t1 - x.t0, n0 = x.two ? n : (n + 1) / 2, n1 = x.two ? n : n / 2;
+        auto stage = [&](int w, int i) { return base + (x.two ? i : 2 * i + w); };
+        auto scores = [&](int w, int i) {
+          const uint32_t t = stage(w, i);
+          if (!mb::mbar_wait(&k_full[t & 1], (t >> 1) & 1, p.status, MB_ST_TIMEOUT_MMA)) return false;
+          mb::tc_fence_after();
+#pragma unroll
+          for (int h = 0; h < kSpans; ++h)
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+              mb::umma_f16(tmem + w * 128, mb::umma_desc_sw128(aQ + (x.two ? w : 0) * kQB + h * (128 * 128) + s * 32),
+                           mb::umma_desc_sw128(aK + (t & 1) * kTileB + h * (kT * 128) + s * 32), kIdS, (h | s) != 0);
+          mb::tc_commit(&s_full[w]);
+          if (!x.two || w == 1) mb::tc_commit(&k_empty[t & 1]);
+          return true;
+        };
+        auto values = [&](int w, int i) {
+          const uint32_t t = stage(w, i);
+          if (!mb::mbar_wait(&v_full[t & 1], (t >> 1) & 1, p.status, MB_ST_TIMEOUT_MMA) ||
+              !mb::mbar_wait(&p_full[w], (done[w] + i) & 1, p.status, MB_ST_TIMEOUT_MMA))
+            return false;
+          mb::tc_fence_after();
+#pragma unroll
+          for (int s = 0; s < kT / 16; ++s)
+            umma_f16_ta(tmem + 256 + w * 128, tmem + w * 128 + s * 8, mb::umma_desc_sw128_mn(aV + (t & 1) * kTileB + s * 2048, kT * 128, 1024), kIdO, (i | s) != 0);
+          if (!x.two || w == 1) mb::tc_commit(&v_empty[t & 1]);
+          return true;
+        };
+        // both accumulators' rows are written, and their former outputs read
+        ok = mb::mbar_wait(&q_full[0], part & 1, p.status, MB_ST_TIMEOUT_MMA) && mb::mbar_wait(&q_full[1], part & 1, p.status, MB_ST_TIMEOUT_MMA);
+        if (ok) ok = scores(0, 0);
+        if (ok && n1 > 0) ok = scores(1, 0);
+        for (int i = 0; i < n0 && ok; ++i) {
+          ok = values(0, i);
+          if (!ok) break;
+          if (i + 1 < n0) ok = scores(0, i + 1);
+          else mb::tc_commit(&o_full[0]);
+          if (!ok || i >= n1) break;
+          ok = values(1, i);
+          if (!ok) break;
+          if (i + 1 < n1) ok = scores(1, i + 1);
+          else mb::tc_commit(&o_full[1]);
+        }
+        base += n;
+        done[0] += n0;
+        done[1] += n1;
+        ++part;
+      }
+    }
+    __syncwarp();
+  }
+  __syncthreads();
+  if (warp == 12) {
+    mb::tc_fence_after();
+    mb::tmem_dealloc(tmem, 512);
+  }
+}
+
+// Heads of 256 dims: one tile of 128 rows a CTA (its outputs are half of TMEM), tiles of 64 cached tokens, two tiles of scores in turn: the products of the
+// next one run under the softmax of this one. Warps 0-3 softmax, 4-7 loader, 8 products.
+template <bool FP8>
+__global__ void __launch_bounds__(288, 1) shared_prefix256_kernel(const MbSharedArgs p, const Ws ws) {
+  constexpr int D = 256, kT = 64, kQB = 128 * D * 2, kTileB = kT * D * 2, kSpans = D / 64;
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  uint8_t* sQ = smem_raw + ((1024u - (mb::smem_u32(smem_raw) & 1023u)) & 1023u);   // 4 spans x [128 rows x 128 B]
+  uint8_t* sK = sQ + kQB;                                 // 2 stages x 4 spans x [64 tokens x 128 B]
+  uint8_t* sV = sK + 2 * kTileB;
+  Plan& plan = *reinterpret_cast<Plan*>(sV + 2 * kTileB);
+  __shared__ __align__(8) uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_done, o_full;
+  __shared__ uint32_t s_tmem;
+  __shared__ float s_qscale[2][128];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = p.Hq / p.Hkv;
+  mb::pdl_wait();
+  if (warp == 0) {
+    make_plan<D>(p, plan, lane);
+  } else if (warp == 1 && lane == 0) {
+    mb::mbar_init(&q_full, 4);
+    mb::mbar_init(&o_done, 1);
+    mb::mbar_init(&o_full, 1);
+    for (int i = 0; i < 2; ++i) {
+      mb::mbar_init(&k_full[i], 4);
+      mb::mbar_init(&v_full[i], 4);
+      mb::mbar_init(&k_empty[i], 1);
+      mb::mbar_init(&v_empty[i], 1);
+      mb::mbar_init(&s_full[i], 1);
+      mb::mbar_init(&p_full[i], 4);
+    }
+    mb::mbar_fence_init();
+  }
+  if (warp == 8) mb::tmem_alloc(&s_tmem, 512);
+  mb::tc_fence_before();
+  __syncthreads();
+  mb::tc_fence_after();
+  mb::pdl_launch_dependents();
+  const uint32_t tmem = s_tmem;                           // S0 0-63, S1 64-127, O 256-511
+  const long long W = plan.base[p.groups];
+  const long long begin = place_of(blockIdx.x, ws.ctas, W), end = place_of(blockIdx.x + 1, ws.ctas, W);
+
+  if (warp < 4) {
+    // ------------------------------------------------------------ softmax
+    const uint32_t lanes = (uint32_t)(warp * 32) << 16;
+    const uint32_t tO = tmem + lanes + 256;
+    const float sc0 = p.scale * (FP8 ? *p.k_scale : 1.f) * 1.44269504088896f;
+    uint32_t part = 0, base = 0;                          // parts, tiles that are done
+    bool ok = true;
+    long long pos = begin;
+    Part x;
+    while (ok && next_part<D>(p, plan, pos, end, x)) {
+      const int n = x.t1 - x.t0, last = x.rows - 1;
+      const size_t row0 = (size_t)plan.start[x.group] * p.q_len * G + x.row0;
+      // 128 rows x 32 pieces of 8 dims, sixteen of a thread's loads in flight together (rows past the last one are zeros)
+#pragma unroll 1
+      for (int half = 0; half < 2; ++half) {
+        uint4 v[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const size_t at = row0 + min(warp + 4 * (half * 16 + i), last), tok = at / G;
+          v[i] = *(reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(p.q) + (tok * p.Hq + x.kvh * G + (at - tok * G)) * D) + lane);
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int qr = warp + 4 * (half * 16 + i);
+          if (qr > last) v[i] = make_uint4(0, 0, 0, 0);
+          float back = 1.f;
+          v[i] = query_piece<D, FP8>(v[i], back);
+          if (FP8 && lane == 0) s_qscale[part & 1][qr] = back;
+          *reinterpret_cast<uint4*>(sQ + (lane >> 3) * (128 * 128) + sw_off(qr, lane & 7)) = v[i];
+        }
+      }
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) mb::mbar_arrive(&q_full);
+      float sc = sc0;
+      if constexpr (FP8) {
+        ok = mb::mbar_wait(&q_full, part & 1, p.status, MB_ST_TIMEOUT_MMA);
+        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+        sc *= s_qscale[part & 1][tid];
+      }
+      const bool live = tid <= last, some = warp * 32 <= last;
+      const int len = plan.len[x.group];
+      float m_run = -INFINITY, l_run = 0.f;
+      for (int i = 0; i < n; ++i) {
+        const uint32_t j = base + i, tS = tmem + lanes + (j & 1) * kT;
+        ok = mb::mbar_wait(&s_full[j & 1], (j >> 1) & 1, p.status, MB_ST_TIMEOUT_MMA);
+        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+        mb::tc_fence_after();
+        if (some) {
+          float s[kT];
+#pragma unroll
+          for (int c = 0; c < kT; c += 32) mb::tmem_ld32_async(tS + c, s + c);
+          mb::tmem_ld_wait(s);
+          const int seen = len - (x.t0 + i) * kT;
+          if (seen < kT) {
+#pragma unroll
+            for (int k = 0; k < kT; ++k)
+              if (k >= seen) s[k] = -INFINITY;
+          }
+          float mx4[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+          for (int k = 4; k < kT; ++k) mx4[k & 3] = fmaxf(mx4[k & 3], s[k]);
+          const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * sc;
+          float alpha = 1.f;
+          const bool move = mx > m_run + 8.f;
+          if (move) {
+            alpha = ex2(m_run - mx);
+            m_run = mx;
+          }
+          if (i > 0 && __any_sync(0xffffffffu, move)) {
+            ok = mb::mbar_wait(&o_done, (j - 1) & 1, p.status, MB_ST_TIMEOUT_MMA);     // P V of the tile before: that of this one waits for this warp
+            if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+            mb::tc_fence_after();
+#pragma unroll
+            for (int c = 0; c < D; c += 16) {
+              float ov[16];
+              mb::tmem_ld16(tO + c, ov);
+#pragma unroll
+              for (int k = 0; k < 16; ++k) ov[k] *= alpha;
+              mb::tmem_st16(tO + c, ov);
+            }
+          }
+          const float nm = m_run == -INFINITY ? 0.f : (FP8 ? kLift : 0.f) - m_run;
+          const float2 sc2 = make_float2(sc, sc), nm2 = make_float2(nm, nm);
+          float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+          uint32_t pk[32];
+#pragma unroll
+          for (int k = 0; k < 32; ++k) {
+            float2 e = fma2(make_float2(s[2 * k], s[2 * k + 1]), sc2, nm2);
+            e.x = ex2(e.x);
+            e.y = ex2(e.y);
+            sum[k & 1] = add2(sum[k & 1], e);
+            pk[k] = pack2<FP8>(e.x, e.y);
+          }
+          tmem_st32(tS, pk);
+          mb::tmem_st_wait();
+          l_run = l_run * alpha + ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y));
+        }
+        mb::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mb::mbar_arrive(&p_full[j & 1]);
+      }
+      if (!ok) break;
+      ok = mb::mbar_wait(&o_full, part & 1, p.status, MB_ST_TIMEOUT_MMA);
+      if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+      mb::tc_fence_after();
+      const Place to = x.t0 == 0 ? place_first<D>(p, ws, plan, x.group, x.kvh, x.row0, 0) : place_rest<D>(p, ws, blockIdx.x, 0);
+      if (some) {
+#pragma unroll 1
+        for (int c0 = 0; c0 < D; c0 += 64) {
+          float o[64];
+          mb::tmem_ld32_async(tO + c0, o);
+          mb::tmem_ld32_async(tO + c0 + 32, o + 32);
+          mb::tmem_ld_wait(o);
+          if (live)
+#pragma unroll
+            for (int c = 0; c < 16; ++c) to.o[(c0 / 4 + c) * to.pitch + tid] = make_float4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
+        }
+      }
+      if (live) to.ml[tid] = make_float2(m_run - (FP8 ? kLift : 0.f), l_run);
+      mb::tc_fence_before();
+      base += n;
+      ++part;
+    }
+  } else if (warp < 8) {
+    load_tiles<D, FP8, kT>(p, plan, begin, end, sK, sV, k_full, k_empty, v_full, v_empty, tid - 128);
+  } else {
+    if (mb::elect_one()) {
+      // ---------------------------------------------------------- products
+      constexpr uint32_t kF = FP8 ? 0 : 1;
+      constexpr uint32_t kIdS = mb::umma_idesc(kF, kF, 128, kT), kIdO = mb::umma_idesc(kF, kF, 128, D, 0, 1);
+      const uint32_t aQ = mb::smem_u32(sQ), aK = mb::smem_u32(sK), aV = mb::smem_u32(sV);
+      uint32_t part = 0, base = 0;
+      bool ok = true;
+      long long pos = begin;
+      Part x;
+      auto scores = [&](uint32_t j) {
+        if (!mb::mbar_wait(&k_full[j & 1], (j >> 1) & 1, p.status, MB_ST_TIMEOUT_MMA)) return false;
+        mb::tc_fence_after();
+#pragma unroll
+        for (int h = 0; h < kSpans; ++h)
+#pragma unroll
+          for (int s = 0; s < 4; ++s)
+            mb::umma_f16(tmem + (j & 1) * kT, mb::umma_desc_sw128(aQ + h * (128 * 128) + s * 32),
+                         mb::umma_desc_sw128(aK + (j & 1) * kTileB + h * (kT * 128) + s * 32), kIdS, (h | s) != 0);
+        mb::tc_commit(&s_full[j & 1]);
+        mb::tc_commit(&k_empty[j & 1]);
+        return true;
+      };
+      while (ok && next_part<D>(p, plan, pos, end, x)) {
+        const int n = x.t1 - x.t0;
+        ok = mb::mbar_wait(&q_full, part & 1, p.status, MB_ST_TIMEOUT_MMA) && scores(base);
+        for (int i = 0; i < n && ok; ++i) {
+          const uint32_t j = base + i, b = j & 1;
+          if (i + 1 < n) {                                // over P of the tile before, whose product was issued in front
+            ok = scores(j + 1);
+            if (!ok) break;
+          }
+          ok = mb::mbar_wait(&v_full[b], (j >> 1) & 1, p.status, MB_ST_TIMEOUT_MMA) && mb::mbar_wait(&p_full[b], (j >> 1) & 1, p.status, MB_ST_TIMEOUT_MMA);
+          if (!ok) break;
+          mb::tc_fence_after();
+#pragma unroll
+          for (int s = 0; s < kT / 16; ++s)
+            umma_f16_ta(tmem + 256, tmem + b * kT + s * 8, mb::umma_desc_sw128_mn(aV + b * kTileB + s * 2048, kT * 128, 1024), kIdO, (i | s) != 0);
+          mb::tc_commit(&v_empty[b]);
+          mb::tc_commit(&o_done);
+          if (i + 1 == n) mb::tc_commit(&o_full);
+        }
+        base += n;
+        ++part;
+      }
+    }
+    __syncwarp();
+  }
+  __syncthreads();
+  if (warp == 8) {
+    mb::tc_fence_after();
+    mb::tmem_dealloc(tmem, 512);
+  }
+}
+
+template <int D, bool FP8>
+int launch_prefix(const MbSharedArgs& a, const Ws& ws, cudaStream_t stream) {
+  void (*kern)(const MbSharedArgs, const Ws);
+  int threads, smem;
+  if constexpr (D == 256) {
+    kern = shared_prefix256_kernel<FP8>;
+    threads = 288;
+    smem = 128 * D * 2 + 4 * 64 * D * 2 + 1024 + (int)sizeof(Plan);
+  } else {
+    kern = shared_prefix_kernel<D, FP8>;
+    threads = PrefixCfg<D, FP8>::kThreads;
+    smem = PrefixCfg<D, FP8>::kSmem;
+  }
+  static std::atomic<uint64_t> asked{0};
+  const cudaError_t e = mb::allow_smem(reinterpret_cast<const void*>(kern), smem, asked);
+  if (e != cudaSuccess) return (int)e;
+  return (int)mb::launch_kernel(kern, dim3(ws.ctas), dim3(threads), smem, stream, a, ws);
+}
+
+}  // namespace mbs

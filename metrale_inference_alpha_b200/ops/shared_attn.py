@@ -49,6 +49,18 @@ def _library():
     return _lib
 
 
+_ws_bytes: dict = {}
+
+
+def _workspace(name: str, *sizes) -> int:
+    fn = _ws_bytes.get(name)
+    if fn is None:
+        fn = getattr(_library(), name)
+        fn.restype, fn.argtypes = C.c_size_t, [C.c_int] * len(sizes)
+        _ws_bytes[name] = fn
+    return fn(*sizes)
+
+
 def _bad(where: str, what: str):
     raise ValueError(f"{where}: {what}")
 
@@ -120,8 +132,8 @@ def shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     Hq = q.shape[1]
     if Hq == 0 or Hq % Hkv != 0 or Hq // Hkv > MAX_GROUP:
         _bad(where, f"{Hq} query heads over {Hkv} kv heads: whole groups of up to {MAX_GROUP}")
-    if T * Hq > 1 << 26:
-        _bad(where, f"{T} tokens of {Hq} heads are more than 2^26 rows")
+    if T * Hq * D > 1 << 29:
+        _bad(where, f"{T} tokens of {Hq} heads of {D} dims are more than 2^29 elements: a step of a batch is meant, not its prompts")
     if not scale > 0:
         _bad(where, "scale is positive")
     fp8 = dtype == torch.uint8
@@ -149,11 +161,13 @@ def shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
         out.zero_()
         return (out, lse.fill_(-float("inf"))) if return_lse else out
     rt = runtime(q.device)
+    need = _workspace("mb_shared_attn_ws", S, q_len, groups, Hq, Hkv, D, max_prefix, max_ctx, rt.sm_count)
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device)
     a = _SHARED_ARGS.pack(qp, kp, vp, prefix_table.data_ptr(), prefix_table.stride(0), prefix_len.data_ptr(), group_start.data_ptr(), block_table.data_ptr(),
-                          block_table.stride(0), ctx_len.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(), 0, 0, k_scale.data_ptr() if fp8 else 0,
+                          block_table.stride(0), ctx_len.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(), ws.data_ptr(), need, k_scale.data_ptr() if fp8 else 0,
                           v_scale.data_ptr() if fp8 else 0, rt.status.data_ptr(), nb, S, q_len, groups, Hq, Hkv, D, bs, int(fp8), max_prefix, max_ctx, rt.sm_count, scale)
     _native.check(_library().mb_shared_attn(a, _stream()), "shared_attn")
-    _count()
+    _count(1 + (groups > 0 and max_prefix > 0) + (max_ctx > 0))          # the join, prefixes, own rows; further steps, which go by the sizes, are not counted
     return (out, lse) if return_lse else out
 
 
