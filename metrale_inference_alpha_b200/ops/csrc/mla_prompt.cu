@@ -24,66 +24,86 @@ struct GatherParams {
   int num_seqs, block_size, max_ctx;
 };
 
+constexpr int kGather = 32;                                // rows of a CTA, four a warp
+
 __global__ void __launch_bounds__(256) gather_kernel(const GatherParams p) {
   mb::pdl_wait();
-  __shared__ long long s_first[2];
+  mb::pdl_launch_dependents();
+  __shared__ long long s_at;
+  __shared__ int s_seq, s_bad[8];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const long long r0 = (long long)blockIdx.x * 128;
-  if (tid == 0) {
+  const long long r0 = (long long)blockIdx.x * kGather;
+  if (tid == 0) s_seq = -1;
+  __syncthreads();
+  if (warp == 0) {
     long long at = 0;
-    int found = -1;
-    for (int s = 0; s < p.num_seqs; ++s) {
-      const int n = p.ctx_len[s], len = min(max(n, 0), p.max_ctx);
-      const long long end = at + ((len + 127) & ~127);
-      if (n > p.max_ctx || end > p.kv_rows)
-        if (p.status) atomicCAS(p.status, 0u, MB_ST_BOUNDS);
-      if (blockIdx.x == 0) p.first[s] = (int)min(at, p.kv_rows);
-      if (r0 >= at && r0 < end) {
-        found = s;
-        s_first[1] = at;
+    for (int s0 = 0; s0 < p.num_seqs; s0 += 32) {
+      const int s = s0 + lane;
+      int n = 0;
+      if (s < p.num_seqs) n = p.ctx_len[s];
+      const long long len = (min(max(n, 0), p.max_ctx) + 127) & ~127;
+      long long x = len;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const long long y = __shfl_up_sync(0xffffffffu, x, d);
+        if (lane >= d) x += y;
       }
-      at = end;
+      const long long end = at + x, begin = end - len;
+      if (s < p.num_seqs) {
+        if (blockIdx.x == 0) {
+          p.first[s] = (int)min(begin, p.kv_rows);
+          if ((n > p.max_ctx || end > p.kv_rows) && p.status) atomicCAS(p.status, 0u, MB_ST_BOUNDS);
+        }
+        if (r0 >= begin && r0 < end) {
+          s_seq = s;
+          s_at = begin;
+        }
+      }
+      at = __shfl_sync(0xffffffffu, end, 31);
+      if (blockIdx.x > 0 && at > r0) break;
     }
-    s_first[0] = found;
   }
   __syncthreads();
-  const int s = (int)s_first[0];
+  const int s = s_seq;
   if (s < 0) return;
-  const int j0 = (int)(r0 - s_first[1]), n = min(max(p.ctx_len[s], 0), p.max_ctx);
-  int bad = 0x7fffffff;
-  for (int r = warp; r < 128; r += 8) {
+  const int j0 = (int)(r0 - s_at) + warp * 4, n = min(max(p.ctx_len[s], 0), p.max_ctx);
+  // a warp's rows: places first, then everything that is read, then the stores
+  const uint4* src[4];
+  uint4 v[4][3];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
     const int j = j0 + r;
-    uint4* dst = reinterpret_cast<uint4*>(p.lat + (r0 + r) * kRow);
-    const uint4* src = nullptr;
+    src[r] = nullptr;
     if (j < n) {
       int b = p.block_table[s * p.table_ld + j / p.block_size];
       if (b < 0 || b >= p.num_blocks) {
         if (lane == 0 && p.status) atomicCAS(p.status, 0u, MB_ST_BOUNDS);
         b = 0;
       }
-      src = reinterpret_cast<const uint4*>(p.cache + ((size_t)b * p.block_size + j % p.block_size) * kRow);
-    }
-    uint4 v[3];
-    bool odd = false;
-#pragma unroll
-    for (int i = 0; i < 3; ++i) {
-      const int c = lane + 32 * i;
-      v[i] = src && c < kRow / 8 ? src[c] : make_uint4(0, 0, 0, 0);
-      if (c < kLat / 8) {
-        const uint32_t x[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) odd |= (x[k] & 0x7f80u) == 0x7f80u || (x[k] & 0x7f800000u) == 0x7f800000u;
-      }
-    }
-    odd = __any_sync(0xffffffffu, odd);
-    if (odd) bad = min(bad, j);
-#pragma unroll
-    for (int i = 0; i < 3; ++i) {
-      const int c = lane + 32 * i;
-      if (c < kRow / 8) dst[c] = odd && c < kLat / 8 ? make_uint4(0, 0, 0, 0) : v[i];
+      src[r] = reinterpret_cast<const uint4*>(p.cache + ((size_t)b * p.block_size + j % p.block_size) * kRow);
     }
   }
-  __shared__ int s_bad[8];
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+#pragma unroll
+    for (int i = 0; i < 3; ++i) v[r][i] = src[r] && lane + 32 * i < kRow / 8 ? src[r][lane + 32 * i] : make_uint4(0, 0, 0, 0);
+  int bad = 0x7fffffff;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    bool odd = false;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {                          // the latent: 64 pieces of 8
+      const uint32_t x[4] = {v[r][i].x, v[r][i].y, v[r][i].z, v[r][i].w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) odd |= (x[k] & 0x7f80u) == 0x7f80u || (x[k] & 0x7f800000u) == 0x7f800000u;
+    }
+    odd = __any_sync(0xffffffffu, odd);
+    if (odd) bad = min(bad, j0 + r);
+    uint4* dst = reinterpret_cast<uint4*>(p.lat + (r0 + warp * 4 + r) * kRow) + lane;
+#pragma unroll
+    for (int i = 0; i < 3; ++i)
+      if (lane + 32 * i < kRow / 8) dst[32 * i] = odd && i < 2 ? make_uint4(0, 0, 0, 0) : v[r][i];
+  }
   if (lane == 0) s_bad[warp] = bad;
   __syncthreads();
   if (tid == 0) {
@@ -224,7 +244,7 @@ mla_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     }
     // the first cached token that is no number, of those that the tile sees: it lies in the expanded rows as zeros
     int bad = 0x7fffffff;
-    for (int j = lane; j < mine; j += 32) bad = min(bad, p.bad[first / kT + j]);
+    for (int j = lane; j < mine * (kT / kGather); j += 32) bad = min(bad, p.bad[first / kGather + j]);
     bad = __reduce_min_sync(0xffffffffu, bad);
     if (ok && mine > 0) {
       ok = mb::mbar_wait(&o_full[w], 0, p.status, MB_ST_TIMEOUT_MMA);
@@ -367,7 +387,7 @@ int mb_mla_gather(const void* cache, const int* block_table, long long table_ld,
   if (!cache || !block_table || !ctx_len || !lat || !first || !bad || num_blocks <= 0 || kv_rows <= 0 || kv_rows % 128 || num_seqs <= 0 || block_size <= 0 || max_ctx <= 0)
     return MB_ERR_BAD_ARG;
   GatherParams p{(const __nv_bfloat16*)cache, block_table, table_ld, ctx_len, (__nv_bfloat16*)lat, first, bad, status, num_blocks, kv_rows, num_seqs, block_size, max_ctx};
-  return (int)mb::launch_kernel(gather_kernel, dim3((unsigned)(kv_rows / 128)), dim3(256), 0, stream, p);
+  return (int)mb::launch_kernel(gather_kernel, dim3((unsigned)(kv_rows / kGather)), dim3(256), 0, stream, p);
 }
 
 int mb_mla_prompt(const MbMlaPromptArgs* a, cudaStream_t stream) {
@@ -386,7 +406,7 @@ int mb_mla_prompt(const MbMlaPromptArgs* a, cudaStream_t stream) {
   static std::atomic<uint64_t> asked{0};
   const cudaError_t e = mb::allow_smem(reinterpret_cast<const void*>(mla_prompt_kernel), kSmem, asked);
   if (e != cudaSuccess) return (int)e;
-  return (int)mb::launch_kernel(mla_prompt_kernel, dim3(a->heads, tiles, a->num_seqs), dim3(kThreads), kSmem, stream, tm[0], tm[1], tm[2], tm[3], *a);
+  return (int)mb::launch_kernel_ex(mla_prompt_kernel, dim3(a->heads, tiles, a->num_seqs), dim3(kThreads), kSmem, stream, 1, mb_pdl_enabled() != 0, tm[0], tm[1], tm[2], tm[3], *a);
 }
 
 }  // extern "C"

@@ -47,42 +47,54 @@ Ws workspace(const MbSharedArgs& a) {
   return w;
 }
 
-// 32 rows (tokens x heads of a group) of a kv head a CTA, lane = row; warp w has dims w D / 8 to (w + 1) D / 8 of them.
+// 32 rows (tokens x heads of a group) of a kv head and 32 dims a CTA, lane = row. A row's partial results are shared out over the eight warps, each of
+// which asks for maximum, sum and dims together, and the warps' sums are joined in shared memory: few rows have many parts, and their latencies do not add up.
+constexpr int kJoinDims = 32;
+
 template <int D, bool FP8>
 __global__ void __launch_bounds__(256) shared_join_kernel(const MbSharedArgs p, const Ws ws, int tok0, int tokens) {
   __shared__ Plan plan;
+  __shared__ float4 s_o[8][kJoinDims / 4][32];
+  __shared__ float2 s_ml[8][32];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = p.Hq / p.Hkv, kvh = blockIdx.y;
+  constexpr int kC = kJoinDims / 4;
+  const int c0 = blockIdx.z * kC;                          // fours of dims
   mb::pdl_wait();
   const bool prefixes = p.groups > 0 && p.max_prefix > 0;
   if (prefixes) {
     if (warp == 0) make_plan<D>(p, plan, lane);
     __syncthreads();
   }
-  const long long R = (long long)blockIdx.x * 32 + lane;   // of the step's rows
-  if (R >= (long long)tokens * G) return;
-  const int step_tok = (int)(R / G), head = (int)(R - (long long)step_tok * G), tok = tok0 + step_tok, seq = tok / p.q_len;
-  constexpr int kC = D / 32;                               // fours of dims of a thread
+  const int R = blockIdx.x * 32 + lane;                    // of the step's rows
+  const bool live = R < tokens * G;
+  const int step_tok = live ? R / G : 0, head = live ? R - step_tok * G : 0, tok = tok0 + step_tok, seq = tok / p.q_len;
   float m = -INFINITY, l = 0.f;
   float4 acc[kC];
 #pragma unroll
   for (int c = 0; c < kC; ++c) acc[c] = make_float4(0.f, 0.f, 0.f, 0.f);
-  auto add = [&](float2 ml, auto&& out) {
-    if (ml.y == 0.f) return;                               // nothing seen: what lies there is not looked at
-    const float mn = fmaxf(m, ml.x), base = mn == -INFINITY ? 0.f : mn;      // all scores NaN leave no maximum, but a sum that is NaN
-    const float fa = m == -INFINITY ? 0.f : ex2(m - base), fb = ex2(ml.x - base);
-    const float fb1 = ml.x == -INFINITY ? 1.f : fb;
+  auto add = [&](float2 ml, const float4* x) {
+    const bool none = ml.y == 0.f;                         // nothing seen: what lies there does not count
+    const float mn = none ? m : fmaxf(m, ml.x), base = mn == -INFINITY ? 0.f : mn;      // all scores NaN leave no maximum, but a sum that is NaN
+    const float fa = m == -INFINITY ? 0.f : ex2(m - base), fb = ml.x == -INFINITY ? 1.f : ex2(ml.x - base);
     m = mn;
-    l = l * fa + ml.y * fb1;
+    if (none) return;
+    l = l * fa + ml.y * fb;
 #pragma unroll
     for (int c = 0; c < kC; ++c) {
-      const float4 x = out(c);
-      acc[c].x = acc[c].x * fa + x.x * fb1;
-      acc[c].y = acc[c].y * fa + x.y * fb1;
-      acc[c].z = acc[c].z * fa + x.z * fb1;
-      acc[c].w = acc[c].w * fa + x.w * fb1;
+      acc[c].x = acc[c].x * fa + x[c].x * fb;
+      acc[c].y = acc[c].y * fa + x[c].y * fb;
+      acc[c].z = acc[c].z * fa + x[c].z * fb;
+      acc[c].w = acc[c].w * fa + x[c].w * fb;
     }
   };
-  if (prefixes && seq >= plan.start[0] && seq < plan.start[p.groups]) {
+  int own = 0, own_parts = 0;                              // asked for beside the prefix's parts
+  if (live && p.max_ctx > 0) {
+    own = min(max(p.ctx_len[seq], 0), p.max_ctx);
+    own = max(0, own - p.q_len + (tok - seq * p.q_len) + 1);
+    own_parts = own > 0 ? own_part_count(own, part_tokens_of(p.Hkv, D)) : 0;
+  }
+  int at_warp = warp;                                      // this warp's next part of those that come
+  if (live && prefixes && seq >= plan.start[0] && seq < plan.start[p.groups]) {
     int lo = 0, hi = p.groups;                             // start[lo] <= seq < start[hi]
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
@@ -94,46 +106,68 @@ __global__ void __launch_bounds__(256) shared_join_kernel(const MbSharedArgs p, 
       const int row = (tok - plan.start[lo] * p.q_len) * G + head;
       int doubles, singles;
       unit_count<D>(rows, doubles, singles);
-      const long long W = plan.base[p.groups];
+      const int W = plan.base[p.groups];
+      const Share share(W, used_ctas<D>(W, ws.ctas));
       const int two = row < doubles * 256, u = two ? row >> 8 : (row - doubles * 256) >> 7;
-      const long long at = plan.base[lo] + kvh * line_of_head<D>(rows, tiles) + (two ? 2ll * tiles * u : (2ll * doubles + u) * tiles);
+      const int at = plan.base[lo] + kvh * line_of_head<D>(rows, tiles) + (two ? 2 * tiles * u : (2 * doubles + u) * tiles);
       const int side = two ? (row >> 7) & 1 : 0, sides = two || D == 256 ? 1 : 2;
-      const int c0 = cta_of(at, ws.ctas, W), c1 = cta_of(at + ((long long)(tiles - 1) << two), ws.ctas, W);
-      for (int c = c0; c <= c1; ++c) {
+      const int cta0 = share.owner(at), n = (share.owner(at + ((tiles - 1) << two)) - cta0 + 1) * sides;
+      for (; at_warp < n; at_warp += 8) {
+        const int c = cta0 + at_warp / sides, k = at_warp % sides;
         int t0, t1;
-        tiles_in(at, tiles, two, place_of(c, ws.ctas, W), place_of(c + 1, ws.ctas, W), t0, t1);
+        tiles_in(at, tiles, two, share.first(c), share.first(c + 1), t0, t1);
         if (t1 <= t0) continue;
-        for (int k = 0; k < sides; ++k) {
-          const Place from = t0 == 0 ? place_first<D>(p, ws, plan, lo, kvh, row, k) : place_rest<D>(p, ws, c, two ? side : k);
-          const int r = t0 == 0 ? 0 : row & 127;
-          add(__ldcg(from.ml + r), [&](int i) { return __ldcg(from.o + (warp * kC + i) * from.pitch + r); });
-        }
+        const Place from = t0 == 0 ? place_first<D>(p, ws, plan, lo, kvh, row, k) : place_rest<D>(p, ws, c, two ? side : k);
+        const int r = t0 == 0 ? 0 : row & 127;
+        float4 x[kC];
+        const float2 ml = __ldcg(from.ml + r);
+#pragma unroll
+        for (int i = 0; i < kC; ++i) x[i] = __ldcg(from.o + (c0 + i) * from.pitch + r);
+        add(ml, x);
       }
+      at_warp -= n;
     }
   }
-  if (p.max_ctx > 0) {
-    int own = min(max(p.ctx_len[seq], 0), p.max_ctx);
-    own = max(0, own - p.q_len + (tok - seq * p.q_len) + 1);
-    if (own > 0) {
-      const int parts = own_part_count(own, part_tokens_of(p.Hkv, D));
-      const size_t at = ((size_t)step_tok * p.Hq + kvh * G + head) * ws.parts;
-      const float4* o = reinterpret_cast<const float4*>(reinterpret_cast<const uint8_t*>(p.ws) + ws.own) + at * (D / 4) + warp * kC;
-      const float2* ml = reinterpret_cast<const float2*>(reinterpret_cast<const uint8_t*>(p.ws) + ws.own_ml) + at;
-      for (int i = 0; i < parts; ++i) add(__ldcg(ml + i), [&](int c) { return __ldcg(o + (size_t)i * (D / 4) + c); });
+  {
+    const size_t at = ((size_t)step_tok * p.Hq + kvh * G + head) * ws.parts;
+    const float4* o = reinterpret_cast<const float4*>(reinterpret_cast<const uint8_t*>(p.ws) + ws.own) + at * (D / 4) + c0;
+    const float2* ml = reinterpret_cast<const float2*>(reinterpret_cast<const uint8_t*>(p.ws) + ws.own_ml) + at;
+    for (; at_warp < own_parts; at_warp += 8) {
+      float4 x[kC];
+      const float2 y = __ldcg(ml + at_warp);
+#pragma unroll
+      for (int c = 0; c < kC; ++c) x[c] = __ldcg(o + (size_t)at_warp * (D / 4) + c);
+      add(y, x);
     }
   }
-  const float inv = l == 0.f ? 0.f : (FP8 ? *p.v_scale : 1.f) / l;
+  s_ml[warp][lane] = make_float2(m, l);
+#pragma unroll
+  for (int c = 0; c < kC; ++c) s_o[warp][c][lane] = acc[c];
+  __syncthreads();
+  // warp w sums dims 4 w to 4 w + 3 of the 32 rows
+  float mx = -INFINITY;
+  float2 ml[8];
+#pragma unroll
+  for (int w = 0; w < 8; ++w) {
+    ml[w] = s_ml[w][lane];
+    if (ml[w].y != 0.f) mx = fmaxf(mx, ml[w].x);
+  }
+  const float base = mx == -INFINITY ? 0.f : mx;
+  float sum = 0.f;
+  float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+  for (int w = 0; w < 8; ++w) {
+    if (ml[w].y == 0.f) continue;
+    const float f = ml[w].x == -INFINITY ? 1.f : ex2(ml[w].x - base);
+    const float4 x = s_o[w][warp][lane];
+    sum += ml[w].y * f;
+    y.x += x.x * f; y.y += x.y * f; y.z += x.z * f; y.w += x.w * f;
+  }
+  if (!live) return;
+  const float inv = sum == 0.f ? 0.f : (FP8 ? *p.v_scale : 1.f) / sum;
   const size_t row = (size_t)tok * p.Hq + kvh * G + head;
-  uint32_t y[2 * kC];
-#pragma unroll
-  for (int c = 0; c < kC; ++c) {
-    y[2 * c] = pack2<false>(acc[c].x * inv, acc[c].y * inv);
-    y[2 * c + 1] = pack2<false>(acc[c].z * inv, acc[c].w * inv);
-  }
-  uint4* out = reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(p.out) + row * D + warp * (D / 8));
-#pragma unroll
-  for (int c = 0; c < kC / 2; ++c) out[c] = make_uint4(y[4 * c], y[4 * c + 1], y[4 * c + 2], y[4 * c + 3]);
-  if (p.lse && warp == 0) p.lse[row] = l == 0.f ? -INFINITY : ((m == -INFINITY ? 0.f : m) + log2f(l)) * 0.693147180559945f;
+  *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(p.out) + row * D + (c0 + warp) * 4) = make_uint2(pack2<false>(y.x * inv, y.y * inv), pack2<false>(y.z * inv, y.w * inv));
+  if (p.lse && warp == 0 && blockIdx.z == 0) p.lse[row] = sum == 0.f ? -INFINITY : (base + log2f(sum)) * 0.693147180559945f;
 }
 
 bool bad_shape(const MbSharedArgs& a) {
@@ -157,7 +191,7 @@ int run(const MbSharedArgs& a, const Ws& w, cudaStream_t stream) {
     if (a.max_ctx > 0)
       if (const int rc = mb_decode_parts(a, t, n, reinterpret_cast<float*>(ws + w.own), reinterpret_cast<float*>(ws + w.own_ml), w.parts, prefixes && t == 0, stream)) return rc;
     const long long blocks = ((long long)n * G + 31) / 32;
-    const cudaError_t e = mb::launch_kernel_ex(shared_join_kernel<D, FP8>, dim3((unsigned)blocks, a.Hkv), dim3(256), 0, stream, 1, mb_pdl_enabled() != 0, a, w, t, n);
+    const cudaError_t e = mb::launch_kernel_ex(shared_join_kernel<D, FP8>, dim3((unsigned)blocks, a.Hkv, D / kJoinDims), dim3(256), 0, stream, 1, mb_pdl_enabled() != 0, a, w, t, n);
     if (e != cudaSuccess) return (int)e;
   }
   return 0;
@@ -180,6 +214,11 @@ size_t mb_shared_attn_ws(int num_seqs, int q_len, int groups, int Hq, int Hkv, i
 
 int mb_shared_attn(const MbSharedArgs* a, cudaStream_t stream) {
   if (!a || bad_shape(*a)) return MB_ERR_BAD_ARG;
+  const long long G = a->Hq / a->Hkv, rows = (long long)a->num_seqs * a->q_len * G;
+  if (rows * a->Hkv > (1ll << 26)) return MB_ERR_TOO_LARGE;
+  // places of the line that prefixes are shared out along, at most (shared_plan.cuh)
+  const long long units = rows / 128 + (a->groups < a->num_seqs ? a->groups : a->num_seqs);
+  if (a->groups > 0 && (units + 1) * a->Hkv * (a->max_prefix / (a->D == 256 ? 64 : 128) + 1) >= (1ll << 31)) return MB_ERR_TOO_LARGE;
   const Ws w = workspace(*a);
   if (w.bytes > 0 && (!a->ws || a->ws_bytes < w.bytes)) return MB_ERR_TOO_LARGE;
   switch (a->D) {

@@ -46,7 +46,7 @@ struct MbMlaPromptArgs {
   const int* q_len;
   const int* ctx_len;
   const int* first;          // [seqs]: a sequence's first expanded row
-  const int* bad;            // [expanded rows / 128]: the place in its sequence of the first row that is no number, or 2^31 - 1
+  const int* bad;            // [expanded rows / 32]: the place in its sequence of the first row that is no number, or 2^31 - 1
   void* out;                 // [rows, H, 128] bf16
   uint32_t* status;
   long long q_rows, kv_rows;

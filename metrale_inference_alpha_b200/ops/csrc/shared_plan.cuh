@@ -17,13 +17,14 @@ template <int D>
 struct Shape {
   static constexpr bool kDouble = D <= 128;                // double units
   static constexpr int kT = kDouble ? 128 : 64;            // cached tokens of a tile
+  static constexpr int kLeast = 1;
 };
 
 // Groups of a call, in shared memory: first sequences (rising and inside the batch, whatever the caller's are), rows of the prefix, first place on the line
 struct Plan {
   int start[kMaxGroups + 1];
   int len[kMaxGroups];
-  long long base[kMaxGroups + 1];
+  int base[kMaxGroups + 1];
 };
 
 __device__ __forceinline__ int row_count(const MbSharedArgs& p, const Plan& s, int g) { return (s.start[g + 1] - s.start[g]) * p.q_len * (p.Hq / p.Hkv); }
@@ -41,10 +42,10 @@ __device__ __forceinline__ void unit_count(int rows, int& doubles, int& singles)
   }
 }
 template <int D>
-__device__ __forceinline__ long long line_of_head(int rows, int tiles) {
+__device__ __forceinline__ int line_of_head(int rows, int tiles) {
   int doubles, singles;
   unit_count<D>(rows, doubles, singles);
-  return (long long)tiles * (2 * doubles + singles);
+  return tiles * (2 * doubles + singles);                  // the launcher sees to it that a call's line has fewer than 2^31 places
 }
 
 // by one warp
@@ -70,26 +71,24 @@ __device__ __forceinline__ void make_plan(const MbSharedArgs& p, Plan& s, int la
     top = __shfl_sync(0xffffffffu, a, 31);
   }
   __syncwarp();
-  long long at = 0;
+  int at = 0;
   for (int g0 = 0; g0 < p.groups; g0 += 32) {
     const int g = g0 + lane;
-    long long n = 0;
+    int n = 0;
     if (g < p.groups) {
-      int len = 0;
-      if (s.start[g + 1] > s.start[g]) {
-        len = max(p.prefix_len[g], 0);
-        if (len > p.max_prefix) {
-          if (p.status) atomicCAS(p.status, 0u, MB_ST_BOUNDS);
-          len = p.max_prefix;
-        }
+      int len = max(p.prefix_len[g], 0);
+      if (s.start[g + 1] <= s.start[g]) len = 0;
+      if (len > p.max_prefix) {
+        if (p.status) atomicCAS(p.status, 0u, MB_ST_BOUNDS);
+        len = p.max_prefix;
       }
       s.len[g] = len;
       n = p.Hkv * line_of_head<D>(row_count(p, s, g), (len + Shape<D>::kT - 1) / Shape<D>::kT);
     }
-    long long x = n;
+    int x = n;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-      const long long y = __shfl_up_sync(0xffffffffu, x, d);
+      const int y = __shfl_up_sync(0xffffffffu, x, d);
       if (lane >= d) x += y;
     }
     if (g < p.groups) s.base[g] = at + x - n;
@@ -98,24 +97,30 @@ __device__ __forceinline__ void make_plan(const MbSharedArgs& p, Plan& s, int la
   if (lane == 0) s.base[p.groups] = at;
 }
 
-// first place of CTA c of `ctas`, and the CTA that has place x
-__device__ __forceinline__ long long place_of(int c, int ctas, long long W) { return c * W / ctas; }
-__device__ __forceinline__ int cta_of(long long x, int ctas, long long W) { return (int)(((x + 1) * ctas + W - 1) / W) - 1; }
+// The line's W places over `ctas`: the first place of CTA c, and the CTA that has place x
+struct Share {
+  int each, more;                          // CTAs in front of `more` have a place more
+  __device__ __forceinline__ Share(int W, int ctas) : each(W / ctas), more(W % ctas) {}
+  __device__ __forceinline__ int first(int c) const { return c * each + min(c, more); }
+  __device__ __forceinline__ int owner(int x) const { return x < more * (each + 1) ? x / (each + 1) : more + (x - more * (each + 1)) / each; }
+};
+// CTAs that take part: a part of a place or two would cost the join what it saves here
+template <int D>
+__device__ __forceinline__ int used_ctas(int W, int ctas) { return max(1, min(ctas, W / Shape<D>::kLeast)); }
 
 struct Part {
   int group, kvh, row0, rows, two;         // a unit: its first row in the group, its rows, whether it is a double one
   int t0, t1;                              // tiles of the part
 };
 // tiles [t0, t1) of a unit that begins at place `at` with `tiles` of them, which lie in places [b0, b1)
-__device__ __forceinline__ void tiles_in(long long at, int tiles, int two, long long b0, long long b1, int& t0, int& t1) {
-  const long long a = max(b0 - at, 0ll), b = min(max(b1 - at, 0ll), (long long)tiles << two);
-  t0 = (int)((a + two) >> two);
-  t1 = (int)((b + two) >> two);
+__device__ __forceinline__ void tiles_in(int at, int tiles, int two, int b0, int b1, int& t0, int& t1) {
+  t0 = (max(b0 - at, 0) + two) >> two;
+  t1 = (min(max(b1 - at, 0), tiles << two) + two) >> two;
 }
 
 // The part at `pos`, which moves behind it; false at the end. Parts without tiles are left out.
 template <int D>
-__device__ __forceinline__ bool next_part(const MbSharedArgs& p, const Plan& s, long long& pos, long long end, Part& x) {
+__device__ __forceinline__ bool next_part(const MbSharedArgs& p, const Plan& s, int& pos, int end, Part& x) {
   while (pos < end) {
     int lo = 0, hi = p.groups;             // base[lo] <= pos < base[hi]
     while (hi - lo > 1) {
@@ -127,24 +132,16 @@ __device__ __forceinline__ bool next_part(const MbSharedArgs& p, const Plan& s, 
     const int rows = row_count(p, s, lo), tiles = (s.len[lo] + Shape<D>::kT - 1) / Shape<D>::kT;
     int doubles, singles;
     unit_count<D>(rows, doubles, singles);
-    const long long head = (long long)tiles * (2 * doubles + singles), in = pos - s.base[lo];
-    x.kvh = (int)(in / head);
-    const long long w = in - x.kvh * head, d = 2ll * tiles * doubles;
-    long long at;
-    if (w < d) {
-      const int u = (int)(w / (2ll * tiles));
-      x.two = 1;
-      x.row0 = u * 256;
-      at = pos - (w - 2ll * tiles * u);
-    } else {
-      const int u = (int)((w - d) / tiles);
-      x.two = 0;
-      x.row0 = doubles * 256 + u * 128;
-      at = pos - (w - d - (long long)tiles * u);
-    }
+    const unsigned head = (unsigned)tiles * (2 * doubles + singles), in = pos - s.base[lo];
+    x.kvh = in / head;
+    const unsigned w = in - x.kvh * head, d = 2u * tiles * doubles;
+    x.two = w < d;
+    const unsigned size = (unsigned)tiles << x.two, v = x.two ? w : w - d, u = v / size;
+    x.row0 = x.two ? u * 256 : doubles * 256 + u * 128;
+    const int at = pos - (int)(v - u * size);
     x.rows = min(rows - x.row0, x.two ? 256 : 128);
     tiles_in(at, tiles, x.two, pos, end, x.t0, x.t1);
-    pos = min(end, at + ((long long)tiles << x.two));
+    pos = min(end, at + (int)size);
     if (x.t1 > x.t0) return true;
   }
   return false;

@@ -44,6 +44,30 @@ __device__ __forceinline__ Place place_rest(const MbSharedArgs& p, const Ws& w, 
   return {reinterpret_cast<float4*>(ws + w.rest) + i * (D / 4) * kRowTile, reinterpret_cast<float2*>(ws + w.rest_ml) + i * kRowTile, kRowTile};
 }
 
+// A unit's query rows, every `by`th from one on: one division in front
+struct QueryRow {
+  const __nv_bfloat16* q;
+  size_t ld;                               // heads of a token
+  int tok, head, G, by_tok, by_head, kvh;
+  __device__ __forceinline__ QueryRow(const MbSharedArgs& p, const Part& x, int G_, int tok0, int row, int by)
+      : q(reinterpret_cast<const __nv_bfloat16*>(p.q)), ld(p.Hq), G(G_), kvh(x.kvh) {
+    const int at = x.row0 + row, t = at / G;
+    tok = tok0 + t;
+    head = at - t * G;
+    by_tok = by / G;
+    by_head = by - by_tok * G;
+  }
+  __device__ __forceinline__ const __nv_bfloat16* row(int D) const { return q + (tok * ld + kvh * G + head) * D; }
+  __device__ __forceinline__ void step() {
+    tok += by_tok;
+    head += by_head;
+    if (head >= G) {
+      head -= G;
+      ++tok;
+    }
+  }
+};
+
 // Queries of row r0 + r of a unit, 16-byte piece c of D / 8; an e4m3 cache wants them in f16, scaled (`scale`: what scores are then too small by)
 template <int D, bool FP8>
 __device__ __forceinline__ uint4 query_piece(uint4 v, float& scale) {
@@ -72,7 +96,7 @@ __device__ __forceinline__ uint4 query_piece(uint4 v, float& scale) {
 
 // K and V tiles of kT cached tokens of this CTA's parts, one after the other, into two stages each: 128 threads, t the number of this one
 template <int D, bool FP8, int kT>
-__device__ __forceinline__ void load_tiles(const MbSharedArgs& p, const Plan& plan, long long begin, long long end, uint8_t* sK, uint8_t* sV, uint64_t* k_full,
+__device__ __forceinline__ void load_tiles(const MbSharedArgs& p, const Plan& plan, int begin, int end, uint8_t* sK, uint8_t* sV, uint64_t* k_full,
                                            uint64_t* k_empty, uint64_t* v_full, uint64_t* v_empty, int t) {
   constexpr int kTileB = kT * D * 2;
   const int lane = t & 31;
@@ -81,7 +105,7 @@ __device__ __forceinline__ void load_tiles(const MbSharedArgs& p, const Plan& pl
   const int r0 = t / kPieces, c = t % kPieces;
   const size_t row_bytes = (size_t)D * (FP8 ? 1 : 2), pitch = (size_t)p.Hkv * row_bytes;
   const int shift = (p.block_size & (p.block_size - 1)) == 0 ? 31 - __clz(p.block_size) : -1;
-  long long pos = begin;
+  int pos = begin;
   Part x;
   x.t0 = x.t1 = 0;
   int at = 0;                                           // the tile whose places are looked up next
@@ -257,8 +281,10 @@ __global__ void __launch_bounds__(512, 1) shared_prefix_kernel(const MbSharedArg
   mb::tc_fence_after();
   mb::pdl_launch_dependents();                            // behind this kernel's own wait: what the step before it wrote is there for them too
   const uint32_t tmem = s_tmem;                           // S0 0-127, S1 128-255, O0 256-, O1 384-
-  const long long W = plan.base[p.groups];
-  const long long begin = place_of(blockIdx.x, ws.ctas, W), end = place_of(blockIdx.x + 1, ws.ctas, W);
+  const int W = plan.base[p.groups], used = used_ctas<D>(W, ws.ctas);
+  const Share share(W, used);
+  const bool idle = (int)blockIdx.x >= used;
+  const int begin = idle ? 0 : share.first(blockIdx.x), end = idle ? 0 : share.first(blockIdx.x + 1);
 
   if (warp < 8) {
     // ------------------------------------------------------------ softmax
@@ -269,20 +295,20 @@ __global__ void __launch_bounds__(512, 1) shared_prefix_kernel(const MbSharedArg
     const float sc0 = p.scale * (FP8 ? *p.k_scale : 1.f) * 1.44269504088896f;
     uint32_t part = 0, done = 0, outs = 0;                // parts, tiles and outputs that this accumulator has had
     bool ok = true;
-    long long pos = begin;
+    int pos = begin;
     Part x;
     while (ok && next_part<D>(p, plan, pos, end, x)) {
       const int n = x.t1 - x.t0, mine = x.two ? n : (n + 1 - w) / 2;
-      const size_t row0 = (size_t)plan.start[x.group] * p.q_len * G + x.row0;      // of the kv head's rows
       if (x.two || w == 0) {
         // 128 rows x D / 8 pieces of 8 dims, a thread's loads in flight together (rows past the last one read it again and become zeros)
         constexpr int kPieces = D / 8, kQ = kPieces, kStep = 128 / kPieces;
         const int c = r % kPieces, first = r / kPieces, last = x.rows - w * 128 - 1;
         uint4 v[kQ];
+        QueryRow at(p, x, G, plan.start[x.group] * p.q_len, w * 128 + min(first, last), kStep);
 #pragma unroll
         for (int i = 0; i < kQ; ++i) {
-          const size_t at = row0 + w * 128 + min(first + kStep * i, last), tok = at / G;
-          v[i] = *(reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(p.q) + (tok * p.Hq + x.kvh * G + (at - tok * G)) * D) + c);
+          v[i] = *(reinterpret_cast<const uint4*>(at.row(D)) + c);
+          if (first + kStep * (i + 1) <= last) at.step();
         }
 #pragma unroll
         for (int i = 0; i < kQ; ++i) {
@@ -409,7 +435,7 @@ __global__ void __launch_bounds__(512, 1) shared_prefix_kernel(const MbSharedArg
       const uint32_t aQ = mb::smem_u32(sQ), aK = mb::smem_u32(sK), aV = mb::smem_u32(sV);
       uint32_t part = 0, base = 0, done[2] = {0, 0};      // parts, tiles brought, tiles that either accumulator has had
       bool ok = true;
-      long long pos = begin;
+      int pos = begin;
       Part x;
       while (ok && next_part<D>(p, plan, pos, end, x)) {
         const int n = x.t1 - x.t0, n0 = x.two ? n : (n + 1) / 2, n1 = x.two ? n : n / 2;
@@ -507,8 +533,10 @@ __global__ void __launch_bounds__(288, 1) shared_prefix256_kernel(const MbShared
   mb::tc_fence_after();
   mb::pdl_launch_dependents();
   const uint32_t tmem = s_tmem;                           // S0 0-63, S1 64-127, O 256-511
-  const long long W = plan.base[p.groups];
-  const long long begin = place_of(blockIdx.x, ws.ctas, W), end = place_of(blockIdx.x + 1, ws.ctas, W);
+  const int W = plan.base[p.groups], used = used_ctas<D>(W, ws.ctas);
+  const Share share(W, used);
+  const bool idle = (int)blockIdx.x >= used;
+  const int begin = idle ? 0 : share.first(blockIdx.x), end = idle ? 0 : share.first(blockIdx.x + 1);
 
   if (warp < 4) {
     // ------------------------------------------------------------ softmax
@@ -517,19 +545,19 @@ __global__ void __launch_bounds__(288, 1) shared_prefix256_kernel(const MbShared
     const float sc0 = p.scale * (FP8 ? *p.k_scale : 1.f) * 1.44269504088896f;
     uint32_t part = 0, base = 0;                          // parts, tiles that are done
     bool ok = true;
-    long long pos = begin;
+    int pos = begin;
     Part x;
     while (ok && next_part<D>(p, plan, pos, end, x)) {
       const int n = x.t1 - x.t0, last = x.rows - 1;
-      const size_t row0 = (size_t)plan.start[x.group] * p.q_len * G + x.row0;
       // 128 rows x 32 pieces of 8 dims, sixteen of a thread's loads in flight together (rows past the last one are zeros)
 #pragma unroll 1
       for (int half = 0; half < 2; ++half) {
         uint4 v[16];
+        QueryRow at(p, x, G, plan.start[x.group] * p.q_len, min(warp + 64 * half, last), 4);
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const size_t at = row0 + min(warp + 4 * (half * 16 + i), last), tok = at / G;
-          v[i] = *(reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(p.q) + (tok * p.Hq + x.kvh * G + (at - tok * G)) * D) + lane);
+          v[i] = *(reinterpret_cast<const uint4*>(at.row(D)) + lane);
+          if (warp + 4 * (half * 16 + i + 1) <= last) at.step();
         }
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
@@ -644,7 +672,7 @@ __global__ void __launch_bounds__(288, 1) shared_prefix256_kernel(const MbShared
       const uint32_t aQ = mb::smem_u32(sQ), aK = mb::smem_u32(sK), aV = mb::smem_u32(sV);
       uint32_t part = 0, base = 0;
       bool ok = true;
-      long long pos = begin;
+      int pos = begin;
       Part x;
       auto scores = [&](uint32_t j) {
         if (!mb::mbar_wait(&k_full[j & 1], (j >> 1) & 1, p.status, MB_ST_TIMEOUT_MMA)) return false;

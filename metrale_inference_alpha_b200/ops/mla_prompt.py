@@ -88,7 +88,7 @@ def mla_prompt_attention(q: torch.Tensor, cache: torch.Tensor, block_table: torc
         return torch.zeros(T, H, VALUE, dtype=torch.bfloat16, device=dev)
     out = torch.empty(T, H, VALUE, dtype=torch.bfloat16, device=dev)
     L, rt = _library(), runtime(dev)
-    lat, first = torch.empty(rows, ROW, dtype=torch.bfloat16, device=dev), torch.empty(S + rows // 128, dtype=torch.int32, device=dev)
+    lat, first = torch.empty(rows, ROW, dtype=torch.bfloat16, device=dev), torch.empty(S + rows // 32, dtype=torch.int32, device=dev)
     bad, status, stream = first.data_ptr() + 4 * S, rt.status.data_ptr(), _stream()
     _native.check(L.mb_mla_gather(cache.data_ptr(), block_table.data_ptr(), block_table.stride(0), ctx_len.data_ptr(), lat.data_ptr(), first.data_ptr(), bad, status,
                                   nb, rows, S, bs, max_ctx, stream), "mla_gather")
@@ -99,8 +99,8 @@ def mla_prompt_attention(q: torch.Tensor, cache: torch.Tensor, block_table: torc
     for h in range(0, H, each):
         n = min(each, H - h)
         part = kv.view(-1)[:rows * n * KV].view(rows, n * KV)
-        # one split: the shared workspace of split sums stays out of it
-        linear(act, QuantWeight("bf16", n * KV, LATENT, w_kv[h:h + n].view(n * KV, LATENT)), out=part, force_splits=1)
+        # without splits, which have a workspace that all launches share: more than 256 rows have none of this depth
+        linear(act, QuantWeight("bf16", n * KV, LATENT, w_kv[h:h + n].view(n * KV, LATENT)), out=part, force_splits=int(rows <= 256))
         a = _ARGS.pack(q.data_ptr(), part.data_ptr(), lat.data_ptr(), q_start.data_ptr(), q_len.data_ptr(), ctx_len.data_ptr(), first.data_ptr(), bad, out.data_ptr(),
                        status, T, rows, S, H, h, n, max_q_len, max_ctx, scale)
         _native.check(L.mb_mla_prompt(a, stream), "mla_prompt")
