@@ -2,7 +2,7 @@
 // as usual. Per head and pair 192 + 128 multiply-adds instead of the 576 + 512 of the absorbed form, for 512 x 256 a cached row and head in front.
 #include "common.cuh"
 #include "shared_attn.h"
-#include "attention_rows.cuh"
+#include "softmax_rows.cuh"
 #include "smem_limit.h"
 #include "tensormap.h"
 
@@ -113,12 +113,15 @@ __global__ void __launch_bounds__(256) gather_kernel(const GatherParams p) {
   }
 }
 
-// ---- attention: two tiles of 128 query tokens of one head a CTA in turn on the tensor cores, as in attention_rows.cu
-//   warps 0-3, 4-7   softmax of row tile 0 / 1, thread = row: S from TMEM, P back to TMEM (over S), the output row at the end
+// ---- attention: two tiles of 128 query tokens of one head a CTA on the tensor cores
+//   warps 0-3, 4-7   softmax of row tile 0 / 1, thread = row: S from TMEM, the weights back to TMEM (over S) in two halves of 64 tokens
 //   warp 8           copies by TMA: Q once; per 128 cached tokens five pieces of 16 KB in a ring of eight: K in three spans of 64 dims (the
 //                    third is the rotated part, which all heads share), V in two halves of 64 tokens
-//   warp 9           issues the products: S0 S1 | PV0 S0' PV1 S1' | ... so that one tile's softmax runs under the other tile's products
+//   warp 9           issues the products: S0 S1 | PV0 S0' PV1 S1' | ..., so that one tile's softmax runs under the other tile's products. With a warp for
+//                    either tile's the two batches were interleaved and done at the same time, and both softmaxes then ran at once (325 us instead of 300)
 //   warps 10, 11     give their registers to the softmax
+// Weights through shared memory, which would let S of the next tile be made under the softmax, were slower (331 us instead of 314 for 8192 tokens of 16 heads):
+// 128 x 128 products of operands in shared memory read 128 bytes a cycle, all that it has.
 constexpr int kT = 128, kPiece = 16384, kRing = 8, kPer = 5, kThreads = 384;
 constexpr int kQTile = 3 * kPiece;
 constexpr int kSmem = 2 * kQTile + kRing * kPiece + 1024;
@@ -135,7 +138,7 @@ mla_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   extern __shared__ __align__(16) uint8_t smem_raw[];
   uint8_t* sQ = smem_raw + ((1024u - (mb::smem_u32(smem_raw) & 1023u)) & 1023u);   // 2 row tiles x 3 spans x [128 rows x 128 B]
   uint8_t* sR = sQ + 2 * kQTile;
-  __shared__ __align__(8) uint64_t q_full, full[kRing], empty[kRing], s_full[2], p_full[2], o_full[2];
+  __shared__ __align__(8) uint64_t q_full, full[kRing], empty[kRing], s_full[2], p_full[2][2], o_full[2];
   __shared__ uint32_t s_tmem;
   const int h = blockIdx.x, seq = blockIdx.z, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   mb::pdl_wait();
@@ -162,7 +165,8 @@ mla_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     }
     for (int i = 0; i < 2; ++i) {
       mb::mbar_init(&s_full[i], 1);
-      mb::mbar_init(&p_full[i], 4);
+      mb::mbar_init(&p_full[i][0], 4);
+      mb::mbar_init(&p_full[i][1], 4);
       mb::mbar_init(&o_full[i], 1);
     }
     mb::mbar_fence_init();
@@ -195,22 +199,13 @@ mla_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       for (int c = 0; c < kT; c += 32) mb::tmem_ld32_async(tS + c, s + c);
       mb::tmem_ld_wait(s);
       const int seen = limit - j * kT;                    // columns below this are visible
-      if (!__all_sync(0xffffffffu, seen >= kT)) {
+      const bool masked = !__all_sync(0xffffffffu, seen >= kT);
+      if (masked) {
 #pragma unroll
         for (int i = 0; i < kT; ++i)
           if (i >= seen) s[i] = -INFINITY;
       }
-      float mx4[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-      for (int i = 4; i < kT; ++i) mx4[i & 3] = fmaxf(mx4[i & 3], s[i]);
-      const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * sc;
-      float alpha = 1.f;
-      const bool move = mx > m_run + 8.f;                 // also true on a row's first finite tile
-      if (move) {
-        alpha = ex2(m_run - mx);                          // 0 when the row had seen nothing yet
-        m_run = mx;
-      }
-      if (j > 0 && __any_sync(0xffffffffu, move)) {
+      auto rescale = [&](float alpha) {                   // S seen: the products that were issued in front of it are done
 #pragma unroll
         for (int c = 0; c < kV; c += 16) {
           float ov[16];
@@ -219,28 +214,15 @@ mla_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           for (int i = 0; i < 16; ++i) ov[i] *= alpha;
           mb::tmem_st16(tO + c, ov);
         }
-      }
-      const float nm = m_run == -INFINITY ? 0.f : -m_run;
-      const float2 sc2 = make_float2(sc, sc), nm2 = make_float2(nm, nm);
-      float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        uint32_t pk[32];
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          float2 t = fma2(make_float2(s[q * 64 + 2 * i], s[q * 64 + 2 * i + 1]), sc2, nm2);
-          t.x = ex2(t.x);
-          t.y = ex2(t.y);
-          sum[i & 1] = add2(sum[i & 1], t);
-          pk[i] = pack2<false>(t.x, t.y);
-        }
+      };
+      auto publish = [&](int q, const uint32_t (&pk)[32]) {
         tmem_st32(tS + q * 32, pk);
-      }
-      mb::tmem_st_wait();
-      mb::tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mb::mbar_arrive(&p_full[w]);
-      l_run = l_run * alpha + ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y));
+        mb::tmem_st_wait();
+        mb::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mb::mbar_arrive(&p_full[w][q]);
+      };
+      softmax_tile<false, 0>(s, sc, 0.f, j == 0, masked, m_run, l_run, rescale, publish);
     }
     // the first cached token that is no number, of those that the tile sees: it lies in the expanded rows as zeros
     int bad = 0x7fffffff;
@@ -287,27 +269,28 @@ mla_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       int slot = 0, i = 0;
       uint32_t parity = 1;
       bool ok = true;
-      for (int j = 0; j < n && ok; ++j) {
+      auto bring = [&](int j, int c) {                    // piece c of tile j
+        if (!ok) return;
+        ok = mb::mbar_wait(&empty[slot], parity, p.status, MB_ST_TIMEOUT_TMA);
+        if (!ok) return;
         const int at = (int)first + j * kT;
-        for (int c = 0; c < kPer; ++c) {
-          ok = mb::mbar_wait(&empty[slot], parity, p.status, MB_ST_TIMEOUT_TMA);
-          if (!ok) break;
-          uint8_t* dst = sR + slot * kPiece;
-          mb::mbar_expect_tx(&full[slot], kPiece);
-          if (c < 2) {
-            mb::tma_load_2d(dst, &tmK, &full[slot], hk + c * 64, at);
-          } else if (c == 2) {
-            mb::tma_load_2d(dst, &tmR, &full[slot], kLat, at);
-          } else {
-            for (int d = 0; d < 2; ++d) mb::tma_load_2d(dst + d * (kPiece / 2), &tmV, &full[slot], hk + kNope + d * 64, at + (c - 3) * 64);
-          }
-          ++i;
-          if (++slot == kRing) {
-            slot = 0;
-            parity ^= 1;
-          }
+        uint8_t* dst = sR + slot * kPiece;
+        mb::mbar_expect_tx(&full[slot], kPiece);
+        if (c < 2) {
+          mb::tma_load_2d(dst, &tmK, &full[slot], hk + c * 64, at);
+        } else if (c == 2) {
+          mb::tma_load_2d(dst, &tmR, &full[slot], kLat, at);
+        } else {
+          for (int d = 0; d < 2; ++d) mb::tma_load_2d(dst + d * (kPiece / 2), &tmV, &full[slot], hk + kNope + d * 64, at + (c - 3) * 64);
         }
-      }
+        ++i;
+        if (++slot == kRing) {
+          slot = 0;
+          parity ^= 1;
+        }
+      };
+      for (int j = 0; j < n && ok; ++j)
+        for (int c = 0; c < kPer; ++c) bring(j, c);
       // given up: no copy may still be under way when the CTA ends
       if (!ok) {
         mb::mbar_wait(&q_full, 0, p.status, MB_ST_TIMEOUT_TMA);
@@ -317,38 +300,42 @@ mla_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     if (warp == 9 && mb::elect_one() && n > 0) {
       // ---------------------------------------------------------- products
       constexpr uint32_t kIdS = mb::umma_idesc(1, 1, 128, kT), kIdO = mb::umma_idesc(1, 1, 128, kV, 0, 1);
-      const uint32_t aQ = mb::smem_u32(sQ), aR = mb::smem_u32(sR);
+      // descriptors count 16 bytes: an operand's next step is an addition
+      const uint64_t dQ = mb::umma_desc_sw128(mb::smem_u32(sQ)), dK = mb::umma_desc_sw128(mb::smem_u32(sR)),
+                     dV = mb::umma_desc_sw128_mn(mb::smem_u32(sR), kPiece / 2, 1024);
       auto there = [&](int i) { return mb::mbar_wait(&full[i % kRing], (i / kRing) & 1, p.status, MB_ST_TIMEOUT_MMA); };
-      auto release = [&](int i) { mb::tc_commit(&empty[i % kRing]); };
       auto scores = [&](int w, int j) {
-        for (int c = 0; c < 3; ++c) {
-          if (!there(j * kPer + c)) return false;
-          mb::tc_fence_after();
 #pragma unroll
-          for (int s = 0; s < 4; ++s)
-            mb::umma_f16(tmem + w * 128, mb::umma_desc_sw128(aQ + w * kQTile + c * kPiece + s * 32),
-                         mb::umma_desc_sw128(aR + (j * kPer + c) % kRing * kPiece + s * 32), kIdS, (c | s) != 0);
+        for (int c = 0; c < 3; ++c) {
+          const int i = j * kPer + c;
+          if (!there(i)) return false;
+          mb::tc_fence_after();
+          const uint64_t q = dQ + w * (kQTile >> 4) + ((c * kPiece) >> 4), k = dK + (i % kRing) * (kPiece >> 4);
+#pragma unroll
+          for (int s = 0; s < 4; ++s) mb::umma_f16(tmem + w * 128, q + ((s * 32) >> 4), k + ((s * 32) >> 4), kIdS, (c | s) != 0);
         }
         mb::tc_commit(&s_full[w]);
         return true;
       };
       auto values = [&](int w, int j) {
-        if (!mb::mbar_wait(&p_full[w], j & 1, p.status, MB_ST_TIMEOUT_MMA)) return false;
-        for (int c = 0; c < 2; ++c) {
-          if (!there(j * kPer + 3 + c)) return false;
-          mb::tc_fence_after();
 #pragma unroll
-          for (int s = 0; s < 4; ++s)
-            umma_f16_ta(tmem + 256 + w * 128, tmem + w * 128 + (c * 4 + s) * 8,
-                        mb::umma_desc_sw128_mn(aR + (j * kPer + 3 + c) % kRing * kPiece + s * 2048, kPiece / 2, 1024), kIdO, (j | c | s) != 0);
+        for (int h = 0; h < 2; ++h) {
+          const int i = j * kPer + 3 + h;
+          if (!there(i) || !mb::mbar_wait(&p_full[w][h], j & 1, p.status, MB_ST_TIMEOUT_MMA)) return false;
+          mb::tc_fence_after();
+          const uint64_t v = dV + (i % kRing) * (kPiece >> 4);
+#pragma unroll
+          for (int s = 0; s < 4; ++s) umma_f16_ta(tmem + 256 + w * 128, tmem + w * 128 + (h * 4 + s) * 8, v + ((s * 2048) >> 4), kIdO, (j | h | s) != 0);
         }
         return true;
+      };
+      auto release = [&](int i, int k) {
+        for (; k > 0; --k, ++i) mb::tc_commit(&empty[i % kRing]);
       };
       bool ok = mb::mbar_wait(&q_full, 0, p.status, MB_ST_TIMEOUT_MMA);
       if (ok && n0 > 0) ok = scores(0, 0);
       if (ok && n1 > 0) ok = scores(1, 0);
-      if (ok)
-        for (int c = 0; c < 3; ++c) release(c);
+      if (ok) release(0, 3);
       for (int j = 0; j < n && ok; ++j) {
         if (j < n0) {
           ok = values(0, j);
@@ -357,16 +344,13 @@ mla_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           else mb::tc_commit(&o_full[0]);
           if (!ok) break;
         }
-        if (j < n1) {
-          ok = values(1, j);
-          if (!ok) break;
-        }
-        for (int c = 3; c < kPer; ++c) release(j * kPer + c);
+        if (j < n1) ok = values(1, j);
+        if (!ok) break;
+        release(j * kPer + 3, 2);
         if (j + 1 < n1) ok = scores(1, j + 1);
         else if (j + 1 == n1) mb::tc_commit(&o_full[1]);
         if (!ok) break;
-        if (j + 1 < n)
-          for (int c = 0; c < 3; ++c) release((j + 1) * kPer + c);
+        if (j + 1 < n) release((j + 1) * kPer, 3);
       }
     }
     __syncwarp();

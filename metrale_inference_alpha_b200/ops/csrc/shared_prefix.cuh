@@ -3,17 +3,21 @@
 //
 // As in attention_rows.cu the rows are tokens x heads of a group, 128 a tile, products on the tensor cores with S, P and O in TMEM, and two tiles in
 // turn, so that the softmax of one runs under the products of the other. Behind a prefix few rows are the rule: where a unit has one tile of rows (up to
-// 128), both accumulators take the cached tiles of this one in turn. Roles (512 threads, one CTA an SM, registers moved with setmaxnreg):
+// 128), both accumulators take the cached tiles of this one in turn. Roles (one CTA an SM, registers moved with setmaxnreg):
 //   warps 0-3, 4-7   softmax of accumulator 0 / 1, thread = row; they load their rows' queries and write their outputs
-//   warps 8-11       K and V tiles of 128 cached tokens into two stages, an e4m3 cache as f16 (exact), a bf16 cache by asynchronous copies
-//   warp 12          the products
-// The loading warps and the products run on from part to part; queries wait for the products of the part in front of theirs only.
+//   warps 8, 10, 11  copies by TMA, a box of up to 16 cached rows each (as many as lie in one block): a bf16 cache into a ring of pieces as
+//                    the products take them, an e4m3 cache as stored into a ring of its own; piece by piece in turn, since a warp needs some 90 cycles a box
+//   warp 9           the products
+//   warps 12-15      (e4m3 cache) make f16 pieces of what was copied: exact, one conversion per two values
+// A piece is 16 KB: 64 dims of 128 keys, or 64 values of 128 dims. All roles run on from part to part; queries wait for the products of the part in front
+// of theirs only.
 // With an e4m3 cache a row's queries are scaled by the power of two that takes their largest to [2^14, 2^15) and weights are held 2^7 larger, as
 // there: neither then loses the range that bf16 gives.
 #pragma once
-#include "attention_rows.cuh"
+#include "softmax_rows.cuh"
 #include "shared_plan.cuh"
 #include "smem_limit.h"
+#include "tensormap.h"
 
 namespace mbs {
 
@@ -239,43 +243,81 @@ __device__ __forceinline__ void load_tiles(const MbSharedArgs& p, const Plan& pl
   if (bad && p.status) atomicCAS(p.status, 0u, MB_ST_BOUNDS);
 }
 
-template <int D, bool FP8>
-struct PrefixCfg {
-  static constexpr int kT = 128, kThreads = 512;
-  static constexpr int kQB = 128 * D * 2, kTileB = kT * D * 2;
-  static constexpr int kSmem = 2 * kQB + 4 * kTileB + 1024 + (int)sizeof(Plan);
+// How cached rows are copied: boxes of 16 >> bits rows, the largest that every block is a multiple of
+struct Boxes {
+  int bits;
 };
 
 template <int D, bool FP8>
-__global__ void __launch_bounds__(512, 1) shared_prefix_kernel(const MbSharedArgs p, const Ws ws) {
+struct PrefixCfg {
+  static constexpr int kT = 128, kThreads = FP8 ? 512 : 384;
+  static constexpr int kQB = 128 * D * 2, kPiece = 16384, kSpans = D / 64;
+  static constexpr int kPer = 2 * kSpans;                 // pieces of a tile: K in spans, V in as many runs of tokens
+  static constexpr int kVTok = kT / kSpans;               // tokens of a V piece
+  static constexpr int kRing = FP8 ? 6 : 9;
+  static constexpr int kRawB = 8192, kRawTok = kRawB / D, kRawRing = FP8 ? 6 : 0;       // pieces as stored: tokens of all dims
+  static constexpr int kRawPer = 2 * kT / kRawTok;
+  static constexpr int kSmem = 2 * kQB + kRing * kPiece + kRawRing * kRawB + 1024 + (int)sizeof(Plan);
+};
+
+// Places in a ring
+template <int N>
+struct Cursor {
+  int slot = 0;
+  uint32_t parity = 0;
+  __device__ __forceinline__ void step() {
+    if (++slot == N) {
+      slot = 0;
+      parity ^= 1;
+    }
+  }
+  __device__ __forceinline__ void step(int n) {
+    slot += n;
+    if (slot >= N) {
+      slot -= N;
+      parity ^= 1;
+    }
+  }
+};
+
+template <int D, bool FP8>
+__global__ void __launch_bounds__(PrefixCfg<D, FP8>::kThreads, 1)
+shared_prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmK1,
+                     const __grid_constant__ CUtensorMap tmV1, const Boxes boxes, const MbSharedArgs p, const Ws ws) {
   using C = PrefixCfg<D, FP8>;
-  constexpr int kT = C::kT, kQB = C::kQB, kTileB = C::kTileB, kSpans = D / 64;
+  constexpr int kT = C::kT, kQB = C::kQB, kPiece = C::kPiece, kSpans = C::kSpans, kRing = C::kRing, kRaw = FP8 ? C::kRawRing : 1;
   extern __shared__ __align__(16) uint8_t smem_raw[];
   uint8_t* sQ = smem_raw + ((1024u - (mb::smem_u32(smem_raw) & 1023u)) & 1023u);   // 2 row tiles x spans of 64 dims x [128 rows x 128 B]
-  uint8_t* sK = sQ + 2 * kQB;                             // 2 stages x spans x [128 tokens x 128 B]
-  uint8_t* sV = sK + 2 * kTileB;
-  Plan& plan = *reinterpret_cast<Plan*>(sV + 2 * kTileB);
-  __shared__ __align__(8) uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2];
+  uint8_t* sR = sQ + 2 * kQB;                             // ring of pieces
+  uint8_t* sB = sR + kRing * kPiece;                      // ring of pieces as stored
+  Plan& plan = *reinterpret_cast<Plan*>(sB + C::kRawRing * C::kRawB);
+  __shared__ __align__(8) uint64_t q_full[2], q_free, full[kRing], empty[kRing], raw_full[kRaw], raw_empty[kRaw], s_full[2], p_full[2][2], o_full[2];
   __shared__ uint32_t s_tmem;
-  __shared__ float s_qscale[2][2][128];                   // what a row's scores are too large by (e4m3 cache), of parts in turn
+  __shared__ float s_qscale[FP8 ? 2 : 1][2][128];         // what a row's scores are too large by (e4m3 cache), of parts in turn
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = p.Hq / p.Hkv;
   mb::pdl_wait();
   if (warp == 0) {
     make_plan<D>(p, plan, lane);
   } else if (warp == 1 && lane == 0) {
+    mb::mbar_init(&q_free, 1);
     for (int i = 0; i < 2; ++i) {
       mb::mbar_init(&q_full[i], 4);
-      mb::mbar_init(&k_full[i], 4);
-      mb::mbar_init(&v_full[i], 4);
-      mb::mbar_init(&k_empty[i], 1);
-      mb::mbar_init(&v_empty[i], 1);
       mb::mbar_init(&s_full[i], 1);
-      mb::mbar_init(&p_full[i], 4);
+      mb::mbar_init(&p_full[i][0], 4);
+      mb::mbar_init(&p_full[i][1], 4);
       mb::mbar_init(&o_full[i], 1);
+    }
+    for (int i = 0; i < kRing; ++i) {
+      mb::mbar_init(&full[i], FP8 ? 4 : 1);
+      mb::mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < kRaw; ++i) {
+      mb::mbar_init(&raw_full[i], 1);
+      mb::mbar_init(&raw_empty[i], 4);
     }
     mb::mbar_fence_init();
   }
-  if (warp == 12) mb::tmem_alloc(&s_tmem, 512);
+  if (warp == 9) mb::tmem_alloc(&s_tmem, 512);
   mb::tc_fence_before();
   __syncthreads();
   mb::tc_fence_after();
@@ -285,20 +327,25 @@ __global__ void __launch_bounds__(512, 1) shared_prefix_kernel(const MbSharedArg
   const Share share(W, used);
   const bool idle = (int)blockIdx.x >= used;
   const int begin = idle ? 0 : share.first(blockIdx.x), end = idle ? 0 : share.first(blockIdx.x + 1);
+  int pos = begin;
+  Part x;
 
   if (warp < 8) {
     // ------------------------------------------------------------ softmax
-    more_regs<184>();
+    if constexpr (FP8) more_regs<184>();                  // 184 + 184 + 72 + 72 are the 4 x 128 of the launch
+    else more_regs<216>();                                // 216 + 216 + 72 are the 3 x 168
     const int w = warp >> 2, r = tid & 127;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t tS = tmem + lanes + w * 128, tO = tmem + lanes + 256 + w * 128;
     const float sc0 = p.scale * (FP8 ? *p.k_scale : 1.f) * 1.44269504088896f;
     uint32_t part = 0, done = 0, outs = 0;                // parts, tiles and outputs that this accumulator has had
     bool ok = true;
-    int pos = begin;
-    Part x;
     while (ok && next_part<D>(p, plan, pos, end, x)) {
       const int n = x.t1 - x.t0, mine = x.two ? n : (n + 1 - w) / 2;
+      // a wait tells a phase from its neighbours only: no warp may be two parts ahead of one that waits, so every part's queries wait for all products
+      // of the former one's
+      if (part > 0) ok = mb::mbar_wait(&q_free, (part - 1) & 1, p.status, MB_ST_TIMEOUT_MMA);
+      if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
       if (x.two || w == 0) {
         // 128 rows x D / 8 pieces of 8 dims, a thread's loads in flight together (rows past the last one read it again and become zeros)
         constexpr int kPieces = D / 8, kQ = kPieces, kStep = 128 / kPieces;
@@ -321,8 +368,7 @@ __global__ void __launch_bounds__(512, 1) shared_prefix_kernel(const MbSharedArg
         }
         fence_async_smem();
       }
-      // A wait tells a phase from its neighbours only, so no warp may be a part ahead of one that waits: where the rows are those of the other
-      // accumulator, their arrival is seen before this one's is announced, which the products and with them the next part wait for
+      // where the rows are those of the other accumulator, their arrival is seen before this one's is announced
       const int side = x.two ? w : 0;                     // whose rows these are
       if (side != w) {
         ok = mb::mbar_wait(&q_full[side], part & 1, p.status, MB_ST_TIMEOUT_MMA);
@@ -340,71 +386,55 @@ __global__ void __launch_bounds__(512, 1) shared_prefix_kernel(const MbSharedArg
       const bool live = r < left, some = (warp & 3) * 32 < left;
       const int len = plan.len[x.group];
       float m_run = -INFINITY, l_run = 0.f;
+      auto rescale = [&](float alpha) {                   // S seen: the products that were issued in front of it are done
+#pragma unroll
+        for (int c = 0; c < D; c += 16) {
+          float ov[16];
+          mb::tmem_ld16(tO + c, ov);
+#pragma unroll
+          for (int k = 0; k < 16; ++k) ov[k] *= alpha;
+          mb::tmem_st16(tO + c, ov);
+        }
+      };
+      auto announce = [&](int h) {
+        mb::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mb::mbar_arrive(&p_full[w][h]);
+      };
+      auto publish = [&](int h, const uint32_t (&pk)[32]) {
+        tmem_st32(tS + h * 32, pk);
+        mb::tmem_st_wait();
+        announce(h);
+      };
       for (int i = 0; i < mine; ++i) {
         const int t = x.t0 + (x.two ? i : 2 * i + w);
         ok = mb::mbar_wait(&s_full[w], (done + i) & 1, p.status, MB_ST_TIMEOUT_MMA);
         if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
         mb::tc_fence_after();
-        if (some) {                                       // warps without rows hand on what the columns hold: it meets no other row
-          float s[kT];
-#pragma unroll
-          for (int c = 0; c < kT; c += 32) mb::tmem_ld32_async(tS + c, s + c);
-          mb::tmem_ld_wait(s);
-          const int seen = len - t * kT;                  // columns below this are cached tokens
-          if (seen < kT) {
-#pragma unroll
-            for (int k = 0; k < kT; ++k)
-              if (k >= seen) s[k] = -INFINITY;
-          }
-          float mx4[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-          for (int k = 4; k < kT; ++k) mx4[k & 3] = fmaxf(mx4[k & 3], s[k]);
-          const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * sc;
-          float alpha = 1.f;
-          const bool move = mx > m_run + 8.f;             // also true on a row's first finite tile
-          if (move) {
-            alpha = ex2(m_run - mx);                      // 0 when the row had seen nothing yet
-            m_run = mx;
-          }
-          if (i > 0 && __any_sync(0xffffffffu, move)) {
-#pragma unroll
-            for (int c = 0; c < D; c += 16) {
-              float ov[16];
-              mb::tmem_ld16(tO + c, ov);
-#pragma unroll
-              for (int k = 0; k < 16; ++k) ov[k] *= alpha;
-              mb::tmem_st16(tO + c, ov);
-            }
-          }
-          const float nm = m_run == -INFINITY ? 0.f : (FP8 ? kLift : 0.f) - m_run;
-          const float2 sc2 = make_float2(sc, sc), nm2 = make_float2(nm, nm);
-          float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint32_t pk[32];
-#pragma unroll
-            for (int k = 0; k < 32; ++k) {
-              float2 e = fma2(make_float2(s[h * 64 + 2 * k], s[h * 64 + 2 * k + 1]), sc2, nm2);
-              e.x = ex2(e.x);
-              e.y = ex2(e.y);
-              sum[k & 1] = add2(sum[k & 1], e);
-              pk[k] = pack2<FP8>(e.x, e.y);
-            }
-            tmem_st32(tS + h * 32, pk);
-          }
-          mb::tmem_st_wait();
-          l_run = l_run * alpha + ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y));
+        if (!some) {                                      // warps without rows hand on what the columns hold: it meets no other row
+          announce(0);
+          announce(1);
+          continue;
         }
-        mb::tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mb::mbar_arrive(&p_full[w]);
+        float s[kT];
+#pragma unroll
+        for (int c = 0; c < kT; c += 32) mb::tmem_ld32_async(tS + c, s + c);
+        mb::tmem_ld_wait(s);
+        const int seen = len - t * kT;                    // columns below this are cached tokens
+        if (seen < kT) {
+#pragma unroll
+          for (int k = 0; k < kT; ++k)
+            if (k >= seen) s[k] = -INFINITY;
+        }
+        softmax_tile<FP8, 5>(s, sc, FP8 ? kLift : 0.f, i == 0, seen < kT, m_run, l_run, rescale, publish);
       }
       if (!ok) break;
-      // without a tile of its own an accumulator waits for the other's outputs, which every part has: its rows are announced a part at a time
-      ok = mine > 0 ? mb::mbar_wait(&o_full[w], outs & 1, p.status, MB_ST_TIMEOUT_MMA) : mb::mbar_wait(&o_full[0], part & 1, p.status, MB_ST_TIMEOUT_MMA);
-      if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-      mb::tc_fence_after();
-      outs += mine > 0;
+      if (mine > 0) {
+        ok = mb::mbar_wait(&o_full[w], outs & 1, p.status, MB_ST_TIMEOUT_MMA);
+        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+        mb::tc_fence_after();
+        ++outs;
+      }
       const Place to = x.t0 == 0 ? place_first<D>(p, ws, plan, x.group, x.kvh, x.row0 + (x.two ? w * 128 : 0), x.two ? 0 : w) : place_rest<D>(p, ws, blockIdx.x, w);
       if (mine > 0 && some) {
 #pragma unroll 1
@@ -422,75 +452,258 @@ __global__ void __launch_bounds__(512, 1) shared_prefix_kernel(const MbSharedArg
       done += mine;
       ++part;
     }
-  } else if (warp < 12) {
-    // ------------------------------------------------------------ loader
-    fewer_regs<96>();
-    load_tiles<D, FP8, kT>(p, plan, begin, end, sK, sV, k_full, k_empty, v_full, v_empty, tid - 256);
   } else {
-    fewer_regs<48>();
-    if (warp == 12 && mb::elect_one()) {
+    fewer_regs<72>();
+    if (warp < 12 && warp != 9) {
+      // ---------------------------------------------------------- copies
+      const int bits = boxes.bits, box = 16 >> bits, count = kT / box;       // rows of a box, boxes of a tile
+      constexpr int kMost = 4;                                               // of a lane: 128 boxes of one row
+      const int shift = (p.block_size & (p.block_size - 1)) == 0 ? 31 - __clz(p.block_size) : -1;
+      const int nowhere = (int)(p.num_blocks * p.block_size);                // rows from here on read as zeros
+      constexpr int kSlots = FP8 ? kRaw : kRing;
+      int turn = warp == 8 ? 0 : warp - 9;                                   // pieces until this warp's next
+      Cursor<kSlots> at;
+      uint32_t asked = 0, parities = 0;                                      // slots that this warp has filled, and with which parity the last time
+      bool ok = true;
+      int bad = 0;
+      while (ok && next_part<D>(p, plan, pos, end, x)) {
+        const int len = plan.len[x.group];
+        const int* bt = p.prefix_table + (size_t)x.group * p.prefix_ld;
+        // a tile's boxes: lane l has boxes l, l + 32, ...; looked up a tile ahead
+        auto places = [&](int t, int (&place)[kMost]) {
+#pragma unroll
+          for (int i = 0; i < kMost; ++i) {
+            const int b = lane + 32 * i, tok = t * kT + b * box;
+            place[i] = nowhere;
+            if (b < count && t < x.t1 && tok < len) {
+              const int bi = shift >= 0 ? tok >> shift : tok / p.block_size;
+              int blk = bt[bi];
+              if ((unsigned)blk >= (unsigned long long)p.num_blocks) {
+                bad = 1;
+                blk = 0;
+              }
+              place[i] = blk * p.block_size + (tok - bi * p.block_size);
+            }
+          }
+        };
+        int now[kMost], next[kMost];
+        places(x.t0, next);
+        for (int t = x.t0; t < x.t1 && ok; ++t) {
+#pragma unroll
+          for (int i = 0; i < kMost; ++i) now[i] = next[i];
+          places(t + 1, next);
+          // tokens [tok0, tok0 + n) of the tile, 128 bytes (or a whole shorter row) of each from byte c0 on, to dst
+          auto bring = [&](bool keys, uint64_t* bar, uint8_t* dst, int tok0, int n, int c0) {
+            constexpr int kRowB = FP8 ? D : 128;
+            const CUtensorMap *m = keys ? &tmK : &tmV, *m1 = keys ? &tmK1 : &tmV1;
+#pragma unroll
+            for (int i = 0; i < kMost; ++i) {
+              const int b = lane + 32 * i, in = b * box - tok0;              // the box's first row in the piece
+              if (in < 0 || in >= n || b >= count) continue;
+              const int left = len - (t * kT + b * box);
+              if (FP8 || left <= 0 || left >= box) {
+                mb::tma_load_3d(dst + in * kRowB, m, bar, c0, x.kvh, now[i]);
+              } else {                                                       // the prefix ends inside: values behind it must be zeros
+                for (int k = 0; k < box; ++k) mb::tma_load_3d(dst + (in + k) * kRowB, m1, bar, c0, x.kvh, k < left ? now[i] + k : nowhere);
+              }
+            }
+          };
+          constexpr int kN = FP8 ? C::kRawPer : C::kPer;
+          for (int c = 0; c < kN; ++c) {
+            if (turn == 0) {
+              uint64_t* bar = FP8 ? &raw_full[at.slot] : &full[at.slot];
+              ok = ok && mb::mbar_wait(FP8 ? &raw_empty[at.slot] : &empty[at.slot], at.parity ^ 1, p.status, MB_ST_TIMEOUT_TMA);
+              if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+              if (lane == 0) mb::mbar_expect_tx(bar, FP8 ? C::kRawB : kPiece);
+              __syncwarp();
+              if constexpr (FP8) {
+                bring(c < kN / 2, bar, sB + at.slot * C::kRawB, (c % (kN / 2)) * C::kRawTok, C::kRawTok, 0);
+              } else {
+                uint8_t* dst = sR + at.slot * kPiece;
+                if (c < kSpans) bring(true, bar, dst, 0, kT, c * 128);
+                else
+                  for (int d = 0; d < kSpans; ++d) bring(false, bar, dst + d * (kPiece / kSpans), (c - kSpans) * C::kVTok, C::kVTok, d * 128);
+              }
+              __syncwarp();
+              asked |= 1u << at.slot;
+              parities = (parities & ~(1u << at.slot)) | at.parity << at.slot;
+              turn = 3;
+            }
+            --turn;
+            at.step();
+          }
+        }
+      }
+      // given up: no copy may still be under way when the CTA ends
+      if (!ok)
+        for (int i = 0; i < kSlots; ++i)
+          if (asked >> i & 1) mb::mbar_wait(FP8 ? &raw_full[i] : &full[i], parities >> i & 1, p.status, MB_ST_TIMEOUT_TMA);
+      if (bad && p.status) atomicCAS(p.status, 0u, MB_ST_BOUNDS);
+    } else if (warp >= 12) {
+      // ---------------------------------------------------------- e4m3 to f16
+      if constexpr (FP8) {
+        const int t128 = tid - 384;
+        constexpr int kPieces = D / 16, kStep = 128 / kPieces, kN = C::kRawTok / kStep;   // 16-byte pieces of a row, rows between a thread's, and how many
+        const int c = t128 % kPieces, r0 = t128 / kPieces, sub = c >> 2, chunk = (c & 3) * 2;
+        Cursor<kRaw> raw;
+        Cursor<kRing> at;
+        bool ok = true;
+        // one piece as stored: row r to dst + sw_off(row0 + r); rows from `left` on are zeros
+        auto turn = [&](uint8_t* dst, int row0, int left) {
+          ok = mb::mbar_wait(&raw_full[raw.slot], raw.parity, p.status, MB_ST_TIMEOUT_TMA);
+          if (!__all_sync(0xffffffffu, ok)) { ok = false; return; }
+          const uint8_t* src = sB + raw.slot * C::kRawB;
+          uint4 v[kN];
+#pragma unroll
+          for (int i = 0; i < kN; ++i) v[i] = *reinterpret_cast<const uint4*>(src + (r0 + kStep * i) * D + c * 16);
+#pragma unroll
+          for (int i = 0; i < kN; ++i) {
+            const int r = r0 + kStep * i;
+            if (r >= left) v[i] = make_uint4(0, 0, 0, 0);
+            const uint32_t y[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+            uint32_t h[8];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              h[2 * k] = e4m3x2(y[k]);
+              h[2 * k + 1] = e4m3x2(y[k] >> 16);
+            }
+            // the second half of the lanes stores its pieces in the other order: eight lanes' stores then meet eight bank groups
+            const int odd = (D == 128 ? c >> 2 : c >> 1) & 1;
+            *reinterpret_cast<uint4*>(dst + sw_off(row0 + r, chunk + odd)) = odd ? make_uint4(h[4], h[5], h[6], h[7]) : make_uint4(h[0], h[1], h[2], h[3]);
+            *reinterpret_cast<uint4*>(dst + sw_off(row0 + r, chunk + 1 - odd)) = odd ? make_uint4(h[0], h[1], h[2], h[3]) : make_uint4(h[4], h[5], h[6], h[7]);
+          }
+          __syncwarp();
+          if (lane == 0) mb::mbar_arrive(&raw_empty[raw.slot]);
+          raw.step();
+        };
+        auto room = [&](int slot, uint32_t parity) {
+          ok = ok && mb::mbar_wait(&empty[slot], parity ^ 1, p.status, MB_ST_TIMEOUT_TMA);
+          if (!__all_sync(0xffffffffu, ok)) ok = false;
+          return ok;
+        };
+        auto announce = [&](int slot) {
+          if (lane == 0) mb::mbar_arrive(&full[slot]);
+        };
+        while (ok && next_part<D>(p, plan, pos, end, x)) {
+          const int len = plan.len[x.group];
+          for (int t = x.t0; t < x.t1 && ok; ++t) {
+            const int left = len - t * kT;
+            // K: every piece as stored holds tokens of all dims, every span of 64 dims is a piece of the ring
+            Cursor<kRing> span = at;
+            int slot[kSpans];
+#pragma unroll
+            for (int h = 0; h < kSpans; ++h) {
+              if (!room(span.slot, span.parity)) break;
+              slot[h] = span.slot;
+              span.step();
+            }
+            if (!ok) break;
+            uint8_t* dst = sR + (kSpans == 1 || sub == 0 ? slot[0] : slot[kSpans - 1]) * kPiece;
+            for (int h = 0; h < C::kRawPer / 2 && ok; ++h) turn(dst, h * C::kRawTok, left - h * C::kRawTok);
+            if (!ok) break;
+            fence_async_smem();
+            __syncwarp();
+#pragma unroll
+            for (int h = 0; h < kSpans; ++h) announce(slot[h]);
+            at = span;
+            // V: as many tokens in either
+            for (int h = 0; h < kSpans && ok; ++h) {
+              if (!room(at.slot, at.parity)) break;
+              turn(sR + at.slot * kPiece + sub * (kPiece / kSpans), 0, left - h * C::kRawTok);
+              if (!ok) break;
+              fence_async_smem();
+              __syncwarp();
+              announce(at.slot);
+              at.step();
+            }
+          }
+        }
+      }
+    } else if (warp == 9 && mb::elect_one()) {
       // ---------------------------------------------------------- products
       constexpr uint32_t kF = FP8 ? 0 : 1;
       constexpr uint32_t kIdS = mb::umma_idesc(kF, kF, 128, kT), kIdO = mb::umma_idesc(kF, kF, 128, D, 0, 1);
-      const uint32_t aQ = mb::smem_u32(sQ), aK = mb::smem_u32(sK), aV = mb::smem_u32(sV);
-      uint32_t part = 0, base = 0, done[2] = {0, 0};      // parts, tiles brought, tiles that either accumulator has had
+      // descriptors count 16 bytes: an operand's next step is an addition
+      const uint64_t dQ = mb::umma_desc_sw128(mb::smem_u32(sQ)), dK = mb::umma_desc_sw128(mb::smem_u32(sR)),
+                     dV = mb::umma_desc_sw128_mn(mb::smem_u32(sR), kPiece / kSpans, 1024);
+      Cursor<kRing> base;                                 // the part's first piece
+      uint32_t part = 0, done0 = 0, done1 = 0;            // parts, tiles that either accumulator has had
       bool ok = true;
-      int pos = begin;
-      Part x;
+      auto there = [&](const Cursor<kRing>& c) { return mb::mbar_wait(&full[c.slot], c.parity, p.status, MB_ST_TIMEOUT_MMA); };
       while (ok && next_part<D>(p, plan, pos, end, x)) {
         const int n = x.t1 - x.t0, n0 = x.two ? n : (n + 1) / 2, n1 = x.two ? n : n / 2;
-        auto stage = [&](int w, int i) { return base + (x.two ? i : 2 * i + w); };
-        auto scores = [&](int w, int i) {
-          const uint32_t t = stage(w, i);
-          if (!mb::mbar_wait(&k_full[t & 1], (t >> 1) & 1, p.status, MB_ST_TIMEOUT_MMA)) return false;
-          mb::tc_fence_after();
+        Cursor<kRing> k0 = base, k1 = base, v0, v1;       // where either accumulator's next keys and values lie
+        if (!x.two) k1.step(C::kPer);
+        v0 = k0;
+        v1 = k1;
+        v0.step(kSpans);
+        v1.step(kSpans);
+        auto ahead = [&](Cursor<kRing>& c) {
+          c.step(C::kPer);
+          if (!x.two) c.step(C::kPer);
+        };
+        // w: accumulator; `last`: nobody else takes these pieces
+        auto scores = [&](int w, Cursor<kRing>& at, bool last) {
+          Cursor<kRing> c = at;
 #pragma unroll
-          for (int h = 0; h < kSpans; ++h)
+          for (int h = 0; h < kSpans; ++h) {
+            if (!there(c)) return false;
+            mb::tc_fence_after();
+            const uint64_t q = dQ + (x.two ? w : 0) * (kQB >> 4) + ((h * 16384) >> 4), k = dK + c.slot * (kPiece >> 4);
 #pragma unroll
-            for (int s = 0; s < 4; ++s)
-              mb::umma_f16(tmem + w * 128, mb::umma_desc_sw128(aQ + (x.two ? w : 0) * kQB + h * (128 * 128) + s * 32),
-                           mb::umma_desc_sw128(aK + (t & 1) * kTileB + h * (kT * 128) + s * 32), kIdS, (h | s) != 0);
+            for (int s = 0; s < 4; ++s) mb::umma_f16(tmem + w * 128, q + ((s * 32) >> 4), k + ((s * 32) >> 4), kIdS, (h | s) != 0);
+            if (last) mb::tc_commit(&empty[c.slot]);
+            c.step();
+          }
           mb::tc_commit(&s_full[w]);
-          if (!x.two || w == 1) mb::tc_commit(&k_empty[t & 1]);
+          ahead(at);
           return true;
         };
-        auto values = [&](int w, int i) {
-          const uint32_t t = stage(w, i);
-          if (!mb::mbar_wait(&v_full[t & 1], (t >> 1) & 1, p.status, MB_ST_TIMEOUT_MMA) ||
-              !mb::mbar_wait(&p_full[w], (done[w] + i) & 1, p.status, MB_ST_TIMEOUT_MMA))
-            return false;
-          mb::tc_fence_after();
+        auto values = [&](int w, Cursor<kRing>& at, bool last, uint32_t done, bool fresh) {
+          Cursor<kRing> c = at;
 #pragma unroll
-          for (int s = 0; s < kT / 16; ++s)
-            umma_f16_ta(tmem + 256 + w * 128, tmem + w * 128 + s * 8, mb::umma_desc_sw128_mn(aV + (t & 1) * kTileB + s * 2048, kT * 128, 1024), kIdO, (i | s) != 0);
-          if (!x.two || w == 1) mb::tc_commit(&v_empty[t & 1]);
+          for (int h = 0; h < 2; ++h) {
+            if (!there(c) || !mb::mbar_wait(&p_full[w][h], done & 1, p.status, MB_ST_TIMEOUT_MMA)) return false;
+            mb::tc_fence_after();
+            const uint64_t v = dV + c.slot * (kPiece >> 4) + (kSpans == 1 ? h * 4 * (2048 >> 4) : 0);
+#pragma unroll
+            for (int s = 0; s < 4; ++s) umma_f16_ta(tmem + 256 + w * 128, tmem + w * 128 + (h * 4 + s) * 8, v + ((s * 2048) >> 4), kIdO, !(fresh && h == 0 && s == 0));
+            if (h == 1 || kSpans == 2) {
+              if (last) mb::tc_commit(&empty[c.slot]);
+              c.step();
+            }
+          }
+          ahead(at);
           return true;
         };
-        // both accumulators' rows are written, and their former outputs read
+        // rows are written, and the outputs of the part in front read
         ok = mb::mbar_wait(&q_full[0], part & 1, p.status, MB_ST_TIMEOUT_MMA) && mb::mbar_wait(&q_full[1], part & 1, p.status, MB_ST_TIMEOUT_MMA);
-        if (ok) ok = scores(0, 0);
-        if (ok && n1 > 0) ok = scores(1, 0);
+        if (ok) ok = scores(0, k0, !x.two);
+        if (ok && n1 > 0) ok = scores(1, k1, true);
         for (int i = 0; i < n0 && ok; ++i) {
-          ok = values(0, i);
+          ok = values(0, v0, !x.two, done0 + i, i == 0);
           if (!ok) break;
-          if (i + 1 < n0) ok = scores(0, i + 1);
+          if (i + 1 < n0) ok = scores(0, k0, !x.two);
           else mb::tc_commit(&o_full[0]);
           if (!ok || i >= n1) break;
-          ok = values(1, i);
+          ok = values(1, v1, true, done1 + i, i == 0);
           if (!ok) break;
-          if (i + 1 < n1) ok = scores(1, i + 1);
+          if (i + 1 < n1) ok = scores(1, k1, true);
           else mb::tc_commit(&o_full[1]);
         }
-        base += n;
-        done[0] += n0;
-        done[1] += n1;
+        mb::tc_commit(&q_free);
+        const int total = base.slot + n * C::kPer;
+        base.parity ^= (total / kRing) & 1;
+        base.slot = total % kRing;
+        done0 += n0;
+        done1 += n1;
         ++part;
       }
     }
     __syncwarp();
   }
   __syncthreads();
-  if (warp == 12) {
+  if (warp == 9) {
     mb::tc_fence_after();
     mb::tmem_dealloc(tmem, 512);
   }
@@ -721,21 +934,31 @@ __global__ void __launch_bounds__(288, 1) shared_prefix256_kernel(const MbShared
 
 template <int D, bool FP8>
 int launch_prefix(const MbSharedArgs& a, const Ws& ws, cudaStream_t stream) {
-  void (*kern)(const MbSharedArgs, const Ws);
-  int threads, smem;
-  if constexpr (D == 256) {
-    kern = shared_prefix256_kernel<FP8>;
-    threads = 288;
-    smem = 128 * D * 2 + 4 * 64 * D * 2 + 1024 + (int)sizeof(Plan);
-  } else {
-    kern = shared_prefix_kernel<D, FP8>;
-    threads = PrefixCfg<D, FP8>::kThreads;
-    smem = PrefixCfg<D, FP8>::kSmem;
-  }
   static std::atomic<uint64_t> asked{0};
-  const cudaError_t e = mb::allow_smem(reinterpret_cast<const void*>(kern), smem, asked);
-  if (e != cudaSuccess) return (int)e;
-  return (int)mb::launch_kernel(kern, dim3(ws.ctas), dim3(threads), smem, stream, a, ws);
+  if constexpr (D == 256) {
+    auto kern = shared_prefix256_kernel<FP8>;
+    constexpr int smem = 128 * D * 2 + 4 * 64 * D * 2 + 1024 + (int)sizeof(Plan);
+    const cudaError_t e = mb::allow_smem(reinterpret_cast<const void*>(kern), smem, asked);
+    if (e != cudaSuccess) return (int)e;
+    return (int)mb::launch_kernel(kern, dim3(ws.ctas), dim3(288), smem, stream, a, ws);
+  } else {
+    using C = PrefixCfg<D, FP8>;
+    auto kern = shared_prefix_kernel<D, FP8>;
+    Boxes boxes{0};
+    while (a.block_size % (16 >> boxes.bits)) ++boxes.bits;
+    constexpr uint32_t row = FP8 ? D : 2 * D, width = row < 128 ? row : 128;
+    const CUtensorMapSwizzle sw = FP8 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B;
+    CUtensorMap tm[4];
+    for (int i = 0; i < (FP8 ? 2 : 4); ++i) {
+      const int rc = mbh::encode_3d(&tm[i], CU_TENSOR_MAP_DATA_TYPE_UINT8, i & 1 ? a.v_cache : a.k_cache, row, a.Hkv, (uint64_t)a.num_blocks * a.block_size, row,
+                                    (uint64_t)a.Hkv * row, width, 1, i < 2 ? 16 >> boxes.bits : 1, sw);
+      if (rc) return rc;
+    }
+    if (FP8) tm[2] = tm[3] = tm[0];                        // not used
+    const cudaError_t e = mb::allow_smem(reinterpret_cast<const void*>(kern), C::kSmem, asked);
+    if (e != cudaSuccess) return (int)e;
+    return (int)mb::launch_kernel(kern, dim3(ws.ctas), dim3(C::kThreads), C::kSmem, stream, tm[0], tm[1], tm[2], tm[3], boxes, a, ws);
+  }
 }
 
 }  // namespace mbs
