@@ -5,14 +5,18 @@
 // turn, so that the softmax of one runs under the products of the other. Behind a prefix few rows are the rule: where a unit has one tile of rows (up to
 // 128), both accumulators take the cached tiles of this one in turn. Roles (one CTA an SM, registers moved with setmaxnreg):
 //   warps 0-3, 4-7   softmax of accumulator 0 / 1, thread = row; they load their rows' queries and write their outputs
-//   warps 8, 10, 11  copies by TMA, a box of up to 16 cached rows each (as many as lie in one block): a bf16 cache into a ring of pieces as
-//                    the products take them, an e4m3 cache as stored into a ring of its own; piece by piece in turn, since a warp needs some 90 cycles a box
+//   warps 8, 10, 11  copies by TMA, a box of up to 16 cached rows each (as many as lie in one block), into rings of pieces of keys and of values; a
+//                    warp fills every third place of a ring, since it needs some 90 cycles a box
 //   warp 9           the products
-//   warps 12-15      (e4m3 cache) make f16 pieces of what was copied: exact, one conversion per two values
-// A piece is 16 KB: 64 dims of 128 keys, or 64 values of 128 dims. All roles run on from part to part; queries wait for the products of the part in front
-// of theirs only.
-// With an e4m3 cache a row's queries are scaled by the power of two that takes their largest to [2^14, 2^15) and weights are held 2^7 larger, as
-// there: neither then loses the range that bf16 gives.
+//   warps 12-15      (e4m3 cache) make f16 of the values as stored: exact, one conversion per two
+// A piece of a bf16 cache is 64 dims of 128 keys, or 64 values of 128 dims. All roles run on from part to part; queries wait for the products of the part in
+// front of theirs only.
+//
+// e4m3 keys are multiplied as they are, by queries that are the sum of two e4m3 numbers: scaled by the power of two that takes a row's largest element to
+// [2^7, 2^8), an element's 8 bits are the 4 of its rounding and a remainder of 4, which e4m3 holds exactly down to 2^-2. Elements that are less than
+// 2^-9 of the row's largest are off by 2^-17 of it at most, those under 2^-18 of it vanish. That is as many products as of f16 operands, at twice the rate;
+// keys of f16 made from e4m3 kept the converting warps busy for as long again as values do (128 sequences behind 32768 tokens 203 us).
+// Weights are f16, held 2^7 larger than the running maximum says, as in attention_rows.cu.
 #pragma once
 #include "softmax_rows.cuh"
 #include "shared_plan.cuh"
@@ -96,6 +100,48 @@ __device__ __forceinline__ uint4 query_piece(uint4 v, float& scale) {
     return make_uint4(h[0], h[1], h[2], h[3]);
   }
   return v;
+}
+
+// Eight dims of a query row as two e4m3 numbers each, for keys of e4m3; lanes of a row are D / 8 neighbours
+template <int D>
+__device__ __forceinline__ void query_pair(uint4 v, uint2 (&out)[2], float& scale) {
+  const uint32_t x[4] = {v.x, v.y, v.z, v.w};
+  uint32_t top = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) top = __vmaxu2(top, x[j] & 0x7fff7fffu);       // bf16 bits without the sign order like the values
+#pragma unroll
+  for (int d = 1; d < D / 8; d <<= 1) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, d));
+  const int e = (int)(max(top & 0xffff, top >> 16) >> 7), up = e == 255 ? 0 : 134 - max(e, 8);
+  const float f = __int_as_float((127 + up) << 23);
+  uint32_t h[2][4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    float2 y = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&x[j]));
+    y.x *= f;
+    y.y *= f;
+    if (e == 255) {                                        // the type has no infinities: they become NaN
+      if (isinf(y.x)) y.x = __int_as_float(0x7fffffff);
+      if (isinf(y.y)) y.y = __int_as_float(0x7fffffff);
+    }
+    h[0][j] = __nv_cvt_float2_to_fp8x2(y, __NV_SATFINITE, __NV_E4M3);
+    const uint32_t back = e4m3x2(h[0][j]);
+    const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&back));
+    h[1][j] = __nv_cvt_float2_to_fp8x2(make_float2(y.x - b.x, y.y - b.y), __NV_SATFINITE, __NV_E4M3);
+  }
+#pragma unroll
+  for (int t = 0; t < 2; ++t) out[t] = make_uint2(h[t][0] | h[t][1] << 16, h[t][2] | h[t][3] << 16);
+  scale = __int_as_float((127 - up) << 23);
+}
+
+// Operand rows of 64 bytes: pieces of 16 bytes exchanged by (row / 2) mod 4, eight rows 512 bytes
+__device__ __forceinline__ uint64_t umma_desc_sw64(uint32_t saddr) {
+  uint64_t d = 0;
+  d |= (uint64_t)((saddr & 0x3FFFF) >> 4);
+  d |= (uint64_t)1 << 16;
+  d |= (uint64_t)(512 >> 4) << 32;
+  d |= (uint64_t)1 << 46;
+  d |= (uint64_t)4 << 61;
+  return d;
 }
 
 // K and V tiles of kT cached tokens of this CTA's parts, one after the other, into two stages each: 128 threads, t the number of this one
@@ -251,13 +297,13 @@ struct Boxes {
 template <int D, bool FP8>
 struct PrefixCfg {
   static constexpr int kT = 128, kThreads = FP8 ? 512 : 384;
-  static constexpr int kQB = 128 * D * 2, kPiece = 16384, kSpans = D / 64;
-  static constexpr int kPer = 2 * kSpans;                 // pieces of a tile: K in spans, V in as many runs of tokens
-  static constexpr int kVTok = kT / kSpans;               // tokens of a V piece
-  static constexpr int kRing = FP8 ? 6 : 9;
-  static constexpr int kRawB = 8192, kRawTok = kRawB / D, kRawRing = FP8 ? 6 : 0;       // pieces as stored: tokens of all dims
-  static constexpr int kRawPer = 2 * kT / kRawTok;
-  static constexpr int kSmem = 2 * kQB + kRing * kPiece + kRawRing * kRawB + 1024 + (int)sizeof(Plan);
+  static constexpr int kQB = 128 * D * 2, kSpans = D / 64;
+  // pieces of keys (bf16: a span of 64 dims, e4m3: a tile as stored) and of values (as many runs of tokens as there are spans)
+  static constexpr int kKeyB = FP8 ? kT * D : 16384, kKeys = FP8 ? 1 : kSpans, kKeyRing = FP8 ? 49152 / kKeyB : 5;
+  static constexpr int kValB = 16384, kVals = kSpans, kValTok = kT / kVals, kValRing = 4;
+  static constexpr int kRawB = FP8 ? kT * D : 0, kRawRing = FP8 ? 32768 / kRawB : 0;     // values of a tile as stored
+  static constexpr int kRing = kKeyRing * kKeyB + kValRing * kValB + kRawRing * kRawB;
+  static constexpr int kSmem = 2 * kQB + kRing + 1024 + (int)sizeof(Plan);
 };
 
 // Places in a ring
@@ -272,11 +318,9 @@ struct Cursor {
     }
   }
   __device__ __forceinline__ void step(int n) {
-    slot += n;
-    if (slot >= N) {
-      slot -= N;
-      parity ^= 1;
-    }
+    const int total = slot + n;
+    parity ^= (total / N) & 1;
+    slot = total % N;
   }
 };
 
@@ -285,13 +329,15 @@ __global__ void __launch_bounds__(PrefixCfg<D, FP8>::kThreads, 1)
 shared_prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmK1,
                      const __grid_constant__ CUtensorMap tmV1, const Boxes boxes, const MbSharedArgs p, const Ws ws) {
   using C = PrefixCfg<D, FP8>;
-  constexpr int kT = C::kT, kQB = C::kQB, kPiece = C::kPiece, kSpans = C::kSpans, kRing = C::kRing, kRaw = FP8 ? C::kRawRing : 1;
+  constexpr int kT = C::kT, kQB = C::kQB, kSpans = C::kSpans, kKeyRing = C::kKeyRing, kValRing = C::kValRing, kRaw = FP8 ? C::kRawRing : 1;
   extern __shared__ __align__(16) uint8_t smem_raw[];
   uint8_t* sQ = smem_raw + ((1024u - (mb::smem_u32(smem_raw) & 1023u)) & 1023u);   // 2 row tiles x spans of 64 dims x [128 rows x 128 B]
-  uint8_t* sR = sQ + 2 * kQB;                             // ring of pieces
-  uint8_t* sB = sR + kRing * kPiece;                      // ring of pieces as stored
+  uint8_t* sK = sQ + 2 * kQB;                             // rings of keys, of values, of values as stored
+  uint8_t* sV = sK + kKeyRing * C::kKeyB;
+  uint8_t* sB = sV + kValRing * C::kValB;
   Plan& plan = *reinterpret_cast<Plan*>(sB + C::kRawRing * C::kRawB);
-  __shared__ __align__(8) uint64_t q_full[2], q_free, full[kRing], empty[kRing], raw_full[kRaw], raw_empty[kRaw], s_full[2], p_full[2][2], o_full[2];
+  __shared__ __align__(8) uint64_t q_full[2], q_free, k_full[kKeyRing], k_empty[kKeyRing], v_full[kValRing], v_empty[kValRing], raw_full[kRaw], raw_empty[kRaw], s_full[2],
+      p_full[2][2], o_full[2];
   __shared__ uint32_t s_tmem;
   __shared__ float s_qscale[FP8 ? 2 : 1][2][128];         // what a row's scores are too large by (e4m3 cache), of parts in turn
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = p.Hq / p.Hkv;
@@ -307,9 +353,13 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
       mb::mbar_init(&p_full[i][1], 4);
       mb::mbar_init(&o_full[i], 1);
     }
-    for (int i = 0; i < kRing; ++i) {
-      mb::mbar_init(&full[i], FP8 ? 4 : 1);
-      mb::mbar_init(&empty[i], 1);
+    for (int i = 0; i < kKeyRing; ++i) {
+      mb::mbar_init(&k_full[i], 1);
+      mb::mbar_init(&k_empty[i], 1);
+    }
+    for (int i = 0; i < kValRing; ++i) {
+      mb::mbar_init(&v_full[i], FP8 ? 4 : 1);
+      mb::mbar_init(&v_empty[i], 1);
     }
     for (int i = 0; i < kRaw; ++i) {
       mb::mbar_init(&raw_full[i], 1);
@@ -361,10 +411,17 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
         for (int i = 0; i < kQ; ++i) {
           const int qr = first + kStep * i;
           if (qr > last) v[i] = make_uint4(0, 0, 0, 0);
-          float back = 1.f;
-          v[i] = query_piece<D, FP8>(v[i], back);
-          if (FP8 && c == 0) s_qscale[part & 1][w][qr] = back;
-          *reinterpret_cast<uint4*>(sQ + w * kQB + (c >> 3) * (128 * 128) + sw_off(qr, c & 7)) = v[i];
+          if constexpr (FP8) {
+            float back;
+            uint2 h[2];
+            query_pair<D>(v[i], h, back);
+            if (c == 0) s_qscale[part & 1][w][qr] = back;
+            const int at16 = D == 128 ? (c >> 1) ^ (qr & 7) : (c >> 1) ^ ((qr >> 1) & 3);
+#pragma unroll
+            for (int t = 0; t < 2; ++t) *reinterpret_cast<uint2*>(sQ + w * kQB + t * (128 * D) + qr * D + at16 * 16 + (c & 1) * 8) = h[t];
+          } else {
+            *reinterpret_cast<uint4*>(sQ + w * kQB + (c >> 3) * (128 * 128) + sw_off(qr, c & 7)) = v[i];
+          }
         }
         fence_async_smem();
       }
@@ -460,10 +517,12 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
       constexpr int kMost = 4;                                               // of a lane: 128 boxes of one row
       const int shift = (p.block_size & (p.block_size - 1)) == 0 ? 31 - __clz(p.block_size) : -1;
       const int nowhere = (int)(p.num_blocks * p.block_size);                // rows from here on read as zeros
-      constexpr int kSlots = FP8 ? kRaw : kRing;
-      int turn = warp == 8 ? 0 : warp - 9;                                   // pieces until this warp's next
-      Cursor<kSlots> at;
-      uint32_t asked = 0, parities = 0;                                      // slots that this warp has filled, and with which parity the last time
+      const int who = warp == 8 ? 0 : warp - 9;
+      constexpr int kValSlots = FP8 ? kRaw : kValRing;
+      uint64_t *val_full = FP8 ? raw_full : v_full, *val_empty = FP8 ? raw_empty : v_empty;
+      Cursor<kKeyRing> at_key;
+      Cursor<kValSlots> at_val;
+      uint32_t keys_asked = 0, vals_asked = 0, key_parities = 0, val_parities = 0;      // slots that this warp has filled, with which parity the last time
       bool ok = true;
       int bad = 0;
       while (ok && next_part<D>(p, plan, pos, end, x)) {
@@ -508,112 +567,102 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
               }
             }
           };
-          constexpr int kN = FP8 ? C::kRawPer : C::kPer;
-          for (int c = 0; c < kN; ++c) {
-            if (turn == 0) {
-              uint64_t* bar = FP8 ? &raw_full[at.slot] : &full[at.slot];
-              ok = ok && mb::mbar_wait(FP8 ? &raw_empty[at.slot] : &empty[at.slot], at.parity ^ 1, p.status, MB_ST_TIMEOUT_TMA);
-              if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-              if (lane == 0) mb::mbar_expect_tx(bar, FP8 ? C::kRawB : kPiece);
+          // Whether a place is this warp's to fill, and it is empty. A place is always the same warp's: a wait tells a phase from its neighbours only, and a warp
+          // that took another's place could be two rounds of it ahead of the products
+          auto mine = [&](int owner, uint64_t* empty, uint32_t parity) {
+            if (owner % 3 != who) return false;
+            ok = ok && mb::mbar_wait(empty, parity ^ 1, p.status, MB_ST_TIMEOUT_TMA);
+            if (!__all_sync(0xffffffffu, ok)) ok = false;
+            return ok;
+          };
+          for (int c = 0; c < C::kKeys && ok; ++c) {
+            if (mine(at_key.slot, &k_empty[at_key.slot], at_key.parity)) {
+              uint64_t* bar = &k_full[at_key.slot];
+              if (lane == 0) mb::mbar_expect_tx(bar, C::kKeyB);
+              __syncwarp();
+              bring(true, bar, sK + at_key.slot * C::kKeyB, 0, kT, c * 128);
+              __syncwarp();
+              keys_asked |= 1u << at_key.slot;
+              key_parities = (key_parities & ~(1u << at_key.slot)) | at_key.parity << at_key.slot;
+            }
+            at_key.step();
+          }
+          for (int c = 0; c < (FP8 ? 1 : C::kVals) && ok; ++c) {
+            if (mine(at_val.slot + (FP8 ? 1 : 2), &val_empty[at_val.slot], at_val.parity)) {
+              uint64_t* bar = &val_full[at_val.slot];
+              if (lane == 0) mb::mbar_expect_tx(bar, FP8 ? C::kRawB : C::kValB);
               __syncwarp();
               if constexpr (FP8) {
-                bring(c < kN / 2, bar, sB + at.slot * C::kRawB, (c % (kN / 2)) * C::kRawTok, C::kRawTok, 0);
+                bring(false, bar, sB + at_val.slot * C::kRawB, 0, kT, 0);
               } else {
-                uint8_t* dst = sR + at.slot * kPiece;
-                if (c < kSpans) bring(true, bar, dst, 0, kT, c * 128);
-                else
-                  for (int d = 0; d < kSpans; ++d) bring(false, bar, dst + d * (kPiece / kSpans), (c - kSpans) * C::kVTok, C::kVTok, d * 128);
+                uint8_t* dst = sV + at_val.slot * C::kValB;
+                for (int d = 0; d < kSpans; ++d) bring(false, bar, dst + d * (C::kValB / kSpans), c * C::kValTok, C::kValTok, d * 128);
               }
               __syncwarp();
-              asked |= 1u << at.slot;
-              parities = (parities & ~(1u << at.slot)) | at.parity << at.slot;
-              turn = 3;
+              vals_asked |= 1u << at_val.slot;
+              val_parities = (val_parities & ~(1u << at_val.slot)) | at_val.parity << at_val.slot;
             }
-            --turn;
-            at.step();
+            at_val.step();
           }
         }
       }
       // given up: no copy may still be under way when the CTA ends
-      if (!ok)
-        for (int i = 0; i < kSlots; ++i)
-          if (asked >> i & 1) mb::mbar_wait(FP8 ? &raw_full[i] : &full[i], parities >> i & 1, p.status, MB_ST_TIMEOUT_TMA);
+      if (!ok) {
+        for (int i = 0; i < kKeyRing; ++i)
+          if (keys_asked >> i & 1) mb::mbar_wait(&k_full[i], key_parities >> i & 1, p.status, MB_ST_TIMEOUT_TMA);
+        for (int i = 0; i < kValSlots; ++i)
+          if (vals_asked >> i & 1) mb::mbar_wait(&val_full[i], val_parities >> i & 1, p.status, MB_ST_TIMEOUT_TMA);
+      }
       if (bad && p.status) atomicCAS(p.status, 0u, MB_ST_BOUNDS);
     } else if (warp >= 12) {
       // ---------------------------------------------------------- e4m3 to f16
       if constexpr (FP8) {
         const int t128 = tid - 384;
-        constexpr int kPieces = D / 16, kStep = 128 / kPieces, kN = C::kRawTok / kStep;   // 16-byte pieces of a row, rows between a thread's, and how many
+        constexpr int kPieces = D / 16, kStep = 128 / kPieces, kN = kT / kStep;           // 16-byte pieces of a row, rows between a thread's, and how many
         const int c = t128 % kPieces, r0 = t128 / kPieces, sub = c >> 2, chunk = (c & 3) * 2;
+        // half of the lanes stores its pieces in the other order: eight lanes' stores then meet eight bank groups
+        const int odd = (D == 128 ? c >> 2 : c >> 1) & 1;
         Cursor<kRaw> raw;
-        Cursor<kRing> at;
+        Cursor<kValRing> at;
         bool ok = true;
-        // one piece as stored: row r to dst + sw_off(row0 + r); rows from `left` on are zeros
-        auto turn = [&](uint8_t* dst, int row0, int left) {
-          ok = mb::mbar_wait(&raw_full[raw.slot], raw.parity, p.status, MB_ST_TIMEOUT_TMA);
-          if (!__all_sync(0xffffffffu, ok)) { ok = false; return; }
-          const uint8_t* src = sB + raw.slot * C::kRawB;
-          uint4 v[kN];
-#pragma unroll
-          for (int i = 0; i < kN; ++i) v[i] = *reinterpret_cast<const uint4*>(src + (r0 + kStep * i) * D + c * 16);
-#pragma unroll
-          for (int i = 0; i < kN; ++i) {
-            const int r = r0 + kStep * i;
-            if (r >= left) v[i] = make_uint4(0, 0, 0, 0);
-            const uint32_t y[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-            uint32_t h[8];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              h[2 * k] = e4m3x2(y[k]);
-              h[2 * k + 1] = e4m3x2(y[k] >> 16);
-            }
-            // the second half of the lanes stores its pieces in the other order: eight lanes' stores then meet eight bank groups
-            const int odd = (D == 128 ? c >> 2 : c >> 1) & 1;
-            *reinterpret_cast<uint4*>(dst + sw_off(row0 + r, chunk + odd)) = odd ? make_uint4(h[4], h[5], h[6], h[7]) : make_uint4(h[0], h[1], h[2], h[3]);
-            *reinterpret_cast<uint4*>(dst + sw_off(row0 + r, chunk + 1 - odd)) = odd ? make_uint4(h[0], h[1], h[2], h[3]) : make_uint4(h[4], h[5], h[6], h[7]);
-          }
-          __syncwarp();
-          if (lane == 0) mb::mbar_arrive(&raw_empty[raw.slot]);
-          raw.step();
-        };
-        auto room = [&](int slot, uint32_t parity) {
-          ok = ok && mb::mbar_wait(&empty[slot], parity ^ 1, p.status, MB_ST_TIMEOUT_TMA);
-          if (!__all_sync(0xffffffffu, ok)) ok = false;
-          return ok;
-        };
-        auto announce = [&](int slot) {
-          if (lane == 0) mb::mbar_arrive(&full[slot]);
-        };
         while (ok && next_part<D>(p, plan, pos, end, x)) {
           const int len = plan.len[x.group];
+#pragma unroll 1
           for (int t = x.t0; t < x.t1 && ok; ++t) {
-            const int left = len - t * kT;
-            // K: every piece as stored holds tokens of all dims, every span of 64 dims is a piece of the ring
-            Cursor<kRing> span = at;
-            int slot[kSpans];
+            const int left = len - t * kT;                 // rows from here on are zeros
+            ok = mb::mbar_wait(&raw_full[raw.slot], raw.parity, p.status, MB_ST_TIMEOUT_TMA);
+            if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+            const uint8_t* src = sB + raw.slot * C::kRawB + r0 * D + c * 16;
+            uint4 y[kN];
 #pragma unroll
-            for (int h = 0; h < kSpans; ++h) {
-              if (!room(span.slot, span.parity)) break;
-              slot[h] = span.slot;
-              span.step();
-            }
-            if (!ok) break;
-            uint8_t* dst = sR + (kSpans == 1 || sub == 0 ? slot[0] : slot[kSpans - 1]) * kPiece;
-            for (int h = 0; h < C::kRawPer / 2 && ok; ++h) turn(dst, h * C::kRawTok, left - h * C::kRawTok);
-            if (!ok) break;
-            fence_async_smem();
+            for (int i = 0; i < kN; ++i) y[i] = *reinterpret_cast<const uint4*>(src + kStep * i * D);
             __syncwarp();
+            if (lane == 0) mb::mbar_arrive(&raw_empty[raw.slot]);
+            raw.step();
 #pragma unroll
-            for (int h = 0; h < kSpans; ++h) announce(slot[h]);
-            at = span;
-            // V: as many tokens in either
-            for (int h = 0; h < kSpans && ok; ++h) {
-              if (!room(at.slot, at.parity)) break;
-              turn(sR + at.slot * kPiece + sub * (kPiece / kSpans), 0, left - h * C::kRawTok);
-              if (!ok) break;
+            for (int v = 0; v < C::kVals; ++v) {
+              ok = ok && mb::mbar_wait(&v_empty[at.slot], at.parity ^ 1, p.status, MB_ST_TIMEOUT_TMA);
+              if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+              uint8_t* dst = sV + at.slot * C::kValB + sub * (C::kValB / kSpans);
+#pragma unroll
+              for (int i = v * kN / C::kVals; i < (v + 1) * kN / C::kVals; ++i) {
+                const int r = r0 + kStep * i;
+                if (r >= left) y[i] = make_uint4(0, 0, 0, 0);
+                const uint32_t z[4] = {y[i].x, y[i].y, y[i].z, y[i].w};
+                uint32_t h[8];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                  h[2 * k] = e4m3x2(z[k]);
+                  h[2 * k + 1] = e4m3x2(z[k] >> 16);
+                }
+                uint8_t *to = dst + sw_off(r % C::kValTok, chunk), *also = dst + sw_off(r % C::kValTok, chunk + 1);
+                const uint4 lo = make_uint4(h[0], h[1], h[2], h[3]), hi = make_uint4(h[4], h[5], h[6], h[7]);
+                *reinterpret_cast<uint4*>(odd ? also : to) = odd ? hi : lo;
+                *reinterpret_cast<uint4*>(odd ? to : also) = odd ? lo : hi;
+              }
               fence_async_smem();
               __syncwarp();
-              announce(at.slot);
+              if (lane == 0) mb::mbar_arrive(&v_full[at.slot]);
               at.step();
             }
           }
@@ -621,59 +670,66 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
       }
     } else if (warp == 9 && mb::elect_one()) {
       // ---------------------------------------------------------- products
-      constexpr uint32_t kF = FP8 ? 0 : 1;
+      constexpr uint32_t kF = FP8 ? 0 : 1;                 // of f16 / bf16 operands; e4m3 is 0 among its own
       constexpr uint32_t kIdS = mb::umma_idesc(kF, kF, 128, kT), kIdO = mb::umma_idesc(kF, kF, 128, D, 0, 1);
       // descriptors count 16 bytes: an operand's next step is an addition
-      const uint64_t dQ = mb::umma_desc_sw128(mb::smem_u32(sQ)), dK = mb::umma_desc_sw128(mb::smem_u32(sR)),
-                     dV = mb::umma_desc_sw128_mn(mb::smem_u32(sR), kPiece / kSpans, 1024);
-      Cursor<kRing> base;                                 // the part's first piece
+      const bool narrow = FP8 && D == 64;
+      const uint64_t dQ = narrow ? umma_desc_sw64(mb::smem_u32(sQ)) : mb::umma_desc_sw128(mb::smem_u32(sQ)),
+                     dK = narrow ? umma_desc_sw64(mb::smem_u32(sK)) : mb::umma_desc_sw128(mb::smem_u32(sK)),
+                     dV = mb::umma_desc_sw128_mn(mb::smem_u32(sV), C::kValB / kSpans, 1024);
+      Cursor<kKeyRing> key;                               // the part's first pieces
+      Cursor<kValRing> val;
       uint32_t part = 0, done0 = 0, done1 = 0;            // parts, tiles that either accumulator has had
       bool ok = true;
-      auto there = [&](const Cursor<kRing>& c) { return mb::mbar_wait(&full[c.slot], c.parity, p.status, MB_ST_TIMEOUT_MMA); };
       while (ok && next_part<D>(p, plan, pos, end, x)) {
-        const int n = x.t1 - x.t0, n0 = x.two ? n : (n + 1) / 2, n1 = x.two ? n : n / 2;
-        Cursor<kRing> k0 = base, k1 = base, v0, v1;       // where either accumulator's next keys and values lie
-        if (!x.two) k1.step(C::kPer);
-        v0 = k0;
-        v1 = k1;
-        v0.step(kSpans);
-        v1.step(kSpans);
-        auto ahead = [&](Cursor<kRing>& c) {
-          c.step(C::kPer);
-          if (!x.two) c.step(C::kPer);
-        };
+        const int n = x.t1 - x.t0, n0 = x.two ? n : (n + 1) / 2, n1 = x.two ? n : n / 2, by = x.two ? 1 : 2;
+        Cursor<kKeyRing> k0 = key, k1 = key;              // where either accumulator's next keys and values lie
+        Cursor<kValRing> v0 = val, v1 = val;
+        if (!x.two) {
+          k1.step(C::kKeys);
+          v1.step(C::kVals);
+        }
         // w: accumulator; `last`: nobody else takes these pieces
-        auto scores = [&](int w, Cursor<kRing>& at, bool last) {
-          Cursor<kRing> c = at;
+        auto scores = [&](int w, Cursor<kKeyRing>& at, bool last) {
+          Cursor<kKeyRing> c = at;
 #pragma unroll
-          for (int h = 0; h < kSpans; ++h) {
-            if (!there(c)) return false;
+          for (int h = 0; h < C::kKeys; ++h) {
+            if (!mb::mbar_wait(&k_full[c.slot], c.parity, p.status, MB_ST_TIMEOUT_MMA)) return false;
             mb::tc_fence_after();
-            const uint64_t q = dQ + (x.two ? w : 0) * (kQB >> 4) + ((h * 16384) >> 4), k = dK + c.slot * (kPiece >> 4);
+            const uint64_t q = dQ + (x.two ? w : 0) * (kQB >> 4) + ((h * 16384) >> 4), k = dK + c.slot * (C::kKeyB >> 4);
+            if constexpr (FP8) {
 #pragma unroll
-            for (int s = 0; s < 4; ++s) mb::umma_f16(tmem + w * 128, q + ((s * 32) >> 4), k + ((s * 32) >> 4), kIdS, (h | s) != 0);
-            if (last) mb::tc_commit(&empty[c.slot]);
+              for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int s = 0; s < D / 32; ++s) mb::umma_f8f6f4(tmem + w * 128, q + ((t * 128 * D + s * 32) >> 4), k + ((s * 32) >> 4), kIdS, (t | s) != 0);
+            } else {
+#pragma unroll
+              for (int s = 0; s < 4; ++s) mb::umma_f16(tmem + w * 128, q + ((s * 32) >> 4), k + ((s * 32) >> 4), kIdS, (h | s) != 0);
+            }
+            if (last) mb::tc_commit(&k_empty[c.slot]);
             c.step();
           }
           mb::tc_commit(&s_full[w]);
-          ahead(at);
+          at.step(by * C::kKeys);
           return true;
         };
-        auto values = [&](int w, Cursor<kRing>& at, bool last, uint32_t done, bool fresh) {
-          Cursor<kRing> c = at;
+        auto values = [&](int w, Cursor<kValRing>& at, bool last, uint32_t done, bool fresh) {
+          Cursor<kValRing> c = at;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            if (!there(c) || !mb::mbar_wait(&p_full[w][h], done & 1, p.status, MB_ST_TIMEOUT_MMA)) return false;
+            if (!mb::mbar_wait(&v_full[c.slot], c.parity, p.status, MB_ST_TIMEOUT_MMA) ||
+                !mb::mbar_wait(&p_full[w][h], done & 1, p.status, MB_ST_TIMEOUT_MMA))
+              return false;
             mb::tc_fence_after();
-            const uint64_t v = dV + c.slot * (kPiece >> 4) + (kSpans == 1 ? h * 4 * (2048 >> 4) : 0);
+            const uint64_t v = dV + c.slot * (C::kValB >> 4) + (kSpans == 1 ? h * 4 * (2048 >> 4) : 0);
 #pragma unroll
             for (int s = 0; s < 4; ++s) umma_f16_ta(tmem + 256 + w * 128, tmem + w * 128 + (h * 4 + s) * 8, v + ((s * 2048) >> 4), kIdO, !(fresh && h == 0 && s == 0));
             if (h == 1 || kSpans == 2) {
-              if (last) mb::tc_commit(&empty[c.slot]);
+              if (last) mb::tc_commit(&v_empty[c.slot]);
               c.step();
             }
           }
-          ahead(at);
+          at.step(by * C::kVals);
           return true;
         };
         // rows are written, and the outputs of the part in front read
@@ -692,9 +748,8 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
           else mb::tc_commit(&o_full[1]);
         }
         mb::tc_commit(&q_free);
-        const int total = base.slot + n * C::kPer;
-        base.parity ^= (total / kRing) & 1;
-        base.slot = total % kRing;
+        key.step(n * C::kKeys);
+        val.step(n * C::kVals);
         done0 += n0;
         done1 += n1;
         ++part;
@@ -947,11 +1002,11 @@ int launch_prefix(const MbSharedArgs& a, const Ws& ws, cudaStream_t stream) {
     Boxes boxes{0};
     while (a.block_size % (16 >> boxes.bits)) ++boxes.bits;
     constexpr uint32_t row = FP8 ? D : 2 * D, width = row < 128 ? row : 128;
-    const CUtensorMapSwizzle sw = FP8 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B;
     CUtensorMap tm[4];
     for (int i = 0; i < (FP8 ? 2 : 4); ++i) {
       const int rc = mbh::encode_3d(&tm[i], CU_TENSOR_MAP_DATA_TYPE_UINT8, i & 1 ? a.v_cache : a.k_cache, row, a.Hkv, (uint64_t)a.num_blocks * a.block_size, row,
-                                    (uint64_t)a.Hkv * row, width, 1, i < 2 ? 16 >> boxes.bits : 1, sw);
+                                    (uint64_t)a.Hkv * row, width, 1, i < 2 ? 16 >> boxes.bits : 1,
+                                    FP8 && i == 1 ? CU_TENSOR_MAP_SWIZZLE_NONE : width == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B);
       if (rc) return rc;
     }
     if (FP8) tm[2] = tm[3] = tm[0];                        // not used

@@ -71,10 +71,16 @@ def _rows(cache, table, n, scale=None):
     return x.view(torch.float8_e4m3fn).double() * scale.double() if cache.dtype == torch.uint8 else x.double()
 
 
-def score_error(dim, size, kmax, scale):
-    """What a score may be off by, natural logarithm: a 32-bit sum of `dim` exact products whose sizes sum to `size`, each addition off by up to 2^-23 of that
-    (a matrix unit may cut instead of round), and the queries' f16 of e4m3 kernels (elements under 2^-14 of a row's scaled range are off by up to 2^-25)."""
-    return dim * 2.0 ** -23 * size + dim * 2.0 ** -25 * kmax * scale
+def score_error(q, k, scale, fp8):
+    """What scores [h, g, n] may be off by, natural logarithm, at most: a 32-bit sum of exact products, each addition off by up to 2^-23 of the sum of their
+    sizes (a matrix unit may cut instead of round); over an e4m3 cache queries are sums of two e4m3 numbers, exact but for elements that are less
+    than 2^-9 of the row's largest, which are off by 2^-17 of it or themselves."""
+    e = q.shape[-1] * 2.0 ** -23 * torch.einsum("hgd,nhd->hgn", q.abs(), k.abs()).nan_to_num(posinf=0.0).amax()
+    if fp8:
+        top = q.abs().amax(-1, keepdim=True)
+        off = torch.where(q.abs() < 2.0 ** -9 * top, torch.minimum(q.abs(), 2.0 ** -17 * top), 0.0)
+        e = e + torch.einsum("hgd,nhd->hgn", off, k.abs()).nan_to_num(posinf=0.0).amax()
+    return float(e) * scale
 
 
 def _softmax(z):
@@ -91,7 +97,6 @@ def shared_exact(c):
     out, tol = (torch.zeros(T, Hq, D, dtype=torch.float64) for _ in range(2))
     lse, ltol = torch.full((T, Hq), -math.inf, dtype=torch.float64), torch.zeros(T, Hq, dtype=torch.float64)
     start = c["start"].tolist()
-    kmax = 28.0 if c["k"].dtype == torch.uint8 else 0.0                       # the largest e4m3 value times the cases' scale
     for s in range(len(c["ctx"])):
         own = max(0, int(c["ctx"][s]))
         k, v = _rows(c["k"], c["table"][s], own, c["k_scale"]), _rows(c["v"], c["table"][s], own, c["v_scale"])
@@ -108,8 +113,7 @@ def shared_exact(c):
             q = c["q"][r].double().view(H, G, D)
             z = torch.einsum("hgd,nhd->hgn", q, k[:m]) * c["scale"]
             w, l = _softmax(z)
-            size = float(torch.einsum("hgd,nhd->hgn", q.abs(), k[:m].abs()).nan_to_num().max()) * c["scale"]
-            e = score_error(D, size, kmax, c["scale"]) + 2.0 ** -21          # and exponentials, of a row's own and of a join
+            e = score_error(q, k[:m], c["scale"], c["k"].dtype == torch.uint8) + 2.0 ** -21          # and exponentials, of a row's own and of a join
             o, a = torch.einsum("hgn,nhd->hgd", w, v[:m]), torch.einsum("hgn,nhd->hgd", w, v[:m].abs())
             out[r], lse[r] = o.reshape(Hq, D), l.reshape(Hq)
             # weights rounded to bf16 (f16 for an e4m3 cache: finer, but what is under 2^-24 of the largest is lost), then the result

@@ -79,6 +79,26 @@ def test_small_queries_over_an_e4m3_cache():
     check_shared(c)
 
 
+def test_queries_of_very_unequal_elements_over_an_e4m3_cache():
+    """One element a thousand and a million times the others: these are held to 2^-17 of it."""
+    for dim, kv_heads in ((64, 1), (128, 2), (256, 1)):
+        c = oracle.shared(34, [40, 3], [300], [0, 2], 8, kv_heads, dim, True)
+        c["q"][0, :, 5] *= 2.0 ** 10
+        c["q"][1, :, 7] *= 2.0 ** 20
+        check_shared(c)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_queries_that_are_no_numbers_over_an_e4m3_cache(dim):
+    c = oracle.shared(35, [20, 20, 20], [150], [0, 3], 4, 2, dim, True)
+    want = oracle.shared_exact(c)
+    c["q"][0, 1, 3], c["q"][2, 0, 0] = float("nan"), float("inf")
+    out, lse = run_shared(cuda(c))
+    assert bool(out[0, 1].isnan().all()) and bool(out[2, 0].isnan().all())
+    for r, h in ((0, 0), (0, 2), (1, 1), (2, 1), (2, 3)):
+        within(out[r, h], want[0][r, h], want[1][r, h], f"row {r}, head {h}")
+
+
 def test_more_sequences_than_a_launch_takes():
     n = 1100
     check_shared(oracle.shared(27, [1 + i % 5 for i in range(n)], [70], [0, n - 3], 4, 2, 64, False))
