@@ -2,7 +2,7 @@
 // as usual. Per head and pair 192 + 128 multiply-adds instead of the 576 + 512 of the absorbed form, for 512 x 256 a cached row and head in front.
 #include "common.cuh"
 #include "shared_attn.h"
-#include "softmax_rows.cuh"
+#include "attention_rows.cuh"
 #include "smem_limit.h"
 #include "tensormap.h"
 
@@ -199,13 +199,22 @@ mla_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       for (int c = 0; c < kT; c += 32) mb::tmem_ld32_async(tS + c, s + c);
       mb::tmem_ld_wait(s);
       const int seen = limit - j * kT;                    // columns below this are visible
-      const bool masked = !__all_sync(0xffffffffu, seen >= kT);
-      if (masked) {
+      if (!__all_sync(0xffffffffu, seen >= kT)) {
 #pragma unroll
         for (int i = 0; i < kT; ++i)
           if (i >= seen) s[i] = -INFINITY;
       }
-      auto rescale = [&](float alpha) {                   // S seen: the products that were issued in front of it are done
+      float mx4[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+      for (int i = 4; i < kT; ++i) mx4[i & 3] = fmaxf(mx4[i & 3], s[i]);
+      const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * sc;
+      float alpha = 1.f;
+      const bool move = mx > m_run + 8.f;                 // also true on a row's first finite tile
+      if (move) {
+        alpha = ex2(m_run - mx);                          // 0 when the row had seen nothing yet
+        m_run = mx;
+      }
+      if (j > 0 && __any_sync(0xffffffffu, move)) {       // S seen: the products that were issued in front of it are done
 #pragma unroll
         for (int c = 0; c < kV; c += 16) {
           float ov[16];
@@ -214,15 +223,28 @@ mla_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           for (int i = 0; i < 16; ++i) ov[i] *= alpha;
           mb::tmem_st16(tO + c, ov);
         }
-      };
-      auto publish = [&](int q, const uint32_t (&pk)[32]) {
+      }
+      const float nm = m_run == -INFINITY ? 0.f : -m_run;
+      const float2 sc2 = make_float2(sc, sc), nm2 = make_float2(nm, nm);
+      float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        uint32_t pk[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          float2 t = fma2(make_float2(s[q * 64 + 2 * i], s[q * 64 + 2 * i + 1]), sc2, nm2);
+          t.x = ex2(t.x);
+          t.y = ex2(t.y);
+          sum[i & 1] = add2(sum[i & 1], t);
+          pk[i] = pack2<false>(t.x, t.y);
+        }
         tmem_st32(tS + q * 32, pk);
         mb::tmem_st_wait();
         mb::tc_fence_before();
         __syncwarp();
         if (lane == 0) mb::mbar_arrive(&p_full[w][q]);
-      };
-      softmax_tile<false, 0>(s, sc, 0.f, j == 0, masked, m_run, l_run, rescale, publish);
+      }
+      l_run = l_run * alpha + ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y));
     }
     // the first cached token that is no number, of those that the tile sees: it lies in the expanded rows as zeros
     int bad = 0x7fffffff;

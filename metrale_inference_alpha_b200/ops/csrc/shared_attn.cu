@@ -18,6 +18,8 @@ Ws workspace(const MbSharedArgs& a) {
   Ws w{};
   const size_t rows = (size_t)a.num_seqs * a.q_len * (a.Hq / a.Hkv), all = rows * a.Hkv, tokens = (size_t)a.num_seqs * a.q_len;
   w.ctas = a.sm_count > 0 ? a.sm_count : 148;
+  w.G = a.Hq / a.Hkv;
+  w.per_seq = a.q_len * w.G;
   auto take = [&](size_t bytes) {
     const size_t at = w.bytes;
     w.bytes += (bytes + 255) & ~size_t(255);
@@ -56,13 +58,13 @@ __global__ void __launch_bounds__(256) shared_join_kernel(const MbSharedArgs p, 
   __shared__ Plan plan;
   __shared__ float4 s_o[8][kJoinDims / 4][32];
   __shared__ float2 s_ml[8][32];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = p.Hq / p.Hkv, kvh = blockIdx.y;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = ws.G, kvh = blockIdx.y;
   constexpr int kC = kJoinDims / 4;
   const int c0 = blockIdx.z * kC;                          // fours of dims
-  mb::pdl_wait();
+  // What is planned by stood before the kernels in front, which have waited for it before they let this one come up: only what they write is waited for
   const bool prefixes = p.groups > 0 && p.max_prefix > 0;
   if (prefixes) {
-    if (warp == 0) make_plan<D>(p, plan, lane);
+    if (warp == 0) make_plan<D>(p, plan, ws.per_seq, lane);
     __syncthreads();
   }
   const int R = blockIdx.x * 32 + lane;                    // of the step's rows
@@ -93,6 +95,7 @@ __global__ void __launch_bounds__(256) shared_join_kernel(const MbSharedArgs p, 
     own = max(0, own - p.q_len + (tok - seq * p.q_len) + 1);
     own_parts = own > 0 ? own_part_count(own, part_tokens_of(p.Hkv, D)) : 0;
   }
+  mb::pdl_wait();
   int at_warp = warp;                                      // this warp's next part of those that come
   if (live && prefixes && seq >= plan.start[0] && seq < plan.start[p.groups]) {
     int lo = 0, hi = p.groups;                             // start[lo] <= seq < start[hi]
@@ -101,7 +104,7 @@ __global__ void __launch_bounds__(256) shared_join_kernel(const MbSharedArgs p, 
       if (plan.start[mid] <= seq) lo = mid;
       else hi = mid;
     }
-    const int rows = row_count(p, plan, lo), tiles = (plan.len[lo] + Shape<D>::kT - 1) / Shape<D>::kT;
+    const int rows = row_count(plan, lo, ws.per_seq), tiles = (plan.len[lo] + Shape<D>::kT - 1) / Shape<D>::kT;
     if (tiles > 0) {
       const int row = (tok - plan.start[lo] * p.q_len) * G + head;
       int doubles, singles;

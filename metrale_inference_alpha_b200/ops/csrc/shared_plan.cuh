@@ -27,7 +27,7 @@ struct Plan {
   int base[kMaxGroups + 1];
 };
 
-__device__ __forceinline__ int row_count(const MbSharedArgs& p, const Plan& s, int g) { return (s.start[g + 1] - s.start[g]) * p.q_len * (p.Hq / p.Hkv); }
+__device__ __forceinline__ int row_count(const Plan& s, int g, int per_seq) { return (s.start[g + 1] - s.start[g]) * per_seq; }      // per_seq: rows of a sequence
 
 // units of a group for a kv head: double ones, and single ones behind them
 template <int D>
@@ -50,8 +50,22 @@ __device__ __forceinline__ int line_of_head(int rows, int tiles) {
 
 // by one warp
 template <int D>
-__device__ __forceinline__ void make_plan(const MbSharedArgs& p, Plan& s, int lane) {
-  int top = 0;
+__device__ __forceinline__ void make_plan(const MbSharedArgs& p, Plan& s, int per_seq, int lane) {
+  if (p.groups == 1) {                                     // the usual call, without the sums over groups
+    const int a = p.group_start[0], b = p.group_start[1], n = p.prefix_len[0];
+    const int first = min(max(a, 0), p.num_seqs), next = max(first, min(max(b, 0), p.num_seqs));
+    const int len = next > first ? min(max(n, 0), p.max_prefix) : 0;
+    if (lane == 0) {
+      if (p.status && (a < 0 || b > p.num_seqs || b < a || (next > first && n > p.max_prefix))) atomicCAS(p.status, 0u, MB_ST_BOUNDS);
+      s.start[0] = first;
+      s.start[1] = next;
+      s.len[0] = len;
+      s.base[0] = 0;
+      s.base[1] = p.Hkv * line_of_head<D>((next - first) * per_seq, (len + Shape<D>::kT - 1) / Shape<D>::kT);
+    }
+    return;
+  }
+  int top = 0, len0 = lane < p.groups ? p.prefix_len[lane] : 0;            // asked for beside the first sequences
   for (int g0 = 0; g0 <= p.groups; g0 += 32) {
     const int g = g0 + lane;
     int a = 0;
@@ -76,14 +90,14 @@ __device__ __forceinline__ void make_plan(const MbSharedArgs& p, Plan& s, int la
     const int g = g0 + lane;
     int n = 0;
     if (g < p.groups) {
-      int len = max(p.prefix_len[g], 0);
+      int len = max(g0 == 0 ? len0 : p.prefix_len[g], 0);
       if (s.start[g + 1] <= s.start[g]) len = 0;
       if (len > p.max_prefix) {
         if (p.status) atomicCAS(p.status, 0u, MB_ST_BOUNDS);
         len = p.max_prefix;
       }
       s.len[g] = len;
-      n = p.Hkv * line_of_head<D>(row_count(p, s, g), (len + Shape<D>::kT - 1) / Shape<D>::kT);
+      n = p.Hkv * line_of_head<D>(row_count(s, g, per_seq), (len + Shape<D>::kT - 1) / Shape<D>::kT);
     }
     int x = n;
 #pragma unroll
@@ -118,25 +132,36 @@ __device__ __forceinline__ void tiles_in(int at, int tiles, int two, int b0, int
   t1 = (min(max(b1 - at, 0), tiles << two) + two) >> two;
 }
 
+// a / b for quotients below 2^20, by a product that is off by one at most
+__device__ __forceinline__ unsigned quotient(unsigned a, unsigned b) {
+  unsigned q = (unsigned)(__uint2float_rn(a) * __fdividef(1.f, __uint2float_rn(b)));
+  int r = (int)(a - q * b);
+  if (r < 0) {
+    --q;
+    r += b;
+  }
+  return r >= (int)b ? q + 1 : q;
+}
+
 // The part at `pos`, which moves behind it; false at the end. Parts without tiles are left out.
 template <int D>
-__device__ __forceinline__ bool next_part(const MbSharedArgs& p, const Plan& s, int& pos, int end, Part& x) {
+__device__ __forceinline__ bool next_part(const Plan& s, int groups, int per_seq, int& pos, int end, Part& x) {
   while (pos < end) {
-    int lo = 0, hi = p.groups;             // base[lo] <= pos < base[hi]
+    int lo = 0, hi = groups;               // base[lo] <= pos < base[hi]
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
       if (s.base[mid] <= pos) lo = mid;
       else hi = mid;
     }
     x.group = lo;
-    const int rows = row_count(p, s, lo), tiles = (s.len[lo] + Shape<D>::kT - 1) / Shape<D>::kT;
+    const int rows = row_count(s, lo, per_seq), tiles = (s.len[lo] + Shape<D>::kT - 1) / Shape<D>::kT;
     int doubles, singles;
     unit_count<D>(rows, doubles, singles);
     const unsigned head = (unsigned)tiles * (2 * doubles + singles), in = pos - s.base[lo];
-    x.kvh = in / head;
+    x.kvh = quotient(in, head);
     const unsigned w = in - x.kvh * head, d = 2u * tiles * doubles;
     x.two = w < d;
-    const unsigned size = (unsigned)tiles << x.two, v = x.two ? w : w - d, u = v / size;
+    const unsigned size = (unsigned)tiles << x.two, v = x.two ? w : w - d, u = quotient(v, size);
     x.row0 = x.two ? u * 256 : doubles * 256 + u * 128;
     const int at = pos - (int)(v - u * size);
     x.rows = min(rows - x.row0, x.two ? 256 : 128);
@@ -152,6 +177,7 @@ __device__ __forceinline__ bool next_part(const MbSharedArgs& p, const Plan& s, 
 struct Ws {
   size_t first, first_ml, rest, rest_ml, own, own_ml, bytes;
   int ctas, parts, step;                   // parts of a sequence's own rows; tokens whose own rows are attended at once
+  int G, per_seq;                          // query heads of a group, rows of a sequence
 };
 
 }  // namespace mbs

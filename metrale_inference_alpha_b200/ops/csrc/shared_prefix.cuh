@@ -41,7 +41,7 @@ struct Place {
 };
 template <int D>
 __device__ __forceinline__ Place place_first(const MbSharedArgs& p, const Ws& w, const Plan& s, int group, int kvh, int row, int side) {
-  const size_t R = (size_t)p.num_seqs * p.q_len * (p.Hq / p.Hkv), at = (size_t)s.start[group] * p.q_len * (p.Hq / p.Hkv) + row, h = (size_t)side * p.Hkv + kvh;
+  const size_t R = (size_t)p.num_seqs * w.per_seq, at = (size_t)s.start[group] * w.per_seq + row, h = (size_t)side * p.Hkv + kvh;
   uint8_t* ws = reinterpret_cast<uint8_t*>(p.ws);
   return {reinterpret_cast<float4*>(ws + w.first) + h * (D / 4) * R + at, reinterpret_cast<float2*>(ws + w.first_ml) + h * R + at, R};
 }
@@ -102,35 +102,45 @@ __device__ __forceinline__ uint4 query_piece(uint4 v, float& scale) {
   return v;
 }
 
-// Eight dims of a query row as two e4m3 numbers each, for keys of e4m3; lanes of a row are D / 8 neighbours
+// A query row as two e4m3 numbers an element, for keys of e4m3, to `dst` (two tiles of 128 rows of D bytes) where `store`; returns what its scores are too large by
 template <int D>
-__device__ __forceinline__ void query_pair(uint4 v, uint2 (&out)[2], float& scale) {
-  const uint32_t x[4] = {v.x, v.y, v.z, v.w};
+__device__ __forceinline__ float query_pairs(const uint4 (&v)[D / 8], uint8_t* dst, int r, bool store) {
   uint32_t top = 0;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) top = __vmaxu2(top, x[j] & 0x7fff7fffu);       // bf16 bits without the sign order like the values
-#pragma unroll
-  for (int d = 1; d < D / 8; d <<= 1) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, d));
-  const int e = (int)(max(top & 0xffff, top >> 16) >> 7), up = e == 255 ? 0 : 134 - max(e, 8);
-  const float f = __int_as_float((127 + up) << 23);
-  uint32_t h[2][4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    float2 y = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&x[j]));
-    y.x *= f;
-    y.y *= f;
-    if (e == 255) {                                        // the type has no infinities: they become NaN
-      if (isinf(y.x)) y.x = __int_as_float(0x7fffffff);
-      if (isinf(y.y)) y.y = __int_as_float(0x7fffffff);
-    }
-    h[0][j] = __nv_cvt_float2_to_fp8x2(y, __NV_SATFINITE, __NV_E4M3);
-    const uint32_t back = e4m3x2(h[0][j]);
-    const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&back));
-    h[1][j] = __nv_cvt_float2_to_fp8x2(make_float2(y.x - b.x, y.y - b.y), __NV_SATFINITE, __NV_E4M3);
+  for (int c = 0; c < D / 8; ++c) {                        // bf16 bits without the sign order like the values
+    top = __vmaxu2(top, __vmaxu2(v[c].x & 0x7fff7fffu, v[c].y & 0x7fff7fffu));
+    top = __vmaxu2(top, __vmaxu2(v[c].z & 0x7fff7fffu, v[c].w & 0x7fff7fffu));
   }
+  const int e = (int)(max(top & 0xffff, top >> 16) >> 7), up = e == 255 ? 0 : 134 - max(e, 8);
+  if (store) {
+    const float f = __int_as_float((127 + up) << 23);
+    const bool odd = e == 255;                             // the type has no infinities: they become NaN
 #pragma unroll
-  for (int t = 0; t < 2; ++t) out[t] = make_uint2(h[t][0] | h[t][1] << 16, h[t][2] | h[t][3] << 16);
-  scale = __int_as_float((127 - up) << 23);
+    for (int c = 0; c < D / 16; ++c) {
+      uint32_t h[2][4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint32_t pair[2][2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const uint4& src = v[2 * c + (j >> 1)];
+          const uint32_t x = (j & 1) ? (k ? src.w : src.z) : (k ? src.y : src.x);
+          float2 y = make_float2(__uint_as_float(x << 16) * f, __uint_as_float(x & 0xffff0000u) * f);
+          if (odd) y = make_float2(y.x - y.x + y.x, y.y - y.y + y.y);
+          pair[0][k] = __nv_cvt_float2_to_fp8x2(y, __NV_SATFINITE, __NV_E4M3);
+          const uint32_t back = e4m3x2(pair[0][k]);
+          const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&back));
+          pair[1][k] = __nv_cvt_float2_to_fp8x2(make_float2(y.x - b.x, y.y - b.y), __NV_SATFINITE, __NV_E4M3);
+        }
+        h[0][j] = pair[0][0] | pair[0][1] << 16;
+        h[1][j] = pair[1][0] | pair[1][1] << 16;
+      }
+      const int at = r * D + ((D == 128 ? c ^ (r & 7) : c ^ ((r >> 1) & 3)) << 4);
+#pragma unroll
+      for (int t = 0; t < 2; ++t) *reinterpret_cast<uint4*>(dst + t * (128 * D) + at) = make_uint4(h[t][0], h[t][1], h[t][2], h[t][3]);
+    }
+  }
+  return __int_as_float((127 - up) << 23);
 }
 
 // Operand rows of 64 bytes: pieces of 16 bytes exchanged by (row / 2) mod 4, eight rows 512 bytes
@@ -146,7 +156,7 @@ __device__ __forceinline__ uint64_t umma_desc_sw64(uint32_t saddr) {
 
 // K and V tiles of kT cached tokens of this CTA's parts, one after the other, into two stages each: 128 threads, t the number of this one
 template <int D, bool FP8, int kT>
-__device__ __forceinline__ void load_tiles(const MbSharedArgs& p, const Plan& plan, int begin, int end, uint8_t* sK, uint8_t* sV, uint64_t* k_full,
+__device__ __forceinline__ void load_tiles(const MbSharedArgs& p, const Ws& ws, const Plan& plan, int begin, int end, uint8_t* sK, uint8_t* sV, uint64_t* k_full,
                                            uint64_t* k_empty, uint64_t* v_full, uint64_t* v_empty, int t) {
   constexpr int kTileB = kT * D * 2;
   const int lane = t & 31;
@@ -164,7 +174,7 @@ __device__ __forceinline__ void load_tiles(const MbSharedArgs& p, const Plan& pl
   int bad = 0;
   auto places = [&](int* place, size_t& off) {
     if (more && at == x.t1) {
-      more = next_part<D>(p, plan, pos, end, x);
+      more = next_part<D>(plan, p.groups, ws.per_seq, pos, end, x);
       at = x.t0;
     }
     if (!more) {
@@ -339,11 +349,10 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
   __shared__ __align__(8) uint64_t q_full[2], q_free, k_full[kKeyRing], k_empty[kKeyRing], v_full[kValRing], v_empty[kValRing], raw_full[kRaw], raw_empty[kRaw], s_full[2],
       p_full[2][2], o_full[2];
   __shared__ uint32_t s_tmem;
-  __shared__ float s_qscale[FP8 ? 2 : 1][2][128];         // what a row's scores are too large by (e4m3 cache), of parts in turn
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = p.Hq / p.Hkv;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = ws.G;
   mb::pdl_wait();
   if (warp == 0) {
-    make_plan<D>(p, plan, lane);
+    make_plan<D>(p, plan, ws.per_seq, lane);
   } else if (warp == 1 && lane == 0) {
     mb::mbar_init(&q_free, 1);
     for (int i = 0; i < 2; ++i) {
@@ -390,55 +399,34 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
     const float sc0 = p.scale * (FP8 ? *p.k_scale : 1.f) * 1.44269504088896f;
     uint32_t part = 0, done = 0, outs = 0;                // parts, tiles and outputs that this accumulator has had
     bool ok = true;
-    while (ok && next_part<D>(p, plan, pos, end, x)) {
+    while (ok && next_part<D>(plan, p.groups, ws.per_seq, pos, end, x)) {
       const int n = x.t1 - x.t0, mine = x.two ? n : (n + 1 - w) / 2;
       // a wait tells a phase from its neighbours only: no warp may be two parts ahead of one that waits, so every part's queries wait for all products
       // of the former one's
       if (part > 0) ok = mb::mbar_wait(&q_free, (part - 1) & 1, p.status, MB_ST_TIMEOUT_MMA);
       if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-      if (x.two || w == 0) {
-        // 128 rows x D / 8 pieces of 8 dims, a thread's loads in flight together (rows past the last one read it again and become zeros)
-        constexpr int kPieces = D / 8, kQ = kPieces, kStep = 128 / kPieces;
-        const int c = r % kPieces, first = r / kPieces, last = x.rows - w * 128 - 1;
-        uint4 v[kQ];
-        QueryRow at(p, x, G, plan.start[x.group] * p.q_len, w * 128 + min(first, last), kStep);
+      // A thread's own row, whole (past the last one zeros, which leave no weight out of range). Where the accumulators share the rows the first one's
+      // threads bring them; the others need what the scores are too large by.
+      const int side = x.two ? w : 0, row = side * 128 + r;
+      float sc = sc0;
+      {
+        QueryRow at(p, x, G, plan.start[x.group] * p.q_len, min(row, x.rows - 1), 1);
+        const uint4* src = reinterpret_cast<const uint4*>(at.row(D));
+        uint4 v[D / 8];
 #pragma unroll
-        for (int i = 0; i < kQ; ++i) {
-          v[i] = *(reinterpret_cast<const uint4*>(at.row(D)) + c);
-          if (first + kStep * (i + 1) <= last) at.step();
-        }
+        for (int c = 0; c < D / 8; ++c) v[c] = row < x.rows ? src[c] : make_uint4(0, 0, 0, 0);
+        if constexpr (FP8) {
+          sc *= query_pairs<D>(v, sQ + w * kQB, r, side == w);
+        } else {
+          if (side == w) {
 #pragma unroll
-        for (int i = 0; i < kQ; ++i) {
-          const int qr = first + kStep * i;
-          if (qr > last) v[i] = make_uint4(0, 0, 0, 0);
-          if constexpr (FP8) {
-            float back;
-            uint2 h[2];
-            query_pair<D>(v[i], h, back);
-            if (c == 0) s_qscale[part & 1][w][qr] = back;
-            const int at16 = D == 128 ? (c >> 1) ^ (qr & 7) : (c >> 1) ^ ((qr >> 1) & 3);
-#pragma unroll
-            for (int t = 0; t < 2; ++t) *reinterpret_cast<uint2*>(sQ + w * kQB + t * (128 * D) + qr * D + at16 * 16 + (c & 1) * 8) = h[t];
-          } else {
-            *reinterpret_cast<uint4*>(sQ + w * kQB + (c >> 3) * (128 * 128) + sw_off(qr, c & 7)) = v[i];
+            for (int c = 0; c < D / 8; ++c) *reinterpret_cast<uint4*>(sQ + w * kQB + (c >> 3) * (128 * 128) + sw_off(r, c & 7)) = v[c];
           }
         }
         fence_async_smem();
       }
-      // where the rows are those of the other accumulator, their arrival is seen before this one's is announced
-      const int side = x.two ? w : 0;                     // whose rows these are
-      if (side != w) {
-        ok = mb::mbar_wait(&q_full[side], part & 1, p.status, MB_ST_TIMEOUT_MMA);
-        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-      }
       __syncwarp();
       if (lane == 0) mb::mbar_arrive(&q_full[w]);
-      float sc = sc0;
-      if constexpr (FP8) {                                // the rows' scales come from other softmax warps
-        if (side == w) ok = mb::mbar_wait(&q_full[w], part & 1, p.status, MB_ST_TIMEOUT_MMA);
-        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-        sc *= s_qscale[part & 1][side][r];
-      }
       const int left = x.two ? x.rows - w * 128 : x.rows; // rows of this tile
       const bool live = r < left, some = (warp & 3) * 32 < left;
       const int len = plan.len[x.group];
@@ -458,11 +446,6 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
         __syncwarp();
         if (lane == 0) mb::mbar_arrive(&p_full[w][h]);
       };
-      auto publish = [&](int h, const uint32_t (&pk)[32]) {
-        tmem_st32(tS + h * 32, pk);
-        mb::tmem_st_wait();
-        announce(h);
-      };
       for (int i = 0; i < mine; ++i) {
         const int t = x.t0 + (x.two ? i : 2 * i + w);
         ok = mb::mbar_wait(&s_full[w], (done + i) & 1, p.status, MB_ST_TIMEOUT_MMA);
@@ -473,17 +456,7 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
           announce(1);
           continue;
         }
-        float s[kT];
-#pragma unroll
-        for (int c = 0; c < kT; c += 32) mb::tmem_ld32_async(tS + c, s + c);
-        mb::tmem_ld_wait(s);
-        const int seen = len - t * kT;                    // columns below this are cached tokens
-        if (seen < kT) {
-#pragma unroll
-          for (int k = 0; k < kT; ++k)
-            if (k >= seen) s[k] = -INFINITY;
-        }
-        softmax_tile<FP8, 5>(s, sc, FP8 ? kLift : 0.f, i == 0, seen < kT, m_run, l_run, rescale, publish);
+        softmax_tile<FP8>(tS, len - t * kT, sc, FP8 ? kLift : 0.f, i == 0, m_run, l_run, rescale, announce);
       }
       if (!ok) break;
       if (mine > 0) {
@@ -525,7 +498,7 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
       uint32_t keys_asked = 0, vals_asked = 0, key_parities = 0, val_parities = 0;      // slots that this warp has filled, with which parity the last time
       bool ok = true;
       int bad = 0;
-      while (ok && next_part<D>(p, plan, pos, end, x)) {
+      while (ok && next_part<D>(plan, p.groups, ws.per_seq, pos, end, x)) {
         const int len = plan.len[x.group];
         const int* bt = p.prefix_table + (size_t)x.group * p.prefix_ld;
         // a tile's boxes: lane l has boxes l, l + 32, ...; looked up a tile ahead
@@ -625,7 +598,7 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
         Cursor<kRaw> raw;
         Cursor<kValRing> at;
         bool ok = true;
-        while (ok && next_part<D>(p, plan, pos, end, x)) {
+        while (ok && next_part<D>(plan, p.groups, ws.per_seq, pos, end, x)) {
           const int len = plan.len[x.group];
 #pragma unroll 1
           for (int t = x.t0; t < x.t1 && ok; ++t) {
@@ -681,7 +654,7 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
       Cursor<kValRing> val;
       uint32_t part = 0, done0 = 0, done1 = 0;            // parts, tiles that either accumulator has had
       bool ok = true;
-      while (ok && next_part<D>(p, plan, pos, end, x)) {
+      while (ok && next_part<D>(plan, p.groups, ws.per_seq, pos, end, x)) {
         const int n = x.t1 - x.t0, n0 = x.two ? n : (n + 1) / 2, n1 = x.two ? n : n / 2, by = x.two ? 1 : 2;
         Cursor<kKeyRing> k0 = key, k1 = key;              // where either accumulator's next keys and values lie
         Cursor<kValRing> v0 = val, v1 = val;
@@ -777,10 +750,10 @@ __global__ void __launch_bounds__(288, 1) shared_prefix256_kernel(const MbShared
   __shared__ __align__(8) uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_done, o_full;
   __shared__ uint32_t s_tmem;
   __shared__ float s_qscale[2][128];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = p.Hq / p.Hkv;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = ws.G;
   mb::pdl_wait();
   if (warp == 0) {
-    make_plan<D>(p, plan, lane);
+    make_plan<D>(p, plan, ws.per_seq, lane);
   } else if (warp == 1 && lane == 0) {
     mb::mbar_init(&q_full, 4);
     mb::mbar_init(&o_done, 1);
@@ -815,7 +788,7 @@ __global__ void __launch_bounds__(288, 1) shared_prefix256_kernel(const MbShared
     bool ok = true;
     int pos = begin;
     Part x;
-    while (ok && next_part<D>(p, plan, pos, end, x)) {
+    while (ok && next_part<D>(plan, p.groups, ws.per_seq, pos, end, x)) {
       const int n = x.t1 - x.t0, last = x.rows - 1;
       // 128 rows x 32 pieces of 8 dims, sixteen of a thread's loads in flight together (rows past the last one are zeros)
 #pragma unroll 1
@@ -931,7 +904,7 @@ __global__ void __launch_bounds__(288, 1) shared_prefix256_kernel(const MbShared
       ++part;
     }
   } else if (warp < 8) {
-    load_tiles<D, FP8, kT>(p, plan, begin, end, sK, sV, k_full, k_empty, v_full, v_empty, tid - 128);
+    load_tiles<D, FP8, kT>(p, ws, plan, begin, end, sK, sV, k_full, k_empty, v_full, v_empty, tid - 128);
   } else {
     if (mb::elect_one()) {
       // ---------------------------------------------------------- products
@@ -955,7 +928,7 @@ __global__ void __launch_bounds__(288, 1) shared_prefix256_kernel(const MbShared
         mb::tc_commit(&k_empty[j & 1]);
         return true;
       };
-      while (ok && next_part<D>(p, plan, pos, end, x)) {
+      while (ok && next_part<D>(plan, p.groups, ws.per_seq, pos, end, x)) {
         const int n = x.t1 - x.t0;
         ok = mb::mbar_wait(&q_full, part & 1, p.status, MB_ST_TIMEOUT_MMA) && scores(base);
         for (int i = 0; i < n && ok; ++i) {
@@ -995,7 +968,7 @@ int launch_prefix(const MbSharedArgs& a, const Ws& ws, cudaStream_t stream) {
     constexpr int smem = 128 * D * 2 + 4 * 64 * D * 2 + 1024 + (int)sizeof(Plan);
     const cudaError_t e = mb::allow_smem(reinterpret_cast<const void*>(kern), smem, asked);
     if (e != cudaSuccess) return (int)e;
-    return (int)mb::launch_kernel(kern, dim3(ws.ctas), dim3(288), smem, stream, a, ws);
+    return (int)mb::launch_kernel_ex(kern, dim3(ws.ctas), dim3(288), smem, stream, 1, mb_pdl_enabled() != 0, a, ws);
   } else {
     using C = PrefixCfg<D, FP8>;
     auto kern = shared_prefix_kernel<D, FP8>;
@@ -1012,7 +985,7 @@ int launch_prefix(const MbSharedArgs& a, const Ws& ws, cudaStream_t stream) {
     if (FP8) tm[2] = tm[3] = tm[0];                        // not used
     const cudaError_t e = mb::allow_smem(reinterpret_cast<const void*>(kern), C::kSmem, asked);
     if (e != cudaSuccess) return (int)e;
-    return (int)mb::launch_kernel(kern, dim3(ws.ctas), dim3(C::kThreads), C::kSmem, stream, tm[0], tm[1], tm[2], tm[3], boxes, a, ws);
+    return (int)mb::launch_kernel_ex(kern, dim3(ws.ctas), dim3(C::kThreads), C::kSmem, stream, 1, mb_pdl_enabled() != 0, tm[0], tm[1], tm[2], tm[3], boxes, a, ws);
   }
 }
 
