@@ -102,43 +102,46 @@ __device__ __forceinline__ uint4 query_piece(uint4 v, float& scale) {
   return v;
 }
 
-// A query row as two e4m3 numbers an element, for keys of e4m3, to `dst` (two tiles of 128 rows of D bytes) where `store`; returns what its scores are too large by
+// Byte offset of 16-byte piece c of row r of an operand of e4m3 numbers, whose rows are D bytes
 template <int D>
-__device__ __forceinline__ float query_pairs(const uint4 (&v)[D / 8], uint8_t* dst, int r, bool store) {
-  uint32_t top = 0;
-#pragma unroll
-  for (int c = 0; c < D / 8; ++c) {                        // bf16 bits without the sign order like the values
-    top = __vmaxu2(top, __vmaxu2(v[c].x & 0x7fff7fffu, v[c].y & 0x7fff7fffu));
-    top = __vmaxu2(top, __vmaxu2(v[c].z & 0x7fff7fffu, v[c].w & 0x7fff7fffu));
+__device__ __forceinline__ uint32_t query_slot(int r, int c) {
+  return (uint32_t)(r * D + ((D == 128 ? c ^ (r & 7) : c ^ ((r >> 1) & 3)) << 4));
+}
+
+// A query row as two e4m3 numbers an element, for keys of e4m3, in two tiles of 128 rows of D bytes. Sixteen elements come from the two places that their
+// numbers go to. Returns what the row's scores are too large by.
+template <int D>
+__device__ __forceinline__ float query_pairs(uint8_t* tile, int r) {
+  uint32_t top = 0;                                        // bf16 bits without the sign order like the values
+#pragma unroll 4
+  for (int c = 0; c < D / 8; ++c) {
+    const uint4 v = *reinterpret_cast<const uint4*>(tile + (c & 1) * (128 * D) + query_slot<D>(r, c >> 1));
+    top = __vmaxu2(top, __vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu));
+    top = __vmaxu2(top, __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu));
   }
   const int e = (int)(max(top & 0xffff, top >> 16) >> 7), up = e == 255 ? 0 : 134 - max(e, 8);
-  if (store) {
-    const float f = __int_as_float((127 + up) << 23);
-    const bool odd = e == 255;                             // the type has no infinities: they become NaN
+  const float f = __int_as_float((127 + up) << 23);
+#pragma unroll 1
+  for (int c = 0; c < D / 16; ++c) {
+    uint8_t *a = tile + query_slot<D>(r, c), *b = a + 128 * D;
+    const uint4 va = *reinterpret_cast<const uint4*>(a), vb = *reinterpret_cast<const uint4*>(b);
+    const uint32_t x[8] = {va.x, va.y, va.z, va.w, vb.x, vb.y, vb.z, vb.w};
+    uint32_t h[2][4] = {};
 #pragma unroll
-    for (int c = 0; c < D / 16; ++c) {
-      uint32_t h[2][4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        uint32_t pair[2][2];
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const uint4& src = v[2 * c + (j >> 1)];
-          const uint32_t x = (j & 1) ? (k ? src.w : src.z) : (k ? src.y : src.x);
-          float2 y = make_float2(__uint_as_float(x << 16) * f, __uint_as_float(x & 0xffff0000u) * f);
-          if (odd) y = make_float2(y.x - y.x + y.x, y.y - y.y + y.y);
-          pair[0][k] = __nv_cvt_float2_to_fp8x2(y, __NV_SATFINITE, __NV_E4M3);
-          const uint32_t back = e4m3x2(pair[0][k]);
-          const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&back));
-          pair[1][k] = __nv_cvt_float2_to_fp8x2(make_float2(y.x - b.x, y.y - b.y), __NV_SATFINITE, __NV_E4M3);
-        }
-        h[0][j] = pair[0][0] | pair[0][1] << 16;
-        h[1][j] = pair[1][0] | pair[1][1] << 16;
+    for (int j = 0; j < 8; ++j) {
+      float2 y = make_float2(__uint_as_float(x[j] << 16) * f, __uint_as_float(x[j] & 0xffff0000u) * f);
+      if (e == 255) {                                      // the type has no infinities: they become NaN
+        if (isinf(y.x)) y.x = __int_as_float(0x7fffffff);
+        if (isinf(y.y)) y.y = __int_as_float(0x7fffffff);
       }
-      const int at = r * D + ((D == 128 ? c ^ (r & 7) : c ^ ((r >> 1) & 3)) << 4);
-#pragma unroll
-      for (int t = 0; t < 2; ++t) *reinterpret_cast<uint4*>(dst + t * (128 * D) + at) = make_uint4(h[t][0], h[t][1], h[t][2], h[t][3]);
+      const uint32_t one = __nv_cvt_float2_to_fp8x2(y, __NV_SATFINITE, __NV_E4M3), back = e4m3x2(one);
+      const float2 z = __half22float2(*reinterpret_cast<const __half2*>(&back));
+      const uint32_t two = __nv_cvt_float2_to_fp8x2(make_float2(y.x - z.x, y.y - z.y), __NV_SATFINITE, __NV_E4M3);
+      h[0][j >> 1] |= one << (16 * (j & 1));
+      h[1][j >> 1] |= two << (16 * (j & 1));
     }
+    *reinterpret_cast<uint4*>(a) = make_uint4(h[0][0], h[0][1], h[0][2], h[0][3]);
+    *reinterpret_cast<uint4*>(b) = make_uint4(h[1][0], h[1][1], h[1][2], h[1][3]);
   }
   return __int_as_float((127 - up) << 23);
 }
@@ -346,9 +349,10 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
   uint8_t* sV = sK + kKeyRing * C::kKeyB;
   uint8_t* sB = sV + kValRing * C::kValB;
   Plan& plan = *reinterpret_cast<Plan*>(sB + C::kRawRing * C::kRawB);
-  __shared__ __align__(8) uint64_t q_full[2], q_free, k_full[kKeyRing], k_empty[kKeyRing], v_full[kValRing], v_empty[kValRing], raw_full[kRaw], raw_empty[kRaw], s_full[2],
+  __shared__ __align__(8) uint64_t q_full[2], q_raw[2], q_free, k_full[kKeyRing], k_empty[kKeyRing], v_full[kValRing], v_empty[kValRing], raw_full[kRaw], raw_empty[kRaw], s_full[2],
       p_full[2][2], o_full[2];
   __shared__ uint32_t s_tmem;
+  __shared__ float s_qscale[FP8 ? 2 : 1][2][128];         // what a row's scores are too large by (e4m3 cache), of parts in turn
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = ws.G;
   mb::pdl_wait();
   if (warp == 0) {
@@ -357,6 +361,7 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
     mb::mbar_init(&q_free, 1);
     for (int i = 0; i < 2; ++i) {
       mb::mbar_init(&q_full[i], 4);
+      mb::mbar_init(&q_raw[i], 4);
       mb::mbar_init(&s_full[i], 1);
       mb::mbar_init(&p_full[i][0], 4);
       mb::mbar_init(&p_full[i][1], 4);
@@ -397,7 +402,7 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t tS = tmem + lanes + w * 128, tO = tmem + lanes + 256 + w * 128;
     const float sc0 = p.scale * (FP8 ? *p.k_scale : 1.f) * 1.44269504088896f;
-    uint32_t part = 0, done = 0, outs = 0;                // parts, tiles and outputs that this accumulator has had
+    uint32_t part = 0, done = 0, outs = 0, raws = 0;      // parts, tiles, outputs and query tiles that this accumulator has had
     bool ok = true;
     while (ok && next_part<D>(plan, p.groups, ws.per_seq, pos, end, x)) {
       const int n = x.t1 - x.t0, mine = x.two ? n : (n + 1 - w) / 2;
@@ -405,30 +410,49 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
       // of the former one's
       if (part > 0) ok = mb::mbar_wait(&q_free, (part - 1) & 1, p.status, MB_ST_TIMEOUT_MMA);
       if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-      // A thread's own row, whole (past the last one zeros, which leave no weight out of range). Where the accumulators share the rows the first one's
-      // threads bring them; the others need what the scores are too large by.
-      const int side = x.two ? w : 0, row = side * 128 + r;
+      // Rows come by whole pieces, neighbours to neighbouring threads (a thread that read a row of its own met a cache line in each of its loads: 12000
+      // cycles a part). Past the last one, up to a multiple of 32, they are zeros; those behind belong to warps that do not look at their scores. Where the
+      // accumulators share the rows the first one's threads bring them.
+      const int side = x.two ? w : 0, left = x.rows - side * 128;            // whose rows these are, and how many
+      const bool live = r < left, some = (warp & 3) * 32 < left;
       float sc = sc0;
-      {
-        QueryRow at(p, x, G, plan.start[x.group] * p.q_len, min(row, x.rows - 1), 1);
-        const uint4* src = reinterpret_cast<const uint4*>(at.row(D));
-        uint4 v[D / 8];
-#pragma unroll
-        for (int c = 0; c < D / 8; ++c) v[c] = row < x.rows ? src[c] : make_uint4(0, 0, 0, 0);
+      if (side == w) {
+        constexpr int kPieces = D / 8, kStep = 128 / kPieces;
+        const int c = r % kPieces, first = r / kPieces, last = min(left, 128) - 1;
+        QueryRow at(p, x, G, plan.start[x.group] * p.q_len, w * 128 + min(first, last), kStep);
+        // bf16 as the products take it; else where the two numbers made of a piece's elements, and its neighbour's, will be
+        uint8_t* dst = sQ + w * kQB + (FP8 ? (c & 1) * (128 * D) : (c >> 3) * (128 * 128));
+#pragma unroll 4
+        for (int i = 0; i < kPieces; ++i) {
+          const int qr = first + kStep * i;
+          if (kStep * i > (last | 31)) break;
+          const uint32_t to = FP8 ? query_slot<D>(qr, c >> 1) : sw_off(qr, c & 7);
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(mb::smem_u32(dst + to)), "l"(reinterpret_cast<const uint4*>(at.row(D)) + c),
+                       "r"(qr <= last ? 16 : 0)
+                       : "memory");
+          if (qr + kStep <= last) at.step();
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
         if constexpr (FP8) {
-          sc *= query_pairs<D>(v, sQ + w * kQB, r, side == w);
-        } else {
-          if (side == w) {
-#pragma unroll
-            for (int c = 0; c < D / 8; ++c) *reinterpret_cast<uint4*>(sQ + w * kQB + (c >> 3) * (128 * 128) + sw_off(r, c & 7)) = v[c];
+          __syncwarp();
+          if (lane == 0) mb::mbar_arrive(&q_raw[w]);
+          ok = mb::mbar_wait(&q_raw[w], raws & 1, p.status, MB_ST_TIMEOUT_MMA);
+          if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+          ++raws;
+          if (some) {
+            const float back = query_pairs<D>(sQ + w * kQB, r);
+            s_qscale[part & 1][w][r] = back;
+            sc *= back;
           }
         }
         fence_async_smem();
+      } else if constexpr (FP8) {
+        ok = mb::mbar_wait(&q_full[0], part & 1, p.status, MB_ST_TIMEOUT_MMA);
+        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+        sc *= s_qscale[part & 1][0][r];
       }
       __syncwarp();
       if (lane == 0) mb::mbar_arrive(&q_full[w]);
-      const int left = x.two ? x.rows - w * 128 : x.rows; // rows of this tile
-      const bool live = r < left, some = (warp & 3) * 32 < left;
       const int len = plan.len[x.group];
       float m_run = -INFINITY, l_run = 0.f;
       auto rescale = [&](float alpha) {                   // S seen: the products that were issued in front of it are done
