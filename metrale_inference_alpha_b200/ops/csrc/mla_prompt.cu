@@ -138,7 +138,7 @@ mla_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   extern __shared__ __align__(16) uint8_t smem_raw[];
   uint8_t* sQ = smem_raw + ((1024u - (mb::smem_u32(smem_raw) & 1023u)) & 1023u);   // 2 row tiles x 3 spans x [128 rows x 128 B]
   uint8_t* sR = sQ + 2 * kQTile;
-  __shared__ __align__(8) uint64_t q_full, full[kRing], empty[kRing], s_full[2], p_full[2][2], o_full[2];
+  __shared__ __align__(8) uint64_t q_full, k_full[2], v_full[2], empty[kRing], s_full[2], p_full[2][2], o_full[2];
   __shared__ uint32_t s_tmem;
   const int h = blockIdx.x, seq = blockIdx.z, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   mb::pdl_wait();
@@ -159,11 +159,10 @@ mla_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 
   if (tid == 0) {
     mb::mbar_init(&q_full, 1);
-    for (int i = 0; i < kRing; ++i) {
-      mb::mbar_init(&full[i], 1);
-      mb::mbar_init(&empty[i], 1);
-    }
+    for (int i = 0; i < kRing; ++i) mb::mbar_init(&empty[i], 1);
     for (int i = 0; i < 2; ++i) {
+      mb::mbar_init(&k_full[i], 3);                       // of every second tile: the ring does not hold the pieces of three
+      mb::mbar_init(&v_full[i], 2);
       mb::mbar_init(&s_full[i], 1);
       mb::mbar_init(&p_full[i][0], 4);
       mb::mbar_init(&p_full[i][1], 4);
@@ -297,13 +296,14 @@ mla_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         if (!ok) return;
         const int at = (int)first + j * kT;
         uint8_t* dst = sR + slot * kPiece;
-        mb::mbar_expect_tx(&full[slot], kPiece);
+        uint64_t* bar = c < 3 ? &k_full[j & 1] : &v_full[j & 1];
+        mb::mbar_expect_tx(bar, kPiece);
         if (c < 2) {
-          mb::tma_load_2d(dst, &tmK, &full[slot], hk + c * 64, at);
+          mb::tma_load_2d(dst, &tmK, bar, hk + c * 64, at);
         } else if (c == 2) {
-          mb::tma_load_2d(dst, &tmR, &full[slot], kLat, at);
+          mb::tma_load_2d(dst, &tmR, bar, kLat, at);
         } else {
-          for (int d = 0; d < 2; ++d) mb::tma_load_2d(dst + d * (kPiece / 2), &tmV, &full[slot], hk + kNope + d * 64, at + (c - 3) * 64);
+          for (int d = 0; d < 2; ++d) mb::tma_load_2d(dst + d * (kPiece / 2), &tmV, bar, hk + kNope + d * 64, at + (c - 3) * 64);
         }
         ++i;
         if (++slot == kRing) {
@@ -313,10 +313,14 @@ mla_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       };
       for (int j = 0; j < n && ok; ++j)
         for (int c = 0; c < kPer; ++c) bring(j, c);
-      // given up: no copy may still be under way when the CTA ends
+      // given up: no copy may still be under way when the CTA ends. A tile whose pieces were not all asked for is waited for until the wait gives up: its
+      // copies are through by then
       if (!ok) {
         mb::mbar_wait(&q_full, 0, p.status, MB_ST_TIMEOUT_TMA);
-        for (int k = max(0, i - kRing); k < i; ++k) mb::mbar_wait(&full[k % kRing], (k / kRing) & 1, p.status, MB_ST_TIMEOUT_TMA);
+        for (int j = max(0, (i - 1) / kPer - 1); j <= (i - 1) / kPer; ++j) {
+          mb::mbar_wait(&k_full[j & 1], (j >> 1) & 1, p.status, MB_ST_TIMEOUT_TMA);
+          mb::mbar_wait(&v_full[j & 1], (j >> 1) & 1, p.status, MB_ST_TIMEOUT_TMA);
+        }
       }
     }
     if (warp == 9 && mb::elect_one() && n > 0) {
@@ -325,13 +329,16 @@ mla_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       // descriptors count 16 bytes: an operand's next step is an addition
       const uint64_t dQ = mb::umma_desc_sw128(mb::smem_u32(sQ)), dK = mb::umma_desc_sw128(mb::smem_u32(sR)),
                      dV = mb::umma_desc_sw128_mn(mb::smem_u32(sR), kPiece / 2, 1024);
-      auto there = [&](int i) { return mb::mbar_wait(&full[i % kRing], (i / kRing) & 1, p.status, MB_ST_TIMEOUT_MMA); };
+      // Every wait takes this thread a hundred cycles, met or not, so that tiles have a barrier for their keys and one for their values, which the first
+      // row tile waits for
       auto scores = [&](int w, int j) {
+        if (w == 0 || j >= n0) {
+          if (!mb::mbar_wait(&k_full[j & 1], (j >> 1) & 1, p.status, MB_ST_TIMEOUT_MMA)) return false;
+          mb::tc_fence_after();
+        }
 #pragma unroll
         for (int c = 0; c < 3; ++c) {
           const int i = j * kPer + c;
-          if (!there(i)) return false;
-          mb::tc_fence_after();
           const uint64_t q = dQ + w * (kQTile >> 4) + ((c * kPiece) >> 4), k = dK + (i % kRing) * (kPiece >> 4);
 #pragma unroll
           for (int s = 0; s < 4; ++s) mb::umma_f16(tmem + w * 128, q + ((s * 32) >> 4), k + ((s * 32) >> 4), kIdS, (c | s) != 0);
@@ -340,10 +347,11 @@ mla_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         return true;
       };
       auto values = [&](int w, int j) {
+        if ((w == 0 || j >= n0) && !mb::mbar_wait(&v_full[j & 1], (j >> 1) & 1, p.status, MB_ST_TIMEOUT_MMA)) return false;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int i = j * kPer + 3 + h;
-          if (!there(i) || !mb::mbar_wait(&p_full[w][h], j & 1, p.status, MB_ST_TIMEOUT_MMA)) return false;
+          if (!mb::mbar_wait(&p_full[w][h], j & 1, p.status, MB_ST_TIMEOUT_MMA)) return false;
           mb::tc_fence_after();
           const uint64_t v = dV + (i % kRing) * (kPiece >> 4);
 #pragma unroll
