@@ -3,12 +3,26 @@
 #include "common.cuh"
 #include "shared_attn.h"
 #include "attention_rows.cuh"
+#include "gemm_args.h"
 #include "smem_limit.h"
 #include "tensormap.h"
 
 namespace {
 
 constexpr int kRow = 576, kLat = 512, kQk = 192, kNope = 128, kV = 128;
+
+struct AttnParams {
+  const int* q_start;
+  const int* q_len;
+  const int* ctx_len;
+  const int* first;          // [seqs]: a sequence's first expanded row
+  const int* bad;            // [expanded rows / 32]: the place in its sequence of the first row that is no number, or 2^31 - 1
+  void* out;
+  uint32_t* status;
+  long long q_rows, kv_rows;
+  int H, head0, max_q_len, max_ctx;
+  float scale;
+};
 
 // ---- cached rows to consecutive ones, sequence s from first[s] on, a multiple of 128
 struct GatherParams {
@@ -134,7 +148,7 @@ __device__ __forceinline__ void fewer_regs() { asm volatile("setmaxnreg.dec.sync
 
 __global__ void __launch_bounds__(kThreads, 1)
 mla_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                  const __grid_constant__ CUtensorMap tmR, const MbMlaPromptArgs p) {
+                  const __grid_constant__ CUtensorMap tmR, const AttnParams p) {
   extern __shared__ __align__(16) uint8_t smem_raw[];
   uint8_t* sQ = smem_raw + ((1024u - (mb::smem_u32(smem_raw) & 1023u)) & 1023u);   // 2 row tiles x 3 spans x [128 rows x 128 B]
   uint8_t* sR = sQ + 2 * kQTile;
@@ -394,33 +408,60 @@ mla_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 
 }  // namespace
 
-extern "C" {
-
-int mb_mla_gather(const void* cache, const int* block_table, long long table_ld, const int* ctx_len, void* lat, int* first, int* bad, uint32_t* status,
-                  long long num_blocks, long long kv_rows, int num_seqs, int block_size, int max_ctx, cudaStream_t stream) {
-  if (!cache || !block_table || !ctx_len || !lat || !first || !bad || num_blocks <= 0 || kv_rows <= 0 || kv_rows % 128 || num_seqs <= 0 || block_size <= 0 || max_ctx <= 0)
-    return MB_ERR_BAD_ARG;
-  GatherParams p{(const __nv_bfloat16*)cache, block_table, table_ld, ctx_len, (__nv_bfloat16*)lat, first, bad, status, num_blocks, kv_rows, num_seqs, block_size, max_ctx};
-  return (int)mb::launch_kernel(gather_kernel, dim3((unsigned)(kv_rows / kGather)), dim3(256), 0, stream, p);
+// Workspace: the cached rows one behind the other, sequences' first rows, places of rows that are no numbers, expanded keys and values of `each` heads
+struct Layout {
+  size_t first, bad, kv, bytes;
+};
+static Layout layout(long long rows, int seqs, int each) {
+  auto up = [](size_t x) { return (x + 255) & ~size_t(255); };
+  Layout l;
+  l.first = up((size_t)rows * kRow * 2);
+  l.bad = l.first + up((size_t)seqs * 4);
+  l.kv = l.bad + up((size_t)rows / kGather * 4);
+  l.bytes = l.kv + (size_t)rows * each * 512;
+  return l;
 }
 
+extern "C" {
+
+size_t mb_mla_prompt_ws(long long kv_rows, int num_seqs, int each) { return layout(kv_rows, num_seqs, each).bytes; }
+
 int mb_mla_prompt(const MbMlaPromptArgs* a, cudaStream_t stream) {
-  if (!a || !a->q || !a->kv || !a->lat || !a->q_start || !a->q_len || !a->ctx_len || !a->first || !a->bad || !a->out || a->num_seqs <= 0 || a->num_seqs > 65535 ||
-      a->H <= 0 || a->heads <= 0 || a->heads > 65535 || a->head0 < 0 || a->head0 + a->heads > a->H || a->max_q_len <= 0 || a->max_ctx <= 0)
+  if (!a || !a->q || !a->cache || !a->block_table || !a->q_start || !a->q_len || !a->ctx_len || !a->w || !a->out || a->num_blocks <= 0 || a->q_rows <= 0 ||
+      a->kv_rows <= 0 || a->kv_rows % 128 || a->num_seqs <= 0 || a->num_seqs > 65535 || a->H <= 0 || a->H > 65535 || a->block_size <= 0 || a->max_q_len <= 0 ||
+      a->max_ctx <= 0 || a->each <= 0)
     return MB_ERR_BAD_ARG;
-  const unsigned tiles = (a->max_q_len + 255) / 256;
-  if (tiles > 65535 || a->q_rows <= 0 || a->kv_rows <= 0 || a->kv_rows % kT) return MB_ERR_TOO_LARGE;
-  CUtensorMap tm[4];
-  const uint64_t pitch = (uint64_t)a->heads * 512;
-  int rc = mbh::encode_2d(&tm[0], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, a->q, (uint64_t)a->H * kQk, a->q_rows, (uint64_t)a->H * kQk * 2, 64, 128);
-  if (!rc) rc = mbh::encode_2d(&tm[1], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, a->kv, (uint64_t)a->heads * 256, a->kv_rows, pitch, 64, 128);
-  if (!rc) rc = mbh::encode_2d(&tm[2], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, a->kv, (uint64_t)a->heads * 256, a->kv_rows, pitch, 64, 64);
-  if (!rc) rc = mbh::encode_2d(&tm[3], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, a->lat, kRow, a->kv_rows, kRow * 2, 64, 128);
-  if (rc) return rc;
-  static std::atomic<uint64_t> asked{0};
-  const cudaError_t e = mb::allow_smem(reinterpret_cast<const void*>(mla_prompt_kernel), kSmem, asked);
+  const unsigned tiles = ((unsigned)a->max_q_len + 255) / 256;
+  if (tiles > 65535 || a->kv_rows >= (1ll << 31)) return MB_ERR_TOO_LARGE;
+  const Layout l = layout(a->kv_rows, a->num_seqs, a->each);
+  if (!a->ws || a->ws_bytes < l.bytes) return MB_ERR_TOO_LARGE;
+  uint8_t* ws = reinterpret_cast<uint8_t*>(a->ws);
+  int *first = reinterpret_cast<int*>(ws + l.first), *bad = reinterpret_cast<int*>(ws + l.bad);
+  const GatherParams g{(const __nv_bfloat16*)a->cache, a->block_table, a->table_ld, a->ctx_len, (__nv_bfloat16*)ws, first, bad, a->status, a->num_blocks, a->kv_rows,
+                       a->num_seqs, a->block_size, a->max_ctx};
+  cudaError_t e = mb::launch_kernel(gather_kernel, dim3((unsigned)(a->kv_rows / kGather)), dim3(256), 0, stream, g);
   if (e != cudaSuccess) return (int)e;
-  return (int)mb::launch_kernel_ex(mla_prompt_kernel, dim3(a->heads, tiles, a->num_seqs), dim3(kThreads), kSmem, stream, 1, mb_pdl_enabled() != 0, tm[0], tm[1], tm[2], tm[3], *a);
+  static std::atomic<uint64_t> asked{0};
+  e = mb::allow_smem(reinterpret_cast<const void*>(mla_prompt_kernel), kSmem, asked);
+  if (e != cudaSuccess) return (int)e;
+  CUtensorMap tm[4];
+  int rc = mbh::encode_2d(&tm[0], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, a->q, (uint64_t)a->H * kQk, a->q_rows, (uint64_t)a->H * kQk * 2, 64, 128);
+  if (!rc) rc = mbh::encode_2d(&tm[3], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, ws, kRow, a->kv_rows, kRow * 2, 64, 128);
+  for (int h = 0; h < a->H && !rc; h += a->each) {
+    const int n = a->H - h < a->each ? a->H - h : a->each;
+    MbGemmArgs m{};
+    m.M = (int)a->kv_rows; m.N = n * 256; m.K = kLat; m.ldo = n * 256;
+    m.W = reinterpret_cast<const __nv_bfloat16*>(a->w) + (size_t)h * 256 * kLat;
+    m.X = ws; m.ldx = kRow; m.out = ws + l.kv; m.alpha = 1.f; m.status = a->status; m.sm_count = a->sm_count;
+    m.flags = a->gemm_flags;                               // without a workspace the product is not split
+    rc = mb_gemm(&m, stream);
+    if (!rc) rc = mbh::encode_2d(&tm[1], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, m.out, (uint64_t)n * 256, a->kv_rows, (uint64_t)n * 512, 64, 128);
+    if (!rc) rc = mbh::encode_2d(&tm[2], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, m.out, (uint64_t)n * 256, a->kv_rows, (uint64_t)n * 512, 64, 64);
+    if (rc) return rc;
+    const AttnParams p{a->q_start, a->q_len, a->ctx_len, first, bad, a->out, a->status, a->q_rows, a->kv_rows, a->H, h, a->max_q_len, a->max_ctx, a->scale};
+    rc = (int)mb::launch_kernel_ex(mla_prompt_kernel, dim3(n, tiles, a->num_seqs), dim3(kThreads), kSmem, stream, 1, mb_pdl_enabled() != 0, tm[0], tm[1], tm[2], tm[3], p);
+  }
+  return rc;
 }
 
 }  // extern "C"

@@ -40,21 +40,25 @@ struct MbMergeArgs {
 
 struct MbMlaPromptArgs {
   const void* q;             // [rows, H, 192] bf16
-  const void* kv;            // [expanded rows, heads of the call, 256] bf16: keys without position, values
-  const void* lat;           // [expanded rows, 576] bf16: the cached rows, of which the rotated part of the keys is read
+  const void* cache;         // [blocks, block, 1, 576] bf16
+  const int* block_table;    // [seqs, blocks of a sequence]
+  long long table_ld;
   const int* q_start;
   const int* q_len;
   const int* ctx_len;
-  const int* first;          // [seqs]: a sequence's first expanded row
-  const int* bad;            // [expanded rows / 32]: the place in its sequence of the first row that is no number, or 2^31 - 1
+  const void* w;             // [H, 256, 512] bf16
   void* out;                 // [rows, H, 128] bf16
+  void* ws;
+  size_t ws_bytes;
   uint32_t* status;
-  long long q_rows, kv_rows;
-  int num_seqs, H, head0, heads, max_q_len, max_ctx;
+  long long num_blocks, q_rows, kv_rows;     // kv_rows: expanded rows, a multiple of 128
+  int num_seqs, H, block_size, max_q_len, max_ctx;
+  int each;                  // heads that are expanded at once
+  int sm_count, gemm_flags;
   float scale;
 };
 
 // as the callers pack them
 static_assert(sizeof(MbSharedArgs) == 192, "field by field in ops/shared_attn.py too");
 static_assert(sizeof(MbMergeArgs) == 296, "field by field in ops/shared_attn.py too");
-static_assert(sizeof(MbMlaPromptArgs) == 128, "field by field in ops/mla_prompt.py too");
+static_assert(sizeof(MbMlaPromptArgs) == 160, "field by field in ops/mla_prompt.py too");

@@ -9,17 +9,16 @@ from typing import Optional
 
 import torch
 
-from . import Act, QuantWeight, _count, _native, _stream, linear, reference as ref, runtime
+from . import _PERSIST_PREFILL, _count, _native, _stream, reference as ref, runtime
 from .shared_attn import _bad, _check_ints, _check_places, _check_table
 
 LATENT, ROPE, NOPE, VALUE = 512, 64, 128, 128
 ROW, QK, KV = LATENT + ROPE, NOPE + ROPE, NOPE + VALUE
 
 # MbMlaPromptArgs of csrc/shared_attn.h, field by field
-_ARGS = struct.Struct("@10P 2q 6i f 4x")
+_ARGS = struct.Struct("@3P q 6P N P 3q 8i f 4x")
 
 _native.register_optional("mb_mla_prompt", [C.c_char_p, C.c_void_p])
-_native.register_optional("mb_mla_gather", [C.c_void_p, C.c_void_p, C.c_longlong] + [C.c_void_p] * 5 + [C.c_longlong] * 2 + [C.c_int] * 3 + [C.c_void_p])
 
 _lib = None
 # most bytes of expanded keys and values that a call holds: more heads go in several steps
@@ -34,6 +33,7 @@ def _library():
         size.argtypes, size.restype = [C.c_int], C.c_size_t
         if size(2) != _ARGS.size:
             raise RuntimeError(f"{_native.LIB_PATH} has argument structures of other sizes: build it again")
+        L.mb_mla_prompt_ws.argtypes, L.mb_mla_prompt_ws.restype = [C.c_longlong, C.c_int, C.c_int], C.c_size_t
         _lib = L
     return _lib
 
@@ -88,23 +88,14 @@ def mla_prompt_attention(q: torch.Tensor, cache: torch.Tensor, block_table: torc
         return torch.zeros(T, H, VALUE, dtype=torch.bfloat16, device=dev)
     out = torch.empty(T, H, VALUE, dtype=torch.bfloat16, device=dev)
     L, rt = _library(), runtime(dev)
-    lat, first = torch.empty(rows, ROW, dtype=torch.bfloat16, device=dev), torch.empty(S + rows // 32, dtype=torch.int32, device=dev)
-    bad, status, stream = first.data_ptr() + 4 * S, rt.status.data_ptr(), _stream()
-    _native.check(L.mb_mla_gather(cache.data_ptr(), block_table.data_ptr(), block_table.stride(0), ctx_len.data_ptr(), lat.data_ptr(), first.data_ptr(), bad, status,
-                                  nb, rows, S, bs, max_ctx, stream), "mla_gather")
-    _count()
     each = max(1, min(H, _WS_BYTES // (rows * KV * 2)))
-    kv = torch.empty(rows, each * KV, dtype=torch.bfloat16, device=dev)
-    act = Act("bf16", rows, LATENT, lat[:, :LATENT])
-    for h in range(0, H, each):
-        n = min(each, H - h)
-        part = kv.view(-1)[:rows * n * KV].view(rows, n * KV)
-        # without splits, which have a workspace that all launches share: more than 256 rows have none of this depth
-        linear(act, QuantWeight("bf16", n * KV, LATENT, w_kv[h:h + n].view(n * KV, LATENT)), out=part, force_splits=int(rows <= 256))
-        a = _ARGS.pack(q.data_ptr(), part.data_ptr(), lat.data_ptr(), q_start.data_ptr(), q_len.data_ptr(), ctx_len.data_ptr(), first.data_ptr(), bad, out.data_ptr(),
-                       status, T, rows, S, H, h, n, max_q_len, max_ctx, scale)
-        _native.check(L.mb_mla_prompt(a, stream), "mla_prompt")
-        _count()
+    need = L.mb_mla_prompt_ws(rows, S, each)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    a = _ARGS.pack(q.data_ptr(), cache.data_ptr(), block_table.data_ptr(), block_table.stride(0), q_start.data_ptr(), q_len.data_ptr(), ctx_len.data_ptr(),
+                   w_kv.data_ptr(), out.data_ptr(), ws.data_ptr(), need, rt.status.data_ptr(), nb, T, rows, S, H, bs, max_q_len, max_ctx, each, rt.sm_count,
+                   _PERSIST_PREFILL, scale)
+    _native.check(L.mb_mla_prompt(a, _stream()), "mla_prompt")
+    _count(1 + 2 * ((H + each - 1) // each))
     return out
 
 
