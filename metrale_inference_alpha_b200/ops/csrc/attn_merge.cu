@@ -1,46 +1,80 @@
 // Attention that was computed in parts over disjoint keys, joined: lse = ln sum_i exp l_i, out = sum_i exp(l_i - lse) o_i. A part of weight zero (l_i = -inf)
-// is not read, so what it holds does not matter; a row without weight gives zeros and -inf. One pass over the parts, a thread a vector of 16 bytes of a row.
+// is not read, so what it holds does not matter; a row without weight gives zeros and -inf. One pass over the parts, bound by memory: a thread asks for the
+// same 16 bytes of all parts, of ITEMS rows, before it uses any of them. Weights and sums are 32 bits.
 #include "common.cuh"
 #include "shared_attn.h"
+#include <type_traits>
 
 namespace {
 
-// V: elements a thread takes at once (16 bytes, or one where rows are no whole vectors)
-template <typename T, int V>
+// V: elements a thread takes at once (16 bytes, or one where rows are no whole vectors); PARTS: most parts
+template <typename T, int V, int PARTS, int ITEMS>
 __global__ void __launch_bounds__(256) merge_kernel(const MbMergeArgs p) {
+  using Vec = typename std::conditional<(V > 1), uint4, T>::type;
   const int per = p.dim / V;
-  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  const long long total = p.rows * per, i0 = (long long)blockIdx.x * (256 * ITEMS) + threadIdx.x;
   mb::pdl_wait();
-  if (i >= p.rows * per) return;
-  const long long row = i / per;
-  const int c = (int)(i - row * per);
-  float l[kMergeParts], top = -INFINITY;
+  float l[ITEMS][PARTS];
+  Vec x[ITEMS][PARTS];
 #pragma unroll
-  for (int k = 0; k < kMergeParts; ++k) {
-    l[k] = k < p.parts ? p.lses[k][row] : -INFINITY;
-    top = fmaxf(top, l[k]);
+  for (int it = 0; it < ITEMS; ++it) {
+    const long long i = i0 + it * 256, row = i / per;
+#pragma unroll
+    for (int k = 0; k < PARTS; ++k) l[it][k] = i < total && k < p.parts ? p.lses[k][row] : -INFINITY;
   }
-  float acc[V], total = 0.f;
 #pragma unroll
-  for (int j = 0; j < V; ++j) acc[j] = 0.f;
+  for (int it = 0; it < ITEMS; ++it)
 #pragma unroll
-  for (int k = 0; k < kMergeParts; ++k) {
-    if (k >= p.parts || l[k] == -INFINITY) continue;
-    const float w = expf(l[k] - top);
-    total += w;
-    T x[V];
-    if constexpr (V > 1) *reinterpret_cast<uint4*>(x) = __ldcs(reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.outs[k]) + row * p.dim) + c);
-    else x[0] = reinterpret_cast<const T*>(p.outs[k])[row * p.dim + c];
+    for (int k = 0; k < PARTS; ++k)
+      if (l[it][k] != -INFINITY) {
+        const Vec* src = reinterpret_cast<const Vec*>(p.outs[k]) + i0 + it * 256;
+        if constexpr (V > 1) x[it][k] = __ldcs(src);
+        else x[it][k] = *src;
+      }
 #pragma unroll
-    for (int j = 0; j < V; ++j) acc[j] += w * (float)x[j];
+  for (int it = 0; it < ITEMS; ++it) {
+    const long long i = i0 + it * 256;
+    if (i >= total) return;
+    float top = -INFINITY, acc[V], sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < PARTS; ++k) top = fmaxf(top, l[it][k]);
+#pragma unroll
+    for (int j = 0; j < V; ++j) acc[j] = 0.f;
+#pragma unroll
+    for (int k = 0; k < PARTS; ++k) {
+      if (l[it][k] == -INFINITY) continue;
+      const float w = expf(l[it][k] - top);
+      sum += w;
+      const T* e = reinterpret_cast<const T*>(&x[it][k]);
+#pragma unroll
+      for (int j = 0; j < V; ++j) acc[j] += w * (float)e[j];
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    Vec y;
+    T* e = reinterpret_cast<T*>(&y);
+#pragma unroll
+    for (int j = 0; j < V; ++j) e[j] = (T)(acc[j] * inv);
+    Vec* dst = reinterpret_cast<Vec*>(p.out) + i;
+    if constexpr (V > 1) __stcs(dst, y);
+    else *dst = y;
+    const long long row = i / per;
+    if (i == row * per) p.lse[row] = sum == 0.f ? -INFINITY : top + logf(sum);
   }
-  const float inv = total == 0.f ? 0.f : 1.f / total;
-  T y[V];
-#pragma unroll
-  for (int j = 0; j < V; ++j) y[j] = (T)(acc[j] * inv);
-  if constexpr (V > 1) reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.out) + row * p.dim)[c] = *reinterpret_cast<uint4*>(y);
-  else reinterpret_cast<T*>(p.out)[row * p.dim + c] = y[0];
-  if (c == 0) p.lse[row] = total == 0.f ? -INFINITY : top + logf(total);
+}
+
+template <typename T, int V, int PARTS, int ITEMS>
+int launch(const MbMergeArgs& a, cudaStream_t stream) {
+  const long long n = (a.rows * (a.dim / V) + 256 * ITEMS - 1) / (256 * ITEMS);
+  if (n > 0x7fffffffll) return MB_ERR_TOO_LARGE;
+  return (int)mb::launch_kernel(merge_kernel<T, V, PARTS, ITEMS>, dim3((unsigned)n), dim3(256), 0, stream, a);
+}
+
+template <typename T, int V>
+int by_parts(const MbMergeArgs& a, cudaStream_t stream) {
+  if (a.parts <= 2) return launch<T, V, 2, 2>(a, stream);
+  if (a.parts <= 4) return launch<T, V, 4, 2>(a, stream);
+  if (a.parts <= 8) return launch<T, V, 8, 1>(a, stream);
+  return launch<T, V, kMergeParts, 1>(a, stream);
 }
 
 template <typename T>
@@ -48,11 +82,7 @@ int run(const MbMergeArgs& a, cudaStream_t stream) {
   constexpr int kV = 16 / sizeof(T);
   uintptr_t low = reinterpret_cast<uintptr_t>(a.out) | (a.dim % kV ? 1 : 0);
   for (int k = 0; k < a.parts; ++k) low |= reinterpret_cast<uintptr_t>(a.outs[k]);
-  const bool wide = !(low & 15);
-  const long long n = (a.rows * (wide ? a.dim / kV : a.dim) + 255) / 256;
-  if (n > 0x7fffffffll) return MB_ERR_TOO_LARGE;
-  return wide ? (int)mb::launch_kernel(merge_kernel<T, kV>, dim3((unsigned)n), dim3(256), 0, stream, a)
-              : (int)mb::launch_kernel(merge_kernel<T, 1>, dim3((unsigned)n), dim3(256), 0, stream, a);
+  return low & 15 ? by_parts<T, 1>(a, stream) : by_parts<T, kV>(a, stream);
 }
 
 }  // namespace
