@@ -42,6 +42,9 @@ class ForwardBatch:
     logit_rows: torch.Tensor           # [R] int64 rows whose logits are needed
     max_q_len: int = 1
     max_ctx: int = 0
+    # sums over the sequences, known on the host: of ctx_len, and of the (row, visible token) pairs; 0 in batches of a fixed shape (graph rungs)
+    total_ctx: int = 0
+    total_pairs: int = 0
     state_slots: Optional[torch.Tensor] = None   # [S] int32 recurrent-state slot per sequence
     num_tokens: int = 0
     num_seqs: int = 0
@@ -106,4 +109,6 @@ class ForwardBatch:
             max_q_len=max(ql) if ql else 1, max_ctx=max(cl) if cl else 0,
             state_slots=mk(sslots, torch.int32), num_tokens=row, num_seqs=len(qs), host_q_len=ql)
         b.real_seqs = real_seqs
+        if not pad_seqs:
+            b.total_ctx, b.total_pairs = sum(cl), sum(n * c - n * (n - 1) // 2 for n, c in zip(ql, cl))
         return b

@@ -80,6 +80,8 @@ class EngineArgs:
     oom_guard_mb: int = 4096                           # device memory left unclaimed when sizing the KV pool
     fp8_kv_calibration_tokens: int = 0                 # fp8 KV without checkpoint scales: calibrate them online over this many tokens (0 = scale 1.0)
     fp8_kv_headroom: float = 1.0
+    latent_prompts: str = "absorbed"                   # absorbed | expanded: latent-attention models attend to prompts with every head's own keys and values
+                                                       # (made from the cached rows) where that costs less than the absorbed form
     pipeline_decode: bool = True                       # launch decode step t + 1 from the device-fed tokens while step t is read back
 
 
@@ -184,7 +186,7 @@ class LLMEngine:
         self.runner = ModelRunner(cfg, self.weights, args.device, blocks, self.sched_cfg, self.tp,
                                   use_graphs=args.use_cuda_graphs, kv_poison=args.kv_poison,
                                   fp8_kv_calibration_tokens=args.fp8_kv_calibration_tokens,
-                                  fp8_kv_headroom=args.fp8_kv_headroom,
+                                  fp8_kv_headroom=args.fp8_kv_headroom, latent_prompts=args.latent_prompts,
                                   num_snapshots=args.state_snapshots or 16 + args.decode_rollback_ring * args.max_num_seqs)
         if self.runner.pool is not None and (args.state_tier_host_bytes > 0 or args.state_tier_dir):
             self.runner.pool.configure_tiers(args.state_tier_host_bytes, args.state_tier_dir)

@@ -23,6 +23,7 @@ from ..utils import nvtx
 from ..cache import KvCacheConfig, PagedKvCache, StatePool
 from ..config.model_config import ModelConfig
 from ..models.decoder import Decoder, LayerCaches, TpContext
+from ..models.mla import keep_joined
 from ..scheduler.policy import SchedulerConfig
 from ..scheduler.types import StepPlan, StepResult
 from ..weights.loader import ModelW
@@ -161,7 +162,7 @@ class ModelRunner:
                  sched: Optional[SchedulerConfig] = None, tp: Optional[TpContext] = None,
                  use_graphs: bool = True, max_state_slots: Optional[int] = None, num_snapshots: int = 16,
                  mtp_drafts: int = 0, kv_poison: bool = False, fp8_kv_calibration_tokens: int = 0,
-                 fp8_kv_headroom: float = 1.0):
+                 fp8_kv_headroom: float = 1.0, latent_prompts: str = "absorbed"):
         self.cfg, self.w, self.device = cfg, weights, torch.device(device)
         self.sched = sched or SchedulerConfig()
         self.tp = tp or TpContext()
@@ -178,6 +179,11 @@ class ModelRunner:
             self.pool = StatePool(shapes, slots, num_snapshots, device)
         self.caches = LayerCaches(cfg, kv=self.kv, state=self.pool, mtp_kv=self.mtp_kv)
         self.decoder = Decoder(cfg, weights, self.tp, device)
+        if latent_prompts == "expanded":
+            keep_joined(cfg, weights)
+            self.decoder.expand_prompts = True
+        elif latent_prompts != "absorbed":
+            raise ValueError(f"latent_prompts must be absorbed | expanded, not {latent_prompts!r}")
         self.dflash = None
         # FP8 KV scales: the checkpoint's (three key spellings, weights/kv_scales.py), else online
         # calibration over the first tokens when asked for, else 1.0
@@ -281,6 +287,7 @@ class ModelRunner:
         nl = 0
         max_q = 1
         max_ctx = 1
+        total_ctx = total_pairs = 0
         for s, it in enumerate(plan.items):
             n = len(it.tokens)
             p0 = it.start_pos
@@ -302,6 +309,8 @@ class ModelRunner:
                 nl += k + 1
             row += n
             max_q, max_ctx = max(max_q, n), max(max_ctx, p0 + n)
+            total_ctx += p0 + n
+            total_pairs += n * (p0 + n) - n * (n - 1) // 2
         S = len(plan.items)
         while S < pad_seqs:                                   # null rows up to the graph rung
             tokens[row:row + pad_q], slots[row:row + pad_q] = 0, -1
@@ -323,6 +332,8 @@ class ModelRunner:
             block_table=dv("bt", None).view(st.S_cap, st.max_blocks)[:S],
             logit_rows=dv("lrows", 2 * nl).view(torch.int64),
             max_q_len=max_q, max_ctx=max_ctx, state_slots=dv("state", S), num_tokens=row, num_seqs=S)
+        if not pad_seqs:
+            b.total_ctx, b.total_pairs = total_ctx, total_pairs
         return b
 
     _fast_sig = None

@@ -89,6 +89,7 @@ class Decoder:
         self.lora = None                   # lora.LoraManager when adapters are served
         self.calib = None                  # dict while calibrating static activation scales (engine/runner.py)
         self._rotary = {}                  # (rotated dims, base, scaling) -> cos / sin tables of layers with their own rotation
+        self.expand_prompts = False        # latent attention: prompts in expanded form where that is the cheaper one (models/mla.py)
         self.side_head = None              # speculative.dflash.DflashDrafter: sees chosen layers' hidden states of every forward
 
     # ------------------------------------------------------------------ helpers

@@ -7,7 +7,8 @@ latent-space output back to per-head values before o_proj.
 On a GPU the block is: projections (tcgen05 GEMMs), the two absorption products as bf16 batched
 GEMMs over heads, one assembly kernel (latent RMSNorm, both rotations, cache row write, absorbed
 query rows: ``mla.cu::mla_prepare_kernel``) and the paged attention kernel (one CTA per 16 query
-rows, the cached tile feeding both products); this file keeps the fp32 restatement used on CPU
+rows, the cached tile feeding both products). Prompts may go in expanded form instead (every head's own keys and
+values, made from the cached rows: ``mla_prompt.cu``; an engine option); this file keeps the fp32 restatement used on CPU
 and as the oracle.
 Reference behaviour: ``kernels/gb10/deepseek-v4-flash/nvfp4/mla_absorbed.cu``
 (``mla_batched_gemv``, ``mla_cache_assemble``), ``paged_decode_attn_mla.cu``.
@@ -19,7 +20,7 @@ import math
 import torch
 
 from .. import ops
-from ..ops import ACT_FOR_WEIGHT, latent, mla_cuda, sparse_attn
+from ..ops import ACT_FOR_WEIGHT, latent, mla_cuda, mla_prompt, sparse_attn
 from ..ops.mixers import act_of
 from ..ops import reference as ref
 
@@ -54,6 +55,12 @@ def mla_block(dec, x, lw, batch, kv, j: int):
         # latent norm + both rotations + the cache write + the query assembly, the paged MLA kernel
         q = q.view(T, H, nope + rope)
         ckv = ops.linear(a, w.kv_a)                                    # [T, L + rope] bf16
+        if sel is None and dec.expand_prompts and hasattr(w, "_w_kv_bf16") and _expanded_pays(batch):
+            mla_cuda.prepare_prompt(q, ckv, w.kv_a_norm, dec.cos, dec.sin, batch.positions, batch.slot_mapping, kv.k[j], nope, c.rms_eps)
+            o = ops.mla_prompt_attention(q, kv.k[j], batch.block_table, batch.q_start, batch.q_len, batch.ctx_len, w._w_kv_bf16, max_q_len=batch.max_q_len,
+                                         max_ctx=batch.max_ctx, scale=scale, total_ctx=batch.total_ctx)
+            oa = ops.quantize_act(o.view(T, H * vd), ACT_FOR_WEIGHT[w.o.fmt])
+            return dec.tp.linear_reduce(oa, w.o, residual=x, defer=True)
         uk = _bf16(w, "w_uk")                                          # [H, nope, L]
         q_lat = torch.bmm(q[..., :nope].transpose(0, 1), uk)           # [H, T, L]
         qq = mla_cuda.prepare(q, q_lat, ckv, w.kv_a_norm, dec.cos, dec.sin, batch.positions, batch.slot_mapping,
@@ -90,6 +97,33 @@ def mla_block(dec, x, lw, batch, kv, j: int):
     o = torch.einsum("thl,hvl->thv", o_lat, w.w_uv.float()).reshape(T, H * vd)
     oa = ops.quantize_act(o.to(torch.bfloat16), ACT_FOR_WEIGHT[w.o.fmt])
     return dec.tp.linear_reduce(oa, w.o, residual=x, defer=True)
+
+
+EXPAND_PAIRS = 48
+
+
+def _expanded_pays(batch) -> bool:
+    """Whether this step's attention is cheaper in expanded form. A head's multiply-adds are 1088 a (row, token) pair and 512 x 256 a row absorbed, 320 a
+    pair and 512 x 256 a cached token expanded: by that count a cached token in front of the rows has to be seen by 171 of them. The absorbed kernel runs
+    further from its peak, so less is enough. Measured with 128 heads, absorbed against expanded: eight portions behind contexts of 2048, of 32 rows 722 and
+    911 us, of 48 1062 and 918, of 96 1945 and 919; one behind 4096, of 32 rows 337 and 222, of 512 2139 and 304; a whole prompt of 1024 1031 and 119. With
+    16 heads expanded is ahead in all of them (eight of 32 rows behind 2048: 192 and 136). Portions of fewer than 32 rows stay with the decode kernels."""
+    return batch.max_q_len >= mla_cuda.TC_MIN_ROWS and batch.total_ctx > 0 and \
+        batch.total_pairs >= EXPAND_PAIRS * (batch.total_ctx - batch.num_tokens)
+
+
+def keep_joined(cfg, weights) -> None:
+    """For the expanded form: keeps [W_uk | W_uv] of every latent layer as one tensor, of which the two become views, so that nothing is held twice.
+    Layers of other sizes, and weights that are not on a GPU, stay as they are (and absorbed)."""
+    layers = list(weights.layers) + ([weights.mtp.layer] if weights.mtp is not None else [])
+    for lw in layers:
+        w = lw.mixer
+        if lw.kind != "mla" or not w.w_uk.is_cuda or w.w_uk.shape[1:] != (mla_prompt.NOPE, mla_prompt.LATENT) \
+                or w.w_uv.shape[1:] != (mla_prompt.VALUE, mla_prompt.LATENT) or cfg.qk_rope_dim != mla_prompt.ROPE:
+            continue
+        joined = w._w_kv_bf16 = torch.cat([w.w_uk, w.w_uv], 1).to(torch.bfloat16).contiguous()
+        w.w_uk, w.w_uv = joined[:, :mla_prompt.NOPE], joined[:, mla_prompt.NOPE:]
+        w._w_uk_bf16, w._w_uv_bf16 = w.w_uk, w.w_uv
 
 
 def latent_mixer(dec, a, w, batch, cache, fmt: str, out):

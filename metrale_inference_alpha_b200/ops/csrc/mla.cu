@@ -664,13 +664,14 @@ int mb_mla_attention(const MbMlaArgs* a, cudaStream_t stream) {
 //     latent with its weight, NeoX rotation of the rope key at the token's position, both written
 //     as one bf16 cache row at the token's slot (rows without a slot write nothing);
 //   * the absorbed query row of every head, [q_lat (L) | rotated q_rope (R)]: q_lat comes from the
-//     batched absorption product q_nope W_uk (laid out [H, T, L]), q_rope from the q projection.
+//     batched absorption product q_nope W_uk (laid out [H, T, L]), q_rope from the q projection. Without
+//     q_lat and qq (the expanded form of prompts, mla_prompt.cu) the rope part of q is rotated in place.
 // grid = T tokens, 256 threads. Reference behaviour: mla_cache_assemble and the rope half of
 // mla_batched_gemv (kernels/gb10/deepseek-v4-flash/nvfp4/mla_absorbed.cu).
 namespace {
 struct MlaPrepParams {
   const __nv_bfloat16* q;        // [T, H, nope + R]
-  const __nv_bfloat16* q_lat;    // [H, T, L]
+  const __nv_bfloat16* q_lat;    // [H, T, L], or null
   const __nv_bfloat16* ckv;      // [T, L + R]
   const __nv_bfloat16* norm_w;   // [L]
   const float* cos_tab;          // [max_pos, R / 2]
@@ -678,7 +679,7 @@ struct MlaPrepParams {
   const int* positions;
   const long long* slots;
   __nv_bfloat16* cache;          // [num_slots, L + R]
-  __nv_bfloat16* qq;             // [T, H, L + R]
+  __nv_bfloat16* qq;             // [T, H, L + R], or q itself where q_lat is null
   int T, H, nope, R, L, max_pos;
   long long num_slots;
   float eps;
@@ -725,8 +726,9 @@ __global__ void __launch_bounds__(256) mla_prepare_kernel(const MlaPrepParams p)
     }
   }
   // absorbed query rows: 16-byte copies of q_lat, then the rotated rope part
-  const int W = p.L + p.R;
-  const int chunks = p.L / 8;
+  const int lead = p.q_lat ? p.L : p.nope;
+  const int W = lead + p.R;
+  const int chunks = p.q_lat ? p.L / 8 : 0;
   for (int i = tid; i < p.H * chunks; i += 256) {
     const int h = i / chunks, c = i - h * chunks;
     *reinterpret_cast<uint4*>(p.qq + ((size_t)t * p.H + h) * W + c * 8) =
@@ -736,7 +738,7 @@ __global__ void __launch_bounds__(256) mla_prepare_kernel(const MlaPrepParams p)
     const int h = i / half, j = i - h * half;
     const __nv_bfloat16* qr = p.q + ((size_t)t * p.H + h) * (p.nope + p.R) + p.nope;
     const float x1 = __bfloat162float(qr[j]), x2 = __bfloat162float(qr[half + j]);
-    __nv_bfloat16* dst = p.qq + ((size_t)t * p.H + h) * W + p.L;
+    __nv_bfloat16* dst = p.qq + ((size_t)t * p.H + h) * W + lead;
     dst[j] = __float2bfloat16(x1 * s_cs[0][j] - x2 * s_cs[1][j]);
     dst[half + j] = __float2bfloat16(x2 * s_cs[0][j] + x1 * s_cs[1][j]);
   }
@@ -748,7 +750,7 @@ extern "C" int mb_mla_prepare(const void* q, const void* q_lat, const void* ckv,
                               void* cache, void* qq, int T, int H, int nope, int R, int L, int max_pos,
                               long long num_slots, float eps, uint32_t* status, cudaStream_t stream) {
   if (T <= 0) return 0;
-  if (R > 128 || (R & 1) || L % 8 != 0 || H <= 0) return MB_ERR_BAD_ARG;
+  if (R > 128 || (R & 1) || L % 8 != 0 || H <= 0 || (q_lat == nullptr && qq != q)) return MB_ERR_BAD_ARG;
   MlaPrepParams p;
   p.q = (const __nv_bfloat16*)q; p.q_lat = (const __nv_bfloat16*)q_lat; p.ckv = (const __nv_bfloat16*)ckv;
   p.norm_w = (const __nv_bfloat16*)norm_w; p.cos_tab = cos_tab; p.sin_tab = sin_tab;

@@ -110,3 +110,17 @@ def prepare(q: torch.Tensor, q_lat: torch.Tensor, ckv: torch.Tensor, norm_w: tor
     _native.check(rc, "mla_prepare")
     _count()
     return qq
+
+
+def prepare_prompt(q: torch.Tensor, ckv: torch.Tensor, norm_w: torch.Tensor, cos, sin, positions, slots, cache: torch.Tensor, nope: int,
+                   eps: float) -> None:
+    """What the expanded form of prompts needs, in one launch: latent RMSNorm + key RoPE + cache row write as in `prepare`, and the rope part of q
+    [T, H, nope + R] rotated in place."""
+    from . import _count, _ptr, _stream, runtime
+    T, H, qd = q.shape
+    rc = _native.lib().mb_mla_prepare(
+        _ptr(q), None, _ptr(ckv), _ptr(norm_w), _ptr(cos), _ptr(sin), _ptr(positions), _ptr(slots),
+        _ptr(cache), _ptr(q), T, H, nope, qd - nope, cache.shape[-1] - (qd - nope), cos.shape[0], cache.shape[0] * cache.shape[1], eps,
+        _ptr(runtime(q.device).status), _stream())
+    _native.check(rc, "mla_prepare")
+    _count()
