@@ -160,7 +160,7 @@ mla_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   const long long first = p.first[seq];
   const int row0 = ((int)gridDim.y - 1 - (int)blockIdx.y) * 256;                   // the longest rows first
   if (row0 >= qlen) return;
-  if (qlen > p.max_q_len || qs < 0 || (long long)qs + qlen > p.q_rows || first + ((ctx + 127) & ~127) > p.kv_rows) {
+  if (qlen > p.max_q_len || p.ctx_len[seq] > p.max_ctx || qs < 0 || (long long)qs + qlen > p.q_rows || first + ((ctx + 127) & ~127) > p.kv_rows) {
     if (tid == 0 && p.status) atomicCAS(p.status, 0u, MB_ST_BOUNDS);
     return;
   }

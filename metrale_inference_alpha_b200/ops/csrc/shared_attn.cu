@@ -110,7 +110,7 @@ __global__ void __launch_bounds__(256) shared_join_kernel(const MbSharedArgs p, 
       int doubles, singles;
       unit_count<D>(rows, doubles, singles);
       const int W = plan.base[p.groups];
-      const Share share(W, used_ctas<D>(W, ws.ctas));
+      const Share share(W, used_ctas(W, ws.ctas));
       const int two = row < doubles * 256, u = two ? row >> 8 : (row - doubles * 256) >> 7;
       const int at = plan.base[lo] + kvh * line_of_head<D>(rows, tiles) + (two ? 2 * tiles * u : (2 * doubles + u) * tiles);
       const int side = two ? (row >> 7) & 1 : 0, sides = two || D == 256 ? 1 : 2;

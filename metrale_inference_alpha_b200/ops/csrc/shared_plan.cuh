@@ -17,7 +17,6 @@ template <int D>
 struct Shape {
   static constexpr bool kDouble = D <= 128;                // double units
   static constexpr int kT = kDouble ? 128 : 64;            // cached tokens of a tile
-  static constexpr int kLeast = 1;
 };
 
 // Groups of a call, in shared memory: first sequences (rising and inside the batch, whatever the caller's are), rows of the prefix, first place on the line
@@ -118,9 +117,8 @@ struct Share {
   __device__ __forceinline__ int first(int c) const { return c * each + min(c, more); }
   __device__ __forceinline__ int owner(int x) const { return x < more * (each + 1) ? x / (each + 1) : more + (x - more * (each + 1)) / each; }
 };
-// CTAs that take part: a part of a place or two would cost the join what it saves here
-template <int D>
-__device__ __forceinline__ int used_ctas(int W, int ctas) { return max(1, min(ctas, W / Shape<D>::kLeast)); }
+// CTAs that take part: short prefixes are latency, so every place may go to a CTA of its own
+__device__ __forceinline__ int used_ctas(int W, int ctas) { return max(1, min(ctas, W)); }
 
 struct Part {
   int group, kvh, row0, rows, two;         // a unit: its first row in the group, its rows, whether it is a double one

@@ -387,7 +387,7 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
   mb::tc_fence_after();
   mb::pdl_launch_dependents();                            // behind this kernel's own wait: what the step before it wrote is there for them too
   const uint32_t tmem = s_tmem;                           // S0 0-127, S1 128-255, O0 256-, O1 384-
-  const int W = plan.base[p.groups], used = used_ctas<D>(W, ws.ctas);
+  const int W = plan.base[p.groups], used = used_ctas(W, ws.ctas);
   const Share share(W, used);
   const bool idle = (int)blockIdx.x >= used;
   const int begin = idle ? 0 : share.first(blockIdx.x), end = idle ? 0 : share.first(blockIdx.x + 1);
@@ -798,7 +798,7 @@ __global__ void __launch_bounds__(288, 1) shared_prefix256_kernel(const MbShared
   mb::tc_fence_after();
   mb::pdl_launch_dependents();
   const uint32_t tmem = s_tmem;                           // S0 0-63, S1 64-127, O 256-511
-  const int W = plan.base[p.groups], used = used_ctas<D>(W, ws.ctas);
+  const int W = plan.base[p.groups], used = used_ctas(W, ws.ctas);
   const Share share(W, used);
   const bool idle = (int)blockIdx.x >= used;
   const int begin = idle ? 0 : share.first(blockIdx.x), end = idle ? 0 : share.first(blockIdx.x + 1);

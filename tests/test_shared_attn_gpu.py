@@ -333,3 +333,58 @@ def test_latent_prompt_agrees_with_the_absorbed_form():
     got = run_latent(c).float()
     # roundings of queries, keys, values and weights to bf16 on either side, of values of about one over 64 tokens and more
     assert float((got - want).abs().max()) < 0.05 and float((got - want).square().mean().sqrt()) < 0.004
+
+
+def test_a_latent_prompt_with_more_cached_tokens_than_stated_is_left_out():
+    c = oracle.latent(60, [30, 20], [64, 48], 4)
+    want = oracle.latent_exact(c)
+    out = run_latent(cuda(c), max_ctx=48, total_ctx=96)
+    with pytest.raises(_native.KernelError):
+        ops.check_status("cuda")
+    within(out[30:], want[0][30:], want[1][30:], "the other sequence")
+
+
+def test_calls_one_behind_the_other_without_a_pause():
+    """Calls of several kinds follow one another on a stream and take up each other's workspace: every one gives what it gives alone."""
+    cases = [(run_shared, cuda(oracle.shared(61, [20, 9, 33, 4, 700], [600], [0, 4], 40, 8, 128, True))), (run_shared, cuda(oracle.shared(62, [3], [2000], [0, 1], 8, 1, 64, False))),
+             (run_latent, cuda(oracle.latent(63, [140, 30], [200, 60], 16))), (run_shared, cuda(oracle.shared(64, [50, 1], [90, 30], [0, 1, 2], 16, 2, 256, True, n=3))),
+             (run_latent, cuda(oracle.latent(65, [5], [1500], 2)))]
+    flat = lambda x: x if isinstance(x, tuple) else (x,)
+    alone = []
+    for run, c in cases:
+        alone.append([t.clone() for t in flat(run(c))])
+        torch.cuda.synchronize()
+    kept = [(i, flat(cases[i][0](cases[i][1]))) for _ in range(8) for i in (0, 1, 2, 3, 4, 3, 1, 0, 2)]
+    joined = [ops.merge_attention([o[0], o[0]], [o[1], o[1]]) for i, o in kept if len(o) == 2]
+    for i, o in kept:
+        assert all(torch.equal(a, b) for a, b in zip(o, alone[i])), i
+    for (i, o), (out, lse) in zip([k for k in kept if len(k[1]) == 2], joined):
+        assert torch.equal(out, o[0])
+
+
+def test_calls_on_two_streams_at_once():
+    cases = [(run_shared, cuda(oracle.shared(66, [20, 9, 33, 4], [3000], [0, 4], 40, 8, 128, True))), (run_latent, cuda(oracle.latent(67, [300], [900], 8)))]
+    alone = [run(c) for run, c in cases]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    for _ in range(10):
+        for k, (run, c) in enumerate(cases):
+            with torch.cuda.stream(streams[k]):
+                got[k].append(run(c))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o[0], alone[0][0]) and torch.equal(o[1], alone[0][1]) for o in got[0]) and all(torch.equal(o, alone[1]) for o in got[1])
+
+
+@pytest.mark.parametrize("seed", range(12))
+def test_shared_prefixes_of_random_shapes(seed):
+    g = torch.Generator().manual_seed(1000 + seed)
+    pick = lambda lo, hi: int(torch.randint(lo, hi + 1, (1,), generator=g))
+    S, n = pick(1, 40), pick(1, 4)
+    dim = (64, 128, 256)[pick(0, 2)]
+    kv = pick(1, 5)
+    heads = kv * pick(1, 12)
+    groups = pick(0, 5)
+    start = sorted(pick(0, S) for _ in range(groups + 1)) if groups else [0]
+    prefix = [pick(0, 900) if pick(0, 3) else pick(0, 3) for _ in range(groups)]
+    ctx = [pick(0, 1) if pick(0, 4) == 0 else pick(0, 150) for _ in range(S)]
+    check_shared(oracle.shared(2000 + seed, ctx, prefix, start, heads, kv, dim, bool(seed & 1), block=(16, 32, 8, 6)[seed % 4], n=n))
