@@ -49,128 +49,133 @@ Ws workspace(const MbSharedArgs& a) {
   return w;
 }
 
-// 32 rows (tokens x heads of a group) of a kv head and 32 dims a CTA, lane = row. A row's partial results are shared out over the eight warps, each of
+// 32 rows (tokens x heads of a group) of a kv head and 32 dims at a time, lane = row. A row's partial results are shared out over the eight warps, each of
 // which asks for maximum, sum and dims together, and the warps' sums are joined in shared memory: few rows have many parts, and their latencies do not add up.
-constexpr int kJoinDims = 32;
+// Bound by latency: 2 to 3 us a unit, of which the first begin before the kernels in front are through. As many CTAs as fit walk the units: with a CTA for
+// each, many of them came up late to plan again (the whole call 89.2 us instead of 87.2 for 128 sequences, 53.3 instead of 50.1 for 64 tokens behind 5000).
+constexpr int kJoinDims = 32, kJoinCtas = 3;
 
 template <int D, bool FP8>
-__global__ void __launch_bounds__(256) shared_join_kernel(const MbSharedArgs p, const Ws ws, int tok0, int tokens) {
+__global__ void __launch_bounds__(256, kJoinCtas) shared_join_kernel(const MbSharedArgs p, const Ws ws, int tok0, int tokens) {
   __shared__ Plan plan;
   __shared__ float4 s_o[8][kJoinDims / 4][32];
   __shared__ float2 s_ml[8][32];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = ws.G, kvh = blockIdx.y;
-  constexpr int kC = kJoinDims / 4;
-  const int c0 = blockIdx.z * kC;                          // fours of dims
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = ws.G;
+  constexpr int kC = kJoinDims / 4, kCuts = D / kJoinDims;
   // What is planned by stood before the kernels in front, which have waited for it before they let this one come up: only what they write is waited for
   const bool prefixes = p.groups > 0 && p.max_prefix > 0;
   if (prefixes) {
     if (warp == 0) make_plan<D>(p, plan, ws.per_seq, lane);
     __syncthreads();
   }
-  const int R = blockIdx.x * 32 + lane;                    // of the step's rows
-  const bool live = R < tokens * G;
-  const int step_tok = live ? R / G : 0, head = live ? R - step_tok * G : 0, tok = tok0 + step_tok, seq = tok / p.q_len;
-  float m = -INFINITY, l = 0.f;
-  float4 acc[kC];
+  const int part_tokens = part_tokens_of(p.Hkv, D), blocks = (tokens * G + 31) / 32, units = blocks * p.Hkv * kCuts;
+  bool waited = false;
+#pragma unroll 1
+  for (int u = blockIdx.x; u < units; u += gridDim.x) {
+    const int kvh = u / kCuts % p.Hkv, c0 = u % kCuts * kC;  // fours of dims
+    const int R = u / (kCuts * p.Hkv) * 32 + lane;         // of the step's rows
+    const bool live = R < tokens * G;
+    const int step_tok = live ? R / G : 0, head = live ? R - step_tok * G : 0, tok = tok0 + step_tok, seq = tok / p.q_len;
+    float m = -INFINITY, l = 0.f;
+    float4 acc[kC];
 #pragma unroll
-  for (int c = 0; c < kC; ++c) acc[c] = make_float4(0.f, 0.f, 0.f, 0.f);
-  auto add = [&](float2 ml, const float4* x) {
-    const bool none = ml.y == 0.f;                         // nothing seen: what lies there does not count
-    const float mn = none ? m : fmaxf(m, ml.x), base = mn == -INFINITY ? 0.f : mn;      // all scores NaN leave no maximum, but a sum that is NaN
-    const float fa = m == -INFINITY ? 0.f : ex2(m - base), fb = ml.x == -INFINITY ? 1.f : ex2(ml.x - base);
-    m = mn;
-    if (none) return;
-    l = l * fa + ml.y * fb;
-#pragma unroll
-    for (int c = 0; c < kC; ++c) {
-      acc[c].x = acc[c].x * fa + x[c].x * fb;
-      acc[c].y = acc[c].y * fa + x[c].y * fb;
-      acc[c].z = acc[c].z * fa + x[c].z * fb;
-      acc[c].w = acc[c].w * fa + x[c].w * fb;
-    }
-  };
-  int own = 0, own_parts = 0;                              // asked for beside the prefix's parts
-  if (live && p.max_ctx > 0) {
-    own = min(max(p.ctx_len[seq], 0), p.max_ctx);
-    own = max(0, own - p.q_len + (tok - seq * p.q_len) + 1);
-    own_parts = own > 0 ? own_part_count(own, part_tokens_of(p.Hkv, D)) : 0;
-  }
-  mb::pdl_wait();
-  int at_warp = warp;                                      // this warp's next part of those that come
-  if (live && prefixes && seq >= plan.start[0] && seq < plan.start[p.groups]) {
-    int lo = 0, hi = p.groups;                             // start[lo] <= seq < start[hi]
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (plan.start[mid] <= seq) lo = mid;
-      else hi = mid;
-    }
-    const int rows = row_count(plan, lo, ws.per_seq), tiles = (plan.len[lo] + Shape<D>::kT - 1) / Shape<D>::kT;
-    if (tiles > 0) {
-      const int row = (tok - plan.start[lo] * p.q_len) * G + head;
-      int doubles, singles;
-      unit_count<D>(rows, doubles, singles);
-      const int W = plan.base[p.groups];
-      const Share share(W, used_ctas(W, ws.ctas));
-      const int two = row < doubles * 256, u = two ? row >> 8 : (row - doubles * 256) >> 7;
-      const int at = plan.base[lo] + kvh * line_of_head<D>(rows, tiles) + (two ? 2 * tiles * u : (2 * doubles + u) * tiles);
-      const int side = two ? (row >> 7) & 1 : 0, sides = two || D == 256 ? 1 : 2;
-      const int cta0 = share.owner(at), n = (share.owner(at + ((tiles - 1) << two)) - cta0 + 1) * sides;
-      for (; at_warp < n; at_warp += 8) {
-        const int c = cta0 + at_warp / sides, k = at_warp % sides;
-        int t0, t1;
-        tiles_in(at, tiles, two, share.first(c), share.first(c + 1), t0, t1);
-        if (t1 <= t0) continue;
-        const Place from = t0 == 0 ? place_first<D>(p, ws, plan, lo, kvh, row, k) : place_rest<D>(p, ws, c, two ? side : k);
-        const int r = t0 == 0 ? 0 : row & 127;
-        float4 x[kC];
-        const float2 ml = __ldcg(from.ml + r);
-#pragma unroll
-        for (int i = 0; i < kC; ++i) x[i] = __ldcg(from.o + (c0 + i) * from.pitch + r);
-        add(ml, x);
-      }
-      at_warp -= n;
-    }
-  }
-  {
-    const size_t at = ((size_t)step_tok * p.Hq + kvh * G + head) * ws.parts;
-    const float4* o = reinterpret_cast<const float4*>(reinterpret_cast<const uint8_t*>(p.ws) + ws.own) + at * (D / 4) + c0;
-    const float2* ml = reinterpret_cast<const float2*>(reinterpret_cast<const uint8_t*>(p.ws) + ws.own_ml) + at;
-    for (; at_warp < own_parts; at_warp += 8) {
+    for (int c = 0; c < kC; ++c) acc[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto add = [&](const float2* pml, const float4* px, size_t pitch) {
+      const float2 ml = __ldcg(pml);
       float4 x[kC];
-      const float2 y = __ldcg(ml + at_warp);
 #pragma unroll
-      for (int c = 0; c < kC; ++c) x[c] = __ldcg(o + (size_t)at_warp * (D / 4) + c);
-      add(y, x);
+      for (int c = 0; c < kC; ++c) x[c] = __ldcg(px + c * pitch);
+      const bool none = ml.y == 0.f;                       // nothing seen: what lies there does not count
+      const float mn = none ? m : fmaxf(m, ml.x), base = mn == -INFINITY ? 0.f : mn;    // all scores NaN leave no maximum, but a sum that is NaN
+      const float fa = m == -INFINITY ? 0.f : ex2(m - base), fb = ml.x == -INFINITY ? 1.f : ex2(ml.x - base);
+      m = mn;
+      if (none) return;
+      l = l * fa + ml.y * fb;
+#pragma unroll
+      for (int c = 0; c < kC; ++c) {
+        acc[c].x = acc[c].x * fa + x[c].x * fb;
+        acc[c].y = acc[c].y * fa + x[c].y * fb;
+        acc[c].z = acc[c].z * fa + x[c].z * fb;
+        acc[c].w = acc[c].w * fa + x[c].w * fb;
+      }
+    };
+    int own_parts = 0;                                     // asked for beside the prefix's parts
+    if (live && p.max_ctx > 0) {
+      const int own = max(0, min(max(p.ctx_len[seq], 0), p.max_ctx) - p.q_len + (tok - seq * p.q_len) + 1);
+      own_parts = own > 0 ? own_part_count(own, part_tokens) : 0;
     }
-  }
-  s_ml[warp][lane] = make_float2(m, l);
+    if (!waited) mb::pdl_wait();
+    waited = true;
+    int at_warp = warp;                                    // this warp's next part of those that come
+    if (live && prefixes && seq >= plan.start[0] && seq < plan.start[p.groups]) {
+      int lo = 0, hi = p.groups;                           // start[lo] <= seq < start[hi]
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (plan.start[mid] <= seq) lo = mid;
+        else hi = mid;
+      }
+      const int rows = row_count(plan, lo, ws.per_seq), tiles = (plan.len[lo] + Shape<D>::kT - 1) / Shape<D>::kT;
+      if (tiles > 0) {
+        const int row = (tok - plan.start[lo] * p.q_len) * G + head;
+        int doubles, singles;
+        unit_count<D>(rows, doubles, singles);
+        const int W = plan.base[p.groups];
+        const Share share(W, used_ctas(W, ws.ctas));
+        const int two = row < doubles * 256, v = two ? row >> 8 : (row - doubles * 256) >> 7;
+        const int at = plan.base[lo] + kvh * line_of_head<D>(rows, tiles) + (two ? 2 * tiles * v : (2 * doubles + v) * tiles);
+        const int side = two ? (row >> 7) & 1 : 0, sides = two || D == 256 ? 1 : 2;
+        const int cta0 = share.owner(at), ctas = share.owner(at + ((tiles - 1) << two)) - cta0 + 1, n = ctas * sides;      // first sides in front
+        for (; at_warp < n; at_warp += 8) {
+          const int k = at_warp >= ctas, c = cta0 + at_warp - k * ctas;
+          int t0, t1;
+          tiles_in(at, tiles, two, share.first(c), share.first(c + 1), t0, t1);
+          if (t1 - t0 <= k) continue;                        // of one tile the second side has nothing (8 rows behind 700: 16.9 us, 18.5 with it read)
+          const Place from = t0 == 0 ? place_first<D>(p, ws, plan, lo, kvh, row, k) : place_rest<D>(p, ws, c, two ? side : k);
+          const int r = t0 == 0 ? 0 : row & 127;
+          add(from.ml + r, from.o + c0 * from.pitch + r, from.pitch);
+        }
+        at_warp -= n;
+      }
+    }
+    const size_t own_at = ((size_t)step_tok * p.Hq + kvh * G + head) * ws.parts;
+    for (; at_warp < own_parts; at_warp += 8) {
+      const size_t at = own_at + at_warp;
+      add(reinterpret_cast<const float2*>(reinterpret_cast<const uint8_t*>(p.ws) + ws.own_ml) + at,
+          reinterpret_cast<const float4*>(reinterpret_cast<const uint8_t*>(p.ws) + ws.own) + at * (D / 4) + c0, 1);
+    }
+    s_ml[warp][lane] = make_float2(m, l);
 #pragma unroll
-  for (int c = 0; c < kC; ++c) s_o[warp][c][lane] = acc[c];
-  __syncthreads();
-  // warp w sums dims 4 w to 4 w + 3 of the 32 rows
-  float mx = -INFINITY;
-  float2 ml[8];
+    for (int c = 0; c < kC; ++c) s_o[warp][c][lane] = acc[c];
+    __syncthreads();
+    // warp w sums dims 4 w to 4 w + 3 of the 32 rows
+    float mx = -INFINITY;
+    float2 ml[8];
 #pragma unroll
-  for (int w = 0; w < 8; ++w) {
-    ml[w] = s_ml[w][lane];
-    if (ml[w].y != 0.f) mx = fmaxf(mx, ml[w].x);
-  }
-  const float base = mx == -INFINITY ? 0.f : mx;
-  float sum = 0.f;
-  float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int w = 0; w < 8; ++w) {
+      ml[w] = s_ml[w][lane];
+      if (ml[w].y != 0.f) mx = fmaxf(mx, ml[w].x);
+    }
+    const float base = mx == -INFINITY ? 0.f : mx;
+    float sum = 0.f;
+    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-  for (int w = 0; w < 8; ++w) {
-    if (ml[w].y == 0.f) continue;
-    const float f = ml[w].x == -INFINITY ? 1.f : ex2(ml[w].x - base);
-    const float4 x = s_o[w][warp][lane];
-    sum += ml[w].y * f;
-    y.x += x.x * f; y.y += x.y * f; y.z += x.z * f; y.w += x.w * f;
+    for (int w = 0; w < 8; ++w) {
+      if (ml[w].y == 0.f) continue;
+      const float f = ml[w].x == -INFINITY ? 1.f : ex2(ml[w].x - base);
+      const float4 x = s_o[w][warp][lane];
+      sum += ml[w].y * f;
+      y.x += x.x * f; y.y += x.y * f; y.z += x.z * f; y.w += x.w * f;
+    }
+    const float inv = sum == 0.f ? 0.f : (FP8 ? *p.v_scale : 1.f) / sum;
+    const uint2 out = make_uint2(pack2<false>(y.x * inv, y.y * inv), pack2<false>(y.z * inv, y.w * inv));
+    const float lse = sum == 0.f ? -INFINITY : (base + log2f(sum)) * 0.693147180559945f;
+    if (live) {
+      const size_t row = (size_t)tok * p.Hq + kvh * G + head;
+      *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(p.out) + row * D + (c0 + warp) * 4) = out;
+      if (p.lse && warp == 0 && c0 == 0) p.lse[row] = lse;
+    }
+    __syncthreads();                                       // the next unit's sums take these places
   }
-  if (!live) return;
-  const float inv = sum == 0.f ? 0.f : (FP8 ? *p.v_scale : 1.f) / sum;
-  const size_t row = (size_t)tok * p.Hq + kvh * G + head;
-  *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(p.out) + row * D + (c0 + warp) * 4) = make_uint2(pack2<false>(y.x * inv, y.y * inv), pack2<false>(y.z * inv, y.w * inv));
-  if (p.lse && warp == 0 && blockIdx.z == 0) p.lse[row] = sum == 0.f ? -INFINITY : (base + log2f(sum)) * 0.693147180559945f;
 }
 
 bool bad_shape(const MbSharedArgs& a) {
@@ -193,8 +198,9 @@ int run(const MbSharedArgs& a, const Ws& w, cudaStream_t stream) {
     // only the first step stands directly behind the prefix kernel; a later one's results take the place of what the join in front reads
     if (a.max_ctx > 0)
       if (const int rc = mb_decode_parts(a, t, n, reinterpret_cast<float*>(ws + w.own), reinterpret_cast<float*>(ws + w.own_ml), w.parts, prefixes && t == 0, stream)) return rc;
-    const long long blocks = ((long long)n * G + 31) / 32;
-    const cudaError_t e = mb::launch_kernel_ex(shared_join_kernel<D, FP8>, dim3((unsigned)blocks, a.Hkv, D / kJoinDims), dim3(256), 0, stream, 1, mb_pdl_enabled() != 0, a, w, t, n);
+    // a CTA takes several units rather than to come up late and plan again
+    const long long units = ((long long)n * G + 31) / 32 * a.Hkv * (D / kJoinDims), most = (long long)w.ctas * kJoinCtas;
+    const cudaError_t e = mb::launch_kernel_ex(shared_join_kernel<D, FP8>, dim3((unsigned)(units < most ? units : most)), dim3(256), 0, stream, 1, mb_pdl_enabled() != 0, a, w, t, n);
     if (e != cudaSuccess) return (int)e;
   }
   return 0;
