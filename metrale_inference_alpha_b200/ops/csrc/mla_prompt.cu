@@ -1,5 +1,9 @@
 // Prompts over a latent cache in expanded form: a cached row's keys and values are made for every head, k = [W_k c | rotated part], v = W_v c, and attended
 // as usual. Per head and pair 192 + 128 multiply-adds instead of the 576 + 512 of the absorbed form, for 512 x 256 a cached row and head in front.
+//
+// Three launches: cached rows to consecutive ones (7 us for 8192 of them, latency), the expansion as one plain product (47 us for 16 heads, 0.73
+// PFLOP/s: sums of 512 are short), and attention (262 us: 1.31 PFLOP/s of what the mask leaves, the tensor pipe 69 % busy, the special function units 56 %).
+// Expanded rows are bf16, as cached keys and values would be: half a step of 2^-8 each, which is as much again as the rounding of the outputs.
 #include "common.cuh"
 #include "shared_attn.h"
 #include "attention_rows.cuh"
@@ -132,9 +136,10 @@ __global__ void __launch_bounds__(256) gather_kernel(const GatherParams p) {
 //   warp 8           copies by TMA: Q once; per 128 cached tokens five pieces of 16 KB in a ring of eight: K in three spans of 64 dims (the
 //                    third is the rotated part, which all heads share), V in two halves of 64 tokens
 //   warp 9           issues the products: S0 S1 | PV0 S0' PV1 S1' | ..., so that one tile's softmax runs under the other tile's products. With a warp for
-//                    either tile's the two batches were interleaved and done at the same time, and both softmaxes then ran at once (325 us instead of 300)
+//                    either tile's the two batches were interleaved and done at the same time, and both softmaxes then ran at once (8192 tokens of 16
+//                    heads then took 325 us in place of 300)
 //   warps 10, 11     give their registers to the softmax
-// Weights through shared memory, which would let S of the next tile be made under the softmax, were slower (331 us instead of 314 for 8192 tokens of 16 heads):
+// Weights through shared memory, which would let S of the next tile be made under the softmax, were slower (331 us in place of 314 then):
 // 128 x 128 products of operands in shared memory read 128 bytes a cycle, all that it has.
 constexpr int kT = 128, kPiece = 16384, kRing = 8, kPer = 5, kThreads = 384;
 constexpr int kQTile = 3 * kPiece;

@@ -15,7 +15,12 @@
 // e4m3 keys are multiplied as they are, by queries that are the sum of two e4m3 numbers: scaled by the power of two that takes a row's largest element to
 // [2^7, 2^8), an element's 8 bits are the 4 of its rounding and a remainder of 4, which e4m3 holds exactly down to 2^-2. Elements that are less than
 // 2^-9 of the row's largest are off by 2^-17 of it at most, those under 2^-18 of it vanish. That is as many products as of f16 operands, at twice the rate;
-// keys of f16 made from e4m3 kept the converting warps busy for as long again as values do (128 sequences behind 32768 tokens 203 us).
+// keys of f16 made from e4m3 kept the converting warps busy for as long again as values do (128 sequences behind 32768 tokens 203 us in place of 149).
+//
+// What bounds it: a double tile takes some 4400 cycles, of which the softmax of either accumulator, and its products and their commits behind it, are one
+// chain; a part costs 8000 to 10000 more (queries, first copies, outputs), so that prefixes of a few tiles a CTA are latency. 128 sequences behind 8192
+// e4m3 tokens (40 / 8 heads) 48 us: the tensor pipe 29 % busy, the special function units 29 %, HBM 5 %. 61 behind five of 16000 bf16 (64 rows a
+// unit and less) 66 us: 243 MB at 3.7 TB/s.
 // Weights are f16, held 2^7 larger than the running maximum says, as in attention_rows.cu.
 #pragma once
 #include "softmax_rows.cuh"
@@ -762,7 +767,8 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
 }
 
 // Heads of 256 dims: one tile of 128 rows a CTA (its outputs are half of TMEM), tiles of 64 cached tokens, two tiles of scores in turn: the products of the
-// next one run under the softmax of this one. Warps 0-3 softmax, 4-7 loader, 8 products.
+// next one run under the softmax of this one. Warps 0-3 softmax, 4-7 loader, 8 products. Short prefixes are latency: 33 sequences behind two of 2047 bf16
+// tokens (16 / 2 heads, one to two tiles a CTA) 17 us, the tensor pipe 4 % busy, HBM 6 %.
 template <bool FP8>
 __global__ void __launch_bounds__(288, 1) shared_prefix256_kernel(const MbSharedArgs p, const Ws ws) {
   constexpr int D = 256, kT = 64, kQB = 128 * D * 2, kTileB = kT * D * 2, kSpans = D / 64;

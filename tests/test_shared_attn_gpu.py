@@ -388,3 +388,27 @@ def test_shared_prefixes_of_random_shapes(seed):
     prefix = [pick(0, 900) if pick(0, 3) else pick(0, 3) for _ in range(groups)]
     ctx = [pick(0, 1) if pick(0, 4) == 0 else pick(0, 150) for _ in range(S)]
     check_shared(oracle.shared(2000 + seed, ctx, prefix, start, heads, kv, dim, bool(seed & 1), block=(16, 32, 8, 6)[seed % 4], n=n))
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(16, 8, 128), (8, 4, 256), (32, 16, 64)])
+def test_shared_prefixes_in_a_cache_beyond_32_bits(heads, kv_heads, dim):
+    c = cuda(oracle.shared(68, [20, 90, 3], [300], [0, 3], heads, kv_heads, dim, False))
+    want = run_shared(c)
+    blocks = 150_000                                             # 16 tokens of 2048 bytes of K: 4.9 GB
+    front = blocks - c["k"].shape[0]
+    big = {**c, "table": c["table"] + front, "prefix_table": c["prefix_table"] + front}
+    for name in ("k", "v"):
+        big[name] = torch.empty(blocks, *c[name].shape[1:], dtype=torch.bfloat16, device="cuda")
+        big[name][front:] = c[name]
+    got = run_shared(big)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_latent_prompt_in_a_cache_beyond_32_bits():
+    c = cuda(oracle.latent(69, [140, 30], [200, 60], 8))
+    want = run_latent(c)
+    blocks = 250_000                                             # 16 tokens of 1152 bytes: 4.6 GB
+    front = blocks - c["cache"].shape[0]
+    big = torch.empty(blocks, 16, 1, 576, dtype=torch.bfloat16, device="cuda")
+    big[front:] = c["cache"]
+    assert torch.equal(run_latent({**c, "cache": big, "table": c["table"] + front}), want)
