@@ -1,9 +1,9 @@
 // Prompts over a latent cache in expanded form: a cached row's keys and values are made for every head, k = [W_k c | rotated part], v = W_v c, and attended
 // as usual. Per head and pair 192 + 128 multiply-adds instead of the 576 + 512 of the absorbed form, for 512 x 256 a cached row and head in front.
 //
-// Three launches: cached rows to consecutive ones (7 us for 8192 of them, latency), the expansion as one plain product (47 us for 16 heads, 0.73
-// PFLOP/s: sums of 512 are short), and attention (262 us: 1.31 PFLOP/s of what the mask leaves, the tensor pipe 69 % busy, the special function units 56 %).
-// Expanded rows are bf16, as cached keys and values would be: half a step of 2^-8 each, which is as much again as the rounding of the outputs.
+// Three launches: cached rows to consecutive ones (6 us for 8192 of them, latency), the expansion (30 us for 16 heads: 1.15 PFLOP/s), and attention
+// (260 us: 1.32 PFLOP/s of what the mask leaves, the tensor pipe 69 % busy, the special function units 56 %). Expanded rows are bf16, as cached keys and
+// values would be: half a step of 2^-8 each, which is as much again as the rounding of the outputs.
 #include "common.cuh"
 #include "shared_attn.h"
 #include "attention_rows.cuh"
@@ -12,6 +12,8 @@
 #include "tensormap.h"
 
 namespace {
+
+using namespace mbr;
 
 constexpr int kRow = 576, kLat = 512, kQk = 192, kNope = 128, kV = 128;
 
@@ -131,6 +133,160 @@ __global__ void __launch_bounds__(256) gather_kernel(const GatherParams p) {
   }
 }
 
+// ---- expansion: kv[row, head, 256] = w[head] c[row], a product whose sums are 512 long
+// A pair of CTAs owns units of 256 cached rows of one head (tcgen05.mma.cta_group::2, M = N = 256). Its rows stay in shared memory, 128 of them in either
+// CTA, while the heads' weights go by, half of a head's in either: with rows fetched again for every head, as the plain product of gemm_rows.cu does, 16
+// heads of 8192 rows read 268 MB out of L2 at some 6 TB/s and took 45 us; here it is half of that, and 30 us. The ring is as deep as shared memory lets it
+// be: weights come as fast as its 96 KB cover L2's latency (of five places 33 us). Units are numbered heads fastest and shared out in runs of equal length.
+//   warp 0      weights by TMA, 64 of the 512 at a time, a ring of six        warp 10   rows, when a run comes to others
+//   warp 1      the leader's issues the products, two accumulators in turn    warps 2-9 take them to bf16, lane = row
+constexpr int kExpThreads = 352, kExpRing = 6, kExpK = kLat / 64, kExpPiece = 128 * 128;
+constexpr int kExpSmem = (kExpK + kExpRing) * kExpPiece + 1024;
+
+struct ExpandParams {
+  __nv_bfloat16* out;        // [rows, heads, 256]
+  long long rows;
+  int heads, units;
+  uint32_t* status;
+};
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kExpThreads, 1)
+expand_kernel(const __grid_constant__ CUtensorMap tmC, const __grid_constant__ CUtensorMap tmW, const ExpandParams p) {
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  uint8_t* sC = smem_raw + ((1024u - (mb::smem_u32(smem_raw) & 1023u)) & 1023u);   // 8 x [128 rows x 128 B]
+  uint8_t* sW = sC + kExpK * kExpPiece;
+  __shared__ __align__(8) uint64_t c_full[kExpK], w_full[kExpRing];                // used in the leader: both CTAs' bytes
+  __shared__ __align__(8) uint64_t c_empty, w_empty[kExpRing], acc_full[2];        // in each CTA
+  __shared__ __align__(8) uint64_t acc_empty[2];                                   // used in the leader: both CTAs' warps
+  __shared__ uint32_t s_tmem;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = mb::cluster_rank();
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const int u0 = (int)((long long)p.units * pair / pairs), u1 = (int)((long long)p.units * (pair + 1) / pairs);
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kExpK; ++i) mb::mbar_init(&c_full[i], 1);
+    for (int i = 0; i < kExpRing; ++i) {
+      mb::mbar_init(&w_full[i], 1);
+      mb::mbar_init(&w_empty[i], 1);
+    }
+    mb::mbar_init(&c_empty, 1);
+    for (int i = 0; i < 2; ++i) {
+      mb::mbar_init(&acc_full[i], 1);
+      mb::mbar_init(&acc_empty[i], 2 * 8);
+    }
+    mb::mbar_fence_init();
+  }
+  if (warp == 1) mb::tmem_alloc2(&s_tmem, 512);
+  mb::tc_fence_before();
+  __syncthreads();
+  mb::cluster_sync_all();                                  // barriers of both CTAs stand before either signals the other
+  mb::tc_fence_after();
+  const uint32_t tmem = s_tmem;
+  mb::pdl_launch_dependents();
+  if (warp == 0) {
+    if (mb::elect_one()) {
+      // weights stood before the kernel in front, which has waited for them: they are not waited for
+      const int total = (u1 - u0) * kExpK;
+      int g = 0;
+      for (; g < total; ++g) {
+        const int s = g % kExpRing, h = (u0 + g / kExpK) % p.heads;
+        if (!mb::mbar_wait(&w_empty[s], ((g / kExpRing) & 1) ^ 1, p.status, MB_ST_TIMEOUT_TMA)) break;
+        if (rank == 0) mb::mbar_expect_tx(&w_full[s], 2 * kExpPiece);
+        mb::tma_load_2d_pair(sW + s * kExpPiece, &tmW, mb::dsmem_addr(mb::smem_u32(&w_full[s]), 0), g % kExpK * 64, h * 256 + (int)rank * 128);
+      }
+      // given up: the leader sees both CTAs' copies through, or waits until its waits give up; the pair leaves together
+      if (g < total && rank == 0)
+        for (int i = g > kExpRing ? g - kExpRing : 0; i < g; ++i) mb::mbar_wait(&w_full[i % kExpRing], (i / kExpRing) & 1, p.status, MB_ST_TIMEOUT_TMA);
+    }
+    __syncwarp();
+  } else if (warp == 10) {
+    if (mb::elect_one()) {
+      mb::pdl_wait();
+      int run = 0;
+      for (int u = u0; u < u1; u += p.heads - u % p.heads, ++run) {
+        const bool ok = run == 0 || mb::mbar_wait(&c_empty, (run - 1) & 1, p.status, MB_ST_TIMEOUT_TMA);
+        if (!ok) {
+          if (rank == 0)
+            for (int i = 0; i < kExpK; ++i) mb::mbar_wait(&c_full[i], (run - 1) & 1, p.status, MB_ST_TIMEOUT_TMA);
+          break;
+        }
+        for (int i = 0; i < kExpK; ++i) {
+          if (rank == 0) mb::mbar_expect_tx(&c_full[i], 2 * kExpPiece);
+          mb::tma_load_2d_pair(sC + i * kExpPiece, &tmC, mb::dsmem_addr(mb::smem_u32(&c_full[i]), 0), i * 64, (u / p.heads * 2 + (int)rank) * 128);
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (rank == 0 && mb::elect_one()) {
+      constexpr uint32_t kId = mb::umma_idesc(1, 1, 256, 256);
+      const uint64_t dC = mb::umma_desc_sw128(mb::smem_u32(sC)), dW = mb::umma_desc_sw128(mb::smem_u32(sW));
+      bool ok = true;
+      int g = 0, run = 0;
+      for (int u = u0; u < u1 && ok; ++u) {
+        const int it = u - u0, buf = it & 1;
+        const bool fresh = u == u0 || u % p.heads == 0;    // the first unit of these rows
+        if (fresh && u > u0) ++run;
+        ok = mb::mbar_wait(&acc_empty[buf], ((it >> 1) & 1) ^ 1, p.status, MB_ST_TIMEOUT_MMA);
+        for (int i = 0; i < kExpK && ok; ++i, ++g) {
+          const int s = g % kExpRing;
+          if (fresh) ok = mb::mbar_wait(&c_full[i], run & 1, p.status, MB_ST_TIMEOUT_MMA);
+          ok = ok && mb::mbar_wait(&w_full[s], (g / kExpRing) & 1, p.status, MB_ST_TIMEOUT_MMA);
+          if (!ok) break;
+          mb::tc_fence_after();
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            mb::umma2_f16(tmem + buf * 256, dC + i * (kExpPiece >> 4) + ((j * 32) >> 4), dW + s * (kExpPiece >> 4) + ((j * 32) >> 4), kId, (i | j) != 0);
+          mb::tc_commit2(&w_empty[s]);
+        }
+        if (!ok) break;
+        // the last signal that the pair waits for comes last: none may arrive at a CTA that has left
+        if ((u + 1) % p.heads == 0 && u + 1 < u1) mb::tc_commit2(&c_empty);
+        mb::tc_commit2(&acc_full[buf]);
+      }
+    }
+    __syncwarp();
+  } else {
+    const int q = warp & 3, half = (warp - 2) >> 2;
+    const uint32_t src = tmem + ((uint32_t)(q * 32) << 16) + half * 128;
+    const uint32_t empty0 = mb::dsmem_addr(mb::smem_u32(&acc_empty[0]), 0);
+    mb::pdl_wait();                                        // the results' place may still be read by the kernels in front of the one in front
+    for (int u = u0; u < u1; ++u) {
+      const int it = u - u0, buf = it & 1, h = u % p.heads;
+      const long long row = (long long)(u / p.heads) * 256 + (int)rank * 128 + q * 32 + lane;
+      const bool ok = mb::mbar_wait(&acc_full[buf], (it >> 1) & 1, p.status, MB_ST_TIMEOUT_EPI);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      mb::tc_fence_after();
+      float v[128];
+#pragma unroll
+      for (int c = 0; c < 128; c += 32) mb::tmem_ld32_async(src + buf * 256 + c, v + c);
+      mb::tmem_ld_wait(v);
+      mb::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mb::mbar_arrive_cluster(empty0 + buf * 8);
+      if (row < p.rows) {
+        __nv_bfloat16* dst = p.out + ((size_t)row * p.heads + h) * 256 + half * 128;
+#pragma unroll
+        for (int c = 0; c < 128; c += 16) {                // whole sectors: a warp's store touches 32 rows
+          uint32_t w[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) w[i] = pack2<false>(v[c + 2 * i], v[c + 2 * i + 1]);
+          asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst + c), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]),
+                       "r"(w[6]), "r"(w[7])
+                       : "memory");
+        }
+      }
+    }
+    mb::tc_fence_before();
+  }
+  __syncthreads();
+  mb::cluster_sync_all();                                  // nothing of the pair signals or reads a CTA that has left
+  if (warp == 1) {
+    mb::tc_fence_after();
+    mb::tmem_dealloc2(tmem, 512);
+  }
+}
+
 // ---- attention: two tiles of 128 query tokens of one head a CTA on the tensor cores
 //   warps 0-3, 4-7   softmax of row tile 0 / 1, thread = row: S from TMEM, the weights back to TMEM (over S) in two halves of 64 tokens
 //   warp 8           copies by TMA: Q once; per 128 cached tokens five pieces of 16 KB in a ring of eight: K in three spans of 64 dims (the
@@ -145,7 +301,6 @@ constexpr int kT = 128, kPiece = 16384, kRing = 8, kPer = 5, kThreads = 384;
 constexpr int kQTile = 3 * kPiece;
 constexpr int kSmem = 2 * kQTile + kRing * kPiece + 1024;
 
-using namespace mbr;
 template <int N>
 __device__ __forceinline__ void more_regs() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N>
@@ -449,19 +604,34 @@ int mb_mla_prompt(const MbMlaPromptArgs* a, cudaStream_t stream) {
   static std::atomic<uint64_t> asked{0};
   e = mb::allow_smem(reinterpret_cast<const void*>(mla_prompt_kernel), kSmem, asked);
   if (e != cudaSuccess) return (int)e;
-  CUtensorMap tm[4];
+  static std::atomic<uint64_t> asked_too{0};
+  e = mb::allow_smem(reinterpret_cast<const void*>(expand_kernel), kExpSmem, asked_too);
+  if (e != cudaSuccess) return (int)e;
+  const int pairs = a->sm_count > 1 ? a->sm_count / 2 : 74;
+  CUtensorMap tm[5];
   int rc = mbh::encode_2d(&tm[0], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, a->q, (uint64_t)a->H * kQk, a->q_rows, (uint64_t)a->H * kQk * 2, 64, 128);
   if (!rc) rc = mbh::encode_2d(&tm[3], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, ws, kRow, a->kv_rows, kRow * 2, 64, 128);
   for (int h = 0; h < a->H && !rc; h += a->each) {
     const int n = a->H - h < a->each ? a->H - h : a->each;
-    MbGemmArgs m{};
-    m.M = (int)a->kv_rows; m.N = n * 256; m.K = kLat; m.ldo = n * 256;
-    m.W = reinterpret_cast<const __nv_bfloat16*>(a->w) + (size_t)h * 256 * kLat;
-    m.X = ws; m.ldx = kRow; m.out = ws + l.kv; m.alpha = 1.f; m.status = a->status; m.sm_count = a->sm_count;
-    m.flags = a->gemm_flags;                               // without a workspace the product is not split
-    rc = mb_gemm(&m, stream);
-    if (!rc) rc = mbh::encode_2d(&tm[1], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, m.out, (uint64_t)n * 256, a->kv_rows, (uint64_t)n * 512, 64, 128);
-    if (!rc) rc = mbh::encode_2d(&tm[2], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, m.out, (uint64_t)n * 256, a->kv_rows, (uint64_t)n * 512, 64, 64);
+    const __nv_bfloat16* wh = reinterpret_cast<const __nv_bfloat16*>(a->w) + (size_t)h * 256 * kLat;
+    void* kv = ws + l.kv;
+    const long long units = (a->kv_rows + 255) / 256 * n;
+    if (units > 0x7fffffff) return MB_ERR_TOO_LARGE;
+    // rows of one unit are fetched once by either kernel, and mb_gemm has tiles of half the size for them. The whole call, here / by mb_gemm: 128 rows of 128
+    // heads 30.7 / 27.2 us, of 64 24.4 / 24.6; 384 rows of 128 59.9 / 65.7, 512 of 64 36.0 / 36.8, 1024 of 16 34.9 / 36.9, of 64 59.6 / 70.3, 8192 of 16 294 / 306
+    if (a->kv_rows > 256) {
+      const ExpandParams x{(__nv_bfloat16*)kv, a->kv_rows, n, (int)units, a->status};
+      rc = mbh::encode_2d(&tm[4], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, wh, kLat, (uint64_t)n * 256, kLat * 2, 64, 128);
+      if (!rc) rc = (int)mb::launch_kernel_cluster(expand_kernel, dim3(2 * (unsigned)(units < pairs ? units : pairs)), dim3(kExpThreads), kExpSmem, stream, 1, tm[3], tm[4], x);
+    } else {
+      MbGemmArgs m{};
+      m.M = (int)a->kv_rows; m.N = n * 256; m.K = kLat; m.ldo = n * 256; m.W = wh;
+      m.X = ws; m.ldx = kRow; m.out = kv; m.alpha = 1.f; m.status = a->status; m.sm_count = a->sm_count;
+      m.flags = a->gemm_flags;                             // without a workspace the product is not split
+      rc = mb_gemm(&m, stream);
+    }
+    if (!rc) rc = mbh::encode_2d(&tm[1], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, kv, (uint64_t)n * 256, a->kv_rows, (uint64_t)n * 512, 64, 128);
+    if (!rc) rc = mbh::encode_2d(&tm[2], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, kv, (uint64_t)n * 256, a->kv_rows, (uint64_t)n * 512, 64, 64);
     if (rc) return rc;
     const AttnParams p{a->q_start, a->q_len, a->ctx_len, first, bad, a->out, a->status, a->q_rows, a->kv_rows, a->H, h, a->max_q_len, a->max_ctx, a->scale};
     rc = (int)mb::launch_kernel_ex(mla_prompt_kernel, dim3(n, tiles, a->num_seqs), dim3(kThreads), kSmem, stream, 1, mb_pdl_enabled() != 0, tm[0], tm[1], tm[2], tm[3], p);

@@ -412,3 +412,11 @@ def test_latent_prompt_in_a_cache_beyond_32_bits():
     big = torch.empty(blocks, 16, 1, 576, dtype=torch.bfloat16, device="cuda")
     big[front:] = c["cache"]
     assert torch.equal(run_latent({**c, "cache": big, "table": c["table"] + front}), want)
+
+
+@pytest.mark.parametrize("new,ctx,heads", [([257], [257], 1), ([100, 300], [129, 641], 3), ([40, 8, 30], [384, 8, 1500], 21), ([64], [1200], 80), ([16] * 9, [130] * 9, 5)])
+def test_latent_prompt_rows_of_many_heads(new, ctx, heads):
+    """Units of the expansion that begin and end inside a run of heads, odd numbers of 128 rows, more pairs of CTAs than units and fewer."""
+    c = oracle.latent(70, new, ctx, heads)
+    want = oracle.latent_exact(c)
+    within(run_latent(cuda(c)), want[0], want[1], "outputs")
