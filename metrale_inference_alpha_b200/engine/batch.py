@@ -42,9 +42,6 @@ class ForwardBatch:
     logit_rows: torch.Tensor           # [R] int64 rows whose logits are needed
     max_q_len: int = 1
     max_ctx: int = 0
-    # sums over the sequences, known on the host: of ctx_len, and of the (row, visible token) pairs; 0 in batches of a fixed shape (graph rungs)
-    total_ctx: int = 0
-    total_pairs: int = 0
     state_slots: Optional[torch.Tensor] = None   # [S] int32 recurrent-state slot per sequence
     num_tokens: int = 0
     num_seqs: int = 0
@@ -61,6 +58,9 @@ class ForwardBatch:
     rope_rows: Optional[torch.Tensor] = None     # arange(T) int32: row -> its rotary row
     # speculative verify over recurrent layers: state is left untouched and inputs are retained here
     spec_stash: Optional[SpecStash] = None
+    # sums over the sequences, known on the host: of ctx_len, and of the (row, visible token) pairs; 0 in batches of a fixed shape (graph rungs)
+    total_ctx: int = 0
+    total_pairs: int = 0
 
     @property
     def device(self):

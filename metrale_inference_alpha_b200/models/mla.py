@@ -114,11 +114,11 @@ def _expanded_pays(batch) -> bool:
 
 def keep_joined(cfg, weights) -> None:
     """For the expanded form: keeps [W_uk | W_uv] of every latent layer as one tensor, of which the two become views, so that nothing is held twice.
-    Layers of other sizes, and weights that are not on a GPU, stay as they are (and absorbed)."""
+    To be called before a graph is captured over the two. Layers of other sizes, and weights that are not on a GPU, stay as they are (and absorbed)."""
     layers = list(weights.layers) + ([weights.mtp.layer] if weights.mtp is not None else [])
     for lw in layers:
         w = lw.mixer
-        if lw.kind != "mla" or not w.w_uk.is_cuda or w.w_uk.shape[1:] != (mla_prompt.NOPE, mla_prompt.LATENT) \
+        if lw.kind != "mla" or hasattr(w, "_w_kv_bf16") or not w.w_uk.is_cuda or w.w_uk.shape[1:] != (mla_prompt.NOPE, mla_prompt.LATENT) \
                 or w.w_uv.shape[1:] != (mla_prompt.VALUE, mla_prompt.LATENT) or cfg.qk_rope_dim != mla_prompt.ROPE:
             continue
         joined = w._w_kv_bf16 = torch.cat([w.w_uk, w.w_uv], 1).to(torch.bfloat16).contiguous()
