@@ -1,8 +1,7 @@
 // Attention that was computed in parts over disjoint keys, joined: lse = ln sum_i exp l_i, out = sum_i exp(l_i - lse) o_i. A part of weight zero (l_i = -inf)
 // is not read, so what it holds does not matter; a row without weight gives zeros and -inf. One pass over the parts, bound by memory: a thread asks for the
 // same 16 bytes of all parts, of ITEMS rows, before it uses any of them. Weights and sums are 32 bits. Five parts of 8191 x 32 rows of 128 fp32 dims
-// (811 MB) take 136 us, 6.0 TB/s; 8 of 4096 x 40 bf16 58 us, 6.6 TB/s. With four rows a thread in place of two, and two in place of one for more than four
-// parts, the former takes 171 us: registers leave too few warps.
+// (811 MB) take 125 us, 6.5 TB/s; 8 of 4096 x 40 bf16 58 us, 6.6 TB/s; 16 of 2048 x 40 bf16 77 us, 4.7 TB/s.
 #include "common.cuh"
 #include "shared_attn.h"
 #include <type_traits>
@@ -71,10 +70,14 @@ int launch(const MbMergeArgs& a, cudaStream_t stream) {
   return (int)mb::launch_kernel(merge_kernel<T, V, PARTS, ITEMS>, dim3((unsigned)n), dim3(256), 0, stream, a);
 }
 
+// What is in flight is a thread's loads times the threads, and registers bound the one by the other: five fp32 parts in the kernel of eight 135 us, of six 125,
+// of six with two rows a thread 132; four parts with two rows 105, one 103; two parts of 8191 x 32 x 128 fp32 with one row 66, two 64; ten bf16 parts in a kernel
+// of twelve 112, of sixteen 99.
 template <typename T, int V>
 int by_parts(const MbMergeArgs& a, cudaStream_t stream) {
   if (a.parts <= 2) return launch<T, V, 2, 2>(a, stream);
-  if (a.parts <= 4) return launch<T, V, 4, 2>(a, stream);
+  if (a.parts <= 4) return launch<T, V, 4, 1>(a, stream);
+  if (a.parts <= 6) return launch<T, V, 6, 1>(a, stream);
   if (a.parts <= 8) return launch<T, V, 8, 1>(a, stream);
   return launch<T, V, kMergeParts, 1>(a, stream);
 }
