@@ -176,13 +176,25 @@ __global__ void __launch_bounds__(256, kJoinCtas) shared_join_kernel(const MbSha
     }
     __syncthreads();                                       // the next unit's sums take these places
   }
+  // Lengths and groups are looked at by the kernels in front, which a maximum of 0 leaves out: what is beyond that is reported here
+  if (blockIdx.x == 0 && tok0 == 0 && p.status) {
+    bool beyond = false;
+    if (p.max_ctx == 0)
+      for (int s = tid; s < p.num_seqs; s += 256) beyond |= p.ctx_len[s] > 0;
+    if (p.max_prefix == 0)
+      for (int g = tid; g < p.groups; g += 256) {
+        const int a = p.group_start[g], b = p.group_start[g + 1];
+        beyond |= a < 0 || b > p.num_seqs || b < a || (b > a && p.prefix_len[g] > 0);
+      }
+    if (beyond) atomicCAS(p.status, 0u, MB_ST_BOUNDS);
+  }
 }
 
 bool bad_shape(const MbSharedArgs& a) {
   return a.num_seqs <= 0 || a.q_len <= 0 || a.Hkv <= 0 || a.Hkv > 65535 || a.Hq % a.Hkv || a.Hq / a.Hkv > 64 || (a.D != 64 && a.D != 128 && a.D != 256) ||
-         a.block_size <= 0 || a.num_blocks <= 0 || a.num_blocks * a.block_size >= (1ll << 31) || a.table_ld >= (1ll << 31) || a.max_prefix < 0 || a.max_ctx < 0 || !a.q ||
-         !a.k_cache || !a.v_cache || !a.ctx_len || !a.out || (a.fp8 && (!a.k_scale || !a.v_scale)) || a.groups < 0 || a.groups > kMaxGroups ||
-         (a.groups > 0 && (!a.prefix_table || !a.prefix_len || !a.group_start)) ||
+         a.block_size <= 0 || a.num_blocks < 0 || a.num_blocks * a.block_size >= (1ll << 31) || a.table_ld >= (1ll << 31) || a.max_prefix < 0 || a.max_ctx < 0 ||
+         ((a.max_prefix > 0 || a.max_ctx > 0) && (a.num_blocks == 0 || !a.k_cache || !a.v_cache)) || !a.q || !a.ctx_len || !a.out ||
+         (a.fp8 && (!a.k_scale || !a.v_scale)) || a.groups < 0 || a.groups > kMaxGroups || (a.groups > 0 && (!a.prefix_table || !a.prefix_len || !a.group_start)) ||
          ((reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.k_cache) | reinterpret_cast<uintptr_t>(a.v_cache) | reinterpret_cast<uintptr_t>(a.out)) & 15);
 }
 

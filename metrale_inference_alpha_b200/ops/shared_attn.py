@@ -99,8 +99,8 @@ def shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     to the new tokens, those up to its own. Sequences in front of the first group and behind the last have no prefix. Lengths of zero and less hold
     nothing: a lane that pads the batch stands behind the last group and has length 0. Caches [blocks, block, kv heads, D] bf16, or e4m3 bytes
     with scales. Lengths beyond ``max_prefix`` or ``max_ctx``, blocks that the cache does not have and groups that fall or leave the batch set the status word
-    (`check_status`); on the CPU they are refused. How a prefix is shared out over the GPU, and with it the order of sums, follows from the whole call:
-    unlike with ``paged_attention``, the last bits of a sequence's result may depend on its batch."""
+    (`check_status`); on the CPU they are refused. A CUDA call of no sequences looks at none of them. How a prefix is shared out over the
+    GPU, and with it the order of sums, follows from the whole call: unlike with ``paged_attention``, the last bits of a sequence's result may depend on its batch."""
     where = "shared_prefix_attention"
     shape, dtype = k_cache.shape, k_cache.dtype
     if len(shape) != 4 or (dtype != torch.bfloat16 and dtype != torch.uint8):
@@ -157,9 +157,8 @@ def shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
         _bad(where, f"a cache of {nb} blocks of {bs} has 2^31 rows or more")
     out = torch.empty_like(q)
     lse = torch.empty(T, Hq, dtype=torch.float32, device=q.device) if return_lse else None
-    if T == 0 or nb == 0:
-        out.zero_()
-        return (out, lse.fill_(-float("inf"))) if return_lse else out
+    if T == 0:
+        return (out, lse) if return_lse else out
     rt = runtime(q.device)
     need = _workspace("mb_shared_attn_ws", S, q_len, groups, Hq, Hkv, D, max_prefix, max_ctx, rt.sm_count)
     ws = torch.empty(need, dtype=torch.uint8, device=q.device)

@@ -1,0 +1,15 @@
+"""Edges of attention over shared prefixes, of joins and of expanded latent prompts, on the CPU: what is refused, and what restatements make of it."""
+import pytest
+import torch
+
+import shared_attn_oracle as oracle
+from shared_attn_oracle import run_shared
+
+
+@pytest.mark.parametrize("kw,change", [(dict(max_prefix=0), {}), (dict(max_ctx=0), {}), (dict(max_prefix=0), dict(prefix=[0], start=[0, 9])),
+                                       (dict(max_prefix=0), dict(prefix=[0], start=[1, 0]))], ids=str)
+def test_maxima_of_zero_refuse_what_is_longer(kw, change):
+    c = oracle.shared(1, [5, 9], [40], [0, 2], 4, 2, 64, False)
+    c.update({k: torch.tensor(x, dtype=torch.int32) for k, x in change.items()})
+    with pytest.raises(ValueError, match="shared_prefix_attention"):
+        run_shared(c, **kw)

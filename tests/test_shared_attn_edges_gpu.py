@@ -1,0 +1,56 @@
+"""Edges of attention over shared prefixes, of joins and of expanded latent prompts, on the kernels: what is reported, and calls at the ends of what is allowed."""
+import pytest
+import torch
+
+import shared_attn_oracle as oracle
+from metrale_inference_alpha_b200 import ops
+from metrale_inference_alpha_b200.ops import _native
+from shared_attn_oracle import run_shared, within
+
+pytestmark = pytest.mark.gpu
+
+
+def cuda(c):
+    return {k: v.cuda() if isinstance(v, torch.Tensor) else v for k, v in c.items()}
+
+
+@pytest.fixture(autouse=True)
+def _status():
+    yield
+    ops.check_status("cuda")
+
+
+def reported():
+    with pytest.raises(_native.KernelError):
+        ops.check_status("cuda")
+
+
+@pytest.mark.parametrize("dim,heads,kv_heads", [(64, 4, 2), (256, 4, 1)])
+def test_maxima_of_zero_report_what_is_longer(dim, heads, kv_heads):
+    """Without a kernel over the prefixes, or over own rows, their lengths and groups are looked at all the same."""
+    c = oracle.shared(1, [5, 9, 0], [40], [0, 2], heads, kv_heads, dim, False)
+    none = lambda n: torch.zeros(n, dtype=torch.int32)
+    for kw, change, seen in ((dict(max_prefix=0), {}, dict(prefix=none(1))), (dict(max_ctx=0), {}, dict(ctx=none(3))),
+                             (dict(max_prefix=0, max_ctx=0), {}, dict(prefix=none(1), ctx=none(3))),
+                             (dict(max_prefix=0), dict(prefix=none(1), start=torch.tensor([0, 9], dtype=torch.int32)), dict(prefix=none(1))),
+                             (dict(max_prefix=0), dict(prefix=none(1), start=torch.tensor([-1, 2], dtype=torch.int32)), dict(prefix=none(1)))):
+        out, lse = run_shared(cuda({**c, **change}), **kw)
+        reported()
+        want = oracle.shared_exact({**c, **seen})
+        within(out, want[0], want[1], "outputs")
+        within(lse, want[2], want[3], "log-sum-exps")
+        # with lengths that the maxima allow nothing is reported
+        run_shared(cuda({**c, **seen}), **kw)
+        ops.check_status("cuda")
+
+
+def test_a_cache_without_blocks():
+    """It holds nothing, which is all that such a call may ask for."""
+    c = cuda(oracle.shared(2, [0, 0], [0], [0, 2], 4, 2, 64, False))
+    c.update(k=c["k"][:0], v=c["v"][:0])
+    out, lse = run_shared(c)
+    assert bool((out == 0).all()) and bool((lse == -float("inf")).all())
+    ops.check_status("cuda")
+    c["ctx"][1] = 3
+    run_shared(c)
+    reported()
