@@ -194,7 +194,7 @@ bool bad_shape(const MbSharedArgs& a) {
   return a.num_seqs <= 0 || a.q_len <= 0 || a.Hkv <= 0 || a.Hkv > 65535 || a.Hq % a.Hkv || a.Hq / a.Hkv > 64 || (a.D != 64 && a.D != 128 && a.D != 256) ||
          a.block_size <= 0 || a.num_blocks < 0 || a.num_blocks * a.block_size >= (1ll << 31) || a.table_ld >= (1ll << 31) || a.max_prefix < 0 || a.max_ctx < 0 ||
          ((a.max_prefix > 0 || a.max_ctx > 0) && (a.num_blocks == 0 || !a.k_cache || !a.v_cache)) || !a.q || !a.ctx_len || !a.out ||
-         (a.fp8 && (!a.k_scale || !a.v_scale)) || a.groups < 0 || a.groups > kMaxGroups || (a.groups > 0 && (!a.prefix_table || !a.prefix_len || !a.group_start)) ||
+         (a.fp8 && (!a.k_scale || !a.v_scale)) || a.groups < 0 || a.groups > kMaxGroups || (a.groups > 0 && ((a.max_prefix > 0 && !a.prefix_table) || !a.prefix_len || !a.group_start)) ||
          ((reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.k_cache) | reinterpret_cast<uintptr_t>(a.v_cache) | reinterpret_cast<uintptr_t>(a.out)) & 15);
 }
 

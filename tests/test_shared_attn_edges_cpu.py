@@ -13,3 +13,11 @@ def test_maxima_of_zero_refuse_what_is_longer(kw, change):
     c.update({k: torch.tensor(x, dtype=torch.int32) for k, x in change.items()})
     with pytest.raises(ValueError, match="shared_prefix_attention"):
         run_shared(c, **kw)
+
+
+def test_tables_without_columns():
+    c = oracle.shared(3, [5, 9], [40], [0, 2], 4, 2, 64, False)
+    for name, lengths, most in (("prefix_table", "prefix", "max_prefix"), ("table", "ctx", "max_ctx")):
+        d = {**c, lengths: torch.zeros_like(c[lengths]), most: 0}
+        want, got = run_shared(d), run_shared({**d, name: c[name][:, :0]})
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])

@@ -54,3 +54,13 @@ def test_a_cache_without_blocks():
     c["ctx"][1] = 3
     run_shared(c)
     reported()
+
+
+def test_tables_without_columns():
+    """A maximum of 0 needs no table: prefixes of which a step has none, sequences that have nothing of their own."""
+    c = oracle.shared(3, [5, 9], [40], [0, 2], 4, 2, 64, False)
+    for name, lengths, most in (("prefix_table", "prefix", "max_prefix"), ("table", "ctx", "max_ctx")):
+        d = {**c, lengths: torch.zeros_like(c[lengths]), most: 0}
+        want = run_shared(cuda(d))
+        got = run_shared(cuda({**d, name: c[name][:, :0]}))
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
