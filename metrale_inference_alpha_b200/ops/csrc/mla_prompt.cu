@@ -133,6 +133,33 @@ __global__ void __launch_bounds__(256) gather_kernel(const GatherParams p) {
   }
 }
 
+// ---- calls in which nothing can be attended, since a maximum or a sum is 0 or q has no rows: what the others report is looked at here. One CTA.
+struct NothingParams {
+  const int* q_start;
+  const int* q_len;
+  const int* ctx_len;
+  uint32_t* status;
+  long long q_rows, kv_rows;
+  int num_seqs, max_q_len, max_ctx;
+};
+
+__global__ void __launch_bounds__(256) nothing_kernel(const NothingParams p) {
+  mb::pdl_wait();
+  __shared__ unsigned long long s_rows;
+  if (threadIdx.x == 0) s_rows = 0;
+  __syncthreads();
+  bool beyond = false;
+  unsigned long long rows = 0;
+  for (int s = threadIdx.x; s < p.num_seqs; s += 256) {
+    const int n = p.ctx_len[s], qlen = p.q_len[s];
+    beyond |= n > p.max_ctx || qlen > p.max_q_len || (qlen > 0 && (p.q_start[s] < 0 || (long long)p.q_start[s] + qlen > p.q_rows));
+    rows += (min(max(n, 0), p.max_ctx) + 127) & ~127;
+  }
+  if (rows) atomicAdd(&s_rows, rows);
+  __syncthreads();
+  if ((beyond || s_rows > (unsigned long long)p.kv_rows) && p.status) atomicCAS(p.status, 0u, MB_ST_BOUNDS);
+}
+
 // ---- expansion: kv[row, head, 256] = w[head] c[row], a product whose sums are 512 long
 // A pair of CTAs owns units of 256 cached rows of one head (tcgen05.mma.cta_group::2, M = N = 256). Its rows stay in shared memory, 128 of them in either
 // CTA, while the heads' weights go by, half of a head's in either: with rows fetched again for every head, as the plain product of gemm_rows.cu does, 16
@@ -587,6 +614,11 @@ extern "C" {
 size_t mb_mla_prompt_ws(long long kv_rows, int num_seqs, int each) { return layout(kv_rows, num_seqs, each).bytes; }
 
 int mb_mla_prompt(const MbMlaPromptArgs* a, cudaStream_t stream) {
+  if (a && (a->q_rows == 0 || a->kv_rows == 0 || a->max_q_len == 0 || a->max_ctx == 0)) {
+    if (a->q_rows < 0 || a->kv_rows < 0 || a->max_q_len < 0 || a->max_ctx < 0 || a->num_seqs <= 0 || !a->q_start || !a->q_len || !a->ctx_len) return MB_ERR_BAD_ARG;
+    const NothingParams n{a->q_start, a->q_len, a->ctx_len, a->status, a->q_rows, a->kv_rows, a->num_seqs, a->max_q_len, a->max_ctx};
+    return (int)mb::launch_kernel(nothing_kernel, dim3(1), dim3(256), 0, stream, n);
+  }
   if (!a || !a->q || !a->cache || !a->block_table || !a->q_start || !a->q_len || !a->ctx_len || !a->w || !a->out || a->num_blocks <= 0 || a->q_rows <= 0 ||
       a->kv_rows <= 0 || a->kv_rows % 128 || a->num_seqs <= 0 || a->num_seqs > 65535 || a->H <= 0 || a->H > 65535 || a->block_size <= 0 || a->max_q_len <= 0 ||
       a->max_ctx <= 0 || a->each <= 0)

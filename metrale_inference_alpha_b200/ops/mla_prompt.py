@@ -49,7 +49,7 @@ def mla_prompt_attention(q: torch.Tensor, cache: torch.Tensor, block_table: torc
     Keys and values are rounded to bf16, as cached ones would be, and so are the weights in the product with the values. A cached latent that is no
     number makes the rows that see it NaN, and no others. Lengths beyond ``max_q_len``, ``max_ctx`` or ``total_ctx``, rows that q does not have and
     blocks that the cache does not have set the status word (`check_status`), and a sequence with too many rows or cached tokens is left out; on the CPU
-    they are refused."""
+    they are refused. A CUDA call of no sequences looks at nothing and gives zeros."""
     where = "mla_prompt_attention"
     if cache.dim() != 4 or cache.shape[2] != 1 or cache.shape[3] != ROW or cache.dtype != torch.bfloat16 or not cache.is_contiguous():
         _bad(where, f"cache is contiguous bf16 [blocks, block, 1, {ROW}]")
@@ -84,18 +84,19 @@ def mla_prompt_attention(q: torch.Tensor, cache: torch.Tensor, block_table: torc
     if (q.data_ptr() | cache.data_ptr() | w_kv.data_ptr()) & 15:
         _bad(where, "q, cache and w_kv begin on 16 bytes")
     dev = q.device
-    if rows == 0 or max_q_len == 0 or T == 0:
-        return torch.zeros(T, H, VALUE, dtype=torch.bfloat16, device=dev)
-    out = torch.empty(T, H, VALUE, dtype=torch.bfloat16, device=dev)
+    nothing = rows == 0 or max_q_len == 0 or max_ctx == 0 or T == 0         # to be attended: lengths and places are looked at all the same
+    out = (torch.zeros if nothing else torch.empty)(T, H, VALUE, dtype=torch.bfloat16, device=dev)
+    if S == 0:
+        return out
     L, rt = _library(), runtime(dev)
-    each = max(1, min(H, _WS_BYTES // (rows * KV * 2)))
-    need = L.mb_mla_prompt_ws(rows, S, each)
+    each = 1 if nothing else max(1, min(H, _WS_BYTES // (rows * KV * 2)))
+    need = 0 if nothing else L.mb_mla_prompt_ws(rows, S, each)
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
     a = _ARGS.pack(q.data_ptr(), cache.data_ptr(), block_table.data_ptr(), block_table.stride(0), q_start.data_ptr(), q_len.data_ptr(), ctx_len.data_ptr(),
                    w_kv.data_ptr(), out.data_ptr(), ws.data_ptr(), need, rt.status.data_ptr(), nb, T, rows, S, H, bs, max_q_len, max_ctx, each, rt.sm_count,
                    _PERSIST_PREFILL, scale)
     _native.check(L.mb_mla_prompt(a, _stream()), "mla_prompt")
-    _count(1 + 2 * ((H + each - 1) // each))
+    _count(1 if nothing else 1 + 2 * ((H + each - 1) // each))
     return out
 
 

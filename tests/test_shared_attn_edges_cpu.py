@@ -3,7 +3,7 @@ import pytest
 import torch
 
 import shared_attn_oracle as oracle
-from shared_attn_oracle import run_shared
+from shared_attn_oracle import run_latent, run_shared
 
 
 @pytest.mark.parametrize("kw,change", [(dict(max_prefix=0), {}), (dict(max_ctx=0), {}), (dict(max_prefix=0), dict(prefix=[0], start=[0, 9])),
@@ -21,3 +21,15 @@ def test_tables_without_columns():
         d = {**c, lengths: torch.zeros_like(c[lengths]), most: 0}
         want, got = run_shared(d), run_shared({**d, name: c[name][:, :0]})
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("new,ctx,kw", [([5, 1], [5, 9], dict(max_q_len=0)), ([5], [9], dict(total_ctx=0)), ([5], [9], dict(max_ctx=0)), ([0], [9], dict(max_ctx=0, max_q_len=0))], ids=str)
+def test_latent_prompts_of_nothing_refuse_what_is_longer(new, ctx, kw):
+    with pytest.raises(ValueError, match="mla_prompt_attention"):
+        run_latent(oracle.latent(4, new, ctx, 2), **kw)
+
+
+def test_latent_prompts_without_rows_refuse_portions():
+    c = oracle.latent(5, [5, 1], [5, 9], 2)
+    with pytest.raises(ValueError, match="rows of q"):
+        run_latent({**c, "q": c["q"][:0]})

@@ -5,7 +5,7 @@ import torch
 import shared_attn_oracle as oracle
 from metrale_inference_alpha_b200 import ops
 from metrale_inference_alpha_b200.ops import _native
-from shared_attn_oracle import run_shared, within
+from shared_attn_oracle import run_latent, run_shared, within
 
 pytestmark = pytest.mark.gpu
 
@@ -64,3 +64,25 @@ def test_tables_without_columns():
         want = run_shared(cuda(d))
         got = run_shared(cuda({**d, name: c[name][:, :0]}))
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("new,ctx,kw", [([5, 1], [5, 9], dict(max_q_len=0)), ([5], [9], dict(total_ctx=0)), ([5], [9], dict(max_ctx=0)), ([0], [9], dict(max_ctx=0, max_q_len=0)),
+                                        ([0] * 300, [0] * 299 + [3], dict(max_ctx=2, max_q_len=0))], ids=lambda x: str(x)[:40])
+def test_latent_prompts_of_nothing_report_what_is_longer(new, ctx, kw):
+    out = run_latent(cuda(oracle.latent(4, new, ctx, 2)), **kw)
+    assert bool((out == 0).all())
+    reported()
+
+
+def test_latent_prompts_of_nothing():
+    """What the maxima and the sum allow is not reported: portions without rows, sequences without cached tokens, q without rows, no sequences."""
+    c = oracle.latent(5, [5, 1], [5, 9], 2)
+    none = torch.zeros(2, dtype=torch.int32)
+    one = oracle.latent(6, [4], [0], 2)
+    for d in ({**c, "q_len": none, "max_q_len": 0}, {**c, "q_len": none, "q": c["q"][:0]}, {**one, "max_ctx": 0}, {**one, "max_ctx": 0, "table": one["table"][:, :0]},
+              {**c, "ctx": none, "max_ctx": 0, "total_ctx": 0, "table": c["table"][:, :0], "cache": c["cache"][:0]},
+              {**c, **{k: c[k][:0] for k in ("q_start", "q_len", "ctx", "table")}}):
+        assert bool((run_latent(cuda(d)) == 0).all())
+        ops.check_status("cuda")
+    run_latent(cuda({**c, "q": c["q"][:0]}))
+    reported()
