@@ -81,9 +81,14 @@ struct QueryRow {
   }
 };
 
-// Queries of row r0 + r of a unit, 16-byte piece c of D / 8; an e4m3 cache wants them in f16, scaled (`scale`: what scores are then too small by)
+// A factor of scores in the log2 domain, with the scale of an e4m3 cache in it: never 0, which would make numbers of the -inf that a mask leaves (a scale of 0
+// makes scores equal: no score is so large that the smallest normal number does not). A scale that is negative turns the sign of the queries, since the largest
+// score is found before the factor; one that is NaN leaves no numbers.
+__device__ __forceinline__ float score_factor(float f) { return f >= 0.f ? fmaxf(f, 1.17549435e-38f) : __int_as_float(0x7fffffff); }
+
+// Queries of row r0 + r of a unit, 16-byte piece c of D / 8; an e4m3 cache wants them in f16, scaled (`scale`: what scores are then too small by), times `sign`
 template <int D, bool FP8>
-__device__ __forceinline__ uint4 query_piece(uint4 v, float& scale) {
+__device__ __forceinline__ uint4 query_piece(uint4 v, float sign, float& scale) {
   if constexpr (FP8) {
     // bf16 bits without the sign order like the values: the row's largest over its D / 8 lanes
     const uint32_t x[4] = {v.x, v.y, v.z, v.w};
@@ -94,7 +99,7 @@ __device__ __forceinline__ uint4 query_piece(uint4 v, float& scale) {
     for (int d = 1; d < D / 8; d <<= 1) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, d));
     const int e = (int)(max(top & 0xffff, top >> 16) >> 7);
     const int up = e == 255 ? 0 : 141 - max(e, 15);        // zeros and subnormal rows as if their exponent were 15, infinities and NaN as they are
-    const float f = __int_as_float((127 + up) << 23);
+    const float f = sign * __int_as_float((127 + up) << 23);
     uint32_t h[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -114,9 +119,9 @@ __device__ __forceinline__ uint32_t query_slot(int r, int c) {
 }
 
 // A query row as two e4m3 numbers an element, for keys of e4m3, in two tiles of 128 rows of D bytes. Sixteen elements come from the two places that their
-// numbers go to. Returns what the row's scores are too large by.
+// numbers go to, times `sign`. Returns what the row's scores are too large by.
 template <int D>
-__device__ __forceinline__ float query_pairs(uint8_t* tile, int r) {
+__device__ __forceinline__ float query_pairs(uint8_t* tile, int r, float sign) {
   uint32_t top = 0;                                        // bf16 bits without the sign order like the values
 #pragma unroll 4
   for (int c = 0; c < D / 8; ++c) {
@@ -125,7 +130,7 @@ __device__ __forceinline__ float query_pairs(uint8_t* tile, int r) {
     top = __vmaxu2(top, __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu));
   }
   const int e = (int)(max(top & 0xffff, top >> 16) >> 7), up = e == 255 ? 0 : 134 - max(e, 8);
-  const float f = __int_as_float((127 + up) << 23);
+  const float f = sign * __int_as_float((127 + up) << 23);
 #pragma unroll 1
   for (int c = 0; c < D / 16; ++c) {
     uint8_t *a = tile + query_slot<D>(r, c), *b = a + 128 * D;
@@ -406,7 +411,7 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
     const int w = warp >> 2, r = tid & 127;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t tS = tmem + lanes + w * 128, tO = tmem + lanes + 256 + w * 128;
-    const float sc0 = p.scale * (FP8 ? *p.k_scale : 1.f) * 1.44269504088896f;
+    const float ks = FP8 ? *p.k_scale : 1.f, sign = ks < 0.f ? -1.f : 1.f, sc0 = p.scale * fabsf(ks) * 1.44269504088896f;
     uint32_t part = 0, done = 0, outs = 0, raws = 0;      // parts, tiles, outputs and query tiles that this accumulator has had
     bool ok = true;
     while (ok && next_part<D>(plan, p.groups, ws.per_seq, pos, end, x)) {
@@ -445,16 +450,16 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
           if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
           ++raws;
           if (some) {
-            const float back = query_pairs<D>(sQ + w * kQB, r);
+            const float back = query_pairs<D>(sQ + w * kQB, r, sign);
             s_qscale[part & 1][w][r] = back;
-            sc *= back;
+            sc = score_factor(sc * back);
           }
         }
         fence_async_smem();
       } else if constexpr (FP8) {
         ok = mb::mbar_wait(&q_full[0], part & 1, p.status, MB_ST_TIMEOUT_MMA);
         if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-        sc *= s_qscale[part & 1][0][r];
+        sc = score_factor(sc * s_qscale[part & 1][0][r]);
       }
       __syncwarp();
       if (lane == 0) mb::mbar_arrive(&q_full[w]);
@@ -813,7 +818,7 @@ __global__ void __launch_bounds__(288, 1) shared_prefix256_kernel(const MbShared
     // ------------------------------------------------------------ softmax
     const uint32_t lanes = (uint32_t)(warp * 32) << 16;
     const uint32_t tO = tmem + lanes + 256;
-    const float sc0 = p.scale * (FP8 ? *p.k_scale : 1.f) * 1.44269504088896f;
+    const float ks = FP8 ? *p.k_scale : 1.f, sign = ks < 0.f ? -1.f : 1.f, sc0 = p.scale * fabsf(ks) * 1.44269504088896f;
     uint32_t part = 0, base = 0;                          // parts, tiles that are done
     bool ok = true;
     int pos = begin;
@@ -835,7 +840,7 @@ __global__ void __launch_bounds__(288, 1) shared_prefix256_kernel(const MbShared
           const int qr = warp + 4 * (half * 16 + i);
           if (qr > last) v[i] = make_uint4(0, 0, 0, 0);
           float back = 1.f;
-          v[i] = query_piece<D, FP8>(v[i], back);
+          v[i] = query_piece<D, FP8>(v[i], sign, back);
           if (FP8 && lane == 0) s_qscale[part & 1][qr] = back;
           *reinterpret_cast<uint4*>(sQ + (lane >> 3) * (128 * 128) + sw_off(qr, lane & 7)) = v[i];
         }
@@ -847,7 +852,7 @@ __global__ void __launch_bounds__(288, 1) shared_prefix256_kernel(const MbShared
       if constexpr (FP8) {
         ok = mb::mbar_wait(&q_full, part & 1, p.status, MB_ST_TIMEOUT_MMA);
         if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-        sc *= s_qscale[part & 1][tid];
+        sc = score_factor(sc * s_qscale[part & 1][tid]);
       }
       const bool live = tid <= last, some = warp * 32 <= last;
       const int len = plan.len[x.group];

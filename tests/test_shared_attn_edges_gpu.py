@@ -86,3 +86,16 @@ def test_latent_prompts_of_nothing():
         ops.check_status("cuda")
     run_latent(cuda({**c, "q": c["q"][:0]}))
     reported()
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.0, -0.0625, 1e-30, float("nan")])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(4, 2, 64), (10, 2, 128), (8, 1, 256)])
+@pytest.mark.parametrize("seqs", [3, 60])
+def test_scales_of_an_e4m3_cache_at_their_ends(heads, kv_heads, dim, scale, seqs):
+    """A scale of zero makes scores equal, a negative one turns them, one that is no number leaves none; prefixes that end inside a tile, one tile of rows and several."""
+    c = oracle.shared(7, [1 + i * 31 % 90 for i in range(seqs)], [300, 129], [0, seqs - 1, seqs], heads, kv_heads, dim, True)
+    c["k_scale"] = torch.tensor([scale])
+    want = oracle.shared_exact(c)
+    out, lse = run_shared(cuda(c))
+    within(out, want[0], want[1], "outputs")
+    within(lse, want[2], want[3], "log-sum-exps")
