@@ -10,7 +10,7 @@ from typing import Optional
 import torch
 
 from . import _PERSIST_PREFILL, _count, _native, _stream, reference as ref, runtime
-from .shared_attn import _bad, _check_ints, _check_places, _check_table
+from .shared_attn import _bad, _check_ints, _check_places, _check_scale, _check_table
 
 LATENT, ROPE, NOPE, VALUE = 512, 64, 128, 128
 ROW, QK, KV = LATENT + ROPE, NOPE + ROPE, NOPE + VALUE
@@ -75,8 +75,7 @@ def mla_prompt_attention(q: torch.Tensor, cache: torch.Tensor, block_table: torc
     rows = (total + 127 * S) // 128 * 128                    # every sequence begins on a multiple of 128
     if total < 0 or rows >= 1 << 31:
         _bad(where, f"total_ctx {total} is from 0 to 2^31")
-    if not scale > 0:
-        _bad(where, "scale is positive")
+    _check_scale(where, scale)
     _check_places(where, q, cache, block_table, q_start, q_len, ctx_len, w_kv)
     if not q.is_cuda:
         _check_values(where, T, nb, bs, block_table, q_start, q_len, ctx_len, max_q_len, max_ctx, total)

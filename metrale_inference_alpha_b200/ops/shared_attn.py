@@ -75,6 +75,12 @@ def _check_places(where, *tensors) -> None:
         _bad(where, f"tensors lie on device {dev}, the current device is another one")
 
 
+def _check_scale(where, scale) -> None:
+    """The kernels have it in 32 bits, and multiply a mask's -inf by it."""
+    if not 2.0 ** -126 <= scale <= 2.0 ** 126:
+        _bad(where, f"scale is positive, from 2^-126 to 2^126, not {scale}")
+
+
 def _check_ints(where, name, x, n: int) -> None:
     if x.dtype != torch.int32 or x.dim() != 1 or x.shape[0] != n or not x.is_contiguous():
         _bad(where, f"{name} is contiguous int32 [{n}]")
@@ -134,8 +140,7 @@ def shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
         _bad(where, f"{Hq} query heads over {Hkv} kv heads: whole groups of up to {MAX_GROUP}")
     if T * Hq * D > 1 << 29:
         _bad(where, f"{T} tokens of {Hq} heads of {D} dims are more than 2^29 elements: a step of a batch is meant, not its prompts")
-    if not scale > 0:
-        _bad(where, "scale is positive")
+    _check_scale(where, scale)
     fp8 = dtype == torch.uint8
     if fp8:
         if D == 64 and bs % 2:

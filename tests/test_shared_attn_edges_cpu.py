@@ -33,3 +33,12 @@ def test_latent_prompts_without_rows_refuse_portions():
     c = oracle.latent(5, [5, 1], [5, 9], 2)
     with pytest.raises(ValueError, match="rows of q"):
         run_latent({**c, "q": c["q"][:0]})
+
+
+@pytest.mark.parametrize("scale", [0.0, -1.0, 1e-46, 1e39, float("inf"), float("nan")])
+def test_scales_beyond_32_bits_are_refused(scale):
+    """The kernels would multiply a mask's -inf by zero, or scores by infinity."""
+    with pytest.raises(ValueError, match="scale"):
+        run_shared(oracle.shared(8, [5], [9], [0, 1], 4, 2, 64, False), scale=scale)
+    with pytest.raises(ValueError, match="scale"):
+        run_latent(oracle.latent(8, [5], [9], 2), scale=scale)

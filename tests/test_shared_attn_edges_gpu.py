@@ -99,3 +99,17 @@ def test_scales_of_an_e4m3_cache_at_their_ends(heads, kv_heads, dim, scale, seqs
     out, lse = run_shared(cuda(c))
     within(out, want[0], want[1], "outputs")
     within(lse, want[2], want[3], "log-sum-exps")
+
+
+@pytest.mark.parametrize("scale", [2.0 ** -126, 2.0 ** -60])
+def test_the_smallest_scales(scale):
+    """Scores are all but equal; columns that are masked have no weight all the same."""
+    for fp8 in (False, True):
+        c = {**oracle.shared(9, [5, 90, 1], [300], [0, 3], 10, 2, 128, fp8), "scale": scale}
+        want = oracle.shared_exact(c)
+        out, lse = run_shared(cuda(c))
+        within(out, want[0], want[1], "outputs")
+        within(lse, want[2], want[3], "log-sum-exps")
+    c = {**oracle.latent(9, [140], [300], 2), "scale": scale}
+    want = oracle.latent_exact(c)
+    within(run_latent(cuda(c)), want[0], want[1], "outputs")
