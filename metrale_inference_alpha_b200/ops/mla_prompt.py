@@ -66,7 +66,7 @@ def mla_prompt_attention(q: torch.Tensor, cache: torch.Tensor, block_table: torc
     S = ctx_len.shape[0]
     for name, x in (("q_start", q_start), ("q_len", q_len), ("ctx_len", ctx_len)):
         _check_ints(where, name, x, S)
-    _check_table(where, "block_table", block_table, S, bs, max_ctx if S else 0, "max_ctx")
+    _check_table(where, "block_table", block_table, S, bs, max_ctx, "max_ctx")
     if max_q_len < 0 or max_q_len > 1 << 30:
         _bad(where, "max_q_len is from 0 to 2^30")
     if S > 65535 or H > 65535:

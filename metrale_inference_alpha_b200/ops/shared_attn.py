@@ -89,7 +89,7 @@ def _check_ints(where, name, x, n: int) -> None:
 def _check_table(where, name, x, rows: int, bs: int, most: int, what: str) -> None:
     if x.dtype != torch.int32 or x.dim() != 2 or x.shape[0] != rows or (x.shape[1] > 1 and x.stride(1) != 1):
         _bad(where, f"{name} is int32 [{rows}, blocks], a row's blocks next to each other")
-    if most < 0 or most > 1 << 30 or x.shape[1] * bs < most:
+    if most < 0 or most > 1 << 30 or (rows > 0 and x.shape[1] * bs < most):
         _bad(where, f"{what} {most} is beyond the rows of {name} ({x.shape[1] * bs}), or not from 0 to 2^30")
 
 
@@ -128,8 +128,8 @@ def shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     _check_ints(where, "group_start", group_start, groups + 1)
     if groups > MAX_GROUPS:
         _bad(where, f"{groups} groups, at most {MAX_GROUPS} are served")
-    _check_table(where, "prefix_table", prefix_table, groups, bs, max_prefix if groups else 0, "max_prefix")
-    _check_table(where, "block_table", block_table, S, bs, max_ctx if S else 0, "max_ctx")
+    _check_table(where, "prefix_table", prefix_table, groups, bs, max_prefix, "max_prefix")
+    _check_table(where, "block_table", block_table, S, bs, max_ctx, "max_ctx")
     if q_len < 1 or q_len > 1 << 16:
         _bad(where, "q_len is from 1 to 65536")
     T = S * q_len

@@ -42,3 +42,19 @@ def test_scales_beyond_32_bits_are_refused(scale):
         run_shared(oracle.shared(8, [5], [9], [0, 1], 4, 2, 64, False), scale=scale)
     with pytest.raises(ValueError, match="scale"):
         run_latent(oracle.latent(8, [5], [9], 2), scale=scale)
+
+
+@pytest.mark.parametrize("most", [-1, 1 << 31, 10 ** 12])
+def test_maxima_are_looked_at_without_groups_and_sequences(most):
+    """What no group and no sequence needs goes to the library all the same."""
+    c = oracle.shared(10, [5, 9], [40], [0, 2], 4, 2, 64, False)
+    alone = {**c, "prefix": c["prefix"][:0], "prefix_table": c["prefix_table"][:0], "start": c["start"][:1]}
+    with pytest.raises(ValueError, match="max_prefix"):
+        run_shared(alone, max_prefix=most)
+    run_shared(alone, max_prefix=1 << 20)
+    nobody = {**c, **{k: c[k][:0] for k in ("q", "ctx", "table")}, "start": torch.zeros(2, dtype=torch.int32)}
+    with pytest.raises(ValueError, match="max_ctx"):
+        run_shared(nobody, max_ctx=most)
+    e = oracle.latent(10, [5], [9], 2)
+    with pytest.raises(ValueError, match="max_ctx"):
+        run_latent({**e, **{k: e[k][:0] for k in ("q_start", "q_len", "ctx", "table")}}, max_ctx=most)
