@@ -603,9 +603,13 @@ def shared_prefix_attention(q, k_cache, v_cache, prefix_table, prefix_len, group
     return out.to(torch.bfloat16), lse
 
 
+def merged_lse(l):
+    """Of log-sum-exps [parts, ...]; a part that has +inf leaves no number."""
+    return torch.logsumexp(torch.where(l == float("inf"), float("nan"), l), 0)
+
+
 def merge_attention(outs, lses):
-    l = torch.stack(list(lses))
-    lse = torch.logsumexp(torch.where(l == float("inf"), float("nan"), l), 0)
+    lse = merged_lse(torch.stack(list(lses)))
     total = torch.zeros(outs[0].shape)
     for o, x in zip(outs, lses):
         total += torch.where((x == float("-inf"))[..., None], 0.0, torch.exp(x - lse)[..., None] * o.float())

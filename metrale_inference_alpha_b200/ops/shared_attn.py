@@ -213,7 +213,7 @@ def merge_attention(outs: Sequence[torch.Tensor], lses: Sequence[torch.Tensor]) 
     out, lse = torch.empty_like(outs[0]), torch.empty_like(lses[0])
     rows = shape[0] * shape[1]
     if rows == 0 or shape[2] == 0:
-        return (out, lse) if rows == 0 else (out, torch.logsumexp(torch.stack(list(lses)), 0))
+        return (out, lse) if rows == 0 else (out, ref.merged_lse(torch.stack(list(lses))))
     pad = [0] * (MAX_PARTS - n)
     a = _MERGE_ARGS.pack(*[o.data_ptr() for o in outs], *pad, *[l.data_ptr() for l in lses], *pad, out.data_ptr(), lse.data_ptr(), rows, n, shape[2],
                          int(dtype == torch.float32), runtime(out.device).sm_count)

@@ -3,6 +3,7 @@ import pytest
 import torch
 
 import shared_attn_oracle as oracle
+from metrale_inference_alpha_b200 import ops
 from shared_attn_oracle import run_latent, run_shared
 
 
@@ -58,3 +59,9 @@ def test_maxima_are_looked_at_without_groups_and_sequences(most):
     e = oracle.latent(10, [5], [9], 2)
     with pytest.raises(ValueError, match="max_ctx"):
         run_latent({**e, **{k: e[k][:0] for k in ("q_start", "q_len", "ctx", "table")}}, max_ctx=most)
+
+
+def test_merge_of_rows_without_dims():
+    o, inf = torch.zeros(4, 1, 0), float("inf")
+    out, lse = ops.merge_attention([o, o], [torch.zeros(4, 1), torch.tensor([[0.0], [inf], [float("nan")], [-inf]])])
+    assert out.shape == (4, 1, 0) and lse[0, 0].item() == pytest.approx(0.6931472) and bool(lse[1:3].isnan().all()) and lse[3, 0].item() == 0.0

@@ -113,3 +113,12 @@ def test_the_smallest_scales(scale):
     c = {**oracle.latent(9, [140], [300], 2), "scale": scale}
     want = oracle.latent_exact(c)
     within(run_latent(cuda(c)), want[0], want[1], "outputs")
+
+
+def test_merge_of_rows_without_dims():
+    """The log-sum-exps are those of rows with dims."""
+    inf = float("inf")
+    lses = [torch.zeros(4, 1, device="cuda"), torch.tensor([[0.0], [inf], [float("nan")], [-inf]], device="cuda")]
+    none, some = (ops.merge_attention([torch.zeros(4, 1, d, device="cuda")] * 2, lses) for d in (0, 8))
+    assert none[0].shape == (4, 1, 0)
+    torch.testing.assert_close(none[1], some[1], rtol=1e-6, atol=1e-6, equal_nan=True)
