@@ -102,11 +102,12 @@ def shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
 
     Sequences group_start[g] to group_start[g + 1] (int32 [groups + 1], rising) stand behind the prefix of group g: the first prefix_len[g] rows of
     prefix_table[g]. Every one of their tokens sees the whole of it, and of the sequence's own ctx_len[s] rows in block_table[s], whose last ``q_len`` belong
-    to the new tokens, those up to its own. Sequences in front of the first group and behind the last have no prefix. Lengths of zero and less hold
-    nothing: a lane that pads the batch stands behind the last group and has length 0. Caches [blocks, block, kv heads, D] bf16, or e4m3 bytes
-    with scales. Lengths beyond ``max_prefix`` or ``max_ctx``, blocks that the cache does not have and groups that fall or leave the batch set the status word
-    (`check_status`); on the CPU they are refused. A CUDA call of no sequences looks at none of them. How a prefix is shared out over the
-    GPU, and with it the order of sums, follows from the whole call: unlike with ``paged_attention``, the last bits of a sequence's result may depend on its batch."""
+    to the new tokens, those up to its own. Sequences in front of the first group and behind the last have no prefix; the length and table of a group
+    without sequences are not looked at. Lengths of zero and less hold nothing: a lane that pads the batch stands behind the last group and has length 0.
+    Caches [blocks, block, kv heads, D] bf16, or e4m3 bytes with scales. Lengths beyond ``max_prefix`` or ``max_ctx``, blocks that the cache does not have and
+    groups that fall or leave the batch set the status word (`check_status`); on the CPU they are refused. A CUDA call of no sequences looks at none of them.
+    How a prefix is shared out over the GPU, and with it the order of sums, follows from the whole call: unlike with ``paged_attention``, the last bits of a
+    sequence's result may depend on its batch."""
     where = "shared_prefix_attention"
     shape, dtype = k_cache.shape, k_cache.dtype
     if len(shape) != 4 or (dtype != torch.bfloat16 and dtype != torch.uint8):
@@ -177,12 +178,12 @@ def shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
 
 def _check_values(where, nb, bs, max_prefix, max_ctx, prefix_table, prefix_len, group_start, block_table, ctx_len) -> None:
     """CPU: what the kernels cut and report is refused."""
-    if bool((ctx_len > max_ctx).any()) or bool((prefix_len > max_prefix).any()):
-        _bad(where, f"a length is beyond max_prefix {max_prefix} or max_ctx {max_ctx}")
     S = ctx_len.shape[0]
     if prefix_len.shape[0] and (bool((group_start.diff() < 0).any()) or int(group_start[0]) < 0 or int(group_start[-1]) > S):
         _bad(where, f"group_start falls, or leaves the batch of {S}")
     held = group_start.diff() > 0
+    if bool((ctx_len > max_ctx).any()) or bool((held & (prefix_len > max_prefix)).any()):
+        _bad(where, f"a length is beyond max_prefix {max_prefix} or max_ctx {max_ctx}")
     for table, rows in ((prefix_table, torch.where(held, prefix_len, 0)), (block_table, ctx_len)):
         used = torch.arange(table.shape[1]) * bs < rows[:, None]
         if bool((used & ((table < 0) | (table >= nb))).any()):

@@ -4,7 +4,7 @@ import torch
 
 import shared_attn_oracle as oracle
 from metrale_inference_alpha_b200 import ops
-from shared_attn_oracle import run_latent, run_shared
+from shared_attn_oracle import run_latent, run_shared, within
 
 
 @pytest.mark.parametrize("kw,change", [(dict(max_prefix=0), {}), (dict(max_ctx=0), {}), (dict(max_prefix=0), dict(prefix=[0], start=[0, 9])),
@@ -65,3 +65,20 @@ def test_merge_of_rows_without_dims():
     o, inf = torch.zeros(4, 1, 0), float("inf")
     out, lse = ops.merge_attention([o, o], [torch.zeros(4, 1), torch.tensor([[0.0], [inf], [float("nan")], [-inf]])])
     assert out.shape == (4, 1, 0) and lse[0, 0].item() == pytest.approx(0.6931472) and bool(lse[1:3].isnan().all()) and lse[3, 0].item() == 0.0
+
+
+@pytest.mark.parametrize("start", [[0, 0], [0, 0, 2], [0, 2, 2], [2, 2, 2]], ids=str)
+def test_groups_without_sequences_are_not_looked_at(start):
+    """Their lengths and tables may be of another step."""
+    c = oracle.shared(11, [5, 9], [40, 24], [0, 1, 2], 4, 2, 64, False)
+    n = len(start) - 1
+    c.update(start=torch.tensor(start, dtype=torch.int32), prefix=c["prefix"][:n].clone(), prefix_table=c["prefix_table"][:n].clone())
+    out, tol, lse, ltol = oracle.shared_exact(c)
+    for g in range(n):
+        if start[g] == start[g + 1]:
+            c["prefix"][g], c["prefix_table"][g] = 10 ** 6, -1
+    for most in (c["max_prefix"], 0):
+        if most or all(a == b for a, b in zip(start, start[1:])):
+            a, b = run_shared(c, max_prefix=most)
+            within(a, out, tol, "outputs")
+            within(b, lse, ltol, "log-sum-exps")

@@ -122,3 +122,20 @@ def test_merge_of_rows_without_dims():
     none, some = (ops.merge_attention([torch.zeros(4, 1, d, device="cuda")] * 2, lses) for d in (0, 8))
     assert none[0].shape == (4, 1, 0)
     torch.testing.assert_close(none[1], some[1], rtol=1e-6, atol=1e-6, equal_nan=True)
+
+
+@pytest.mark.parametrize("start", [[0, 0], [0, 0, 2], [0, 2, 2], [2, 2, 2]], ids=str)
+def test_groups_without_sequences_are_not_looked_at(start):
+    """Their lengths and tables may be of another step."""
+    c = oracle.shared(11, [5, 9], [40, 24], [0, 1, 2], 4, 2, 64, False)
+    n = len(start) - 1
+    c.update(start=torch.tensor(start, dtype=torch.int32), prefix=c["prefix"][:n].clone(), prefix_table=c["prefix_table"][:n].clone())
+    out, tol, lse, ltol = oracle.shared_exact(c)
+    for g in range(n):
+        if start[g] == start[g + 1]:
+            c["prefix"][g], c["prefix_table"][g] = 10 ** 6, -1
+    for most in (c["max_prefix"], 0):
+        if most or all(a == b for a, b in zip(start, start[1:])):
+            a, b = run_shared(cuda(c), max_prefix=most)
+            within(a, out, tol, "outputs")
+            within(b, lse, ltol, "log-sum-exps")
