@@ -21,8 +21,22 @@ _ARGS = struct.Struct("@3P q 6P N P 3q 8i f 4x")
 _native.register_optional("mb_mla_prompt", [C.c_char_p, C.c_void_p])
 
 _lib = None
-# most bytes of expanded keys and values that a call holds: more heads go in several steps
+# most bytes of gathered rows and expanded keys and values that a call holds: more heads go in several steps, of one head at the least
 _WS_BYTES = 1 << 30
+_ROW_BYTES = 2 * ROW + 1             # of a gathered row and what is remembered beside it
+
+
+def _cached_rows(total_ctx: int, seqs: int) -> int:
+    return (total_ctx + 127 * seqs) // 128 * 128             # every sequence begins on a multiple of 128
+
+
+def _heads_at_once(rows: int, H: int) -> int:
+    return max(1, min(H, (_WS_BYTES - rows * _ROW_BYTES) // (rows * KV * 2)))
+
+
+def fits(total_ctx: int, seqs: int) -> bool:
+    """Whether a call over so many cached tokens keeps to the workspace of 1 GB: some 640,000 do."""
+    return _cached_rows(total_ctx, seqs) * (_ROW_BYTES + 2 * KV) <= _WS_BYTES
 
 
 def _library():
@@ -44,7 +58,8 @@ def mla_prompt_attention(q: torch.Tensor, cache: torch.Tensor, block_table: torc
     cache [blocks, block, 1, 576] bf16 (512 of the latent, 64 of the rotated key), w_kv [H, 256, 512] bf16 (a head's keys without position, its values)
     -> [rows, H, 128] bf16. Sequence s has rows q_start[s] to q_start[s] + q_len[s], the last q_len[s] of its ctx_len[s] cached tokens; each token sees those
     up to itself, and one that sees none gives zeros. Rows of q that belong to no sequence are not written. ``total_ctx``: the sum of ctx_len, or a bound
-    of it (None: ``max_ctx`` a sequence); memory and the making of keys and values go by it.
+    of it (None: ``max_ctx`` a sequence); memory and the making of keys and values go by it. The workspace is 1152 bytes a cached token and 512 for each of the heads
+    that are made at once: as many as 1 GB has room for, one at least.
 
     Keys and values are rounded to bf16, as cached ones would be, and so are the weights in the product with the values. A cached latent that is no
     number makes the rows that see it NaN, and no others. Lengths beyond ``max_q_len``, ``max_ctx`` or ``total_ctx``, rows that q does not have and
@@ -72,7 +87,7 @@ def mla_prompt_attention(q: torch.Tensor, cache: torch.Tensor, block_table: torc
     if S > 65535 or H > 65535:
         _bad(where, "at most 65535 sequences and heads")
     total = S * max_ctx if total_ctx is None else min(total_ctx, S * max_ctx)
-    rows = (total + 127 * S) // 128 * 128                    # every sequence begins on a multiple of 128
+    rows = _cached_rows(total, S)
     if total < 0 or rows >= 1 << 31:
         _bad(where, f"total_ctx {total} is from 0 to 2^31")
     _check_scale(where, scale)
@@ -88,7 +103,7 @@ def mla_prompt_attention(q: torch.Tensor, cache: torch.Tensor, block_table: torc
     if S == 0:
         return out
     L, rt = _library(), runtime(dev)
-    each = 1 if nothing else max(1, min(H, _WS_BYTES // (rows * KV * 2)))
+    each = 1 if nothing else _heads_at_once(rows, H)
     need = 0 if nothing else L.mb_mla_prompt_ws(rows, S, each)
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
     a = _ARGS.pack(q.data_ptr(), cache.data_ptr(), block_table.data_ptr(), block_table.stride(0), q_start.data_ptr(), q_len.data_ptr(), ctx_len.data_ptr(),

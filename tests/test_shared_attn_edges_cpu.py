@@ -4,6 +4,9 @@ import torch
 
 import shared_attn_oracle as oracle
 from metrale_inference_alpha_b200 import ops
+from metrale_inference_alpha_b200.engine.batch import ForwardBatch
+from metrale_inference_alpha_b200.models import mla
+from metrale_inference_alpha_b200.ops import mla_prompt, shared_attn
 from shared_attn_oracle import run_latent, run_shared, within
 
 
@@ -82,3 +85,24 @@ def test_groups_without_sequences_are_not_looked_at(start):
             a, b = run_shared(c, max_prefix=most)
             within(a, out, tol, "outputs")
             within(b, lse, ltol, "log-sum-exps")
+
+
+@pytest.mark.parametrize("heads", [1, 16, 128])
+@pytest.mark.parametrize("total,seqs", [(1, 1), (8192, 1), (12288, 3), (100_000, 64), (600_000, 200), (640_000, 1), (700_000, 1), (3_000_000, 9)])
+def test_the_workspace_of_latent_prompts_is_bounded(total, seqs, heads):
+    """Gathered rows count as well; with one head at a time nothing can be saved any more."""
+    rows = mla_prompt._cached_rows(total, seqs)
+    assert rows % 128 == 0 and rows >= total
+    each = mla_prompt._heads_at_once(rows, heads)
+    assert 1 <= each <= heads and (each == heads or rows * (1153 + 512 * (each + 1)) > 1 << 30)
+    if not shared_attn._native.available():
+        pytest.skip("not built")
+    need = mla_prompt._library().mb_mla_prompt_ws(rows, seqs, each)
+    assert mla_prompt.fits(total, seqs) == (rows * (1153 + 512) <= 1 << 30)
+    assert not mla_prompt.fits(total, seqs) or need <= (1 << 30) + 1024            # 1024: parts begin on 256 bytes
+
+
+def test_steps_beyond_the_workspace_stay_absorbed():
+    def batch(n, front):
+        return ForwardBatch.build([dict(tokens=[1] * n, start_pos=front, blocks=[1] * ((n + front) // 16 + 2))], 16)
+    assert mla._expanded_pays(batch(8192, 600_000)) and not mla._expanded_pays(batch(8192, 700_000))

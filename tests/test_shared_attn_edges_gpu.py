@@ -4,7 +4,7 @@ import torch
 
 import shared_attn_oracle as oracle
 from metrale_inference_alpha_b200 import ops
-from metrale_inference_alpha_b200.ops import _native
+from metrale_inference_alpha_b200.ops import _native, mla_prompt
 from shared_attn_oracle import run_latent, run_shared, within
 
 pytestmark = pytest.mark.gpu
@@ -139,3 +139,20 @@ def test_groups_without_sequences_are_not_looked_at(start):
             a, b = run_shared(cuda(c), max_prefix=most)
             within(a, out, tol, "outputs")
             within(b, lse, ltol, "log-sum-exps")
+
+
+@pytest.mark.parametrize("heads_at_once", [5, 3, 2, 1])
+def test_the_workspace_of_latent_prompts_is_bounded(heads_at_once, monkeypatch):
+    c = cuda(oracle.latent(12, [140, 30], [2000, 300], 5))
+    want = run_latent(c)
+    rows = mla_prompt._cached_rows(2300, 2)
+    most = rows * (1153 + 512 * heads_at_once) + 600
+    monkeypatch.setattr(mla_prompt, "_WS_BYTES", most)
+    assert mla_prompt._heads_at_once(rows, 5) == heads_at_once
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    got = run_latent(c)
+    assert torch.equal(got, want)
+    assert torch.cuda.max_memory_allocated() - before <= most + 2048 + got.numel() * 2          # parts begin on 256 bytes, tensors on 512
