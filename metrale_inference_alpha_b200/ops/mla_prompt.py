@@ -57,14 +57,15 @@ def mla_prompt_attention(q: torch.Tensor, cache: torch.Tensor, block_table: torc
     """Causal attention of prompts, or portions of prompts, over a paged latent cache: q [rows, H, 192] bf16 (128 dims without position, 64 rotated),
     cache [blocks, block, 1, 576] bf16 (512 of the latent, 64 of the rotated key), w_kv [H, 256, 512] bf16 (a head's keys without position, its values)
     -> [rows, H, 128] bf16. Sequence s has rows q_start[s] to q_start[s] + q_len[s], the last q_len[s] of its ctx_len[s] cached tokens; each token sees those
-    up to itself, and one that sees none gives zeros. Rows of q that belong to no sequence are not written. ``total_ctx``: the sum of ctx_len, or a bound
-    of it (None: ``max_ctx`` a sequence); memory and the making of keys and values go by it. The workspace is 1152 bytes a cached token and 512 for each of the heads
-    that are made at once: as many as 1 GB has room for, one at least.
+    up to itself, and one that sees none gives zeros. Rows of q that belong to no sequence are not written, and none belongs to two (on CUDA the sequences'
+    results would meet in it, 16 bytes from one or the other; on the CPU such portions are refused). ``total_ctx``: the sum of ctx_len, or a bound of it (None:
+    ``max_ctx`` a sequence); memory and the making of keys and values go by it. The workspace is 1152 bytes a cached token and 512 for each of the heads that
+    are made at once: as many as 1 GB has room for, one at least.
 
-    Keys and values are rounded to bf16, as cached ones would be, and so are the weights in the product with the values. A cached latent that is no
-    number makes the rows that see it NaN, and no others. Lengths beyond ``max_q_len``, ``max_ctx`` or ``total_ctx``, rows that q does not have and
-    blocks that the cache does not have set the status word (`check_status`), and a sequence with too many rows or cached tokens is left out; on the CPU
-    they are refused. A CUDA call of no sequences looks at nothing and gives zeros."""
+    Keys and values are rounded to bf16, as cached ones would be (what is beyond its range is infinite), and so are the weights in the product with the
+    values. A cached latent that is no number makes the rows that see it NaN, and no others. Lengths beyond ``max_q_len``, ``max_ctx`` or ``total_ctx``, rows
+    that q does not have and blocks that the cache does not have set the status word (`check_status`), and a sequence with too many rows or cached tokens is
+    left out; on the CPU they are refused. A CUDA call of no sequences looks at nothing and gives zeros."""
     where = "mla_prompt_attention"
     if cache.dim() != 4 or cache.shape[2] != 1 or cache.shape[3] != ROW or cache.dtype != torch.bfloat16 or not cache.is_contiguous():
         _bad(where, f"cache is contiguous bf16 [blocks, block, 1, {ROW}]")
@@ -120,6 +121,10 @@ def _check_values(where, T, nb, bs, block_table, q_start, q_len, ctx_len, max_q_
         _bad(where, f"a length is beyond max_q_len {max_q_len} or max_ctx {max_ctx}, or the sum beyond total_ctx {total}")
     if bool(((q_len > 0) & ((q_start < 0) | (q_start.long() + q_len > T))).any()):
         _bad(where, f"a portion has rows of q beyond its {T}")
+    some = q_len > 0
+    first, order = q_start[some].long().sort()
+    if bool((first[1:] < (first + q_len[some].long()[order])[:-1]).any()):
+        _bad(where, "two portions have a row of q in common")
     used = torch.arange(block_table.shape[1]) * bs < ctx_len[:, None]
     if bool((used & ((block_table < 0) | (block_table >= nb))).any()):
         _bad(where, f"the table has a block that the cache of {nb} does not have")

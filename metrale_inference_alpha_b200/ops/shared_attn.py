@@ -104,7 +104,7 @@ def shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     prefix_table[g]. Every one of their tokens sees the whole of it, and of the sequence's own ctx_len[s] rows in block_table[s], whose last ``q_len`` belong
     to the new tokens, those up to its own. Sequences in front of the first group and behind the last have no prefix; the length and table of a group
     without sequences are not looked at. Lengths of zero and less hold nothing: a lane that pads the batch stands behind the last group and has length 0.
-    Caches [blocks, block, kv heads, D] bf16, or e4m3 bytes with scales. Lengths beyond ``max_prefix`` or ``max_ctx``, blocks that the cache does not have and
+    Caches [blocks, block, kv heads, D] bf16, or e4m3 bytes with scales (behind a prefix of these an infinite query gives NaN). Lengths beyond ``max_prefix`` or ``max_ctx``, blocks that the cache does not have and
     groups that fall or leave the batch set the status word (`check_status`); on the CPU they are refused. A CUDA call of no sequences looks at none of them.
     How a prefix is shared out over the GPU, and with it the order of sums, follows from the whole call: unlike with ``paged_attention``, the last bits of a
     sequence's result may depend on its batch."""

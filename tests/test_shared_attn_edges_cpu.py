@@ -106,3 +106,14 @@ def test_steps_beyond_the_workspace_stay_absorbed():
     def batch(n, front):
         return ForwardBatch.build([dict(tokens=[1] * n, start_pos=front, blocks=[1] * ((n + front) // 16 + 2))], 16)
     assert mla._expanded_pays(batch(8192, 600_000)) and not mla._expanded_pays(batch(8192, 700_000))
+
+
+@pytest.mark.parametrize("starts,fine", [([0, 5, 6], True), ([3, 2, 0], True), ([0, 4, 6], False), ([2, 2, 0], False), ([0, 6, 4], False)], ids=str)
+def test_latent_portions_that_share_rows_are_refused(starts, fine):
+    c = oracle.latent(13, [5, 1, 2], [5, 9, 30], 2)
+    c["q_start"] = torch.tensor(starts, dtype=torch.int32)
+    if fine:
+        run_latent(c)
+        return
+    with pytest.raises(ValueError, match="in common"):
+        run_latent(c)
