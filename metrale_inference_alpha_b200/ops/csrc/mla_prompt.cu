@@ -649,9 +649,10 @@ int mb_mla_prompt(const MbMlaPromptArgs* a, cudaStream_t stream) {
     void* kv = ws + l.kv;
     const long long units = (a->kv_rows + 255) / 256 * n;
     if (units > 0x7fffffff) return MB_ERR_TOO_LARGE;
-    // rows of one unit are fetched once by either kernel, and mb_gemm has tiles of half the size for them. The whole call, here / by mb_gemm: 128 rows of 128
-    // heads 30.7 / 27.2 us, of 64 24.4 / 24.6; 384 rows of 128 59.9 / 65.7, 512 of 64 36.0 / 36.8, 1024 of 16 34.9 / 36.9, of 64 59.6 / 70.3, 8192 of 16 294 / 306
-    if (a->kv_rows > 256) {
+    // 128 rows are half a unit, and mb_gemm has tiles of that size. The whole call replayed, here / by mb_gemm: 128 rows of 128 heads 21.8 / 20.8 us, of 64 18.0 / 18.2,
+    // of 16 17.4 / 17.5; 256 rows of 128 heads 25.7 / 38.4, of 64 21.1 / 26.1, of 16 20.7 / 24.7. Among other calls: 384 rows of 128 59.9 / 65.7, 512 of 64 36.0 / 36.8,
+    // 1024 of 16 34.9 / 36.9, of 64 59.6 / 70.3, 8192 of 16 294 / 306
+    if (a->kv_rows > 128) {
       const ExpandParams x{(__nv_bfloat16*)kv, a->kv_rows, n, (int)units, a->status};
       rc = mbh::encode_2d(&tm[4], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, wh, kLat, (uint64_t)n * 256, kLat * 2, 64, 128);
       if (!rc) rc = (int)mb::launch_kernel_cluster(expand_kernel, dim3(2 * (unsigned)(units < pairs ? units : pairs)), dim3(kExpThreads), kExpSmem, stream, 1, tm[3], tm[4], x);
