@@ -107,8 +107,13 @@ def _expanded_pays(batch) -> bool:
     pair and 512 x 256 a cached token expanded: by that count a cached token in front of the rows has to be seen by 171 of them. The absorbed kernel runs
     further from its peak, so less is enough. Measured with 128 heads, absorbed against expanded: eight portions behind contexts of 2048, of 32 rows 722 and
     911 us, of 48 1062 and 918, of 96 1945 and 919; one behind 4096, of 32 rows 337 and 222, of 512 2139 and 304; a whole prompt of 1024 1031 and 119. With
-    16 heads expanded is ahead in all of them (eight of 32 rows behind 2048: 192 and 136). Portions of fewer than 32 rows stay with the decode kernels.
-    Steps over more cached tokens than the workspace of 1 GB has room for stay absorbed."""
+    16 heads expanded is ahead in all of them (eight of 32 rows behind 2048: 192 and 136). Steps whose longest portion has fewer than 32 rows stay absorbed, and
+    so do those over more cached tokens than the workspace of 1 GB has room for.
+
+    A step goes one way as a whole, as the absorbed form takes one kernel by the longest portion: beside a prompt, sequences that decode are expanded too, and
+    are counted by what they have cached. With 128 heads, absorbed against expanded: 20 of one token behind 4000 beside a prompt of 8192 37010 and 6809 us
+    (expanded is taken), 20 behind 1000 beside 1500 2158 and 1175 (taken), 20 behind 4000 beside 2048 3506 and 4149, 60 behind 4000 beside 4096 12345 and 13545, 64
+    behind 1000 beside 1024 1768 and 3527 (none of these taken)."""
     return batch.max_q_len >= mla_cuda.TC_MIN_ROWS and batch.total_ctx > 0 and mla_prompt.fits(batch.total_ctx, batch.num_seqs) and \
         batch.total_pairs >= EXPAND_PAIRS * (batch.total_ctx - batch.num_tokens)
 

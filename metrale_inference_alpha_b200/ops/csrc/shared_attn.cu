@@ -4,7 +4,7 @@
 // What has no need of the rest is computed on its own: all rows behind a prefix over that prefix, which is read once for all of them (shared_prefix.cuh),
 // and every token over what its sequence has of its own (the decode kernel, attention_decode_parts.cu). Either leaves outputs relative to 2^m, m and sums,
 // and the join here adds them up. The decode kernel comes up under the prefix kernel and does not wait for it until its end, so that the two share the GPU.
-// No atomics: every partial result has one writer, and the join adds them in the order of the tokens.
+// No atomics on results: every partial one has one writer, and the join adds them in an order that follows from the plan (below).
 #include "attention_decode_parts.h"
 #include "shared_prefix.cuh"
 
@@ -49,8 +49,9 @@ Ws workspace(const MbSharedArgs& a) {
   return w;
 }
 
-// 32 rows (tokens x heads of a group) of a kv head and 32 dims at a time, lane = row. A row's partial results are shared out over the eight warps, each of
-// which asks for maximum, sum and dims together, and the warps' sums are joined in shared memory: few rows have many parts, and their latencies do not add up.
+// 32 rows (tokens x heads of a group) of a kv head and 32 dims at a time, lane = row. A row's partial results (a prefix's, of single units all first sides in
+// front of all second ones, then its own) are dealt out to the eight warps, each of which sums every eighth and asks for maximum, sum and dims together; the
+// warps' sums are joined in shared memory from warp 0 to 7. Few rows have many parts, and their latencies do not add up.
 // Bound by latency: 2 to 3 us a unit, of which the first begin before the kernels in front are through. As many CTAs as fit walk the units: with a CTA for
 // each, many of them came up late to plan again (the whole call 89.2 us instead of 87.2 for 128 sequences, 53.3 instead of 50.1 for 64 tokens behind 5000).
 constexpr int kJoinDims = 32, kJoinCtas = 3;
