@@ -156,3 +156,46 @@ def test_the_workspace_of_latent_prompts_is_bounded(heads_at_once, monkeypatch):
     got = run_latent(c)
     assert torch.equal(got, want)
     assert torch.cuda.max_memory_allocated() - before <= most + 2048 + got.numel() * 2          # parts begin on 256 bytes, tensors on 512
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,n", [(10, 2, 128, 40), (8, 1, 64, 129), (4, 2, 256, 17)])
+@pytest.mark.parametrize("fp8", [False, True])
+def test_many_new_tokens(heads, kv_heads, dim, n, fp8):
+    """More of them than some sequences have rows: the first see the prefix alone, or nothing."""
+    c = oracle.shared(14, [n, 3, 2 * n + 5, 0], [200, 0, 70], [0, 1, 2, 3], heads, kv_heads, dim, fp8, n=n)
+    want = oracle.shared_exact(c)
+    out, lse = run_shared(cuda(c))
+    within(out, want[0], want[1], "outputs")
+    within(lse, want[2], want[3], "log-sum-exps")
+
+
+def test_replays_with_other_groups():
+    """A captured step whose groups, prefixes and tables are another step's by the time it is replayed, some of them empty."""
+    c = cuda(oracle.shared(15, [20, 9, 33, 4, 50, 1], [600, 300, 129], [0, 2, 3, 6], 10, 2, 128, True))
+    run_shared(c)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, lse = run_shared(c)
+    for start, prefix, ctx in (([0, 2, 3, 6], [600, 300, 129], [20, 9, 33, 4, 50, 1]), ([0, 0, 0, 0], [0, 0, 0], [20, 9, 33, 4, 50, 1]), ([1, 1, 4, 5], [600, 299, 0], [0, 9, 1, 4, 0, 1]),
+                               ([0, 6, 6, 6], [513, 0, 0], [0, 0, 0, 0, 0, 0])):
+        for name, x in (("start", start), ("prefix", prefix), ("ctx", ctx)):
+            c[name].copy_(torch.tensor(x, dtype=torch.int32))
+        out.zero_()
+        graph.replay()
+        want = oracle.shared_exact({k: v.cpu() if isinstance(v, torch.Tensor) else v for k, v in c.items()})
+        within(out, want[0], want[1], f"outputs with groups {start}")
+        within(lse, want[2], want[3], f"log-sum-exps with groups {start}")
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(32, 16, 128), (16, 8, 256), (64, 32, 64)])
+def test_an_e4m3_cache_beyond_32_bits(heads, kv_heads, dim):
+    c = cuda(oracle.shared(16, [20, 90, 3], [300], [0, 3], heads, kv_heads, dim, True))
+    want = run_shared(c)
+    blocks = 150_000                                             # 16 tokens of 2048 bytes of K: 4.9 GB
+    front = blocks - c["k"].shape[0]
+    big = {**c, "table": c["table"] + front, "prefix_table": c["prefix_table"] + front}
+    for name in ("k", "v"):
+        big[name] = torch.empty(blocks, *c[name].shape[1:], dtype=torch.uint8, device="cuda")
+        big[name][front:] = c[name]
+    got = run_shared(big)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
